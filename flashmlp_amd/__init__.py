@@ -8,9 +8,13 @@ reference module `flashmlp`:
 
 `flashmlp_amd.flashmlp` (torch.ops.flashmlp_amd.fwd / .bwd) is the same computation as a
 registered torch.library operator, for torch.compile and FakeTensor tracing.
+
+A gated block built around it has the gated form  O = (act(X Wg) * (X Wu)) W2  (flashmlp_gated_fwd,
+flashmlp_gated_bwd, GatedFlashMLPFunction, GatedFlashMLP).
 """
 from .flashmlp import FlashMLP, FlashMLPFunction, flashmlp_bwd, flashmlp_fwd
 from .baseline import PyTorchMLP, flashmlp_torch_bwd, flashmlp_torch_fwd
+from .gated import GatedFlashMLP, GatedFlashMLPFunction, flashmlp_gated_bwd, flashmlp_gated_fwd
 from . import ops
 from .ops import flashmlp
 
@@ -24,4 +28,8 @@ __all__ = [
     "flashmlp_torch_bwd",
     "flashmlp",
     "ops",
+    "flashmlp_gated_fwd",
+    "flashmlp_gated_bwd",
+    "GatedFlashMLPFunction",
+    "GatedFlashMLP",
 ]

@@ -1,7 +1,7 @@
 // C ABI of libflashmlp.so (declared in include/flashmlp.h): argument validation,
 // status reporting and dispatch to the gfx950 kernels. No allocation, no synchronisation.
 #include "../../include/flashmlp.h"
-#include "fmlp_launch.h"
+#include "fmlp_block.h"
 
 #include <hip/hip_runtime.h>
 #include <atomic>
@@ -72,6 +72,23 @@ int num_cus_current(int* out) {
   *out = n;
   return FMLP_OK;
 }
+
+}  // namespace
+
+// the same for the other C-ABI translation units
+int fmlp::abi_fail(int status, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  g_last_error = buf;
+  return status;
+}
+int fmlp::abi_ok() { return ok(); }
+int fmlp::abi_num_cus(int* out) { return num_cus_current(out); }
+
+namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -1,0 +1,167 @@
+"""Gated multi-head MLP:  O = (act(X Wg) * (X Wu)) W2  per head, with a recomputing backward.
+
+    flashmlp_gated_fwd(x, wg, wu, w2, activation="") -> o                            (H,B,D)
+    flashmlp_gated_bwd(x, wg, wu, w2, do, activation="") -> (dx, dwg, dwu, dw2)
+    GatedFlashMLPFunction.apply(x, wg, wu, w2, activation)
+    GatedFlashMLP(num_heads, hidden_dim, intermediate_dim, activation="silu", dtype, device)
+
+The gated form of flashmlp_fwd / flashmlp_bwd / FlashMLPFunction / FlashMLP, in their manner: x
+(H, B, D), wg and wu (H, D, E), w2 (H, E, D); act in {"", "silu", "leaky_relu", "sigmoid"}; fp16, bf16
+and fp32 tensors on one GPU, D in {16, 32, 64, 128, 256}, any E >= 1. An x or do of dense rows is read in
+place whatever the distance of its heads, other views are copied. Every call launches the HIP kernels
+of libflashmlp.so asynchronously on torch's current stream of the tensors' device.
+"""
+from __future__ import annotations
+
+from typing import Tuple
+
+import numpy as np
+import torch
+
+from . import _lib
+from .flashmlp import (_HeadMean, _act_code, _alloc_ws, _current_device, _dense_all, _empty_as, _io_code, _ptr, _rows,
+                       _stream_of)
+
+
+def _check(x, wg, wu, w2) -> Tuple[int, int, int, int]:
+    H, B, D = x.shape
+    Hg, Dg, E = wg.shape
+    H2, E2, D2 = w2.shape
+    assert H == Hg and H == H2, "Number of heads must match"
+    assert wu.shape == wg.shape, "Gate and up projections must match"
+    assert D == Dg, "Hidden dimension mismatch"
+    assert E == E2, "Intermediate dimension mismatch"
+    assert D == D2, "Output dimension mismatch"
+    return H, B, D, E
+
+
+class _On:
+    """The library launches on the current device: make it the tensors'."""
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self):
+        self.prev = _current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+        return _stream_of(self.index)
+
+    def __exit__(self, *exc):
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+
+
+def flashmlp_gated_fwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, w2: torch.Tensor,
+                       activation: str = "") -> torch.Tensor:
+    """O = (act(x @ wg) * (x @ wu)) @ w2 per head.
+
+    Args:
+        x: (H, B, D); wg, wu: (H, D, E); w2: (H, E, D); activation: "silu", "leaky_relu",
+        "sigmoid" or "" (linear: a bilinear product).
+    Returns:
+        o (H, B, D), dtype of x. The products are summed in fp32 and h = act(.) * (.) is rounded to
+        the io dtype before the last one.
+    """
+    H, B, D, E = _check(x, wg, wu, w2)
+    dtype = _io_code(x, wg, wu, w2)
+    o = _empty_as(x, (H, B, D))
+    L = _lib.lib()
+    with _On(x.get_device()) as stream:
+        x = _rows(x)
+        wg, wu, w2 = _dense_all(wg, wu, w2)
+        n = L.fmlp_gated_fwd_workspace_bytes(H, B, D, E, dtype)
+        ws = _alloc_ws(n, x.device)
+        st = L.fmlp_gated_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), w2.data_ptr(), o.data_ptr(), H, B, D, E,
+                              x.stride(0), dtype, _act_code(activation), _ptr(ws), n, stream)
+    _lib.check(st, "gated forward")
+    return o
+
+
+def flashmlp_gated_bwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, w2: torch.Tensor, do: torch.Tensor,
+                       activation: str = "", *, _needs: Tuple[bool, bool] = (True, True)):
+    """Gradients of flashmlp_gated_fwd: (dx, dwg, dwu, dw2), shaped like (x, wg, wu, w2).
+
+    Recomputes both projections from x instead of reading stored activations. `_needs` (need dx,
+    need the weights' gradients; GatedFlashMLPFunction passes autograd's needs_input_grad) skips the
+    programs of gradients that nobody asked for and returns None in their place.
+    """
+    H, B, D, E = _check(x, wg, wu, w2)
+    assert x.shape == do.shape, "Gradient shape mismatch"
+    need_dx, need_dw = bool(_needs[0]), bool(_needs[1])
+    dtype = _io_code(x, wg, wu, w2, do)
+    dx = _empty_as(x, (H, B, D)) if need_dx else None
+    dwg, dwu, dw2 = ((_empty_as(t, t.shape) for t in (wg, wu, w2)) if need_dw else (None, None, None))
+    if not (need_dx or need_dw):
+        return dx, dwg, dwu, dw2
+    dtype |= (0 if need_dx else _lib.FMLP_BWD_NO_DX) | (0 if need_dw else _lib.FMLP_BWD_NO_DW)
+    L = _lib.lib()
+    with _On(x.get_device()) as stream:
+        x, do = _rows(x), _rows(do)
+        wg, wu, w2 = _dense_all(wg, wu, w2)
+        n = L.fmlp_gated_bwd_workspace_bytes(H, B, D, E, dtype)
+        ws = _alloc_ws(n, x.device)
+        st = L.fmlp_gated_bwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), w2.data_ptr(), do.data_ptr(), _ptr(dx),
+                              _ptr(dwg), _ptr(dwu), _ptr(dw2), H, B, D, E, x.stride(0), do.stride(0), dtype,
+                              _act_code(activation), _ptr(ws), n, stream)
+    _lib.check(st, "gated backward")
+    return dx, dwg, dwu, dw2
+
+
+class GatedFlashMLPFunction(torch.autograd.Function):
+    """Autograd binding of the gated MLP. Saves only (x, wg, wu, w2)."""
+
+    @staticmethod
+    def forward(ctx, x, wg, wu, w2, activation=""):
+        o = flashmlp_gated_fwd(x, wg, wu, w2, activation)
+        ctx.save_for_backward(x, wg, wu, w2)
+        ctx.activation = activation
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        x, wg, wu, w2 = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, *dw = flashmlp_gated_bwd(x, wg, wu, w2, do, ctx.activation, _needs=(need[0], any(need[1:4])))
+        return (dx, *(g if n else None for g, n in zip(dw, need[1:4])), None)
+
+
+class GatedFlashMLP(torch.nn.Module):
+    """Gated multi-head MLP module (the gated form of FlashMLP).
+
+    Args:
+        num_heads: number of heads H
+        hidden_dim: hidden dimension D
+        intermediate_dim: intermediate dimension E
+        activation: "silu", "leaky_relu", "sigmoid" or ""
+        dtype: weight dtype (float16, bfloat16 or float32)
+        device: device of the weights
+
+    Parameters wg, wu (H, D, E) ~ randn / sqrt(D) and w2 (H, E, D) ~ randn / sqrt(E). A 2-D input
+    (B, D) is expanded to every head and the output is the mean over heads, as in FlashMLP.
+    """
+
+    def __init__(self, num_heads: int, hidden_dim: int, intermediate_dim: int, activation: str = "silu",
+                 dtype=torch.float16, device="cuda"):
+        super().__init__()
+        self.num_heads = num_heads
+        self.hidden_dim = hidden_dim
+        self.intermediate_dim = intermediate_dim
+        self.activation = activation
+
+        def weight(rows, cols):
+            return torch.nn.Parameter(torch.randn(num_heads, rows, cols, dtype=dtype, device=device) / np.sqrt(rows))
+
+        self.wg = weight(hidden_dim, intermediate_dim)
+        self.wu = weight(hidden_dim, intermediate_dim)
+        self.w2 = weight(intermediate_dim, hidden_dim)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        shared = x.dim() == 2
+        if shared:
+            x = x.unsqueeze(0).expand(self.num_heads, -1, -1)
+        o = GatedFlashMLPFunction.apply(x, self.wg, self.wu, self.w2, self.activation)
+        if shared:
+            o = _HeadMean.apply(o) if o.requires_grad else o.mean(dim=0)
+        return o

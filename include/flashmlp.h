@@ -41,7 +41,8 @@ extern "C" {
                               the full recompute launch's dX programs (a workspace where it
                               splits ragged dX tiles). Raised where an entry point that was
                               there changes; added within 4, with no change to the others:
-                              fmlp_shape_dense, fmlp_fwd_strided_ws, fmlp_copy_dense */
+                              fmlp_shape_dense, fmlp_fwd_strided_ws, fmlp_copy_dense, the
+                              fmlp_gated_* calls */
 
 typedef enum {
   FMLP_OK = 0,
@@ -257,6 +258,28 @@ int fmlp_bwd_strided(const void* x, const void* w1, const void* w2, const void* 
 #define FMLP_SCRATCH_MAX_BYTES ((size_t)64 << 20)
 int fmlp_bwd_noalloc(const void* x, const void* w1, const void* w2, const void* dout, void* dx, void* dw1, void* dw2,
                      int64_t H, int64_t B, int64_t D, int64_t E, int dtype, int act, void* stream);
+
+/*
+ * Gated MLP: o = (act(x @ wg) * (x @ wu)) @ w2 per head, x (H,B,D), wg and wu (H,D,E), w2 (H,E,D), and
+ * its gradients  dh = dout @ w2^T, dg = dh * u * act'(g), du = dh * act(g);  dx = dg @ wg^T + du @ wu^T,
+ * dwg = x^T @ dg, dwu = x^T @ du, dw2 = h^T @ dout, with g = x @ wg, u = x @ wu, h = act(g) * u recomputed
+ * from x. No counterpart in the reference, whose block has no gate. Sums in fp32; h, dg and du are
+ * rounded to the io dtype before the products that take them (not for fp32 io), as act(.) is in fmlp_fwd.
+ * Weights and outputs are dense, 16-byte aligned; x and dout have dense rows and heads *_head_stride
+ * elements apart (any multiple of 16 bytes, 0: one matrix shared by every head). D in {16, 32, 64, 128,
+ * 256}, E >= 1, H, B >= 0; B = 0 leaves zero weight gradients. dtype: fp16, bf16 or fp32; the backward
+ * also takes FMLP_BWD_NO_DX and FMLP_BWD_NO_DW. The workspace (16-byte aligned, scratch for the duration
+ * of the call on `stream`) is at least *_workspace_bytes() for the same arguments, and may be NULL where
+ * that is 0. Results do not depend on the workspace's content and are bitwise repeatable.
+ */
+size_t fmlp_gated_fwd_workspace_bytes(int64_t H, int64_t B, int64_t D, int64_t E, int dtype);
+int fmlp_gated_fwd(const void* x, const void* wg, const void* wu, const void* w2, void* o, int64_t H, int64_t B,
+                   int64_t D, int64_t E, int64_t x_head_stride, int dtype, int act, void* workspace,
+                   size_t workspace_bytes, void* stream);
+size_t fmlp_gated_bwd_workspace_bytes(int64_t H, int64_t B, int64_t D, int64_t E, int dtype);
+int fmlp_gated_bwd(const void* x, const void* wg, const void* wu, const void* w2, const void* dout, void* dx,
+                   void* dwg, void* dwu, void* dw2, int64_t H, int64_t B, int64_t D, int64_t E, int64_t x_head_stride,
+                   int64_t dout_head_stride, int dtype, int act, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
