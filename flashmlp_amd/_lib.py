@@ -28,10 +28,26 @@ FMLP_BWD_NO_DX = 0x1000
 FMLP_BWD_NO_DW = 0x2000
 ACT_CODES = {"": 0, "silu": 1, "leaky_relu": 2, "sigmoid": 3}
 
+
+
+class Join(ctypes.Structure):
+    """fmlp_join of include/flashmlp.h"""
+    _fields_ = ([(n, ctypes.c_void_p) for n in (
+        "r", "o", "w_post", "gate", "w_pre", "r_out", "y", "rs_o", "rs_r", "dr_out", "dy", "dr", "d_o", "dw_post",
+        "dgate", "dw_pre")]
+        + [(n, ctypes.c_int64) for n in (
+            "B", "H", "D", "groups", "r_stride", "o_head_stride", "o_row_stride", "y_head_stride", "y_row_stride",
+            "dr_out_stride", "d_o_head_stride", "d_o_row_stride")]
+        + [("scale", ctypes.c_float), ("eps", ctypes.c_float), ("dtype", ctypes.c_int), ("r_dtype", ctypes.c_int),
+           ("post", ctypes.c_int)])
+
+
 # (name, restype, argtypes) for every symbol include/flashmlp.h declares
 _i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
 _i64p = ctypes.POINTER(ctypes.c_int64)
+_vpp = ctypes.POINTER(_vp)
+_intp = ctypes.POINTER(ctypes.c_int)
 SIGNATURES = {
     "fmlp_abi_version": (ctypes.c_int, []),
     "fmlp_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -61,6 +77,13 @@ SIGNATURES = {
     "fmlp_gated_fwd": (ctypes.c_int, [_vp] * 5 + [_i64] * 5 + [ctypes.c_int, ctypes.c_int, _vp, ctypes.c_size_t, _vp]),
     "fmlp_gated_bwd_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, ctypes.c_int]),
     "fmlp_gated_bwd": (ctypes.c_int, [_vp] * 9 + [_i64] * 6 + [ctypes.c_int, ctypes.c_int, _vp, ctypes.c_size_t, _vp]),
+    "fmlp_join_fwd": (ctypes.c_int, [ctypes.POINTER(Join), _vp]),
+    "fmlp_join_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Join)]),
+    "fmlp_join_bwd": (ctypes.c_int, [ctypes.POINTER(Join), _vp, ctypes.c_size_t, _vp]),
+    "fmlp_clip_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, _i64p]),
+    "fmlp_grad_norm": (ctypes.c_int, [ctypes.c_int, _vpp, _i64p, _intp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "fmlp_clip_grads": (ctypes.c_int, [ctypes.c_int, _vpp, _vpp, _i64p, _intp, _intp, ctypes.c_float, _vp, _vp,
+                                       ctypes.c_size_t, _vp]),
     "fmlp_bwd_noalloc": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_int,
                                         ctypes.c_int, _vp]),
 }

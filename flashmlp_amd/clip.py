@@ -1,0 +1,134 @@
+"""Global gradient norm over many tensors, and clipping.
+
+    grad_norm(grads) -> norm
+    clip_grads(grads, max_norm, *, out=None) -> (out, norm)
+    clip_grad_norm_(parameters, max_norm, *, error_if_nonfinite=False) -> norm
+
+    norm = sqrt(sum of all squares),  out = grad * min(1, max_norm / (norm + 1e-6))
+
+The norm is an fp32 number on the tensors' device; nothing waits for it (error_if_nonfinite does).
+Gradients are fp16, bf16 or fp32 in any mix, on one GPU. The squares are summed in 64 bits in a fixed order,
+so that no finite gradients overflow and results repeat bitwise. A norm that is infinite or NaN scales by 0
+or NaN, as torch.nn.utils.clip_grad_norm_ does.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Iterable, List, Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib
+from .flashmlp import _DTYPES
+from .gated import _On
+
+
+def _one_run(t: torch.Tensor) -> bool:
+    # the tensor's elements are one run of memory, each once, in whatever order
+    if t.is_contiguous():
+        return not t.is_neg()
+    return torch.ops.aten.is_non_overlapping_and_dense.default(t) and not t.is_neg()
+
+
+def _check(ts: Sequence[torch.Tensor], what: str):
+    dev = ts[0].device
+    if dev.type != "cuda":
+        raise RuntimeError(f"FlashMLP runs on an AMD GPU through HIP; got a tensor on {dev} (move inputs to 'cuda')")
+    for t in ts:
+        if t.device != dev:
+            raise RuntimeError(f"all {what} must be on one device ({dev} vs {t.device})")
+        if t.dtype not in _DTYPES:
+            raise TypeError(f"FlashMLP supports float16, bfloat16 and float32 {what}, got {t.dtype}")
+        if t.layout != torch.strided:
+            raise TypeError(f"{what} must be dense tensors, got {t.layout}")
+    return dev
+
+
+def _pointers(ts):
+    return (ctypes.c_void_p * len(ts))(*(t.data_ptr() for t in ts))
+
+
+def _codes(ts):
+    return (ctypes.c_int * len(ts))(*(_DTYPES[t.dtype] for t in ts))
+
+
+def _run(grads, outs, max_norm, dev):
+    L, n = _lib.lib(), len(grads)
+    numels = (ctypes.c_int64 * n)(*(g.numel() for g in grads))
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    with _On(dev.index) as stream:
+        size = L.fmlp_clip_workspace_bytes(n, numels)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        if outs is None:
+            st = L.fmlp_grad_norm(n, _pointers(grads), numels, _codes(grads), norm.data_ptr(), ws.data_ptr(), size, stream)
+        else:
+            st = L.fmlp_clip_grads(n, _pointers(grads), _pointers(outs), numels, _codes(grads), _codes(outs), max_norm,
+                                   norm.data_ptr(), ws.data_ptr(), size, stream)
+    _lib.check(st, "gradient norm" if outs is None else "gradient clipping")
+    return norm
+
+
+def grad_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
+    """The L2 norm over all elements of all tensors, a 0-dim fp32 tensor."""
+    grads = list(grads)
+    if not grads:
+        return torch.zeros(())
+    dev = _check(grads, "gradients")
+    return _run([g if _one_run(g) else g.contiguous() for g in grads], None, 0.0, dev)
+
+
+def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *,
+               out: Optional[Iterable[torch.Tensor]] = None) -> Tuple[List[torch.Tensor], torch.Tensor]:
+    """Gradients scaled so that their global norm is at most max_norm.
+
+    Args:
+        out: tensors of the gradients' shapes, each of any of the dtypes (an optimizer's full precision
+            buffers, say), overlapping neither the gradients nor each other; None clips in place.
+    Returns:
+        (out, norm): the clipped tensors and the norm before the clipping.
+    """
+    grads = list(grads)
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    outs = grads if out is None else list(out)
+    if len(outs) != len(grads):
+        raise ValueError(f"{len(grads)} gradients, {len(outs)} outputs")
+    if not grads:
+        return outs, torch.zeros(())
+    dev = _check(grads, "gradients")
+    if out is not None:
+        if _check(outs, "outputs") != dev:
+            raise RuntimeError(f"gradients and outputs must be on one device ({dev} vs {outs[0].device})")
+        for g, o in zip(grads, outs):
+            if g.shape != o.shape:
+                raise ValueError(f"output of shape {tuple(o.shape)} for a gradient of {tuple(g.shape)}")
+    src, dst, back = [], [], []
+    for g, o in zip(grads, outs):
+        if _one_run(o) and (g is o or g.stride() == o.stride()):
+            src.append(g if g is o or _one_run(g) else g.contiguous())
+            dst.append(o)
+            continue
+        # other layouts through dense tensors
+        s = g.contiguous()
+        d = o if o.is_contiguous() and not o.is_neg() else torch.empty(o.shape, dtype=o.dtype, device=dev)
+        src.append(s)
+        dst.append(d)
+        if d is not o:
+            back.append((o, d))
+    norm = _run(src, dst, max_norm, dev)
+    with torch.no_grad():
+        for o, d in back:
+            o.copy_(d)
+    return outs, norm
+
+
+def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, *,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """torch.nn.utils.clip_grad_norm_ (L2) on these kernels: clips the parameters' .grad in place and
+    returns their norm. error_if_nonfinite waits for the norm, and raises before any gradient is changed."""
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in params if p.grad is not None]
+    if error_if_nonfinite and grads and not torch.isfinite(grad_norm(grads)):
+        raise RuntimeError("the total norm of the gradients is not finite, so it cannot be clipped")
+    return clip_grads(grads, max_norm)[1]

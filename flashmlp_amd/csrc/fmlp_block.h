@@ -38,4 +38,74 @@ hipError_t launch_gated_gen_fwd(const GatedArgs& a, hipStream_t st);
 hipError_t launch_gated_gen_dx(const GatedArgs& a, hipStream_t st);
 hipError_t launch_gated_gen_dw(const GatedArgs& a, hipStream_t st);
 
+// A block's join (fmlp_join.hip): the stream r (B, C), C = H D; o, y and their gradients (head, row, column)
+// with unit column stride. Pointers that are null leave their part out: o (no block output: only y is
+// taken from r), w_post, gate, w_pre (factors of one), r_out, y (results nobody asked for), and in the
+// backward dy, dr_out (gradients that are zero), dr, d_o, dw_post, dgate, dw_pre (not asked for).
+struct JoinArgs {
+  const void* r;
+  const void* o;
+  const void* w_post;
+  const void* gate;  // (groups, C): row g for rows g rows_per_gate ..
+  const void* w_pre;
+  void* r_out;  // forward: r' (dense rows); backward: the r' that was saved, rows r_sr apart
+  void* y;
+  float* rs_o;  // (B) 1 / rms of o and of r', written by the forward (or null) and read by the backward
+  float* rs_r;
+  const void* dr_out;
+  const void* dy;
+  void* dr;   // dense rows
+  void* d_o;
+  void* dw_post;
+  void* dgate;
+  void* dw_pre;
+  long long B, C, D, groups, rows_per_gate;
+  long long r_sr, dr_sr, o_sh, o_sr, y_sh, y_sr, do_sh, do_sr;  // element strides (y's: of dy in the backward)
+  float scale, eps;
+  int io;       // IoType of o, y, the weights and the gate
+  int r_f32;    // the stream is fp32 beside 16-bit io
+  int post;     // o is normalised
+  int aligned;  // D % 8 == 0, every pointer 16-byte aligned and every stride a multiple of 16 bytes
+};
+
+// Backward units (fmlp_join.hip): `parts` per gate group, or groups_per_unit whole groups each.
+struct JoinPlan {
+  long long units, groups_per_unit, rows_per_part;
+  int parts;
+  bool gate_partials;
+  size_t off_pre, off_post, off_gate, ws_bytes;
+  float* pre;
+  float* post;
+  float* gate;
+};
+struct JoinSum {
+  const float* src;
+  void* dst;
+  int rows, groups;
+};
+struct JoinReduce {
+  JoinSum t[3];
+};
+constexpr int64_t kJoinMaxC = 16384;  // 1024 threads of two vectors of 8 columns
+JoinPlan join_plan(int64_t B, int64_t C, int64_t groups, bool dpre, bool dpost, bool dgate, int num_cus);
+hipError_t launch_join_fwd(const JoinArgs& a, hipStream_t st);
+hipError_t launch_join_bwd(const JoinArgs& a, JoinPlan p, void* ws, hipStream_t st);
+
+// Gradient norm and clipping (fmlp_clip.hip): n tensors of `numel` elements; io / out_io IoType codes. outs[i]
+// null: nothing is written; equal to grads[i]: in place. ws: clip_plan's bytes.
+struct ClipTensor {
+  const void* grad;
+  void* out;
+  long long numel;
+  int io, out_io;
+};
+struct ClipPlan {
+  long long chunk;   // elements per workgroup
+  long long blocks;  // workgroups over all tensors
+  size_t ws_bytes;   // one double per workgroup and the coefficient
+};
+ClipPlan clip_plan(int n, const int64_t* numel, int num_cus);
+hipError_t launch_clip(int n, const ClipTensor* t, const ClipPlan& p, bool clip, float max_norm, float* norm, void* ws,
+                       hipStream_t st);
+
 }  // namespace fmlp

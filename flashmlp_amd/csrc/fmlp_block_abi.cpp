@@ -3,6 +3,9 @@
 #include "../../include/flashmlp.h"
 #include "fmlp_block.h"
 
+#include <new>
+#include <vector>
+
 #define FMLP_EXPORT extern "C" __attribute__((visibility("default")))
 
 using fmlp::abi_fail;
@@ -144,4 +147,221 @@ FMLP_EXPORT int fmlp_gated_bwd(const void* x, const void* wg, const void* wu, co
   if (e == hipSuccess && want_dx) e = fmlp::launch_gated_gen_dx(a, (hipStream_t)stream);
   if (e != hipSuccess) return abi_fail(FMLP_ERR_HIP, "gated backward launch: %s", hipGetErrorString(e));
   return abi_ok();
+}
+
+// ---------------------------------------------------------------------------------------------
+// join
+// ---------------------------------------------------------------------------------------------
+namespace {
+
+// a pointer of the call, aligned to its elements; *vec is cleared where it is not a 16-byte vector's
+int join_ptr(const void* p, const char* name, bool needed, size_t es, int* vec) {
+  if (p == nullptr) return needed ? abi_fail(FMLP_ERR_INVALID_ARG, "%s is NULL", name) : FMLP_OK;
+  if ((reinterpret_cast<uintptr_t>(p) % es) != 0)
+    return abi_fail(FMLP_ERR_INVALID_ARG, "%s is not %zu-byte aligned", name, es);
+  if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0) *vec = 0;
+  return FMLP_OK;
+}
+
+int join_stride(int64_t s, const char* name, bool used, size_t es, int* vec) {
+  if (!used) return FMLP_OK;
+  if (s < 0) return abi_fail(FMLP_ERR_INVALID_ARG, "%s stride is negative (%lld)", name, (long long)s);
+  if ((s * (int64_t)es) % 16 != 0) *vec = 0;
+  return FMLP_OK;
+}
+
+int check_join(const fmlp_join* j, bool bwd, fmlp::JoinArgs* a) {
+  if (j == nullptr) return abi_fail(FMLP_ERR_INVALID_ARG, "the call's description is NULL");
+  if (j->B < 0 || j->H < 1 || j->D < 1 || j->groups < 1)
+    return abi_fail(FMLP_ERR_INVALID_ARG, "dimensions B=%lld H=%lld D=%lld groups=%lld", (long long)j->B, (long long)j->H,
+                    (long long)j->D, (long long)j->groups);
+  if (j->dtype != FMLP_DTYPE_F16 && j->dtype != FMLP_DTYPE_BF16 && j->dtype != FMLP_DTYPE_F32)
+    return abi_fail(FMLP_ERR_UNSUPPORTED, "dtype code %d: fp16 (0), bf16 (1) or fp32 (2)", j->dtype);
+  if (j->r_dtype != j->dtype && j->r_dtype != FMLP_DTYPE_F32)
+    return abi_fail(FMLP_ERR_UNSUPPORTED, "stream dtype code %d: the blocks' dtype or fp32", j->r_dtype);
+  if (j->H > fmlp::kJoinMaxC || j->D > fmlp::kJoinMaxC || j->H * j->D > fmlp::kJoinMaxC)
+    return abi_fail(FMLP_ERR_UNSUPPORTED, "%lld x %lld columns: at most %lld", (long long)j->H, (long long)j->D,
+                    (long long)fmlp::kJoinMaxC);
+  if (j->B > 0x7fffffffLL) return abi_fail(FMLP_ERR_INVALID_ARG, "too many rows (%lld)", (long long)j->B);
+  if (j->B % j->groups != 0)
+    return abi_fail(FMLP_ERR_INVALID_ARG, "%lld rows are no multiple of the gate's %lld", (long long)j->B,
+                    (long long)j->groups);
+  if (!(j->eps >= 0)) return abi_fail(FMLP_ERR_INVALID_ARG, "eps is negative or NaN");
+  if (!j->post && j->w_post) return abi_fail(FMLP_ERR_INVALID_ARG, "w_post without the post norm");
+  const size_t es = elem_bytes(j->dtype), rs = elem_bytes(j->r_dtype);
+  const bool rows = j->B > 0, has_o = j->o != nullptr, has_y = bwd ? j->dy != nullptr : j->y != nullptr;
+  if (rows && !bwd && !has_y && j->r_out == nullptr) return abi_fail(FMLP_ERR_INVALID_ARG, "no output is asked for");
+  if (rows && !has_o && (j->w_post || j->gate)) return abi_fail(FMLP_ERR_INVALID_ARG, "w_post or gate without o");
+  if (rows && !has_y && j->w_pre && !bwd) return abi_fail(FMLP_ERR_INVALID_ARG, "w_pre without y");
+  int vec = j->D % 8 == 0 ? 1 : 0, st;
+  if ((st = join_ptr(j->r, "r", rows && !bwd, rs, &vec)) || (st = join_ptr(j->o, "o", false, es, &vec)) ||
+      (st = join_ptr(j->w_post, "w_post", false, es, &vec)) || (st = join_ptr(j->gate, "gate", false, es, &vec)) ||
+      (st = join_ptr(j->w_pre, "w_pre", false, es, &vec)) ||
+      (st = join_ptr(j->r_out, "r_out", rows && bwd && has_y, rs, &vec)) ||
+      (st = join_ptr(j->y, "y", false, es, &vec)) || (st = join_stride(j->r_stride, "r", true, rs, &vec)) ||
+      (st = join_stride(j->o_head_stride, "o head", has_o && j->H > 1, es, &vec)) ||
+      (st = join_stride(j->o_row_stride, "o row", has_o, es, &vec)) ||
+      (st = join_stride(j->y_head_stride, "y head", has_y && j->H > 1, es, &vec)) ||
+      (st = join_stride(j->y_row_stride, "y row", has_y, es, &vec)))
+    return st;
+  if (bwd) {
+    int v4 = 1;
+    if ((st = join_ptr(j->dr_out, "dr_out", false, rs, &vec)) || (st = join_ptr(j->dy, "dy", false, es, &vec)) ||
+        (st = join_ptr(j->dr, "dr", false, rs, &vec)) || (st = join_ptr(j->d_o, "d_o", false, es, &vec)) ||
+        (st = join_ptr(j->dw_post, "dw_post", false, es, &vec)) || (st = join_ptr(j->dgate, "dgate", false, es, &vec)) ||
+        (st = join_ptr(j->dw_pre, "dw_pre", false, es, &vec)) ||
+        (st = join_stride(j->dr_out_stride, "dr_out", j->dr_out != nullptr, rs, &vec)) ||
+        (st = join_stride(j->d_o_head_stride, "d_o head", j->d_o != nullptr && j->H > 1, es, &vec)) ||
+        (st = join_stride(j->d_o_row_stride, "d_o row", j->d_o != nullptr, es, &vec)) ||
+        (st = join_ptr(j->rs_o, "rs_o", rows && has_o && j->post, 4, &v4)) ||
+        (st = join_ptr(j->rs_r, "rs_r", rows && has_y, 4, &v4)))
+      return st;
+    if (rows && !has_o && (j->d_o || j->dw_post || j->dgate)) return abi_fail(FMLP_ERR_INVALID_ARG, "gradients of o's part without o");
+    if (j->dw_post && !j->post) return abi_fail(FMLP_ERR_INVALID_ARG, "dw_post without the post norm");
+  }
+  a->r = j->r;
+  a->o = j->o;
+  a->w_post = j->w_post;
+  a->gate = j->gate;
+  a->w_pre = j->w_pre;
+  a->r_out = j->r_out;
+  a->y = j->y;
+  a->rs_o = j->rs_o;
+  a->rs_r = j->rs_r;
+  a->dr_out = j->dr_out;
+  a->dy = j->dy;
+  a->dr = j->dr;
+  a->d_o = j->d_o;
+  a->dw_post = j->dw_post;
+  a->dgate = j->dgate;
+  a->dw_pre = j->dw_pre;
+  a->B = j->B;
+  a->C = j->H * j->D;
+  a->D = j->D;
+  a->groups = j->groups;
+  a->rows_per_gate = j->B / j->groups;
+  a->r_sr = j->r_stride;
+  a->dr_sr = j->dr_out_stride;
+  a->o_sh = j->o_head_stride;
+  a->o_sr = j->o_row_stride;
+  a->y_sh = j->y_head_stride;
+  a->y_sr = j->y_row_stride;
+  a->do_sh = j->d_o_head_stride;
+  a->do_sr = j->d_o_row_stride;
+  a->scale = j->scale;
+  a->eps = j->eps;
+  a->io = io_type(j->dtype);
+  a->r_f32 = j->r_dtype == FMLP_DTYPE_F32 && j->dtype != FMLP_DTYPE_F32;
+  a->post = j->post ? 1 : 0;
+  a->aligned = vec;
+  return FMLP_OK;
+}
+
+int join_bwd_plan(const fmlp_join* j, const fmlp::JoinArgs& a, fmlp::JoinPlan* p) {
+  int cus = 0;
+  const int st = fmlp::abi_num_cus(&cus);
+  if (st) return st;
+  *p = fmlp::join_plan(a.B, a.C, j->groups, j->dw_pre != nullptr, j->dw_post != nullptr, j->dgate != nullptr, cus);
+  return FMLP_OK;
+}
+
+}  // namespace
+
+FMLP_EXPORT int fmlp_join_fwd(const fmlp_join* j, void* stream) {
+  fmlp::JoinArgs a{};
+  const int st = check_join(j, false, &a);
+  if (st) return st;
+  const hipError_t e = fmlp::launch_join_fwd(a, (hipStream_t)stream);
+  if (e != hipSuccess) return abi_fail(FMLP_ERR_HIP, "join forward launch: %s", hipGetErrorString(e));
+  return abi_ok();
+}
+
+FMLP_EXPORT size_t fmlp_join_bwd_workspace_bytes(const fmlp_join* j) {
+  fmlp::JoinArgs a{};
+  fmlp::JoinPlan p{};
+  if (check_join(j, true, &a) || join_bwd_plan(j, a, &p)) return 0;
+  return p.ws_bytes;
+}
+
+FMLP_EXPORT int fmlp_join_bwd(const fmlp_join* j, void* workspace, size_t workspace_bytes, void* stream) {
+  fmlp::JoinArgs a{};
+  fmlp::JoinPlan p{};
+  int st;
+  if ((st = check_join(j, true, &a)) || (st = join_bwd_plan(j, a, &p)) ||
+      (st = check_vec(workspace, "workspace", workspace != nullptr)))
+    return st;
+  if (p.ws_bytes > 0 && (workspace == nullptr || workspace_bytes < p.ws_bytes))
+    return abi_fail(FMLP_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0,
+                    p.ws_bytes);
+  const hipError_t e = fmlp::launch_join_bwd(a, p, workspace, (hipStream_t)stream);
+  if (e != hipSuccess) return abi_fail(FMLP_ERR_HIP, "join backward launch: %s", hipGetErrorString(e));
+  return abi_ok();
+}
+
+// ---------------------------------------------------------------------------------------------
+// gradient norm and clipping
+// ---------------------------------------------------------------------------------------------
+namespace {
+
+int clip_impl(int n, const void* const* grads, void* const* outs, const int64_t* numels, const int* dtypes,
+              const int* out_dtypes, bool clip, float max_norm, float* norm, void* ws, size_t ws_bytes, void* stream) {
+  if (n < 0) return abi_fail(FMLP_ERR_INVALID_ARG, "%d tensors", n);
+  if (n > 0 && (grads == nullptr || numels == nullptr || dtypes == nullptr || (clip && (outs == nullptr || out_dtypes == nullptr))))
+    return abi_fail(FMLP_ERR_INVALID_ARG, "tensor arrays must not be NULL");
+  if (norm == nullptr || (reinterpret_cast<uintptr_t>(norm) & 3u) != 0)
+    return abi_fail(FMLP_ERR_INVALID_ARG, "norm is NULL or not 4-byte aligned");
+  if (clip && !(max_norm >= 0)) return abi_fail(FMLP_ERR_INVALID_ARG, "max_norm is negative or NaN");
+  std::vector<fmlp::ClipTensor> t;
+  try {
+    t.resize((size_t)n);
+  } catch (const std::bad_alloc&) {
+    return abi_fail(FMLP_ERR_INVALID_ARG, "no host memory for %d tensors", n);
+  }
+  for (int i = 0; i < n; ++i) {
+    const int ins[2] = {dtypes[i], clip ? out_dtypes[i] : dtypes[i]};
+    for (int d : ins)
+      if (d != FMLP_DTYPE_F16 && d != FMLP_DTYPE_BF16 && d != FMLP_DTYPE_F32)
+        return abi_fail(FMLP_ERR_UNSUPPORTED, "tensor %d: dtype code %d: fp16 (0), bf16 (1) or fp32 (2)", i, d);
+    if (numels[i] < 0 || numels[i] > (1LL << 40))
+      return abi_fail(FMLP_ERR_INVALID_ARG, "tensor %d: %lld elements", i, (long long)numels[i]);
+    const void* g = grads[i];
+    void* o = clip ? outs[i] : nullptr;
+    if (numels[i] > 0) {
+      if (g == nullptr || (reinterpret_cast<uintptr_t>(g) % elem_bytes(ins[0])) != 0)
+        return abi_fail(FMLP_ERR_INVALID_ARG, "gradient %d is NULL or not aligned to its elements", i);
+      if (clip && (o == nullptr || (reinterpret_cast<uintptr_t>(o) % elem_bytes(ins[1])) != 0))
+        return abi_fail(FMLP_ERR_INVALID_ARG, "output %d is NULL or not aligned to its elements", i);
+    }
+    t[(size_t)i] = fmlp::ClipTensor{g, o, numels[i], io_type(ins[0]), io_type(ins[1])};
+  }
+  int cus = 0, st;
+  if ((st = fmlp::abi_num_cus(&cus))) return st;
+  const fmlp::ClipPlan p = fmlp::clip_plan(n, numels, cus);
+  if ((st = check_vec(ws, "workspace", true))) return st;
+  if (ws_bytes < p.ws_bytes)
+    return abi_fail(FMLP_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", ws_bytes, p.ws_bytes);
+  const hipError_t e = fmlp::launch_clip(n, t.data(), p, clip, max_norm, norm, ws, (hipStream_t)stream);
+  if (e != hipSuccess) return abi_fail(FMLP_ERR_HIP, "gradient clipping launch: %s", hipGetErrorString(e));
+  return abi_ok();
+}
+
+}  // namespace
+
+FMLP_EXPORT size_t fmlp_clip_workspace_bytes(int n, const int64_t* numels) {
+  int cus = 0;
+  if (n < 0 || (n > 0 && numels == nullptr) || fmlp::abi_num_cus(&cus)) return 0;
+  for (int i = 0; i < n; ++i)
+    if (numels[i] < 0 || numels[i] > (1LL << 40)) return 0;
+  return fmlp::clip_plan(n, numels, cus).ws_bytes;
+}
+
+FMLP_EXPORT int fmlp_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* dtypes, float* norm,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  return clip_impl(n, grads, nullptr, numels, dtypes, nullptr, false, 0.f, norm, workspace, workspace_bytes, stream);
+}
+
+FMLP_EXPORT int fmlp_clip_grads(int n, const void* const* grads, void* const* outs, const int64_t* numels,
+                                const int* dtypes, const int* out_dtypes, float max_norm, float* norm, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  return clip_impl(n, grads, outs, numels, dtypes, out_dtypes, true, max_norm, norm, workspace, workspace_bytes, stream);
 }

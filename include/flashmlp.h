@@ -42,7 +42,7 @@ extern "C" {
                               splits ragged dX tiles). Raised where an entry point that was
                               there changes; added within 4, with no change to the others:
                               fmlp_shape_dense, fmlp_fwd_strided_ws, fmlp_copy_dense, the
-                              fmlp_gated_* calls */
+                              fmlp_gated_*, fmlp_join_* and fmlp_clip_* calls, fmlp_grad_norm */
 
 typedef enum {
   FMLP_OK = 0,
@@ -280,6 +280,70 @@ size_t fmlp_gated_bwd_workspace_bytes(int64_t H, int64_t B, int64_t D, int64_t E
 int fmlp_gated_bwd(const void* x, const void* wg, const void* wu, const void* w2, const void* dout, void* dx,
                    void* dwg, void* dwu, void* dw2, int64_t H, int64_t B, int64_t D, int64_t E, int64_t x_head_stride,
                    int64_t dout_head_stride, int dtype, int act, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * A block's output joined to its residual stream, and the next block's input taken from it, in one pass:
+ *   n = o / sqrt(mean(o^2) + eps), p = n * w_post (without the post norm p = o)
+ *   r_out = r + scale * gate * p,  y = r_out / sqrt(mean(r_out^2) + eps) * w_pre
+ * over rows of C = H D columns, and the gradients. No counterpart in the reference, which has the MLP
+ * alone. r, r_out and their gradients are (B, C); o, y and theirs (H, B, D) with any head and row stride
+ * (head-major, as the MLP's tensors are, or with H = 1 plain rows); weights (C), gate (groups, C): row g
+ * for the rows g B/groups .. of the stream. Columns have stride one. o, w_post, gate, w_pre, r_out or y may
+ * be NULL: without o only y is taken (r_out then has to be NULL or is a copy of r), without a weight or
+ * gate its factor is one, a NULL result is not written. dtype: of o, y, weights and gate; r_dtype: of the
+ * stream, the same or fp32. rs_o, rs_r (B, fp32): the rows' 1 / rms, written by the forward where not NULL
+ * and read by the backward. Sums are fp32; y is taken from the unrounded r_out. Any alignment; 16-byte
+ * aligned tensors with D % 8 == 0 and strides of whole 16 bytes take vector accesses. C <= 16384.
+ * Backward: from dr_out and dy (NULL: zero), r_out (the stored one, rows r_stride apart; needed with dy),
+ * o and rs_*, writes those of dr (dense rows), d_o, dw_post, dgate, dw_pre that are not NULL; the gradients
+ * of weights and gate through fp32 partial sums in the workspace, added in a fixed order.
+ */
+typedef struct {
+  const void* r;
+  const void* o;
+  const void* w_post;
+  const void* gate;
+  const void* w_pre;
+  void* r_out;
+  void* y;
+  float* rs_o;
+  float* rs_r;
+  const void* dr_out;
+  const void* dy;
+  void* dr;
+  void* d_o;
+  void* dw_post;
+  void* dgate;
+  void* dw_pre;
+  int64_t B, H, D, groups;
+  int64_t r_stride;                      /* elements between the rows of r (backward: of r_out); r_out is dense */
+  int64_t o_head_stride, o_row_stride;
+  int64_t y_head_stride, y_row_stride;   /* of y; in the backward of dy */
+  int64_t dr_out_stride;
+  int64_t d_o_head_stride, d_o_row_stride;
+  float scale, eps;
+  int dtype, r_dtype;
+  int post;                              /* the post norm is applied */
+} fmlp_join;
+int fmlp_join_fwd(const fmlp_join* call, void* stream);
+size_t fmlp_join_bwd_workspace_bytes(const fmlp_join* call);
+int fmlp_join_bwd(const fmlp_join* call, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Global L2 norm of n gradients, and clipping: *norm = sqrt(sum of all squares) (fp32, on the device),
+ * outs[i] = grads[i] * min(1, max_norm / (norm + 1e-6)). No counterpart in the reference. Tensors are
+ * dense runs of numels[i] elements of dtypes[i] / out_dtypes[i] (fp16, bf16, fp32, each its own), aligned to
+ * their elements; outs[i] == grads[i] clips in place (and writes nothing where the norm is within
+ * max_norm), other overlaps are not allowed. Squares are summed in 64 bits in a fixed order. A norm that
+ * is infinite or NaN gives the coefficient 0 or NaN, as torch's clipping does. n = 0: the norm is 0. The
+ * arrays are read on the host before the call returns. workspace: fmlp_clip_workspace_bytes, never NULL.
+ */
+size_t fmlp_clip_workspace_bytes(int n, const int64_t* numels);
+int fmlp_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* dtypes, float* norm,
+                   void* workspace, size_t workspace_bytes, void* stream);
+int fmlp_clip_grads(int n, const void* const* grads, void* const* outs, const int64_t* numels, const int* dtypes,
+                    const int* out_dtypes, float max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                    void* stream);
 
 #ifdef __cplusplus
 }
