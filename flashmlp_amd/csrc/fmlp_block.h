@@ -38,6 +38,17 @@ hipError_t launch_gated_gen_fwd(const GatedArgs& a, hipStream_t st);
 hipError_t launch_gated_gen_dx(const GatedArgs& a, hipStream_t st);
 hipError_t launch_gated_gen_dw(const GatedArgs& a, hipStream_t st);
 
+// 16-bit io on LDS-staged kernels (fmlp_gated_fwd.hip): `tiles` row tiles of the large or small form, each split
+// over xs workgroups of nct chunks of 32 columns, whose fp32 partials take ws_bytes when xs > 1.
+struct GatedFwdPlan {
+  bool small;
+  long long tiles;
+  int xs, nct;
+  size_t ws_bytes;
+};
+GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus);
+hipError_t launch_gated_fwd(const GatedArgs& a, const GatedFwdPlan& p, hipStream_t st);
+
 // A block's join (fmlp_join.hip): the stream r (B, C), C = H D; o, y and their gradients (head, row, column)
 // with unit column stride. Pointers that are null leave their part out: o (no block output: only y is
 // taken from r), w_post, gate, w_pre (factors of one), r_out, y (results nobody asked for), and in the

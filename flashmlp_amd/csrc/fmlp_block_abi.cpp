@@ -55,13 +55,37 @@ int check_head_stride(int64_t s, const char* name, int64_t H, size_t es) {
   return FMLP_OK;
 }
 
+// Wg and Wu where rows of E elements are no whole 16-byte vectors: padded copies at the workspace's start
+size_t gated_pad_bytes(int64_t H, int64_t D, int64_t E, int io) {
+  return io == FMLP_DTYPE_F32 ? 0 : 2 * fmlp::w1_pad_bytes(H, D, E, (int)elem_bytes(io));
+}
+hipError_t gated_pad(fmlp::GatedArgs* a, hipStream_t st) {
+  const size_t one = fmlp::w1_pad_bytes(a->H, a->D, a->E, 2);
+  a->ldw = fmlp::w1_pitch(a->E, 2);
+  if (one == 0) return hipSuccess;
+  char* ws = (char*)a->ws;
+  hipError_t e = fmlp::launch_pad_w1(a->wg, ws, a->H, a->D, a->E, 2, st);
+  if (e == hipSuccess) e = fmlp::launch_pad_w1(a->wu, ws + one, a->H, a->D, a->E, 2, st);
+  a->wg = ws;
+  a->wu = ws + one;
+  a->ws = ws + 2 * one;
+  a->ws_bytes -= 2 * one;
+  return e;
+}
+int check_ws(const void* ws, size_t have, size_t need) {
+  if (need > 0 && (ws == nullptr || have < need))
+    return abi_fail(FMLP_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? have : (size_t)0, need);
+  return FMLP_OK;
+}
+
 int io_type(int io) { return io == FMLP_DTYPE_F32 ? fmlp::IO_F32 : io == FMLP_DTYPE_BF16 ? fmlp::IO_BF16 : fmlp::IO_F16; }
 
 }  // namespace
 
 FMLP_EXPORT size_t fmlp_gated_fwd_workspace_bytes(int64_t H, int64_t B, int64_t D, int64_t E, int dtype) {
-  (void)H, (void)B, (void)D, (void)E, (void)dtype;
-  return 0;
+  int cus = 0;
+  if (check_gated(H, B, D, E, dtype, 0) || dtype == FMLP_DTYPE_F32 || fmlp::abi_num_cus(&cus)) return 0;
+  return gated_pad_bytes(H, D, E, dtype) + fmlp::gated_fwd_plan(H, B, D, E, cus).ws_bytes;
 }
 
 FMLP_EXPORT size_t fmlp_gated_bwd_workspace_bytes(int64_t H, int64_t B, int64_t D, int64_t E, int dtype) {
@@ -99,7 +123,15 @@ FMLP_EXPORT int fmlp_gated_fwd(const void* x, const void* wg, const void* wu, co
   a.ws = workspace;
   a.ws_bytes = workspace != nullptr ? workspace_bytes : 0;
   if ((st = fmlp::abi_num_cus(&a.num_cus))) return st;
-  const hipError_t e = fmlp::launch_gated_gen_fwd(a, (hipStream_t)stream);
+  hipError_t e;
+  if (a.io == fmlp::IO_F32) {
+    e = fmlp::launch_gated_gen_fwd(a, (hipStream_t)stream);
+  } else {
+    const fmlp::GatedFwdPlan p = fmlp::gated_fwd_plan(H, B, D, E, a.num_cus);
+    if ((st = check_ws(workspace, workspace_bytes, gated_pad_bytes(H, D, E, dtype) + p.ws_bytes))) return st;
+    e = gated_pad(&a, (hipStream_t)stream);
+    if (e == hipSuccess) e = fmlp::launch_gated_fwd(a, p, (hipStream_t)stream);
+  }
   if (e != hipSuccess) return abi_fail(FMLP_ERR_HIP, "gated forward launch: %s", hipGetErrorString(e));
   return abi_ok();
 }
