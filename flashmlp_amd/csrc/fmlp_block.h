@@ -48,6 +48,18 @@ struct GatedFwdPlan {
 };
 GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus);
 hipError_t launch_gated_fwd(const GatedArgs& a, const GatedFwdPlan& p, hipStream_t st);
+// dX on the same forms and plan (fmlp_gated_dx.hip)
+hipError_t launch_gated_dx(const GatedArgs& a, const GatedFwdPlan& p, hipStream_t st);
+
+// dW programs (fmlp_gated_dw.hip): nE tiles of E and nS ranges of rows a head, whose fp32 partials
+// ([nS][dWg, dWu, dW2]) take ws_bytes when nS > 1.
+struct GatedDwPlan {
+  int nE, nS, rows_per_split;
+  long long programs;
+  size_t ws_bytes;
+};
+GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus);
+hipError_t launch_gated_dw(const GatedArgs& a, const GatedDwPlan& p, hipStream_t st);
 
 // A block's join (fmlp_join.hip): the stream r (B, C), C = H D; o, y and their gradients (head, row, column)
 // with unit column stride. Pointers that are null leave their part out: o (no block output: only y is

@@ -88,9 +88,21 @@ FMLP_EXPORT size_t fmlp_gated_fwd_workspace_bytes(int64_t H, int64_t B, int64_t 
   return gated_pad_bytes(H, D, E, dtype) + fmlp::gated_fwd_plan(H, B, D, E, cus).ws_bytes;
 }
 
+namespace {
+
+// the row sums' and the tile sums' partials share the workspace behind the padded weights
+size_t gated_bwd_ws(int64_t H, int64_t B, int64_t D, int64_t E, int dtype, int cus) {
+  const size_t dw = (dtype & FMLP_BWD_NO_DW) ? 0 : fmlp::gated_dw_plan(H, B, D, E, cus).ws_bytes;
+  const size_t dx = (dtype & FMLP_BWD_NO_DX) ? 0 : fmlp::gated_fwd_plan(H, B, D, E, cus).ws_bytes;
+  return gated_pad_bytes(H, D, E, io_of(dtype)) + (dw > dx ? dw : dx);
+}
+
+}  // namespace
+
 FMLP_EXPORT size_t fmlp_gated_bwd_workspace_bytes(int64_t H, int64_t B, int64_t D, int64_t E, int dtype) {
-  (void)H, (void)B, (void)D, (void)E, (void)dtype;
-  return 0;
+  int cus = 0;
+  if (check_gated(H, B, D, E, dtype, 0) || io_of(dtype) == FMLP_DTYPE_F32 || fmlp::abi_num_cus(&cus)) return 0;
+  return gated_bwd_ws(H, B, D, E, dtype, cus);
 }
 
 FMLP_EXPORT int fmlp_gated_fwd(const void* x, const void* wg, const void* wu, const void* w2, void* o, int64_t H,
@@ -174,9 +186,17 @@ FMLP_EXPORT int fmlp_gated_bwd(const void* x, const void* wg, const void* wu, co
   a.ws = workspace;
   a.ws_bytes = workspace != nullptr ? workspace_bytes : 0;
   if ((st = fmlp::abi_num_cus(&a.num_cus))) return st;
+  const hipStream_t hs = (hipStream_t)stream;
   hipError_t e = hipSuccess;
-  if (want_dw) e = fmlp::launch_gated_gen_dw(a, (hipStream_t)stream);
-  if (e == hipSuccess && want_dx) e = fmlp::launch_gated_gen_dx(a, (hipStream_t)stream);
+  if (a.io == fmlp::IO_F32) {
+    if (want_dw) e = fmlp::launch_gated_gen_dw(a, hs);
+    if (e == hipSuccess && want_dx) e = fmlp::launch_gated_gen_dx(a, hs);
+  } else if (want_dw || want_dx) {
+    if ((st = check_ws(workspace, workspace_bytes, gated_bwd_ws(H, B, D, E, dtype, a.num_cus)))) return st;
+    e = gated_pad(&a, hs);
+    if (e == hipSuccess && want_dw) e = fmlp::launch_gated_dw(a, fmlp::gated_dw_plan(H, B, D, E, a.num_cus), hs);
+    if (e == hipSuccess && want_dx) e = fmlp::launch_gated_dx(a, fmlp::gated_fwd_plan(H, B, D, E, a.num_cus), hs);
+  }
   if (e != hipSuccess) return abi_fail(FMLP_ERR_HIP, "gated backward launch: %s", hipGetErrorString(e));
   return abi_ok();
 }

@@ -18,6 +18,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+#include <utility>
+
 namespace fmlp {
 
 typedef unsigned short u16;
@@ -366,6 +369,16 @@ __device__ __forceinline__ constexpr int sched_index(int j, int n1, int n2) {
 // could be hoisted out of it, which collapses the interleave.
 __device__ __forceinline__ constexpr int sched_elem_begin(int j, int nsteps, int n_elem) {
   return (j * n_elem + nsteps - 1) / nsteps;
+}
+
+// f(integral_constant 0) .. f(integral_constant N - 1): a loop that is unrolled however large its body
+template <typename F, int... I>
+__device__ __forceinline__ void static_for_each(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F f) {
+  static_for_each(f, std::make_integer_sequence<int, N>{});
 }
 
 // ---------------------------------------------------------------------------------

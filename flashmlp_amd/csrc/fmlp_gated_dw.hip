@@ -1,0 +1,430 @@
+// Gated MLP backward for gfx950, 16-bit io: the weight gradients
+//   dWg = X^T dG, dWu = X^T dU, dW2 = h^T dO,   with  G = X Wg, U = X Wu, dH = dO W2^T,
+//   h = act(G) U, dG = dH U act'(G), dU = dH act(G)   recomputed per 32-row subtile.
+//
+// A wave owns 32 columns of E and, at D <= 128, all of D: its three gradient tiles (3 D / 32 accumulators of 16
+// values) and its columns of the weights stay in registers over the whole row range. G, U and dH come out with one
+// lane per column of E, which is the operand layout of the gradients' products, so h, dG and dU (rounded to the
+// io type) never leave registers. The four waves of a workgroup share the rows: X and dO subtiles land in an LDS
+// ring by buffer loads, swizzled so that the row reads (operands of G, U, dH) and the transposed reads (operands
+// of the gradients) are both free of bank conflicts. At D = 256 a wave owns half of D, and two waves compute the
+// same h, dG and dU.
+//
+// Bound by matrix and vector issue: a subtile has 6 D / 16 products (at D = 256 per wave 4.5 D / 16) and 16
+// activations with their derivatives a lane. One product and a share of vector work a step:
+//     G(i+1)     | dG(i), dU(i) packed
+//     gradients of subtile i, U(i+1)  | act, act' of i + 1
+//     dH(i+1)    | h(i+1) packed, U act'
+// Rows are split over nS programs where the columns of E alone leave CUs idle; their fp32 partials are added in
+// order by a second launch.
+#include <algorithm>
+#include <type_traits>
+
+#include "fmlp_block.h"
+#include "fmlp_device.h"
+
+namespace fmlp {
+namespace {
+
+// EW groups of 32 columns, DP parts of D, NS ring slots; WREG: weight matrices held in registers (3; 2: W2 in LDS;
+// 0: all in LDS)
+struct Form {
+  int ew, dp, ns, oc, wreg;
+};
+__host__ __device__ constexpr Form dw_form(int D) {
+  return D == 32 ? Form{4, 1, 4, 2, 3} : D == 64 ? Form{4, 1, 4, 2, 0} : D == 128 ? Form{4, 1, 4, 1, 3} : Form{2, 2, 4, 1, 2};
+}
+__host__ __device__ constexpr int dw_lds(int D) {
+  const Form f = dw_form(D);
+  const int w = f.wreg == 3 ? 0 : f.wreg == 2 ? 64 * D * f.ew : 192 * D * f.ew;
+  return f.ns * 128 * D + w;
+}
+
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+  if constexpr (D == 32) return (r >> 2) & 3;
+  else return (int)swz16<D == 64 ? 64 : 128>((unsigned)r);
+}
+
+template <bool BF16, int D, int DG, int ACT>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(dw_form(D).oc, dw_form(D).oc)))
+gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16* __restrict__ Wu,
+                const u16* __restrict__ W2, const u16* __restrict__ dO, void* __restrict__ dWg, void* __restrict__ dWu,
+                void* __restrict__ dW2, int H, int B, int E, int ldw, long long sx, long long sdo, int nE, int nS,
+                int rows_per_split, float* __restrict__ ws) {
+  constexpr Form F = dw_form(D);
+  constexpr int EW = F.ew, DP = F.dp, NS = F.ns, PF = NS - 1, WREG = F.wreg;
+  constexpr int KS = DG / 16, NTO = D / 32 / DP, ROWB = 2 * D, PPR = D / 8, SLOT = 128 * D, DOO = 64 * D;
+  constexpr int NPR = D >= 64 ? D / 64 : 1, NLD = D >= 64 ? 2 * NPR : 1;  // loads a thread for X (and dO)
+  constexpr int WL = NS * SLOT, W2L = WL + (WREG == 0 ? 128 * D * EW : 0);  // weights in LDS behind the ring
+  static_assert(EW * DP == 4 && NLD * (PF - 2) < 64 && 128 * D * EW <= NS * SLOT, "form");
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int eg = DP == 1 ? wave : wave & (EW - 1), dp = DP == 1 ? 0 : wave / EW;
+  const int G = lane >> 4, i16 = lane & 15, g = lane >> 5, l32 = lane & 31;
+
+  const unsigned t = (unsigned)xcd_remap(blockIdx.x, gridDim.x);
+  const int et = (int)(t % (unsigned)nE);
+  const unsigned hs = t / (unsigned)nE;
+  const int s = (int)(hs % (unsigned)nS), h = (int)(hs / (unsigned)nS);
+  const int e0 = (et * EW + eg) * 32;
+  const int r0 = s * rows_per_split, r1 = min(B, r0 + rows_per_split), NSUB = max(0, (r1 - r0 + 31) >> 5);
+  const u16* Xh = X + (size_t)h * sx;
+  const u16* dOh = dO + (size_t)h * sdo;
+  const u16* Wgh = Wg + (size_t)h * DG * ldw;
+  const u16* Wuh = Wu + (size_t)h * DG * ldw;
+  const u16* W2h = W2 + (size_t)h * E * DG;
+
+  // ---- weights: this wave's columns of Wg, Wu as [D][32] tiles through LDS (the ring's place, or their own) ----
+  u32x4 wg[WREG ? KS : 1], wu[WREG ? KS : 1], w2[WREG == 3 ? KS : 1];
+  const int laneA = (8 * g + (i16 >> 2)) * 64 + 32 * (G & 1) + 8 * (i16 & 3);
+  const int wt = (WREG ? 0 : WL) + eg * 64 * D;
+  auto opWt = [&](int m, int k) {
+    const int a = wt + m * 64 * D * EW + laneA + k * 1024;
+    return cat(lds_read_tr(a), lds_read_tr(a + 256));
+  };
+  {
+    const int lim = E - e0, rem = clamp0(DG * ldw * 2 - 2 * e0, 0x7fffffff);
+    const i32x4 rg = make_rsrc_words(Wgh + e0, rem), ru = make_rsrc_words(Wuh + e0, rem);
+#pragma unroll
+    for (int i = 0; i < D / 16 / DP; ++i) {
+      const int k = i * DP + dp;
+      const unsigned p = (unsigned)(k * 64 + lane), q = (p & 3u) * 8u;
+      const unsigned o = (int)q < lim && (p >> 2) < (unsigned)DG ? (p >> 2) * (unsigned)ldw * 2u + q * 2u : BUF_OOB;
+      buf_load16_lds(rg, o, wt + k * 1024);
+      buf_load16_lds(ru, o, wt + 64 * D * EW + k * 1024);
+    }
+    if constexpr (WREG == 3) {
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        w2[k] = u32x4{0u, 0u, 0u, 0u};
+        if (e0 + l32 < E) w2[k] = *(const u32x4*)(W2h + (size_t)(e0 + l32) * DG + k * 16 + g * 8);
+      }
+    } else {  // rows e of the whole E-tile, swizzled as the subtiles are
+      const int eb = et * EW * 32;
+      const i32x4 r2 = make_rsrc_words(W2h + (size_t)eb * DG, clamp0(E - eb, EW * 32) * DG * 2);
+#pragma unroll
+      for (int i = 0; i < EW * 32 * PPR / 256; ++i) {
+        const int p = i * 256 + tid, r = p / PPR, q = (p % PPR) ^ swz<D>(r);
+        buf_load16_lds(r2, q * 8 < DG ? (unsigned)(r * DG * 2 + q * 16) : BUF_OOB, W2L + i * 4096 + wave * 1024);
+      }
+    }
+  }
+  auto barrier = [&]() {
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  wait_vmcnt<0>();
+  barrier();
+  if constexpr (WREG > 0) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      wg[k] = opWt(0, k);
+      wu[k] = opWt(1, k);
+    }
+    barrier();  // before the ring's loads land on the tiles
+  }
+
+  // ---- subtiles: X and dO rows r0 + 32 i .., 16-byte piece q of row r at place q ^ swz(r) ----
+  unsigned so[NPR];
+#pragma unroll
+  for (int k = 0; k < NPR; ++k) {
+    const int p = D >= 64 ? k * 256 + tid : tid & 127, r = p / PPR, q = (p % PPR) ^ swz<D>(r);
+    so[k] = q * 8 < DG ? (unsigned)(r * DG * 2 + q * 16) : BUF_OOB;
+  }
+  auto load_sub = [&](int i, int slot) {
+    const int b = r0 + 32 * i, n = clamp0(r1 - b, 32) * DG * 2;
+    const i32x4 rx = make_rsrc_words(Xh + (size_t)b * DG, n), rd = make_rsrc_words(dOh + (size_t)b * DG, n);
+    const int at = slot * SLOT + wave * 1024;
+    if constexpr (D < 64) {  // waves 0 and 1 load X, 2 and 3 dO
+      i32x4 r;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = __builtin_amdgcn_readfirstlane(wave < 2 ? rx[j] : rd[j]);
+      buf_load16_lds(r, so[0], at);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NPR; ++k) {
+        buf_load16_lds(rx, so[k], at + k * 4096);
+        buf_load16_lds(rd, so[k], at + DOO + k * 4096);
+      }
+    }
+  };
+  // row reads (row l32, columns 16 k + 8 g ..) and transposed reads (rows 16 s + 8 r + 4 g + i16 / 4, columns
+  // 32 nt + 16 (G % 2) + 4 (i16 % 4) ..)
+  int ro[KS], to[NTO][2];
+#pragma unroll
+  for (int k = 0; k < KS; ++k) ro[k] = l32 * ROWB + (((2 * k + g) ^ swz<D>(l32)) << 4);
+#pragma unroll
+  for (int n = 0; n < NTO; ++n)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = 8 * r + 4 * g + (i16 >> 2), q = 4 * (dp * NTO + n) + 2 * (G & 1) + ((i16 & 3) >> 1);
+      to[n][r] = row * ROWB + ((q ^ swz<D>(row)) << 4) + ((i16 & 1) << 3);
+    }
+  auto opRow = [&](int base, int k) { return lds_read16(base + ro[k]); };
+  auto opCol = [&](int base, int s2, int n) {
+    const int a = base + s2 * 16 * ROWB;
+    return cat(lds_read_tr(a + to[n][0]), lds_read_tr(a + to[n][1]));
+  };
+  auto weight = [&](int m, int k) -> u32x4 {
+    if constexpr (WREG == 3) return m == 0 ? wg[k] : m == 1 ? wu[k] : w2[k];
+    if (m == 2) return lds_read16(W2L + eg * 32 * ROWB + ro[k]);
+    if constexpr (WREG == 2) return m == 0 ? wg[k] : wu[k];
+    return opWt(m, k);
+  };
+
+  f32x16 ag[NTO], au[NTO], a2[NTO], zg, zu, dh;
+  float sv[16], fv[16];
+  u32x4 ph[2], pg[2], pu[2];
+#pragma unroll
+  for (int n = 0; n < NTO; ++n) ag[n] = au[n] = a2[n] = zero16();
+
+  if (NSUB > 0) {
+#pragma unroll
+    for (int i = 0; i < PF; ++i) load_sub(i, i);
+    wait_vmcnt<NLD*(PF > 2 ? PF - 2 : 0)>();
+    barrier();
+    zg = zu = dh = zero16();
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const u32x4 x = opRow(0, k);
+      zg = mfma<BF16>(x, weight(0, k), zg);
+      zu = mfma<BF16>(x, weight(1, k), zu);
+      dh = mfma<BF16>(opRow(DOO, k), weight(2, k), dh);
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) act_hf<ACT>(zg[e], sv[e], fv[e]);
+    auto make_h = [&](int e) {
+      fv[e] *= zu[e];
+      if (e & 1) ph[e >> 3][(e >> 1) & 3] = pack2<BF16>(sv[e - 1] * zu[e - 1], sv[e] * zu[e]);
+    };
+    auto make_d = [&](int e) {
+      if ((e & 1) == 0) return;
+      pg[e >> 3][(e >> 1) & 3] = pack2<BF16>(dh[e - 1] * fv[e - 1], dh[e] * fv[e]);
+      pu[e >> 3][(e >> 1) & 3] = pack2<BF16>(dh[e - 1] * sv[e - 1], dh[e] * sv[e]);
+    };
+#pragma unroll
+    for (int e = 0; e < 16; ++e) make_h(e);
+
+    // subtile i in `cur`, i + 1 in `nxt`; M: there is a subtile i + 1
+    auto iter = [&](auto MORE, int cur, int nxt) {
+      constexpr bool M = decltype(MORE)::value;
+      constexpr int N1 = M ? KS : 0, N2 = 6 * NTO, NOPS = 3 * N1 + N2;
+      const int b1 = nxt * SLOT, b2 = cur * SLOT;
+      // products: G, then (s, n) of the three gradients (one operand for dWg and dWu), then U, then dH
+      struct Op {
+        u32x4 a, w;
+      };
+      auto fetch = [&](auto J) {
+        constexpr int j = decltype(J)::value, i = j - N1, i2 = i - N2, i3 = i2 - N1;
+        Op op;
+        if constexpr (i < 0) {
+          op.a = opRow(b1, j);
+          if constexpr (WREG == 0) op.w = weight(0, j);
+        } else if constexpr (i2 < 0) {
+          constexpr int m = i % 3, n = i / 3 % NTO, s2 = i / 3 / NTO;
+          if constexpr (m == 0) op.a = opCol(b2, s2, n);
+          if constexpr (m == 2) op.a = opCol(b2 + DOO, s2, n);
+        } else if constexpr (i3 < 0) {
+          op.a = opRow(b1, i2);
+          if constexpr (WREG == 0) op.w = weight(1, i2);
+        } else {
+          op.a = opRow(b1 + DOO, i3);
+          if constexpr (WREG != 3) op.w = weight(2, i3);
+        }
+        return op;
+      };
+      constexpr int PD = 2;
+      Op ring[PD + 1];
+      static_for<PD>([&](auto J) { ring[J] = fetch(J); });
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (!M) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) make_d(e);
+      }
+      u32x4 xt;  // the operand that dWg and dWu share
+      static_for<NOPS>([&](auto J) {
+        constexpr int j = decltype(J)::value, i = j - N1, i2 = i - N2, i3 = i2 - N1;
+        const Op op = ring[j % (PD + 1)];
+        if constexpr (j + PD < NOPS) ring[(j + PD) % (PD + 1)] = fetch(std::integral_constant<int, j + PD>{});
+        if constexpr (i < 0) {
+          zg = mfma<BF16>(op.a, WREG ? wg[WREG ? j : 0] : op.w, j == 0 ? zero16() : zg);
+#pragma unroll
+          for (int e = 16 * j / N1; e < 16 * (j + 1) / N1; ++e) make_d(e);
+        } else if constexpr (i2 < 0) {
+          constexpr int m = i % 3, n = i / 3 % NTO, s2 = i / 3 / NTO;
+          if constexpr (m == 0) {
+            xt = op.a;
+            ag[n] = mfma<BF16>(xt, pg[s2], ag[n]);
+          } else if constexpr (m == 1) {
+            au[n] = mfma<BF16>(xt, pu[s2], au[n]);
+          } else {
+            a2[n] = mfma<BF16>(ph[s2], op.a, a2[n]);
+          }
+        } else if constexpr (i3 < 0) {
+          zu = mfma<BF16>(op.a, WREG ? wu[WREG ? i2 : 0] : op.w, i2 == 0 ? zero16() : zu);
+        } else {
+          dh = mfma<BF16>(op.a, WREG == 3 ? w2[WREG == 3 ? i3 : 0] : op.w, i3 == 0 ? zero16() : dh);
+#pragma unroll
+          for (int e = 16 * i3 / N1; e < 16 * (i3 + 1) / N1; ++e) make_h(e);
+        }
+        if constexpr (M && i >= 0 && i3 < 0) {
+          constexpr int NV = N2 + N1;
+#pragma unroll
+          for (int e = 16 * i / NV; e < 16 * (i + 1) / NV; ++e) act_hf<ACT>(zg[e], sv[e], fv[e]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    };
+    int cur = 0;
+    for (int i = 0; i + 1 < NSUB; ++i) {
+      const int nxt = cur + 1 == NS ? 0 : cur + 1, far = cur == 0 ? NS - 1 : cur - 1;
+      load_sub(i + PF, far);
+      iter(std::true_type{}, cur, nxt);
+      wait_vmcnt<NLD*(PF - 2)>();  // subtile i + 2
+      barrier();
+      cur = nxt;
+    }
+    iter(std::false_type{}, cur, cur);
+    wait_vmcnt<0>();  // subtiles past the last are still landing, as zeros
+  }
+
+  // ---- dW2 tiles: rows e, lane = column d; dWg, dWu tiles: rows d, lane = column e ----
+  const size_t n1 = (size_t)H * E * DG;  // values of each gradient
+  void *og = dWg, *ou = dWu, *o2 = dW2;
+  const bool f32 = nS > 1;
+  if (f32) {
+    og = ws + (size_t)s * 3 * n1;
+    ou = ws + ((size_t)s * 3 + 1) * n1;
+    o2 = ws + ((size_t)s * 3 + 2) * n1;
+  }
+#pragma unroll
+  for (int n = 0; n < NTO; ++n) {
+    const int d0 = (dp * NTO + n) * 32;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = 8 * (i >> 2) + 4 * g + (i & 3);
+      if (e0 + r < E && d0 + l32 < DG) {
+        const size_t at = ((size_t)h * E + e0 + r) * DG + d0 + l32;
+        if (f32) ((float*)o2)[at] = a2[n][i];
+        else ((u16*)o2)[at] = from_f32<BF16>(a2[n][i]);
+      }
+      if (e0 + l32 < E && d0 + r < DG) {
+        const size_t at = ((size_t)h * DG + d0 + r) * E + e0 + l32;
+        if (f32) {
+          ((float*)og)[at] = ag[n][i];
+          ((float*)ou)[at] = au[n][i];
+        } else {
+          ((u16*)og)[at] = from_f32<BF16>(ag[n][i]);
+          ((u16*)ou)[at] = from_f32<BF16>(au[n][i]);
+        }
+      }
+    }
+  }
+}
+
+// Sum of the row splits' partials in order, four values a thread.
+template <bool BF16>
+__global__ void __launch_bounds__(256) gated_dw_reduce(const float* __restrict__ ws, u16* dWg, u16* dWu, u16* dW2,
+                                                       long long quads, int nS) {
+  const long long q = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (q >= 3 * quads) return;
+  const int m = q >= 2 * quads ? 2 : q >= quads ? 1 : 0;
+  const float4* src = (const float4*)ws + q;
+  float4 v = src[0];
+  for (int s = 1; s < nS; ++s) {
+    const float4 u = src[(size_t)s * 3 * quads];
+    v.x += u.x;
+    v.y += u.y;
+    v.z += u.z;
+    v.w += u.w;
+  }
+  u16* dst = (m == 0 ? dWg : m == 1 ? dWu : dW2) + 4 * (q - m * quads);
+  *(u32x2*)dst = u32x2{pack2<BF16>(v.x, v.y), pack2<BF16>(v.z, v.w)};
+}
+
+struct Args {
+  const GatedArgs& a;
+  const GatedDwPlan& p;
+  hipStream_t st;
+};
+
+template <bool BF16, int D, int DG, int ACT>
+hipError_t launch(const Args& q) {
+  auto k = gated_dw_kernel<BF16, D, DG, ACT>;
+  constexpr int lds = dw_lds(D);
+  static std::atomic<unsigned long long> done{0};
+  hipError_t e = set_lds_once((const void*)k, lds, done);
+  if (e != hipSuccess) return e;
+  const GatedArgs& a = q.a;
+  hipLaunchKernelGGL(k, dim3((unsigned)q.p.programs), dim3(256), lds, q.st, (const u16*)a.x, (const u16*)a.wg,
+                     (const u16*)a.wu, (const u16*)a.w2, (const u16*)a.dout, a.dwg, a.dwu, a.dw2, (int)a.H, (int)a.B,
+                     (int)a.E, (int)a.ldw, (long long)a.sx, (long long)a.sdo, q.p.nE, q.p.nS, q.p.rows_per_split,
+                     (float*)a.ws);
+  if ((e = hipGetLastError()) != hipSuccess || q.p.nS == 1) return e;
+  const long long quads = (long long)a.H * a.E * a.D / 4, blocks = (3 * quads + 255) / 256;
+  hipLaunchKernelGGL(gated_dw_reduce<BF16>, dim3((unsigned)blocks), dim3(256), 0, q.st, (const float*)a.ws, (u16*)a.dwg,
+                     (u16*)a.dwu, (u16*)a.dw2, quads, q.p.nS);
+  return hipGetLastError();
+}
+template <bool BF16, int D, int DG = D>
+hipError_t by_act(const Args& q) {
+  switch (q.a.act) {
+    case ACT_SILU: return launch<BF16, D, DG, ACT_SILU>(q);
+    case ACT_LEAKY: return launch<BF16, D, DG, ACT_LEAKY>(q);
+    case ACT_SIGMOID: return launch<BF16, D, DG, ACT_SIGMOID>(q);
+    default: return launch<BF16, D, DG, ACT_NONE>(q);
+  }
+}
+template <bool BF16>
+hipError_t by_d(const Args& q) {
+  switch (q.a.D) {
+    case 16: return by_act<BF16, 32, 16>(q);
+    case 32: return by_act<BF16, 32>(q);
+    case 64: return by_act<BF16, 64>(q);
+    case 128: return by_act<BF16, 128>(q);
+    default: return by_act<BF16, 256>(q);
+  }
+}
+
+}  // namespace
+
+GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus) {
+  const int DT = D < 32 ? 32 : (int)D;
+  const Form F = dw_form(DT);
+  GatedDwPlan p{};
+  p.nE = (int)((E + 32 * F.ew - 1) / (32 * F.ew));
+  const long long base = H * p.nE, slots = (long long)std::max(num_cus, 1) * F.oc, subs = (B + 31) / 32;
+  static const int force = env_int("FMLP_GATED_NS", -1);
+  // rounds of programs, each a fixed part and its subtiles; a split adds the partials' traffic and a launch
+  const double sub_us = (DT == 32 ? 0.35 : DT == 64 ? 0.6 : DT == 128 ? 1.0 : 1.6), fixed_us = 4.0;
+  double best = 0;
+  p.nS = 1;
+  p.rows_per_split = (int)std::max<long long>(subs * 32, 32);
+  for (long long n = 1; n <= 64 && (n == 1 || n <= subs / 2); ++n) {
+    if (force > 0 && n != std::min<long long>(force, std::max<long long>(subs / 2, 1))) continue;
+    const long long per = (subs + n - 1) / n, m = per > 0 ? (subs + per - 1) / per : 1;
+    if (m != n && n > 1) continue;
+    const double rounds = (double)((base * n + slots - 1) / slots);
+    double t = rounds * (fixed_us + sub_us * (double)per);
+    if (n > 1) t += 4.0 + (double)(3 * H * D * E) * 4.0 * (double)n * 2.0 / 3.0e6;
+    if (best == 0 || t < best) {
+      best = t;
+      p.nS = (int)n;
+      p.rows_per_split = (int)std::max<long long>(per * 32, 32);
+    }
+  }
+  p.programs = base * p.nS;
+  p.ws_bytes = p.nS > 1 ? (size_t)p.nS * 3 * H * D * E * sizeof(float) : 0;
+  return p;
+}
+
+hipError_t launch_gated_dw(const GatedArgs& a, const GatedDwPlan& p, hipStream_t st) {
+  if (p.programs <= 0) return hipSuccess;
+  const Args q{a, p, st};
+  return a.io == IO_BF16 ? by_d<true>(q) : by_d<false>(q);
+}
+
+}  // namespace fmlp
