@@ -61,6 +61,13 @@ struct GatedDwPlan {
 GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus);
 hipError_t launch_gated_dw(const GatedArgs& a, const GatedDwPlan& p, hipStream_t st);
 
+// fp32 io at D <= 128 (fmlp_gated_f32.hip): tiles of 128 rows, E-tiles of 128 columns.
+GatedFwdPlan gated32_rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus);
+GatedDwPlan gated32_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus);
+hipError_t launch_gated32_fwd(const GatedArgs& a, const GatedFwdPlan& p, hipStream_t st);
+hipError_t launch_gated32_dx(const GatedArgs& a, const GatedFwdPlan& p, hipStream_t st);
+hipError_t launch_gated32_dw(const GatedArgs& a, const GatedDwPlan& p, hipStream_t st);
+
 // A block's join (fmlp_join.hip): the stream r (B, C), C = H D; o, y and their gradients (head, row, column)
 // with unit column stride. Pointers that are null leave their part out: o (no block output: only y is
 // taken from r), w_post, gate, w_pre (factors of one), r_out, y (results nobody asked for), and in the

@@ -55,22 +55,32 @@ int check_head_stride(int64_t s, const char* name, int64_t H, size_t es) {
   return FMLP_OK;
 }
 
+// fp32 at D = 256 alone runs on the kernels that read operands from global memory, without a workspace
+bool gated_staged(int64_t D, int io) { return io != FMLP_DTYPE_F32 || D <= 128; }
+
 // Wg and Wu where rows of E elements are no whole 16-byte vectors: padded copies at the workspace's start
 size_t gated_pad_bytes(int64_t H, int64_t D, int64_t E, int io) {
-  return io == FMLP_DTYPE_F32 ? 0 : 2 * fmlp::w1_pad_bytes(H, D, E, (int)elem_bytes(io));
+  return 2 * fmlp::w1_pad_bytes(H, D, E, (int)elem_bytes(io));
 }
 hipError_t gated_pad(fmlp::GatedArgs* a, hipStream_t st) {
-  const size_t one = fmlp::w1_pad_bytes(a->H, a->D, a->E, 2);
-  a->ldw = fmlp::w1_pitch(a->E, 2);
+  const int es = a->io == fmlp::IO_F32 ? 4 : 2;
+  const size_t one = fmlp::w1_pad_bytes(a->H, a->D, a->E, es);
+  a->ldw = fmlp::w1_pitch(a->E, es);
   if (one == 0) return hipSuccess;
   char* ws = (char*)a->ws;
-  hipError_t e = fmlp::launch_pad_w1(a->wg, ws, a->H, a->D, a->E, 2, st);
-  if (e == hipSuccess) e = fmlp::launch_pad_w1(a->wu, ws + one, a->H, a->D, a->E, 2, st);
+  hipError_t e = fmlp::launch_pad_w1(a->wg, ws, a->H, a->D, a->E, es, st);
+  if (e == hipSuccess) e = fmlp::launch_pad_w1(a->wu, ws + one, a->H, a->D, a->E, es, st);
   a->wg = ws;
   a->wu = ws + one;
   a->ws = ws + 2 * one;
   a->ws_bytes -= 2 * one;
   return e;
+}
+fmlp::GatedFwdPlan rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int io, int cus) {
+  return io == FMLP_DTYPE_F32 ? fmlp::gated32_rows_plan(H, B, D, E, cus) : fmlp::gated_fwd_plan(H, B, D, E, cus);
+}
+fmlp::GatedDwPlan dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int io, int cus) {
+  return io == FMLP_DTYPE_F32 ? fmlp::gated32_dw_plan(H, B, D, E, cus) : fmlp::gated_dw_plan(H, B, D, E, cus);
 }
 int check_ws(const void* ws, size_t have, size_t need) {
   if (need > 0 && (ws == nullptr || have < need))
@@ -84,24 +94,25 @@ int io_type(int io) { return io == FMLP_DTYPE_F32 ? fmlp::IO_F32 : io == FMLP_DT
 
 FMLP_EXPORT size_t fmlp_gated_fwd_workspace_bytes(int64_t H, int64_t B, int64_t D, int64_t E, int dtype) {
   int cus = 0;
-  if (check_gated(H, B, D, E, dtype, 0) || dtype == FMLP_DTYPE_F32 || fmlp::abi_num_cus(&cus)) return 0;
-  return gated_pad_bytes(H, D, E, dtype) + fmlp::gated_fwd_plan(H, B, D, E, cus).ws_bytes;
+  if (check_gated(H, B, D, E, dtype, 0) || !gated_staged(D, dtype) || fmlp::abi_num_cus(&cus)) return 0;
+  return gated_pad_bytes(H, D, E, dtype) + rows_plan(H, B, D, E, dtype, cus).ws_bytes;
 }
 
 namespace {
 
 // the row sums' and the tile sums' partials share the workspace behind the padded weights
 size_t gated_bwd_ws(int64_t H, int64_t B, int64_t D, int64_t E, int dtype, int cus) {
-  const size_t dw = (dtype & FMLP_BWD_NO_DW) ? 0 : fmlp::gated_dw_plan(H, B, D, E, cus).ws_bytes;
-  const size_t dx = (dtype & FMLP_BWD_NO_DX) ? 0 : fmlp::gated_fwd_plan(H, B, D, E, cus).ws_bytes;
-  return gated_pad_bytes(H, D, E, io_of(dtype)) + (dw > dx ? dw : dx);
+  const int io = io_of(dtype);
+  const size_t dw = (dtype & FMLP_BWD_NO_DW) ? 0 : dw_plan(H, B, D, E, io, cus).ws_bytes;
+  const size_t dx = (dtype & FMLP_BWD_NO_DX) ? 0 : rows_plan(H, B, D, E, io, cus).ws_bytes;
+  return gated_pad_bytes(H, D, E, io) + (dw > dx ? dw : dx);
 }
 
 }  // namespace
 
 FMLP_EXPORT size_t fmlp_gated_bwd_workspace_bytes(int64_t H, int64_t B, int64_t D, int64_t E, int dtype) {
   int cus = 0;
-  if (check_gated(H, B, D, E, dtype, 0) || io_of(dtype) == FMLP_DTYPE_F32 || fmlp::abi_num_cus(&cus)) return 0;
+  if (check_gated(H, B, D, E, dtype, 0) || !gated_staged(D, io_of(dtype)) || fmlp::abi_num_cus(&cus)) return 0;
   return gated_bwd_ws(H, B, D, E, dtype, cus);
 }
 
@@ -135,14 +146,15 @@ FMLP_EXPORT int fmlp_gated_fwd(const void* x, const void* wg, const void* wu, co
   a.ws = workspace;
   a.ws_bytes = workspace != nullptr ? workspace_bytes : 0;
   if ((st = fmlp::abi_num_cus(&a.num_cus))) return st;
+  const hipStream_t hs = (hipStream_t)stream;
   hipError_t e;
-  if (a.io == fmlp::IO_F32) {
-    e = fmlp::launch_gated_gen_fwd(a, (hipStream_t)stream);
+  if (!gated_staged(D, dtype)) {
+    e = fmlp::launch_gated_gen_fwd(a, hs);
   } else {
-    const fmlp::GatedFwdPlan p = fmlp::gated_fwd_plan(H, B, D, E, a.num_cus);
+    const fmlp::GatedFwdPlan p = rows_plan(H, B, D, E, dtype, a.num_cus);
     if ((st = check_ws(workspace, workspace_bytes, gated_pad_bytes(H, D, E, dtype) + p.ws_bytes))) return st;
-    e = gated_pad(&a, (hipStream_t)stream);
-    if (e == hipSuccess) e = fmlp::launch_gated_fwd(a, p, (hipStream_t)stream);
+    e = gated_pad(&a, hs);
+    if (e == hipSuccess) e = a.io == fmlp::IO_F32 ? fmlp::launch_gated32_fwd(a, p, hs) : fmlp::launch_gated_fwd(a, p, hs);
   }
   if (e != hipSuccess) return abi_fail(FMLP_ERR_HIP, "gated forward launch: %s", hipGetErrorString(e));
   return abi_ok();
@@ -187,15 +199,22 @@ FMLP_EXPORT int fmlp_gated_bwd(const void* x, const void* wg, const void* wu, co
   a.ws_bytes = workspace != nullptr ? workspace_bytes : 0;
   if ((st = fmlp::abi_num_cus(&a.num_cus))) return st;
   const hipStream_t hs = (hipStream_t)stream;
+  const int io = io_of(dtype);
   hipError_t e = hipSuccess;
-  if (a.io == fmlp::IO_F32) {
+  if (!gated_staged(D, io)) {
     if (want_dw) e = fmlp::launch_gated_gen_dw(a, hs);
     if (e == hipSuccess && want_dx) e = fmlp::launch_gated_gen_dx(a, hs);
   } else if (want_dw || want_dx) {
     if ((st = check_ws(workspace, workspace_bytes, gated_bwd_ws(H, B, D, E, dtype, a.num_cus)))) return st;
     e = gated_pad(&a, hs);
-    if (e == hipSuccess && want_dw) e = fmlp::launch_gated_dw(a, fmlp::gated_dw_plan(H, B, D, E, a.num_cus), hs);
-    if (e == hipSuccess && want_dx) e = fmlp::launch_gated_dx(a, fmlp::gated_fwd_plan(H, B, D, E, a.num_cus), hs);
+    if (e == hipSuccess && want_dw) {
+      const fmlp::GatedDwPlan p = dw_plan(H, B, D, E, io, a.num_cus);
+      e = a.io == fmlp::IO_F32 ? fmlp::launch_gated32_dw(a, p, hs) : fmlp::launch_gated_dw(a, p, hs);
+    }
+    if (e == hipSuccess && want_dx) {
+      const fmlp::GatedFwdPlan p = rows_plan(H, B, D, E, io, a.num_cus);
+      e = a.io == fmlp::IO_F32 ? fmlp::launch_gated32_dx(a, p, hs) : fmlp::launch_gated_dx(a, p, hs);
+    }
   }
   if (e != hipSuccess) return abi_fail(FMLP_ERR_HIP, "gated backward launch: %s", hipGetErrorString(e));
   return abi_ok();
