@@ -23,7 +23,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .flashmlp import _DTYPES, _alloc_ws, _ptr
+from .flashmlp import _DTYPES, _alloc_ws, _fast, _ptr
 from .gated import _On
 
 
@@ -208,6 +208,10 @@ def block_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, heads:
         dtype: of the result (the weight's, or x's without a weight); x may be fp32 beside a 16-bit one.
     """
     dtype = dtype or (weight.dtype if weight is not None else x.dtype)
+    if _fast is not None and dtype in _DTYPES and heads != 0:  # tensors that need no copies and no error: else None
+        r = _fast.join(x, None, None, None, weight, 1.0, True, eps, heads or 0, _DTYPES[dtype])
+        if r is not None:
+            return r[1]
     if _needs_grad(x, weight):
         return BlockJoinFunction.apply(x, None, None, None, weight, 1.0, True, True, eps, heads, dtype)[1]
     return block_join_fwd(x, None, pre_weight=weight, eps=eps, heads=heads, dtype=dtype)[1]
@@ -223,6 +227,10 @@ def block_join(residual: torch.Tensor, o: torch.Tensor, post_weight: Optional[to
         gate: (C,) or (G, C) with B % G == 0, or None; scale: a number; post=False joins o without its
         norm; pre=False leaves y out.
     """
+    if _fast is not None and pre and o is not None:  # as in block_norm
+        r = _fast.join(residual, o, post_weight, gate, pre_weight, scale, post, eps, 0, 0)
+        if r is not None:
+            return r
     if _needs_grad(residual, o, post_weight, gate, pre_weight):
         return BlockJoinFunction.apply(residual, o, post_weight, gate, pre_weight, scale, post, pre, eps, None, None)
     return block_join_fwd(residual, o, post_weight, gate, scale, pre_weight=pre_weight, post=post, pre=pre, eps=eps)[:2]

@@ -19,7 +19,7 @@ from typing import Iterable, List, Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
-from .flashmlp import _DTYPES
+from .flashmlp import _DTYPES, _fast
 from .gated import _On
 
 
@@ -73,6 +73,9 @@ def grad_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
     grads = list(grads)
     if not grads:
         return torch.zeros(())
+    norm = _fast.clip(grads, None, 0.0) if _fast is not None else None  # dense tensors on one GPU: else None
+    if norm is not None:
+        return norm
     dev = _check(grads, "gradients")
     return _run([g if _one_run(g) else g.contiguous() for g in grads], None, 0.0, dev)
 
@@ -96,6 +99,9 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *,
         raise ValueError(f"{len(grads)} gradients, {len(outs)} outputs")
     if not grads:
         return outs, torch.zeros(())
+    norm = _fast.clip(grads, outs, max_norm) if _fast is not None else None  # as in grad_norm
+    if norm is not None:
+        return outs, norm
     dev = _check(grads, "gradients")
     if out is not None:
         if _check(outs, "outputs") != dev:

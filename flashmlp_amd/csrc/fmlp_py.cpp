@@ -1,4 +1,5 @@
-// _fmlp_fast: the per-call fast path of flashmlp_fwd / flashmlp_bwd (flashmlp_amd/flashmlp.py).
+// _fmlp_fast: the per-call fast path of flashmlp_fwd / flashmlp_bwd (flashmlp_amd/flashmlp.py), and of the gated
+// block's operators (gated.py, block.py, clip.py; below).
 //
 // A CPython module (METH_FASTCALL) over the C ABI of libflashmlp.so for the common case:
 // inputs on one GPU, a shape with kernels of its own (views that they do not read in place are copied
@@ -15,9 +16,12 @@
 #include <c10/hip/HIPStream.h>
 #include <c10/util/Exception.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstdint>
+#include <vector>
 
 #include "flashmlp.h"
 
@@ -248,13 +252,435 @@ PyObject* fast_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------------------------
+// The gated block's operators. Calls that need no copies and no error message run here, with their
+// autograd nodes in C++; for any other call these return None and the Python module takes its general path.
+// ---------------------------------------------------------------------------------------------
+[[noreturn]] void raise_status(int st, const char* what) {
+  TORCH_CHECK(false, "flashmlp ", what, " failed: ", fmlp_status_string(st), ": ", fmlp_last_error());
+  __builtin_unreachable();
+}
+void check_status(int st, const char* what) {
+  if (st != FMLP_OK) raise_status(st, what);
+}
+
+// a second derivative would need these backward passes to be differentiable
+void check_once() {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "FlashMLP's gradients cannot be differentiated again (create_graph=True)");
+}
+
+// x (0), weights (1 .. 3) and dout (4) as the kernels read them in place
+bool gated_ok(const at::Tensor* const* ts, int n, int* code) {
+  const at::Tensor& x = *ts[0];
+  if (!x.is_cuda()) return false;
+  *code = io_code(x);
+  if (*code < 0) return false;
+  for (int i = 0; i < n; ++i) {
+    const at::Tensor& t = *ts[i];
+    if (t.scalar_type() != x.scalar_type() || t.device() != x.device() || t.layout() != at::kStrided || t.dim() != 3 ||
+        t.is_neg())
+      return false;
+    if (!dense16(t) && !((i == 0 || i == 4) && rows16(t))) return false;
+  }
+  const at::Tensor &wg = *ts[1], &wu = *ts[2], &w2 = *ts[3];
+  const int64_t H = x.size(0), D = x.size(2), E = wg.size(2);
+  if (wg.size(0) != H || wg.size(1) != D || wu.sizes() != wg.sizes() || w2.size(0) != H || w2.size(1) != E || w2.size(2) != D)
+    return false;
+  return n < 5 || ts[4]->sizes() == x.sizes();
+}
+
+at::Tensor gated_fwd_run(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& w2, int code,
+                         int act) {
+  const int64_t H = x.size(0), B = x.size(1), D = x.size(2), E = wg.size(2);
+  c10::DeviceGuard guard(x.device());
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(x.device().index()).stream();
+  at::Tensor o = empty_dense(x), ws;
+  const size_t n = fmlp_gated_fwd_workspace_bytes(H, B, D, E, code);
+  if (n) ws = bytes_on(x, n);
+  check_status(fmlp_gated_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), w2.data_ptr(), o.data_ptr(), H, B, D, E,
+                              x.stride(0), code, act, n ? ws.data_ptr() : nullptr, n, stream),
+               "gated forward");
+  return o;
+}
+
+// (dx, dwg, dwu, dw2); those that are not wanted undefined
+std::vector<at::Tensor> gated_bwd_run(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& w2,
+                                      const at::Tensor& dout, int code, int act, bool need_dx, bool need_dw) {
+  std::vector<at::Tensor> g(4);
+  if (!need_dx && !need_dw) return g;
+  const int64_t H = x.size(0), B = x.size(1), D = x.size(2), E = wg.size(2);
+  c10::DeviceGuard guard(x.device());
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(x.device().index()).stream();
+  if (need_dx) g[0] = empty_dense(x);
+  if (need_dw) {
+    g[1] = at::empty_like(wg);
+    g[2] = at::empty_like(wu);
+    g[3] = at::empty_like(w2);
+  }
+  const int flags = code | (need_dx ? 0 : FMLP_BWD_NO_DX) | (need_dw ? 0 : FMLP_BWD_NO_DW);
+  at::Tensor ws;
+  const size_t n = fmlp_gated_bwd_workspace_bytes(H, B, D, E, flags);
+  if (n) ws = bytes_on(x, n);
+  auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  check_status(fmlp_gated_bwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), w2.data_ptr(), dout.data_ptr(), ptr(g[0]),
+                              ptr(g[1]), ptr(g[2]), ptr(g[3]), H, B, D, E, x.stride(0), dout.stride(0), flags, act,
+                              n ? ws.data_ptr() : nullptr, n, stream),
+               "gated backward");
+  return g;
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct GatedFn : torch::autograd::Function<GatedFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
+                            const at::Tensor& w2, int64_t code, int64_t act) {
+    ctx->save_for_backward({x, wg, wu, w2});
+    ctx->saved_data["code"] = code;
+    ctx->saved_data["act"] = act;
+    return gated_fwd_run(x, wg, wu, w2, (int)code, (int)act);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_once();
+    const auto s = ctx->get_saved_variables();
+    const int code = (int)ctx->saved_data["code"].toInt(), act = (int)ctx->saved_data["act"].toInt();
+    at::Tensor dout = grads[0];
+    if (!dout.defined()) return variable_list(6);
+    if (!rows16(dout) || dout.is_neg()) {
+      dout = dout.contiguous();
+      if (!dense16(dout)) dout = dout.clone(at::MemoryFormat::Contiguous);
+    }
+    const bool dw = ctx->needs_input_grad(1) || ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
+    auto g = gated_bwd_run(s[0], s[1], s[2], s[3], dout, code, act, ctx->needs_input_grad(0), dw);
+    variable_list r(6);
+    for (int i = 0; i < 4; ++i)
+      if (ctx->needs_input_grad(i)) r[i] = g[i];
+    return r;
+  }
+};
+
+bool unpack(PyObject* const* args, int n, const at::Tensor** ts) {
+  for (int i = 0; i < n; ++i) {
+    if (!THPVariable_Check(args[i])) return false;
+    ts[i] = &THPVariable_Unpack(args[i]);
+  }
+  return true;
+}
+
+// gated_fwd(x, wg, wu, w2, act) -> o, or None
+PyObject* fast_gated_fwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* ts[4];
+  int code = 0;
+  if (nargs != 5 || !unpack(args, 4, ts) || !gated_ok(ts, 4, &code)) Py_RETURN_NONE;
+  const int act = (int)PyLong_AsLong(args[4]);
+  if (act == -1 && PyErr_Occurred()) return nullptr;
+  return THPVariable_Wrap(gated_fwd_run(*ts[0], *ts[1], *ts[2], *ts[3], code, act));
+  END_HANDLE_TH_ERRORS
+}
+
+// gated(x, wg, wu, w2, act) -> o with its autograd node, or None
+PyObject* fast_gated(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* ts[4];
+  int code = 0;
+  if (nargs != 5 || !unpack(args, 4, ts) || !gated_ok(ts, 4, &code)) Py_RETURN_NONE;
+  const int act = (int)PyLong_AsLong(args[4]);
+  if (act == -1 && PyErr_Occurred()) return nullptr;
+  return THPVariable_Wrap(GatedFn::apply(*ts[0], *ts[1], *ts[2], *ts[3], (int64_t)code, (int64_t)act));
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_bwd(x, wg, wu, w2, do, act, need_dx, need_dw) -> (dx, dwg, dwu, dw2), or None
+PyObject* fast_gated_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* ts[5];
+  int code = 0;
+  if (nargs != 8 || !unpack(args, 5, ts) || !gated_ok(ts, 5, &code)) Py_RETURN_NONE;
+  const int act = (int)PyLong_AsLong(args[5]);
+  if (act == -1 && PyErr_Occurred()) return nullptr;
+  auto g = gated_bwd_run(*ts[0], *ts[1], *ts[2], *ts[3], *ts[4], code, act, PyObject_IsTrue(args[6]) == 1,
+                         PyObject_IsTrue(args[7]) == 1);
+  return Py_BuildValue("(NNNN)", wrap_or_none(g[0]), wrap_or_none(g[1]), wrap_or_none(g[2]), wrap_or_none(g[3]));
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- join ----
+struct JoinCfg {
+  double scale, eps;
+  bool post;
+  int64_t heads;  // without o: heads of y, 0 for rows
+  at::ScalarType dtype;
+};
+
+const void* cptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void* mptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void head_strides(const at::Tensor& t, int64_t* sh, int64_t* sr) {
+  *sh = t.dim() == 3 ? t.stride(0) : 0;
+  *sr = t.stride(t.dim() - 2);
+}
+int code_of(at::ScalarType t) { return t == at::kHalf ? FMLP_DTYPE_F16 : t == at::kBFloat16 ? FMLP_DTYPE_BF16 : FMLP_DTYPE_F32; }
+
+fmlp_join join_call(const at::Tensor& r, const at::Tensor& o, const at::Tensor& w_post, const at::Tensor& gate,
+                    const at::Tensor& w_pre, const JoinCfg& c) {
+  fmlp_join j{};
+  j.o = cptr(o);
+  j.w_post = cptr(w_post);
+  j.gate = cptr(gate);
+  j.w_pre = cptr(w_pre);
+  j.B = r.size(0);
+  j.H = o.defined() ? (o.dim() == 3 ? o.size(0) : 1) : std::max<int64_t>(c.heads, 1);
+  j.D = r.size(1) / j.H;
+  j.groups = gate.defined() && gate.dim() == 2 ? gate.size(0) : 1;
+  j.r_stride = r.stride(0);
+  if (o.defined()) head_strides(o, &j.o_head_stride, &j.o_row_stride);
+  j.scale = (float)c.scale;
+  j.eps = (float)c.eps;
+  j.post = c.post ? 1 : 0;
+  j.dtype = code_of(c.dtype);
+  j.r_dtype = code_of(r.scalar_type());
+  return j;
+}
+
+bool cols1(const at::Tensor& t) { return t.stride(t.dim() - 1) == 1 && !t.is_neg(); }
+
+// the call needs no copies, and no error: (r (B, C), o (H, B, D) or (B, C) or none, vectors of C)
+bool join_ok(const at::Tensor& r, const at::Tensor& o, const at::Tensor& w_post, const at::Tensor& gate,
+             const at::Tensor& w_pre, const JoinCfg& c) {
+  if (!r.is_cuda() || r.layout() != at::kStrided || r.dim() != 2 || r.size(1) < 1 || !cols1(r)) return false;
+  if (c.dtype != at::kHalf && c.dtype != at::kBFloat16 && c.dtype != at::kFloat) return false;
+  if (r.scalar_type() != c.dtype && r.scalar_type() != at::kFloat) return false;
+  const int64_t B = r.size(0), C = r.size(1);
+  for (const at::Tensor* t : {&o, &w_post, &gate, &w_pre})
+    if (t->defined() && (t->scalar_type() != c.dtype || t->device() != r.device() || t->layout() != at::kStrided || t->is_neg()))
+      return false;
+  if (o.defined()) {
+    if (o.dim() != 2 && o.dim() != 3) return false;
+    if (o.size(o.dim() - 2) != B || !cols1(o) || (o.dim() == 3 ? o.size(0) * o.size(2) : o.size(1)) != C) return false;
+  } else if (w_post.defined() || gate.defined() || c.heads < 0 || (c.heads > 0 && C % c.heads != 0)) {
+    return false;
+  }
+  if (w_post.defined() && !c.post) return false;
+  for (const at::Tensor* t : {&w_post, &w_pre})
+    if (t->defined() && (t->dim() != 1 || t->size(0) != C || !t->is_contiguous())) return false;
+  if (gate.defined()) {
+    if ((gate.dim() != 1 && gate.dim() != 2) || gate.size(gate.dim() - 1) != C || !gate.is_contiguous()) return false;
+    if (gate.dim() == 2 && (gate.size(0) < 1 || B % gate.size(0) != 0)) return false;
+  }
+  return true;
+}
+
+// (r', y, rs); r' undefined without o, rs (2, B) undefined unless saved
+std::tuple<at::Tensor, at::Tensor, at::Tensor> join_fwd_run(const at::Tensor& r, const at::Tensor& o, const at::Tensor& w_post,
+                                                            const at::Tensor& gate, const at::Tensor& w_pre,
+                                                            const JoinCfg& c, bool save) {
+  c10::DeviceGuard guard(r.device());
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(r.device().index()).stream();
+  fmlp_join j = join_call(r, o, w_post, gate, w_pre, c);
+  at::Tensor r2, y, rs;
+  const auto opt = r.options().dtype(c.dtype);
+  if (o.defined()) r2 = r.is_contiguous() ? at::empty_like(r) : at::empty(r.sizes(), r.options());
+  if (o.defined() ? o.dim() == 3 : c.heads > 0) y = at::empty({j.H, j.B, j.D}, opt);
+  else y = at::empty({j.B, j.D}, opt);
+  if (save) rs = at::empty({2, j.B}, r.options().dtype(at::kFloat));
+  j.r = cptr(r);
+  j.r_out = mptr(r2);
+  j.y = mptr(y);
+  head_strides(y, &j.y_head_stride, &j.y_row_stride);
+  if (save) {
+    j.rs_o = rs.data_ptr<float>();
+    j.rs_r = j.rs_o + j.B;
+  }
+  check_status(fmlp_join_fwd(&j, stream), "join forward");
+  return {r2, y, rs};
+}
+
+at::Tensor cols(const at::Tensor& t) { return !t.defined() || cols1(t) ? t : t.contiguous(); }
+
+// (dr, do, dw_post, dgate, dw_pre); those that are not wanted undefined
+std::vector<at::Tensor> join_bwd_run(const at::Tensor& r2, const at::Tensor& o, const at::Tensor& rs, at::Tensor dr2,
+                                     at::Tensor dy, const at::Tensor& w_post, const at::Tensor& gate,
+                                     const at::Tensor& w_pre, const JoinCfg& c, const bool* need) {
+  c10::DeviceGuard guard(r2.device());
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(r2.device().index()).stream();
+  fmlp_join j = join_call(r2, o, w_post, gate, w_pre, c);
+  std::vector<at::Tensor> g(5);
+  dr2 = cols(dr2);
+  dy = cols(dy);
+  if (need[0]) g[0] = at::empty(r2.sizes(), r2.options());
+  if (need[1] && o.defined()) g[1] = at::empty(o.sizes(), o.options());
+  if (need[2] && w_post.defined()) g[2] = at::empty_like(w_post);
+  if (need[3] && gate.defined()) g[3] = at::empty_like(gate);
+  if (need[4] && w_pre.defined()) g[4] = dy.defined() ? at::empty_like(w_pre) : at::zeros_like(w_pre);
+  j.r_out = const_cast<void*>(cptr(r2));
+  j.rs_o = rs.data_ptr<float>();
+  j.rs_r = j.rs_o + j.B;
+  j.dr_out = cptr(dr2);
+  j.dy = cptr(dy);
+  if (!dy.defined()) j.w_pre = nullptr;
+  j.dr = mptr(g[0]);
+  j.d_o = mptr(g[1]);
+  j.dw_post = mptr(g[2]);
+  j.dgate = mptr(g[3]);
+  j.dw_pre = dy.defined() ? mptr(g[4]) : nullptr;
+  if (dr2.defined()) j.dr_out_stride = dr2.stride(0);
+  if (dy.defined()) head_strides(dy, &j.y_head_stride, &j.y_row_stride);
+  if (g[1].defined()) head_strides(g[1], &j.d_o_head_stride, &j.d_o_row_stride);
+  at::Tensor ws;
+  const size_t n = fmlp_join_bwd_workspace_bytes(&j);
+  if (n) ws = bytes_on(r2, n);
+  check_status(fmlp_join_bwd(&j, n ? ws.data_ptr() : nullptr, n, stream), "join backward");
+  return g;
+}
+
+struct JoinFn : torch::autograd::Function<JoinFn> {
+  using Opt = std::optional<at::Tensor>;
+  // with o: (r', y); without: (y)
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& r, const Opt& o_, const Opt& w_post_,
+                               const Opt& gate_, const Opt& w_pre_, const JoinCfg& c) {
+    const at::Tensor o = o_.value_or(at::Tensor()), w_post = w_post_.value_or(at::Tensor()),
+                     gate = gate_.value_or(at::Tensor()), w_pre = w_pre_.value_or(at::Tensor());
+    auto [r2, y, rs] = join_fwd_run(r, o, w_post, gate, w_pre, c, true);
+    ctx->save_for_backward({r2.defined() ? r2 : r, o, rs, w_post, gate, w_pre});
+    ctx->saved_data["scale"] = c.scale;
+    ctx->saved_data["eps"] = c.eps;
+    ctx->saved_data["post"] = c.post;
+    ctx->saved_data["heads"] = c.heads;
+    ctx->saved_data["dtype"] = (int64_t)c.dtype;
+    ctx->set_materialize_grads(false);
+    if (!r2.defined()) return {y};
+    return {r2, y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_once();
+    const auto s = ctx->get_saved_variables();
+    const bool with_o = s[1].defined();
+    const JoinCfg c{ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["post"].toBool(),
+                    ctx->saved_data["heads"].toInt(), (at::ScalarType)ctx->saved_data["dtype"].toInt()};
+    const at::Tensor dr2 = with_o ? grads[0] : at::Tensor(), dy = with_o ? grads[1] : grads[0];
+    variable_list r(6);
+    if (!dr2.defined() && !dy.defined()) return r;
+    // the node has an edge for each tensor that is there
+    const bool there[5] = {true, with_o, s[3].defined(), s[4].defined(), s[5].defined()};
+    bool need[5];
+    for (int i = 0, edge = 0; i < 5; ++i) need[i] = there[i] && ctx->needs_input_grad(edge++);
+    auto g = join_bwd_run(s[0], s[1], s[2], dr2, dy, s[3], s[4], s[5], c, need);
+    for (int i = 0; i < 5; ++i) r[i] = g[i];
+    return r;
+  }
+};
+
+at::Tensor or_none(PyObject* o, bool* ok) {
+  if (o == Py_None) return at::Tensor();
+  if (!THPVariable_Check(o)) {
+    *ok = false;
+    return at::Tensor();
+  }
+  return THPVariable_Unpack(o);
+}
+
+// join(r, o, w_post, gate, w_pre, scale, post, eps, heads, dtype_of) -> (r', y), or None. o None: block_norm, with
+// heads (0: rows) and the dtype of `dtype_of` (0 fp16, 1 bf16, 2 fp32)
+PyObject* fast_join(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 10) Py_RETURN_NONE;
+  at::Tensor t[5];
+  bool ok = true;
+  for (int i = 0; i < 5; ++i) t[i] = or_none(args[i], &ok);
+  if (!ok || !t[0].defined()) Py_RETURN_NONE;
+  JoinCfg c{PyFloat_AsDouble(args[5]), PyFloat_AsDouble(args[7]), PyObject_IsTrue(args[6]) == 1, PyLong_AsLong(args[8]),
+            at::kFloat};
+  const long code = PyLong_AsLong(args[9]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  c.dtype = t[1].defined() ? t[1].scalar_type() : code == 0 ? at::kHalf : code == 1 ? at::kBFloat16 : at::kFloat;
+  if (!(c.eps >= 0) || !join_ok(t[0], t[1], t[2], t[3], t[4], c)) Py_RETURN_NONE;
+  bool grad = false;
+  if (at::GradMode::is_enabled())
+    for (auto& v : t) grad = grad || (v.defined() && v.requires_grad());
+  at::Tensor r2, y;
+  if (grad) {
+    const auto opt = [&](int i) { return t[i].defined() ? JoinFn::Opt(t[i]) : JoinFn::Opt(); };
+    variable_list out = JoinFn::apply(t[0], opt(1), opt(2), opt(3), opt(4), c);
+    if (out.size() == 2) r2 = out[0];
+    y = out.back();
+  } else {
+    std::tie(r2, y, std::ignore) = join_fwd_run(t[0], t[1], t[2], t[3], t[4], c, false);
+  }
+  return Py_BuildValue("(NN)", wrap_or_none(r2), wrap_or_none(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- clipping ----
+// clip(grads, outs, max_norm) -> norm, or None; lists of tensors, outs None for the norm alone
+PyObject* fast_clip(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 3 || !PyList_Check(args[0]) || (args[1] != Py_None && !PyList_Check(args[1]))) Py_RETURN_NONE;
+  const bool clip = args[1] != Py_None;
+  const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+  if (n == 0 || n > (1 << 24) || (clip && PyList_GET_SIZE(args[1]) != n)) Py_RETURN_NONE;
+  const double max_norm = PyFloat_AsDouble(args[2]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  if (!(max_norm >= 0)) Py_RETURN_NONE;
+  std::vector<const void*> g((size_t)n);
+  std::vector<void*> o((size_t)(clip ? n : 0));
+  std::vector<int64_t> numel((size_t)n);
+  std::vector<int> gt((size_t)n), ot(o.size());
+  const at::Tensor* first = nullptr;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject *a = PyList_GET_ITEM(args[0], i), *b = clip ? PyList_GET_ITEM(args[1], i) : nullptr;
+    if (!THPVariable_Check(a) || (b && !THPVariable_Check(b))) Py_RETURN_NONE;
+    const at::Tensor& t = THPVariable_Unpack(a);
+    if (i == 0) {
+      if (!t.is_cuda()) Py_RETURN_NONE;
+      first = &t;
+    }
+    const auto fits = [&](const at::Tensor& v, int* code) {
+      *code = io_code(v);
+      return *code >= 0 && v.layout() == at::kStrided && v.device() == first->device() && v.is_contiguous() && !v.is_neg();
+    };
+    if (!fits(t, &gt[i])) Py_RETURN_NONE;
+    g[i] = t.data_ptr();
+    numel[i] = t.numel();
+    if (b) {
+      const at::Tensor& v = THPVariable_Unpack(b);
+      if (!fits(v, &ot[i]) || v.sizes() != t.sizes()) Py_RETURN_NONE;
+      o[i] = v.data_ptr();
+    }
+  }
+  c10::DeviceGuard guard(first->device());
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(first->device().index()).stream();
+  at::Tensor norm = at::empty({}, first->options().dtype(at::kFloat));
+  const size_t bytes = fmlp_clip_workspace_bytes((int)n, numel.data());
+  at::Tensor ws = bytes_on(*first, bytes);
+  const int st = clip ? fmlp_clip_grads((int)n, g.data(), o.data(), numel.data(), gt.data(), ot.data(), (float)max_norm,
+                                        norm.data_ptr<float>(), ws.data_ptr(), bytes, stream)
+                      : fmlp_grad_norm((int)n, g.data(), numel.data(), gt.data(), norm.data_ptr<float>(), ws.data_ptr(),
+                                       bytes, stream);
+  check_status(st, clip ? "gradient clipping" : "gradient norm");
+  return THPVariable_Wrap(norm);
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
     {"fwd", (PyCFunction)(void (*)(void))fast_fwd, METH_FASTCALL, "fwd(x, w1, w2, act) -> (status, o) or None"},
     {"bwd", (PyCFunction)(void (*)(void))fast_bwd, METH_FASTCALL,
      "bwd(x, w1, w2, do, act, flags) -> (status, dx, dw1, dw2) or None"},
+    {"gated_fwd", (PyCFunction)(void (*)(void))fast_gated_fwd, METH_FASTCALL, "gated_fwd(x, wg, wu, w2, act) -> o or None"},
+    {"gated", (PyCFunction)(void (*)(void))fast_gated, METH_FASTCALL, "gated(x, wg, wu, w2, act) -> o or None"},
+    {"gated_bwd", (PyCFunction)(void (*)(void))fast_gated_bwd, METH_FASTCALL,
+     "gated_bwd(x, wg, wu, w2, do, act, need_dx, need_dw) -> (dx, dwg, dwu, dw2) or None"},
+    {"join", (PyCFunction)(void (*)(void))fast_join, METH_FASTCALL,
+     "join(r, o, w_post, gate, w_pre, scale, post, eps, heads, dtype) -> (r', y) or None"},
+    {"clip", (PyCFunction)(void (*)(void))fast_clip, METH_FASTCALL, "clip(grads, outs, max_norm) -> norm or None"},
     {nullptr, nullptr, 0, nullptr}};
 
-PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fmlp_fast", "fast path of flashmlp_fwd / flashmlp_bwd", -1, kMethods};
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fmlp_fast", "fast path of the Python wrappers", -1, kMethods};
 
 }  // namespace
 

@@ -19,8 +19,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from .flashmlp import (_HeadMean, _act_code, _alloc_ws, _current_device, _dense_all, _empty_as, _io_code, _ptr, _rows,
-                       _stream_of)
+from .flashmlp import (_HeadMean, _act_code, _alloc_ws, _current_device, _dense_all, _empty_as, _fast, _io_code, _ptr,
+                       _rows, _stream_of)
 
 
 def _check(x, wg, wu, w2) -> Tuple[int, int, int, int]:
@@ -63,6 +63,10 @@ def flashmlp_gated_fwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, w2: 
         o (H, B, D), dtype of x. The products are summed in fp32 and h = act(.) * (.) is rounded to
         the io dtype before the last one.
     """
+    if _fast is not None:  # one GPU, tensors that the kernels read in place: else None
+        o = _fast.gated_fwd(x, wg, wu, w2, _act_code(activation))
+        if o is not None:
+            return o
     H, B, D, E = _check(x, wg, wu, w2)
     dtype = _io_code(x, wg, wu, w2)
     o = _empty_as(x, (H, B, D))
@@ -86,9 +90,13 @@ def flashmlp_gated_bwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, w2: 
     need the weights' gradients; GatedFlashMLPFunction passes autograd's needs_input_grad) skips the
     programs of gradients that nobody asked for and returns None in their place.
     """
+    need_dx, need_dw = bool(_needs[0]), bool(_needs[1])
+    if _fast is not None:  # as in flashmlp_gated_fwd
+        g = _fast.gated_bwd(x, wg, wu, w2, do, _act_code(activation), need_dx, need_dw)
+        if g is not None:
+            return g
     H, B, D, E = _check(x, wg, wu, w2)
     assert x.shape == do.shape, "Gradient shape mismatch"
-    need_dx, need_dw = bool(_needs[0]), bool(_needs[1])
     dtype = _io_code(x, wg, wu, w2, do)
     dx = _empty_as(x, (H, B, D)) if need_dx else None
     dwg, dwu, dw2 = ((_empty_as(t, t.shape) for t in (wg, wu, w2)) if need_dw else (None, None, None))
@@ -161,7 +169,10 @@ class GatedFlashMLP(torch.nn.Module):
         shared = x.dim() == 2
         if shared:
             x = x.unsqueeze(0).expand(self.num_heads, -1, -1)
-        o = GatedFlashMLPFunction.apply(x, self.wg, self.wu, self.w2, self.activation)
+        # the same autograd node in C++ where the kernels read the tensors in place
+        o = _fast.gated(x, self.wg, self.wu, self.w2, _act_code(self.activation)) if _fast is not None else None
+        if o is None:
+            o = GatedFlashMLPFunction.apply(x, self.wg, self.wu, self.w2, self.activation)
         if shared:
             o = _HeadMean.apply(o) if o.requires_grad else o.mean(dim=0)
         return o
