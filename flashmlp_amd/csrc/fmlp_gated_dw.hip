@@ -34,10 +34,12 @@ struct Form {
 __host__ __device__ constexpr Form dw_form(int D) {
   return D == 32 ? Form{4, 1, 4, 2, 3} : D == 64 ? Form{4, 1, 4, 2, 0} : D == 128 ? Form{4, 1, 4, 1, 3} : Form{2, 2, 4, 1, 2};
 }
+// LDS: the ring, then the tiles of Wg and Wu (for good where they are read from there; else for the start only, and
+// in the ring's place where they do not fit beside it), then W2's
+__host__ __device__ constexpr bool dw_own_stage(int D) { return dw_form(D).wreg == 0 || D <= 128; }
 __host__ __device__ constexpr int dw_lds(int D) {
   const Form f = dw_form(D);
-  const int w = f.wreg == 3 ? 0 : f.wreg == 2 ? 64 * D * f.ew : 192 * D * f.ew;
-  return f.ns * 128 * D + w;
+  return f.ns * 128 * D + (dw_own_stage(D) ? 128 * D * f.ew : 0) + (f.wreg == 3 ? 0 : 64 * D * f.ew);
 }
 
 template <int D>
@@ -56,8 +58,9 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
   constexpr int EW = F.ew, DP = F.dp, NS = F.ns, PF = NS - 1, WREG = F.wreg;
   constexpr int KS = DG / 16, NTO = D / 32 / DP, ROWB = 2 * D, PPR = D / 8, SLOT = 128 * D, DOO = 64 * D;
   constexpr int NPR = D >= 64 ? D / 64 : 1, NLD = D >= 64 ? 2 * NPR : 1;  // loads a thread for X (and dO)
-  constexpr int WL = NS * SLOT, W2L = WL + (WREG == 0 ? 128 * D * EW : 0);  // weights in LDS behind the ring
-  static_assert(EW * DP == 4 && NLD * (PF - 2) < 64 && 128 * D * EW <= NS * SLOT, "form");
+  constexpr bool STAGE = dw_own_stage(D);
+  constexpr int WL = STAGE ? NS * SLOT : 0, W2L = NS * SLOT + (STAGE ? 128 * D * EW : 0);
+  static_assert(EW * DP == 4 && NLD * PF < 64 && 128 * D * EW <= NS * SLOT, "form");
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int eg = DP == 1 ? wave : wave & (EW - 1), dp = DP == 1 ? 0 : wave / EW;
@@ -78,7 +81,7 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
   // ---- weights: this wave's columns of Wg, Wu as [D][32] tiles through LDS (the ring's place, or their own) ----
   u32x4 wg[WREG ? KS : 1], wu[WREG ? KS : 1], w2[WREG == 3 ? KS : 1];
   const int laneA = (8 * g + (i16 >> 2)) * 64 + 32 * (G & 1) + 8 * (i16 & 3);
-  const int wt = (WREG ? 0 : WL) + eg * 64 * D;
+  const int wt = WL + eg * 64 * D;
   auto opWt = [&](int m, int k) {
     const int a = wt + m * 64 * D * EW + laneA + k * 1024;
     return cat(lds_read_tr(a), lds_read_tr(a + 256));
@@ -110,23 +113,6 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
       }
     }
   }
-  auto barrier = [&]() {
-    __builtin_amdgcn_s_waitcnt(0xC07F);
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-  };
-  wait_vmcnt<0>();
-  barrier();
-  if constexpr (WREG > 0) {
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      wg[k] = opWt(0, k);
-      wu[k] = opWt(1, k);
-    }
-    barrier();  // before the ring's loads land on the tiles
-  }
-
   // ---- subtiles: X and dO rows r0 + 32 i .., 16-byte piece q of row r at place q ^ swz(r) ----
   unsigned so[NPR];
 #pragma unroll
@@ -151,6 +137,30 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
       }
     }
   };
+  auto barrier = [&]() {
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  auto load_first = [&]() {
+#pragma unroll
+    for (int i = 0; i < PF; ++i) load_sub(i, i);
+  };
+  if constexpr (STAGE) load_first();
+  if constexpr (WREG > 0) {
+    wait_vmcnt<STAGE ? NLD * PF : 0>();  // the weights' tiles
+    barrier();
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      wg[k] = opWt(0, k);
+      wu[k] = opWt(1, k);
+    }
+    if constexpr (!STAGE) {
+      barrier();  // before the ring's loads land on the tiles
+      load_first();
+    }
+  }
   // row reads (row l32, columns 16 k + 8 g ..) and transposed reads (rows 16 s + 8 r + 4 g + i16 / 4, columns
   // 32 nt + 16 (G % 2) + 4 (i16 % 4) ..)
   int ro[KS], to[NTO][2];
@@ -182,8 +192,6 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
   for (int n = 0; n < NTO; ++n) ag[n] = au[n] = a2[n] = zero16();
 
   if (NSUB > 0) {
-#pragma unroll
-    for (int i = 0; i < PF; ++i) load_sub(i, i);
     wait_vmcnt<NLD*(PF > 2 ? PF - 2 : 0)>();
     barrier();
     zg = zu = dh = zero16();
@@ -257,11 +265,11 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
           constexpr int m = i % 3, n = i / 3 % NTO, s2 = i / 3 / NTO;
           if constexpr (m == 0) {
             xt = op.a;
-            ag[n] = mfma<BF16>(xt, pg[s2], ag[n]);
+            ag[n] = mfma<BF16>(pg[s2], xt, ag[n]);
           } else if constexpr (m == 1) {
-            au[n] = mfma<BF16>(xt, pu[s2], au[n]);
+            au[n] = mfma<BF16>(pu[s2], xt, au[n]);
           } else {
-            a2[n] = mfma<BF16>(ph[s2], op.a, a2[n]);
+            a2[n] = mfma<BF16>(op.a, ph[s2], a2[n]);
           }
         } else if constexpr (i3 < 0) {
           zu = mfma<BF16>(op.a, WREG ? wu[WREG ? i2 : 0] : op.w, i2 == 0 ? zero16() : zu);
@@ -288,61 +296,121 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
       cur = nxt;
     }
     iter(std::false_type{}, cur, cur);
-    wait_vmcnt<0>();  // subtiles past the last are still landing, as zeros
   }
+  wait_vmcnt<0>();  // subtiles past the last are still landing, as zeros
 
-  // ---- dW2 tiles: rows e, lane = column d; dWg, dWu tiles: rows d, lane = column e ----
-  const size_t n1 = (size_t)H * E * DG;  // values of each gradient
-  void *og = dWg, *ou = dWu, *o2 = dW2;
-  const bool f32 = nS > 1;
-  if (f32) {
-    og = ws + (size_t)s * 3 * n1;
-    ou = ws + ((size_t)s * 3 + 1) * n1;
-    o2 = ws + ((size_t)s * 3 + 2) * n1;
+  // ---- dWg, dWu tiles: lane = row d, values along e; dW2 tiles: lane = row e, values along d ----
+  const int d0 = dp * NTO * 32;
+  if (nS > 1) {  // fp32 partials as the accumulators lie: 1 KB per store
+    float4* part = (float4*)ws + ((((size_t)s * H + h) * nE + et) * 4 + wave) * (3 * NTO * 256) + lane;
+#pragma unroll
+    for (int m = 0; m < 3; ++m)
+#pragma unroll
+      for (int n = 0; n < NTO; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x16& t = m == 0 ? ag[n] : m == 1 ? au[n] : a2[n];
+          part[((m * NTO + n) * 4 + q) * 64] = float4{t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3]};
+        }
+    return;
   }
+  // through LDS, so that rows leave as whole 16-byte pieces: 2-byte stores from the accumulators' layout took 8 of the
+  // 18 us of a program with one subtile (H=32 B=4 D=128 E=1024)
+  barrier();  // the ring is read
+  const int area = wave * 2048 * NTO;
+  auto fence = [&]() {  // the area belongs to this wave alone: its own reads and writes in order
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    asm volatile("" ::: "memory");
+  };
 #pragma unroll
-  for (int n = 0; n < NTO; ++n) {
-    const int d0 = (dp * NTO + n) * 32;
+  for (int m = 0; m < 2; ++m) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int r = 8 * (i >> 2) + 4 * g + (i & 3);
-      if (e0 + r < E && d0 + l32 < DG) {
-        const size_t at = ((size_t)h * E + e0 + r) * DG + d0 + l32;
-        if (f32) ((float*)o2)[at] = a2[n][i];
-        else ((u16*)o2)[at] = from_f32<BF16>(a2[n][i]);
+    for (int n = 0; n < NTO; ++n)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x16& t = m == 0 ? ag[n] : au[n];
+        lds_write8(area + (n * 32 + l32) * 64 + ((q ^ ((l32 >> 2) & 3)) << 4) + g * 8,
+                   u32x2{pack2<BF16>(t[4 * q], t[4 * q + 1]), pack2<BF16>(t[4 * q + 2], t[4 * q + 3])});
       }
-      if (e0 + l32 < E && d0 + r < DG) {
-        const size_t at = ((size_t)h * DG + d0 + r) * E + e0 + l32;
-        if (f32) {
-          ((float*)og)[at] = ag[n][i];
-          ((float*)ou)[at] = au[n][i];
+    fence();
+    u16* out = (u16*)(m == 0 ? dWg : dWu);
+#pragma unroll
+    for (int i = 0; i < 2 * NTO; ++i) {
+      const int p = i * 64 + lane, r = p >> 2, e = e0 + ((p & 3) ^ ((r >> 2) & 3)) * 8;
+      const u32x4 v = lds_read16(area + p * 16);
+      if (d0 + r < DG && e < E) {
+        u16* at = out + ((size_t)h * DG + d0 + r) * E + e;
+        if ((E & 7) == 0) {
+          *(u32x4*)at = v;
         } else {
-          ((u16*)og)[at] = from_f32<BF16>(ag[n][i]);
-          ((u16*)ou)[at] = from_f32<BF16>(au[n][i]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (e + j < E) at[j] = (u16)(v[j >> 1] >> (16 * (j & 1)));
         }
       }
     }
+    fence();
+  }
+  constexpr int PW = 4 * NTO;  // pieces of a row of the dW2 tiles
+#pragma unroll
+  for (int n = 0; n < NTO; ++n)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      lds_write8(area + l32 * (PW * 16) + (((n * 4 + q) ^ (l32 & (PW - 1))) << 4) + g * 8,
+                 u32x2{pack2<BF16>(a2[n][4 * q], a2[n][4 * q + 1]), pack2<BF16>(a2[n][4 * q + 2], a2[n][4 * q + 3])});
+  fence();
+#pragma unroll
+  for (int i = 0; i < 2 * NTO; ++i) {
+    const int p = i * 64 + lane, r = p / PW, d = d0 + ((p % PW) ^ (r & (PW - 1))) * 8;
+    const u32x4 v = lds_read16(area + p * 16);
+    if (e0 + r < E && d < DG) *(u32x4*)((u16*)dW2 + ((size_t)h * E + e0 + r) * DG + d) = v;
   }
 }
 
-// Sum of the row splits' partials in order, four values a thread.
-template <bool BF16>
-__global__ void __launch_bounds__(256) gated_dw_reduce(const float* __restrict__ ws, u16* dWg, u16* dWu, u16* dW2,
+// Sum of the row splits' partials in order: four values of one accumulator a thread, along a row of the gradient.
+template <bool BF16, int D, int DG>
+__global__ void __launch_bounds__(256) gated_dw_reduce(const float* __restrict__ ws, u16* __restrict__ dWg,
+                                                       u16* __restrict__ dWu, u16* __restrict__ dW2, int E, int nE,
                                                        long long quads, int nS) {
-  const long long q = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (q >= 3 * quads) return;
-  const int m = q >= 2 * quads ? 2 : q >= quads ? 1 : 0;
-  const float4* src = (const float4*)ws + q;
+  constexpr Form F = dw_form(D);
+  constexpr int NTO = D / 32 / F.dp;
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;  // (quads is a multiple of 256)
+  const float4* src = (const float4*)ws + id;
   float4 v = src[0];
   for (int s = 1; s < nS; ++s) {
-    const float4 u = src[(size_t)s * 3 * quads];
+    const float4 u = src[(size_t)s * quads];
     v.x += u.x;
     v.y += u.y;
     v.z += u.z;
     v.w += u.w;
   }
-  u16* dst = (m == 0 ? dWg : m == 1 ? dWu : dW2) + 4 * (q - m * quads);
-  *(u32x2*)dst = u32x2{pack2<BF16>(v.x, v.y), pack2<BF16>(v.z, v.w)};
+  const int lane = (int)(id & 63), q = (int)(id >> 6) & 3;
+  long long t = id >> 8;
+  const int n = (int)(t % NTO);
+  t /= NTO;
+  const int m = (int)(t % 3);
+  t /= 3;
+  const int wave = (int)(t & 3);
+  t >>= 2;
+  const int et = (int)(t % nE), eg = F.dp == 1 ? wave : wave & (F.ew - 1), dp = F.dp == 1 ? 0 : wave / F.ew;
+  const size_t h = (size_t)(t / nE);
+  const int e0 = (et * F.ew + eg) * 32, d0 = (dp * NTO + n) * 32, l32 = lane & 31, along = 8 * q + 4 * (lane >> 5);
+  const u32x2 w = {pack2<BF16>(v.x, v.y), pack2<BF16>(v.z, v.w)};
+  if (m == 2) {
+    const int e = e0 + l32, d = d0 + along;
+    if (e < E && d < DG) *(u32x2*)(dW2 + (h * E + e) * DG + d) = w;
+  } else {
+    const int d = d0 + l32, e = e0 + along;
+    if (d >= DG || e >= E) return;
+    u16* at = (m == 0 ? dWg : dWu) + (h * DG + d) * E + e;
+    if ((E & 3) == 0) {
+      *(u32x2*)at = w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (e + j < E) at[j] = (u16)(w[j >> 1] >> (16 * (j & 1)));
+    }
+  }
 }
 
 struct Args {
@@ -364,9 +432,9 @@ hipError_t launch(const Args& q) {
                      (int)a.E, (int)a.ldw, (long long)a.sx, (long long)a.sdo, q.p.nE, q.p.nS, q.p.rows_per_split,
                      (float*)a.ws);
   if ((e = hipGetLastError()) != hipSuccess || q.p.nS == 1) return e;
-  const long long quads = (long long)a.H * a.E * a.D / 4, blocks = (3 * quads + 255) / 256;
-  hipLaunchKernelGGL(gated_dw_reduce<BF16>, dim3((unsigned)blocks), dim3(256), 0, q.st, (const float*)a.ws, (u16*)a.dwg,
-                     (u16*)a.dwu, (u16*)a.dw2, quads, q.p.nS);
+  const long long quads = (long long)a.H * q.p.nE * 4 * (3 * (D / 32 / dw_form(D).dp) * 256);
+  hipLaunchKernelGGL((gated_dw_reduce<BF16, D, DG>), dim3((unsigned)(quads / 256)), dim3(256), 0, q.st, (const float*)a.ws,
+                     (u16*)a.dwg, (u16*)a.dwu, (u16*)a.dw2, (int)a.E, q.p.nE, quads, q.p.nS);
   return hipGetLastError();
 }
 template <bool BF16, int D, int DG = D>
@@ -417,7 +485,7 @@ GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cu
     }
   }
   p.programs = base * p.nS;
-  p.ws_bytes = p.nS > 1 ? (size_t)p.nS * 3 * H * D * E * sizeof(float) : 0;
+  p.ws_bytes = p.nS > 1 ? (size_t)p.programs * 4 * (3 * (DT / 32 / F.dp) * 256) * sizeof(float4) : 0;
   return p;
 }
 

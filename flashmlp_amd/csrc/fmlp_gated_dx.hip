@@ -203,11 +203,11 @@ gated_dx_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
   for (int c = 0; c + 1 < NC; ++c) {
     const int nxt = cur + 1 == NS ? 0 : cur + 1, far = cur == 0 ? NS - 1 : cur - 1;
     load_chunk(c + PF, far);
-    iter(std::true_type{}, cur, nxt);
+    if (b_wave < B) iter(std::true_type{}, cur, nxt);  // a wave without rows only loads
     sync(std::integral_constant<int, NLD*(PF - 2)>{});
     cur = nxt;
   }
-  iter(std::false_type{}, cur, cur);
+  if (b_wave < B) iter(std::false_type{}, cur, cur);
 
   wait_vmcnt<0>();  // chunks past the last are still landing, as zeros
   if constexpr (ES > 1) {
@@ -243,25 +243,15 @@ gated_dx_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
     store_rows<BF16, D, DG>(o, dX, (size_t)h * B * DG, B, b_wave, g, l32, 0);
 }
 
-struct Form {
-  int nw, es, ns, oc;
-};
-__host__ __device__ constexpr Form large_form(int D) {
-  return D == 32 ? Form{2, 1, 4, 3} : D == 64 ? Form{4, 1, 4, 2} : D == 128 ? Form{8, 1, 4, 2} : Form{4, 1, 3, 1};
-}
-__host__ __device__ constexpr Form small_form(int D) {
-  return D == 32 ? Form{1, 4, 4, 1} : D == 64 ? Form{2, 4, 3, 2} : D == 128 ? Form{2, 2, 3, 1} : Form{4, 1, 3, 1};
-}
-
 struct Args {
   const GatedArgs& a;
   const GatedFwdPlan& p;
   hipStream_t st;
 };
 
-template <bool BF16, int D, int DG, int ACT, bool SMALL>
+template <bool BF16, int D, int DG, int ACT, int FORM>
 hipError_t launch(const Args& q) {
-  constexpr Form F = SMALL ? small_form(D) : large_form(D);
+  constexpr GatedForm F = gated_form(D, FORM, true);
   constexpr int lds = F.es * F.ns * 192 * D;
   auto k = gated_dx_kernel<BF16, D, DG, ACT, F.nw, F.es, F.ns, F.oc>;
   static std::atomic<unsigned long long> done{0};
@@ -279,9 +269,11 @@ hipError_t launch(const Args& q) {
 
 template <bool BF16, int D, int DG, int ACT>
 hipError_t by_form(const Args& q) {
-  if constexpr (large_form(D).nw != small_form(D).nw || large_form(D).es != small_form(D).es)
-    if (q.p.small) return launch<BF16, D, DG, ACT, true>(q);
-  return launch<BF16, D, DG, ACT, false>(q);
+  if constexpr (D <= 128)
+    if (q.p.form == 2) return launch<BF16, D, DG, ACT, 2>(q);
+  if constexpr (D == 128)
+    if (q.p.form == 1) return launch<BF16, D, DG, ACT, 1>(q);
+  return launch<BF16, D, DG, ACT, 0>(q);
 }
 template <bool BF16, int D, int DG = D>
 hipError_t by_act(const Args& q) {

@@ -196,12 +196,12 @@ gated_fwd_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u1
   for (int c = 0; c + 1 < NC; ++c) {
     const int nxt = cur + 1 == NS ? 0 : cur + 1, far = cur == 0 ? NS - 1 : cur - 1;
     load_chunk(c + PF, far);
-    // (chunk c + 1 landed before the last barrier)
-    iter(std::true_type{}, cur, nxt);
+    // (chunk c + 1 landed before the last barrier; a wave without rows only loads)
+    if (b_wave < B) iter(std::true_type{}, cur, nxt);
     sync(std::integral_constant<int, NLD*(PF - 2)>{});  // chunk c + 2
     cur = nxt;
   }
-  iter(std::false_type{}, cur, cur);
+  if (b_wave < B) iter(std::false_type{}, cur, cur);
 
   if constexpr (ES > 1) {
     wait_vmcnt<0>();  // chunks past the last are still landing, as zeros
@@ -239,26 +239,15 @@ gated_fwd_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u1
     store_rows<BF16, D, DG>(o, O, (size_t)h * B * DG, B, b_wave, g, l32, 0);
 }
 
-// waves per E part, parts, ring slots and waves per SIMD of the two forms of each D
-struct Form {
-  int nw, es, ns, oc;
-};
-__host__ __device__ constexpr Form large_form(int D) {
-  return D == 32 ? Form{2, 1, 4, 3} : D == 64 ? Form{4, 1, 4, 3} : D == 128 ? Form{8, 1, 4, 2} : Form{4, 1, 3, 1};
-}
-__host__ __device__ constexpr Form small_form(int D) {
-  return D == 32 ? Form{1, 4, 4, 1} : D == 64 ? Form{2, 4, 3, 2} : D == 128 ? Form{2, 2, 3, 1} : Form{4, 1, 3, 1};
-}
-
 struct Args {
   const GatedArgs& a;
   const GatedFwdPlan& p;
   hipStream_t st;
 };
 
-template <bool BF16, int D, int DG, int ACT, bool SMALL>
+template <bool BF16, int D, int DG, int ACT, int FORM>
 hipError_t launch(const Args& q) {
-  constexpr Form F = SMALL ? small_form(D) : large_form(D);
+  constexpr GatedForm F = gated_form(D, FORM, false);
   constexpr int lds = F.es * F.ns * 192 * D;
   auto k = gated_fwd_kernel<BF16, D, DG, ACT, F.nw, F.es, F.ns, F.oc>;
   static std::atomic<unsigned long long> done{0};
@@ -276,9 +265,11 @@ hipError_t launch(const Args& q) {
 
 template <bool BF16, int D, int DG, int ACT>
 hipError_t by_form(const Args& q) {
-  if constexpr (large_form(D).nw != small_form(D).nw || large_form(D).es != small_form(D).es)
-    if (q.p.small) return launch<BF16, D, DG, ACT, true>(q);
-  return launch<BF16, D, DG, ACT, false>(q);
+  if constexpr (D <= 128)
+    if (q.p.form == 2) return launch<BF16, D, DG, ACT, 2>(q);
+  if constexpr (D == 128)
+    if (q.p.form == 1) return launch<BF16, D, DG, ACT, 1>(q);
+  return launch<BF16, D, DG, ACT, 0>(q);
 }
 template <bool BF16, int D, int DG = D>
 hipError_t by_act(const Args& q) {
@@ -304,27 +295,34 @@ hipError_t by_d(const Args& q) {
 
 GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus) {
   const int DT = D < 32 ? 32 : (int)D;
-  const Form L = large_form(DT), S = small_form(DT);
   const long long N = num_cus > 0 ? num_cus : 1, nch = (E + 31) / 32;
-  GatedFwdPlan p{};
-  p.xs = 1;
-  p.nct = (int)nch;
-  p.tiles = H * ((B + 32 * L.nw - 1) / (32 * L.nw));
-  static const int force = env_int("FMLP_GATED_FORM", -1);  // 0 / 1: the large / small form
-  p.small = force >= 0 ? force != 0 : p.tiles <= N;
-  if (p.small) p.tiles = H * ((B + 32 * S.nw - 1) / (32 * S.nw));
-  const Form F = p.small ? S : L;
-  // workgroups of one round, each with at least one chunk a part
-  static const int xs_env = env_int("FMLP_GATED_XS", -1);
-  long long xs = std::min<long long>(N / std::max<long long>(p.tiles, 1), nch / F.es);
-  if (xs_env > 0) xs = std::min<long long>(xs_env, nch);
-  xs = std::min<long long>(xs, 16);
-  if (xs > 1 && p.tiles > 0) {
-    p.nct = (int)((nch + xs - 1) / xs);
-    p.xs = (int)((nch + p.nct - 1) / p.nct);
-    if (p.xs > 1) p.ws_bytes = (size_t)p.tiles * p.xs * 32 * F.nw * D * sizeof(float);
+  static const int force = env_int("FMLP_GATED_FORM", -1), xs_env = env_int("FMLP_GATED_XS", -1);
+  GatedFwdPlan best{};
+  double best_us = 0;
+  for (int form = 0; form < 3; ++form) {
+    const GatedForm F = gated_form(DT, form, false);
+    if (F.nw == 0 || (force >= 0 && form != force)) continue;
+    const long long tiles = H * ((B + 32 * F.nw - 1) / (32 * F.nw));
+    for (long long want = 1; want <= 16 && want <= nch; ++want) {
+      const long long nct = (nch + want - 1) / want, xs = (nch + nct - 1) / nct;
+      if (xs != want || (xs_env > 0 && want != std::min<long long>(xs_env, nch))) continue;
+      // full rounds of F.per_cu workgroups a CU, and what is left; a split adds a launch and the partials' bytes
+      const long long slots = N * F.per_cu, full = tiles * xs / slots, rest = tiles * xs % slots;
+      const double steps = (double)((nct + F.es - 1) / F.es);
+      double us = (double)full * (F.fixed_us + F.full_us * steps);
+      if (rest > 0) us += F.fixed_us + steps * std::max(F.chunk_us, F.full_us * (double)rest / (double)slots);
+      if (xs > 1) us += 2.8 + (double)(H * B * D * xs) * 8.0 / 4.2e6;
+      if (best_us == 0 || us < best_us) {
+        best_us = us;
+        best.form = form;
+        best.tiles = tiles;
+        best.xs = (int)xs;
+        best.nct = (int)nct;
+        best.ws_bytes = xs > 1 ? (size_t)(tiles * xs) * 32 * F.nw * D * sizeof(float) : 0;
+      }
+    }
   }
-  return p;
+  return best;
 }
 
 hipError_t launch_gated_fwd(const GatedArgs& a, const GatedFwdPlan& p, hipStream_t st) {
