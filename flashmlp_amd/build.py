@@ -24,9 +24,14 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libflashmlp.so"
-# fmlp_bwd.hip is compiled once per part (file:part): the kernels of one D each, and the rest
+# fmlp_bwd.hip and fmlp_gated_dw.hip are compiled once per part (file:part): the kernels of one D each, and the rest
 SOURCES = ["fmlp_bwd.hip:64", "fmlp_bwd.hip:128", "fmlp_bwd.hip:0", "fmlp_bwd.hip:32", "fmlp_fwd.hip", "fmlp_f32.hip", "fmlp_gen.hip",
-           "fmlp_gated_fwd.hip", "fmlp_gated_dx.hip", "fmlp_gated_dw.hip", "fmlp_gated_f32.hip", "fmlp_gated_gen.hip", "fmlp_join.hip", "fmlp_clip.hip", "fmlp_scratch.hip", "fmlp_abi.cpp", "fmlp_block_abi.cpp"]
+           "fmlp_gated_fwd.hip", "fmlp_gated_dx.hip", "fmlp_gated_dw.hip:128", "fmlp_gated_dw.hip:0", "fmlp_gated_f32.hip", "fmlp_gated_gen.hip", "fmlp_join.hip", "fmlp_clip.hip", "fmlp_scratch.hip", "fmlp_abi.cpp", "fmlp_block_abi.cpp"]
+PART_MACRO = {"fmlp_bwd.hip": "FMLP_BWD_PART", "fmlp_gated_dw.hip": "FMLP_GATED_DW_PART"}
+# Products that write vector registers: with the compiler's choice (accumulation registers, as the kernel holds more
+# than 256 values) every value the activation takes is copied first. dW at H=32 B=16384 D=128 E=1024 bf16 SiLU 728 us,
+# so 707; at D = 256 it is slower (90 us, so 110), the other D do not hold as many.
+EXTRA_FLAGS = {"fmlp_gated_dw.hip:128": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 CEILING_SRC = "fmlp_ceiling.hip"
 CEILING_LIB = PKG / "libfmlp_ceiling.so"
 FAST_SRC = "fmlp_py.cpp"
@@ -51,7 +56,8 @@ def _hipcc() -> str:
 def _compile(src: str, verbose: bool) -> Path:
     src, _, part = src.partition(":")
     obj = BUILD / (src.rsplit(".", 1)[0] + (f"_{part}" if part else "") + ".o")
-    defs = [f"-DFMLP_BWD_PART={part}"] if part else []
+    defs = [f"-D{PART_MACRO[src]}={part}"] if part else []
+    defs += EXTRA_FLAGS.get(f"{src}:{part}", [])
     cmd = [_hipcc(), *COMMON, *DEVICE_FLAGS, *defs, "-x", "hip", "-c", str(CSRC / src), "-o", str(obj)]
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -33,6 +33,11 @@ struct GatedArgs {
   size_t ws_bytes;
 };
 
+// Rows of E elements of both matrices copied to rows of ldw elements (whole 16-byte vectors, zeros behind the
+// last element), one after the other at dst, in one launch (fmlp_gated_gen.hip).
+hipError_t launch_gated_pad(const void* wg, const void* wu, void* dst, int64_t rows, int64_t E, int64_t ldw, int es,
+                            hipStream_t st);
+
 // The kernels that read their operands from global memory (fmlp_gated_gen.hip): every io type and D.
 hipError_t launch_gated_gen_fwd(const GatedArgs& a, hipStream_t st);
 hipError_t launch_gated_gen_dx(const GatedArgs& a, hipStream_t st);
@@ -80,6 +85,7 @@ struct GatedDwPlan {
 };
 GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus);
 hipError_t launch_gated_dw(const GatedArgs& a, const GatedDwPlan& p, hipStream_t st);
+hipError_t launch_gated_dw128(const GatedArgs& a, const GatedDwPlan& p, hipStream_t st);
 
 // fp32 io at D <= 128 (fmlp_gated_f32.hip): tiles of 128 rows, E-tiles of 128 columns.
 GatedFwdPlan gated32_rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus);

@@ -60,32 +60,33 @@ bool gated_staged(int64_t D, int io) { return io != FMLP_DTYPE_F32 || D <= 128; 
 
 // Wg and Wu where rows of E elements are no whole 16-byte vectors: padded copies at the workspace's start
 size_t gated_pad_bytes(int64_t H, int64_t D, int64_t E, int io) {
-  return 2 * fmlp::w1_pad_bytes(H, D, E, (int)elem_bytes(io));
+  const int es = (int)elem_bytes(io);
+  const int64_t ldw = fmlp::w1_pitch(E, es);
+  return ldw == E ? 0 : ((size_t)(2 * H * D * ldw) * es + 255) / 256 * 256;
 }
 hipError_t gated_pad(fmlp::GatedArgs* a, hipStream_t st) {
   const int es = a->io == fmlp::IO_F32 ? 4 : 2;
-  const size_t one = fmlp::w1_pad_bytes(a->H, a->D, a->E, es);
   a->ldw = fmlp::w1_pitch(a->E, es);
-  if (one == 0) return hipSuccess;
+  if (a->ldw == a->E) return hipSuccess;
+  const size_t one = (size_t)(a->H * a->D * a->ldw) * es, all = (2 * one + 255) / 256 * 256;
   char* ws = (char*)a->ws;
-  hipError_t e = fmlp::launch_pad_w1(a->wg, ws, a->H, a->D, a->E, es, st);
-  if (e == hipSuccess) e = fmlp::launch_pad_w1(a->wu, ws + one, a->H, a->D, a->E, es, st);
+  const hipError_t e = fmlp::launch_gated_pad(a->wg, a->wu, ws, a->H * a->D, a->E, a->ldw, es, st);
   a->wg = ws;
   a->wu = ws + one;
-  a->ws = ws + 2 * one;
-  a->ws_bytes -= 2 * one;
+  a->ws = ws + all;
+  a->ws_bytes -= all;
   return e;
+}
+int check_ws(const void* ws, size_t have, size_t need) {
+  if (need > 0 && (ws == nullptr || have < need))
+    return abi_fail(FMLP_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? have : (size_t)0, need);
+  return FMLP_OK;
 }
 fmlp::GatedFwdPlan rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int io, int cus) {
   return io == FMLP_DTYPE_F32 ? fmlp::gated32_rows_plan(H, B, D, E, cus) : fmlp::gated_fwd_plan(H, B, D, E, cus);
 }
 fmlp::GatedDwPlan dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int io, int cus) {
   return io == FMLP_DTYPE_F32 ? fmlp::gated32_dw_plan(H, B, D, E, cus) : fmlp::gated_dw_plan(H, B, D, E, cus);
-}
-int check_ws(const void* ws, size_t have, size_t need) {
-  if (need > 0 && (ws == nullptr || have < need))
-    return abi_fail(FMLP_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? have : (size_t)0, need);
-  return FMLP_OK;
 }
 
 int io_type(int io) { return io == FMLP_DTYPE_F32 ? fmlp::IO_F32 : io == FMLP_DTYPE_BF16 ? fmlp::IO_BF16 : fmlp::IO_F16; }

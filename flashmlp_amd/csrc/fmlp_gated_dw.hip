@@ -448,26 +448,42 @@ hipError_t by_act(const Args& q) {
 }
 template <bool BF16>
 hipError_t by_d(const Args& q) {
+#if FMLP_GATED_DW_PART == 128
+  return by_act<BF16, 128>(q);
+#else
   switch (q.a.D) {
     case 16: return by_act<BF16, 32, 16>(q);
     case 32: return by_act<BF16, 32>(q);
     case 64: return by_act<BF16, 64>(q);
-    case 128: return by_act<BF16, 128>(q);
     default: return by_act<BF16, 256>(q);
   }
+#endif
 }
 
 }  // namespace
 
+// Built in two parts: D = 128, whose accumulators fill half the registers, with matrix products that write vector
+// registers (build.py); the others with the compiler's choice.
+#if FMLP_GATED_DW_PART == 128
+hipError_t launch_gated_dw128(const GatedArgs& a, const GatedDwPlan& p, hipStream_t st) {
+  const Args q{a, p, st};
+  return a.io == IO_BF16 ? by_d<true>(q) : by_d<false>(q);
+}
+#else
 GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus) {
   const int DT = D < 32 ? 32 : (int)D;
   const Form F = dw_form(DT);
   GatedDwPlan p{};
   p.nE = (int)((E + 32 * F.ew - 1) / (32 * F.ew));
   const long long base = H * p.nE, slots = (long long)std::max(num_cus, 1) * F.oc, subs = (B + 31) / 32;
+  const size_t tile_bytes = (size_t)4 * (3 * (DT / 32 / F.dp) * 256) * sizeof(float4);  // a program's partials
   static const int force = env_int("FMLP_GATED_NS", -1);
-  // rounds of programs, each a fixed part and its subtiles; a split adds the partials' traffic and a launch
-  const double sub_us = (DT == 32 ? 0.35 : DT == 64 ? 0.6 : DT == 128 ? 1.0 : 1.6), fixed_us = 4.0;
+  // Measured: a program takes fixed_us and, for a subtile, sub_us alone on its CU or full_us on a full device (two a
+  // CU at D <= 64, where they gain little on each other: vector issue is shared; one CU with two sets the time). A
+  // split adds the sum's launch and the partials' bytes. H=8 B=2048 D=128 E=512: 79 us unsplit, 34 split in eight.
+  const double sub_us = DT == 32 ? 0.61 : DT == 64 ? 0.86 : DT == 128 ? 1.15 : 1.73;
+  const double full_us = DT == 32 ? 0.96 : DT == 64 ? 1.66 : DT == 128 ? 1.45 : 2.0;
+  const double fixed_us = DT <= 64 ? 5.0 : 8.0;
   double best = 0;
   p.nS = 1;
   p.rows_per_split = (int)std::max<long long>(subs * 32, 32);
@@ -475,9 +491,11 @@ GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cu
     if (force > 0 && n != std::min<long long>(force, std::max<long long>(subs / 2, 1))) continue;
     const long long per = (subs + n - 1) / n, m = per > 0 ? (subs + per - 1) / per : 1;
     if (m != n && n > 1) continue;
-    const double rounds = (double)((base * n + slots - 1) / slots);
-    double t = rounds * (fixed_us + sub_us * (double)per);
-    if (n > 1) t += 4.0 + (double)(3 * H * D * E) * 4.0 * (double)n * 2.0 / 3.0e6;
+    const long long full = base * n / slots, rest = base * n % slots;
+    double t = (double)full * (fixed_us + full_us * (double)per);
+    const double share = (double)((rest * F.oc + slots - 1) / slots) / (double)F.oc;  // of a CU's programs, the fullest's
+    if (rest > 0) t += fixed_us + (double)per * std::max(sub_us, F.oc > 1 ? full_us * share : full_us * (double)rest / (double)slots);
+    if (n > 1) t += 5.0 + (double)(tile_bytes * (size_t)(base * n)) * 2.0 / 6.5e6;
     if (best == 0 || t < best) {
       best = t;
       p.nS = (int)n;
@@ -485,14 +503,16 @@ GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cu
     }
   }
   p.programs = base * p.nS;
-  p.ws_bytes = p.nS > 1 ? (size_t)p.programs * 4 * (3 * (DT / 32 / F.dp) * 256) * sizeof(float4) : 0;
+  p.ws_bytes = p.nS > 1 ? (size_t)p.programs * tile_bytes : 0;
   return p;
 }
 
 hipError_t launch_gated_dw(const GatedArgs& a, const GatedDwPlan& p, hipStream_t st) {
   if (p.programs <= 0) return hipSuccess;
+  if (a.D == 128) return launch_gated_dw128(a, p, st);
   const Args q{a, p, st};
   return a.io == IO_BF16 ? by_d<true>(q) : by_d<false>(q);
 }
+#endif
 
 }  // namespace fmlp

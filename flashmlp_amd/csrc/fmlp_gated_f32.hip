@@ -368,13 +368,14 @@ GatedFwdPlan gated32_rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int n
   p.nct = (int)nch;
   p.tiles = H * ((B + 127) / 128);
   if (p.tiles <= 0) return p;
-  const double chunk_us = 2.9 * (double)std::max<long long>(D, 32) / 64.0;
+  const double chunk_us = 3.4 * (double)std::max<long long>(D, 32) / 64.0;
+  static const int xs_env = env_int("FMLP_GATED_XS", -1);
   double best = 0;
   for (long long want = 1; want <= 16 && want <= nch; ++want) {
     const long long nct = (nch + want - 1) / want, xs = (nch + nct - 1) / nct;
-    if (xs != want) continue;
+    if (xs != want || (xs_env > 0 && xs_env != want)) continue;
     double t = (double)((p.tiles * xs + N - 1) / N) * (double)nct * chunk_us;
-    if (xs > 1) t += 3.0 + (double)(H * B * D * xs) * 8.0 / 3.0e6;
+    if (xs > 1) t += 3.0 + (double)(H * B * D * xs) * 8.0 / 4.2e6;
     if (best == 0 || t < best) {
       best = t;
       p.xs = (int)xs;
@@ -391,10 +392,12 @@ GatedDwPlan gated32_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_
   p.nE = (int)((E + 127) / 128);
   const long long base = H * p.nE;
   const double sub_us = 5.8 * (double)std::max<long long>(D, 32) / 64.0;
+  static const int force = env_int("FMLP_GATED_NS", -1);
   double best = 0;
   p.nS = 1;
   p.rows_per_split = (int)std::max<long long>(subs * 32, 32);
   for (long long n = 1; n <= 32 && (n == 1 || n <= subs); ++n) {
+    if (force > 0 && n != std::min<long long>(force, std::max<long long>(subs, 1))) continue;
     const long long per = std::max<long long>((subs + n - 1) / n, 1);
     if (n > 1 && (subs + per - 1) / per != n) continue;
     double t = (double)((base * n + N - 1) / N) * (4.0 + sub_us * (double)per);

@@ -310,7 +310,8 @@ GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_
       const long long slots = N * F.per_cu, full = tiles * xs / slots, rest = tiles * xs % slots;
       const double steps = (double)((nct + F.es - 1) / F.es);
       double us = (double)full * (F.fixed_us + F.full_us * steps);
-      if (rest > 0) us += F.fixed_us + steps * std::max(F.chunk_us, F.full_us * (double)rest / (double)slots);
+      const double share = F.per_cu == 1 ? (double)rest / (double)slots : (double)((rest + N - 1) / N) / (double)F.per_cu;
+      if (rest > 0) us += F.fixed_us + steps * std::max(F.chunk_us, F.full_us * share);
       if (xs > 1) us += 2.8 + (double)(H * B * D * xs) * 8.0 / 4.2e6;
       if (best_us == 0 || us < best_us) {
         best_us = us;
