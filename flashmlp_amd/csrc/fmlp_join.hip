@@ -255,16 +255,22 @@ __global__ void __launch_bounds__(MULTI ? 1024 : 256) join_fwd_kernel(JoinArgs a
 // ---------------------------------------------------------------------------------
 // Backward. A worker (a workgroup when MULTI, else a wave) walks the rows [r0, r1) of its unit, keeping its
 // columns' sums of dw_pre, dw_post and dgate in registers, and stores them as its row of the partial arrays;
-// join_reduce_kernel adds the workers' rows in order. Units never cross a gate group unless they hold
+// join_reduce_kernel adds the workgroups' rows in order (a workgroup's four waves are added first). Units never cross a gate group unless they hold
 // whole groups, whose dgate rows are then stored as they end.
 // ---------------------------------------------------------------------------------
-template <int IO, int RIO, int VPT, bool ALIGNED, bool MULTI>
-__global__ void __launch_bounds__(MULTI ? 1024 : 256) join_bwd_kernel(JoinArgs a, JoinPlan p) {
+// MULTI = 2: more than 512 threads. A 16-bit stream's rows of up to 512 threads run two workgroups a CU, within 128
+// registers; an fp32 stream's data do not fit those, and one workgroup requests the next row's data ahead instead
+// (16384 x 4096, sums' launch included: bf16 177 us, with the next row ahead 189 at two workgroups and 194 at one;
+// fp32 stream, 4096 x 2048: 42 us, 53 the first way).
+__host__ __device__ constexpr bool join_ahead(int RIO, int VPT, int MULTI) { return RIO == IO_F32 && VPT == 1 && MULTI == 1; }
+template <int IO, int RIO, int VPT, bool ALIGNED, int MULTI>
+__global__ void __launch_bounds__(MULTI == 2 ? 1024 : MULTI ? 512 : 256, MULTI == 1 && !join_ahead(RIO, VPT, MULTI) ? 4 : 1)
+join_bwd_kernel(JoinArgs a, JoinPlan p) {
+  constexpr bool AHEAD = join_ahead(RIO, VPT, MULTI);
   __shared__ float part[2][2][16];
   const int tpr = MULTI ? (int)blockDim.x : 64, t = MULTI ? (int)threadIdx.x : (int)(threadIdx.x & 63);
   const int nw = blockDim.x >> 6, C = (int)a.C;
   const long long unit = MULTI ? (long long)blockIdx.x : (long long)blockIdx.x * nw + (threadIdx.x >> 6);
-  if (unit >= p.units) return;
   const HeadRows ho{a.o_sh, a.o_sr, (int)a.D}, hy{a.y_sh, a.y_sr, (int)a.D}, hd{a.do_sh, a.do_sr, (int)a.D};
   const float rc = 1.0f / (float)C;
   // the unit's rows: part `unit % parts` of a group, or `groups_per_unit` whole groups
@@ -272,10 +278,10 @@ __global__ void __launch_bounds__(MULTI ? 1024 : 256) join_bwd_kernel(JoinArgs a
   const long long T = a.rows_per_gate;
   if (p.parts > 1) {
     const long long g = unit / p.parts, q = unit % p.parts;
-    r0 = g * T + q * p.rows_per_part;
+    r0 = g * T + min(T, q * p.rows_per_part);
     r1 = min(g * T + T, r0 + p.rows_per_part);
   } else {
-    r0 = unit * p.groups_per_unit * T;
+    r0 = min(a.B, unit * p.groups_per_unit * T);
     r1 = min(a.B, r0 + p.groups_per_unit * T);
   }
   Vec<IO> wq[VPT], gq[VPT], wp[VPT];
@@ -290,19 +296,34 @@ __global__ void __launch_bounds__(MULTI ? 1024 : 256) join_bwd_kernel(JoinArgs a
 #pragma unroll
     for (int j = 0; j < 8; ++j) s_pre[k][j] = s_post[k][j] = s_gate[k][j] = 0.f;
   long long in_group = 0;  // rows of the current group done by this unit
-  for (long long row = r0; row < r1; ++row) {
-    const int db = (int)(row & 1);  // the row sums' buffers alternate: one barrier a sum
+  // a row's data, where they fit requested while the row before it is worked on
+  struct Row {
     Vec<RIO> r2[VPT], dr[VPT];
     Vec<IO> dy[VPT], o[VPT];
+    float rr, ro;
+  };
+  auto load = [&](long long row, Row& x) {
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
       if (a.dy) {
-        dy[k] = load_heads<IO, ALIGNED>(a.dy, hy, row, C, t, tpr, k);
-        r2[k] = load_row<RIO, ALIGNED>(a.r_out, row * a.r_sr, C, t, tpr, k);
+        x.dy[k] = load_heads<IO, ALIGNED>(a.dy, hy, row, C, t, tpr, k);
+        x.r2[k] = load_row<RIO, ALIGNED>(a.r_out, row * a.r_sr, C, t, tpr, k);
       }
-      if (a.dr_out) dr[k] = load_row<RIO, ALIGNED>(a.dr_out, row * a.dr_sr, C, t, tpr, k);
-      if (a.o) o[k] = load_heads<IO, ALIGNED>(a.o, ho, row, C, t, tpr, k);
+      if (a.dr_out) x.dr[k] = load_row<RIO, ALIGNED>(a.dr_out, row * a.dr_sr, C, t, tpr, k);
+      if (a.o) x.o[k] = load_heads<IO, ALIGNED>(a.o, ho, row, C, t, tpr, k);
     }
+    if (a.dy) x.rr = a.rs_r[row];
+    x.ro = a.o && a.post ? a.rs_o[row] : 1.f;
+  };
+  Row next;
+  if (AHEAD && r0 < r1) load(r0, next);
+  for (long long row = r0; row < r1; ++row) {
+    const int db = (int)(row & 1);  // the row sums' buffers alternate: one barrier a sum
+    if (!AHEAD) load(row, next);
+    const Row x = next;
+    const auto &r2 = x.r2, &dr = x.dr;
+    const auto &dy = x.dy, &o = x.o;
+    if (AHEAD && row + 1 < r1) load(row + 1, next);
     if (a.gate && in_group == 0) {
       const long long grow = row / T * a.C;
 #pragma unroll
@@ -310,7 +331,7 @@ __global__ void __launch_bounds__(MULTI ? 1024 : 256) join_bwd_kernel(JoinArgs a
     }
     float d[VPT][8];  // the stream's gradient
     if (a.dy) {
-      const float rr = a.rs_r[row];
+      const float rr = x.rr;
       float s = 0.f;
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
@@ -322,7 +343,7 @@ __global__ void __launch_bounds__(MULTI ? 1024 : 256) join_bwd_kernel(JoinArgs a
           s = __builtin_fmaf(dm, m, s);
           d[k][j] = dm;
         }
-      const float mean = row_sum<MULTI>(s, part[db][0], nw) * rc;
+      const float mean = row_sum<(MULTI > 0)>(s, part[db][0], nw) * rc;
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
 #pragma unroll
@@ -340,7 +361,7 @@ __global__ void __launch_bounds__(MULTI ? 1024 : 256) join_bwd_kernel(JoinArgs a
     for (int k = 0; k < VPT; ++k)
       if (a.dr) store_row<RIO, ALIGNED>(a.dr, row * a.C, C, t, tpr, k, d[k]);
     if (a.o) {
-      const float ro = a.post ? a.rs_o[row] : 1.f;
+      const float ro = x.ro;
       float s = 0.f;
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
@@ -356,7 +377,7 @@ __global__ void __launch_bounds__(MULTI ? 1024 : 256) join_bwd_kernel(JoinArgs a
         }
       if (a.d_o) {
         if (a.post) {
-          const float mean = row_sum<MULTI>(s, part[db][1], nw) * rc;
+          const float mean = row_sum<(MULTI > 0)>(s, part[db][1], nw) * rc;
 #pragma unroll
           for (int k = 0; k < VPT; ++k)
 #pragma unroll
@@ -378,9 +399,32 @@ __global__ void __launch_bounds__(MULTI ? 1024 : 256) join_bwd_kernel(JoinArgs a
       }
     }
   }
+  if constexpr (MULTI == 0) {  // the four waves' sums in wave order, through LDS
+    __shared__ float sum[3][VPT * 8 * 64];
+    const int w = threadIdx.x >> 6;
+    const auto fold = [&](float (&v)[VPT][8]) {
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < VPT; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (w > 0) sum[w - 1][(k * 8 + j) * 64 + t] = v[k][j];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+#pragma unroll
+        for (int k = 0; k < VPT; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[k][j] += sum[i][(k * 8 + j) * 64 + t];
+    };
+    if (p.pre) fold(s_pre);
+    if (p.post) fold(s_post);
+    if (p.gate) fold(s_gate);
+    if (w > 0) return;
+  }
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
-    const long long at = unit * a.C;
+    const long long at = (long long)blockIdx.x * a.C;
     if (p.pre) store_row<IO_F32, ALIGNED>(p.pre, at, C, t, tpr, k, s_pre[k]);
     if (p.post) store_row<IO_F32, ALIGNED>(p.post, at, C, t, tpr, k, s_post[k]);
     if (p.gate) store_row<IO_F32, ALIGNED>(p.gate, at, C, t, tpr, k, s_gate[k]);
@@ -398,8 +442,17 @@ __global__ void __launch_bounds__(1024) join_reduce_kernel(JoinReduce q, int C, 
   const int g = b / col_blocks, c = (b % col_blocks) * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
   const float* src = u.src + (size_t)g * u.rows * C + c;
   float s = 0.f;
-  if (c < C)
-    for (int i = w; i < u.rows; i += 16) s += src[(size_t)i * C];
+  if (c < C) {
+    int i = w;
+    for (; i + 7 * 16 < u.rows; i += 8 * 16) {  // eight rows requested at once: 26 -> 9 us at 512 rows of 3 x 4096
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = src[(size_t)(i + 16 * j) * C];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += v[j];
+    }
+    for (; i < u.rows; i += 16) s += src[(size_t)i * C];
+  }
   part[w][threadIdx.x & 63] = s;
   __syncthreads();
   if (w != 0 || c >= C) return;
@@ -421,6 +474,8 @@ hipError_t by_shape(int vpt, F f) {
   return vpt == 1 ? f(std::integral_constant<int, 1>{}) : f(std::integral_constant<int, 2>{});
 }
 
+// One wave a row up to 1024 columns, beyond a workgroup of as many threads as the row has vectors (two a thread past
+// 8192 columns).
 RowShape row_shape(int64_t C) {
   const int vecs = (int)((C + 7) / 8);
   if (vecs <= 128) return {vecs <= 64 ? 1 : 2, false, 256};
@@ -454,13 +509,14 @@ hipError_t bwd_t(const JoinArgs& a, const JoinPlan& p, hipStream_t st) {
     const hipError_t e = by_shape(s.vpt, [&](auto V) {
       constexpr int VPT = decltype(V)::value;
       const dim3 g((unsigned)grid), b((unsigned)s.threads);
-      if (a.aligned) {
-        if (s.multi) hipLaunchKernelGGL((join_bwd_kernel<IO, RIO, VPT, true, true>), g, b, 0, st, a, p);
-        else hipLaunchKernelGGL((join_bwd_kernel<IO, RIO, VPT, true, false>), g, b, 0, st, a, p);
-      } else {
-        if (s.multi) hipLaunchKernelGGL((join_bwd_kernel<IO, RIO, VPT, false, true>), g, b, 0, st, a, p);
-        else hipLaunchKernelGGL((join_bwd_kernel<IO, RIO, VPT, false, false>), g, b, 0, st, a, p);
-      }
+      const auto run = [&](auto A) {
+        constexpr bool AL = decltype(A)::value;
+        if (!s.multi) hipLaunchKernelGGL((join_bwd_kernel<IO, RIO, VPT, AL, 0>), g, b, 0, st, a, p);
+        else if (VPT == 1 && s.threads <= 512) hipLaunchKernelGGL((join_bwd_kernel<IO, RIO, 1, AL, 1>), g, b, 0, st, a, p);
+        else hipLaunchKernelGGL((join_bwd_kernel<IO, RIO, VPT, AL, 2>), g, b, 0, st, a, p);
+      };
+      if (a.aligned) run(std::true_type{});
+      else run(std::false_type{});
       return hipGetLastError();
     });
     if (e != hipSuccess) return e;
@@ -473,9 +529,10 @@ hipError_t bwd_t(const JoinArgs& a, const JoinPlan& p, hipStream_t st) {
     q.t[n++] = JoinSum{src, dst, (int)rows, (int)g};
     groups += g;
   };
-  add(p.pre, a.dw_pre, p.units, 1);
-  add(p.post, a.dw_post, p.units, 1);
-  if (p.gate) add(p.gate, a.dgate, p.parts, a.groups);
+  const int per = s.multi ? 1 : 4;  // units of a workgroup
+  add(p.pre, a.dw_pre, grid, 1);
+  add(p.post, a.dw_post, grid, 1);
+  if (p.gate) add(p.gate, a.dgate, p.parts / per, a.groups);
   else if (a.B == 0) add(nullptr, a.dgate, 0, a.groups);  // (sums of no rows)
   if (n == 0) return hipSuccess;
   const int col_blocks = (int)((a.C + 63) / 64);
@@ -499,13 +556,14 @@ JoinPlan join_plan(int64_t B, int64_t C, int64_t groups, bool dpre, bool dpost, 
     p.parts = (int)((T + rows - 1) / rows);
     p.rows_per_part = (T + p.parts - 1) / p.parts;
     p.parts = (int)((T + p.rows_per_part - 1) / p.rows_per_part);
+    if (!s.multi) p.parts = (p.parts + 3) / 4 * 4;  // a workgroup's four units in one group (the last ones may be empty)
     p.units = groups * p.parts;
   } else if (T > 0) {
     p.groups_per_unit = rows / T;
     p.units = (groups + p.groups_per_unit - 1) / p.groups_per_unit;
   }
   size_t at = 0;
-  const size_t one = (size_t)p.units * C * sizeof(float);
+  const size_t one = (size_t)(s.multi ? p.units : (p.units + 3) / 4) * C * sizeof(float);
   const auto take = [&](bool on) {
     const size_t off = at;
     if (on) at += (one + 255) / 256 * 256;
