@@ -16,6 +16,8 @@
 namespace fmlp {
 namespace {
 
+// Elements of a workgroup of the scaling: 302 M bf16 gradients into fp32 in 390 us with 64 K, 361 with 16 K, 354 with 8 K.
+constexpr long long kScaleChunk = 8192;
 constexpr int kMaxTensors = 112;  // per launch: the table below stays within 4 KB of kernel arguments
 
 struct ClipTable {
@@ -192,46 +194,49 @@ ClipPlan clip_plan(int n, const int64_t* numel, int num_cus) {
   return p;
 }
 
+// f(table, workgroups, workgroups before it) for as many tables as the tensors take, in chunks of `chunk` elements
+template <typename F>
+static hipError_t for_tables(int n, const ClipTensor* t, long long chunk, F f) {
+  long long done = 0;
+  for (int i = 0; i < n;) {
+    ClipTable tab{};
+    long long blocks = 0;
+    for (; i < n && tab.n < kMaxTensors; ++i) {
+      const long long b = (t[i].numel + chunk - 1) / chunk;
+      if (b == 0) continue;
+      if (b > 0x7fffffffLL) return hipErrorInvalidValue;
+      if (blocks + b > 0x7fffffffLL) break;
+      const int k = tab.n++;
+      tab.grad[k] = t[i].grad;
+      tab.out[k] = t[i].out;
+      tab.numel[k] = (unsigned long long)t[i].numel;
+      tab.first[k] = (unsigned)blocks;
+      tab.io[k] = (unsigned char)t[i].io;
+      tab.out_io[k] = (unsigned char)t[i].out_io;
+      blocks += b;
+    }
+    if (blocks == 0) continue;
+    f(tab, blocks, done);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    done += blocks;
+  }
+  return hipSuccess;
+}
+
 hipError_t launch_clip(int n, const ClipTensor* t, const ClipPlan& p, bool clip, float max_norm, float* norm, void* ws,
                        hipStream_t st) {
   double* part = (double*)ws;
   float* coef = clip ? (float*)(part + p.blocks) : nullptr;
-  for (int pass = 0; pass < (clip ? 2 : 1); ++pass) {
-    long long done = 0;
-    int i = 0;
-    while (i < n) {
-      ClipTable tab{};
-      long long blocks = 0;
-      for (; i < n && tab.n < kMaxTensors; ++i) {
-        const long long b = (t[i].numel + p.chunk - 1) / p.chunk;
-        if (b == 0) continue;
-        if (blocks + b > 0x7fffffffLL) break;
-        const int k = tab.n++;
-        tab.grad[k] = t[i].grad;
-        tab.out[k] = t[i].out;
-        tab.numel[k] = (unsigned long long)t[i].numel;
-        tab.first[k] = (unsigned)blocks;
-        tab.io[k] = (unsigned char)t[i].io;
-        tab.out_io[k] = (unsigned char)t[i].out_io;
-        blocks += b;
-      }
-      if (blocks > 0) {
-        if (pass == 0)
-          hipLaunchKernelGGL(norm_kernel, dim3((unsigned)blocks), dim3(256), 0, st, tab, p.chunk, part + done);
-        else
-          hipLaunchKernelGGL(scale_kernel, dim3((unsigned)blocks), dim3(256), 0, st, tab, p.chunk, coef);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-      }
-      done += blocks;
-    }
-    if (pass == 0) {
-      hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(1024), 0, st, part, p.blocks, max_norm, norm, coef);
-      const hipError_t e = hipGetLastError();
-      if (e != hipSuccess) return e;
-    }
-  }
-  return hipSuccess;
+  hipError_t e = for_tables(n, t, p.chunk, [&](const ClipTable& tab, long long blocks, long long done) {
+    hipLaunchKernelGGL(norm_kernel, dim3((unsigned)blocks), dim3(256), 0, st, tab, p.chunk, part + done);
+  });
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(1024), 0, st, part, p.blocks, max_norm, norm, coef);
+  if ((e = hipGetLastError()) != hipSuccess || !clip) return e;
+  return for_tables(n, t, kScaleChunk, [&](const ClipTable& tab, long long blocks, long long) {
+    hipLaunchKernelGGL(scale_kernel, dim3((unsigned)blocks), dim3(256), 0, st, tab, (long long)kScaleChunk, coef);
+  });
 }
 
 }  // namespace fmlp
