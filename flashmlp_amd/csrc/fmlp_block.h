@@ -71,7 +71,7 @@ struct GatedFwdPlan {
   int xs, nct;
   size_t ws_bytes;
 };
-GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus);
+GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus, bool dx);
 hipError_t launch_gated_fwd(const GatedArgs& a, const GatedFwdPlan& p, hipStream_t st);
 // dX on the same forms and plan (fmlp_gated_dx.hip)
 hipError_t launch_gated_dx(const GatedArgs& a, const GatedFwdPlan& p, hipStream_t st);

@@ -82,8 +82,8 @@ int check_ws(const void* ws, size_t have, size_t need) {
     return abi_fail(FMLP_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? have : (size_t)0, need);
   return FMLP_OK;
 }
-fmlp::GatedFwdPlan rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int io, int cus) {
-  return io == FMLP_DTYPE_F32 ? fmlp::gated32_rows_plan(H, B, D, E, cus) : fmlp::gated_fwd_plan(H, B, D, E, cus);
+fmlp::GatedFwdPlan rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int io, int cus, bool dx) {
+  return io == FMLP_DTYPE_F32 ? fmlp::gated32_rows_plan(H, B, D, E, cus) : fmlp::gated_fwd_plan(H, B, D, E, cus, dx);
 }
 fmlp::GatedDwPlan dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int io, int cus) {
   return io == FMLP_DTYPE_F32 ? fmlp::gated32_dw_plan(H, B, D, E, cus) : fmlp::gated_dw_plan(H, B, D, E, cus);
@@ -96,7 +96,7 @@ int io_type(int io) { return io == FMLP_DTYPE_F32 ? fmlp::IO_F32 : io == FMLP_DT
 FMLP_EXPORT size_t fmlp_gated_fwd_workspace_bytes(int64_t H, int64_t B, int64_t D, int64_t E, int dtype) {
   int cus = 0;
   if (check_gated(H, B, D, E, dtype, 0) || !gated_staged(D, dtype) || fmlp::abi_num_cus(&cus)) return 0;
-  return gated_pad_bytes(H, D, E, dtype) + rows_plan(H, B, D, E, dtype, cus).ws_bytes;
+  return gated_pad_bytes(H, D, E, dtype) + rows_plan(H, B, D, E, dtype, cus, false).ws_bytes;
 }
 
 namespace {
@@ -105,7 +105,7 @@ namespace {
 size_t gated_bwd_ws(int64_t H, int64_t B, int64_t D, int64_t E, int dtype, int cus) {
   const int io = io_of(dtype);
   const size_t dw = (dtype & FMLP_BWD_NO_DW) ? 0 : dw_plan(H, B, D, E, io, cus).ws_bytes;
-  const size_t dx = (dtype & FMLP_BWD_NO_DX) ? 0 : rows_plan(H, B, D, E, io, cus).ws_bytes;
+  const size_t dx = (dtype & FMLP_BWD_NO_DX) ? 0 : rows_plan(H, B, D, E, io, cus, true).ws_bytes;
   return gated_pad_bytes(H, D, E, io) + (dw > dx ? dw : dx);
 }
 
@@ -152,7 +152,7 @@ FMLP_EXPORT int fmlp_gated_fwd(const void* x, const void* wg, const void* wu, co
   if (!gated_staged(D, dtype)) {
     e = fmlp::launch_gated_gen_fwd(a, hs);
   } else {
-    const fmlp::GatedFwdPlan p = rows_plan(H, B, D, E, dtype, a.num_cus);
+    const fmlp::GatedFwdPlan p = rows_plan(H, B, D, E, dtype, a.num_cus, false);
     if ((st = check_ws(workspace, workspace_bytes, gated_pad_bytes(H, D, E, dtype) + p.ws_bytes))) return st;
     e = gated_pad(&a, hs);
     if (e == hipSuccess) e = a.io == fmlp::IO_F32 ? fmlp::launch_gated32_fwd(a, p, hs) : fmlp::launch_gated_fwd(a, p, hs);
@@ -213,7 +213,7 @@ FMLP_EXPORT int fmlp_gated_bwd(const void* x, const void* wg, const void* wu, co
       e = a.io == fmlp::IO_F32 ? fmlp::launch_gated32_dw(a, p, hs) : fmlp::launch_gated_dw(a, p, hs);
     }
     if (e == hipSuccess && want_dx) {
-      const fmlp::GatedFwdPlan p = rows_plan(H, B, D, E, io, a.num_cus);
+      const fmlp::GatedFwdPlan p = rows_plan(H, B, D, E, io, a.num_cus, true);
       e = a.io == fmlp::IO_F32 ? fmlp::launch_gated32_dx(a, p, hs) : fmlp::launch_gated_dx(a, p, hs);
     }
   }

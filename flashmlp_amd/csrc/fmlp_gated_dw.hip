@@ -26,21 +26,29 @@
 namespace fmlp {
 namespace {
 
-// EW groups of 32 columns, DP parts of D, NS ring slots; WREG: weight matrices held in registers (3; 2: W2 in LDS;
-// 0: all in LDS)
+// EW groups of 32 columns, DP parts of D, NS ring slots; WREG: weight matrices held in registers (3; 2: W2 in LDS; 1: Wu
+// too; 0: all in LDS)
 struct Form {
   int ew, dp, ns, oc, wreg;
 };
 __host__ __device__ constexpr Form dw_form(int D) {
-  return D == 32 ? Form{4, 1, 4, 2, 3} : D == 64 ? Form{4, 1, 4, 2, 0} : D == 128 ? Form{4, 1, 4, 1, 3} : Form{2, 2, 4, 1, 2};
+  return D == 32 ? Form{4, 1, 4, 2, 3} : D == 64 ? Form{4, 1, 4, 2, 0} : D == 128 ? Form{4, 1, 4, 1, 3} : Form{2, 2, 3, 1, 1};
 }
 // LDS: the ring, then the tiles of Wg and Wu (for good where they are read from there; else for the start only, and
 // in the ring's place where they do not fit beside it), then W2's
-__host__ __device__ constexpr bool dw_own_stage(int D) { return dw_form(D).wreg == 0 || D <= 128; }
-__host__ __device__ constexpr int dw_lds(int D) {
+__host__ __device__ constexpr int dw_wg_off(int D) {
   const Form f = dw_form(D);
-  return f.ns * 128 * D + (dw_own_stage(D) ? 128 * D * f.ew : 0) + (f.wreg == 3 ? 0 : 64 * D * f.ew);
+  return f.wreg == 0 || (f.wreg >= 2 && D <= 128) ? f.ns * 128 * D : 0;
 }
+__host__ __device__ constexpr int dw_wu_off(int D) {
+  const Form f = dw_form(D);
+  return f.wreg == 1 ? f.ns * 128 * D : dw_wg_off(D) + 64 * D * f.ew;
+}
+__host__ __device__ constexpr int dw_w2_off(int D) {
+  const Form f = dw_form(D);
+  return dw_wu_off(D) >= f.ns * 128 * D ? dw_wu_off(D) + 64 * D * f.ew : f.ns * 128 * D;
+}
+__host__ __device__ constexpr int dw_lds(int D) { return dw_w2_off(D) + (dw_form(D).wreg == 3 ? 0 : 64 * D * dw_form(D).ew); }
 
 template <int D>
 __device__ __forceinline__ int swz(int r) {
@@ -58,9 +66,9 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
   constexpr int EW = F.ew, DP = F.dp, NS = F.ns, PF = NS - 1, WREG = F.wreg;
   constexpr int KS = DG / 16, NTO = D / 32 / DP, ROWB = 2 * D, PPR = D / 8, SLOT = 128 * D, DOO = 64 * D;
   constexpr int NPR = D >= 64 ? D / 64 : 1, NLD = D >= 64 ? 2 * NPR : 1;  // loads a thread for X (and dO)
-  constexpr bool STAGE = dw_own_stage(D);
-  constexpr int WL = STAGE ? NS * SLOT : 0, W2L = NS * SLOT + (STAGE ? 128 * D * EW : 0);
-  static_assert(EW * DP == 4 && NLD * PF < 64 && 128 * D * EW <= NS * SLOT, "form");
+  constexpr bool STAGE = dw_wg_off(D) >= NS * SLOT;  // the start's tiles beside the ring
+  constexpr int W2L = dw_w2_off(D);
+  static_assert(EW * DP == 4 && NLD * PF < 64 && 128 * D * EW <= NS * SLOT && dw_lds(D) <= 160 * 1024, "form");
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int eg = DP == 1 ? wave : wave & (EW - 1), dp = DP == 1 ? 0 : wave / EW;
@@ -79,11 +87,11 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
   const u16* W2h = W2 + (size_t)h * E * DG;
 
   // ---- weights: this wave's columns of Wg, Wu as [D][32] tiles through LDS (the ring's place, or their own) ----
-  u32x4 wg[WREG ? KS : 1], wu[WREG ? KS : 1], w2[WREG == 3 ? KS : 1];
+  u32x4 wg[WREG ? KS : 1], wu[WREG >= 2 ? KS : 1], w2[WREG == 3 ? KS : 1];
   const int laneA = (8 * g + (i16 >> 2)) * 64 + 32 * (G & 1) + 8 * (i16 & 3);
-  const int wt = WL + eg * 64 * D;
+  const int wt[2] = {dw_wg_off(D) + eg * 64 * D, dw_wu_off(D) + eg * 64 * D};
   auto opWt = [&](int m, int k) {
-    const int a = wt + m * 64 * D * EW + laneA + k * 1024;
+    const int a = wt[m] + laneA + k * 1024;
     return cat(lds_read_tr(a), lds_read_tr(a + 256));
   };
   {
@@ -94,8 +102,8 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
       const int k = i * DP + dp;
       const unsigned p = (unsigned)(k * 64 + lane), q = (p & 3u) * 8u;
       const unsigned o = (int)q < lim && (p >> 2) < (unsigned)DG ? (p >> 2) * (unsigned)ldw * 2u + q * 2u : BUF_OOB;
-      buf_load16_lds(rg, o, wt + k * 1024);
-      buf_load16_lds(ru, o, wt + 64 * D * EW + k * 1024);
+      buf_load16_lds(rg, o, wt[0] + k * 1024);
+      buf_load16_lds(ru, o, wt[1] + k * 1024);
     }
     if constexpr (WREG == 3) {
 #pragma unroll
@@ -154,7 +162,7 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       wg[k] = opWt(0, k);
-      wu[k] = opWt(1, k);
+      if constexpr (WREG >= 2) wu[k] = opWt(1, k);
     }
     if constexpr (!STAGE) {
       barrier();  // before the ring's loads land on the tiles
@@ -182,6 +190,8 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
     if constexpr (WREG == 3) return m == 0 ? wg[k] : m == 1 ? wu[k] : w2[k];
     if (m == 2) return lds_read16(W2L + eg * 32 * ROWB + ro[k]);
     if constexpr (WREG == 2) return m == 0 ? wg[k] : wu[k];
+    if constexpr (WREG == 1)
+      if (m == 0) return wg[k];
     return opWt(m, k);
   };
 
@@ -237,7 +247,7 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
           if constexpr (m == 2) op.a = opCol(b2 + DOO, s2, n);
         } else if constexpr (i3 < 0) {
           op.a = opRow(b1, i2);
-          if constexpr (WREG == 0) op.w = weight(1, i2);
+          if constexpr (WREG < 2) op.w = weight(1, i2);
         } else {
           op.a = opRow(b1 + DOO, i3);
           if constexpr (WREG != 3) op.w = weight(2, i3);
@@ -272,7 +282,7 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
             a2[n] = mfma<BF16>(op.a, ph[s2], a2[n]);
           }
         } else if constexpr (i3 < 0) {
-          zu = mfma<BF16>(op.a, WREG ? wu[WREG ? i2 : 0] : op.w, i2 == 0 ? zero16() : zu);
+          zu = mfma<BF16>(op.a, WREG >= 2 ? wu[WREG >= 2 ? i2 : 0] : op.w, i2 == 0 ? zero16() : zu);
         } else {
           dh = mfma<BF16>(op.a, WREG == 3 ? w2[WREG == 3 ? i3 : 0] : op.w, i3 == 0 ? zero16() : dh);
 #pragma unroll

@@ -293,7 +293,7 @@ hipError_t by_d(const Args& q) {
 
 }  // namespace
 
-GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus) {
+GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus, bool dx) {
   const int DT = D < 32 ? 32 : (int)D;
   const long long N = num_cus > 0 ? num_cus : 1, nch = (E + 31) / 32;
   static const int force = env_int("FMLP_GATED_FORM", -1), xs_env = env_int("FMLP_GATED_XS", -1);
@@ -308,11 +308,11 @@ GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_
       if (xs != want || (xs_env > 0 && want != std::min<long long>(xs_env, nch))) continue;
       // full rounds of F.per_cu workgroups a CU, and what is left; a split adds a launch and the partials' bytes
       const long long slots = N * F.per_cu, full = tiles * xs / slots, rest = tiles * xs % slots;
-      const double steps = (double)((nct + F.es - 1) / F.es);
+      const double steps = (dx ? 1.4 : 1.0) * (double)((nct + F.es - 1) / F.es);
       double us = (double)full * (F.fixed_us + F.full_us * steps);
       const double share = F.per_cu == 1 ? (double)rest / (double)slots : (double)((rest + N - 1) / N) / (double)F.per_cu;
       if (rest > 0) us += F.fixed_us + steps * std::max(F.chunk_us, F.full_us * share);
-      if (xs > 1) us += 2.8 + (double)(H * B * D * xs) * 8.0 / 4.2e6;
+      if (xs > 1) us += 2.8 + (double)(H * B * D * xs) * 8.0 / 4.8e6;
       if (best_us == 0 || us < best_us) {
         best_us = us;
         best.form = form;
