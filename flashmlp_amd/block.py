@@ -199,6 +199,7 @@ def _needs_grad(*ts) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
+@torch.compiler.disable  # (torch.compile breaks its graph here)
 def block_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, heads: Optional[int] = None,
                dtype: Optional[torch.dtype] = None, eps: float = 1e-6) -> torch.Tensor:
     """RMS norm of a stream x (B, C) into the first block's input.
@@ -217,6 +218,7 @@ def block_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, heads:
     return block_join_fwd(x, None, pre_weight=weight, eps=eps, heads=heads, dtype=dtype)[1]
 
 
+@torch.compiler.disable
 def block_join(residual: torch.Tensor, o: torch.Tensor, post_weight: Optional[torch.Tensor] = None,
                gate: Optional[torch.Tensor] = None, scale: float = 1.0, *, pre_weight: Optional[torch.Tensor] = None,
                post: bool = True, pre: bool = True, eps: float = 1e-6):

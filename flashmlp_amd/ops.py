@@ -1,9 +1,11 @@
 """torch.library registration of the FlashMLP operators (torch.compile / FakeTensor support).
 
-Two custom operators wrap the same C ABI calls as flashmlp_fwd / flashmlp_bwd:
+Custom operators wrap the same C ABI calls as flashmlp_fwd / flashmlp_bwd and their gated forms:
 
     torch.ops.flashmlp_amd.fwd(x, w1, w2, activation="") -> o
     torch.ops.flashmlp_amd.bwd(x, w1, w2, do, activation="", accurate_dw=False) -> (dx, dw1, dw2)
+    torch.ops.flashmlp_amd.gated_fwd(x, wg, wu, w2, activation="") -> o
+    torch.ops.flashmlp_amd.gated_bwd(x, wg, wu, w2, do, activation="") -> (dx, dwg, dwu, dw2)
 
 Each has a fake (meta) implementation that only checks shapes and allocates outputs, so
 FakeTensor tracing, torch.export and torch.compile see through them without launching
@@ -22,6 +24,7 @@ from typing import Tuple
 import torch
 
 from .flashmlp import flashmlp_bwd, flashmlp_fwd
+from .gated import flashmlp_gated_bwd, flashmlp_gated_fwd
 
 
 def _check_shapes(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor) -> None:
@@ -82,3 +85,51 @@ def flashmlp(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, activation: st
              accurate_dw: bool = False) -> torch.Tensor:
     """Differentiable FlashMLP through the registered operator (traceable by torch.compile)."""
     return torch.ops.flashmlp_amd.fwd(x, w1, w2, activation, accurate_dw)
+
+
+# ---------------------------------------------------------------------------------------------
+# the gated MLP:  torch.ops.flashmlp_amd.gated_fwd / gated_bwd
+# ---------------------------------------------------------------------------------------------
+def _check_gated(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, w2: torch.Tensor) -> None:
+    _check_shapes(x, wg, w2)
+    torch._check(wu.dim() == 3 and wu.shape[0] == wg.shape[0] and wu.shape[1] == wg.shape[1]
+                 and wu.shape[2] == wg.shape[2], lambda: "Gate and up projections must match")
+
+
+@torch.library.custom_op("flashmlp_amd::gated_fwd", mutates_args=(), device_types="cuda")
+def gated_fwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, w2: torch.Tensor,
+              activation: str = "") -> torch.Tensor:
+    """O = (act(x @ wg) * (x @ wu)) @ w2 per head on the gfx950 kernels."""
+    return flashmlp_gated_fwd(x, wg, wu, w2, activation)
+
+
+@gated_fwd.register_fake
+def _gated_fwd_fake(x, wg, wu, w2, activation=""):
+    _check_gated(x, wg, wu, w2)
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op("flashmlp_amd::gated_bwd", mutates_args=(), device_types="cuda")
+def gated_bwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, w2: torch.Tensor, do: torch.Tensor,
+              activation: str = "") -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dwg, dwu, dw2) with recomputation on the gfx950 kernels."""
+    return flashmlp_gated_bwd(x, wg, wu, w2, do, activation)
+
+
+@gated_bwd.register_fake
+def _gated_bwd_fake(x, wg, wu, w2, do, activation=""):
+    _check_gated(x, wg, wu, w2)
+    torch._check(x.shape == do.shape, lambda: "Gradient shape mismatch")
+    return x.new_empty(x.shape), wg.new_empty(wg.shape), wu.new_empty(wu.shape), w2.new_empty(w2.shape)
+
+
+def _gated_setup_context(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:4])
+    ctx.activation = inputs[4]
+
+
+def _gated_backward(ctx, do):
+    return (*gated_bwd(*ctx.saved_tensors, do, ctx.activation), None)
+
+
+gated_fwd.register_autograd(_gated_backward, setup_context=_gated_setup_context)
