@@ -76,7 +76,9 @@ SIGNATURES = {
     "fmlp_gated_fwd_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, ctypes.c_int]),
     "fmlp_gated_fwd": (ctypes.c_int, [_vp] * 5 + [_i64] * 5 + [ctypes.c_int, ctypes.c_int, _vp, ctypes.c_size_t, _vp]),
     "fmlp_gated_bwd_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, ctypes.c_int]),
-    "fmlp_gated_bwd": (ctypes.c_int, [_vp] * 9 + [_i64] * 6 + [ctypes.c_int, ctypes.c_int, _vp, ctypes.c_size_t, _vp]),
+    "fmlp_gated_bwd": (ctypes.c_int, [_vp] * 9 + [_i64] * 6 + [ctypes.c_int, ctypes.c_int, ctypes.c_float, _vp,
+                                                               ctypes.c_size_t, _vp]),
+    "fmlp_head_sum": (ctypes.c_int, [_vp, _vp, _i64, _i64, ctypes.c_float, ctypes.c_int, _vp]),
     "fmlp_join_fwd": (ctypes.c_int, [ctypes.POINTER(Join), _vp]),
     "fmlp_join_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Join)]),
     "fmlp_join_bwd": (ctypes.c_int, [ctypes.POINTER(Join), _vp, ctypes.c_size_t, _vp]),

@@ -31,12 +31,17 @@ struct GatedArgs {
   int num_cus;
   void* ws;
   size_t ws_bytes;
+  int out_f32;      // o and dx as fp32 sums (FMLP_OUT_F32)
+  float dw_scale;   // factor of the weight gradients
 };
 
 // Rows of E elements of both matrices copied to rows of ldw elements (whole 16-byte vectors, zeros behind the
 // last element), one after the other at dst, in one launch (fmlp_gated_gen.hip).
 hipError_t launch_gated_pad(const void* wg, const void* wu, void* dst, int64_t rows, int64_t E, int64_t ldw, int es,
                             hipStream_t st);
+
+// dst[i] = scale * sum over H of src[h][i] (n values, a multiple of 4), rounded to io (fmlp_gated_gen.hip).
+hipError_t launch_head_sum(const float* src, void* dst, int64_t n, int64_t H, float scale, int io, hipStream_t st);
 
 // The kernels that read their operands from global memory (fmlp_gated_gen.hip): every io type and D.
 hipError_t launch_gated_gen_fwd(const GatedArgs& a, hipStream_t st);

@@ -13,7 +13,7 @@ using fmlp::abi_ok;
 
 namespace {
 
-constexpr int kGatedFlags = FMLP_BWD_NO_DX | FMLP_BWD_NO_DW;
+constexpr int kGatedFlags = FMLP_BWD_NO_DX | FMLP_BWD_NO_DW | FMLP_OUT_F32;
 
 int io_of(int dtype) { return dtype & ~kGatedFlags; }
 size_t elem_bytes(int io) { return io == FMLP_DTYPE_F32 ? 4 : 2; }
@@ -95,6 +95,7 @@ int io_type(int io) { return io == FMLP_DTYPE_F32 ? fmlp::IO_F32 : io == FMLP_DT
 
 FMLP_EXPORT size_t fmlp_gated_fwd_workspace_bytes(int64_t H, int64_t B, int64_t D, int64_t E, int dtype) {
   int cus = 0;
+  dtype &= ~FMLP_OUT_F32;
   if (check_gated(H, B, D, E, dtype, 0) || !gated_staged(D, dtype) || fmlp::abi_num_cus(&cus)) return 0;
   return gated_pad_bytes(H, D, E, dtype) + rows_plan(H, B, D, E, dtype, cus, false).ws_bytes;
 }
@@ -120,6 +121,8 @@ FMLP_EXPORT size_t fmlp_gated_bwd_workspace_bytes(int64_t H, int64_t B, int64_t 
 FMLP_EXPORT int fmlp_gated_fwd(const void* x, const void* wg, const void* wu, const void* w2, void* o, int64_t H,
                                int64_t B, int64_t D, int64_t E, int64_t x_head_stride, int dtype, int act,
                                void* workspace, size_t workspace_bytes, void* stream) {
+  const bool out_f32 = (dtype & FMLP_OUT_F32) != 0;
+  dtype &= ~FMLP_OUT_F32;
   if (dtype & kGatedFlags)
     return abi_fail(FMLP_ERR_INVALID_ARG, "FMLP_BWD_NO_DX / FMLP_BWD_NO_DW apply to the backward only");
   int st = check_gated(H, B, D, E, dtype, act);
@@ -144,6 +147,8 @@ FMLP_EXPORT int fmlp_gated_fwd(const void* x, const void* wg, const void* wu, co
   a.sx = x_head_stride;
   a.io = io_type(dtype);
   a.act = act;
+  a.out_f32 = out_f32 ? 1 : 0;
+  a.dw_scale = 1.f;
   a.ws = workspace;
   a.ws_bytes = workspace != nullptr ? workspace_bytes : 0;
   if ((st = fmlp::abi_num_cus(&a.num_cus))) return st;
@@ -163,8 +168,8 @@ FMLP_EXPORT int fmlp_gated_fwd(const void* x, const void* wg, const void* wu, co
 
 FMLP_EXPORT int fmlp_gated_bwd(const void* x, const void* wg, const void* wu, const void* w2, const void* dout,
                                void* dx, void* dwg, void* dwu, void* dw2, int64_t H, int64_t B, int64_t D, int64_t E,
-                               int64_t x_head_stride, int64_t dout_head_stride, int dtype, int act, void* workspace,
-                               size_t workspace_bytes, void* stream) {
+                               int64_t x_head_stride, int64_t dout_head_stride, int dtype, int act, float dw_scale,
+                               void* workspace, size_t workspace_bytes, void* stream) {
   int st = check_gated(H, B, D, E, dtype, act);
   if (st) return st;
   const bool rows = H > 0 && B > 0, want_dx = (dtype & FMLP_BWD_NO_DX) == 0, want_dw = (dtype & FMLP_BWD_NO_DW) == 0;
@@ -194,6 +199,8 @@ FMLP_EXPORT int fmlp_gated_bwd(const void* x, const void* wg, const void* wu, co
   a.ldw = E;
   a.sx = x_head_stride;
   a.sdo = dout_head_stride;
+  a.out_f32 = (dtype & FMLP_OUT_F32) ? 1 : 0;
+  a.dw_scale = dw_scale;
   a.io = io_type(io_of(dtype));
   a.act = act;
   a.ws = workspace;
@@ -218,6 +225,18 @@ FMLP_EXPORT int fmlp_gated_bwd(const void* x, const void* wg, const void* wu, co
     }
   }
   if (e != hipSuccess) return abi_fail(FMLP_ERR_HIP, "gated backward launch: %s", hipGetErrorString(e));
+  return abi_ok();
+}
+
+FMLP_EXPORT int fmlp_head_sum(const float* src, void* dst, int64_t H, int64_t n, float scale, int dtype, void* stream) {
+  if (H < 1 || H > (1LL << 30) || n < 0 || n % 4 != 0)
+    return abi_fail(FMLP_ERR_INVALID_ARG, "H=%lld n=%lld: at least one head, n a multiple of 4", (long long)H, (long long)n);
+  if (dtype != FMLP_DTYPE_F16 && dtype != FMLP_DTYPE_BF16 && dtype != FMLP_DTYPE_F32)
+    return abi_fail(FMLP_ERR_UNSUPPORTED, "dtype code %d: fp16 (0), bf16 (1) or fp32 (2)", dtype);
+  int st;
+  if ((st = check_vec(src, "src", n > 0)) || (st = check_vec(dst, "dst", n > 0))) return st;
+  const hipError_t e = fmlp::launch_head_sum(src, dst, n, H, scale, io_type(dtype), (hipStream_t)stream);
+  if (e != hipSuccess) return abi_fail(FMLP_ERR_HIP, "head sum launch: %s", hipGetErrorString(e));
   return abi_ok();
 }
 

@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(dw_for
 gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16* __restrict__ Wu,
                 const u16* __restrict__ W2, const u16* __restrict__ dO, void* __restrict__ dWg, void* __restrict__ dWu,
                 void* __restrict__ dW2, int H, int B, int E, int ldw, long long sx, long long sdo, int nE, int nS,
-                int rows_per_split, float* __restrict__ ws) {
+                int rows_per_split, float scale, float* __restrict__ ws) {
   constexpr Form F = dw_form(D);
   constexpr int EW = F.ew, DP = F.dp, NS = F.ns, PF = NS - 1, WREG = F.wreg;
   constexpr int KS = DG / 16, NTO = D / 32 / DP, ROWB = 2 * D, PPR = D / 8, SLOT = 128 * D, DOO = 64 * D;
@@ -300,12 +300,12 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
     for (int i = 0; i + 1 < NSUB; ++i) {
       const int nxt = cur + 1 == NS ? 0 : cur + 1, far = cur == 0 ? NS - 1 : cur - 1;
       load_sub(i + PF, far);
-      iter(std::true_type{}, cur, nxt);
+      if (D == 256 || e0 < E) iter(std::true_type{}, cur, nxt);  // a wave past the last column only loads (D = 256: spills)
       wait_vmcnt<NLD*(PF - 2)>();  // subtile i + 2
       barrier();
       cur = nxt;
     }
-    iter(std::false_type{}, cur, cur);
+    if (D == 256 || e0 < E) iter(std::false_type{}, cur, cur);
   }
   wait_vmcnt<0>();  // subtiles past the last are still landing, as zeros
 
@@ -324,6 +324,14 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
         }
     return;
   }
+#pragma unroll
+  for (int n = 0; n < NTO; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      ag[n][i] *= scale;
+      au[n][i] *= scale;
+      a2[n][i] *= scale;
+    }
   // through LDS, so that rows leave as whole 16-byte pieces: 2-byte stores from the accumulators' layout took 8 of the
   // 18 us of a program with one subtile (H=32 B=4 D=128 E=1024)
   barrier();  // the ring is read
@@ -381,7 +389,7 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
 template <bool BF16, int D, int DG>
 __global__ void __launch_bounds__(256) gated_dw_reduce(const float* __restrict__ ws, u16* __restrict__ dWg,
                                                        u16* __restrict__ dWu, u16* __restrict__ dW2, int E, int nE,
-                                                       long long quads, int nS) {
+                                                       long long quads, int nS, float scale) {
   constexpr Form F = dw_form(D);
   constexpr int NTO = D / 32 / F.dp;
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x;  // (quads is a multiple of 256)
@@ -405,7 +413,7 @@ __global__ void __launch_bounds__(256) gated_dw_reduce(const float* __restrict__
   const int et = (int)(t % nE), eg = F.dp == 1 ? wave : wave & (F.ew - 1), dp = F.dp == 1 ? 0 : wave / F.ew;
   const size_t h = (size_t)(t / nE);
   const int e0 = (et * F.ew + eg) * 32, d0 = (dp * NTO + n) * 32, l32 = lane & 31, along = 8 * q + 4 * (lane >> 5);
-  const u32x2 w = {pack2<BF16>(v.x, v.y), pack2<BF16>(v.z, v.w)};
+  const u32x2 w = {pack2<BF16>(v.x * scale, v.y * scale), pack2<BF16>(v.z * scale, v.w * scale)};
   if (m == 2) {
     const int e = e0 + l32, d = d0 + along;
     if (e < E && d < DG) *(u32x2*)(dW2 + (h * E + e) * DG + d) = w;
@@ -440,11 +448,11 @@ hipError_t launch(const Args& q) {
   hipLaunchKernelGGL(k, dim3((unsigned)q.p.programs), dim3(256), lds, q.st, (const u16*)a.x, (const u16*)a.wg,
                      (const u16*)a.wu, (const u16*)a.w2, (const u16*)a.dout, a.dwg, a.dwu, a.dw2, (int)a.H, (int)a.B,
                      (int)a.E, (int)a.ldw, (long long)a.sx, (long long)a.sdo, q.p.nE, q.p.nS, q.p.rows_per_split,
-                     (float*)a.ws);
+                     a.dw_scale, (float*)a.ws);
   if ((e = hipGetLastError()) != hipSuccess || q.p.nS == 1) return e;
   const long long quads = (long long)a.H * q.p.nE * 4 * (3 * (D / 32 / dw_form(D).dp) * 256);
   hipLaunchKernelGGL((gated_dw_reduce<BF16, D, DG>), dim3((unsigned)(quads / 256)), dim3(256), 0, q.st, (const float*)a.ws,
-                     (u16*)a.dwg, (u16*)a.dwu, (u16*)a.dw2, (int)a.E, q.p.nE, quads, q.p.nS);
+                     (u16*)a.dwg, (u16*)a.dwu, (u16*)a.dw2, (int)a.E, q.p.nE, quads, q.p.nS, a.dw_scale);
   return hipGetLastError();
 }
 template <bool BF16, int D, int DG = D>
@@ -487,7 +495,6 @@ GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cu
   p.nE = (int)((E + 32 * F.ew - 1) / (32 * F.ew));
   const long long base = H * p.nE, slots = (long long)std::max(num_cus, 1) * F.oc, subs = (B + 31) / 32;
   const size_t tile_bytes = (size_t)4 * (3 * (DT / 32 / F.dp) * 256) * sizeof(float4);  // a program's partials
-  static const int force = env_int("FMLP_GATED_NS", -1);
   // Measured: a program takes fixed_us and, for a subtile, sub_us alone on its CU or full_us on a full device (two a
   // CU at D <= 64, where they gain little on each other: vector issue is shared; one CU with two sets the time). A
   // split adds the sum's launch and the partials' bytes. H=8 B=2048 D=128 E=512: 79 us unsplit, 34 split in eight.
@@ -498,7 +505,6 @@ GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cu
   p.nS = 1;
   p.rows_per_split = (int)std::max<long long>(subs * 32, 32);
   for (long long n = 1; n <= 64 && (n == 1 || n <= subs / 2); ++n) {
-    if (force > 0 && n != std::min<long long>(force, std::max<long long>(subs / 2, 1))) continue;
     const long long per = (subs + n - 1) / n, m = per > 0 ? (subs + per - 1) / per : 1;
     if (m != n && n > 1) continue;
     const long long full = base * n / slots, rest = base * n % slots;

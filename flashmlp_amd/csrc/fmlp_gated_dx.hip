@@ -25,7 +25,8 @@ template <bool BF16, int D, int DG, int ACT, int NW, int ES, int NS, int OC>
 __global__ void __launch_bounds__(NW * ES * 64) __attribute__((amdgpu_waves_per_eu(OC, OC)))
 gated_dx_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16* __restrict__ Wu,
                 const u16* __restrict__ W2, const u16* __restrict__ dO, void* __restrict__ dX, int B, int E, int ldw,
-                long long sx, long long sdo, int H, int T, int xs, int nct, float* __restrict__ ws) {
+                long long sx, long long sdo, int H, int T, int xs, int nct, int outf32,
+                float* __restrict__ ws) {
   constexpr int NT = NW * 64, KS = DG / 16, NTN = D / 32, NPR = 4 * D / NT, NLD = 3 * NPR;
   constexpr int SLOT = 192 * D, WU = 64 * D, W2O = 128 * D, PF = NS - 1;
   static_assert(NPR * NT == 4 * D && NS >= 3 && NLD * (PF - 2) < 64, "chunk loads");
@@ -240,7 +241,7 @@ gated_dx_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
   if (xs > 1)
     store_rows<BF16, D, DG>(o, ws, (size_t)blockIdx.x * (NW * 32) * DG, B - bt * NW * 32, wave * 32, g, l32, 1);
   else
-    store_rows<BF16, D, DG>(o, dX, (size_t)h * B * DG, B, b_wave, g, l32, 0);
+    store_rows<BF16, D, DG>(o, dX, (size_t)h * B * DG, B, b_wave, g, l32, outf32);
 }
 
 struct Args {
@@ -261,10 +262,10 @@ hipError_t launch(const Args& q) {
   const long long grid = q.p.tiles * q.p.xs;
   hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * F.nw * F.es), lds, q.st, (const u16*)a.x, (const u16*)a.wg,
                      (const u16*)a.wu, (const u16*)a.w2, (const u16*)a.dout, a.dx, (int)a.B, (int)a.E, (int)a.ldw,
-                     (long long)a.sx, (long long)a.sdo, (int)a.H, (int)(q.p.tiles / a.H), q.p.xs, q.p.nct, (float*)a.ws);
+                     (long long)a.sx, (long long)a.sdo, (int)a.H, (int)(q.p.tiles / a.H), q.p.xs, q.p.nct, a.out_f32, (float*)a.ws);
   if ((e = hipGetLastError()) != hipSuccess || q.p.xs == 1) return e;
   return launch_tile_reduce((const float*)a.ws, a.dx, BF16, (int)a.B, DG, 32 * F.nw, (int)a.H, (int)(q.p.tiles / a.H),
-                            q.p.xs, (int)q.p.tiles, 0, q.st);
+                            q.p.xs, (int)q.p.tiles, a.out_f32, q.st);
 }
 
 template <bool BF16, int D, int DG, int ACT>

@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
 gated32_dw_kernel(const float* __restrict__ X, const float* __restrict__ Wg, const float* __restrict__ Wu,
                   const float* __restrict__ W2, const float* __restrict__ dO, float* __restrict__ dWg,
                   float* __restrict__ dWu, float* __restrict__ dW2, int H, int B, int E, int ldw, long long sx,
-                  long long sdo, int nE, int nS, int rows_per_split, float* __restrict__ ws) {
+                  long long sdo, int nE, int nS, int rows_per_split, float scale, float* __restrict__ ws) {
   constexpr int KQ = DG / 2, NTN = D / 32, SLOT = 256 * D, NP = 8 * D / 256;
   constexpr bool W2LDS = D > 64;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -269,6 +269,7 @@ gated32_dw_kernel(const float* __restrict__ X, const float* __restrict__ Wg, con
   wait_vmcnt<0>();  // (loads that no subtile waited for)
   const size_t n1 = (size_t)H * E * DG;
   if (nS > 1) {
+    scale = 1.f;  // the sum applies it
     dWg = ws + (size_t)s * 3 * n1;
     dWu = dWg + n1;
     dW2 = dWu + n1;
@@ -278,17 +279,17 @@ gated32_dw_kernel(const float* __restrict__ X, const float* __restrict__ Wg, con
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int r = crow(i, g), c = n * 32;
-      if (e0 + r < E && c + l32 < DG) dW2[((size_t)h * E + e0 + r) * DG + c + l32] = a2[n][i];
+      if (e0 + r < E && c + l32 < DG) dW2[((size_t)h * E + e0 + r) * DG + c + l32] = a2[n][i] * scale;
       if (e < E && c + r < DG) {
         const size_t at = ((size_t)h * DG + c + r) * E + e;
-        dWg[at] = ag[n][i];
-        dWu[at] = au[n][i];
+        dWg[at] = ag[n][i] * scale;
+        dWu[at] = au[n][i] * scale;
       }
     }
 }
 
 __global__ void __launch_bounds__(256) gated32_dw_reduce(const float* __restrict__ ws, float* dWg, float* dWu, float* dW2,
-                                                         long long quads, int nS) {
+                                                         long long quads, int nS, float scale) {
   const long long q = (long long)blockIdx.x * 256 + threadIdx.x;
   if (q >= 3 * quads) return;
   const int m = q >= 2 * quads ? 2 : q >= quads ? 1 : 0;
@@ -301,6 +302,10 @@ __global__ void __launch_bounds__(256) gated32_dw_reduce(const float* __restrict
     v.z += u.z;
     v.w += u.w;
   }
+  v.x *= scale;
+  v.y *= scale;
+  v.z *= scale;
+  v.w *= scale;
   *(float4*)((m == 0 ? dWg : m == 1 ? dWu : dW2) + 4 * (q - m * quads)) = v;
 }
 
@@ -330,11 +335,11 @@ hipError_t launch_dw(const GatedArgs& a, const GatedDwPlan& p, hipStream_t st) {
   hipLaunchKernelGGL(k, dim3((unsigned)p.programs), dim3(256), lds, st, (const float*)a.x, (const float*)a.wg,
                      (const float*)a.wu, (const float*)a.w2, (const float*)a.dout, (float*)a.dwg, (float*)a.dwu,
                      (float*)a.dw2, (int)a.H, (int)a.B, (int)a.E, (int)a.ldw, (long long)a.sx, (long long)a.sdo, p.nE,
-                     p.nS, p.rows_per_split, (float*)a.ws);
+                     p.nS, p.rows_per_split, a.dw_scale, (float*)a.ws);
   if ((e = hipGetLastError()) != hipSuccess || p.nS == 1) return e;
   const long long quads = (long long)a.H * a.E * a.D / 4, blocks = (3 * quads + 255) / 256;
   hipLaunchKernelGGL(gated32_dw_reduce, dim3((unsigned)blocks), dim3(256), 0, st, (const float*)a.ws, (float*)a.dwg,
-                     (float*)a.dwu, (float*)a.dw2, quads, p.nS);
+                     (float*)a.dwu, (float*)a.dw2, quads, p.nS, a.dw_scale);
   return hipGetLastError();
 }
 
@@ -369,11 +374,10 @@ GatedFwdPlan gated32_rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int n
   p.tiles = H * ((B + 127) / 128);
   if (p.tiles <= 0) return p;
   const double chunk_us = 3.4 * (double)std::max<long long>(D, 32) / 64.0;
-  static const int xs_env = env_int("FMLP_GATED_XS", -1);
   double best = 0;
   for (long long want = 1; want <= 16 && want <= nch; ++want) {
     const long long nct = (nch + want - 1) / want, xs = (nch + nct - 1) / nct;
-    if (xs != want || (xs_env > 0 && xs_env != want)) continue;
+    if (xs != want) continue;
     double t = (double)((p.tiles * xs + N - 1) / N) * (double)nct * chunk_us;
     if (xs > 1) t += 3.0 + (double)(H * B * D * xs) * 8.0 / 4.2e6;
     if (best == 0 || t < best) {
@@ -392,12 +396,10 @@ GatedDwPlan gated32_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_
   p.nE = (int)((E + 127) / 128);
   const long long base = H * p.nE;
   const double sub_us = 5.8 * (double)std::max<long long>(D, 32) / 64.0;
-  static const int force = env_int("FMLP_GATED_NS", -1);
   double best = 0;
   p.nS = 1;
   p.rows_per_split = (int)std::max<long long>(subs * 32, 32);
   for (long long n = 1; n <= 32 && (n == 1 || n <= subs); ++n) {
-    if (force > 0 && n != std::min<long long>(force, std::max<long long>(subs, 1))) continue;
     const long long per = std::max<long long>((subs + n - 1) / n, 1);
     if (n > 1 && (subs + per - 1) / per != n) continue;
     double t = (double)((base * n + N - 1) / N) * (4.0 + sub_us * (double)per);

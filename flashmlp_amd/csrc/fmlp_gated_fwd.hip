@@ -33,7 +33,7 @@ template <bool BF16, int D, int DG, int ACT, int NW, int ES, int NS, int OC>
 __global__ void __launch_bounds__(NW * ES * 64) __attribute__((amdgpu_waves_per_eu(OC, OC)))
 gated_fwd_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16* __restrict__ Wu,
                  const u16* __restrict__ W2, void* __restrict__ O, int B, int E, int ldw, long long sx, int H, int T,
-                 int xs, int nct, float* __restrict__ ws) {
+                 int xs, int nct, int outf32, float* __restrict__ ws) {
   constexpr int NT = NW * 64, KS = DG / 16, NTN = D / 32, NPR = 4 * D / NT, NLD = 3 * NPR;
   constexpr int SLOT = 192 * D, WU = 64 * D, W2O = 128 * D, PF = NS - 1;
   static_assert(NPR * NT == 4 * D && NS >= 3 && NLD * (PF - 2) < 64, "chunk loads");
@@ -236,7 +236,7 @@ gated_fwd_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u1
   if (xs > 1)
     store_rows<BF16, D, DG>(o, ws, (size_t)blockIdx.x * (NW * 32) * DG, B - bt * NW * 32, wave * 32, g, l32, 1);
   else
-    store_rows<BF16, D, DG>(o, O, (size_t)h * B * DG, B, b_wave, g, l32, 0);
+    store_rows<BF16, D, DG>(o, O, (size_t)h * B * DG, B, b_wave, g, l32, outf32);
 }
 
 struct Args {
@@ -257,10 +257,10 @@ hipError_t launch(const Args& q) {
   const long long grid = q.p.tiles * q.p.xs;
   hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * F.nw * F.es), lds, q.st, (const u16*)a.x, (const u16*)a.wg,
                      (const u16*)a.wu, (const u16*)a.w2, a.o, (int)a.B, (int)a.E, (int)a.ldw, (long long)a.sx, (int)a.H,
-                     (int)(q.p.tiles / a.H), q.p.xs, q.p.nct, (float*)a.ws);
+                     (int)(q.p.tiles / a.H), q.p.xs, q.p.nct, a.out_f32, (float*)a.ws);
   if ((e = hipGetLastError()) != hipSuccess || q.p.xs == 1) return e;
   return launch_tile_reduce((const float*)a.ws, a.o, BF16, (int)a.B, DG, 32 * F.nw, (int)a.H, (int)(q.p.tiles / a.H),
-                            q.p.xs, (int)q.p.tiles, 0, q.st);
+                            q.p.xs, (int)q.p.tiles, a.out_f32, q.st);
 }
 
 template <bool BF16, int D, int DG, int ACT>
@@ -296,16 +296,15 @@ hipError_t by_d(const Args& q) {
 GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus, bool dx) {
   const int DT = D < 32 ? 32 : (int)D;
   const long long N = num_cus > 0 ? num_cus : 1, nch = (E + 31) / 32;
-  static const int force = env_int("FMLP_GATED_FORM", -1), xs_env = env_int("FMLP_GATED_XS", -1);
   GatedFwdPlan best{};
   double best_us = 0;
   for (int form = 0; form < 3; ++form) {
     const GatedForm F = gated_form(DT, form, false);
-    if (F.nw == 0 || (force >= 0 && form != force)) continue;
+    if (F.nw == 0) continue;
     const long long tiles = H * ((B + 32 * F.nw - 1) / (32 * F.nw));
     for (long long want = 1; want <= 16 && want <= nch; ++want) {
       const long long nct = (nch + want - 1) / want, xs = (nch + nct - 1) / nct;
-      if (xs != want || (xs_env > 0 && want != std::min<long long>(xs_env, nch))) continue;
+      if (xs != want) continue;
       // full rounds of F.per_cu workgroups a CU, and what is left; a split adds a launch and the partials' bytes
       const long long slots = N * F.per_cu, full = tiles * xs / slots, rest = tiles * xs % slots;
       const double steps = (dx ? 1.4 : 1.0) * (double)((nct + F.es - 1) / F.es);

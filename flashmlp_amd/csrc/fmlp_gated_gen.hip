@@ -271,10 +271,10 @@ __global__ void __launch_bounds__(64) gated_gen_dw(GatedArgs a, int etiles) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int r = crow(i, g), d = d0 + n * 32;
-      if (e0 + r < E && d + l32 < D) put<IO>(a.dw2, ((size_t)h * E + e0 + r) * D + d + l32, s2[n][i]);
+      if (e0 + r < E && d + l32 < D) put<IO>(a.dw2, ((size_t)h * E + e0 + r) * D + d + l32, s2[n][i] * a.dw_scale);
       if (d + r < D && e < E) {
-        put<IO>(a.dwg, ((size_t)h * D + d + r) * E + e, sg[n][i]);
-        put<IO>(a.dwu, ((size_t)h * D + d + r) * E + e, su[n][i]);
+        put<IO>(a.dwg, ((size_t)h * D + d + r) * E + e, sg[n][i] * a.dw_scale);
+        put<IO>(a.dwu, ((size_t)h * D + d + r) * E + e, su[n][i] * a.dw_scale);
       }
     }
 }
@@ -329,7 +329,50 @@ __global__ void __launch_bounds__(256) pad_pair_kernel(const T* __restrict__ wg,
   *(u32x4*)(dst + p * N) = w;
 }
 
+// dst[i] = scale * sum over the heads of src[head][i], in head order, four values a thread.
+template <int IO>
+__global__ void __launch_bounds__(256) head_sum_kernel(const float* __restrict__ src, void* __restrict__ dst, long long n,
+                                                       int H, float scale) {
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  float4 v = *(const float4*)(src + i);
+  int h = 1;
+  for (; h + 4 <= H; h += 4) {
+    float4 u[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) u[k] = *(const float4*)(src + (size_t)(h + k) * n + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v.x += u[k].x;
+      v.y += u[k].y;
+      v.z += u[k].z;
+      v.w += u[k].w;
+    }
+  }
+  for (; h < H; ++h) {
+    const float4 u = *(const float4*)(src + (size_t)h * n + i);
+    v.x += u.x;
+    v.y += u.y;
+    v.z += u.z;
+    v.w += u.w;
+  }
+  v = float4{v.x * scale, v.y * scale, v.z * scale, v.w * scale};
+  if constexpr (IO == IO_F32) *(float4*)((float*)dst + i) = v;
+  else *(u32x2*)((u16*)dst + i) = u32x2{pack2<IO == IO_BF16>(v.x, v.y), pack2<IO == IO_BF16>(v.z, v.w)};
+}
+
 }  // namespace
+
+hipError_t launch_head_sum(const float* src, void* dst, int64_t n, int64_t H, float scale, int io, hipStream_t st) {
+  const long long blocks = (n / 4 + 255) / 256;
+  if (blocks <= 0) return hipSuccess;
+  if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+  const dim3 g((unsigned)blocks), b(256);
+  if (io == IO_F32) hipLaunchKernelGGL(head_sum_kernel<IO_F32>, g, b, 0, st, src, dst, (long long)n, (int)H, scale);
+  else if (io == IO_BF16) hipLaunchKernelGGL(head_sum_kernel<IO_BF16>, g, b, 0, st, src, dst, (long long)n, (int)H, scale);
+  else hipLaunchKernelGGL(head_sum_kernel<IO_F16>, g, b, 0, st, src, dst, (long long)n, (int)H, scale);
+  return hipGetLastError();
+}
 
 hipError_t launch_gated_pad(const void* wg, const void* wu, void* dst, int64_t rows, int64_t E, int64_t ldw, int es,
                             hipStream_t st) {

@@ -289,12 +289,14 @@ bool gated_ok(const at::Tensor* const* ts, int n, int* code) {
   return n < 5 || ts[4]->sizes() == x.sizes();
 }
 
+// (x may be one matrix for every head: its head stride is 0; out_f32: unrounded)
 at::Tensor gated_fwd_run(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& w2, int code,
-                         int act) {
+                         int act, bool out_f32 = false) {
   const int64_t H = x.size(0), B = x.size(1), D = x.size(2), E = wg.size(2);
   c10::DeviceGuard guard(x.device());
   const hipStream_t stream = c10::hip::getCurrentHIPStream(x.device().index()).stream();
-  at::Tensor o = empty_dense(x), ws;
+  at::Tensor o = out_f32 ? at::empty(x.sizes(), x.options().dtype(at::kFloat)) : empty_dense(x), ws;
+  if (out_f32) code |= FMLP_OUT_F32;
   const size_t n = fmlp_gated_fwd_workspace_bytes(H, B, D, E, code);
   if (n) ws = bytes_on(x, n);
   check_status(fmlp_gated_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), w2.data_ptr(), o.data_ptr(), H, B, D, E,
@@ -305,25 +307,26 @@ at::Tensor gated_fwd_run(const at::Tensor& x, const at::Tensor& wg, const at::Te
 
 // (dx, dwg, dwu, dw2); those that are not wanted undefined
 std::vector<at::Tensor> gated_bwd_run(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& w2,
-                                      const at::Tensor& dout, int code, int act, bool need_dx, bool need_dw) {
+                                      const at::Tensor& dout, int code, int act, bool need_dx, bool need_dw,
+                                      bool out_f32 = false, float dw_scale = 1.f) {
   std::vector<at::Tensor> g(4);
   if (!need_dx && !need_dw) return g;
   const int64_t H = x.size(0), B = x.size(1), D = x.size(2), E = wg.size(2);
   c10::DeviceGuard guard(x.device());
   const hipStream_t stream = c10::hip::getCurrentHIPStream(x.device().index()).stream();
-  if (need_dx) g[0] = empty_dense(x);
+  if (need_dx) g[0] = out_f32 ? at::empty(x.sizes(), x.options().dtype(at::kFloat)) : empty_dense(x);
   if (need_dw) {
     g[1] = at::empty_like(wg);
     g[2] = at::empty_like(wu);
     g[3] = at::empty_like(w2);
   }
-  const int flags = code | (need_dx ? 0 : FMLP_BWD_NO_DX) | (need_dw ? 0 : FMLP_BWD_NO_DW);
+  const int flags = code | (need_dx ? 0 : FMLP_BWD_NO_DX) | (need_dw ? 0 : FMLP_BWD_NO_DW) | (out_f32 ? FMLP_OUT_F32 : 0);
   at::Tensor ws;
   const size_t n = fmlp_gated_bwd_workspace_bytes(H, B, D, E, flags);
   if (n) ws = bytes_on(x, n);
   auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
   check_status(fmlp_gated_bwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), w2.data_ptr(), dout.data_ptr(), ptr(g[0]),
-                              ptr(g[1]), ptr(g[2]), ptr(g[3]), H, B, D, E, x.stride(0), dout.stride(0), flags, act,
+                              ptr(g[1]), ptr(g[2]), ptr(g[3]), H, B, D, E, x.stride(0), dout.stride(0), flags, act, dw_scale,
                               n ? ws.data_ptr() : nullptr, n, stream),
                "gated backward");
   return g;
@@ -359,6 +362,49 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
   }
 };
 
+at::Tensor head_sum(const at::Tensor& t, float scale, const at::Tensor& like) {
+  c10::DeviceGuard guard(t.device());
+  at::Tensor out = at::empty({t.size(1), t.size(2)}, like.options());
+  check_status(fmlp_head_sum(t.data_ptr<float>(), out.data_ptr(), t.size(0), out.numel(), scale, io_code(like),
+                             c10::hip::getCurrentHIPStream(t.device().index()).stream()),
+               "head sum");
+  return out;
+}
+at::Tensor every_head(const at::Tensor& t, int64_t H) { return t.unsqueeze(0).expand({H, t.size(0), t.size(1)}); }
+
+// One input (B, D) through every head, the mean over heads (gated.py's _SharedGatedFunction)
+struct SharedGatedFn : torch::autograd::Function<SharedGatedFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
+                            const at::Tensor& w2, int64_t code, int64_t act) {
+    ctx->save_for_backward({x, wg, wu, w2});
+    ctx->saved_data["code"] = code;
+    ctx->saved_data["act"] = act;
+    const int64_t H = wg.size(0);
+    return head_sum(gated_fwd_run(every_head(x, H), wg, wu, w2, (int)code, (int)act, true), 1.f / (float)H, x);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_once();
+    const auto s = ctx->get_saved_variables();
+    const int code = (int)ctx->saved_data["code"].toInt(), act = (int)ctx->saved_data["act"].toInt();
+    variable_list r(6);
+    if (!grads[0].defined()) return r;
+    const int64_t H = s[1].size(0);
+    at::Tensor dout = every_head(grads[0], H);
+    if (!rows16(dout) || dout.is_neg()) {
+      at::Tensor d = grads[0].contiguous();
+      if ((reinterpret_cast<uintptr_t>(d.data_ptr()) & 15u) != 0) d = d.clone(at::MemoryFormat::Contiguous);
+      dout = every_head(d, H);
+    }
+    const bool dw = ctx->needs_input_grad(1) || ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
+    const float scale = 1.f / (float)H;
+    auto g = gated_bwd_run(every_head(s[0], H), s[1], s[2], s[3], dout, code, act, ctx->needs_input_grad(0), dw, true, scale);
+    if (ctx->needs_input_grad(0)) r[0] = head_sum(g[0], scale, s[0]);
+    for (int i = 1; i < 4; ++i)
+      if (ctx->needs_input_grad(i)) r[i] = g[i];
+    return r;
+  }
+};
+
 bool unpack(PyObject* const* args, int n, const at::Tensor** ts) {
   for (int i = 0; i < n; ++i) {
     if (!THPVariable_Check(args[i])) return false;
@@ -388,6 +434,21 @@ PyObject* fast_gated(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int act = (int)PyLong_AsLong(args[4]);
   if (act == -1 && PyErr_Occurred()) return nullptr;
   return THPVariable_Wrap(GatedFn::apply(*ts[0], *ts[1], *ts[2], *ts[3], (int64_t)code, (int64_t)act));
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_shared(x (B, D), wg, wu, w2, act) -> the mean over heads with its autograd node, or None
+PyObject* fast_gated_shared(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* ts[4];
+  int code = 0;
+  if (nargs != 5 || !unpack(args, 4, ts) || ts[0]->dim() != 2 || ts[1]->dim() != 3 || !ts[0]->is_cuda()) Py_RETURN_NONE;
+  const at::Tensor x3 = every_head(ts[0]->detach(), ts[1]->size(0));
+  const at::Tensor* t3[4] = {&x3, ts[1], ts[2], ts[3]};
+  if (!gated_ok(t3, 4, &code)) Py_RETURN_NONE;
+  const int act = (int)PyLong_AsLong(args[4]);
+  if (act == -1 && PyErr_Occurred()) return nullptr;
+  return THPVariable_Wrap(SharedGatedFn::apply(*ts[0], *ts[1], *ts[2], *ts[3], (int64_t)code, (int64_t)act));
   END_HANDLE_TH_ERRORS
 }
 
@@ -673,6 +734,8 @@ PyMethodDef kMethods[] = {
      "bwd(x, w1, w2, do, act, flags) -> (status, dx, dw1, dw2) or None"},
     {"gated_fwd", (PyCFunction)(void (*)(void))fast_gated_fwd, METH_FASTCALL, "gated_fwd(x, wg, wu, w2, act) -> o or None"},
     {"gated", (PyCFunction)(void (*)(void))fast_gated, METH_FASTCALL, "gated(x, wg, wu, w2, act) -> o or None"},
+    {"gated_shared", (PyCFunction)(void (*)(void))fast_gated_shared, METH_FASTCALL,
+     "gated_shared(x, wg, wu, w2, act) -> the mean over heads or None"},
     {"gated_bwd", (PyCFunction)(void (*)(void))fast_gated_bwd, METH_FASTCALL,
      "gated_bwd(x, wg, wu, w2, do, act, need_dx, need_dw) -> (dx, dwg, dwu, dw2) or None"},
     {"join", (PyCFunction)(void (*)(void))fast_join, METH_FASTCALL,

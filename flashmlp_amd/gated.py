@@ -19,7 +19,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .flashmlp import (_HeadMean, _act_code, _alloc_ws, _current_device, _dense_all, _empty_as, _fast, _io_code, _ptr,
+from .flashmlp import (_DTYPES, _act_code, _alloc_ws, _current_device, _dense_all, _empty_as, _fast, _io_code, _ptr,
                        _rows, _stream_of)
 
 
@@ -52,6 +52,58 @@ class _On:
             torch.cuda.set_device(self.prev)
 
 
+def _fwd(x, wg, wu, w2, activation, out_f32=False):
+    """the general path: views and bases that the kernels do not read are copied first"""
+    H, B, D, E = _check(x, wg, wu, w2)
+    dtype = _io_code(x, wg, wu, w2)
+    o = torch.empty((H, B, D), dtype=torch.float32, device=x.device) if out_f32 else _empty_as(x, (H, B, D))
+    dtype |= _lib.FMLP_OUT_F32 if out_f32 else 0
+    L = _lib.lib()
+    with _On(x.get_device()) as stream:
+        x = _rows(x)
+        wg, wu, w2 = _dense_all(wg, wu, w2)
+        n = L.fmlp_gated_fwd_workspace_bytes(H, B, D, E, dtype)
+        ws = _alloc_ws(n, x.device)
+        st = L.fmlp_gated_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), w2.data_ptr(), o.data_ptr(), H, B, D, E,
+                              x.stride(0), dtype, _act_code(activation), _ptr(ws), n, stream)
+    _lib.check(st, "gated forward")
+    return o
+
+
+def _bwd(x, wg, wu, w2, do, activation, need_dx, need_dw, out_f32=False, dw_scale=1.0):
+    H, B, D, E = _check(x, wg, wu, w2)
+    assert x.shape == do.shape, "Gradient shape mismatch"
+    dtype = _io_code(x, wg, wu, w2, do)
+    dx = None
+    if need_dx:
+        dx = torch.empty((H, B, D), dtype=torch.float32, device=x.device) if out_f32 else _empty_as(x, (H, B, D))
+    dwg, dwu, dw2 = ((_empty_as(t, t.shape) for t in (wg, wu, w2)) if need_dw else (None, None, None))
+    if not (need_dx or need_dw):
+        return dx, dwg, dwu, dw2
+    dtype |= (0 if need_dx else _lib.FMLP_BWD_NO_DX) | (0 if need_dw else _lib.FMLP_BWD_NO_DW)
+    dtype |= _lib.FMLP_OUT_F32 if out_f32 else 0
+    L = _lib.lib()
+    with _On(x.get_device()) as stream:
+        x, do = _rows(x), _rows(do)
+        wg, wu, w2 = _dense_all(wg, wu, w2)
+        n = L.fmlp_gated_bwd_workspace_bytes(H, B, D, E, dtype)
+        ws = _alloc_ws(n, x.device)
+        st = L.fmlp_gated_bwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), w2.data_ptr(), do.data_ptr(), _ptr(dx),
+                              _ptr(dwg), _ptr(dwu), _ptr(dw2), H, B, D, E, x.stride(0), do.stride(0), dtype,
+                              _act_code(activation), dw_scale, _ptr(ws), n, stream)
+    _lib.check(st, "gated backward")
+    return dx, dwg, dwu, dw2
+
+
+def _head_sum(t: torch.Tensor, scale: float, dtype: torch.dtype) -> torch.Tensor:
+    """scale * the sum over heads of fp32 (H, B, D), rounded once"""
+    out = torch.empty(t.shape[1:], dtype=dtype, device=t.device)
+    with _On(t.get_device()) as stream:
+        st = _lib.lib().fmlp_head_sum(t.data_ptr(), out.data_ptr(), t.shape[0], out.numel(), scale, _DTYPES[dtype], stream)
+    _lib.check(st, "head sum")
+    return out
+
+
 def flashmlp_gated_fwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, w2: torch.Tensor,
                        activation: str = "") -> torch.Tensor:
     """O = (act(x @ wg) * (x @ wu)) @ w2 per head.
@@ -67,19 +119,7 @@ def flashmlp_gated_fwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, w2: 
         o = _fast.gated_fwd(x, wg, wu, w2, _act_code(activation))
         if o is not None:
             return o
-    H, B, D, E = _check(x, wg, wu, w2)
-    dtype = _io_code(x, wg, wu, w2)
-    o = _empty_as(x, (H, B, D))
-    L = _lib.lib()
-    with _On(x.get_device()) as stream:
-        x = _rows(x)
-        wg, wu, w2 = _dense_all(wg, wu, w2)
-        n = L.fmlp_gated_fwd_workspace_bytes(H, B, D, E, dtype)
-        ws = _alloc_ws(n, x.device)
-        st = L.fmlp_gated_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), w2.data_ptr(), o.data_ptr(), H, B, D, E,
-                              x.stride(0), dtype, _act_code(activation), _ptr(ws), n, stream)
-    _lib.check(st, "gated forward")
-    return o
+    return _fwd(x, wg, wu, w2, activation)
 
 
 def flashmlp_gated_bwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, w2: torch.Tensor, do: torch.Tensor,
@@ -95,25 +135,7 @@ def flashmlp_gated_bwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, w2: 
         g = _fast.gated_bwd(x, wg, wu, w2, do, _act_code(activation), need_dx, need_dw)
         if g is not None:
             return g
-    H, B, D, E = _check(x, wg, wu, w2)
-    assert x.shape == do.shape, "Gradient shape mismatch"
-    dtype = _io_code(x, wg, wu, w2, do)
-    dx = _empty_as(x, (H, B, D)) if need_dx else None
-    dwg, dwu, dw2 = ((_empty_as(t, t.shape) for t in (wg, wu, w2)) if need_dw else (None, None, None))
-    if not (need_dx or need_dw):
-        return dx, dwg, dwu, dw2
-    dtype |= (0 if need_dx else _lib.FMLP_BWD_NO_DX) | (0 if need_dw else _lib.FMLP_BWD_NO_DW)
-    L = _lib.lib()
-    with _On(x.get_device()) as stream:
-        x, do = _rows(x), _rows(do)
-        wg, wu, w2 = _dense_all(wg, wu, w2)
-        n = L.fmlp_gated_bwd_workspace_bytes(H, B, D, E, dtype)
-        ws = _alloc_ws(n, x.device)
-        st = L.fmlp_gated_bwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), w2.data_ptr(), do.data_ptr(), _ptr(dx),
-                              _ptr(dwg), _ptr(dwu), _ptr(dw2), H, B, D, E, x.stride(0), do.stride(0), dtype,
-                              _act_code(activation), _ptr(ws), n, stream)
-    _lib.check(st, "gated backward")
-    return dx, dwg, dwu, dw2
+    return _bwd(x, wg, wu, w2, do, activation, need_dx, need_dw)
 
 
 class GatedFlashMLPFunction(torch.autograd.Function):
@@ -135,6 +157,29 @@ class GatedFlashMLPFunction(torch.autograd.Function):
         return (dx, *(g if n else None for g, n in zip(dw, need[1:4])), None)
 
 
+class _SharedGatedFunction(torch.autograd.Function):
+    """One input (B, D) through every head, the mean over heads: per head in fp32, rounded once behind the sum. The
+    gradient of the mean is the same for every head; its 1 / H goes into the sums' and gradients' rounding."""
+
+    @staticmethod
+    def forward(ctx, x, wg, wu, w2, activation):
+        H = wg.shape[0]
+        o = _fwd(x.unsqueeze(0).expand(H, *x.shape), wg, wu, w2, activation, out_f32=True)
+        ctx.save_for_backward(x, wg, wu, w2)
+        ctx.activation = activation
+        return _head_sum(o, 1.0 / H, x.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        x, wg, wu, w2 = ctx.saved_tensors
+        H, need = wg.shape[0], ctx.needs_input_grad
+        dx, *dw = _bwd(x.unsqueeze(0).expand(H, *x.shape), wg, wu, w2, do.unsqueeze(0).expand(H, *do.shape),
+                       ctx.activation, need[0], any(need[1:4]), out_f32=True, dw_scale=1.0 / H)
+        dx = _head_sum(dx, 1.0 / H, x.dtype) if need[0] else None
+        return (dx, *(g if n else None for g, n in zip(dw, need[1:4])), None)
+
+
 class GatedFlashMLP(torch.nn.Module):
     """Gated multi-head MLP module (the gated form of FlashMLP).
 
@@ -147,7 +192,8 @@ class GatedFlashMLP(torch.nn.Module):
         device: device of the weights
 
     Parameters wg, wu (H, D, E) ~ randn / sqrt(D) and w2 (H, E, D) ~ randn / sqrt(E). A 2-D input
-    (B, D) is expanded to every head and the output is the mean over heads, as in FlashMLP.
+    (B, D) goes through every head and the output is the mean over heads, as in FlashMLP; the heads'
+    results, and the gradient of x, are summed in fp32 and rounded once.
     """
 
     def __init__(self, num_heads: int, hidden_dim: int, intermediate_dim: int, activation: str = "silu",
@@ -166,16 +212,14 @@ class GatedFlashMLP(torch.nn.Module):
         self.w2 = weight(intermediate_dim, hidden_dim)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        w, act = (self.wg, self.wu, self.w2), self.activation
         shared = x.dim() == 2
-        if shared:
-            x = x.unsqueeze(0).expand(self.num_heads, -1, -1)
         if torch.compiler.is_compiling():  # the registered operator is what torch.compile traces through
-            o = torch.ops.flashmlp_amd.gated_fwd(x, self.wg, self.wu, self.w2, self.activation)
+            xh = x.unsqueeze(0).expand(self.num_heads, -1, -1) if shared else x
+            o = torch.ops.flashmlp_amd.gated_fwd(xh, *w, act)
             return o.mean(dim=0) if shared else o
-        # the same autograd node in C++ where the kernels read the tensors in place
-        o = _fast.gated(x, self.wg, self.wu, self.w2, _act_code(self.activation)) if _fast is not None else None
-        if o is None:
-            o = GatedFlashMLPFunction.apply(x, self.wg, self.wu, self.w2, self.activation)
-        if shared:
-            o = _HeadMean.apply(o) if o.requires_grad else o.mean(dim=0)
-        return o
+        if _fast is not None:  # the same autograd nodes in C++ where the kernels read the tensors in place
+            o = (_fast.gated_shared if shared else _fast.gated)(x, *w, _act_code(act))
+            if o is not None:
+                return o
+        return (_SharedGatedFunction if shared else GatedFlashMLPFunction).apply(x, *w, act)

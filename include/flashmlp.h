@@ -42,7 +42,8 @@ extern "C" {
                               splits ragged dX tiles). Raised where an entry point that was
                               there changes; added within 4, with no change to the others:
                               fmlp_shape_dense, fmlp_fwd_strided_ws, fmlp_copy_dense, the
-                              fmlp_gated_*, fmlp_join_* and fmlp_clip_* calls, fmlp_grad_norm */
+                              fmlp_gated_*, fmlp_join_* and fmlp_clip_* calls, fmlp_head_sum,
+                              fmlp_grad_norm */
 
 typedef enum {
   FMLP_OK = 0,
@@ -268,7 +269,9 @@ int fmlp_bwd_noalloc(const void* x, const void* w1, const void* w2, const void* 
  * Weights and outputs are dense, 16-byte aligned; x and dout have dense rows and heads *_head_stride
  * elements apart (any multiple of 16 bytes, 0: one matrix shared by every head). D in {16, 32, 64, 128,
  * 256}, E >= 1, H, B >= 0; B = 0 leaves zero weight gradients. dtype: fp16, bf16 or fp32; the backward
- * also takes FMLP_BWD_NO_DX and FMLP_BWD_NO_DW. The workspace (16-byte aligned, scratch for the duration
+ * also takes FMLP_BWD_NO_DX and FMLP_BWD_NO_DW. With FMLP_OUT_F32 o and dx are fp32 arrays of the unrounded sums (the
+ * weight gradients keep the io dtype). dw_scale multiplies the weight gradients before their rounding (1 for the
+ * gradients themselves). The workspace (16-byte aligned, scratch for the duration
  * of the call on `stream`) is at least *_workspace_bytes() for the same arguments, and may be NULL where
  * that is 0. Results do not depend on the workspace's content and are bitwise repeatable.
  */
@@ -279,7 +282,12 @@ int fmlp_gated_fwd(const void* x, const void* wg, const void* wu, const void* w2
 size_t fmlp_gated_bwd_workspace_bytes(int64_t H, int64_t B, int64_t D, int64_t E, int dtype);
 int fmlp_gated_bwd(const void* x, const void* wg, const void* wu, const void* w2, const void* dout, void* dx,
                    void* dwg, void* dwu, void* dw2, int64_t H, int64_t B, int64_t D, int64_t E, int64_t x_head_stride,
-                   int64_t dout_head_stride, int dtype, int act, void* workspace, size_t workspace_bytes, void* stream);
+                   int64_t dout_head_stride, int dtype, int act, float dw_scale, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* dst[i] = scale * (src[0][i] + src[1][i] + ...) over H heads of n values (a multiple of 4), summed in head order and
+ * rounded to dtype once: the mean or sum over heads of fp32 outputs (FMLP_OUT_F32). 16-byte aligned. */
+int fmlp_head_sum(const float* src, void* dst, int64_t H, int64_t n, float scale, int dtype, void* stream);
 
 /*
  * A block's output joined to its residual stream, and the next block's input taken from it, in one pass:

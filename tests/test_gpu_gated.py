@@ -104,22 +104,28 @@ def test_views(dt):
     assert all(torch.equal(a, b) for a, b in zip(got, ref))
 
 
-@pytest.mark.parametrize("dt", [BF, FL])
-def test_module_and_shared_input(dt):
-    """2-D input: expanded to every head, mean over heads; its gradient is the sum over heads."""
+@pytest.mark.parametrize("dt,H,B,D,E", [(BF, 4, 50, 64, 96), (HF, 12, 33, 128, 100), (FL, 3, 40, 64, 45), (FL, 2, 9, 256, 20),
+                                        (BF, 1, 1, 16, 8)])
+@pytest.mark.parametrize("view", [False, True])
+def test_module_and_shared_input(dt, H, B, D, E, view):
+    """2-D input: through every head, mean over heads. Each output is a sum over heads of the heads' own results, whose
+    operands are rounded as ever and which is rounded once itself: the bounds of the heads add up."""
     torch.manual_seed(1)
-    H, B, D, E = 4, 50, 64, 96
     m = GatedFlashMLP(H, D, E, dtype=dt)
-    x = torch.randn(B, D, dtype=dt, device="cuda", requires_grad=True)
-    gy = torch.randn(B, D, dtype=dt, device="cuda")
+    x = torch.randn(B, D, device="cuda").to(dt)
+    gy = torch.randn(B, D, device="cuda").to(dt)
+    if view:  # columns that are not dense: the general path
+        x, gy = (torch.stack([v, v], -1).flatten(-2)[:, ::2] for v in (x, gy))
+    x.requires_grad_(True)
     o = m(x)
-    g = torch.autograd.grad(o, (x, m.wg, m.wu, m.w2), gy)
-    xe = x.detach().expand(H, B, D).contiguous()
-    w = [p.detach() for p in (m.wg, m.wu, m.w2)]
-    o3 = flashmlp_gated_fwd(xe, *w, "silu")
-    d3 = flashmlp_gated_bwd(xe, *w, (gy / H).expand(H, B, D).contiguous(), "silu")
-    assert torch.equal(o, o3.mean(0)) and torch.equal(g[0], d3[0].sum(0))
-    assert all(torch.equal(a, b) for a, b in zip(g[1:], d3[1:]))
+    got = (o, *torch.autograd.grad(o, (x, m.wg, m.wu, m.w2), gy))
+    t = (x.detach().expand(H, B, D), m.wg.detach(), m.wu.detach(), m.w2.detach(), gy.expand(H, B, D))
+    want, bounds = gated64(*t, "silu")
+    for name, a, w, (rounded, summed) in zip(NAMES, got, want, bounds):
+        if name in ("o", "dx"):
+            w, rounded, summed = (v.sum(0) for v in (w, rounded, summed))
+        e = excess(a, w / H, (rounded / H, summed * 1.01 / H), dt)  # (1.01: the sum over heads in fp32)
+        assert e <= 1.0, (name, e)
 
 
 def test_gradients_against_differences():

@@ -100,7 +100,8 @@ def test_registered_operator_and_compile():
     (dx,) = torch.autograd.grad(f(x), (x,), do)
     assert torch.equal(f(x), o) and torch.equal(dx, g[0])
     shared = torch.randn(40, 32, dtype=torch.bfloat16, device="cuda")
-    assert torch.equal(f(shared), m(shared))
+    # (compiled, the mean is torch's over the heads' rounded results)
+    assert torch.allclose(f(shared).float(), m(shared).float(), rtol=2.0 ** -6, atol=2.0 ** -6)
 
 
 def test_join_and_norm_under_compile():
