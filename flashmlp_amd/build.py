@@ -26,7 +26,7 @@ BUILD = PKG / "_build"
 LIB = PKG / "libflashmlp.so"
 # fmlp_bwd.hip and fmlp_gated_dw.hip are compiled once per part (file:part): the kernels of one D each, and the rest
 SOURCES = ["fmlp_bwd.hip:64", "fmlp_bwd.hip:128", "fmlp_bwd.hip:0", "fmlp_bwd.hip:32", "fmlp_fwd.hip", "fmlp_f32.hip", "fmlp_gen.hip",
-           "fmlp_gated_fwd.hip", "fmlp_gated_dx.hip", "fmlp_gated_dw.hip:128", "fmlp_gated_dw.hip:0", "fmlp_gated_f32.hip", "fmlp_gated_gen.hip", "fmlp_join.hip", "fmlp_clip.hip", "fmlp_scratch.hip", "fmlp_abi.cpp", "fmlp_block_abi.cpp"]
+           "fmlp_gated_fwd.hip", "fmlp_gated_dx.hip", "fmlp_gated_dw.hip:128", "fmlp_gated_dw.hip:0", "fmlp_gated_f32.hip", "fmlp_gated_util.hip", "fmlp_join.hip", "fmlp_clip.hip", "fmlp_scratch.hip", "fmlp_abi.cpp", "fmlp_block_abi.cpp"]
 PART_MACRO = {"fmlp_bwd.hip": "FMLP_BWD_PART", "fmlp_gated_dw.hip": "FMLP_GATED_DW_PART"}
 # Products that write vector registers: with the compiler's choice (accumulation registers, as the kernel holds more
 # than 256 values) every value the activation takes is copied first. dW at H=32 B=16384 D=128 E=1024 bf16 SiLU 728 us,

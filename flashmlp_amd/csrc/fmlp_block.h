@@ -36,17 +36,12 @@ struct GatedArgs {
 };
 
 // Rows of E elements of both matrices copied to rows of ldw elements (whole 16-byte vectors, zeros behind the
-// last element), one after the other at dst, in one launch (fmlp_gated_gen.hip).
+// last element), one after the other at dst, in one launch (fmlp_gated_util.hip).
 hipError_t launch_gated_pad(const void* wg, const void* wu, void* dst, int64_t rows, int64_t E, int64_t ldw, int es,
                             hipStream_t st);
 
-// dst[i] = scale * sum over H of src[h][i] (n values, a multiple of 4), rounded to io (fmlp_gated_gen.hip).
+// dst[i] = scale * sum over H of src[h][i] (n values, a multiple of 4), rounded to io (fmlp_gated_util.hip).
 hipError_t launch_head_sum(const float* src, void* dst, int64_t n, int64_t H, float scale, int io, hipStream_t st);
-
-// The kernels that read their operands from global memory (fmlp_gated_gen.hip): every io type and D.
-hipError_t launch_gated_gen_fwd(const GatedArgs& a, hipStream_t st);
-hipError_t launch_gated_gen_dx(const GatedArgs& a, hipStream_t st);
-hipError_t launch_gated_gen_dw(const GatedArgs& a, hipStream_t st);
 
 // 16-bit io on LDS-staged kernels (fmlp_gated_fwd.hip). Forms of the row kernels: nw waves of 32 rows in each of es
 // sets that take every chunk of a part of E, ns ring slots a set, oc waves per SIMD; nw = 0: no such form.
@@ -92,7 +87,7 @@ GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cu
 hipError_t launch_gated_dw(const GatedArgs& a, const GatedDwPlan& p, hipStream_t st);
 hipError_t launch_gated_dw128(const GatedArgs& a, const GatedDwPlan& p, hipStream_t st);
 
-// fp32 io at D <= 128 (fmlp_gated_f32.hip): tiles of 128 rows, E-tiles of 128 columns.
+// fp32 io (fmlp_gated_f32.hip): tiles of 128 rows, E-tiles of 128 columns (32 at D = 256).
 GatedFwdPlan gated32_rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus);
 GatedDwPlan gated32_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus);
 hipError_t launch_gated32_fwd(const GatedArgs& a, const GatedFwdPlan& p, hipStream_t st);

@@ -55,9 +55,6 @@ int check_head_stride(int64_t s, const char* name, int64_t H, size_t es) {
   return FMLP_OK;
 }
 
-// fp32 at D = 256 alone runs on the kernels that read operands from global memory, without a workspace
-bool gated_staged(int64_t D, int io) { return io != FMLP_DTYPE_F32 || D <= 128; }
-
 // Wg and Wu where rows of E elements are no whole 16-byte vectors: padded copies at the workspace's start
 size_t gated_pad_bytes(int64_t H, int64_t D, int64_t E, int io) {
   const int es = (int)elem_bytes(io);
@@ -96,7 +93,7 @@ int io_type(int io) { return io == FMLP_DTYPE_F32 ? fmlp::IO_F32 : io == FMLP_DT
 FMLP_EXPORT size_t fmlp_gated_fwd_workspace_bytes(int64_t H, int64_t B, int64_t D, int64_t E, int dtype) {
   int cus = 0;
   dtype &= ~FMLP_OUT_F32;
-  if (check_gated(H, B, D, E, dtype, 0) || !gated_staged(D, dtype) || fmlp::abi_num_cus(&cus)) return 0;
+  if (check_gated(H, B, D, E, dtype, 0) || fmlp::abi_num_cus(&cus)) return 0;
   return gated_pad_bytes(H, D, E, dtype) + rows_plan(H, B, D, E, dtype, cus, false).ws_bytes;
 }
 
@@ -114,7 +111,7 @@ size_t gated_bwd_ws(int64_t H, int64_t B, int64_t D, int64_t E, int dtype, int c
 
 FMLP_EXPORT size_t fmlp_gated_bwd_workspace_bytes(int64_t H, int64_t B, int64_t D, int64_t E, int dtype) {
   int cus = 0;
-  if (check_gated(H, B, D, E, dtype, 0) || !gated_staged(D, io_of(dtype)) || fmlp::abi_num_cus(&cus)) return 0;
+  if (check_gated(H, B, D, E, dtype, 0) || fmlp::abi_num_cus(&cus)) return 0;
   return gated_bwd_ws(H, B, D, E, dtype, cus);
 }
 
@@ -153,15 +150,10 @@ FMLP_EXPORT int fmlp_gated_fwd(const void* x, const void* wg, const void* wu, co
   a.ws_bytes = workspace != nullptr ? workspace_bytes : 0;
   if ((st = fmlp::abi_num_cus(&a.num_cus))) return st;
   const hipStream_t hs = (hipStream_t)stream;
-  hipError_t e;
-  if (!gated_staged(D, dtype)) {
-    e = fmlp::launch_gated_gen_fwd(a, hs);
-  } else {
-    const fmlp::GatedFwdPlan p = rows_plan(H, B, D, E, dtype, a.num_cus, false);
-    if ((st = check_ws(workspace, workspace_bytes, gated_pad_bytes(H, D, E, dtype) + p.ws_bytes))) return st;
-    e = gated_pad(&a, hs);
-    if (e == hipSuccess) e = a.io == fmlp::IO_F32 ? fmlp::launch_gated32_fwd(a, p, hs) : fmlp::launch_gated_fwd(a, p, hs);
-  }
+  const fmlp::GatedFwdPlan p = rows_plan(H, B, D, E, dtype, a.num_cus, false);
+  if ((st = check_ws(workspace, workspace_bytes, gated_pad_bytes(H, D, E, dtype) + p.ws_bytes))) return st;
+  hipError_t e = gated_pad(&a, hs);
+  if (e == hipSuccess) e = a.io == fmlp::IO_F32 ? fmlp::launch_gated32_fwd(a, p, hs) : fmlp::launch_gated_fwd(a, p, hs);
   if (e != hipSuccess) return abi_fail(FMLP_ERR_HIP, "gated forward launch: %s", hipGetErrorString(e));
   return abi_ok();
 }
@@ -209,10 +201,7 @@ FMLP_EXPORT int fmlp_gated_bwd(const void* x, const void* wg, const void* wu, co
   const hipStream_t hs = (hipStream_t)stream;
   const int io = io_of(dtype);
   hipError_t e = hipSuccess;
-  if (!gated_staged(D, io)) {
-    if (want_dw) e = fmlp::launch_gated_gen_dw(a, hs);
-    if (e == hipSuccess && want_dx) e = fmlp::launch_gated_gen_dx(a, hs);
-  } else if (want_dw || want_dx) {
+  if (want_dw || want_dx) {
     if ((st = check_ws(workspace, workspace_bytes, gated_bwd_ws(H, B, D, E, dtype, a.num_cus)))) return st;
     e = gated_pad(&a, hs);
     if (e == hipSuccess && want_dw) {

@@ -1,4 +1,4 @@
-// Gated MLP for gfx950, fp32 io at D <= 128: forward, dX and weight gradients on v_mfma_f32_32x32x2_f32, whose
+// Gated MLP for gfx950, fp32 io: forward, dX and weight gradients on v_mfma_f32_32x32x2_f32, whose
 // 64 clocks per product (16 times a 16-bit one's) are what bounds all three; nothing is rounded before the
 // results. The same shapes as the 16-bit kernels: chunks of E or subtiles of rows in a double buffer in LDS filled
 // by buffer loads, everything else in registers. One LDS read of four bytes a lane feeds a product, so the
@@ -96,6 +96,7 @@ gated32_rows_kernel(const float* __restrict__ X, const float* __restrict__ Wg, c
                     const float* __restrict__ W2, const float* __restrict__ dO, float* __restrict__ out, int B, int E,
                     int ldw, long long sx, long long sdo, int H, int T, int xs, int nct, float* __restrict__ ws) {
   constexpr int KQ = DG / 2, NTN = D / 32, SLOT = 384 * D;
+  constexpr bool TWO = D <= 128;  // two chunks fit the LDS
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int g = lane >> 5, l32 = lane & 31;
   int h, bt, cb = 0, ce = (E + 31) >> 5;
@@ -133,9 +134,13 @@ gated32_rows_kernel(const float* __restrict__ X, const float* __restrict__ Wg, c
 #pragma unroll
   for (int k = 0; k < 8; ++k) row8[k] = off32(2 * k + g, l32);
   for (int c = cb; c < ce; ++c) {
-    const int at = ((c - cb) & 1) * SLOT;
+    const int at = TWO ? ((c - cb) & 1) * SLOT : 0;
+    if (!TWO && c > cb) {
+      barrier_all();
+      ch.load(c, 0);
+    }
     barrier_all();  // chunk c has landed, and chunk c - 1 is read
-    if (c + 1 < ce) ch.load(c + 1, SLOT - at);
+    if (TWO && c + 1 < ce) ch.load(c + 1, SLOT - at);
     f32x16 zg = zero16(), zu = zero16(), dh = zero16();
 #pragma unroll
     for (int q = 0; q < KQ; ++q) {
@@ -143,6 +148,7 @@ gated32_rows_kernel(const float* __restrict__ X, const float* __restrict__ Wg, c
       zg = mma(lds_f32(a), x[q], zg);
       zu = mma(lds_f32(a + 128 * D), x[q], zu);
       if constexpr (BWD) dh = mma(lds_f32(at + 256 * D + offD<D>(l32, 2 * q + g)), d[q], dh);
+      if (D == 256 && (q & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // (reads moved further ahead spill registers)
     }
     if constexpr (!BWD) {
 #pragma unroll
@@ -163,6 +169,7 @@ gated32_rows_kernel(const float* __restrict__ X, const float* __restrict__ Wg, c
           o[n] = mma(dg, lds_f32(a), o[n]);
           o[n] = mma(du, lds_f32(a + 128 * D), o[n]);
         }
+        if (D == 256) __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -179,22 +186,26 @@ gated32_rows_kernel(const float* __restrict__ X, const float* __restrict__ Wg, c
 }
 
 // Weight gradients: four waves of 32 columns of E; X and dO subtiles of 32 rows. W2's columns stay in LDS at
-// D = 128, where three matrices and three gradient tiles do not fit the registers.
+// D = 128, where three matrices and three gradient tiles do not fit the registers. At D = 256 the four waves share
+// 32 columns of E and own a quarter of D each: of the weights, of the contractions over d, whose partial G, U and
+// dH go through LDS and are added in wave order by all, and of the gradients.
 template <int D, int DG, int ACT>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
 gated32_dw_kernel(const float* __restrict__ X, const float* __restrict__ Wg, const float* __restrict__ Wu,
                   const float* __restrict__ W2, const float* __restrict__ dO, float* __restrict__ dWg,
                   float* __restrict__ dWu, float* __restrict__ dW2, int H, int B, int E, int ldw, long long sx,
                   long long sdo, int nE, int nS, int rows_per_split, float scale, float* __restrict__ ws) {
-  constexpr int KQ = DG / 2, NTN = D / 32, SLOT = 256 * D, NP = 8 * D / 256;
-  constexpr bool W2LDS = D > 64;
+  constexpr bool QUARTER = D == 256;
+  constexpr int DW = QUARTER ? 64 : D;  // columns of D of a wave
+  constexpr int KQ = (QUARTER ? DW : DG) / 2, NTN = DW / 32, SLOT = 256 * D, NP = 8 * D / 256;
+  constexpr bool W2LDS = D == 128, TWO = !QUARTER;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int g = lane >> 5, l32 = lane & 31;
   const unsigned t = (unsigned)xcd_remap(blockIdx.x, gridDim.x);
   const int et = (int)(t % (unsigned)nE);
   const unsigned hs = t / (unsigned)nE;
   const int s = (int)(hs % (unsigned)nS), h = (int)(hs / (unsigned)nS);
-  const int e0 = (et * 4 + wave) * 32, e = e0 + l32;
+  const int e0 = (QUARTER ? et : et * 4 + wave) * 32, e = e0 + l32, d0 = QUARTER ? wave * DW : 0;
   const int r0 = s * rows_per_split, r1 = min(B, r0 + rows_per_split), NSUB = max(0, (r1 - r0 + 31) >> 5);
   const float* Xh = X + (size_t)h * sx;
   const float* dOh = dO + (size_t)h * sdo;
@@ -228,27 +239,52 @@ gated32_dw_kernel(const float* __restrict__ X, const float* __restrict__ Wg, con
   float wg[KQ], wu[KQ], w2[W2LDS ? 1 : KQ];
 #pragma unroll
   for (int q = 0; q < KQ; ++q) {
-    const size_t at = ((size_t)h * DG + 2 * q + g) * ldw + e;
+    const int d = d0 + 2 * q + g;
+    const size_t at = ((size_t)h * DG + d) * ldw + e;
     wg[q] = e < E ? Wg[at] : 0.f;
     wu[q] = e < E ? Wu[at] : 0.f;
-    if constexpr (!W2LDS) w2[q] = e < E ? W2[((size_t)h * E + e) * DG + 2 * q + g] : 0.f;
+    if constexpr (!W2LDS) w2[q] = e < E ? W2[((size_t)h * E + e) * DG + d] : 0.f;
   }
   f32x16 ag[NTN], au[NTN], a2[NTN];
 #pragma unroll
   for (int n = 0; n < NTN; ++n) ag[n] = au[n] = a2[n] = zero16();
   for (int i = 0; i < NSUB; ++i) {
-    const int at = (i & 1) * SLOT;
+    const int at = TWO ? (i & 1) * SLOT : 0;
+    if (!TWO && i > 0) {
+      barrier_all();
+      load_sub(i, 0);
+    }
     barrier_all();
-    if (i + 1 < NSUB) load_sub(i + 1, SLOT - at);
+    if (TWO && i + 1 < NSUB) load_sub(i + 1, SLOT - at);
     f32x16 zg = zero16(), zu = zero16(), dh = zero16();
 #pragma unroll
     for (int q = 0; q < KQ; ++q) {
-      const int a = offD<D>(l32, 2 * q + g);
+      const int a = offD<D>(l32, d0 + 2 * q + g);
       const float x = lds_f32(at + a);
       zg = mma(x, wg[q], zg);
       zu = mma(x, wu[q], zu);
       dh = mma(lds_f32(at + 128 * D + a), W2LDS ? lds_f32(2 * SLOT + wave * 128 * D + a) : w2[W2LDS ? 0 : q], dh);
       if (W2LDS && (q & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // (reads moved further ahead spill registers)
+    }
+    if constexpr (QUARTER) {  // the waves' partial sums, [wave][12][lane] of four values behind the subtile
+#pragma unroll
+      for (int k = 0; k < 12; ++k) {
+        const f32x16& v = k < 4 ? zg : k < 8 ? zu : dh;
+        const int j = 4 * (k & 3);
+        lds_write16(SLOT + ((wave * 12 + k) * 64 + lane) * 16, u32x4{__float_as_uint(v[j]), __float_as_uint(v[j + 1]),
+                                                                     __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3])});
+      }
+      barrier_all();
+      zg = zu = dh = zero16();
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int k = 0; k < 12; ++k) {
+          const u32x4 u = lds_read16(SLOT + ((w * 12 + k) * 64 + lane) * 16);
+          f32x16& v = k < 4 ? zg : k < 8 ? zu : dh;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[4 * (k & 3) + j] += __uint_as_float(u[j]);
+        }
     }
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
@@ -257,7 +293,7 @@ gated32_dw_kernel(const float* __restrict__ X, const float* __restrict__ Wg, con
       const float hv = sv * zu[k], dg = dh[k] * f * zu[k], du = dh[k] * sv;
 #pragma unroll
       for (int n = 0; n < NTN; ++n) {
-        const int a = at + offD<D>(crow(k, g), n * 32 + l32);
+        const int a = at + offD<D>(crow(k, g), d0 + n * 32 + l32);
         const float x = lds_f32(a);
         ag[n] = mma(x, dg, ag[n]);
         au[n] = mma(x, du, au[n]);
@@ -278,7 +314,7 @@ gated32_dw_kernel(const float* __restrict__ X, const float* __restrict__ Wg, con
   for (int n = 0; n < NTN; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int r = crow(i, g), c = n * 32;
+      const int r = crow(i, g), c = d0 + n * 32;
       if (e0 + r < E && c + l32 < DG) dW2[((size_t)h * E + e0 + r) * DG + c + l32] = a2[n][i] * scale;
       if (e < E && c + r < DG) {
         const size_t at = ((size_t)h * DG + c + r) * E + e;
@@ -312,7 +348,7 @@ __global__ void __launch_bounds__(256) gated32_dw_reduce(const float* __restrict
 template <int D, int DG, int ACT, bool BWD>
 hipError_t launch_rows(const GatedArgs& a, const GatedFwdPlan& p, hipStream_t st) {
   auto k = gated32_rows_kernel<D, DG, ACT, BWD>;
-  constexpr int lds = 2 * 384 * D;
+  constexpr int lds = (D <= 128 ? 2 : 1) * 384 * D;
   static std::atomic<unsigned long long> done{0};
   hipError_t e = set_lds_once((const void*)k, lds, done);
   if (e != hipSuccess) return e;
@@ -328,7 +364,7 @@ hipError_t launch_rows(const GatedArgs& a, const GatedFwdPlan& p, hipStream_t st
 template <int D, int DG, int ACT>
 hipError_t launch_dw(const GatedArgs& a, const GatedDwPlan& p, hipStream_t st) {
   auto k = gated32_dw_kernel<D, DG, ACT>;
-  constexpr int lds = 512 * D + (D > 64 ? 512 * D : 0);
+  constexpr int lds = D == 256 ? 256 * D + 48 * 1024 : 512 * D + (D == 128 ? 512 * D : 0);
   static std::atomic<unsigned long long> done{0};
   hipError_t e = set_lds_once((const void*)k, lds, done);
   if (e != hipSuccess) return e;
@@ -358,7 +394,8 @@ hipError_t by_d(const GatedArgs& a, F f) {
     case 16: return by_act<32, 16>(a.act, f);
     case 32: return by_act<32, 32>(a.act, f);
     case 64: return by_act<64, 64>(a.act, f);
-    default: return by_act<128, 128>(a.act, f);
+    case 128: return by_act<128, 128>(a.act, f);
+    default: return by_act<256, 256>(a.act, f);
   }
 }
 
@@ -393,9 +430,9 @@ GatedFwdPlan gated32_rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int n
 GatedDwPlan gated32_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus) {
   GatedDwPlan p{};
   const long long N = std::max(num_cus, 1), subs = (B + 31) / 32;
-  p.nE = (int)((E + 127) / 128);
+  p.nE = (int)(D == 256 ? (E + 31) / 32 : (E + 127) / 128);
   const long long base = H * p.nE;
-  const double sub_us = 5.8 * (double)std::max<long long>(D, 32) / 64.0;
+  const double sub_us = D == 256 ? 8.0 : 5.8 * (double)std::max<long long>(D, 32) / 64.0;
   double best = 0;
   p.nS = 1;
   p.rows_per_split = (int)std::max<long long>(subs * 32, 32);
