@@ -15,6 +15,10 @@
 //     G(i+1)     | dG(i), dU(i) packed
 //     gradients of subtile i, U(i+1)  | act, act' of i + 1
 //     dH(i+1)    | h(i+1) packed, U act'
+// H=32 B=16384 D=128 E=1024 bf16 SiLU 694 us, 1189 TFLOP/s executed, products 60 % and vector instructions 50 % of the
+// cycles at 1.87 GHz (one wave a SIMD: they take turns; spreading the activations' stages over the steps, or reading
+// operands further ahead, changed nothing). Weights from LDS instead of registers 767 us at D = 128; at D = 64, where
+// they leave room for two programs a CU, 234 us at H=8 B=16384 E=2048.
 // Rows are split over nS programs where the columns of E alone leave CUs idle; their fp32 partials are added in
 // order by a second launch.
 #include <algorithm>

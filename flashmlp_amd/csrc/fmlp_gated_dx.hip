@@ -12,6 +12,9 @@
 //     G(c+1)               | dG(c), dU(c) from dH, U, act, act' of c
 //     dX += dG Wg^T + ..   | act, act' of c + 1
 //     U(c+1), dH(c+1)      | the rest of them
+// H=32 B=16384 D=128 E=1024 bf16 SiLU 600 us, 1145 TFLOP/s executed, products 61 % and vector instructions 50 % of the
+// SIMDs' cycles at 1.76 GHz. Reading stored dG and dU instead would save its 6 D / 16 recomputed products and the
+// activations at the price of 2.1 GB written and read; the backward's memory stays O(weights) here.
 #include <algorithm>
 #include <type_traits>
 

@@ -13,7 +13,8 @@
 // that need all of them and the results, so that the forward reads o and r and writes r' and y, and the
 // backward reads r', o, dr', dy and writes dr, do. o and y are head-major (H, B, D), the layout of the
 // MLP kernels, or rows of C columns; the transposition costs nothing, a vector of 8 columns lies in one
-// head. Both are bound by HBM bytes; sums are fp32.
+// head. Both are bound by HBM bytes; sums are fp32. 16384 x 4096 bf16: forward 112 us (537 MB, 4.8 TB/s), backward 174
+// (805 MB, 4.6 TB/s) and 6 for the column sums; a copy of 1 GiB reaches 5.0 TB/s. Four rows: 5.9 us a call, all launch.
 #include <algorithm>
 
 #include "fmlp_block.h"
