@@ -7,10 +7,9 @@
 // lane per column of E, which is the operand layout of the gradients' products, so h, dG and dU (rounded to the
 // io type) never leave registers. The four waves of a workgroup share the rows: X and dO subtiles land in an LDS
 // ring by buffer loads, swizzled so that the row reads (operands of G, U, dH) and the transposed reads (operands
-// of the gradients) are both free of bank conflicts. At D = 256 a wave owns half of D, and two waves compute the
-// same h, dG and dU.
+// of the gradients) are both free of bank conflicts. D = 256: gated_dw256_kernel.
 //
-// Bound by matrix and vector issue: a subtile has 6 D / 16 products (at D = 256 per wave 4.5 D / 16) and 16
+// Bound by matrix and vector issue: a subtile has 6 D / 16 products and 16
 // activations with their derivatives a lane. One product and a share of vector work a step:
 //     G(i+1)     | dG(i), dU(i) packed
 //     gradients of subtile i, U(i+1)  | act, act' of i + 1
@@ -30,34 +29,107 @@
 namespace fmlp {
 namespace {
 
-// EW groups of 32 columns, DP parts of D, NS ring slots; WREG: weight matrices held in registers (3; 2: W2 in LDS; 1: Wu
-// too; 0: all in LDS)
+// Waves of a workgroup: EW groups of 32 columns of E times DP parts of D. NS ring slots; OC waves per SIMD; WREG: the
+// weights are held in registers, else in LDS.
 struct Form {
-  int ew, dp, ns, oc, wreg;
+  int ew, dp, ns, oc;
+  bool wreg;
 };
 __host__ __device__ constexpr Form dw_form(int D) {
-  return D == 32 ? Form{4, 1, 4, 2, 3} : D == 64 ? Form{4, 1, 4, 2, 0} : D == 128 ? Form{4, 1, 4, 1, 3} : Form{2, 2, 3, 1, 1};
+  return D == 32 ? Form{4, 1, 4, 2, true} : D == 64 ? Form{4, 1, 4, 2, false} : D == 128 ? Form{4, 1, 4, 1, true} : Form{2, 2, 4, 1, true};
 }
-// LDS: the ring, then the tiles of Wg and Wu (for good where they are read from there; else for the start only, and
-// in the ring's place where they do not fit beside it), then W2's
-__host__ __device__ constexpr int dw_wg_off(int D) {
+// LDS: the ring, then at D <= 128 the tiles of Wg and Wu (for the start only where registers hold them) and W2's (not
+// there), at D = 256 the waves' partial sums
+__host__ __device__ constexpr int dw_lds(int D) {
   const Form f = dw_form(D);
-  return f.wreg == 0 || (f.wreg >= 2 && D <= 128) ? f.ns * 128 * D : 0;
+  return f.ns * 128 * D + (D == 256 ? 4 * 6144 : 128 * D * f.ew + (f.wreg ? 0 : 64 * D * f.ew));
 }
-__host__ __device__ constexpr int dw_wu_off(int D) {
-  const Form f = dw_form(D);
-  return f.wreg == 1 ? f.ns * 128 * D : dw_wg_off(D) + 64 * D * f.ew;
-}
-__host__ __device__ constexpr int dw_w2_off(int D) {
-  const Form f = dw_form(D);
-  return dw_wu_off(D) >= f.ns * 128 * D ? dw_wu_off(D) + 64 * D * f.ew : f.ns * 128 * D;
-}
-__host__ __device__ constexpr int dw_lds(int D) { return dw_w2_off(D) + (dw_form(D).wreg == 3 ? 0 : 64 * D * dw_form(D).ew); }
 
 template <int D>
 __device__ __forceinline__ int swz(int r) {
   if constexpr (D == 32) return (r >> 2) & 3;
   else return (int)swz16<D == 64 ? 64 : 128>((unsigned)r);
+}
+
+// The end of a program: dWg, dWu tiles (lane = row d, values along e) and dW2 tiles (lane = row e, values along d) of a
+// wave's 32 columns e0 .. of E and 32 NTO columns d0 .. of D, as the gradients (every wave has read the ring, whose
+// place they pass through) or as this split's partials.
+template <bool BF16, int DG, int NTO>
+__device__ __forceinline__ void dw_finish(f32x16 (&ag)[NTO], f32x16 (&au)[NTO], f32x16 (&a2)[NTO], void* dWg, void* dWu,
+                                          void* dW2, float* ws, float scale, int H, int E, int nE, int nS, int s, int h,
+                                          int et, int wave, int lane, int e0, int d0) {
+  const int g = lane >> 5, l32 = lane & 31;
+  if (nS > 1) {  // fp32 partials as the accumulators lie: 1 KB per store
+    float4* part = (float4*)ws + ((((size_t)s * H + h) * nE + et) * 4 + wave) * (3 * NTO * 256) + lane;
+#pragma unroll
+    for (int m = 0; m < 3; ++m)
+#pragma unroll
+      for (int n = 0; n < NTO; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x16& t = m == 0 ? ag[n] : m == 1 ? au[n] : a2[n];
+          part[((m * NTO + n) * 4 + q) * 64] = float4{t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3]};
+        }
+    return;
+  }
+#pragma unroll
+  for (int n = 0; n < NTO; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      ag[n][i] *= scale;
+      au[n][i] *= scale;
+      a2[n][i] *= scale;
+    }
+  // through LDS, so that rows leave as whole 16-byte pieces: 2-byte stores from the accumulators' layout took 8 of the
+  // 18 us of a program with one subtile (H=32 B=4 D=128 E=1024)
+  const int area = wave * 2048 * NTO;
+  auto fence = [&]() {  // the area belongs to this wave alone: its own reads and writes in order
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    asm volatile("" ::: "memory");
+  };
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+#pragma unroll
+    for (int n = 0; n < NTO; ++n)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x16& t = m == 0 ? ag[n] : au[n];
+        lds_write8(area + (n * 32 + l32) * 64 + ((q ^ ((l32 >> 2) & 3)) << 4) + g * 8,
+                   u32x2{pack2<BF16>(t[4 * q], t[4 * q + 1]), pack2<BF16>(t[4 * q + 2], t[4 * q + 3])});
+      }
+    fence();
+    u16* out = (u16*)(m == 0 ? dWg : dWu);
+#pragma unroll
+    for (int i = 0; i < 2 * NTO; ++i) {
+      const int p = i * 64 + lane, r = p >> 2, e = e0 + ((p & 3) ^ ((r >> 2) & 3)) * 8;
+      const u32x4 v = lds_read16(area + p * 16);
+      if (d0 + r < DG && e < E) {
+        u16* at = out + ((size_t)h * DG + d0 + r) * E + e;
+        if ((E & 7) == 0) {
+          *(u32x4*)at = v;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (e + j < E) at[j] = (u16)(v[j >> 1] >> (16 * (j & 1)));
+        }
+      }
+    }
+    fence();
+  }
+  constexpr int PW = 4 * NTO;  // pieces of a row of the dW2 tiles
+#pragma unroll
+  for (int n = 0; n < NTO; ++n)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      lds_write8(area + l32 * (PW * 16) + (((n * 4 + q) ^ (l32 & (PW - 1))) << 4) + g * 8,
+                 u32x2{pack2<BF16>(a2[n][4 * q], a2[n][4 * q + 1]), pack2<BF16>(a2[n][4 * q + 2], a2[n][4 * q + 3])});
+  fence();
+#pragma unroll
+  for (int i = 0; i < 2 * NTO; ++i) {
+    const int p = i * 64 + lane, r = p / PW, d = d0 + ((p % PW) ^ (r & (PW - 1))) * 8;
+    const u32x4 v = lds_read16(area + p * 16);
+    if (e0 + r < E && d < DG) *(u32x4*)((u16*)dW2 + ((size_t)h * E + e0 + r) * DG + d) = v;
+  }
 }
 
 template <bool BF16, int D, int DG, int ACT>
@@ -67,22 +139,21 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
                 void* __restrict__ dW2, int H, int B, int E, int ldw, long long sx, long long sdo, int nE, int nS,
                 int rows_per_split, float scale, float* __restrict__ ws) {
   constexpr Form F = dw_form(D);
-  constexpr int EW = F.ew, DP = F.dp, NS = F.ns, PF = NS - 1, WREG = F.wreg;
-  constexpr int KS = DG / 16, NTO = D / 32 / DP, ROWB = 2 * D, PPR = D / 8, SLOT = 128 * D, DOO = 64 * D;
+  constexpr int EW = F.ew, NS = F.ns, PF = NS - 1;
+  constexpr bool WREG = F.wreg;
+  constexpr int KS = DG / 16, NTO = D / 32, ROWB = 2 * D, PPR = D / 8, SLOT = 128 * D, DOO = 64 * D;
   constexpr int NPR = D >= 64 ? D / 64 : 1, NLD = D >= 64 ? 2 * NPR : 1;  // loads a thread for X (and dO)
-  constexpr bool STAGE = dw_wg_off(D) >= NS * SLOT;  // the start's tiles beside the ring
-  constexpr int W2L = dw_w2_off(D);
-  static_assert(EW * DP == 4 && NLD * PF < 64 && 128 * D * EW <= NS * SLOT && dw_lds(D) <= 160 * 1024, "form");
+  constexpr int WL = NS * SLOT, W2L = WL + 128 * D * EW;
+  static_assert(D <= 128 && EW == 4 && NLD * PF < 64 && dw_lds(D) <= 160 * 1024, "form");
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int eg = DP == 1 ? wave : wave & (EW - 1), dp = DP == 1 ? 0 : wave / EW;
   const int G = lane >> 4, i16 = lane & 15, g = lane >> 5, l32 = lane & 31;
 
   const unsigned t = (unsigned)xcd_remap(blockIdx.x, gridDim.x);
   const int et = (int)(t % (unsigned)nE);
   const unsigned hs = t / (unsigned)nE;
   const int s = (int)(hs % (unsigned)nS), h = (int)(hs / (unsigned)nS);
-  const int e0 = (et * EW + eg) * 32;
+  const int e0 = (et * EW + wave) * 32;
   const int r0 = s * rows_per_split, r1 = min(B, r0 + rows_per_split), NSUB = max(0, (r1 - r0 + 31) >> 5);
   const u16* Xh = X + (size_t)h * sx;
   const u16* dOh = dO + (size_t)h * sdo;
@@ -90,10 +161,10 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
   const u16* Wuh = Wu + (size_t)h * DG * ldw;
   const u16* W2h = W2 + (size_t)h * E * DG;
 
-  // ---- weights: this wave's columns of Wg, Wu as [D][32] tiles through LDS (the ring's place, or their own) ----
-  u32x4 wg[WREG ? KS : 1], wu[WREG >= 2 ? KS : 1], w2[WREG == 3 ? KS : 1];
+  // ---- weights: this wave's columns of Wg, Wu as [D][32] tiles through LDS ----
+  u32x4 wg[WREG ? KS : 1], wu[WREG ? KS : 1], w2[WREG ? KS : 1];
   const int laneA = (8 * g + (i16 >> 2)) * 64 + 32 * (G & 1) + 8 * (i16 & 3);
-  const int wt[2] = {dw_wg_off(D) + eg * 64 * D, dw_wu_off(D) + eg * 64 * D};
+  const int wt[2] = {WL + wave * 64 * D, WL + 64 * D * EW + wave * 64 * D};
   auto opWt = [&](int m, int k) {
     const int a = wt[m] + laneA + k * 1024;
     return cat(lds_read_tr(a), lds_read_tr(a + 256));
@@ -102,14 +173,13 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
     const int lim = E - e0, rem = clamp0(DG * ldw * 2 - 2 * e0, 0x7fffffff);
     const i32x4 rg = make_rsrc_words(Wgh + e0, rem), ru = make_rsrc_words(Wuh + e0, rem);
 #pragma unroll
-    for (int i = 0; i < D / 16 / DP; ++i) {
-      const int k = i * DP + dp;
+    for (int k = 0; k < D / 16; ++k) {
       const unsigned p = (unsigned)(k * 64 + lane), q = (p & 3u) * 8u;
       const unsigned o = (int)q < lim && (p >> 2) < (unsigned)DG ? (p >> 2) * (unsigned)ldw * 2u + q * 2u : BUF_OOB;
       buf_load16_lds(rg, o, wt[0] + k * 1024);
       buf_load16_lds(ru, o, wt[1] + k * 1024);
     }
-    if constexpr (WREG == 3) {
+    if constexpr (WREG) {
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         w2[k] = u32x4{0u, 0u, 0u, 0u};
@@ -159,18 +229,13 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
 #pragma unroll
     for (int i = 0; i < PF; ++i) load_sub(i, i);
   };
-  if constexpr (STAGE) load_first();
-  if constexpr (WREG > 0) {
-    wait_vmcnt<STAGE ? NLD * PF : 0>();  // the weights' tiles
-    barrier();
+  load_first();
+  if constexpr (WREG) {
+    wait_vmcnt<NLD * PF>();  // the weights' tiles (a wave's own)
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       wg[k] = opWt(0, k);
-      if constexpr (WREG >= 2) wu[k] = opWt(1, k);
-    }
-    if constexpr (!STAGE) {
-      barrier();  // before the ring's loads land on the tiles
-      load_first();
+      wu[k] = opWt(1, k);
     }
   }
   // row reads (row l32, columns 16 k + 8 g ..) and transposed reads (rows 16 s + 8 r + 4 g + i16 / 4, columns
@@ -182,7 +247,7 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
   for (int n = 0; n < NTO; ++n)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int row = 8 * r + 4 * g + (i16 >> 2), q = 4 * (dp * NTO + n) + 2 * (G & 1) + ((i16 & 3) >> 1);
+      const int row = 8 * r + 4 * g + (i16 >> 2), q = 4 * n + 2 * (G & 1) + ((i16 & 3) >> 1);
       to[n][r] = row * ROWB + ((q ^ swz<D>(row)) << 4) + ((i16 & 1) << 3);
     }
   auto opRow = [&](int base, int k) { return lds_read16(base + ro[k]); };
@@ -191,12 +256,8 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
     return cat(lds_read_tr(a + to[n][0]), lds_read_tr(a + to[n][1]));
   };
   auto weight = [&](int m, int k) -> u32x4 {
-    if constexpr (WREG == 3) return m == 0 ? wg[k] : m == 1 ? wu[k] : w2[k];
-    if (m == 2) return lds_read16(W2L + eg * 32 * ROWB + ro[k]);
-    if constexpr (WREG == 2) return m == 0 ? wg[k] : wu[k];
-    if constexpr (WREG == 1)
-      if (m == 0) return wg[k];
-    return opWt(m, k);
+    if constexpr (WREG) return m == 0 ? wg[k] : m == 1 ? wu[k] : w2[k];
+    return m == 2 ? lds_read16(W2L + wave * 32 * ROWB + ro[k]) : opWt(m, k);
   };
 
   f32x16 ag[NTO], au[NTO], a2[NTO], zg, zu, dh;
@@ -244,17 +305,17 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
         Op op;
         if constexpr (i < 0) {
           op.a = opRow(b1, j);
-          if constexpr (WREG == 0) op.w = weight(0, j);
+          if constexpr (!WREG) op.w = weight(0, j);
         } else if constexpr (i2 < 0) {
           constexpr int m = i % 3, n = i / 3 % NTO, s2 = i / 3 / NTO;
           if constexpr (m == 0) op.a = opCol(b2, s2, n);
           if constexpr (m == 2) op.a = opCol(b2 + DOO, s2, n);
         } else if constexpr (i3 < 0) {
           op.a = opRow(b1, i2);
-          if constexpr (WREG < 2) op.w = weight(1, i2);
+          if constexpr (!WREG) op.w = weight(1, i2);
         } else {
           op.a = opRow(b1 + DOO, i3);
-          if constexpr (WREG != 3) op.w = weight(2, i3);
+          if constexpr (!WREG) op.w = weight(2, i3);
         }
         return op;
       };
@@ -286,9 +347,9 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
             a2[n] = mfma<BF16>(op.a, ph[s2], a2[n]);
           }
         } else if constexpr (i3 < 0) {
-          zu = mfma<BF16>(op.a, WREG >= 2 ? wu[WREG >= 2 ? i2 : 0] : op.w, i2 == 0 ? zero16() : zu);
+          zu = mfma<BF16>(op.a, WREG ? wu[WREG ? i2 : 0] : op.w, i2 == 0 ? zero16() : zu);
         } else {
-          dh = mfma<BF16>(op.a, WREG == 3 ? w2[WREG == 3 ? i3 : 0] : op.w, i3 == 0 ? zero16() : dh);
+          dh = mfma<BF16>(op.a, WREG ? w2[WREG ? i3 : 0] : op.w, i3 == 0 ? zero16() : dh);
 #pragma unroll
           for (int e = 16 * i3 / N1; e < 16 * (i3 + 1) / N1; ++e) make_h(e);
         }
@@ -304,89 +365,269 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
     for (int i = 0; i + 1 < NSUB; ++i) {
       const int nxt = cur + 1 == NS ? 0 : cur + 1, far = cur == 0 ? NS - 1 : cur - 1;
       load_sub(i + PF, far);
-      if (D == 256 || e0 < E) iter(std::true_type{}, cur, nxt);  // a wave past the last column only loads (D = 256: spills)
+      if (e0 < E) iter(std::true_type{}, cur, nxt);  // a wave past the last column only loads
       wait_vmcnt<NLD*(PF - 2)>();  // subtile i + 2
       barrier();
       cur = nxt;
     }
-    if (D == 256 || e0 < E) iter(std::false_type{}, cur, cur);
+    if (e0 < E) iter(std::false_type{}, cur, cur);
   }
   wait_vmcnt<0>();  // subtiles past the last are still landing, as zeros
 
-  // ---- dWg, dWu tiles: lane = row d, values along e; dW2 tiles: lane = row e, values along d ----
-  const int d0 = dp * NTO * 32;
-  if (nS > 1) {  // fp32 partials as the accumulators lie: 1 KB per store
-    float4* part = (float4*)ws + ((((size_t)s * H + h) * nE + et) * 4 + wave) * (3 * NTO * 256) + lane;
-#pragma unroll
-    for (int m = 0; m < 3; ++m)
-#pragma unroll
-      for (int n = 0; n < NTO; ++n)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x16& t = m == 0 ? ag[n] : m == 1 ? au[n] : a2[n];
-          part[((m * NTO + n) * 4 + q) * 64] = float4{t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3]};
-        }
-    return;
-  }
-#pragma unroll
-  for (int n = 0; n < NTO; ++n)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      ag[n][i] *= scale;
-      au[n][i] *= scale;
-      a2[n][i] *= scale;
-    }
-  // through LDS, so that rows leave as whole 16-byte pieces: 2-byte stores from the accumulators' layout took 8 of the
-  // 18 us of a program with one subtile (H=32 B=4 D=128 E=1024)
-  barrier();  // the ring is read
-  const int area = wave * 2048 * NTO;
-  auto fence = [&]() {  // the area belongs to this wave alone: its own reads and writes in order
+  if (nS == 1) barrier();  // the ring is read
+  dw_finish<BF16, DG, NTO>(ag, au, a2, dWg, dWu, dW2, ws, scale, H, E, nE, nS, s, h, et, wave, lane, e0, 0);
+}
+
+// D = 256: a wave owns 32 columns of E and half of D: of the weights (in registers), of the contractions over d and of
+// the gradients. The two waves of a column group share a subtile's sums and activations: each gives the other its half
+// sums of 16 rows, activates the 16 rows it keeps (rows are read in such an order that these are the low half of its
+// accumulators), and hands back h, dG and dU. One step of the loop:
+//     half sums of i + 1        | act, act', h, dG, dU of this wave's rows of i, stored for the other wave
+//     barrier 1                 | (all have left subtile i - 1: i + 3 is loaded in its place)
+//     gradients of i, own rows  | the other wave's h, dG, dU read, half sums of i + 1 stored
+//     barrier 2                 | (i + 2 is there)
+//     gradients of i, its rows  | half sums of i + 1 read and added
+// H=8 B=8192 E=1024 bf16 SiLU 228 us (903 TFLOP/s of 12 u); both waves summing over all of D 290, all sums exchanged and
+// both activating 283, an element's activation in one step 241; operands read 3 to 8 steps ahead within 1 %. A subtile
+// takes about 1.6 us, of which its 48 products are 0.85.
+template <bool BF16, int ACT>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
+gated_dw256_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16* __restrict__ Wu,
+                   const u16* __restrict__ W2, const u16* __restrict__ dO, void* __restrict__ dWg, void* __restrict__ dWu,
+                   void* __restrict__ dW2, int H, int B, int E, int ldw, long long sx, long long sdo, int nE, int nS,
+                   int rows_per_split, float scale, float* __restrict__ ws) {
+  constexpr int D = 256, DH = 128, KS = DH / 16, NTO = DH / 32, ROWB = 2 * D, PPR = D / 8, SLOT = 128 * D, DOO = 64 * D;
+  constexpr int NS = dw_form(D).ns, NPR = D / 64, NLD = 2 * NPR, EX = NS * SLOT;
+  static_assert(NS == 4, "the loop's waits");
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), eg = wave & 1, dp = wave >> 1;
+  const int G = lane >> 4, i16 = lane & 15, g = lane >> 5, l32 = lane & 31;
+  const unsigned t = (unsigned)xcd_remap(blockIdx.x, gridDim.x);
+  const int et = (int)(t % (unsigned)nE);
+  const unsigned hs = t / (unsigned)nE;
+  const int s = (int)(hs % (unsigned)nS), h = (int)(hs / (unsigned)nS);
+  const int e0 = (et * 2 + eg) * 32, d0 = dp * DH;
+  const int r0 = s * rows_per_split, r1 = min(B, r0 + rows_per_split), NSUB = max(0, (r1 - r0 + 31) >> 5);
+  const u16* Xh = X + (size_t)h * sx;
+  const u16* dOh = dO + (size_t)h * sdo;
+  auto barrier = [&]() {
     __builtin_amdgcn_s_waitcnt(0xC07F);
     asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   };
+
+  // ---- weights: rows d0 .. of Wg, Wu as [128][32] tiles of this wave's own in the ring's place ----
+  u32x4 wg[KS], wu[KS], w2[KS];
+  {
+    const int lim = E - e0, rem = clamp0((D - d0) * ldw * 2 - 2 * e0, 0x7fffffff), at = wave * 16384;
+    const size_t base = ((size_t)h * D + d0) * ldw + e0;
+    const i32x4 rg = make_rsrc_words(Wg + base, rem), ru = make_rsrc_words(Wu + base, rem);
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-#pragma unroll
-    for (int n = 0; n < NTO; ++n)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x16& t = m == 0 ? ag[n] : au[n];
-        lds_write8(area + (n * 32 + l32) * 64 + ((q ^ ((l32 >> 2) & 3)) << 4) + g * 8,
-                   u32x2{pack2<BF16>(t[4 * q], t[4 * q + 1]), pack2<BF16>(t[4 * q + 2], t[4 * q + 3])});
-      }
-    fence();
-    u16* out = (u16*)(m == 0 ? dWg : dWu);
-#pragma unroll
-    for (int i = 0; i < 2 * NTO; ++i) {
-      const int p = i * 64 + lane, r = p >> 2, e = e0 + ((p & 3) ^ ((r >> 2) & 3)) * 8;
-      const u32x4 v = lds_read16(area + p * 16);
-      if (d0 + r < DG && e < E) {
-        u16* at = out + ((size_t)h * DG + d0 + r) * E + e;
-        if ((E & 7) == 0) {
-          *(u32x4*)at = v;
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (e + j < E) at[j] = (u16)(v[j >> 1] >> (16 * (j & 1)));
-        }
-      }
+    for (int k = 0; k < KS; ++k) {
+      const unsigned p = (unsigned)(k * 64 + lane), q = (p & 3u) * 8u;
+      const unsigned o = (int)q < lim ? (p >> 2) * (unsigned)ldw * 2u + q * 2u : BUF_OOB;
+      buf_load16_lds(rg, o, at + k * 1024);
+      buf_load16_lds(ru, o, at + 8192 + k * 1024);
     }
-    fence();
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      w2[k] = u32x4{0u, 0u, 0u, 0u};
+      if (e0 + l32 < E) w2[k] = *(const u32x4*)(W2 + ((size_t)h * E + e0 + l32) * D + d0 + k * 16 + g * 8);
+    }
+    wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    const int a = at + (8 * g + (i16 >> 2)) * 64 + 32 * (G & 1) + 8 * (i16 & 3);
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      wg[k] = cat(lds_read_tr(a + k * 1024), lds_read_tr(a + k * 1024 + 256));
+      wu[k] = cat(lds_read_tr(a + 8192 + k * 1024), lds_read_tr(a + 8192 + k * 1024 + 256));
+    }
+    barrier();  // before the ring's loads land on the tiles
   }
-  constexpr int PW = 4 * NTO;  // pieces of a row of the dW2 tiles
+
+  unsigned so[NPR];
+#pragma unroll
+  for (int k = 0; k < NPR; ++k) {
+    const int p = k * 256 + tid, r = p / PPR, q = (p % PPR) ^ swz<D>(r);
+    so[k] = (unsigned)(r * D * 2 + q * 16);
+  }
+  auto load_piece = [&](int i, int slot, int k) {  // k = 0 .. NLD - 1
+    const int b = r0 + 32 * i, n = clamp0(r1 - b, 32) * D * 2;
+    buf_load16_lds(make_rsrc_words((k & 1 ? dOh : Xh) + (size_t)b * D, n), so[k >> 1],
+                   slot * SLOT + wave * 1024 + (k & 1) * DOO + (k >> 1) * 4096);
+  };
+  auto load_sub = [&](int i, int slot) {
+#pragma unroll
+    for (int k = 0; k < NLD; ++k) load_piece(i, slot, k);
+  };
+  load_sub(0, 0);
+  load_sub(1, 1);
+  load_sub(2, 2);
+  int ro[KS], to[NTO][2];
+  const int row = l32 ^ (16 * dp);  // own rows first
+#pragma unroll
+  for (int k = 0; k < KS; ++k) ro[k] = row * ROWB + (((2 * (dp * KS + k) + g) ^ swz<D>(row)) << 4);
 #pragma unroll
   for (int n = 0; n < NTO; ++n)
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      lds_write8(area + l32 * (PW * 16) + (((n * 4 + q) ^ (l32 & (PW - 1))) << 4) + g * 8,
-                 u32x2{pack2<BF16>(a2[n][4 * q], a2[n][4 * q + 1]), pack2<BF16>(a2[n][4 * q + 2], a2[n][4 * q + 3])});
-  fence();
+    for (int r = 0; r < 2; ++r) {
+      const int rr = 8 * r + 4 * g + (i16 >> 2), q = 4 * (dp * NTO + n) + 2 * (G & 1) + ((i16 & 3) >> 1);
+      to[n][r] = rr * ROWB + ((q ^ swz<D>(rr)) << 4) + ((i16 & 1) << 3);
+    }
+  const int own = dp * 16 * ROWB, its = 16 * ROWB - own;
+  auto opCol = [&](int a, int n) { return cat(lds_read_tr(a + to[n][0]), lds_read_tr(a + to[n][1])); };
+
+  // A wave's 6 KB: its half sums for the other wave, which puts the other's h, dG and dU there once it has read them
+  const int mine = EX + wave * 6144 + lane * 16, other = EX + (wave ^ 2) * 6144 + lane * 16;
+  f32x16 ag[NTO], au[NTO], a2[NTO], y[3];  // y: half sums of G, U, dH
+  float z[3][8];                           // G, U, dH of the own rows
+  u32x4 po[3], pi[3];                      // h, dG, dU of the own rows and of the other wave's
 #pragma unroll
-  for (int i = 0; i < 2 * NTO; ++i) {
-    const int p = i * 64 + lane, r = p / PW, d = d0 + ((p % PW) ^ (r & (PW - 1))) * 8;
-    const u32x4 v = lds_read16(area + p * 16);
-    if (e0 + r < E && d < DG) *(u32x4*)((u16*)dW2 + ((size_t)h * E + e0 + r) * DG + d) = v;
+  for (int n = 0; n < NTO; ++n) ag[n] = au[n] = a2[n] = zero16();
+  auto give = [&](int k) {  // k = 0 .. 5
+    const f32x16& u = y[k >> 1];
+    const int j = 8 + 4 * (k & 1);
+    lds_write16(mine + k * 1024, u32x4{__float_as_uint(u[j]), __float_as_uint(u[j + 1]), __float_as_uint(u[j + 2]),
+                                       __float_as_uint(u[j + 3])});
+  };
+  auto add = [&](int k, u32x4 u) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) z[k >> 1][4 * (k & 1) + j] = y[k >> 1][4 * (k & 1) + j] + __uint_as_float(u[j]);
+  };
+  float ez, sv, fv, hv, gv, uv;  // an element between its thirds; an even one's h, dG and dU until the odd one's are there
+  auto element = [&](int e, int third) {
+    constexpr bool S = ACT == ACT_SILU || ACT == ACT_SIGMOID;
+    if (third == 0) {
+      if constexpr (S) ez = 1.0f + __builtin_amdgcn_exp2f(z[0][e] * -1.4426950408889634f);
+    } else if (third == 1) {
+      if constexpr (S) {  // act_hf in two parts
+        const float s = __builtin_amdgcn_rcpf(ez);
+        sv = ACT == ACT_SILU ? z[0][e] * s : s;
+        fv = ACT == ACT_SILU ? __builtin_fmaf(sv, 1.0f - s, s) : s - s * s;
+      } else {
+        act_hf<ACT>(z[0][e], sv, fv);
+      }
+    } else {
+      const float a = sv * z[1][e], b = z[2][e] * (fv * z[1][e]), c = z[2][e] * sv;
+      if (e & 1) {
+        po[0][e >> 1] = pack2<BF16>(hv, a);
+        po[1][e >> 1] = pack2<BF16>(gv, b);
+        po[2][e >> 1] = pack2<BF16>(uv, c);
+      } else {
+        hv = a;
+        gv = b;
+        uv = c;
+      }
+    }
+  };
+  auto give_packs = [&]() {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) lds_write16(other + k * 1024, po[k]);
+  };
+  // subtile sub in slot cur, the next in slot nxt (M: there is such a subtile)
+  auto iter = [&](auto MORE, int sub, int cur, int nxt) {
+    constexpr bool M = decltype(MORE)::value;
+    constexpr int N1 = M ? 3 * KS : 0, N2 = 3 * NTO, NOPS = N1 + 2 * N2;
+    constexpr int B1 = N1 + 3, B2 = N1 + N2 + 3;  // steps that the barriers stand before
+    const int b1 = nxt * SLOT, b2 = cur * SLOT;
+    auto fetch = [&](auto J) -> u32x4 {
+      constexpr int j = decltype(J)::value;
+      if constexpr (j < N1) {
+        if constexpr (j % 3 == 0) return lds_read16(b1 + ro[j / 3]);
+        else if constexpr (j % 3 == 2) return lds_read16(b1 + DOO + ro[j / 3]);
+        else return u32x4{0u, 0u, 0u, 0u};
+      } else {
+        constexpr int i = j - N1, m = i % 3, n = i / 3 % NTO;
+        const int a = b2 + (i < N2 ? own : its);
+        if constexpr (m == 0) return opCol(a, n);
+        else if constexpr (m == 2) return opCol(a + DOO, n);
+        else return u32x4{0u, 0u, 0u, 0u};
+      }
+    };
+    constexpr int PD = 4;
+    u32x4 ring[PD + 1], xt, sums[6];
+    static_for<PD>([&](auto J) { ring[J] = fetch(J); });
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (!M) {
+#pragma unroll
+      for (int e = 0; e < 24; ++e) element(e / 3, e % 3);
+      give_packs();
+    }
+    static_for<NOPS>([&](auto J) {
+      constexpr int j = decltype(J)::value;
+      if constexpr (M && j == N1) give_packs();
+      if constexpr (j == B1) {
+        barrier();
+#pragma unroll
+        for (int k = 0; k < 3; ++k) pi[k] = lds_read16(mine + k * 1024);
+      }
+      if constexpr (M && j == B2) {
+        wait_vmcnt<NLD>();  // subtile sub + 2
+        barrier();
+      }
+      const u32x4 op = ring[j % (PD + 1)];
+      if constexpr (j + PD < NOPS) ring[(j + PD) % (PD + 1)] = fetch(std::integral_constant<int, j + PD>{});
+      if constexpr (j < N1) {
+        constexpr int c = j % 3, k = j / 3;
+        if constexpr (c == 0) xt = op;
+        y[c] = mfma<BF16>(c == 1 ? xt : op, c == 0 ? wg[k] : c == 1 ? wu[k] : w2[k], k == 0 ? zero16() : y[c]);
+        element(j / 3, j % 3);
+      } else {
+        constexpr int i = j - N1, m = i % 3, n = i / 3 % NTO, half = i / N2;
+        const u32x4(&p)[3] = half ? pi : po;
+        if constexpr (m == 0) {
+          xt = op;
+          ag[n] = mfma<BF16>(p[1], xt, ag[n]);
+        } else if constexpr (m == 1) {
+          au[n] = mfma<BF16>(p[2], xt, au[n]);
+        } else {
+          a2[n] = mfma<BF16>(op, p[0], a2[n]);
+        }
+        if constexpr (M && j > B1 && j <= B1 + 6) give(j - B1 - 1);
+        if constexpr (M && j >= B1 && j < B1 + NLD) load_piece(sub + 3, (cur + NS - 1) & (NS - 1), j - B1);
+        if constexpr (M && j >= B2 && j < B2 + 3) {
+          sums[2 * (j - B2)] = lds_read16(other + (2 * (j - B2)) * 1024);
+          sums[2 * (j - B2) + 1] = lds_read16(other + (2 * (j - B2) + 1) * 1024);
+        }
+        if constexpr (M && j >= NOPS - 3) {
+          add(2 * (j - NOPS + 3), sums[2 * (j - NOPS + 3)]);
+          add(2 * (j - NOPS + 3) + 1, sums[2 * (j - NOPS + 3) + 1]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+
+  if (NSUB > 0) {
+    wait_vmcnt<2 * NLD>();  // subtile 0
+    barrier();
+#pragma unroll
+    for (int c = 0; c < 3; ++c) y[c] = zero16();
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const u32x4 x = lds_read16(ro[k]);
+      y[0] = mfma<BF16>(x, wg[k], y[0]);
+      y[1] = mfma<BF16>(x, wu[k], y[1]);
+      y[2] = mfma<BF16>(lds_read16(DOO + ro[k]), w2[k], y[2]);
+    }
+#pragma unroll
+    for (int k = 0; k < 6; ++k) give(k);
+    wait_vmcnt<NLD>();  // subtile 1
+    barrier();
+#pragma unroll
+    for (int k = 0; k < 6; ++k) add(k, lds_read16(other + k * 1024));
+    int cur = 0;
+    for (int i = 0; i + 1 < NSUB; ++i) {
+      const int nxt = (cur + 1) & (NS - 1);
+      iter(std::true_type{}, i, cur, nxt);
+      cur = nxt;
+    }
+    iter(std::false_type{}, 0, cur, cur);
   }
+  wait_vmcnt<0>();  // subtiles past the last are still landing, as zeros
+  if (nS == 1) barrier();  // the ring is read
+  dw_finish<BF16, D, NTO>(ag, au, a2, dWg, dWu, dW2, ws, scale, H, E, nE, nS, s, h, et, wave, lane, e0, d0);
 }
 
 // Sum of the row splits' partials in order: four values of one accumulator a thread, along a row of the gradient.
@@ -443,7 +684,10 @@ struct Args {
 
 template <bool BF16, int D, int DG, int ACT>
 hipError_t launch(const Args& q) {
-  auto k = gated_dw_kernel<BF16, D, DG, ACT>;
+  const auto k = [] {
+    if constexpr (D == 256) return gated_dw256_kernel<BF16, ACT>;
+    else return gated_dw_kernel<BF16, D, DG, ACT>;
+  }();
   constexpr int lds = dw_lds(D);
   static std::atomic<unsigned long long> done{0};
   hipError_t e = set_lds_once((const void*)k, lds, done);

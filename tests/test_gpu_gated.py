@@ -55,6 +55,33 @@ def test_forward_and_gradients(H, B, D, E, dt, act):
     check(both(*t, act), t, act)
 
 
+LARGE_CASES = [
+    # many heads of one to a few tiles: more workgroups than run at once, the larger row tiles of every D
+    (200, 70, 32, 64, BF, "silu"), (1200, 40, 32, 100, HF, "sigmoid"), (300, 100, 64, 64, HF, "silu"),
+    (800, 130, 64, 32, BF, "leaky_relu"), (300, 200, 128, 64, BF, "silu"), (260, 250, 128, 93, HF, ""),
+    (520, 120, 128, 64, BF, "silu"), (600, 40, 256, 64, BF, "silu"), (300, 130, 256, 40, HF, "leaky_relu"),
+    # few heads of many rows: the weight gradients' rows are split, down to one subtile of 32 rows in the last range
+    (2, 9000, 32, 64, BF, "silu"), (1, 20000, 64, 72, HF, "silu"), (1, 9000, 128, 100, BF, "sigmoid"),
+    (1, 6000, 256, 72, BF, "silu"), (1, 6049, 256, 33, HF, ""), (1, 700, 256, 130, BF, "silu"),
+    (2, 9000, 32, 64, FL, "silu"), (1, 9000, 128, 100, FL, "silu"), (1, 6000, 256, 72, FL, "sigmoid"),
+    (400, 40, 64, 36, FL, "silu"),
+]
+
+
+@pytest.mark.parametrize("H,B,D,E,dt,act", LARGE_CASES)
+def test_many_workgroups(H, B, D, E, dt, act):
+    print(f"[gated] H={H} B={B} D={D} E={E} {dt} act='{act}'", flush=True)
+    t = make(H, B, D, E, dt, seed=B + E)
+    check(both(*t, act), t, act)
+
+
+@pytest.mark.parametrize("B", [1, 32, 33, 64, 65, 96, 97, 128, 129, 160, 224])
+def test_weight_gradients_over_few_subtiles(B):
+    """Every fill of the ring of row subtiles at D = 256, where two waves share a subtile's sums."""
+    t = make(2, B, 256, 70, BF, seed=B)
+    check(both(*t, "silu"), t, "silu")
+
+
 @pytest.mark.parametrize("D", [16, 64, 128, 256])
 def test_no_rows(D):
     t = make(2, 0, D, 40, BF)
