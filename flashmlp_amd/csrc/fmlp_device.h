@@ -160,6 +160,27 @@ __device__ __forceinline__ void act_hf(float z, float& h, float& f) {
   }
 }
 
+// act_hf in two parts, for steps that stand between products: the denominator of the sigmoid, then the rest
+template <int ACT>
+__device__ __forceinline__ float act_den(float z) {
+  if constexpr (ACT == ACT_SILU || ACT == ACT_SIGMOID) return 1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f);
+  else return z;
+}
+template <int ACT>
+__device__ __forceinline__ void act_hf_den(float z, float den, float& h, float& f) {
+  if constexpr (ACT == ACT_SILU) {
+    const float s = __builtin_amdgcn_rcpf(den);
+    h = z * s;
+    f = __builtin_fmaf(h, 1.0f - s, s);
+  } else if constexpr (ACT == ACT_SIGMOID) {
+    const float s = __builtin_amdgcn_rcpf(den);
+    h = s;
+    f = s - s * s;
+  } else {
+    act_hf<ACT>(z, h, f);
+  }
+}
+
 // act'(z) alone
 template <int ACT>
 __device__ __forceinline__ float act_d(float z) {

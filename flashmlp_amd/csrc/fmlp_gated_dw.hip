@@ -388,8 +388,8 @@ gated_dw_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16
 //     barrier 2                 | (i + 2 is there)
 //     gradients of i, its rows  | half sums of i + 1 read and added
 // H=8 B=8192 E=1024 bf16 SiLU 228 us (903 TFLOP/s of 12 u); both waves summing over all of D 290, all sums exchanged and
-// both activating 283, an element's activation in one step 241; operands read 3 to 8 steps ahead within 1 %. A subtile
-// takes about 1.6 us, of which its 48 products are 0.85.
+// both activating 283, a subtile's loads in one burst and an element's activation in one step 241 (the latter alone 2 %);
+// operands read 3 to 8 steps ahead within 1 %. A subtile takes about 1.6 us, of which its 48 products are 0.85.
 template <bool BF16, int ACT>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
 gated_dw256_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u16* __restrict__ Wu,
@@ -497,17 +497,10 @@ gated_dw256_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const 
   };
   float ez, sv, fv, hv, gv, uv;  // an element between its thirds; an even one's h, dG and dU until the odd one's are there
   auto element = [&](int e, int third) {
-    constexpr bool S = ACT == ACT_SILU || ACT == ACT_SIGMOID;
     if (third == 0) {
-      if constexpr (S) ez = 1.0f + __builtin_amdgcn_exp2f(z[0][e] * -1.4426950408889634f);
+      ez = act_den<ACT>(z[0][e]);
     } else if (third == 1) {
-      if constexpr (S) {  // act_hf in two parts
-        const float s = __builtin_amdgcn_rcpf(ez);
-        sv = ACT == ACT_SILU ? z[0][e] * s : s;
-        fv = ACT == ACT_SILU ? __builtin_fmaf(sv, 1.0f - s, s) : s - s * s;
-      } else {
-        act_hf<ACT>(z[0][e], sv, fv);
-      }
+      act_hf_den<ACT>(z[0][e], ez, sv, fv);
     } else {
       const float a = sv * z[1][e], b = z[2][e] * (fv * z[1][e]), c = z[2][e] * sv;
       if (e & 1) {

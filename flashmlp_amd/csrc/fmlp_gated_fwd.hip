@@ -40,6 +40,9 @@ gated_fwd_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u1
                  int xs, int nct, int outf32, float* __restrict__ ws) {
   constexpr int NT = NW * 64, KS = DG / 16, NTN = D / 32, NPR = 4 * D / NT, NLD = 3 * NPR;
   constexpr int SLOT = 192 * D, WU = 64 * D, W2O = 128 * D, PF = NS - 1;
+  // D = 256 runs lone waves: a chunk's loads stand one by one between products, which hides their address work
+  // (H=8 B=8192 E=1024 bf16 122 -> 119 us); short chunks lose by the later issue (D = 32, a wave alone: 6.1 -> 6.8 us)
+  constexpr bool SPREAD = D == 256;
   static_assert(NPR * NT == 4 * D && NS >= 3 && NLD * (PF - 2) < 64, "chunk loads");
   const int lane = threadIdx.x & 63;
   const int part = ES == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / NT);
@@ -84,20 +87,26 @@ gated_fwd_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u1
       if ((p & 3u) * 8u >= (unsigned)DG) o2[k] = BUF_OOB;
     }
   }
-  auto load_chunk = [&](int c, int slot) {
+  struct Dst {
+    i32x4 r[3];
+    int lim, at;
+  };
+  auto chunk_at = [&](int c, int slot) {
     const int cg = c0 + c, lim = e_end - cg * 32;
     const int rem = clamp0(DG * ldw * 2 - 64 * cg, 0x7fffffff);
-    const i32x4 rg = make_rsrc_words(Wgh + (size_t)cg * 32, rem);
-    const i32x4 ru = make_rsrc_words(Wuh + (size_t)cg * 32, rem);
-    const i32x4 r2 = make_rsrc_words(W2h + (size_t)cg * 32 * DG, clamp0(lim, 32) * DG * 2);
-    const int at = RB + slot * SLOT + wave * 1024;
+    return Dst{{make_rsrc_words(Wgh + (size_t)cg * 32, rem), make_rsrc_words(Wuh + (size_t)cg * 32, rem),
+                make_rsrc_words(W2h + (size_t)cg * 32 * DG, clamp0(lim, 32) * DG * 2)},
+               lim,
+               RB + slot * SLOT + wave * 1024};
+  };
+  auto load_piece = [&](const Dst& d, int q) {
+    const int k = q / 3, m = q % 3;
+    buf_load16_lds(d.r[m], m == 2 ? o2[k] : colq[k] < d.lim ? o1[k] : BUF_OOB, d.at + m * WU + k * NT * 16);
+  };
+  auto load_chunk = [&](int c, int slot) {
+    const Dst d = chunk_at(c, slot);
 #pragma unroll
-    for (int k = 0; k < NPR; ++k) {
-      const unsigned o = colq[k] < lim ? o1[k] : BUF_OOB;
-      buf_load16_lds(rg, o, at + k * NT * 16);
-      buf_load16_lds(ru, o, at + WU + k * NT * 16);
-      buf_load16_lds(r2, o2[k], at + W2O + k * NT * 16);
-    }
+    for (int q = 0; q < NLD; ++q) load_piece(d, q);
   };
   // at most N of this wave's loads in flight; a part of one wave reads nothing that others load
   auto sync = [&](auto N) {
@@ -146,8 +155,10 @@ gated_fwd_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u1
   for (int e = 0; e < 16; ++e) sv[e] = act_f<ACT>(zg[e]);
 
   // chunk c in `cur`, chunk c + 1 in `nxt`; more: there is a chunk c + 1
-  auto iter = [&](auto MORE, int cur, int nxt) {
+  auto iter = [&](auto MORE, int c, int cur, int nxt, int far) {
     constexpr bool M = decltype(MORE)::value;
+    Dst dst;
+    if constexpr (M && SPREAD) dst = chunk_at(c + PF, far);
     constexpr int N1 = M ? KS : 0, N2 = 2 * NTN, NOPS = 2 * N1 + N2;
     const int b1 = RB + nxt * SLOT, b2 = RB + cur * SLOT;
     auto fetch = [&](int j) {
@@ -193,19 +204,20 @@ gated_fwd_kernel(const u16* __restrict__ X, const u16* __restrict__ Wg, const u1
           for (int e = 16 * (j - N1) / NV; e < 16 * (j - N1 + 1) / NV; ++e) sv[e] = act_f<ACT>(zg[e]);
         }
       }
+      if (M && SPREAD && j < NLD) load_piece(dst, j);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
   int cur = 0;
   for (int c = 0; c + 1 < NC; ++c) {
     const int nxt = cur + 1 == NS ? 0 : cur + 1, far = cur == 0 ? NS - 1 : cur - 1;
-    load_chunk(c + PF, far);
+    if (!SPREAD || b_wave >= B) load_chunk(c + PF, far);
     // (chunk c + 1 landed before the last barrier; a wave without rows only loads)
-    if (b_wave < B) iter(std::true_type{}, cur, nxt);
+    if (b_wave < B) iter(std::true_type{}, c, cur, nxt, far);
     sync(std::integral_constant<int, NLD*(PF - 2)>{});  // chunk c + 2
     cur = nxt;
   }
-  if (b_wave < B) iter(std::false_type{}, cur, cur);
+  if (b_wave < B) iter(std::false_type{}, 0, cur, cur, cur);
 
   if constexpr (ES > 1) {
     wait_vmcnt<0>();  // chunks past the last are still landing, as zeros
