@@ -739,8 +739,8 @@ GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cu
   // Measured: a program takes fixed_us and, for a subtile, sub_us alone on its CU or full_us on a full device (two a
   // CU at D <= 64, where they gain little on each other: vector issue is shared; one CU with two sets the time). A
   // split adds the sum's launch and the partials' bytes. H=8 B=2048 D=128 E=512: 79 us unsplit, 34 split in eight.
-  const double sub_us = DT == 32 ? 0.61 : DT == 64 ? 0.86 : DT == 128 ? 1.15 : 1.73;
-  const double full_us = DT == 32 ? 0.96 : DT == 64 ? 1.66 : DT == 128 ? 1.45 : 2.0;
+  const double sub_us = DT == 32 ? 0.61 : DT == 64 ? 0.86 : DT == 128 ? 1.15 : 1.35;
+  const double full_us = DT == 32 ? 0.96 : DT == 64 ? 1.66 : DT == 128 ? 1.45 : 1.55;
   const double fixed_us = DT <= 64 ? 5.0 : 8.0;
   double best = 0;
   p.nS = 1;
