@@ -86,7 +86,8 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *,
 
     Args:
         out: tensors of the gradients' shapes, each of any of the dtypes (an optimizer's full precision
-            buffers, say), overlapping neither the gradients nor each other; None clips in place.
+            buffers, say), overlapping neither the gradients nor each other; None clips in place
+            (gradients that do not overlap).
     Returns:
         (out, norm): the clipped tensors and the norm before the clipping.
     """
@@ -123,6 +124,8 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *,
         if d is not o:
             back.append((o, d))
     norm = _run(src, dst, max_norm, dev)
+    # autograd notices a saved tensor that has changed (copy_ below says so itself)
+    torch.autograd.graph.increment_version([o for o, d in zip(outs, dst) if d is o and not o.is_inference()])
     with torch.no_grad():
         for o, d in back:
             o.copy_(d)

@@ -724,6 +724,11 @@ PyObject* fast_clip(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                       : fmlp_grad_norm((int)n, g.data(), numel.data(), gt.data(), norm.data_ptr<float>(), ws.data_ptr(),
                                        bytes, stream);
   check_status(st, clip ? "gradient clipping" : "gradient norm");
+  if (clip)  // as any in-place operation, so that autograd notices a saved tensor that has changed
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      const at::Tensor& v = THPVariable_Unpack(PyList_GET_ITEM(args[1], i));
+      if (!v.is_inference()) v.unsafeGetTensorImpl()->bump_version();
+    }
   return THPVariable_Wrap(norm);
   END_HANDLE_TH_ERRORS
 }

@@ -186,6 +186,21 @@ def test_repeatable_on_streams_and_in_graphs():
         assert torch.equal(n3, n4) and all(torch.equal(a, b) for a, b in zip(o3, o4))
 
 
+def test_autograd_notices_a_saved_tensor_that_was_clipped():
+    for g in (torch.full((64,), 3.0, device="cuda"), torch.full((8, 16), 3.0, device="cuda").t(),
+              torch.full((8, 16), 3.0, device="cuda")[:, ::2]):
+        w = torch.ones_like(g).requires_grad_(True)
+        y = (w * g).sum()  # saves g
+        clip_grads([g], 0.5)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        with torch.inference_mode():
+            h = torch.full((64,), 3.0, device="cuda")
+            clip_grads([h, torch.full((8, 16), 3.0, device="cuda").t()], 0.5)
+        clip_grads([h], 0.25)
+        assert abs(h.norm().item() - 0.25) <= 1e-5
+
+
 def test_refusals():
     g = tensors([(4,), (5,)], (FL,))
     with pytest.raises(ValueError, match="max_norm"):
