@@ -135,8 +135,10 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *,
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, *,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_ (L2) on these kernels: clips the parameters' .grad in place and
-    returns their norm. error_if_nonfinite waits for the norm, and raises before any gradient is changed."""
+    returns their norm. A parameter that is listed twice (shared weights) counts once. error_if_nonfinite waits
+    for the norm, and raises before any gradient is changed."""
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    params = list({id(p): p for p in params}.values())  # two workgroups would scale a shared one at once
     grads = [p.grad for p in params if p.grad is not None]
     if error_if_nonfinite and grads and not torch.isfinite(grad_norm(grads)):
         raise RuntimeError("the total norm of the gradients is not finite, so it cannot be clipped")

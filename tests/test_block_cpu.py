@@ -133,3 +133,14 @@ def test_library_refuses_clip_arguments(L):
     assert call(dtype=9) == UNSUPPORTED and call(odt=3) == UNSUPPORTED
     assert call(g=None) == INVALID and call(g=15) == INVALID and call(o=18) == INVALID and call(norm=None) == INVALID
     assert call(max_norm=-1.0) == INVALID and call(max_norm=float("nan")) == INVALID
+
+
+def test_a_parameter_listed_twice_is_clipped_once(monkeypatch):
+    import flashmlp_amd.clip as clip
+
+    p, q, r = (torch.nn.Parameter(torch.zeros(3)) for _ in range(3))
+    p.grad, q.grad = torch.ones(3), torch.ones(3)
+    seen = []
+    monkeypatch.setattr(clip, "clip_grads", lambda grads, max_norm: (seen.append(list(grads)), 1.0))
+    clip.clip_grad_norm_([p, q, r, p, q], 1.0)
+    assert len(seen) == 1 and len(seen[0]) == 2 and seen[0][0] is p.grad and seen[0][1] is q.grad

@@ -201,6 +201,14 @@ def test_autograd_notices_a_saved_tensor_that_was_clipped():
         assert abs(h.norm().item() - 0.25) <= 1e-5
 
 
+def test_a_parameter_listed_twice_counts_once():
+    p, q = (torch.nn.Parameter(torch.zeros(n, device="cuda")) for n in (100001, 7))
+    p.grad, q.grad = torch.full_like(p, 2.0), torch.full_like(q, 3.0)
+    before = [p.grad.clone(), q.grad.clone()]
+    norm = clip_grad_norm_([p, q, p], 1.0)
+    check(None, [p.grad, q.grad], norm, before, 1.0)
+
+
 def test_refusals():
     g = tensors([(4,), (5,)], (FL,))
     with pytest.raises(ValueError, match="max_norm"):
