@@ -121,10 +121,15 @@ def block_join_fwd(residual, o, post_weight=None, gate=None, scale=1.0, *, pre_w
 
 
 def block_join_bwd(residual_out, o, rs_o, rs_r, dresidual, dy, post_weight=None, gate=None, scale=1.0, *,
-                   pre_weight=None, post=True, eps=1e-6, heads=None, dtype=None, _needs=(True,) * 5):
+                   pre_weight=None, post=True, eps=1e-6, heads=None, dtype=None, residual=None, _needs=(True,) * 5):
     """Gradients (dresidual_in, do, dpost_weight, dgate, dpre_weight) of block_join_fwd's outputs, which gave
-    residual_out (the stream itself without o), rs_o and rs_r. dresidual or dy may be None (zero). `_needs`
+    residual_out (the stream itself without o), rs_o and rs_r. With `residual`, a 16-bit stream
+    before the join, the unrounded residual' is made again from it and residual_out is not read: the gradients lose
+    nothing to the stream's rounding, as under autograd. dresidual or dy may be None (zero). `_needs`
     says which are wanted; the others, and those of inputs that are None, come back as None."""
+    from_r = residual is not None and o is not None and residual.dtype != torch.float32
+    if from_r:
+        residual_out = residual
     dtype = (o.dtype if o is not None else dtype or residual_out.dtype)
     pre = dy is not None
     B, H, D, groups = _check_join(residual_out, o, post_weight, gate, pre_weight if pre else None, heads, dtype, post, pre)
@@ -150,7 +155,8 @@ def block_join_bwd(residual_out, o, rs_o, rs_r, dresidual, dy, post_weight=None,
     dres, dyy = _dense_cols(dresidual), _dense_cols(dy)
     ws_ = [_flat(w) for w in (post_weight, gate, pre_weight if pre else None)]
     j = _call(B, H, D, groups, scale, eps, dtype, residual_out.dtype, post)
-    j.r_out, j.o, j.w_post, j.gate, j.w_pre = (_ptr(t) for t in (r2, oo, *ws_))
+    j.r, j.r_out = (_ptr(r2), None) if from_r else (None, _ptr(r2))
+    j.o, j.w_post, j.gate, j.w_pre = (_ptr(t) for t in (oo, *ws_))
     j.rs_o, j.rs_r, j.dr_out, j.dy = (_ptr(t) for t in (rs_o, rs_r, dres, dyy))
     j.dr, j.d_o, j.dw_post, j.dgate, j.dw_pre = (_ptr(t) for t in (dr, d_o, dpost, dgate, dpre if pre else None))
     j.r_stride = r2.stride(0)
@@ -172,13 +178,15 @@ def block_join_bwd(residual_out, o, rs_o, rs_r, dresidual, dy, post_weight=None,
 
 
 class BlockJoinFunction(torch.autograd.Function):
-    """Autograd binding of the join. Saves the stream after it, o, the weights and two floats a row."""
+    """Autograd binding of the join. Saves the stream (a 16-bit one before it, else after it), o, the weights and two
+    floats a row."""
 
     @staticmethod
     def forward(ctx, residual, o, post_weight, gate, pre_weight, scale, post, pre, eps, heads, dtype):
         r2, y, rs_o, rs_r = block_join_fwd(residual, o, post_weight, gate, scale, pre_weight=pre_weight, post=post,
                                            pre=pre, eps=eps, heads=heads, dtype=dtype, _save=True)
-        ctx.save_for_backward(residual if r2 is None else r2, o, rs_o, rs_r, post_weight, gate, pre_weight)
+        before = r2 is None or residual.dtype != torch.float32
+        ctx.save_for_backward(residual if before else r2, o, rs_o, rs_r, post_weight, gate, pre_weight)
         ctx.args = (scale, post, eps, heads, dtype)
         ctx.set_materialize_grads(False)
         return r2, y
@@ -191,7 +199,7 @@ class BlockJoinFunction(torch.autograd.Function):
         if dr2 is None and dy is None:
             return (None,) * 11
         g = block_join_bwd(r2, o, rs_o, rs_r, dr2, dy, post_weight, gate, scale, pre_weight=pre_weight, post=post,
-                           eps=eps, heads=heads, dtype=dtype, _needs=ctx.needs_input_grad[:5])
+                           eps=eps, heads=heads, dtype=dtype, residual=r2, _needs=ctx.needs_input_grad[:5])
         return (*g, *(None,) * 6)
 
 

@@ -99,12 +99,12 @@ hipError_t launch_gated32_dw(const GatedArgs& a, const GatedDwPlan& p, hipStream
 // taken from r), w_post, gate, w_pre (factors of one), r_out, y (results nobody asked for), and in the
 // backward dy, dr_out (gradients that are zero), dr, d_o, dw_post, dgate, dw_pre (not asked for).
 struct JoinArgs {
-  const void* r;
+  const void* r;  // backward: null, or what r' is computed from again, rows r_sr apart
   const void* o;
   const void* w_post;
   const void* gate;  // (groups, C): row g for rows g rows_per_gate ..
   const void* w_pre;
-  void* r_out;  // forward: r' (dense rows); backward: the r' that was saved, rows r_sr apart
+  void* r_out;  // forward: r' (dense rows); backward without r: the r' that was saved, rows r_sr apart
   void* y;
   float* rs_o;  // (B) 1 / rms of o and of r', written by the forward (or null) and read by the backward
   float* rs_r;

@@ -273,11 +273,13 @@ int check_join(const fmlp_join* j, bool bwd, fmlp::JoinArgs* a) {
   if (rows && !bwd && !has_y && j->r_out == nullptr) return abi_fail(FMLP_ERR_INVALID_ARG, "no output is asked for");
   if (rows && !has_o && (j->w_post || j->gate)) return abi_fail(FMLP_ERR_INVALID_ARG, "w_post or gate without o");
   if (rows && !has_y && j->w_pre && !bwd) return abi_fail(FMLP_ERR_INVALID_ARG, "w_pre without y");
+  // the backward of a 16-bit stream with r makes the unrounded r' again
+  const bool from_r = bwd && j->r && has_o && has_y && j->r_dtype != FMLP_DTYPE_F32;
   int vec = j->D % 8 == 0 ? 1 : 0, st;
-  if ((st = join_ptr(j->r, "r", rows && !bwd, rs, &vec)) || (st = join_ptr(j->o, "o", false, es, &vec)) ||
+  if ((st = join_ptr(bwd && !from_r ? nullptr : j->r, "r", rows && !bwd, rs, &vec)) || (st = join_ptr(j->o, "o", false, es, &vec)) ||
       (st = join_ptr(j->w_post, "w_post", false, es, &vec)) || (st = join_ptr(j->gate, "gate", false, es, &vec)) ||
       (st = join_ptr(j->w_pre, "w_pre", false, es, &vec)) ||
-      (st = join_ptr(j->r_out, "r_out", rows && bwd && has_y, rs, &vec)) ||
+      (st = join_ptr(j->r_out, "r_out", rows && bwd && has_y && !from_r, rs, &vec)) ||
       (st = join_ptr(j->y, "y", false, es, &vec)) || (st = join_stride(j->r_stride, "r", true, rs, &vec)) ||
       (st = join_stride(j->o_head_stride, "o head", has_o && j->H > 1, es, &vec)) ||
       (st = join_stride(j->o_row_stride, "o row", has_o, es, &vec)) ||
@@ -299,7 +301,7 @@ int check_join(const fmlp_join* j, bool bwd, fmlp::JoinArgs* a) {
     if (rows && !has_o && (j->d_o || j->dw_post || j->dgate)) return abi_fail(FMLP_ERR_INVALID_ARG, "gradients of o's part without o");
     if (j->dw_post && !j->post) return abi_fail(FMLP_ERR_INVALID_ARG, "dw_post without the post norm");
   }
-  a->r = j->r;
+  a->r = bwd && !from_r ? nullptr : j->r;
   a->o = j->o;
   a->w_post = j->w_post;
   a->gate = j->gate;

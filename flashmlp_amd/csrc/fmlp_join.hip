@@ -11,7 +11,7 @@
 //
 // One pass over the data each way: a row's C = heads x D columns stay in registers between the sums
 // that need all of them and the results, so that the forward reads o and r and writes r' and y, and the
-// backward reads r', o, dr', dy and writes dr, do. o and y are head-major (H, B, D), the layout of the
+// backward reads r (or r'), o, dr', dy and writes dr, do. o and y are head-major (H, B, D), the layout of the
 // MLP kernels, or rows of C columns; the transposition costs nothing, a vector of 8 columns lies in one
 // head. Both are bound by HBM bytes; sums are fp32. 16384 x 4096 bf16: forward 112 us (537 MB, 4.8 TB/s), backward 174
 // (805 MB, 4.6 TB/s) and 6 for the column sums; a copy of 1 GiB reaches 5.0 TB/s. Four rows: 5.9 us a call, all launch.
@@ -51,11 +51,23 @@ struct Vec {
     if constexpr (IO == IO_F32) return __uint_as_float(v[j >> 2][j & 3]);
     else return (j & 1) ? hi_f32<IO == IO_BF16>(v[0][j >> 1]) : lo_f32<IO == IO_BF16>(v[0][j >> 1]);
   }
+  __device__ __forceinline__ void put(const float (&f)[8]) {
+    static_assert(IO != IO_F32, "16-bit elements");
+    constexpr bool BF = IO == IO_BF16;
+    v[0] = u32x4{pack2<BF>(f[0], f[1]), pack2<BF>(f[2], f[3]), pack2<BF>(f[4], f[5]), pack2<BF>(f[6], f[7])};
+  }
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (auto& q : v) q = u32x4{0u, 0u, 0u, 0u};
   }
 };
+
+// what was computed from v is not kept: the compiler takes v for new (no instruction)
+template <int IO>
+__device__ __forceinline__ void forget(Vec<IO>& v) {
+#pragma unroll
+  for (auto& q : v.v) asm volatile("" : "+v"(q));
+}
 
 // A row's columns over the tpr threads that own it. Vectors (ALIGNED): thread t's vector k holds columns
 // 8 (t + k tpr) .. + 7. Else element j of it is column t + (8 k + j) tpr, read and written by itself.
@@ -308,7 +320,7 @@ join_bwd_kernel(JoinArgs a, JoinPlan p) {
     for (int k = 0; k < VPT; ++k) {
       if (a.dy) {
         x.dy[k] = load_heads<IO, ALIGNED>(a.dy, hy, row, C, t, tpr, k);
-        x.r2[k] = load_row<RIO, ALIGNED>(a.r_out, row * a.r_sr, C, t, tpr, k);
+        x.r2[k] = load_row<RIO, ALIGNED>(RIO != IO_F32 && a.r ? a.r : a.r_out, row * a.r_sr, C, t, tpr, k);
       }
       if (a.dr_out) x.dr[k] = load_row<RIO, ALIGNED>(a.dr_out, row * a.dr_sr, C, t, tpr, k);
       if (a.o) x.o[k] = load_heads<IO, ALIGNED>(a.o, ho, row, C, t, tpr, k);
@@ -321,8 +333,14 @@ join_bwd_kernel(JoinArgs a, JoinPlan p) {
   for (long long row = r0; row < r1; ++row) {
     const int db = (int)(row & 1);  // the row sums' buffers alternate: one barrier a sum
     if (!AHEAD) load(row, next);
-    const Row x = next;
+    Row x = next;
     const auto &r2 = x.r2, &dr = x.dr;
+    if constexpr (RIO != IO_F32)  // (the weights stay packed)
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) {
+        if (a.w_post) forget(wq[k]);
+        if (a.w_pre) forget(wp[k]);
+      }
     const auto &dy = x.dy, &o = x.o;
     if (AHEAD && row + 1 < r1) load(row + 1, next);
     if (a.gate && in_group == 0) {
@@ -335,15 +353,36 @@ join_bwd_kernel(JoinArgs a, JoinPlan p) {
       const float rr = x.rr;
       float s = 0.f;
 #pragma unroll
-      for (int k = 0; k < VPT; ++k)
+      for (int k = 0; k < VPT; ++k) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = r2[k].get(j);
+        if constexpr (RIO != IO_F32) {
+          // A 16-bit stream's unrounded r' is made again where r is given: dw_pre's error is then its own rounding (with
+          // the rounded r' 1.4 times that; 16384 x 4096 bf16: step 297 -> 306 us). Below, beside the row's mean, the
+          // rounded one is enough, in half the registers; what is unpacked here is not kept across the sum
+          // (kept, 8 more registers spill: 333 us).
+          if (a.r) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              float q = o[k].get(j) * x.ro;
+              if (a.w_post) q *= wq[k].get(j);
+              if (a.gate) q *= gq[k].get(j);
+              v[j] = __builtin_fmaf(a.scale, q, v[j]);
+            }
+            x.r2[k].put(v);
+            forget(x.o[k]);
+          }
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float m = r2[k].get(j) * rr, g = dy[k].get(j);
+          const float m = v[j] * rr, g = dy[k].get(j);
           const float dm = a.w_pre ? g * wp[k].get(j) : g;
           s_pre[k][j] = __builtin_fmaf(g, m, s_pre[k][j]);
           s = __builtin_fmaf(dm, m, s);
           d[k][j] = dm;
         }
+      }
       const float mean = row_sum<(MULTI > 0)>(s, part[db][0], nw) * rc;
 #pragma unroll
       for (int k = 0; k < VPT; ++k)

@@ -558,7 +558,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> join_fwd_run(const at::Tensor& r,
 
 at::Tensor cols(const at::Tensor& t) { return !t.defined() || cols1(t) ? t : t.contiguous(); }
 
-// (dr, do, dw_post, dgate, dw_pre); those that are not wanted undefined
+// A 16-bit stream's backward makes the unrounded r' again from r; else r' itself is what is saved.
+bool from_r(const at::Tensor& r, const at::Tensor& o) { return o.defined() && r.scalar_type() != at::kFloat; }
+
+// (dr, do, dw_post, dgate, dw_pre); those that are not wanted undefined. r2: r' or, where from_r, r
 std::vector<at::Tensor> join_bwd_run(const at::Tensor& r2, const at::Tensor& o, const at::Tensor& rs, at::Tensor dr2,
                                      at::Tensor dy, const at::Tensor& w_post, const at::Tensor& gate,
                                      const at::Tensor& w_pre, const JoinCfg& c, const bool* need) {
@@ -573,7 +576,8 @@ std::vector<at::Tensor> join_bwd_run(const at::Tensor& r2, const at::Tensor& o, 
   if (need[2] && w_post.defined()) g[2] = at::empty_like(w_post);
   if (need[3] && gate.defined()) g[3] = at::empty_like(gate);
   if (need[4] && w_pre.defined()) g[4] = dy.defined() ? at::empty_like(w_pre) : at::zeros_like(w_pre);
-  j.r_out = const_cast<void*>(cptr(r2));
+  if (from_r(r2, o)) j.r = cptr(r2);
+  else j.r_out = const_cast<void*>(cptr(r2));
   j.rs_o = rs.data_ptr<float>();
   j.rs_r = j.rs_o + j.B;
   j.dr_out = cptr(dr2);
@@ -602,7 +606,7 @@ struct JoinFn : torch::autograd::Function<JoinFn> {
     const at::Tensor o = o_.value_or(at::Tensor()), w_post = w_post_.value_or(at::Tensor()),
                      gate = gate_.value_or(at::Tensor()), w_pre = w_pre_.value_or(at::Tensor());
     auto [r2, y, rs] = join_fwd_run(r, o, w_post, gate, w_pre, c, true);
-    ctx->save_for_backward({r2.defined() ? r2 : r, o, rs, w_post, gate, w_pre});
+    ctx->save_for_backward({r2.defined() && !from_r(r, o) ? r2 : r, o, rs, w_post, gate, w_pre});
     ctx->saved_data["scale"] = c.scale;
     ctx->saved_data["eps"] = c.eps;
     ctx->saved_data["post"] = c.post;

@@ -302,8 +302,9 @@ int fmlp_head_sum(const float* src, void* dst, int64_t H, int64_t n, float scale
  * stream, the same or fp32. rs_o, rs_r (B, fp32): the rows' 1 / rms, written by the forward where not NULL
  * and read by the backward. Sums are fp32; y is taken from the unrounded r_out. Any alignment; 16-byte
  * aligned tensors with D % 8 == 0 and strides of whole 16 bytes take vector accesses. C <= 16384.
- * Backward: from dr_out and dy (NULL: zero), r_out (the stored one, rows r_stride apart; needed with dy),
- * o and rs_*, writes those of dr (dense rows), d_o, dw_post, dgate, dw_pre that are not NULL; the gradients
+ * Backward: from dr_out and dy (NULL: zero), o, rs_* and, with dy, r_out (the stored one, rows r_stride
+ * apart) or, of a 16-bit stream with o, r where that is not NULL (the same, from which the unrounded r_out is
+ * made again: gradients without the stream's rounding; r_out is not read), writes those of dr (dense rows), d_o, dw_post, dgate, dw_pre that are not NULL; the gradients
  * of weights and gate through fp32 partial sums in the workspace, added in a fixed order.
  */
 typedef struct {
@@ -324,7 +325,7 @@ typedef struct {
   void* dgate;
   void* dw_pre;
   int64_t B, H, D, groups;
-  int64_t r_stride;                      /* elements between the rows of r (backward: of r_out); r_out is dense */
+  int64_t r_stride;                      /* elements between the rows of r (backward: of the one read); r_out is dense */
   int64_t o_head_stride, o_row_stride;
   int64_t y_head_stride, y_row_stride;   /* of y; in the backward of dy */
   int64_t dr_out_stride;

@@ -7,7 +7,8 @@ infrastructure only).
     dp = s gate dr, dgate = sum s dr p, dw_post = sum dp n, dn = dp w_post, do = ro (dn - n mean(dn n))
 
 The kernels work in fp32 (a few roundings of 2^-24 a value, C or B terms a sum) and round the results
-(unit roundoff u, the stream's ur); the backward reads r' as it was rounded, so its m is off by up to ur |m|.
+(unit roundoff u, the stream's ur); the backward of an fp32 stream, and of any where r is not given, reads r' as it was rounded, so its m is off by up
+to ur |m| (stream_rounded); beside the row's mean it is always the rounded one.
 """
 from __future__ import annotations
 
@@ -16,7 +17,7 @@ import torch
 from .gated import UNIT
 
 
-def join64(r, o, w_post, gate, w_pre, scale, eps, post, dr2, dy):
+def join64(r, o, w_post, gate, w_pre, scale, eps, post, dr2, dy, stream_rounded=True):
     """All arguments on (B, C) rows; o, weights, gate, dr2 and dy may be None. Returns dicts of results and
     of their error bounds: r2, y, dr, do, dw_post, dgate, dw_pre."""
     u = UNIT[(o if o is not None else dy if dy is not None else r).dtype]
@@ -51,12 +52,12 @@ def join64(r, o, w_post, gate, w_pre, scale, eps, post, dr2, dy):
     zero = torch.zeros_like(r)
     d2 = zero if dr2 is None else dr2
     if dy is not None:
-        em = em + ur * m.abs()
+        em = em + ur * m.abs() if stream_rounded else em
         dm = dy * wp
         mean, amean = (dm * m).mean(1, keepdim=True), (dm * m).abs().mean(1, keepdim=True)
         dr = d2 + rr * (dm - m * mean)
         emean = (dm.abs() * em).mean(1, keepdim=True) + k * amean
-        edr = rr * (em * mean.abs() + m.abs() * emean) + 4 * k * (d2.abs() + rr * (dm.abs() + m.abs() * amean))
+        edr = rr * ((em + ur * m.abs()) * mean.abs() + m.abs() * emean) + 4 * k * (d2.abs() + rr * (dm.abs() + m.abs() * amean))
         edr = 1.01 * (edr + rr * er2.pow(2).mean(1, keepdim=True).sqrt() * (dr - d2).abs())
         t = (dy * m).sum(0)
         res["dw_pre"] = t

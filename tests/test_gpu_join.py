@@ -277,3 +277,29 @@ def test_refusals():
         block_norm(torch.zeros(1, 16392, dtype=BF, device="cuda"))
     with pytest.raises(RuntimeError, match="eps"):
         block_norm(r, eps=-1.0)
+
+
+@pytest.mark.parametrize("B,H,D,groups,dt", [(1, 3, 64, 1, BF), (95, 2, 128, 95, BF), (300, 3, 50, 2, HF), (64, 12, 128, 1, HF),
+                                             (40, 32, 128, 4, BF), (70, 64, 130, 1, BF), (12, 64, 200, 1, HF)])
+@pytest.mark.parametrize("drop", [(), ("w_post", "gate"), ("w_pre",), ("dr2",)])
+def test_gradients_of_a_16_bit_stream_lose_nothing_to_its_rounding(B, H, D, groups, dt, drop):
+    """made from r again, the backward's stream is the unrounded one: bounds without its rounding"""
+    t = {k: v for k, v in make(B, H, D, groups, dt, dt, seed=B).items() if k not in drop}
+    names = [k for k in ("r", "o", "w_post", "gate", "w_pre") if k in t]
+    ins = {k: t[k].detach().requires_grad_(True) for k in names}
+    r2, y = block_join(ins["r"], ins["o"], ins.get("w_post"), ins.get("gate"), 0.5, pre_weight=ins.get("w_pre"), eps=EPS)
+    outs, dout = ((r2, y), (t["dr2"], t["dy"])) if "dr2" in t else ((y,), (t["dy"],))
+    auto = dict(zip(names, torch.autograd.grad(outs, list(ins.values()), dout)))
+    a = (t["o"], t.get("w_post"), t.get("gate"), 0.5)
+    r2, y, rs_o, rs_r = block_join_fwd(t["r"], *a, pre_weight=t.get("w_pre"), eps=EPS, _save=True)
+    direct = block_join_bwd(None, t["o"], rs_o, rs_r, t.get("dr2"), t["dy"], *a[1:], pre_weight=t.get("w_pre"), eps=EPS,
+                            residual=t["r"])
+    want, bound = join64(t["r"], rows(t["o"], H), *a[1:3], t.get("w_pre"), 0.5, EPS, True, t.get("dr2"),
+                         rows(t["dy"], H), stream_rounded=False)
+    for (k, name), d in zip((("r", "dr"), ("o", "do"), ("w_post", "dw_post"), ("gate", "dgate"), ("w_pre", "dw_pre")), direct):
+        if k not in t:
+            assert d is None
+            continue
+        assert torch.equal(d, auto[k]), name
+        v = rows(d, H) if k == "o" else d
+        assert excess(v, want[name], bound[name], dt) <= 1.0, name
