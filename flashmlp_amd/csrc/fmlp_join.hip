@@ -13,8 +13,8 @@
 // that need all of them and the results, so that the forward reads o and r and writes r' and y, and the
 // backward reads r (or r'), o, dr', dy and writes dr, do. o and y are head-major (H, B, D), the layout of the
 // MLP kernels, or rows of C columns; the transposition costs nothing, a vector of 8 columns lies in one
-// head. Both are bound by HBM bytes; sums are fp32. 16384 x 4096 bf16: forward 112 us (537 MB, 4.8 TB/s), backward 174
-// (805 MB, 4.6 TB/s) and 6 for the column sums; a copy of 1 GiB reaches 5.0 TB/s. Four rows: 5.9 us a call, all launch.
+// head. Both are bound by HBM bytes; sums are fp32. 16384 x 4096 bf16: forward 112 us (537 MB, 4.8 TB/s), backward 188
+// (805 MB, 4.3 TB/s; from the rounded r' 177) and 6 for the column sums; a copy of 1 GiB reaches 5.0 TB/s. Four rows: 5.9 us a call, all launch.
 #include <algorithm>
 
 #include "fmlp_block.h"
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(MULTI ? 1024 : 256) join_fwd_kernel(JoinArgs a
 // ---------------------------------------------------------------------------------
 // MULTI = 2: more than 512 threads. A 16-bit stream's rows of up to 512 threads run two workgroups a CU, within 128
 // registers; an fp32 stream's data do not fit those, and one workgroup requests the next row's data ahead instead
-// (16384 x 4096, sums' launch included: bf16 177 us, with the next row ahead 189 at two workgroups and 194 at one;
+// (16384 x 4096, sums' launch included, from the rounded r': bf16 177 us, with the next row ahead 189 at two workgroups and 194 at one;
 // fp32 stream, 4096 x 2048: 42 us, 53 the first way).
 __host__ __device__ constexpr bool join_ahead(int RIO, int VPT, int MULTI) { return RIO == IO_F32 && VPT == 1 && MULTI == 1; }
 template <int IO, int RIO, int VPT, bool ALIGNED, int MULTI>

@@ -193,7 +193,8 @@ class GatedFlashMLP(torch.nn.Module):
 
     Parameters wg, wu (H, D, E) ~ randn / sqrt(D) and w2 (H, E, D) ~ randn / sqrt(E). A 2-D input
     (B, D) goes through every head and the output is the mean over heads, as in FlashMLP; the heads'
-    results, and the gradient of x, are summed in fp32 and rounded once.
+    results, and the gradient of x, are summed in fp32 and rounded once (under torch.compile, which traces the
+    registered per-head operator, each head's are rounded first).
     """
 
     def __init__(self, num_heads: int, hidden_dim: int, intermediate_dim: int, activation: str = "silu",
