@@ -28,10 +28,10 @@ from .gated import _On
 
 
 def _dense_cols(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    # unit column stride and no negative or lazily negated data
+    # unit column stride and no lazily negated data
     if t is None or (t.stride(-1) == 1 or t.shape[-1] <= 1) and not t.is_neg():
         return t
-    return t.contiguous()
+    return t.resolve_neg().contiguous()
 
 
 def _heads3(t: torch.Tensor) -> Tuple[int, int]:
@@ -86,7 +86,7 @@ def _call(B, H, D, groups, scale, eps, dtype, r_dtype, post) -> _lib.Join:
 
 def _flat(w):
     # weights and gate as dense rows
-    return None if w is None else w.contiguous()
+    return None if w is None else w.resolve_neg().contiguous()
 
 
 def block_join_fwd(residual, o, post_weight=None, gate=None, scale=1.0, *, pre_weight=None, post=True, pre=True,

@@ -113,11 +113,11 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *,
     src, dst, back = [], [], []
     for g, o in zip(grads, outs):
         if _one_run(o) and (g is o or g.stride() == o.stride()):
-            src.append(g if g is o or _one_run(g) else g.contiguous())
+            src.append(g if g is o or _one_run(g) else g.resolve_neg().contiguous())
             dst.append(o)
             continue
         # other layouts through dense tensors
-        s = g.contiguous()
+        s = g.resolve_neg().contiguous()
         d = o if o.is_contiguous() and not o.is_neg() else torch.empty(o.shape, dtype=o.dtype, device=dev)
         src.append(s)
         dst.append(d)

@@ -61,12 +61,10 @@ bool eligible(PyObject* const* args, int n, const at::Tensor** ts, int* code, un
   *copy = 0;
   for (int i = 0; i < n; ++i) {
     const at::Tensor& t = *ts[i];
-    if (t.scalar_type() != x.scalar_type() || t.device() != x.device() || t.layout() != at::kStrided || t.dim() != 3)
+    if (t.scalar_type() != x.scalar_type() || t.device() != x.device() || t.layout() != at::kStrided || t.dim() != 3 ||
+        t.is_neg())  // (a lazily negated view: its memory holds the other sign)
       return false;
-    if (!dense16(t) && !((i == 0 || i == 3) && rows16(t))) {
-      if (t.is_neg() || t.is_conj()) return false;  // (a lazily negated view: its copy has to apply the sign)
-      *copy |= 1u << i;
-    }
+    if (!dense16(t) && !((i == 0 || i == 3) && rows16(t))) *copy |= 1u << i;
   }
   *code = c;
   return true;
@@ -350,7 +348,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     at::Tensor dout = grads[0];
     if (!dout.defined()) return variable_list(6);
     if (!rows16(dout) || dout.is_neg()) {
-      dout = dout.contiguous();
+      dout = dout.resolve_neg().contiguous();
       if (!dense16(dout)) dout = dout.clone(at::MemoryFormat::Contiguous);
     }
     const bool dw = ctx->needs_input_grad(1) || ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
@@ -391,7 +389,7 @@ struct SharedGatedFn : torch::autograd::Function<SharedGatedFn> {
     const int64_t H = s[1].size(0);
     at::Tensor dout = every_head(grads[0], H);
     if (!rows16(dout) || dout.is_neg()) {
-      at::Tensor d = grads[0].contiguous();
+      at::Tensor d = grads[0].resolve_neg().contiguous();
       if ((reinterpret_cast<uintptr_t>(d.data_ptr()) & 15u) != 0) d = d.clone(at::MemoryFormat::Contiguous);
       dout = every_head(d, H);
     }
@@ -556,7 +554,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> join_fwd_run(const at::Tensor& r,
   return {r2, y, rs};
 }
 
-at::Tensor cols(const at::Tensor& t) { return !t.defined() || cols1(t) ? t : t.contiguous(); }
+at::Tensor cols(const at::Tensor& t) { return !t.defined() || cols1(t) ? t : t.resolve_neg().contiguous(); }
 
 // A 16-bit stream's backward makes the unrounded r' again from r; else r' itself is what is saved.
 bool from_r(const at::Tensor& r, const at::Tensor& o) { return o.defined() && r.scalar_type() != at::kFloat; }

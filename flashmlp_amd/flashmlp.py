@@ -88,8 +88,9 @@ def _fwd_ws_bytes(device_index: int, H: int, B: int, D: int, E: int, dtype: int)
 
 def _dense(t: torch.Tensor) -> torch.Tensor:
     # the tuned kernels use 16-byte vector accesses on dense tensors: a strided view, or one at
-    # a storage offset that is not a multiple of 16 bytes, is copied
-    t = t.contiguous()
+    # a storage offset that is not a multiple of 16 bytes, is copied; so is a lazily negated view (its memory
+    # holds the other sign, and contiguous() alone keeps it where it is dense)
+    t = t.resolve_neg().contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -141,7 +142,7 @@ def _io_code(x: torch.Tensor, *ts: torch.Tensor):
 
 def _dense_all(*ts: torch.Tensor):
     # the tuned kernels' weights: unchanged when all are dense and 16-byte aligned
-    if all(t.is_contiguous() and t.data_ptr() % 16 == 0 for t in ts):
+    if all(t.is_contiguous() and t.data_ptr() % 16 == 0 and not t.is_neg() for t in ts):
         return ts
     return tuple(_dense(t) for t in ts)
 
@@ -161,7 +162,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     # x and do of the tuned kernels: rows dense and 16-byte aligned, heads any multiple of 16
     # bytes apart (0 for one matrix expanded to every head); anything else is copied
     s = t.stride()
-    if s[2] == 1 and s[1] == t.shape[2] and s[0] * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
+    if (s[2] == 1 and s[1] == t.shape[2] and s[0] * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0
+            and not t.is_neg()):
         return t
     return _dense(t)
 
@@ -222,6 +224,7 @@ def flashmlp_fwd(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, activation
                                        _act_code(activation), ws.data_ptr() if ws is not None else None, ws_bytes,
                                        stream)
         else:
+            x, w1, w2 = (t.resolve_neg() for t in (x, w1, w2))
             st = L.fmlp_fwd_strided(x.data_ptr(), w1.data_ptr(), w2.data_ptr(), o.data_ptr(), H, B, D, E,
                                     _lib.strides(x), _lib.strides(w1), _lib.strides(w2), dtype,
                                     _act_code(activation), stream)
@@ -314,6 +317,7 @@ def flashmlp_bwd(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, do: torch.
                 ws = _alloc_ws(ws_bytes, x.device)
             except torch.OutOfMemoryError:
                 ws, ws_bytes = None, 0
+            x, w1, w2, do = (t.resolve_neg() for t in (x, w1, w2, do))
             st = L.fmlp_bwd_strided(x.data_ptr(), w1.data_ptr(), w2.data_ptr(), do.data_ptr(), _ptr(dx),
                                     _ptr(dw1), _ptr(dw2), H, B, D, E, _lib.strides(x), _lib.strides(w1),
                                     _lib.strides(w2), _lib.strides(do), flags, _act_code(activation),
