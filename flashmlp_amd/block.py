@@ -24,7 +24,7 @@ import torch
 
 from . import _lib
 from .flashmlp import _DTYPES, _alloc_ws, _fast, _ptr
-from .gated import _On
+from .gated import _not_traced, _On
 
 
 def _dense_cols(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -93,6 +93,11 @@ def block_join_fwd(residual, o, post_weight=None, gate=None, scale=1.0, *, pre_w
                    eps=1e-6, heads=None, dtype=None, _save=False):
     """(residual', y, rs_o, rs_r): block_join without autograd. residual' is None without o; y is None with
     pre=False; rs_o, rs_r (the rows' 1 / rms, what the backward reads) are None unless `_save`."""
+    _not_traced("block_join_fwd")
+    return _join_fwd(residual, o, post_weight, gate, scale, pre_weight, post, pre, eps, heads, dtype, _save)
+
+
+def _join_fwd(residual, o, post_weight, gate, scale, pre_weight, post, pre, eps, heads, dtype, _save):
     dtype = (o.dtype if o is not None else dtype or residual.dtype)
     B, H, D, groups = _check_join(residual, o, post_weight, gate, pre_weight, heads, dtype, post, pre)
     dev = residual.device
@@ -127,6 +132,13 @@ def block_join_bwd(residual_out, o, rs_o, rs_r, dresidual, dy, post_weight=None,
     before the join, the unrounded residual' is made again from it and residual_out is not read: the gradients lose
     nothing to the stream's rounding, as under autograd. dresidual or dy may be None (zero). `_needs`
     says which are wanted; the others, and those of inputs that are None, come back as None."""
+    _not_traced("block_join_bwd")
+    return _join_bwd(residual_out, o, rs_o, rs_r, dresidual, dy, post_weight, gate, scale, pre_weight, post, eps, heads,
+                     dtype, residual, _needs)
+
+
+def _join_bwd(residual_out, o, rs_o, rs_r, dresidual, dy, post_weight, gate, scale, pre_weight, post, eps, heads, dtype,
+              residual, _needs):
     from_r = residual is not None and o is not None and residual.dtype != torch.float32
     if from_r:
         residual_out = residual
@@ -183,8 +195,7 @@ class BlockJoinFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, residual, o, post_weight, gate, pre_weight, scale, post, pre, eps, heads, dtype):
-        r2, y, rs_o, rs_r = block_join_fwd(residual, o, post_weight, gate, scale, pre_weight=pre_weight, post=post,
-                                           pre=pre, eps=eps, heads=heads, dtype=dtype, _save=True)
+        r2, y, rs_o, rs_r = _join_fwd(residual, o, post_weight, gate, scale, pre_weight, post, pre, eps, heads, dtype, True)
         before = r2 is None or residual.dtype != torch.float32
         ctx.save_for_backward(residual if before else r2, o, rs_o, rs_r, post_weight, gate, pre_weight)
         ctx.args = (scale, post, eps, heads, dtype)
@@ -198,12 +209,15 @@ class BlockJoinFunction(torch.autograd.Function):
         scale, post, eps, heads, dtype = ctx.args
         if dr2 is None and dy is None:
             return (None,) * 11
-        g = block_join_bwd(r2, o, rs_o, rs_r, dr2, dy, post_weight, gate, scale, pre_weight=pre_weight, post=post,
-                           eps=eps, heads=heads, dtype=dtype, residual=r2, _needs=ctx.needs_input_grad[:5])
+        g = _join_bwd(r2, o, rs_o, rs_r, dr2, dy, post_weight, gate, scale, pre_weight, post, eps, heads, dtype, r2,
+                      ctx.needs_input_grad[:5])
         return (*g, *(None,) * 6)
 
 
-def _needs_grad(*ts) -> bool:
+def _through_function(*ts) -> bool:
+    # whether a call is to be a Function: for its gradients, or as the operation that a traced graph holds
+    if torch.jit.is_tracing():
+        return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
@@ -221,9 +235,9 @@ def block_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, heads:
         r = _fast.join(x, None, None, None, weight, 1.0, True, eps, heads or 0, _DTYPES[dtype])
         if r is not None:
             return r[1]
-    if _needs_grad(x, weight):
+    if _through_function(x, weight):
         return BlockJoinFunction.apply(x, None, None, None, weight, 1.0, True, True, eps, heads, dtype)[1]
-    return block_join_fwd(x, None, pre_weight=weight, eps=eps, heads=heads, dtype=dtype)[1]
+    return _join_fwd(x, None, None, None, 1.0, weight, True, True, eps, heads, dtype, False)[1]
 
 
 @torch.compiler.disable
@@ -241,6 +255,6 @@ def block_join(residual: torch.Tensor, o: torch.Tensor, post_weight: Optional[to
         r = _fast.join(residual, o, post_weight, gate, pre_weight, scale, post, eps, 0, 0)
         if r is not None:
             return r
-    if _needs_grad(residual, o, post_weight, gate, pre_weight):
+    if _through_function(residual, o, post_weight, gate, pre_weight):
         return BlockJoinFunction.apply(residual, o, post_weight, gate, pre_weight, scale, post, pre, eps, None, None)
-    return block_join_fwd(residual, o, post_weight, gate, scale, pre_weight=pre_weight, post=post, pre=pre, eps=eps)[:2]
+    return _join_fwd(residual, o, post_weight, gate, scale, pre_weight, post, pre, eps, None, None, False)[:2]

@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from .flashmlp import _DTYPES, _fast
-from .gated import _On
+from .gated import _not_traced, _On
 
 
 def _one_run(t: torch.Tensor) -> bool:
@@ -76,6 +76,7 @@ def grad_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
     norm = _fast.clip(grads, None, 0.0) if _fast is not None else None  # dense tensors on one GPU: else None
     if norm is not None:
         return norm
+    _not_traced("grad_norm")
     dev = _check(grads, "gradients")
     return _run([g if _one_run(g) else g.contiguous() for g in grads], None, 0.0, dev)
 
@@ -103,6 +104,7 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *,
     norm = _fast.clip(grads, outs, max_norm) if _fast is not None else None  # as in grad_norm
     if norm is not None:
         return outs, norm
+    _not_traced("clip_grads")
     dev = _check(grads, "gradients")
     if out is not None:
         if _check(outs, "outputs") != dev:

@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <c10/util/Exception.h>
@@ -403,7 +404,12 @@ struct SharedGatedFn : torch::autograd::Function<SharedGatedFn> {
   }
 };
 
+// Under torch.jit.trace a call that launches by itself would leave its allocations in the graph, never filled: the Python
+// modules call what the graph can hold.
+bool traced() { return at::tracer::impl::is_dispatch_enabled(); }
+
 bool unpack(PyObject* const* args, int n, const at::Tensor** ts) {
+  if (traced()) return false;
   for (int i = 0; i < n; ++i) {
     if (!THPVariable_Check(args[i])) return false;
     ts[i] = &THPVariable_Unpack(args[i]);
@@ -646,7 +652,7 @@ at::Tensor or_none(PyObject* o, bool* ok) {
 // heads (0: rows) and the dtype of `dtype_of` (0 fp16, 1 bf16, 2 fp32)
 PyObject* fast_join(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 10) Py_RETURN_NONE;
+  if (nargs != 10 || traced()) Py_RETURN_NONE;
   at::Tensor t[5];
   bool ok = true;
   for (int i = 0; i < 5; ++i) t[i] = or_none(args[i], &ok);
@@ -680,7 +686,7 @@ PyObject* fast_join(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // clip(grads, outs, max_norm) -> norm, or None; lists of tensors, outs None for the norm alone
 PyObject* fast_clip(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 3 || !PyList_Check(args[0]) || (args[1] != Py_None && !PyList_Check(args[1]))) Py_RETURN_NONE;
+  if (nargs != 3 || traced() || !PyList_Check(args[0]) || (args[1] != Py_None && !PyList_Check(args[1]))) Py_RETURN_NONE;
   const bool clip = args[1] != Py_None;
   const Py_ssize_t n = PyList_GET_SIZE(args[0]);
   if (n == 0 || n > (1 << 24) || (clip && PyList_GET_SIZE(args[1]) != n)) Py_RETURN_NONE;

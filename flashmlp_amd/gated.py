@@ -35,6 +35,12 @@ def _check(x, wg, wu, w2) -> Tuple[int, int, int, int]:
     return H, B, D, E
 
 
+def _not_traced(what: str):
+    # (the graph would hold the outputs' allocation and not the launch that fills them)
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{what} cannot be traced by torch.jit.trace: it is no operation that a graph can hold")
+
+
 class _On:
     """The library launches on the current device: make it the tensors'."""
 
@@ -119,6 +125,8 @@ def flashmlp_gated_fwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, w2: 
         o = _fast.gated_fwd(x, wg, wu, w2, _act_code(activation))
         if o is not None:
             return o
+    if torch.jit.is_tracing():  # the operation that the graph holds
+        return torch.ops.flashmlp_amd.gated_fwd(x, wg, wu, w2, activation)
     return _fwd(x, wg, wu, w2, activation)
 
 
@@ -135,6 +143,9 @@ def flashmlp_gated_bwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, w2: 
         g = _fast.gated_bwd(x, wg, wu, w2, do, _act_code(activation), need_dx, need_dw)
         if g is not None:
             return g
+    if torch.jit.is_tracing():  # as in flashmlp_gated_fwd; it computes them all
+        g = torch.ops.flashmlp_amd.gated_bwd(x, wg, wu, w2, do, activation)
+        return tuple(v if n else None for v, n in zip(g, (need_dx, need_dw, need_dw, need_dw)))
     return _bwd(x, wg, wu, w2, do, activation, need_dx, need_dw)
 
 
@@ -223,4 +234,5 @@ class GatedFlashMLP(torch.nn.Module):
             o = (_fast.gated_shared if shared else _fast.gated)(x, *w, _act_code(act))
             if o is not None:
                 return o
+        # (under torch.jit.trace too, whose graph holds these Functions)
         return (_SharedGatedFunction if shared else GatedFlashMLPFunction).apply(x, *w, act)
