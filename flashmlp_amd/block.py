@@ -21,6 +21,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 from .flashmlp import _DTYPES, _alloc_ws, _fast, _ptr
@@ -215,10 +216,12 @@ class BlockJoinFunction(torch.autograd.Function):
 
 
 def _through_function(*ts) -> bool:
-    # whether a call is to be a Function: for its gradients, or as the operation that a traced graph holds
+    # whether a call is to be a Function: for its gradients, as the operation that a traced graph holds, or to refuse
+    # forward mode
     if torch.jit.is_tracing():
         return True
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    ts = [t for t in ts if t is not None]
+    return torch.is_grad_enabled() and any(t.requires_grad for t in ts) or any(unpack_dual(t).tangent is not None for t in ts)
 
 
 @torch.compiler.disable  # (torch.compile breaks its graph here)

@@ -666,9 +666,9 @@ PyObject* fast_join(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
   c.dtype = t[1].defined() ? t[1].scalar_type() : code == 0 ? at::kHalf : code == 1 ? at::kBFloat16 : at::kFloat;
   if (!(c.eps >= 0) || !join_ok(t[0], t[1], t[2], t[3], t[4], c)) Py_RETURN_NONE;
+  // a tensor with a tangent goes to the node too, which refuses forward mode
   bool grad = false;
-  if (at::GradMode::is_enabled())
-    for (auto& v : t) grad = grad || (v.defined() && v.requires_grad());
+  for (auto& v : t) grad = grad || (v.defined() && ((at::GradMode::is_enabled() && v.requires_grad()) || v._fw_grad(0).defined()));
   at::Tensor r2, y;
   if (grad) {
     const auto opt = [&](int i) { return t[i].defined() ? JoinFn::Opt(t[i]) : JoinFn::Opt(); };
