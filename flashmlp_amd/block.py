@@ -18,6 +18,7 @@ as long as the columns are dense (other views are copied).
 """
 from __future__ import annotations
 
+import numbers
 from typing import Optional, Tuple
 
 import torch
@@ -77,6 +78,12 @@ def _check_join(r, o, w_post, gate, w_pre, heads, dtype, post, pre):
     return B, H, D, groups
 
 
+def _check_number(v, name):
+    # (a tensor would be read on the host, and get no gradient)
+    if not isinstance(v, numbers.Real):
+        raise TypeError(f"{name} must be a number, got {type(v).__name__}")
+
+
 def _call(B, H, D, groups, scale, eps, dtype, r_dtype, post) -> _lib.Join:
     j = _lib.Join()
     j.B, j.H, j.D, j.groups = B, H, D, groups
@@ -99,6 +106,8 @@ def block_join_fwd(residual, o, post_weight=None, gate=None, scale=1.0, *, pre_w
 
 
 def _join_fwd(residual, o, post_weight, gate, scale, pre_weight, post, pre, eps, heads, dtype, _save):
+    _check_number(scale, "scale")
+    _check_number(eps, "eps")
     dtype = (o.dtype if o is not None else dtype or residual.dtype)
     B, H, D, groups = _check_join(residual, o, post_weight, gate, pre_weight, heads, dtype, post, pre)
     dev = residual.device
@@ -140,6 +149,8 @@ def block_join_bwd(residual_out, o, rs_o, rs_r, dresidual, dy, post_weight=None,
 
 def _join_bwd(residual_out, o, rs_o, rs_r, dresidual, dy, post_weight, gate, scale, pre_weight, post, eps, heads, dtype,
               residual, _needs):
+    _check_number(scale, "scale")
+    _check_number(eps, "eps")
     from_r = residual is not None and o is not None and residual.dtype != torch.float32
     if from_r:
         residual_out = residual

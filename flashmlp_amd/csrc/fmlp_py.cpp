@@ -657,6 +657,8 @@ PyObject* fast_join(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   bool ok = true;
   for (int i = 0; i < 5; ++i) t[i] = or_none(args[i], &ok);
   if (!ok || !t[0].defined()) Py_RETURN_NONE;
+  for (int i : {5, 7})  // scale and eps are numbers: a tensor's value would be taken, and its gradient lost
+    if (!PyFloat_Check(args[i]) && !PyLong_Check(args[i])) Py_RETURN_NONE;
   JoinCfg c{PyFloat_AsDouble(args[5]), PyFloat_AsDouble(args[7]), PyObject_IsTrue(args[6]) == 1, PyLong_AsLong(args[8]),
             at::kFloat};
   const long code = PyLong_AsLong(args[9]);
