@@ -87,8 +87,8 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *,
 
     Args:
         out: tensors of the gradients' shapes, each of any of the dtypes (an optimizer's full precision
-            buffers, say), overlapping neither the gradients nor each other; None clips in place
-            (gradients that do not overlap).
+            buffers, say); None clips in place. Outputs that overlap each other, or a gradient that is
+            not clipped in place, are refused.
     Returns:
         (out, norm): the clipped tensors and the norm before the clipping.
     """
@@ -125,6 +125,8 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *,
         dst.append(d)
         if d is not o:
             back.append((o, d))
+    if len({(o.data_ptr(), o.shape, o.stride()) for o, _ in back}) < len(back):  # (dense ones: the library's own check)
+        raise RuntimeError("an output is listed twice: outputs must not overlap")
     norm = _run(src, dst, max_norm, dev)
     # autograd notices a saved tensor that has changed (copy_ below says so itself)
     torch.autograd.graph.increment_version([o for o, d in zip(outs, dst) if d is o and not o.is_inference()])
@@ -134,14 +136,21 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *,
     return outs, norm
 
 
+def _memory(t: torch.Tensor):
+    # equal for tensors that are one and the same memory
+    if t.layout != torch.strided or t.numel() == 0:
+        return id(t)
+    return t.data_ptr(), t.dtype, t.shape, t.stride()
+
+
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, *,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_ (L2) on these kernels: clips the parameters' .grad in place and
-    returns their norm. A parameter that is listed twice (shared weights) counts once. error_if_nonfinite waits
-    for the norm, and raises before any gradient is changed."""
+    returns their norm. A gradient that is there twice (a parameter listed twice, or parameters that share one
+    gradient) counts and is scaled once. error_if_nonfinite waits for the norm, and raises before any gradient is
+    changed."""
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    params = list({id(p): p for p in params}.values())  # two workgroups would scale a shared one at once
-    grads = [p.grad for p in params if p.grad is not None]
+    grads = list({_memory(p.grad): p.grad for p in params if p.grad is not None}.values())
     if error_if_nonfinite and grads and not torch.isfinite(grad_norm(grads)):
         raise RuntimeError("the total norm of the gradients is not finite, so it cannot be clipped")
     return clip_grads(grads, max_norm)[1]

@@ -3,6 +3,7 @@
 #include "../../include/flashmlp.h"
 #include "fmlp_block.h"
 
+#include <algorithm>
 #include <new>
 #include <vector>
 
@@ -385,6 +386,32 @@ FMLP_EXPORT int fmlp_join_bwd(const fmlp_join* j, void* workspace, size_t worksp
 // ---------------------------------------------------------------------------------------------
 namespace {
 
+// One run of memory of a clipping call: an output, or a gradient that is read and has another output.
+struct ClipRange {
+  uintptr_t lo, hi;
+  int i;
+  bool write;
+};
+
+// Workgroups write the outputs in no order: an output that shares memory with another tensor of the call than its own
+// gradient, in place, would be a race. Sets the two tensors' indices.
+bool clip_overlap(std::vector<ClipRange>& r, int* a, int* b) {
+  const auto by_lo = [](const ClipRange& x, const ClipRange& y) { return x.lo < y.lo; };
+  if (!std::is_sorted(r.begin(), r.end(), by_lo)) std::sort(r.begin(), r.end(), by_lo);
+  const ClipRange *w = nullptr, *any = nullptr;  // those that reach furthest so far
+  for (const ClipRange& x : r) {
+    const ClipRange* o = x.write ? any : w;
+    if (o != nullptr && x.lo < o->hi) {
+      *a = std::min(x.i, o->i);
+      *b = std::max(x.i, o->i);
+      return true;
+    }
+    if (any == nullptr || x.hi > any->hi) any = &x;
+    if (x.write && (w == nullptr || x.hi > w->hi)) w = &x;
+  }
+  return false;
+}
+
 int clip_impl(int n, const void* const* grads, void* const* outs, const int64_t* numels, const int* dtypes,
               const int* out_dtypes, bool clip, float max_norm, float* norm, void* ws, size_t ws_bytes, void* stream) {
   if (n < 0) return abi_fail(FMLP_ERR_INVALID_ARG, "%d tensors", n);
@@ -394,8 +421,10 @@ int clip_impl(int n, const void* const* grads, void* const* outs, const int64_t*
     return abi_fail(FMLP_ERR_INVALID_ARG, "norm is NULL or not 4-byte aligned");
   if (clip && !(max_norm >= 0)) return abi_fail(FMLP_ERR_INVALID_ARG, "max_norm is negative or NaN");
   std::vector<fmlp::ClipTensor> t;
+  std::vector<ClipRange> ranges;
   try {
     t.resize((size_t)n);
+    if (clip) ranges.reserve(2 * (size_t)n);
   } catch (const std::bad_alloc&) {
     return abi_fail(FMLP_ERR_INVALID_ARG, "no host memory for %d tensors", n);
   }
@@ -415,7 +444,15 @@ int clip_impl(int n, const void* const* grads, void* const* outs, const int64_t*
         return abi_fail(FMLP_ERR_INVALID_ARG, "output %d is NULL or not aligned to its elements", i);
     }
     t[(size_t)i] = fmlp::ClipTensor{g, o, numels[i], io_type(ins[0]), io_type(ins[1])};
+    if (clip && numels[i] > 0) {
+      const uintptr_t gi = reinterpret_cast<uintptr_t>(g), oi = reinterpret_cast<uintptr_t>(o);
+      ranges.push_back(ClipRange{oi, oi + (uintptr_t)numels[i] * elem_bytes(ins[1]), i, true});
+      if (g != o || ins[0] != ins[1]) ranges.push_back(ClipRange{gi, gi + (uintptr_t)numels[i] * elem_bytes(ins[0]), i, false});
+    }
   }
+  int one, two;
+  if (clip && clip_overlap(ranges, &one, &two))
+    return abi_fail(FMLP_ERR_INVALID_ARG, "the output of tensor %d or %d overlaps a tensor of the call", one, two);
   int cus = 0, st;
   if ((st = fmlp::abi_num_cus(&cus))) return st;
   const fmlp::ClipPlan p = fmlp::clip_plan(n, numels, cus);

@@ -342,8 +342,8 @@ int fmlp_join_bwd(const fmlp_join* call, void* workspace, size_t workspace_bytes
  * Global L2 norm of n gradients, and clipping: *norm = sqrt(sum of all squares) (fp32, on the device),
  * outs[i] = grads[i] * min(1, max_norm / (norm + 1e-6)). No counterpart in the reference. Tensors are
  * dense runs of numels[i] elements of dtypes[i] / out_dtypes[i] (fp16, bf16, fp32, each its own), aligned to
- * their elements; outs[i] == grads[i] clips in place (and writes nothing where the norm is within
- * max_norm), other overlaps are not allowed. Squares are summed in 64 bits in a fixed order. A norm that
+ * their elements; outs[i] == grads[i] of one dtype clips in place (and writes nothing where the norm is
+ * within max_norm), an output that overlaps any other tensor of the call is refused (FMLP_ERR_INVALID_ARG). Squares are summed in 64 bits in a fixed order. A norm that
  * is infinite or NaN gives the coefficient 0 or NaN, as torch's clipping does. n = 0: the norm is 0. The
  * arrays are read on the host before the call returns. workspace: fmlp_clip_workspace_bytes, never NULL.
  */
