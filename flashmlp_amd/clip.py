@@ -7,9 +7,10 @@
     norm = sqrt(sum of all squares),  out = grad * min(1, max_norm / (norm + 1e-6))
 
 The norm is an fp32 number on the tensors' device; nothing waits for it (error_if_nonfinite does).
-Gradients are fp16, bf16 or fp32 in any mix, on one GPU. The squares are summed in 64 bits in a fixed order,
-so that no finite gradients overflow and results repeat bitwise. A norm that is infinite or NaN scales by 0
-or NaN, as torch.nn.utils.clip_grad_norm_ does.
+Gradients are fp16, bf16 or fp32 in any mix, on one GPU. The squares are summed in 64 bits in a fixed order:
+results repeat bitwise, and finite gradients whose norm is beyond fp32, which comes back as infinity, are clipped by
+their true norm. A norm that is infinite or NaN because a gradient is scales by 0 or NaN, as
+torch.nn.utils.clip_grad_norm_ does.
 """
 from __future__ import annotations
 

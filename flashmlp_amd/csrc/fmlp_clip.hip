@@ -10,6 +10,7 @@
 // behind the loads (32-bit squares measured the same). 302 M bf16 gradients into fp32: norm 114 us (5.3 TB/s), scaling
 // 355 (1.8 GB, 5.1 TB/s); non-temporal stores 490, the second pass in reverse order no gain. Partial sums go through the workspace and are added in a fixed order.
 #include <algorithm>
+#include <cfloat>
 
 #include "fmlp_block.h"
 #include "fmlp_device.h"
@@ -122,9 +123,10 @@ __global__ void __launch_bounds__(256) norm_kernel(ClipTable t, long long chunk,
   if (threadIdx.x == 0) part[blockIdx.x] = (w[0] + w[1]) + (w[2] + w[3]);
 }
 
-// The norm, and the coefficient torch's clipping uses (a NaN norm stays one: min would drop it).
+// The norm, and the coefficient torch's clipping uses (a NaN norm stays one: min would drop it): an fp32 number, but
+// where a finite norm is beyond fp32, which is then kept in 64 bits.
 __global__ void __launch_bounds__(1024) norm_finish_kernel(const double* part, long long n, float max_norm, float* norm,
-                                                           float* coef) {
+                                                           double* coef) {
   __shared__ double w[16];
   double s = 0;
   for (long long i = threadIdx.x; i < n; i += 1024) s += part[i];
@@ -135,11 +137,13 @@ __global__ void __launch_bounds__(1024) norm_finish_kernel(const double* part, l
   double v = 0;
 #pragma unroll
   for (int i = 0; i < 16; ++i) v += w[i];
-  const float r = (float)__builtin_sqrt(v);
+  v = __builtin_sqrt(v);
+  const float r = (float)v;
   *norm = r;
   if (coef) {
-    const float c = max_norm / (r + 1e-6f);
-    *coef = c > 1.f ? 1.f : c;
+    const bool beyond = r > FLT_MAX && v <= DBL_MAX;
+    const double c = beyond ? (double)max_norm / v : (double)(max_norm / (r + 1e-6f));
+    *coef = c > 1. ? 1. : c;
   }
 }
 
@@ -163,6 +167,17 @@ __device__ __forceinline__ void chunk_scale(const void* g, void* out, long long 
       if (i + j < i1) store1f<OIO>(out, i + j, load1f<IO>(g, i + j) * c);
 }
 
+// The same with a coefficient of 64 bits, for norms beyond fp32: rare, so element by element.
+__device__ __forceinline__ void chunk_scale64(int io, int out_io, const void* g, void* out, long long i0, long long i1, double c) {
+  for (long long i = i0 + threadIdx.x; i < i1; i += 256) {
+    const float f = io == IO_F32 ? load1f<IO_F32>(g, i) : io == IO_BF16 ? load1f<IO_BF16>(g, i) : load1f<IO_F16>(g, i);
+    const float v = (float)((double)f * c);
+    if (out_io == IO_F32) store1f<IO_F32>(out, i, v);
+    else if (out_io == IO_BF16) store1f<IO_BF16>(out, i, v);
+    else store1f<IO_F16>(out, i, v);
+  }
+}
+
 template <int IO>
 __device__ __forceinline__ void chunk_scale_to(int out_io, const void* g, void* out, long long i0, long long i1, float c) {
   if (out_io == IO_F32) chunk_scale<IO, IO_F32>(g, out, i0, i1, c);
@@ -170,13 +185,15 @@ __device__ __forceinline__ void chunk_scale_to(int out_io, const void* g, void* 
   else chunk_scale<IO, IO_F16>(g, out, i0, i1, c);
 }
 
-__global__ void __launch_bounds__(256) scale_kernel(ClipTable t, long long chunk, const float* coef) {
-  const float c = *coef;
+__global__ void __launch_bounds__(256) scale_kernel(ClipTable t, long long chunk, const double* coef) {
+  const double c64 = *coef;
+  const float c = (float)c64;
   const int k = tensor_of(t, blockIdx.x);
   if (c == 1.f && t.grad[k] == t.out[k]) return;  // in place and within the limit: the values stay
   const long long i0 = (long long)(blockIdx.x - t.first[k]) * chunk;
   const long long i1 = min((long long)t.numel[k], i0 + chunk);
-  if (t.io[k] == IO_F32) chunk_scale_to<IO_F32>(t.out_io[k], t.grad[k], t.out[k], i0, i1, c);
+  if (c64 == c64 && (double)c != c64) chunk_scale64(t.io[k], t.out_io[k], t.grad[k], t.out[k], i0, i1, c64);
+  else if (t.io[k] == IO_F32) chunk_scale_to<IO_F32>(t.out_io[k], t.grad[k], t.out[k], i0, i1, c);
   else if (t.io[k] == IO_BF16) chunk_scale_to<IO_BF16>(t.out_io[k], t.grad[k], t.out[k], i0, i1, c);
   else chunk_scale_to<IO_F16>(t.out_io[k], t.grad[k], t.out[k], i0, i1, c);
 }
@@ -228,7 +245,7 @@ static hipError_t for_tables(int n, const ClipTensor* t, long long chunk, F f) {
 hipError_t launch_clip(int n, const ClipTensor* t, const ClipPlan& p, bool clip, float max_norm, float* norm, void* ws,
                        hipStream_t st) {
   double* part = (double*)ws;
-  float* coef = clip ? (float*)(part + p.blocks) : nullptr;
+  double* coef = clip ? part + p.blocks : nullptr;
   hipError_t e = for_tables(n, t, p.chunk, [&](const ClipTable& tab, long long blocks, long long done) {
     hipLaunchKernelGGL(norm_kernel, dim3((unsigned)blocks), dim3(256), 0, st, tab, p.chunk, part + done);
   });

@@ -344,7 +344,8 @@ int fmlp_join_bwd(const fmlp_join* call, void* workspace, size_t workspace_bytes
  * dense runs of numels[i] elements of dtypes[i] / out_dtypes[i] (fp16, bf16, fp32, each its own), aligned to
  * their elements; outs[i] == grads[i] of one dtype clips in place (and writes nothing where the norm is
  * within max_norm), an output that overlaps any other tensor of the call is refused (FMLP_ERR_INVALID_ARG). Squares are summed in 64 bits in a fixed order. A norm that
- * is infinite or NaN gives the coefficient 0 or NaN, as torch's clipping does. n = 0: the norm is 0. The
+ * is infinite or NaN because a gradient is gives the coefficient 0 or NaN, as torch's clipping does; a finite one beyond
+ * fp32 is stored as infinity, and clipped by. n = 0: the norm is 0. The
  * arrays are read on the host before the call returns. workspace: fmlp_clip_workspace_bytes, never NULL.
  */
 size_t fmlp_clip_workspace_bytes(int n, const int64_t* numels);
