@@ -26,7 +26,7 @@ from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 from .flashmlp import _DTYPES, _alloc_ws, _fast, _ptr
-from .gated import _not_traced, _On
+from .gated import _not_traced, _On, first_derivatives_only
 
 
 def _dense_cols(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -215,7 +215,7 @@ class BlockJoinFunction(torch.autograd.Function):
         return r2, y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_derivatives_only
     def backward(ctx, dr2, dy):
         r2, o, rs_o, rs_r, post_weight, gate, pre_weight = ctx.saved_tensors
         scale, post, eps, heads, dtype = ctx.args

@@ -18,10 +18,13 @@
 #include <c10/util/Exception.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
 #include <cstdint>
+#include <memory>
 #include <vector>
 
 #include "flashmlp.h"
@@ -263,9 +266,32 @@ void check_status(int st, const char* what) {
   if (st != FMLP_OK) raise_status(st, what);
 }
 
-// a second derivative would need these backward passes to be differentiable
-void check_once() {
-  TORCH_CHECK(!at::GradMode::is_enabled(), "FlashMLP's gradients cannot be differentiated again (create_graph=True)");
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// A second derivative would need these backward passes to be differentiable. Under create_graph=True the gradients of
+// `run`, made from the tensors `of`, are returned with a node that raises once it is differentiated (flashmlp_amd/gated.py's
+// first_derivatives_only).
+template <typename F>
+variable_list once(const variable_list& of, F run) {
+  const bool graph = at::GradMode::is_enabled();
+  variable_list g;
+  {
+    at::AutoGradMode off(false);
+    g = run();
+  }
+  if (!graph || !torch::autograd::any_variable_requires_grad(of)) return g;
+  const auto node = std::make_shared<torch::autograd::Error>("FlashMLP's gradients cannot be differentiated again",
+                                                             torch::autograd::collect_next_edges(of));
+  for (const at::Tensor& t : g)
+    if (t.defined()) torch::autograd::set_history(t, node);
+  return g;
+}
+// the incoming gradients and the saved tensors of a node
+variable_list joined(const variable_list& a, const variable_list& b) {
+  variable_list r(a);
+  r.insert(r.end(), b.begin(), b.end());
+  return r;
 }
 
 // x (0), weights (1 .. 3) and dout (4) as the kernels read them in place
@@ -331,9 +357,6 @@ std::vector<at::Tensor> gated_bwd_run(const at::Tensor& x, const at::Tensor& wg,
   return g;
 }
 
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
 struct GatedFn : torch::autograd::Function<GatedFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
                             const at::Tensor& w2, int64_t code, int64_t act) {
@@ -343,8 +366,10 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     return gated_fwd_run(x, wg, wu, w2, (int)code, (int)act);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    check_once();
     const auto s = ctx->get_saved_variables();
+    return once(joined(grads, s), [&] { return first(ctx, s, grads); });
+  }
+  static variable_list first(AutogradContext* ctx, const variable_list& s, const variable_list& grads) {
     const int code = (int)ctx->saved_data["code"].toInt(), act = (int)ctx->saved_data["act"].toInt();
     at::Tensor dout = grads[0];
     if (!dout.defined()) return variable_list(6);
@@ -382,8 +407,10 @@ struct SharedGatedFn : torch::autograd::Function<SharedGatedFn> {
     return head_sum(gated_fwd_run(every_head(x, H), wg, wu, w2, (int)code, (int)act, true), 1.f / (float)H, x);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    check_once();
     const auto s = ctx->get_saved_variables();
+    return once(joined(grads, s), [&] { return first(ctx, s, grads); });
+  }
+  static variable_list first(AutogradContext* ctx, const variable_list& s, const variable_list& grads) {
     const int code = (int)ctx->saved_data["code"].toInt(), act = (int)ctx->saved_data["act"].toInt();
     variable_list r(6);
     if (!grads[0].defined()) return r;
@@ -621,8 +648,10 @@ struct JoinFn : torch::autograd::Function<JoinFn> {
     return {r2, y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    check_once();
     const auto s = ctx->get_saved_variables();
+    return once(joined(grads, s), [&] { return first(ctx, s, grads); });
+  }
+  static variable_list first(AutogradContext* ctx, const variable_list& s, const variable_list& grads) {
     const bool with_o = s[1].defined();
     const JoinCfg c{ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["post"].toBool(),
                     ctx->saved_data["heads"].toInt(), (at::ScalarType)ctx->saved_data["dtype"].toInt()};

@@ -13,6 +13,7 @@ of libflashmlp.so asynchronously on torch's current stream of the tensors' devic
 """
 from __future__ import annotations
 
+import functools
 from typing import Tuple
 
 import numpy as np
@@ -149,6 +150,38 @@ def flashmlp_gated_bwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, w2: 
     return _bwd(x, wg, wu, w2, do, activation, need_dx, need_dw)
 
 
+class _NoSecond(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, n, *ts):
+        return ts[:n]
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("FlashMLP's gradients cannot be differentiated again")
+
+
+def first_derivatives_only(backward):
+    """A Function's backward that cannot be differentiated: under create_graph=True its gradients come with a node
+    between them and what they are made of that raises once it is. (torch's once_differentiable adds one where the
+    incoming gradients are differentiable, with no connection to the inputs: torch.autograd.grad goes past it, and
+    where the saved tensors alone are differentiable a second derivative is silently left out.)"""
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        of = [t for t in (*grads, *ctx.saved_tensors) if t is not None and t.requires_grad]
+        if not of:
+            return out
+        there = [t for t in out if t is not None]
+        marked = iter(_NoSecond.apply(len(there), *there, *of))
+        return tuple(t if t is None else next(marked) for t in out)
+
+    return run
+
+
 class GatedFlashMLPFunction(torch.autograd.Function):
     """Autograd binding of the gated MLP. Saves only (x, wg, wu, w2)."""
 
@@ -160,7 +193,7 @@ class GatedFlashMLPFunction(torch.autograd.Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_derivatives_only
     def backward(ctx, do):
         x, wg, wu, w2 = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -181,7 +214,7 @@ class _SharedGatedFunction(torch.autograd.Function):
         return _head_sum(o, 1.0 / H, x.dtype)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_derivatives_only
     def backward(ctx, do):
         x, wg, wu, w2 = ctx.saved_tensors
         H, need = wg.shape[0], ctx.needs_input_grad
