@@ -357,6 +357,23 @@ std::vector<at::Tensor> gated_bwd_run(const at::Tensor& x, const at::Tensor& wg,
   return g;
 }
 
+// A node's saved tensors may have been through hooks, which keep values, sizes and type but no layout: they are laid out
+// for the kernels again, and checked again.
+void laid_out(at::Tensor& t, bool fits) {
+  if (fits && !t.is_neg()) return;
+  t = t.resolve_neg().contiguous();
+  if ((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) != 0) t = t.clone(at::MemoryFormat::Contiguous);
+}
+// x (H, B, D), the weights and dout (H, B, D) of a backward pass
+void gated_laid_out(at::Tensor& x, variable_list& s, at::Tensor& dout, int code) {
+  laid_out(x, rows16(x));
+  for (int i = 1; i < 4; ++i) laid_out(s[i], dense16(s[i]));
+  laid_out(dout, rows16(dout));
+  const at::Tensor* ts[5] = {&x, &s[1], &s[2], &s[3], &dout};
+  int now = 0;
+  TORCH_CHECK(gated_ok(ts, 5, &now) && now == code, "a saved tensor of the gated MLP came back with another size, type or device");
+}
+
 struct GatedFn : torch::autograd::Function<GatedFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
                             const at::Tensor& w2, int64_t code, int64_t act) {
@@ -371,14 +388,12 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
   }
   static variable_list first(AutogradContext* ctx, const variable_list& s, const variable_list& grads) {
     const int code = (int)ctx->saved_data["code"].toInt(), act = (int)ctx->saved_data["act"].toInt();
-    at::Tensor dout = grads[0];
+    at::Tensor dout = grads[0], x = s[0];
     if (!dout.defined()) return variable_list(6);
-    if (!rows16(dout) || dout.is_neg()) {
-      dout = dout.resolve_neg().contiguous();
-      if (!dense16(dout)) dout = dout.clone(at::MemoryFormat::Contiguous);
-    }
+    variable_list w = s;
+    gated_laid_out(x, w, dout, code);
     const bool dw = ctx->needs_input_grad(1) || ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
-    auto g = gated_bwd_run(s[0], s[1], s[2], s[3], dout, code, act, ctx->needs_input_grad(0), dw);
+    auto g = gated_bwd_run(x, w[1], w[2], w[3], dout, code, act, ctx->needs_input_grad(0), dw);
     variable_list r(6);
     for (int i = 0; i < 4; ++i)
       if (ctx->needs_input_grad(i)) r[i] = g[i];
@@ -415,15 +430,15 @@ struct SharedGatedFn : torch::autograd::Function<SharedGatedFn> {
     variable_list r(6);
     if (!grads[0].defined()) return r;
     const int64_t H = s[1].size(0);
-    at::Tensor dout = every_head(grads[0], H);
-    if (!rows16(dout) || dout.is_neg()) {
-      at::Tensor d = grads[0].resolve_neg().contiguous();
-      if ((reinterpret_cast<uintptr_t>(d.data_ptr()) & 15u) != 0) d = d.clone(at::MemoryFormat::Contiguous);
-      dout = every_head(d, H);
-    }
+    at::Tensor d2 = grads[0], x2 = s[0];
+    laid_out(d2, rows16(every_head(d2, H)));
+    laid_out(x2, rows16(every_head(x2, H)));
+    at::Tensor dout = every_head(d2, H), x = every_head(x2, H);
+    variable_list w = s;
+    gated_laid_out(x, w, dout, code);
     const bool dw = ctx->needs_input_grad(1) || ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
     const float scale = 1.f / (float)H;
-    auto g = gated_bwd_run(every_head(s[0], H), s[1], s[2], s[3], dout, code, act, ctx->needs_input_grad(0), dw, true, scale);
+    auto g = gated_bwd_run(x, w[1], w[2], w[3], dout, code, act, ctx->needs_input_grad(0), dw, true, scale);
     if (ctx->needs_input_grad(0)) r[0] = head_sum(g[0], scale, s[0]);
     for (int i = 1; i < 4; ++i)
       if (ctx->needs_input_grad(i)) r[i] = g[i];
@@ -662,7 +677,17 @@ struct JoinFn : torch::autograd::Function<JoinFn> {
     const bool there[5] = {true, with_o, s[3].defined(), s[4].defined(), s[5].defined()};
     bool need[5];
     for (int i = 0, edge = 0; i < 5; ++i) need[i] = there[i] && ctx->needs_input_grad(edge++);
-    auto g = join_bwd_run(s[0], s[1], s[2], dr2, dy, s[3], s[4], s[5], c, need);
+    variable_list t = s;
+    t[0] = cols(t[0]);
+    t[1] = cols(t[1]);
+    for (int i = 2; i < 6; ++i)
+      if (t[i].defined()) t[i] = t[i].resolve_neg().contiguous();
+    const at::Tensor& rs = t[2];
+    TORCH_CHECK(join_ok(t[0], t[1], t[3], t[4], t[5], c) && rs.scalar_type() == at::kFloat && rs.device() == t[0].device() &&
+                    rs.dim() == 2 && rs.size(0) == 2 && rs.size(1) == t[0].size(0) &&
+                    (!dr2.defined() || dr2.sizes() == t[0].sizes()) && (!dy.defined() || dy.numel() == t[0].numel()),
+                "a saved tensor of the join came back with another size, type or device");
+    auto g = join_bwd_run(t[0], t[1], rs, dr2, dy, t[3], t[4], t[5], c, need);
     for (int i = 0; i < 5; ++i) r[i] = g[i];
     return r;
   }
