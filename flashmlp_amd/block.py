@@ -84,6 +84,16 @@ def _check_number(v, name):
         raise TypeError(f"{name} must be a number, got {type(v).__name__}")
 
 
+def _row_values(t, B, dev, name):
+    # the rows' 1 / rms as the kernels read them: one fp32 number a row, dense (None where no kernel does)
+    if t is None:
+        return None
+    assert t.shape == (B,), f"{name} must have one value per row"
+    if t.dtype != torch.float32 or t.device != dev:
+        raise TypeError(f"{name} must be float32 on {dev}, got {t.dtype} on {t.device}")
+    return t.resolve_neg().contiguous()
+
+
 def _call(B, H, D, groups, scale, eps, dtype, r_dtype, post) -> _lib.Join:
     j = _lib.Join()
     j.B, j.H, j.D, j.groups = B, H, D, groups
@@ -154,6 +164,7 @@ def _join_bwd(residual_out, o, rs_o, rs_r, dresidual, dy, post_weight, gate, sca
     from_r = residual is not None and o is not None and residual.dtype != torch.float32
     if from_r:
         residual_out = residual
+    assert residual_out is not None, "The stream behind the join is needed (or a 16-bit one before it as residual=)"
     dtype = (o.dtype if o is not None else dtype or residual_out.dtype)
     pre = dy is not None
     B, H, D, groups = _check_join(residual_out, o, post_weight, gate, pre_weight if pre else None, heads, dtype, post, pre)
@@ -163,6 +174,8 @@ def _join_bwd(residual_out, o, rs_o, rs_r, dresidual, dy, post_weight, gate, sca
             raise TypeError(f"the {what}'s gradient must be {dt} on {dev}, got {t.dtype} on {t.device}")
     assert dresidual is None or dresidual.shape == residual_out.shape, "Gradient shape mismatch"
     assert dy is None or tuple(dy.shape) in ((H, B, D), (B, C)) and (dy.dim() == 3 or H == 1), "Gradient shape mismatch"
+    rs_o = _row_values(rs_o if o is not None and post else None, B, dev, "rs_o")
+    rs_r = _row_values(rs_r if pre else None, B, dev, "rs_r")
     nr, no, npost, ngate, npre = _needs
 
     def new(shape, dt, want):
