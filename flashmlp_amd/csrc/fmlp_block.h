@@ -116,6 +116,7 @@ struct JoinArgs {
   void* dgate;
   void* dw_pre;
   long long B, C, D, groups, rows_per_gate;
+  long long row0;  // the forward launch's first row
   long long r_sr, dr_sr, o_sh, o_sr, y_sh, y_sr, do_sh, do_sr;  // element strides (y's: of dy in the backward)
   float scale, eps;
   int io;       // IoType of o, y, the weights and the gate

@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(MULTI ? 1024 : 256) join_fwd_kernel(JoinArgs a
   __shared__ float part[2][16];
   const int tpr = MULTI ? (int)blockDim.x : 64, t = MULTI ? (int)threadIdx.x : (int)(threadIdx.x & 63);
   const int nw = blockDim.x >> 6, C = (int)a.C;
-  const long long row = MULTI ? (long long)blockIdx.x : (long long)blockIdx.x * nw + (threadIdx.x >> 6);
+  const long long row = a.row0 + (MULTI ? (long long)blockIdx.x : (long long)blockIdx.x * nw + (threadIdx.x >> 6));
   if (row >= a.B) return;  // (a whole wave; MULTI workgroups never)
   const HeadRows ho{a.o_sh, a.o_sr, (int)a.D}, hy{a.y_sh, a.y_sr, (int)a.D};
   const float rc = 1.0f / (float)C;
@@ -523,10 +523,11 @@ RowShape row_shape(int64_t C) {
   return {vpt, true, (vecs + vpt * 64 - 1) / (vpt * 64) * 64};
 }
 
+// A launch holds fewer than 2^32 threads: rows beyond 2^31 threads' (2^25 rows of up to 1024 columns) take another.
+constexpr long long kLaunchThreads = 1LL << 31;
+
 template <int IO, int RIO>
-hipError_t fwd_t(const JoinArgs& a, hipStream_t st) {
-  const RowShape s = row_shape(a.C);
-  const long long grid = s.multi ? a.B : (a.B + 3) / 4;
+hipError_t fwd_launch(const JoinArgs& a, const RowShape& s, long long grid, hipStream_t st) {
   return by_shape(s.vpt, [&](auto V) {
     constexpr int VPT = decltype(V)::value;
     const dim3 g((unsigned)grid), b((unsigned)s.threads);
@@ -539,6 +540,19 @@ hipError_t fwd_t(const JoinArgs& a, hipStream_t st) {
     }
     return hipGetLastError();
   });
+}
+
+template <int IO, int RIO>
+hipError_t fwd_t(JoinArgs a, hipStream_t st) {
+  const RowShape s = row_shape(a.C);
+  const int per = s.multi ? 1 : 4;  // rows of a workgroup
+  const long long most = kLaunchThreads / s.threads;
+  for (a.row0 = 0; a.row0 < a.B; a.row0 += most * per) {
+    const long long left = (a.B - a.row0 + per - 1) / per;
+    const hipError_t e = fwd_launch<IO, RIO>(a, s, std::min(left, most), st);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 template <int IO, int RIO>
