@@ -46,7 +46,9 @@ hipError_t launch_head_sum(const float* src, void* dst, int64_t n, int64_t H, fl
 // 16-bit io on LDS-staged kernels (fmlp_gated_fwd.hip). Forms of the row kernels: nw waves of 32 rows in each of es
 // sets that take every chunk of a part of E, ns ring slots a set, oc waves per SIMD; nw = 0: no such form.
 // per_cu workgroups run at once on a CU. A workgroup takes fixed_us and, for a chunk of each set, chunk_us alone or
-// its share of full_us when the CU is full (the forward's measured times; dX takes about 1.4 times as long on each).
+// its share of full_us when the CU is full: the forward's measured times, dX's over the 1.4 that it takes as long on
+// most (dx; at D = 64 it runs two waves a SIMD where the forward runs three: H=16 E=2048 dX of 256 row tiles 54 us, of 512
+// 92, of 768 137).
 struct GatedForm {
   int nw, es, ns, oc, per_cu;
   double chunk_us, full_us, fixed_us;
@@ -55,12 +57,19 @@ constexpr GatedForm gated_form(int D, int form, bool dx) {
   if (D == 32)
     return form == 0 ? GatedForm{2, 1, 4, 3, 6, 0.35, 1.2, 4.5} : form == 2 ? GatedForm{1, 4, 4, 1, 1, 0.45, 0.5, 4} : GatedForm{};
   if (D == 64)
-    return form == 0 ? GatedForm{4, 1, 4, dx ? 2 : 3, 3, 0.5, 1.35, 4} : form == 2 ? GatedForm{2, 4, 3, 2, 1, 0.9, 0.95, 4} : GatedForm{};
+    return form == 0   ? dx ? GatedForm{4, 1, 4, 2, 2, 0.55, 0.94, 4} : GatedForm{4, 1, 4, 3, 3, 0.5, 1.35, 4}
+           : form == 2 ? GatedForm{2, 4, 3, 2, 1, 0.9, dx ? 1.1 : 0.95, 4}
+                       : GatedForm{};
   if (D == 128)
     return form == 0   ? GatedForm{8, 1, 4, 2, 1, 0.94, 1.45, 6}
            : form == 1 ? GatedForm{4, 2, 3, 2, 1, 1.1, 1.45, 6}
                        : GatedForm{2, 2, 3, 1, 1, 1.0, 1.16, 5};
   return form == 0 ? GatedForm{4, 1, 3, 1, 1, 1.3, 1.55, 4.2} : GatedForm{};
+}
+
+// per_cu workgroups fit the waves of the CU's four SIMDs, and its LDS
+constexpr bool gated_form_fits(int D, GatedForm f) {
+  return f.per_cu * f.nw * f.es <= 4 * f.oc && f.per_cu * f.es * f.ns * 192 * D <= 160 * 1024;
 }
 
 // `tiles` row tiles of a form, each split over xs workgroups of nct chunks of 32 columns, whose fp32 partials

@@ -268,6 +268,7 @@ struct Args {
 template <bool BF16, int D, int DG, int ACT, int FORM>
 hipError_t launch(const Args& q) {
   constexpr GatedForm F = gated_form(D, FORM, true);
+  static_assert(gated_form_fits(D, F), "the plan's workgroups a CU");
   constexpr int lds = F.es * F.ns * 192 * D;
   auto k = gated_dx_kernel<BF16, D, DG, ACT, F.nw, F.es, F.ns, F.oc>;
   static std::atomic<unsigned long long> done{0};

@@ -264,6 +264,7 @@ struct Args {
 template <bool BF16, int D, int DG, int ACT, int FORM>
 hipError_t launch(const Args& q) {
   constexpr GatedForm F = gated_form(D, FORM, false);
+  static_assert(gated_form_fits(D, F), "the plan's workgroups a CU");
   constexpr int lds = F.es * F.ns * 192 * D;
   auto k = gated_fwd_kernel<BF16, D, DG, ACT, F.nw, F.es, F.ns, F.oc>;
   static std::atomic<unsigned long long> done{0};
@@ -315,7 +316,7 @@ GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_
   GatedFwdPlan best{};
   double best_us = 0;
   for (int form = 0; form < 3; ++form) {
-    const GatedForm F = gated_form(DT, form, false);
+    const GatedForm F = gated_form(DT, form, dx);
     if (F.nw == 0) continue;
     const long long tiles = H * ((B + 32 * F.nw - 1) / (32 * F.nw));
     for (long long want = 1; want <= 16 && want <= nch; ++want) {
