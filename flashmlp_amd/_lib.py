@@ -73,6 +73,7 @@ SIGNATURES = {
                                 ctypes.c_int, _vp, ctypes.c_size_t, _vp]),
     "fmlp_bwd_strided": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64p, _i64p,
                                         _i64p, _i64p, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_size_t, _vp]),
+    "fmlp_gated_min_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, ctypes.c_int]),
     "fmlp_gated_fwd_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, ctypes.c_int]),
     "fmlp_gated_fwd": (ctypes.c_int, [_vp] * 5 + [_i64] * 5 + [ctypes.c_int, ctypes.c_int, _vp, ctypes.c_size_t, _vp]),
     "fmlp_gated_bwd_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, ctypes.c_int]),

@@ -80,7 +80,8 @@ struct GatedFwdPlan {
   int xs, nct;
   size_t ws_bytes;
 };
-GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus, bool dx);
+// (whole: no split and no partials, for calls whose workspace does not hold them; likewise below)
+GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus, bool dx, bool whole);
 hipError_t launch_gated_fwd(const GatedArgs& a, const GatedFwdPlan& p, hipStream_t st);
 // dX on the same forms and plan (fmlp_gated_dx.hip)
 hipError_t launch_gated_dx(const GatedArgs& a, const GatedFwdPlan& p, hipStream_t st);
@@ -92,13 +93,13 @@ struct GatedDwPlan {
   long long programs;
   size_t ws_bytes;
 };
-GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus);
+GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus, bool whole);
 hipError_t launch_gated_dw(const GatedArgs& a, const GatedDwPlan& p, hipStream_t st);
 hipError_t launch_gated_dw128(const GatedArgs& a, const GatedDwPlan& p, hipStream_t st);
 
 // fp32 io (fmlp_gated_f32.hip): tiles of 128 rows, E-tiles of 128 columns (32 at D = 256).
-GatedFwdPlan gated32_rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus);
-GatedDwPlan gated32_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus);
+GatedFwdPlan gated32_rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus, bool whole);
+GatedDwPlan gated32_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus, bool whole);
 hipError_t launch_gated32_fwd(const GatedArgs& a, const GatedFwdPlan& p, hipStream_t st);
 hipError_t launch_gated32_dx(const GatedArgs& a, const GatedFwdPlan& p, hipStream_t st);
 hipError_t launch_gated32_dw(const GatedArgs& a, const GatedDwPlan& p, hipStream_t st);

@@ -80,16 +80,31 @@ int check_ws(const void* ws, size_t have, size_t need) {
     return abi_fail(FMLP_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? have : (size_t)0, need);
   return FMLP_OK;
 }
-fmlp::GatedFwdPlan rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int io, int cus, bool dx) {
-  return io == FMLP_DTYPE_F32 ? fmlp::gated32_rows_plan(H, B, D, E, cus) : fmlp::gated_fwd_plan(H, B, D, E, cus, dx);
+fmlp::GatedFwdPlan rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int io, int cus, bool dx, bool whole = false) {
+  return io == FMLP_DTYPE_F32 ? fmlp::gated32_rows_plan(H, B, D, E, cus, whole)
+                              : fmlp::gated_fwd_plan(H, B, D, E, cus, dx, whole);
 }
-fmlp::GatedDwPlan dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int io, int cus) {
-  return io == FMLP_DTYPE_F32 ? fmlp::gated32_dw_plan(H, B, D, E, cus) : fmlp::gated_dw_plan(H, B, D, E, cus);
+fmlp::GatedDwPlan dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int io, int cus, bool whole = false) {
+  return io == FMLP_DTYPE_F32 ? fmlp::gated32_dw_plan(H, B, D, E, cus, whole) : fmlp::gated_dw_plan(H, B, D, E, cus, whole);
+}
+// the same for what is left of the workspace behind the padded weights: whole tiles where the partials do not fit
+fmlp::GatedFwdPlan rows_plan(const fmlp::GatedArgs& a, int io, bool dx) {
+  const fmlp::GatedFwdPlan p = rows_plan(a.H, a.B, a.D, a.E, io, a.num_cus, dx);
+  return p.ws_bytes <= a.ws_bytes ? p : rows_plan(a.H, a.B, a.D, a.E, io, a.num_cus, dx, true);
+}
+fmlp::GatedDwPlan dw_plan(const fmlp::GatedArgs& a, int io) {
+  const fmlp::GatedDwPlan p = dw_plan(a.H, a.B, a.D, a.E, io, a.num_cus);
+  return p.ws_bytes <= a.ws_bytes ? p : dw_plan(a.H, a.B, a.D, a.E, io, a.num_cus, true);
 }
 
 int io_type(int io) { return io == FMLP_DTYPE_F32 ? fmlp::IO_F32 : io == FMLP_DTYPE_BF16 ? fmlp::IO_BF16 : fmlp::IO_F16; }
 
 }  // namespace
+
+FMLP_EXPORT size_t fmlp_gated_min_workspace_bytes(int64_t H, int64_t D, int64_t E, int dtype) {
+  if (check_gated(H, 0, D, E, dtype, 0)) return 0;
+  return gated_pad_bytes(H, D, E, io_of(dtype));
+}
 
 FMLP_EXPORT size_t fmlp_gated_fwd_workspace_bytes(int64_t H, int64_t B, int64_t D, int64_t E, int dtype) {
   int cus = 0;
@@ -151,9 +166,9 @@ FMLP_EXPORT int fmlp_gated_fwd(const void* x, const void* wg, const void* wu, co
   a.ws_bytes = workspace != nullptr ? workspace_bytes : 0;
   if ((st = fmlp::abi_num_cus(&a.num_cus))) return st;
   const hipStream_t hs = (hipStream_t)stream;
-  const fmlp::GatedFwdPlan p = rows_plan(H, B, D, E, dtype, a.num_cus, false);
-  if ((st = check_ws(workspace, workspace_bytes, gated_pad_bytes(H, D, E, dtype) + p.ws_bytes))) return st;
+  if ((st = check_ws(workspace, workspace_bytes, gated_pad_bytes(H, D, E, dtype)))) return st;
   hipError_t e = gated_pad(&a, hs);
+  const fmlp::GatedFwdPlan p = rows_plan(a, dtype, false);
   if (e == hipSuccess) e = a.io == fmlp::IO_F32 ? fmlp::launch_gated32_fwd(a, p, hs) : fmlp::launch_gated_fwd(a, p, hs);
   if (e != hipSuccess) return abi_fail(FMLP_ERR_HIP, "gated forward launch: %s", hipGetErrorString(e));
   return abi_ok();
@@ -203,14 +218,14 @@ FMLP_EXPORT int fmlp_gated_bwd(const void* x, const void* wg, const void* wu, co
   const int io = io_of(dtype);
   hipError_t e = hipSuccess;
   if (want_dw || want_dx) {
-    if ((st = check_ws(workspace, workspace_bytes, gated_bwd_ws(H, B, D, E, dtype, a.num_cus)))) return st;
+    if ((st = check_ws(workspace, workspace_bytes, gated_pad_bytes(H, D, E, io)))) return st;
     e = gated_pad(&a, hs);
     if (e == hipSuccess && want_dw) {
-      const fmlp::GatedDwPlan p = dw_plan(H, B, D, E, io, a.num_cus);
+      const fmlp::GatedDwPlan p = dw_plan(a, io);
       e = a.io == fmlp::IO_F32 ? fmlp::launch_gated32_dw(a, p, hs) : fmlp::launch_gated_dw(a, p, hs);
     }
     if (e == hipSuccess && want_dx) {
-      const fmlp::GatedFwdPlan p = rows_plan(H, B, D, E, io, a.num_cus, true);
+      const fmlp::GatedFwdPlan p = rows_plan(a, io, true);
       e = a.io == fmlp::IO_F32 ? fmlp::launch_gated32_dx(a, p, hs) : fmlp::launch_gated_dx(a, p, hs);
     }
   }

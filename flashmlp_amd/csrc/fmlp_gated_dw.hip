@@ -709,7 +709,7 @@ hipError_t launch_gated_dw128(const GatedArgs& a, const GatedDwPlan& p, hipStrea
   return a.io == IO_BF16 ? by_d<true>(q) : by_d<false>(q);
 }
 #else
-GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus) {
+GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus, bool whole) {
   const int DT = D < 32 ? 32 : (int)D;
   const Form F = dw_form(DT);
   GatedDwPlan p{};
@@ -725,7 +725,7 @@ GatedDwPlan gated_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cu
   double best = 0;
   p.nS = 1;
   p.rows_per_split = (int)std::max<long long>(subs * 32, 32);
-  for (long long n = 1; n <= 64 && (n == 1 || n <= subs / 2); ++n) {
+  for (long long n = 1; n <= (whole ? 1 : 64) && (n == 1 || n <= subs / 2); ++n) {
     const long long per = (subs + n - 1) / n, m = per > 0 ? (subs + per - 1) / per : 1;
     if (m != n && n > 1) continue;
     const long long full = base * n / slots, rest = base * n % slots;

@@ -407,7 +407,7 @@ hipError_t by_d(const GatedArgs& a, F f) {
 
 // Tiles of 128 rows, split over E where whole tiles leave CUs idle or cut a last round short: the products of
 // the workgroups of a CU share its matrix units, so a round costs its chunks whether one or three run there.
-GatedFwdPlan gated32_rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus) {
+GatedFwdPlan gated32_rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus, bool whole) {
   const long long N = std::max(num_cus, 1), nch = (E + 31) / 32;
   GatedFwdPlan p{};
   p.xs = 1;
@@ -416,7 +416,7 @@ GatedFwdPlan gated32_rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int n
   if (p.tiles <= 0) return p;
   const double chunk_us = 3.4 * (double)std::max<long long>(D, 32) / 64.0;
   double best = 0;
-  for (long long want = 1; want <= 16 && want <= nch; ++want) {
+  for (long long want = 1; want <= (whole ? 1 : 16) && want <= nch; ++want) {
     const long long nct = (nch + want - 1) / want, xs = (nch + nct - 1) / nct;
     if (xs != want) continue;
     double t = (double)((p.tiles * xs + N - 1) / N) * (double)nct * chunk_us;
@@ -431,7 +431,7 @@ GatedFwdPlan gated32_rows_plan(int64_t H, int64_t B, int64_t D, int64_t E, int n
   return p;
 }
 
-GatedDwPlan gated32_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus) {
+GatedDwPlan gated32_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus, bool whole) {
   GatedDwPlan p{};
   const long long N = std::max(num_cus, 1), subs = (B + 31) / 32;
   p.nE = (int)(D == 256 ? (E + 31) / 32 : (E + 127) / 128);
@@ -440,7 +440,7 @@ GatedDwPlan gated32_dw_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_
   double best = 0;
   p.nS = 1;
   p.rows_per_split = (int)std::max<long long>(subs * 32, 32);
-  for (long long n = 1; n <= 32 && (n == 1 || n <= subs); ++n) {
+  for (long long n = 1; n <= (whole ? 1 : 32) && (n == 1 || n <= subs); ++n) {
     const long long per = std::max<long long>((subs + n - 1) / n, 1);
     if (n > 1 && (subs + per - 1) / per != n) continue;
     double t = (double)((base * n + N - 1) / N) * (4.0 + sub_us * (double)per);

@@ -310,7 +310,7 @@ hipError_t by_d(const Args& q) {
 
 }  // namespace
 
-GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus, bool dx) {
+GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_cus, bool dx, bool whole) {
   const int DT = D < 32 ? 32 : (int)D;
   const long long N = num_cus > 0 ? num_cus : 1, nch = (E + 31) / 32;
   GatedFwdPlan best{};
@@ -319,7 +319,7 @@ GatedFwdPlan gated_fwd_plan(int64_t H, int64_t B, int64_t D, int64_t E, int num_
     const GatedForm F = gated_form(DT, form, dx);
     if (F.nw == 0) continue;
     const long long tiles = H * ((B + 32 * F.nw - 1) / (32 * F.nw));
-    for (long long want = 1; want <= 16 && want <= nch; ++want) {
+    for (long long want = 1; want <= (whole ? 1 : 16) && want <= nch; ++want) {
       const long long nct = (nch + want - 1) / want, xs = (nch + nct - 1) / nct;
       if (xs != want) continue;
       // full rounds of F.per_cu workgroups a CU, and what is left; a split adds a launch and the partials' bytes

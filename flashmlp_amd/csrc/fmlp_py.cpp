@@ -314,16 +314,29 @@ bool gated_ok(const at::Tensor* const* ts, int n, int* code) {
   return n < 5 || ts[4]->sizes() == x.sizes();
 }
 
+// the call's workspace of n bytes; where it does not fit, the least that the call runs with (n is then that)
+at::Tensor gated_ws(const at::Tensor& x, size_t& n, int64_t H, int64_t D, int64_t E, int code) {
+  if (n == 0) return at::Tensor();
+  try {
+    return bytes_on(x, n);
+  } catch (const c10::OutOfMemoryError&) {
+    const size_t least = fmlp_gated_min_workspace_bytes(H, D, E, code);
+    if (least >= n) throw;
+    n = least;
+  }
+  return n ? bytes_on(x, n) : at::Tensor();
+}
+
 // (x may be one matrix for every head: its head stride is 0; out_f32: unrounded)
 at::Tensor gated_fwd_run(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& w2, int code,
                          int act, bool out_f32 = false) {
   const int64_t H = x.size(0), B = x.size(1), D = x.size(2), E = wg.size(2);
   c10::DeviceGuard guard(x.device());
   const hipStream_t stream = c10::hip::getCurrentHIPStream(x.device().index()).stream();
-  at::Tensor o = out_f32 ? at::empty(x.sizes(), x.options().dtype(at::kFloat)) : empty_dense(x), ws;
+  at::Tensor o = out_f32 ? at::empty(x.sizes(), x.options().dtype(at::kFloat)) : empty_dense(x);
   if (out_f32) code |= FMLP_OUT_F32;
-  const size_t n = fmlp_gated_fwd_workspace_bytes(H, B, D, E, code);
-  if (n) ws = bytes_on(x, n);
+  size_t n = fmlp_gated_fwd_workspace_bytes(H, B, D, E, code);
+  const at::Tensor ws = gated_ws(x, n, H, D, E, code);
   check_status(fmlp_gated_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), w2.data_ptr(), o.data_ptr(), H, B, D, E,
                               x.stride(0), code, act, n ? ws.data_ptr() : nullptr, n, stream),
                "gated forward");
@@ -346,9 +359,8 @@ std::vector<at::Tensor> gated_bwd_run(const at::Tensor& x, const at::Tensor& wg,
     g[3] = at::empty_like(w2);
   }
   const int flags = code | (need_dx ? 0 : FMLP_BWD_NO_DX) | (need_dw ? 0 : FMLP_BWD_NO_DW) | (out_f32 ? FMLP_OUT_F32 : 0);
-  at::Tensor ws;
-  const size_t n = fmlp_gated_bwd_workspace_bytes(H, B, D, E, flags);
-  if (n) ws = bytes_on(x, n);
+  size_t n = fmlp_gated_bwd_workspace_bytes(H, B, D, E, flags);
+  const at::Tensor ws = gated_ws(x, n, H, D, E, flags);
   auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
   check_status(fmlp_gated_bwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), w2.data_ptr(), dout.data_ptr(), ptr(g[0]),
                               ptr(g[1]), ptr(g[2]), ptr(g[3]), H, B, D, E, x.stride(0), dout.stride(0), flags, act, dw_scale,

@@ -59,6 +59,17 @@ class _On:
             torch.cuda.set_device(self.prev)
 
 
+def _workspace(L, n: int, H: int, D: int, E: int, dtype: int, device):
+    """(tensor or None, its size): the call's workspace; where it does not fit, the least the call runs with"""
+    try:
+        return _alloc_ws(n, device), n
+    except torch.OutOfMemoryError:
+        least = L.fmlp_gated_min_workspace_bytes(H, D, E, dtype)
+        if least >= n:
+            raise
+        return _alloc_ws(least, device), least
+
+
 def _fwd(x, wg, wu, w2, activation, out_f32=False):
     """the general path: views and bases that the kernels do not read are copied first"""
     H, B, D, E = _check(x, wg, wu, w2)
@@ -69,8 +80,7 @@ def _fwd(x, wg, wu, w2, activation, out_f32=False):
     with _On(x.get_device()) as stream:
         x = _rows(x)
         wg, wu, w2 = _dense_all(wg, wu, w2)
-        n = L.fmlp_gated_fwd_workspace_bytes(H, B, D, E, dtype)
-        ws = _alloc_ws(n, x.device)
+        ws, n = _workspace(L, L.fmlp_gated_fwd_workspace_bytes(H, B, D, E, dtype), H, D, E, dtype, x.device)
         st = L.fmlp_gated_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), w2.data_ptr(), o.data_ptr(), H, B, D, E,
                               x.stride(0), dtype, _act_code(activation), _ptr(ws), n, stream)
     _lib.check(st, "gated forward")
@@ -93,8 +103,7 @@ def _bwd(x, wg, wu, w2, do, activation, need_dx, need_dw, out_f32=False, dw_scal
     with _On(x.get_device()) as stream:
         x, do = _rows(x), _rows(do)
         wg, wu, w2 = _dense_all(wg, wu, w2)
-        n = L.fmlp_gated_bwd_workspace_bytes(H, B, D, E, dtype)
-        ws = _alloc_ws(n, x.device)
+        ws, n = _workspace(L, L.fmlp_gated_bwd_workspace_bytes(H, B, D, E, dtype), H, D, E, dtype, x.device)
         st = L.fmlp_gated_bwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), w2.data_ptr(), do.data_ptr(), _ptr(dx),
                               _ptr(dwg), _ptr(dwu), _ptr(dw2), H, B, D, E, x.stride(0), do.stride(0), dtype,
                               _act_code(activation), dw_scale, _ptr(ws), n, stream)

@@ -272,9 +272,12 @@ int fmlp_bwd_noalloc(const void* x, const void* w1, const void* w2, const void* 
  * also takes FMLP_BWD_NO_DX and FMLP_BWD_NO_DW. With FMLP_OUT_F32 o and dx are fp32 arrays of the unrounded sums (the
  * weight gradients keep the io dtype). dw_scale multiplies the weight gradients before their rounding (1 for the
  * gradients themselves). The workspace (16-byte aligned, scratch for the duration
- * of the call on `stream`) is at least *_workspace_bytes() for the same arguments, and may be NULL where
- * that is 0. Results do not depend on the workspace's content and are bitwise repeatable.
+ * of the call on `stream`) is *_workspace_bytes() for the same arguments; with less, but at least
+ * fmlp_gated_min_workspace_bytes() (the padded copies of wg and wu where E is no multiple of 16 bytes, else 0: NULL
+ * will do), the call runs its tiles whole instead of split over idle CUs. Results do not depend on the workspace's
+ * content and are bitwise repeatable with one size of it.
  */
+size_t fmlp_gated_min_workspace_bytes(int64_t H, int64_t D, int64_t E, int dtype);
 size_t fmlp_gated_fwd_workspace_bytes(int64_t H, int64_t B, int64_t D, int64_t E, int dtype);
 int fmlp_gated_fwd(const void* x, const void* wg, const void* wu, const void* w2, void* o, int64_t H, int64_t B,
                    int64_t D, int64_t E, int64_t x_head_stride, int dtype, int act, void* workspace,
