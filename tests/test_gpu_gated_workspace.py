@@ -69,7 +69,7 @@ def test_general_path(monkeypatch, H, B, D, E, dt, act):
 
 
 def test_fast_path(monkeypatch):
-    """a real allocation failure, under a limit with room for the outputs alone: the bits of the general path without a
+    """a real allocation failure, with room for the outputs alone: the bits of the general path without a
     workspace"""
     H, B, D, E = 16, 4096, 128, 512
     t = [v.cuda() for v in make(H, B, D, E, BF)]
@@ -91,10 +91,14 @@ def test_fast_path(monkeypatch):
     del split
     torch.cuda.synchronize()
     torch.cuda.empty_cache()
-    total = torch.cuda.get_device_properties(0).total_memory
-    allowed = torch.cuda.memory_reserved() + out + (20 << 20)
-    torch.cuda.set_per_process_memory_fraction(allowed / total)
+    # no memory beyond what is reserved, all of it taken but room for the outputs
+    room, hold = torch.empty(out + (12 << 20), dtype=torch.uint8, device="cuda"), []
+    torch.cuda.set_per_process_memory_fraction(torch.cuda.memory_reserved() / torch.cuda.get_device_properties(0).total_memory)
     try:
+        with pytest.raises(torch.OutOfMemoryError):
+            while True:
+                hold.append(torch.empty(2 << 20, dtype=torch.uint8, device="cuda"))
+        del room
         got = flashmlp_gated_bwd(*t, "silu")
         torch.cuda.synchronize()
     finally:
