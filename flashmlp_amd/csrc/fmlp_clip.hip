@@ -8,7 +8,8 @@
 // launch takes as many tensors as its arguments hold (kMaxTensors). Squares are summed in 64 bits: bf16
 // and fp32 gradients reach 1e38, whose squares 32 bits do not hold, and the 64-bit additions hide
 // behind the loads (32-bit squares measured the same). 302 M bf16 gradients into fp32: norm 114 us (5.3 TB/s), scaling
-// 355 (1.8 GB, 5.1 TB/s); non-temporal stores 490, the second pass in reverse order no gain. Partial sums go through the workspace and are added in a fixed order.
+// 355 (1.8 GB, 5.1 TB/s); non-temporal stores 490, the second pass in reverse order no gain. Partial sums go through the
+// workspace and are added in a fixed order. The coefficient is an fp32 number unless the norm is beyond fp32.
 #include <algorithm>
 #include <cfloat>
 

@@ -5,8 +5,9 @@
 // reads, the activations and the barriers fit beside the products without a schedule written down.
 //
 // H=12 B=1024 D=64 E=768 SiLU: forward 48 us, dX 71, weight gradients 93 (products 48-52 % of the cycles: 96 tiles and
-// 72 column tiles split to fill 256 CUs leave rounds uneven); D = 256 H=8 B=1024 E=512: 82, 211, 149 (dX holds X, dO
-// and its sums in registers and spills).
+// 72 column tiles split to fill 256 CUs leave rounds uneven); D = 128 H=8 B=1024 E=512: 49, 71, 95 (the weight
+// gradients spill 45 registers, 96 bytes a lane); D = 256, the same: 82, 211, 149 (dX holds X, dO and its sums in
+// registers and spills 224, 480 bytes a lane; chunks are single-buffered, as two do not fit the LDS).
 //
 // Product q of a contraction over d takes d = 2 q + g from lane half g; a contraction over the rows of a C tile
 // takes element i of it as it lies (row 8 (i / 4) + 4 g + i % 4).
