@@ -84,6 +84,15 @@ def _check_number(v, name):
         raise TypeError(f"{name} must be a number, got {type(v).__name__}")
 
 
+def _input(t):
+    # an input's address, None for one that is not there: what has no memory of its own (a wrapper around other tensors, a
+    # fake one) would pass for that
+    p = _ptr(t)
+    if p == 0 and t.numel() > 0:
+        raise TypeError(f"a tensor without memory of its own ({type(t).__name__}) cannot be read by the kernels")
+    return p
+
+
 def _row_values(t, B, dev, name):
     # the rows' 1 / rms as the kernels read them: one fp32 number a row, dense (None where no kernel does)
     if t is None:
@@ -130,7 +139,8 @@ def _join_fwd(residual, o, post_weight, gate, scale, pre_weight, post, pre, eps,
     r, oo = _dense_cols(residual), _dense_cols(o)
     ws = [_flat(w) for w in (post_weight, gate, pre_weight)]
     j = _call(B, H, D, groups, scale, eps, dtype, residual.dtype, post)
-    j.r, j.o, j.w_post, j.gate, j.w_pre, j.r_out, j.y = (_ptr(t) for t in (r, oo, *ws, r2, y))
+    j.r, j.o, j.w_post, j.gate, j.w_pre = (_input(t) for t in (r, oo, *ws))
+    j.r_out, j.y = _ptr(r2), _ptr(y)
     if rs is not None:
         j.rs_o, j.rs_r = rs[0].data_ptr(), rs[1].data_ptr()
     j.r_stride = r.stride(0)
@@ -192,9 +202,9 @@ def _join_bwd(residual_out, o, rs_o, rs_r, dresidual, dy, post_weight, gate, sca
     dres, dyy = _dense_cols(dresidual), _dense_cols(dy)
     ws_ = [_flat(w) for w in (post_weight, gate, pre_weight if pre else None)]
     j = _call(B, H, D, groups, scale, eps, dtype, residual_out.dtype, post)
-    j.r, j.r_out = (_ptr(r2), None) if from_r else (None, _ptr(r2))
-    j.o, j.w_post, j.gate, j.w_pre = (_ptr(t) for t in (oo, *ws_))
-    j.rs_o, j.rs_r, j.dr_out, j.dy = (_ptr(t) for t in (rs_o, rs_r, dres, dyy))
+    j.r, j.r_out = (_input(r2), None) if from_r else (None, _input(r2))
+    j.o, j.w_post, j.gate, j.w_pre = (_input(t) for t in (oo, *ws_))
+    j.rs_o, j.rs_r, j.dr_out, j.dy = (_input(t) for t in (rs_o, rs_r, dres, dyy))
     j.dr, j.d_o, j.dw_post, j.dgate, j.dw_pre = (_ptr(t) for t in (dr, d_o, dpost, dgate, dpre if pre else None))
     j.r_stride = r2.stride(0)
     if oo is not None:

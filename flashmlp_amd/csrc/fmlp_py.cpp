@@ -532,7 +532,13 @@ struct JoinCfg {
   at::ScalarType dtype;
 };
 
-const void* cptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+// (what has no memory of its own, a wrapper around other tensors, would pass for an input that is not there)
+const void* cptr(const at::Tensor& t) {
+  const void* p = t.defined() ? t.data_ptr() : nullptr;
+  TORCH_CHECK_TYPE(p != nullptr || !t.defined() || t.numel() == 0,
+                   "a tensor without memory of its own cannot be read by the kernels");
+  return p;
+}
 void* mptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void head_strides(const at::Tensor& t, int64_t* sh, int64_t* sr) {
   *sh = t.dim() == 3 ? t.stride(0) : 0;
@@ -570,6 +576,8 @@ bool join_ok(const at::Tensor& r, const at::Tensor& o, const at::Tensor& w_post,
   if (c.dtype != at::kHalf && c.dtype != at::kBFloat16 && c.dtype != at::kFloat) return false;
   if (r.scalar_type() != c.dtype && r.scalar_type() != at::kFloat) return false;
   const int64_t B = r.size(0), C = r.size(1);
+  for (const at::Tensor* t : {&r, &o, &w_post, &gate, &w_pre})
+    if (t->defined() && t->numel() > 0 && t->data_ptr() == nullptr) return false;  // (the general path refuses it)
   for (const at::Tensor* t : {&o, &w_post, &gate, &w_pre})
     if (t->defined() && (t->scalar_type() != c.dtype || t->device() != r.device() || t->layout() != at::kStrided || t->is_neg()))
       return false;
