@@ -87,6 +87,12 @@ SIGNATURES = {
     "fmlp_grad_norm": (ctypes.c_int, [ctypes.c_int, _vpp, _i64p, _intp, _vp, _vp, ctypes.c_size_t, _vp]),
     "fmlp_clip_grads": (ctypes.c_int, [ctypes.c_int, _vpp, _vpp, _i64p, _intp, _intp, ctypes.c_float, _vp, _vp,
                                        ctypes.c_size_t, _vp]),
+    "fmlp_route_fwd": (ctypes.c_int, [_vp] * 3 + [_i64] * 4 + [ctypes.c_int, ctypes.c_int, _vp]),
+    "fmlp_route_bwd": (ctypes.c_int, [_vp] * 5 + [_i64] * 4 + [ctypes.c_int, ctypes.c_int, _vp]),
+    "fmlp_expert_plan_workspace_bytes": (ctypes.c_size_t, [_i64] * 3),
+    "fmlp_expert_plan": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp] + [_i64] * 4 + [_vp, ctypes.c_size_t, _vp]),
+    "fmlp_expert_scatter": (ctypes.c_int, [_vp, _i64] + [_vp] * 6 + [_i64] * 5 + [ctypes.c_int, _vp]),
+    "fmlp_expert_gather": (ctypes.c_int, [_vp] * 4 + [_i64] * 5 + [ctypes.c_int, _vp]),
     "fmlp_bwd_noalloc": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_int,
                                         ctypes.c_int, _vp]),
 }

@@ -1,0 +1,330 @@
+// Tokens sorted by expert and back, for gfx950.
+//
+//   plan:     assignment i = t k + j of token t has its expert's position p = number of earlier assignments to the same
+//             expert, and the slot e capacity + p, or -1 where p >= capacity or its expert is out of [0, N)
+//   scatter:  rows[slot(t, j)] = w(t, j) x(t), zeros behind an expert's last row; dw(t, j) = <rows_in[slot(t, j)], x(t)>
+//   gather:   o(t) = sum over j of w(t, j) rows[slot(t, j)], in fp32 in the order of j, rounded once
+//
+// The plan is a stable counting sort: positions follow the tokens' order whatever the workgroups' order. Chunks of
+// assignments are counted first; then each chunk adds what the chunks before it have of every expert, its waves' counts
+// follow one another, and a wave's 64 assignments find those of their own expert by one ballot for each bit of it.
+//
+// The copies are bound by HBM. A token has a group of lanes, 16 bytes a lane; it is read once and written to its k rows (dispatch), so
+// that no inverse map is needed: what is left of an expert's capacity is filled with zeros by workgroups of their own.
+#include <algorithm>
+
+#include "fmlp_experts.h"
+#include "fmlp_vec.h"
+
+namespace fmlp {
+namespace {
+
+// ---------------------------------------------------------------------------------------------
+// plan
+// ---------------------------------------------------------------------------------------------
+constexpr int kItems = 16;  // assignments of a lane
+
+template <bool WIDE>
+__device__ __forceinline__ int expert_at(const void* experts, long long i, int N) {
+  if constexpr (WIDE) {
+    const long long e = ((const long long*)experts)[i];
+    return e >= 0 && e < N ? (int)e : -1;
+  } else {
+    const int e = ((const int*)experts)[i];
+    return e >= 0 && e < N ? e : -1;
+  }
+}
+
+template <bool WIDE>
+__global__ void __launch_bounds__(256) plan_count_kernel(const void* experts, long long M, int N, int* hist) {
+  extern __shared__ int plan_lds[];
+  for (int e = threadIdx.x; e < N; e += 256) plan_lds[e] = 0;
+  __syncthreads();
+  const long long i0 = (long long)blockIdx.x * (256 * kItems);
+#pragma unroll
+  for (int u = 0; u < kItems; ++u) {
+    const long long i = i0 + u * 256 + threadIdx.x;
+    const int e = i < M ? expert_at<WIDE>(experts, i, N) : -1;
+    if (e >= 0) atomicAdd(&plan_lds[e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < N; e += 256) hist[(long long)blockIdx.x * N + e] = plan_lds[e];
+}
+
+// THREADS * kItems assignments of workgroup blockIdx.x; hist: every chunk's counts, null for one chunk
+template <bool WIDE, int THREADS>
+__global__ void __launch_bounds__(THREADS) plan_kernel(const void* experts, long long M, int N, int bits, long long capacity,
+                                                       int* slots, int* counts, const int* hist) {
+  extern __shared__ int plan_lds[];  // [waves][N]: the wave's counts, then its next position of each expert
+  constexpr int W = THREADS / 64;
+  const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63;
+  for (int e = threadIdx.x; e < W * N; e += THREADS) plan_lds[e] = 0;
+  __syncthreads();
+  int* mine = plan_lds + wave * N;
+  const long long i0 = ((long long)blockIdx.x * W + wave) * (64 * kItems) + lane;
+  int ex[kItems];
+#pragma unroll
+  for (int u = 0; u < kItems; ++u) {
+    const long long i = i0 + u * 64;
+    ex[u] = i < M ? expert_at<WIDE>(experts, i, N) : -1;
+    if (ex[u] >= 0) atomicAdd(&mine[ex[u]], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < N; e += THREADS) {
+    int at = 0;
+    if (hist != nullptr)
+      for (unsigned c = 0; c < blockIdx.x; ++c) at += hist[(long long)c * N + e];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const int n = plan_lds[w * N + e];
+      plan_lds[w * N + e] = at;
+      at += n;
+    }
+    if (blockIdx.x + 1 == gridDim.x) counts[e] = at;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kItems; ++u) {
+    const int e = ex[u];
+    unsigned long long same = __ballot(e >= 0);
+    for (int b = 0; b < bits; ++b) {
+      const unsigned long long v = __ballot((e >> b) & 1);
+      same &= (e >> b) & 1 ? v : ~v;
+    }
+    const long long i = i0 + u * 64;
+    const int before = __popcll(same & ((1ull << lane) - 1));
+    int base = 0;
+    if (e >= 0) {
+      base = mine[e];
+      // (the wave's lanes have all read before the last one of each expert writes: one wave's LDS operations keep
+      // their order)
+      asm volatile("" ::: "memory");
+      if ((same >> lane) == 1) mine[e] = base + before + 1;
+    }
+    asm volatile("" ::: "memory");
+    if (i < M) {
+      const long long p = (long long)base + before;
+      slots[i] = e >= 0 && p < capacity ? (int)(e * capacity + p) : -1;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// copies
+// ---------------------------------------------------------------------------------------------
+constexpr int kFillBytes = 65536;  // of a workgroup that fills with zeros
+
+// Zeros behind expert e's rows, in chunk c of `chunk` rows.
+template <int IO>
+__device__ __forceinline__ void fill_rows(const ExpertCopyArgs& a, long long e, long long r0, long long chunk) {
+  const long long r1 = min(a.capacity, r0 + chunk);
+  const long long from = max(r0, (long long)max(a.counts[e], 0));
+  if (from >= r1) return;
+  constexpr int E = kPiece<IO>;
+  const long long i1 = (e * a.capacity + r1) * a.D;
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  for (long long i = (e * a.capacity + from) * a.D + threadIdx.x * E; i < i1; i += 256 * E)
+    store_piece<IO>(a.rows_out, i, i1 - i < E ? (int)(i1 - i) : E, zero);
+}
+
+// KB: choices of a token in flight; 1 << lg lanes a token. rows_out and dweights may each be null.
+template <int IO, int KB, bool W, bool DOT>
+__global__ void __launch_bounds__(256) scatter_kernel(ExpertCopyArgs a, int lg, unsigned fill_blocks, unsigned fill_chunks,
+                                                      long long fill_rows_each) {
+  if (blockIdx.x < fill_blocks) {
+    fill_rows<IO>(a, blockIdx.x / fill_chunks, (long long)(blockIdx.x % fill_chunks) * fill_rows_each, fill_rows_each);
+    return;
+  }
+  constexpr int E = kPiece<IO>;
+  const int L = 1 << lg, lane = (int)threadIdx.x & (L - 1);
+  const long long t = (long long)(blockIdx.x - fill_blocks) * (256 >> lg) + (threadIdx.x >> lg);
+  const bool there = t < a.T;
+  const long long x0 = there ? t * a.stride : 0, n_rows = a.N * a.capacity;
+  const int D = (int)a.D, k = a.k;
+  for (int j0 = 0; j0 < k; j0 += KB) {
+    int slot[KB];
+    float w[KB], dot[KB];
+#pragma unroll
+    for (int j = 0; j < KB; ++j) {
+      slot[j] = there && j0 + j < k ? a.slots[t * k + j0 + j] : -1;
+      if (slot[j] >= n_rows) slot[j] = -1;
+      if constexpr (W) w[j] = slot[j] >= 0 ? a.weights[t * k + j0 + j] : 0.f;
+      dot[j] = 0.f;
+    }
+    for (int d = lane * E; d < D; d += L * E) {
+      const int n = there ? D - d : 0;
+      const u32x4 v = load_piece<IO>(a.x, x0 + d, n);
+      float f[E];
+      if constexpr (W || DOT) unpack_piece<IO>(v, f);
+      if constexpr (DOT) {
+        u32x4 r[KB];
+#pragma unroll
+        for (int j = 0; j < KB; ++j)
+          r[j] = load_piece<IO>(a.rows_in, slot[j] >= 0 ? (long long)slot[j] * D + d : 0, slot[j] >= 0 ? n : 0);
+#pragma unroll
+        for (int j = 0; j < KB; ++j) {
+          float q[E];
+          unpack_piece<IO>(r[j], q);
+#pragma unroll
+          for (int i = 0; i < E; ++i) dot[j] = __builtin_fmaf(q[i], f[i], dot[j]);
+        }
+      }
+      if (!DOT || a.rows_out != nullptr) {
+#pragma unroll
+        for (int j = 0; j < KB; ++j) {
+          if (slot[j] < 0) continue;
+          if constexpr (W) {
+            float q[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) q[i] = w[j] * f[i];
+            store_piece<IO>(a.rows_out, (long long)slot[j] * D + d, n, pack_piece<IO>(q));
+          } else {
+            store_piece<IO>(a.rows_out, (long long)slot[j] * D + d, n, v);
+          }
+        }
+      }
+    }
+    if constexpr (DOT) {
+#pragma unroll
+      for (int j = 0; j < KB; ++j)
+        for (int s = 1; s < L; s <<= 1) dot[j] += __shfl_xor(dot[j], s, 64);
+      if (there && lane == 0)
+#pragma unroll
+        for (int j = 0; j < KB; ++j)
+          if (j0 + j < k) a.dweights[t * k + j0 + j] = slot[j] >= 0 ? dot[j] : 0.f;  // (0 infinity is no 0)
+    }
+  }
+}
+
+template <int IO, int KB, bool W>
+__global__ void __launch_bounds__(256) gather_kernel(ExpertCopyArgs a, int lg) {
+  constexpr int E = kPiece<IO>;
+  const int L = 1 << lg, lane = (int)threadIdx.x & (L - 1);
+  const long long t = (long long)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
+  if (t >= a.T) return;
+  const long long n_rows = a.N * a.capacity;
+  const int D = (int)a.D, k = a.k;
+  for (int d = lane * E; d < D; d += L * E) {
+    float acc[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[i] = 0.f;
+    for (int j0 = 0; j0 < k; j0 += KB) {
+      u32x4 r[KB];
+      float w[KB];
+#pragma unroll
+      for (int j = 0; j < KB; ++j) {
+        const int slot = j0 + j < k ? a.slots[t * k + j0 + j] : -1;
+        const bool in = slot >= 0 && slot < n_rows;
+        w[j] = !in ? 0.f : W ? a.weights[t * k + j0 + j] : 1.f;
+        r[j] = load_piece<IO>(a.rows_in, in ? (long long)slot * D + d : 0, in ? D - d : 0);
+      }
+#pragma unroll
+      for (int j = 0; j < KB; ++j) {
+        float q[E];
+        unpack_piece<IO>(r[j], q);
+#pragma unroll
+        for (int i = 0; i < E; ++i) acc[i] = W ? __builtin_fmaf(w[j], q[i], acc[i]) : acc[i] + q[i];
+      }
+    }
+    store_piece<IO>(a.o, t * D + d, D - d, pack_piece<IO>(acc));
+  }
+}
+
+// lanes of a token: its 16-byte pieces up to a wave
+int lanes_log2(long long D, int io) {
+  const long long e = io == IO_F32 ? 4 : 8;
+  int lg = 0;
+  while (lg < 6 && (e << lg) < D) ++lg;
+  return lg;
+}
+
+template <typename F>
+void by_io(int io, F f) {
+  if (io == IO_F32) f(std::integral_constant<int, IO_F32>{});
+  else if (io == IO_BF16) f(std::integral_constant<int, IO_BF16>{});
+  else f(std::integral_constant<int, IO_F16>{});
+}
+template <typename F>
+void by_choices(int k, F f) {
+  if (k == 1) f(std::integral_constant<int, 1>{});
+  else if (k == 2) f(std::integral_constant<int, 2>{});
+  else f(std::integral_constant<int, 4>{});
+}
+
+}  // namespace
+
+ExpertPlan expert_plan(int64_t M, int64_t N, int num_cus) {
+  (void)num_cus;
+  ExpertPlan p{};
+  // one workgroup of up to 16 waves does all where its lanes' items suffice: no second launch
+  p.threads = M <= 256 * kItems || M > 1024 * kItems ? 256 : 1024;
+  p.chunk = (long long)p.threads * kItems;
+  p.chunks = M > 0 ? (M + p.chunk - 1) / p.chunk : 1;
+  p.ws_bytes = p.chunks > 1 ? (size_t)(p.chunks * N) * sizeof(int) : 0;
+  return p;
+}
+
+hipError_t launch_expert_plan(const void* experts, bool wide, long long M, int N, long long capacity, int32_t* slots,
+                              int32_t* counts, const ExpertPlan& p, void* ws, hipStream_t st) {
+  int bits = 0;
+  while ((1 << bits) < N) ++bits;
+  int* hist = p.chunks > 1 ? (int*)ws : nullptr;
+  const dim3 grid((unsigned)p.chunks);
+  hipError_t e = hipSuccess;
+  const auto run = [&](auto WIDE) {
+    constexpr bool V = decltype(WIDE)::value;
+    if (hist != nullptr) {
+      hipLaunchKernelGGL((plan_count_kernel<V>), grid, dim3(256), (size_t)N * 4, st, experts, M, N, hist);
+      if ((e = hipGetLastError()) != hipSuccess) return;
+    }
+    const size_t lds = (size_t)p.threads / 64 * N * 4;
+    if (p.threads == 1024)
+      hipLaunchKernelGGL((plan_kernel<V, 1024>), grid, dim3(1024), lds, st, experts, M, N, bits, capacity, slots, counts, hist);
+    else
+      hipLaunchKernelGGL((plan_kernel<V, 256>), grid, dim3(256), lds, st, experts, M, N, bits, capacity, slots, counts, hist);
+    e = hipGetLastError();
+  };
+  if (wide) run(std::true_type{});
+  else run(std::false_type{});
+  return e;
+}
+
+hipError_t launch_expert_scatter(const ExpertCopyArgs& a, hipStream_t st) {
+  const int lg = lanes_log2(a.D, a.io);
+  const long long per = 256 >> lg, blocks = (a.T + per - 1) / per;
+  const long long row_bytes = a.D * (a.io == IO_F32 ? 4 : 2);
+  const long long chunk = std::max(1LL, kFillBytes / row_bytes);
+  const long long chunks = a.rows_out != nullptr ? (a.capacity + chunk - 1) / chunk : 0, fill = chunks * a.N;
+  if (blocks + fill > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (blocks + fill == 0) return hipSuccess;
+  const dim3 grid((unsigned)(blocks + fill));
+  by_io(a.io, [&](auto IO) {
+    by_choices(a.k, [&](auto KB) {
+      constexpr int I = decltype(IO)::value, K = decltype(KB)::value;
+      const auto go = [&](auto k) {
+        hipLaunchKernelGGL(k, grid, dim3(256), 0, st, a, lg, (unsigned)fill, (unsigned)std::max(chunks, 1LL), chunk);
+      };
+      if (a.dweights != nullptr) a.weights ? go(scatter_kernel<I, K, true, true>) : go(scatter_kernel<I, K, false, true>);
+      else a.weights ? go(scatter_kernel<I, K, true, false>) : go(scatter_kernel<I, K, false, false>);
+    });
+  });
+  return hipGetLastError();
+}
+
+hipError_t launch_expert_gather(const ExpertCopyArgs& a, hipStream_t st) {
+  const int lg = lanes_log2(a.D, a.io);
+  const long long per = 256 >> lg, blocks = (a.T + per - 1) / per;
+  if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (blocks == 0) return hipSuccess;
+  const dim3 grid((unsigned)blocks);
+  by_io(a.io, [&](auto IO) {
+    by_choices(a.k, [&](auto KB) {
+      constexpr int I = decltype(IO)::value, K = decltype(KB)::value;
+      if (a.weights) hipLaunchKernelGGL((gather_kernel<I, K, true>), grid, dim3(256), 0, st, a, lg);
+      else hipLaunchKernelGGL((gather_kernel<I, K, false>), grid, dim3(256), 0, st, a, lg);
+    });
+  });
+  return hipGetLastError();
+}
+
+}  // namespace fmlp

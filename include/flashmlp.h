@@ -43,7 +43,7 @@ extern "C" {
                               there changes; added within 4, with no change to the others:
                               fmlp_shape_dense, fmlp_fwd_strided_ws, fmlp_copy_dense, the
                               fmlp_gated_*, fmlp_join_* and fmlp_clip_* calls, fmlp_head_sum,
-                              fmlp_grad_norm */
+                              fmlp_grad_norm, the fmlp_route_* and fmlp_expert_* calls */
 
 typedef enum {
   FMLP_OK = 0,
@@ -357,6 +357,44 @@ int fmlp_grad_norm(int n, const void* const* grads, const int64_t* numels, const
 int fmlp_clip_grads(int n, const void* const* grads, void* const* outs, const int64_t* numels, const int* dtypes,
                     const int* out_dtypes, float max_norm, float* norm, void* workspace, size_t workspace_bytes,
                     void* stream);
+
+/*
+ * Routing: each token's k of N experts, those with the largest logits (ties: the lowest index), in falling order, and
+ * their weights: softmax(logits) of them, or with `normalize` that over its sum over the k. No counterpart in the
+ * reference. logits (T, N) of dtype, rows row_stride elements apart; weights (T, k) fp32 and experts (T, k) dense.
+ * A logit of -infinity is a masked expert, which is never chosen: a token with fewer than k others has -1 with the weight
+ * 0 in place of the rest. NaN counts as the largest; a row that holds NaN or +infinity has NaN weights. Backward: dlogits (T, N) dense,
+ * from what the forward gave and the weights' gradient; logits are read without `normalize` only (NULL with it).
+ * N <= 1024, k <= 32.
+ */
+int fmlp_route_fwd(const void* logits, float* weights, int32_t* experts, int64_t T, int64_t N, int64_t row_stride, int64_t k,
+                   int normalize, int dtype, void* stream);
+int fmlp_route_bwd(const void* logits, const float* weights, const int32_t* experts, const float* dweights, void* dlogits,
+                   int64_t T, int64_t N, int64_t row_stride, int64_t k, int normalize, int dtype, void* stream);
+
+/*
+ * Tokens sorted by expert: slots[t][j] is the row, among N experts of `capacity` rows each, of token t's j-th choice
+ * experts[t][j] (int32, or int64 with index_bytes 8): the choices of an expert have its rows in their order (t, j); -1 where
+ * its rows are used up, and where experts[t][j] is outside [0, N) (-1: no choice). counts[e] is the number of
+ * choices of expert e, dropped ones too. Dense tensors; counts (N) is written for T = 0 too. workspace: scratch of
+ * fmlp_expert_plan_workspace_bytes(). N <= 1024, k <= 32, T k and N capacity < 2^31. No counterpart in the reference.
+ *
+ * fmlp_expert_scatter, for each (t, j) with a slot: rows_out[slot] = weights[t][j] * x[t] (weights NULL: x[t]), the rows behind
+ * an expert's last one are zeros; dweights[t][j] = the dot product of rows_in[slot] and x[t] (0 without a slot). rows_out or dweights may be
+ * NULL. x: rows x_row_stride elements apart; rows (N, capacity, D), weights and dweights (T, k) fp32 dense. This is the copy of
+ * tokens to their experts, and the backward of fmlp_expert_gather (x its output's gradient).
+ * fmlp_expert_gather: o[t] = sum over j of weights[t][j] * rows[slot], summed in fp32 in the order of j (dropped choices left out);
+ * the way back, and with weights NULL the backward of the copy. slots and counts are those of one fmlp_expert_plan
+ * call: no slot is there twice. Slots out of range count as -1. Any alignment, any D < 2^24. rows_out must not overlap an input.
+ */
+size_t fmlp_expert_plan_workspace_bytes(int64_t T, int64_t k, int64_t N);
+int fmlp_expert_plan(const void* experts, int index_bytes, int32_t* slots, int32_t* counts, int64_t T, int64_t k, int64_t N,
+                     int64_t capacity, void* workspace, size_t workspace_bytes, void* stream);
+int fmlp_expert_scatter(const void* x, int64_t x_row_stride, const float* weights, const int32_t* slots, const int32_t* counts,
+                        const void* rows_in, void* rows_out, float* dweights, int64_t T, int64_t k, int64_t N,
+                        int64_t capacity, int64_t D, int dtype, void* stream);
+int fmlp_expert_gather(const void* rows, const float* weights, const int32_t* slots, void* o, int64_t T, int64_t k, int64_t N,
+                       int64_t capacity, int64_t D, int dtype, void* stream);
 
 #ifdef __cplusplus
 }
