@@ -13,7 +13,8 @@ A gated block built around it has the gated form  O = (act(X Wg) * (X Wu)) W2  (
 flashmlp_gated_bwd, GatedFlashMLPFunction, GatedFlashMLP), the norms, gate and residual
 around it (block_norm, block_join) and the clipping of its gradients (grad_norm, clip_grads,
 clip_grad_norm_). Its heads serve as experts that tokens choose (expert_route, expert_plan, expert_dispatch,
-expert_combine, GatedExperts).
+expert_combine, GatedExperts), and its stacks of weights are orthogonalised and stepped by orthogonalize and
+muon_step.
 """
 from .flashmlp import FlashMLP, FlashMLPFunction, flashmlp_bwd, flashmlp_fwd
 from .baseline import PyTorchMLP, flashmlp_torch_bwd, flashmlp_torch_fwd
@@ -21,6 +22,7 @@ from .gated import GatedFlashMLP, GatedFlashMLPFunction, flashmlp_gated_bwd, fla
 from .block import BlockJoinFunction, block_join, block_join_bwd, block_join_fwd, block_norm
 from .clip import clip_grad_norm_, clip_grads, grad_norm
 from .experts import ExpertPlan, GatedExperts, expert_combine, expert_dispatch, expert_plan, expert_route
+from .muon import muon_step, orthogonalize
 from . import ops
 from .ops import flashmlp
 
@@ -52,4 +54,6 @@ __all__ = [
     "expert_dispatch",
     "expert_combine",
     "GatedExperts",
+    "orthogonalize",
+    "muon_step",
 ]

@@ -42,12 +42,19 @@ class Join(ctypes.Structure):
            ("post", ctypes.c_int)])
 
 
+class MuonTensor(ctypes.Structure):
+    """fmlp_muon_tensor of include/flashmlp.h"""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("w", "g", "m")] + [(n, ctypes.c_int64) for n in ("H", "R", "C")]
+                + [(n, ctypes.c_int) for n in ("w_dtype", "g_dtype", "m_dtype")] + [("scale", ctypes.c_float)])
+
+
 # (name, restype, argtypes) for every symbol include/flashmlp.h declares
 _i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
 _i64p = ctypes.POINTER(ctypes.c_int64)
 _vpp = ctypes.POINTER(_vp)
 _intp = ctypes.POINTER(ctypes.c_int)
+_f32p = ctypes.POINTER(ctypes.c_float)
 SIGNATURES = {
     "fmlp_abi_version": (ctypes.c_int, []),
     "fmlp_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -93,6 +100,13 @@ SIGNATURES = {
     "fmlp_expert_plan": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp] + [_i64] * 4 + [_vp, ctypes.c_size_t, _vp]),
     "fmlp_expert_scatter": (ctypes.c_int, [_vp, _i64] + [_vp] * 6 + [_i64] * 5 + [ctypes.c_int, _vp]),
     "fmlp_expert_gather": (ctypes.c_int, [_vp] * 4 + [_i64] * 5 + [ctypes.c_int, _vp]),
+    "fmlp_orthogonalize_workspace_bytes": (ctypes.c_size_t, [_i64] * 3 + [ctypes.c_int, ctypes.c_int]),
+    "fmlp_orthogonalize": (ctypes.c_int, [_vp, _vp] + [_i64] * 3 + [ctypes.c_int, ctypes.c_int, _f32p, ctypes.c_float, _vp,
+                                                                    ctypes.c_size_t, _vp]),
+    "fmlp_muon_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.POINTER(MuonTensor), ctypes.c_int]),
+    "fmlp_muon_step": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(MuonTensor), ctypes.c_double, ctypes.c_double,
+                                      ctypes.c_int, ctypes.c_double, ctypes.c_int, _f32p, ctypes.c_float, _vp,
+                                      ctypes.c_size_t, _vp]),
     "fmlp_bwd_noalloc": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_int,
                                         ctypes.c_int, _vp]),
 }

@@ -1,6 +1,8 @@
 // Host-side launch descriptors of the gated block's operators: the gated MLP, the join of a block
 // with its residual stream, and gradient clipping.
 #pragma once
+#include <vector>
+
 #include "fmlp_launch.h"
 
 namespace fmlp {
@@ -9,6 +11,16 @@ namespace fmlp {
 int abi_fail(int status, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int abi_ok();
 int abi_num_cus(int* out);
+
+// One run of memory of a call over many tensors: what tensor i writes, or what of it is only read.
+struct MemRange {
+  uintptr_t lo, hi;
+  int i;
+  bool write;
+};
+// Workgroups write in no order: memory that a call writes and that another of its ranges holds too would be a race.
+// Sorts the ranges and sets two such tensors' indices.
+bool mem_overlap(std::vector<MemRange>& r, int* a, int* b);
 
 // Gated MLP: X, dO (H, B, D) with dense rows and any head stride, Wg, Wu (H, D, E) with row pitch
 // ldw, W2 (H, E, D), outputs dense.

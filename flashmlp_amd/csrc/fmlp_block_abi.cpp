@@ -101,6 +101,27 @@ int io_type(int io) { return io == FMLP_DTYPE_F32 ? fmlp::IO_F32 : io == FMLP_DT
 
 }  // namespace
 
+namespace fmlp {
+
+bool mem_overlap(std::vector<MemRange>& r, int* a, int* b) {
+  const auto by_lo = [](const MemRange& x, const MemRange& y) { return x.lo < y.lo; };
+  if (!std::is_sorted(r.begin(), r.end(), by_lo)) std::sort(r.begin(), r.end(), by_lo);
+  const MemRange *w = nullptr, *any = nullptr;  // those that reach furthest so far
+  for (const MemRange& x : r) {
+    const MemRange* o = x.write ? any : w;
+    if (o != nullptr && x.lo < o->hi) {
+      *a = std::min(x.i, o->i);
+      *b = std::max(x.i, o->i);
+      return true;
+    }
+    if (any == nullptr || x.hi > any->hi) any = &x;
+    if (x.write && (w == nullptr || x.hi > w->hi)) w = &x;
+  }
+  return false;
+}
+
+}  // namespace fmlp
+
 FMLP_EXPORT size_t fmlp_gated_min_workspace_bytes(int64_t H, int64_t D, int64_t E, int dtype) {
   if (check_gated(H, 0, D, E, dtype, 0)) return 0;
   return gated_pad_bytes(H, D, E, io_of(dtype));
@@ -401,32 +422,6 @@ FMLP_EXPORT int fmlp_join_bwd(const fmlp_join* j, void* workspace, size_t worksp
 // ---------------------------------------------------------------------------------------------
 namespace {
 
-// One run of memory of a clipping call: an output, or a gradient that is read and has another output.
-struct ClipRange {
-  uintptr_t lo, hi;
-  int i;
-  bool write;
-};
-
-// Workgroups write the outputs in no order: an output that shares memory with another tensor of the call than its own
-// gradient, in place, would be a race. Sets the two tensors' indices.
-bool clip_overlap(std::vector<ClipRange>& r, int* a, int* b) {
-  const auto by_lo = [](const ClipRange& x, const ClipRange& y) { return x.lo < y.lo; };
-  if (!std::is_sorted(r.begin(), r.end(), by_lo)) std::sort(r.begin(), r.end(), by_lo);
-  const ClipRange *w = nullptr, *any = nullptr;  // those that reach furthest so far
-  for (const ClipRange& x : r) {
-    const ClipRange* o = x.write ? any : w;
-    if (o != nullptr && x.lo < o->hi) {
-      *a = std::min(x.i, o->i);
-      *b = std::max(x.i, o->i);
-      return true;
-    }
-    if (any == nullptr || x.hi > any->hi) any = &x;
-    if (x.write && (w == nullptr || x.hi > w->hi)) w = &x;
-  }
-  return false;
-}
-
 int clip_impl(int n, const void* const* grads, void* const* outs, const int64_t* numels, const int* dtypes,
               const int* out_dtypes, bool clip, float max_norm, float* norm, void* ws, size_t ws_bytes, void* stream) {
   if (n < 0) return abi_fail(FMLP_ERR_INVALID_ARG, "%d tensors", n);
@@ -436,7 +431,7 @@ int clip_impl(int n, const void* const* grads, void* const* outs, const int64_t*
     return abi_fail(FMLP_ERR_INVALID_ARG, "norm is NULL or not 4-byte aligned");
   if (clip && !(max_norm >= 0)) return abi_fail(FMLP_ERR_INVALID_ARG, "max_norm is negative or NaN");
   std::vector<fmlp::ClipTensor> t;
-  std::vector<ClipRange> ranges;
+  std::vector<fmlp::MemRange> ranges;
   try {
     t.resize((size_t)n);
     if (clip) ranges.reserve(2 * (size_t)n);
@@ -461,12 +456,12 @@ int clip_impl(int n, const void* const* grads, void* const* outs, const int64_t*
     t[(size_t)i] = fmlp::ClipTensor{g, o, numels[i], io_type(ins[0]), io_type(ins[1])};
     if (clip && numels[i] > 0) {
       const uintptr_t gi = reinterpret_cast<uintptr_t>(g), oi = reinterpret_cast<uintptr_t>(o);
-      ranges.push_back(ClipRange{oi, oi + (uintptr_t)numels[i] * elem_bytes(ins[1]), i, true});
-      if (g != o || ins[0] != ins[1]) ranges.push_back(ClipRange{gi, gi + (uintptr_t)numels[i] * elem_bytes(ins[0]), i, false});
+      ranges.push_back(fmlp::MemRange{oi, oi + (uintptr_t)numels[i] * elem_bytes(ins[1]), i, true});
+      if (g != o || ins[0] != ins[1]) ranges.push_back(fmlp::MemRange{gi, gi + (uintptr_t)numels[i] * elem_bytes(ins[0]), i, false});
     }
   }
   int one, two;
-  if (clip && clip_overlap(ranges, &one, &two))
+  if (clip && fmlp::mem_overlap(ranges, &one, &two))
     return abi_fail(FMLP_ERR_INVALID_ARG, "the output of tensor %d or %d overlaps a tensor of the call", one, two);
   int cus = 0, st;
   if ((st = fmlp::abi_num_cus(&cus))) return st;

@@ -1,0 +1,58 @@
+// Host-side launch descriptors of the orthogonalised updates (fmlp_muon.hip, fmlp_muon_iter.hip).
+#pragma once
+#include "fmlp_launch.h"
+
+namespace fmlp {
+
+constexpr int kMuonMaxSmall = 256;  // the smaller side of a matrix
+constexpr int kMuonMaxSteps = 10;
+
+// A stack of H matrices R x C, dense. x (and, with a momentum, m) are read; out is written: the orthogonalised matrices,
+// or with `update` the weights.
+struct MuonTensor {
+  const void* x;
+  void* m;    // momentum, or null
+  void* out;
+  long long H;
+  int R, C;
+  int x_io, m_io, out_io;  // IoType
+  float lr, keep;          // update: keep out - lr O
+};
+
+// What a call does with every tensor: u = x, or with momenta m' = mu m + nu x, u = m' or (nesterov) nu x + mu m';
+// X = u / (|u| + eps); q(l) = a + b l + c l^2 for each step.
+struct MuonCall {
+  float mu, nu;
+  int nesterov, update;
+  float eps;
+  int steps;
+  float abc[kMuonMaxSteps][3];
+  int stage;  // steps taken on one Gram matrix
+};
+
+// Bytes of workspace and where things are in it, for the call's tensors.
+struct MuonPlan {
+  size_t ws_bytes;
+};
+MuonPlan muon_plan(int n, const MuonTensor* t, const MuonCall& c, int num_cus);
+hipError_t launch_muon(int n, const MuonTensor* t, const MuonCall& c, int num_cus, void* ws, hipStream_t st);
+
+// ---- between the two translation units ----
+// Steps on NP x NP Gram matrices, NP 32 to 256: G (`parts` partial sums each, fp32, whole and symmetric) to P, the product
+// of the steps' polynomials, as two fp16 terms times p_scale ([NP][NP] first terms, then second ones, a matrix after the
+// other), and for each matrix info = {scale of the values u for fp16 terms, factor of the products}.
+struct MuonSteps {
+  int steps;
+  float a[kMuonMaxSteps], b[kMuonMaxSteps], c[kMuonMaxSteps];
+  float g_scale[kMuonMaxSteps], q_scale[kMuonMaxSteps], p_scale[kMuonMaxSteps];  // powers of two, for fp16 terms
+  int normalise;
+  float eps;
+};
+struct MuonInfo {
+  float u_scale, factor;
+};
+size_t muon_iter_ws_bytes(int NP, long long matrices);
+hipError_t launch_muon_iter(int NP, long long matrices, const float* G, int parts, unsigned short* P, MuonInfo* info,
+                            const MuonSteps& s, void* ws, hipStream_t st);
+
+}  // namespace fmlp

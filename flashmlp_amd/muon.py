@@ -1,0 +1,174 @@
+"""Stacks of matrices orthogonalised by Newton-Schulz products, and the Muon optimizer's step around it.
+
+    orthogonalize(x, *, steps=5, coefficients=(3.4445, -4.775, 2.0315), eps=1e-7, out=None) -> like x
+    muon_step(params, grads, momenta, lr, *, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, ...)
+
+    X = u / (|u| + eps),  `steps` times  X <- a X + b (X X^T) X + c (X X^T)^2 X        |u| the Frobenius norm
+    m = momentum m + (1 - momentum) g,  u = (1 - momentum) g + momentum m (nesterov) or m
+    w = (1 - lr weight_decay) w - lr scale X
+
+Every matrix of a stack (..., R, C) stands by itself, as the heads of the MLPs' weights (H, D, E) and (H, E, D) do; min(R, C) <=
+256, the other side is any. torch.optim.Muon, whose conventions these are, takes single matrices only. fp16, bf16 or
+fp32; weights, gradients and momenta each of its own type, so that gradients clipped into full precision buffers
+(clip_grads) or 16-bit ones go with full precision weights. Calls are asynchronous on torch's current stream.
+
+The steps are taken on the smaller side's Gram matrix in 32 bits. Directions whose singular values are far below the largest
+(1e-4 of it) come out within 4e-4 of the formula, below a 16-bit result's rounding; an fp32 `orthogonalize` is as
+exact as the formula's products in fp32.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+import numbers
+from typing import Iterable, Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib
+from .flashmlp import _DTYPES, _alloc_ws, _ptr
+from .gated import _not_traced, _On
+
+_COEFFICIENTS = (3.4445, -4.775, 2.0315)
+_MAX_STEPS = 10
+
+
+def _coefficients(coefficients, steps):
+    """a, b, c of every step as the library takes them"""
+    if not 1 <= steps <= _MAX_STEPS:
+        raise ValueError(f"steps must be 1 to {_MAX_STEPS}, got {steps}")
+    c = list(coefficients)
+    if len(c) == 3 and all(isinstance(v, numbers.Real) for v in c):
+        c = [c] * steps
+    if len(c) != steps or any(len(v) != 3 for v in c):
+        raise ValueError(f"coefficients must be three numbers, or three for each of {steps} steps")
+    return (ctypes.c_float * (3 * steps))(*(float(v) for s in c for v in s))
+
+
+def _stack(t: torch.Tensor, what: str) -> Tuple[int, int, int]:
+    """(H, R, C)"""
+    if t.dim() < 2:
+        raise ValueError(f"{what} must be matrices or stacks of them, got {t.dim()} dimensions")
+    R, C = t.shape[-2:]
+    return math.prod(t.shape[:-2]), R, C
+
+
+def _check(t: torch.Tensor, what: str, dev=None):
+    if t.device.type != "cuda":
+        raise RuntimeError(f"FlashMLP runs on an AMD GPU through HIP; got a tensor on {t.device} (move inputs to 'cuda')")
+    if dev is not None and t.device != dev:
+        raise RuntimeError(f"all tensors must be on one device ({dev} vs {t.device})")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"FlashMLP supports float16, bfloat16 and float32 {what}, got {t.dtype}")
+    if t.layout != torch.strided:
+        raise TypeError(f"{what} must be dense tensors, got {t.layout}")
+
+
+def _number(v, name):
+    # (a tensor would be read on the host)
+    if not isinstance(v, numbers.Real):
+        raise TypeError(f"{name} must be a number, got {type(v).__name__}")
+    return float(v)
+
+
+def _plain(t: torch.Tensor) -> bool:
+    return t.is_contiguous() and not t.is_neg()
+
+
+@torch.no_grad()
+def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence = _COEFFICIENTS, eps: float = 1e-7,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The matrices of x (..., R, C) orthogonalised: singular values brought towards one, singular vectors kept.
+
+    Args:
+        steps: 1 to 10; coefficients: (a, b, c), or one such triple for each step;
+        out: of x's shape and type, or x itself.
+    No gradient is kept.
+    """
+    _not_traced("orthogonalize")
+    H, R, C = _stack(x, "x")
+    abc = _coefficients(coefficients, steps)
+    eps = _number(eps, "eps")
+    _check(x, "matrices")
+    if out is not None:
+        _check(out, "outputs", x.device)
+        if out.shape != x.shape or out.dtype != x.dtype:
+            raise ValueError(f"out must be {x.dtype} of shape {tuple(x.shape)}, got {out.dtype} of {tuple(out.shape)}")
+    same = out is x
+    xd = x if _plain(x) else x.resolve_neg().contiguous()
+    o = out if out is not None and _plain(out) else xd if same else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    L = _lib.lib()
+    with _On(x.get_device()) as stream:
+        n = L.fmlp_orthogonalize_workspace_bytes(H, R, C, _DTYPES[x.dtype], steps)
+        ws = _alloc_ws(n, x.device)
+        st = L.fmlp_orthogonalize(xd.data_ptr(), o.data_ptr(), H, R, C, _DTYPES[x.dtype], steps, abc, eps, _ptr(ws), n, stream)
+    _lib.check(st, "orthogonalisation")
+    if out is None:
+        return o
+    if o is out:
+        if not out.is_inference():
+            torch.autograd.graph.increment_version(out)
+    else:
+        out.copy_(o)
+    return out
+
+
+@torch.no_grad()
+def muon_step(params: Union[torch.Tensor, Iterable[torch.Tensor]], grads: Union[torch.Tensor, Iterable[torch.Tensor]],
+              momenta: Union[torch.Tensor, Iterable[torch.Tensor]], lr: float, *, momentum: float = 0.95, nesterov: bool = True,
+              weight_decay: float = 0.0, scale: Optional[float] = None, steps: int = 5,
+              coefficients: Sequence = _COEFFICIENTS, eps: float = 1e-7) -> None:
+    """One step of Muon for many stacks of matrices, in place.
+
+    Args:
+        params, grads, momenta: tensors, or as many of each, of equal shapes (..., R, C); momenta start as zeros;
+        weight_decay: decoupled: w (1 - lr weight_decay);
+        scale: of the update; None: sqrt(max(1, R / C)) (0.2 * sqrt(max(R, C)) has the rms of AdamW's updates);
+        steps, coefficients, eps: as orthogonalize's.
+    A tensor that is in the call twice, or overlaps another one that is written, is refused.
+    """
+    _not_traced("muon_step")
+    params, grads, momenta = ([t] if isinstance(t, torch.Tensor) else list(t) for t in (params, grads, momenta))
+    if not len(params) == len(grads) == len(momenta):
+        raise ValueError(f"{len(params)} parameters, {len(grads)} gradients, {len(momenta)} momenta")
+    lr, momentum, weight_decay, eps = (_number(v, n) for v, n in ((lr, "lr"), (momentum, "momentum"),
+                                                                  (weight_decay, "weight_decay"), (eps, "eps")))
+    scale = None if scale is None else _number(scale, "scale")
+    abc = _coefficients(coefficients, steps)
+    if not (lr >= 0 and weight_decay >= 0 and 0 <= momentum <= 1):
+        raise ValueError(f"lr and weight_decay must not be negative, momentum within [0, 1]: {lr}, {weight_decay}, {momentum}")
+    if not params:
+        return
+    dev = params[0].device
+    calls, held, back = (_lib.MuonTensor * len(params))(), [], []
+    for c, w, g, m in zip(calls, params, grads, momenta):
+        c.H, c.R, c.C = _stack(w, "parameters")
+        if g.shape != w.shape or m.shape != w.shape:
+            raise ValueError(f"a parameter of shape {tuple(w.shape)} with a gradient of {tuple(g.shape)}, a momentum of {tuple(m.shape)}")
+        for t, what in ((w, "parameters"), (g, "gradients"), (m, "momenta")):
+            _check(t, what, dev)
+        g = g if _plain(g) else g.resolve_neg().contiguous()
+        held.append(g)
+        dense = []
+        for t in (w, m):  # other layouts through dense tensors
+            d = t
+            if not _plain(t):
+                d = t.resolve_neg().contiguous()
+                back.append((t, d))
+            dense.append(d)
+        held.extend(dense)
+        c.w, c.g, c.m = dense[0].data_ptr(), g.data_ptr(), dense[1].data_ptr()
+        c.w_dtype, c.g_dtype, c.m_dtype = _DTYPES[w.dtype], _DTYPES[g.dtype], _DTYPES[m.dtype]
+        c.scale = math.sqrt(max(1.0, c.R / c.C if c.C else 1.0)) if scale is None else scale
+    if len({(t.data_ptr(), t.shape, t.stride()) for t, _ in back}) < len(back):  # (dense ones: the library's own check)
+        raise RuntimeError("a tensor is listed twice: parameters and momenta must not overlap")
+    L = _lib.lib()
+    with _On(dev.index) as stream:
+        n = L.fmlp_muon_workspace_bytes(len(params), calls, steps)
+        ws = _alloc_ws(n, dev)
+        st = L.fmlp_muon_step(len(params), calls, lr, momentum, int(nesterov), weight_decay, steps, abc, eps, _ptr(ws), n, stream)
+    _lib.check(st, "muon step")
+    seen = {id(t) for t, _ in back}
+    torch.autograd.graph.increment_version([t for t in (*params, *momenta) if id(t) not in seen and not t.is_inference()])
+    for t, d in back:
+        t.copy_(d)

@@ -43,7 +43,8 @@ extern "C" {
                               there changes; added within 4, with no change to the others:
                               fmlp_shape_dense, fmlp_fwd_strided_ws, fmlp_copy_dense, the
                               fmlp_gated_*, fmlp_join_* and fmlp_clip_* calls, fmlp_head_sum,
-                              fmlp_grad_norm, the fmlp_route_* and fmlp_expert_* calls */
+                              fmlp_grad_norm, the fmlp_route_* and fmlp_expert_* calls,
+                              fmlp_orthogonalize, fmlp_muon_step and their workspaces */
 
 typedef enum {
   FMLP_OK = 0,
@@ -395,6 +396,37 @@ int fmlp_expert_scatter(const void* x, int64_t x_row_stride, const float* weight
                         int64_t capacity, int64_t D, int dtype, void* stream);
 int fmlp_expert_gather(const void* rows, const float* weights, const int32_t* slots, void* o, int64_t T, int64_t k, int64_t N,
                        int64_t capacity, int64_t D, int dtype, void* stream);
+
+/*
+ * Orthogonalised matrices by Newton-Schulz products, and the optimizer's step around them (Muon). No counterpart in the
+ * reference. For a matrix u, R x C, with n = min(R, C) <= 256:
+ *   X = u / (|u| + eps), |u| its Frobenius norm;  for each of `steps` (1 to 10) steps  X <- a X + b (X X^T) X + c (X X^T)^2 X
+ * coefficients: a, b, c of every step, 3 * steps numbers that are read on the host. The steps are taken on the n x n Gram matrix in
+ * 32 bits. Singular values far below the largest come out with an absolute error (of an orthogonal result, relative to 1)
+ * of 4e-4 at most after five steps where the result has 16 bits or goes into weights; an fp32 result of fmlp_orthogonalize takes the Gram matrix anew
+ * after three steps and is as exact as the products above in fp32. |u|^2 has to be within fp32 (|u| < 1.8e19).
+ *
+ * fmlp_orthogonalize: out[h] = X of x[h] for a stack of H matrices, dense, both of dtype; out may be x.
+ * fmlp_muon_step, in place for n stacks of H[i] matrices each (weights w, gradients g, momenta m, dense, each of a type of its own):
+ *   m = momentum m + (1 - momentum) g;  u = m, or with nesterov (1 - momentum) g + momentum m (m as it is stored)
+ *   w = (1 - lr weight_decay) w - lr scale X
+ * Any alignment to the elements. Memory that the call writes (w, m) must not be in it twice (FMLP_ERR_INVALID_ARG). Arrays
+ * are read on the host before the call returns. Sums in a fixed order. workspace: 16-byte aligned, of the *_workspace_bytes.
+ */
+typedef struct {
+  void* w;
+  const void* g;
+  void* m;
+  int64_t H, R, C;
+  int w_dtype, g_dtype, m_dtype;
+  float scale;
+} fmlp_muon_tensor;
+size_t fmlp_orthogonalize_workspace_bytes(int64_t H, int64_t R, int64_t C, int dtype, int steps);
+int fmlp_orthogonalize(const void* x, void* out, int64_t H, int64_t R, int64_t C, int dtype, int steps,
+                       const float* coefficients, float eps, void* workspace, size_t workspace_bytes, void* stream);
+size_t fmlp_muon_workspace_bytes(int n, const fmlp_muon_tensor* tensors, int steps);
+int fmlp_muon_step(int n, const fmlp_muon_tensor* tensors, double lr, double momentum, int nesterov, double weight_decay,
+                   int steps, const float* coefficients, float eps, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

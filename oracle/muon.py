@@ -1,0 +1,78 @@
+"""Newton-Schulz orthogonalisation and the Muon step in 64 bits, with error bounds (test infrastructure only; CPU tensors).
+
+    X = u / (|u| + eps), `steps` times X <- a X + b (X X^T) X + c (X X^T)^2 X
+
+The kernels take the steps on the Gram matrix G in values of 22 bits and 32-bit sums. An error e of G at an eigenvalue l near 0 grows by
+a^2 a step as l itself does, until l is of the size of one: by at most min(a^(2 (s - 1)), 1 / l) over the s steps that one Gram matrix
+serves, and changes the polynomial's value there by b / a of it. Rounding gives e = 2^-22 of G's norm, which is at most 1: so a singular
+value near one is off by 1.4 2^-22 min(...), and no element by more. A Gram matrix serves five steps where the
+result has 16 bits, three where it has 32; in between, the matrices themselves are rounded to 2^-24, twice (the products and
+their factor), which what follows multiplies by a a step.
+"""
+from __future__ import annotations
+
+import torch
+
+from .gated import UNIT
+
+COEFFICIENTS = (3.4445, -4.775, 2.0315)
+
+
+def triples(coefficients, steps):
+    return [tuple(coefficients)] * steps if not isinstance(coefficients[0], (tuple, list)) else [tuple(c) for c in coefficients]
+
+
+def orthogonal64(u, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+    x = u.double()
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT if tall else x
+    x = x / (torch.linalg.matrix_norm(x, keepdim=True) + eps)
+    for a, b, c in triples(coefficients, steps):
+        g = x @ x.mT
+        x = a * x + (b * g + c * (g @ g)) @ x
+    return x.mT if tall else x
+
+
+def bound(u, steps=5, coefficients=COEFFICIENTS, full=False):
+    """of an element of the unrounded result; full: fp32 results"""
+    if u.numel() == 0:
+        return 0.0
+    x = u.double()
+    s = torch.linalg.svdvals(x / torch.linalg.matrix_norm(x, keepdim=True).clamp(min=1e-300))
+    least = (s.reshape(-1, s.shape[-1])[:, -1].min() ** 2).item()  # the smallest eigenvalue of a G
+    most = 1.0
+    a = [abs(c[0]) for c in triples(coefficients, steps)]
+    stage = 3 if full else 5
+    total = 0.0
+    for first in range(0, steps, stage):
+        grow = 1.0
+        for v in a[first:min(first + stage, steps) - 1]:
+            grow *= v * v
+        total += 1.4 * min(grow, 1 / max(least, 1e-300))
+        least = min(1.0, least * grow)
+    after = 1.0
+    for v in a:
+        after *= v
+    total += 2 * min(after, 1 / max(least, 1e-300) ** 0.5)
+    return 2.0 ** -22 * (total + 8) * most
+
+
+def step64(w, g, m, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+    """dict of (value, bound) of w and m"""
+    e = 2.0 ** -24
+    wd, gd, md = w.double(), g.double(), m.double()
+    m2 = momentum * md + (1 - momentum) * gd
+    bm = UNIT[m.dtype] * m2.abs() + 3 * e * (md.abs() + gd.abs())
+    kept = m2.to(torch.float32).to(m.dtype).double()
+    u = (1 - momentum) * gd + momentum * kept if nesterov else kept
+    R, C = w.shape[-2:]
+    s = max(1.0, R / C) ** 0.5 if scale is None else scale
+    o = orthogonal64(u, steps, coefficients, eps)
+    w2 = (1 - lr * weight_decay) * wd - lr * s * o
+    # the stored momentum's rounding may fall the other way: UNIT of m at single elements, which moves u by as much
+    move = 0.0
+    if u.numel():
+        norm = torch.linalg.matrix_norm(u, keepdim=True).clamp(min=1e-300)
+        move = (2 * bm / norm).amax().item() * 485
+    bw = UNIT[w.dtype] * w2.abs() + 4 * e * (wd.abs() + (lr * s * o).abs()) + lr * s * (bound(u, steps, coefficients) + move)
+    return {"w": (w2, bw), "m": (m2, bm)}
