@@ -20,8 +20,7 @@
 #include <cmath>
 #include <vector>
 
-#include "fmlp_muon.h"
-#include "fmlp_vec.h"
+#include "fmlp_muon_device.h"
 
 namespace fmlp {
 namespace {
@@ -121,15 +120,26 @@ struct Tile {
     const int a = base + (k0 + 8 * g + (i16 >> 2)) * PITCH + (s0 + 16 * (G & 1) + 4 * (i16 & 3)) * 2;
     return cat(lds_read_tr(a), lds_read_tr(a + 4 * PITCH));
   }
-  // operand of 32 long indices from l0 and 16 small ones from k0: lane = long index, 8 small ones
+  // operand of 32 long indices from l0 and 16 small ones from k0: lane = long index, 8 small ones in the order that a
+  // result of the matrix instruction has rows in, and so P: 4 g + {0..3, 8..11}
   static __device__ __forceinline__ u32x4 by_long(int base, int l0, int k0, int lane) {
     const int g = lane >> 5, l32 = lane & 31;
-    if constexpr (TALL) return lds_read16(base + at(l0 + l32, (k0 >> 3) + g));
-    // rows k0 + 8 g .., columns l0 + 16 (G & 1) ..: 8-byte halves of the swapped units
+    if constexpr (TALL) return lds_read16(base + at(l0 + l32, (k0 >> 3) + g));  // (put_by_long's order)
+    // rows k0 + 4 g .., columns l0 + 16 (G & 1) ..: 8-byte halves of the swapped units
     const int G = lane >> 4, i16 = lane & 15;
-    const int row = k0 + 8 * g + (i16 >> 2), col = l0 + 16 * (G & 1) + 4 * (i16 & 3);
-    const int a = base + at(row, col >> 3) + (col & 4) * 2, b = base + at(row + 4, col >> 3) + (col & 4) * 2;
+    const int row = k0 + 4 * g + (i16 >> 2), col = l0 + 16 * (G & 1) + 4 * (i16 & 3);
+    const int a = base + at(row, col >> 3) + (col & 4) * 2, b = base + at(row + 8, col >> 3) + (col & 4) * 2;
     return cat(lds_read_tr(a), lds_read_tr(b));
+  }
+  // 8 elements of unit u of a row where by_long finds them: TALL, halves of 4 in P's order
+  static __device__ __forceinline__ void put_by_long(int base, int row, int u, const u32x4& v) {
+    if constexpr (TALL) {
+      const int to = base + at(row, u & ~1) + (u & 1) * 8;
+      lds_write8(to, u32x2{v[0], v[1]});
+      lds_write8(to + 16, u32x2{v[2], v[3]});
+    } else {
+      lds_write16(base + at(row, u), v);
+    }
   }
 };
 
@@ -337,11 +347,11 @@ apply_kernel(Table tab, const u16* __restrict__ P, const MuonInfo* __restrict__ 
 
   // the wave's rows of P
   u32x4 ph[KS], pl[KS];
-  const u16* src = P + (size_t)(t.matrix0 + h) * (2 * NP * NP) + (size_t)(s0 + l32) * NP + 8 * g;
+  const u16* src = P + (size_t)(t.matrix0 + h) * (2 * NP * NP) + muon_chunk<NP>(s0 + l32, 0, g);
 #pragma unroll
   for (int k = 0; k < KS; ++k) {
-    ph[k] = *(const u32x4*)(src + 16 * k);
-    pl[k] = *(const u32x4*)(src + NP * NP + 16 * k);
+    ph[k] = *(const u32x4*)(src + 512 * k);
+    pl[k] = *(const u32x4*)(src + NP * NP + 512 * k);
   }
 
   Raw x[Q], m[Q], w[Q];
@@ -374,9 +384,8 @@ apply_kernel(Table tab, const u16* __restrict__ P, const MuonInfo* __restrict__ 
         hi[j] = pack2<false>(a, b);
         if constexpr (XT == 2) lo[j] = pack2<false>(a - lo_f32<false>(hi[j]), b - hi_f32<false>(hi[j]));
       }
-      const int o = T::at(at.row, at.u);
-      lds_write16(o, hi);
-      if constexpr (XT == 2) lds_write16(T::TERM + o, lo);
+      T::put_by_long(0, at.row, at.u, hi);
+      if constexpr (XT == 2) T::put_by_long(T::TERM, at.row, at.u, lo);
     }
     __syncthreads();
     if (update) {
@@ -505,9 +514,12 @@ Group group_of(int NP, int n, const MuonTensor* t, int cus) {
       r.tiles = std::max(r.tiles, ((long long)std::max(t[i].R, t[i].C) + KT - 1) / KT);
     }
   if (r.matrices == 0) return r;
-  // three workgroups a CU at least, as far as there are tiles
+  // three workgroups a CU at least, as far as there are tiles; of Gram matrices no more than pay: a tile takes about
+  // 2.5 us, a part's sums are written and read at about 4 TB/s (8 matrices of 256 x 1024: 32 parts 18 + 46 us, 9 PARTS9)
   const long long want = (3LL * cus + r.matrices - 1) / r.matrices;
-  r.gram_parts = (int)std::max(1LL, std::min(want, r.tiles));
+  const double part_us = (double)r.matrices * NP * NP * 8 / 4e6;
+  const long long pays = std::max(1LL, std::llround(std::sqrt((double)r.tiles * 2.5 / part_us)));
+  r.gram_parts = (int)std::max(1LL, std::min(std::min(want, pays), r.tiles));
   r.apply_parts = (int)std::max(1LL, std::min(want, r.tiles));
   const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   r.p_off = up((size_t)r.matrices * r.gram_parts * NP * NP * 4);

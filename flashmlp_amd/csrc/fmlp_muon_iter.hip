@@ -12,25 +12,22 @@
 // 32-bit values go through the matrix units as two fp16 terms, hi + lo, of the value times a power of two (22 bits; the
 // host's bounds of the eigenvalues keep them in range), three products with fp32 sums: 3/16 of the time of fp32
 // products at an error of the size of fp32 rounding.
-#include "fmlp_device.h"
-#include "fmlp_muon.h"
+#include "fmlp_muon_device.h"
 
 namespace fmlp {
 namespace {
 
-// hi and lo fp16 terms of 8 values times s
-__device__ __forceinline__ void split8(const float* f, float s, u32x4& hi, u32x4& lo) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float a = f[2 * j] * s, b = f[2 * j + 1] * s;
-    hi[j] = pack2<false>(a, b);
-    lo[j] = pack2<false>(a - lo_f32<false>(hi[j]), b - hi_f32<false>(hi[j]));
-  }
+// ---------------------------------------------------------------------------------------------
+// NP <= 128: a workgroup a matrix, NP / 16 waves of 16 columns each
+// ---------------------------------------------------------------------------------------------
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// 16 x 16 x 32: A lane l row l % 16, B lane l column l % 16, inner slots 8 (l / 16) ..; result column l % 16, rows
+// 4 (l / 16) ..
+__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// ---------------------------------------------------------------------------------------------
-// NP <= 128: a workgroup a matrix, NP / 32 waves
-// ---------------------------------------------------------------------------------------------
 // byte offset of 16-byte unit u of row r of a [NP][NP] fp16 matrix: units are swapped within a row so that 16
 // consecutive rows' units lie on all banks
 template <int NP>
@@ -40,96 +37,87 @@ __device__ __forceinline__ int unit_off(int r, int u) {
   return r * (NP * 2) + ((u ^ f) << 4);
 }
 
-// The wave's columns as rows of the left operand: unit (tile t, half s, g) of row n holds the 8 values that the lane of
-// column n and half g has in acc[t][8 s ..].
+// A wave's 16 columns of a matrix as both fp16 terms: unit k of the lane of column n and quarter q holds rows
+// 32 k + 4 q + {0..3, 16..19}, the order that two tiles of a result have them in
 template <int NP>
-__device__ __forceinline__ void put_left(const f32x16 (&v)[NP / 32], float s, int n, int g) {
+struct Cols {
+  u32x4 hi[NP / 32], lo[NP / 32];
+};
+template <int NP>
+__device__ __forceinline__ void pack_cols(const f32x4 (&v)[NP / 16], float s, Cols<NP>& c) {
 #pragma unroll
-  for (int t = 0; t < NP / 32; ++t)
+  for (int k = 0; k < NP / 32; ++k) {
+    float f[8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float f[8];
+    for (int j = 0; j < 8; ++j) f[j] = v[2 * k + (j >> 2)][j & 3];
+    split8(f, s, c.hi[k], c.lo[k]);
+  }
+}
+// the columns as rows of the left operand
+template <int NP>
+__device__ __forceinline__ void put_left(const Cols<NP>& c, int n, int q) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = v[t][8 * h + j];
-      u32x4 hi, lo;
-      split8(f, s, hi, lo);
-      const int at = unit_off<NP>(n, t * 4 + h * 2 + g);
-      lds_write16(at, hi);
-      lds_write16(NP * NP * 2 + at, lo);
+  for (int k = 0; k < NP / 32; ++k) {
+    const int at = unit_off<NP>(n, 4 * k + q);
+    lds_write16(at, c.hi[k]);
+    lds_write16(NP * NP * 2 + at, c.lo[k]);
+  }
+}
+
+// out = (left operand in LDS) * b, in the terms' scales. A step has 32 of the inner dimension for TP tiles of rows.
+template <int NP>
+__device__ __forceinline__ void product(f32x4 (&out)[NP / 16], const Cols<NP>& b, int q, int l16) {
+  constexpr int TP = 2, GROUPS = NP / 16 / TP, STEPS = NP / 32 * GROUPS, AHEAD = NP == 128 ? 0 : 1;
+  u32x4 ah[AHEAD + 1][TP], al[AHEAD + 1][TP];
+  const auto fetch = [&](int j) {
+    const int k = j / GROUPS, p = j % GROUPS;
+#pragma unroll
+    for (int t = 0; t < TP; ++t) {
+      const int at = unit_off<NP>(l16, 4 * k + q) + (p * TP + t) * (16 * NP * 2);
+      ah[j % (AHEAD + 1)][t] = lds_read16(at);
+      al[j % (AHEAD + 1)][t] = lds_read16(NP * NP * 2 + at);
     }
-}
-
-// out = (left operand in LDS, times its scale) * b, times `back`
-template <int NP>
-__device__ __forceinline__ void product(f32x16 (&out)[NP / 32], const f32x16 (&b)[NP / 32], float sb, float back, int g,
-                                        int l32) {
-  constexpr int RB = NP / 32;
+  };
 #pragma unroll
-  for (int t = 0; t < RB; ++t) out[t] = zero16();
+  for (int j = 0; j < AHEAD; ++j) fetch(j);
 #pragma unroll
-  for (int kt = 0; kt < RB; ++kt)
+  for (int j = 0; j < STEPS; ++j) {
+    const int k = j / GROUPS, p = j % GROUPS, e = j % (AHEAD + 1);
+    if (j + AHEAD < STEPS) fetch(j + AHEAD);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float f[8];
+    for (int t = 0; t < TP; ++t) out[p * TP + t] = mfma16(al[e][t], b.hi[k], k == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : out[p * TP + t]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = b[kt][8 * h + j];
-      u32x4 bh, bl;
-      split8(f, sb, bh, bl);
+    for (int t = 0; t < TP; ++t) out[p * TP + t] = mfma16(ah[e][t], b.lo[k], out[p * TP + t]);
 #pragma unroll
-      for (int t = 0; t < RB; ++t) {
-        const int at = unit_off<NP>(32 * t + l32, kt * 4 + h * 2 + g);
-        const u32x4 ah = lds_read16(at), al = lds_read16(NP * NP * 2 + at);
-        out[t] = mfma<false>(al, bh, out[t]);
-        out[t] = mfma<false>(ah, bl, out[t]);
-        out[t] = mfma<false>(ah, bh, out[t]);
-      }
-    }
-#pragma unroll
-  for (int t = 0; t < RB; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) out[t][i] *= back;
-}
-
-__device__ __forceinline__ MuonInfo info_of(float trace, const MuonSteps& s, float p_scale, float* inv) {
-  const float norm = __builtin_sqrtf(trace);
-  *inv = s.normalise ? 1.f / (norm + s.eps) : 1.f;
-  // |u| <= norm: as fp16 up to 2^14. (Sums of squares below fp32 leave a norm of 0 and values below 2^-74.)
-  int e = 0;
-  (void)frexpf(fmaxf(norm, 0x1p-74f), &e);
-  const float us = ldexpf(1.f, min(max(14 - e, -100), 100));
-  return MuonInfo{us, *inv / us / p_scale};
+    for (int t = 0; t < TP; ++t) out[p * TP + t] = mfma16(ah[e][t], b.hi[k], out[p * TP + t]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 template <int NP>
-__global__ void __launch_bounds__(NP * 2, 2) iter_kernel(const float* __restrict__ G0, int parts, u16* __restrict__ P0,
-                                                         MuonInfo* __restrict__ info, MuonSteps s) {
-  constexpr int RB = NP / 32, SCR = NP * NP * 4;  // LDS: the left operand, then the waves' sums
-  const int lane = (int)threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = wave * 32 + l32;
+__global__ void __launch_bounds__(NP * 4) __attribute__((amdgpu_waves_per_eu(4, 4)))
+iter_kernel(const float* __restrict__ G0, int parts, u16* __restrict__ P0, MuonInfo* __restrict__ info, MuonSteps s) {
+  constexpr int TN = NP / 16, SCR = NP * NP * 4;  // LDS: the left operand, then the waves' sums
+  const int lane = (int)threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = wave * 16 + l16;
   const long long m = blockIdx.x;
 
-  f32x16 G[RB], P[RB], T[RB];
-  const float* src = G0 + m * parts * (NP * NP) + (size_t)n * NP + 4 * g;
+  f32x4 v[TN];
+  const float* src = G0 + m * parts * (NP * NP) + (size_t)n * NP + 4 * q;
 #pragma unroll
-  for (int t = 0; t < RB; ++t) G[t] = zero16();
+  for (int t = 0; t < TN; ++t) v[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int p = 0; p < parts; ++p)
 #pragma unroll
-    for (int t = 0; t < RB; ++t)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4 v = *(const float4*)(src + (size_t)p * (NP * NP) + 32 * t + 8 * q);
-        G[t][4 * q] += v.x;
-        G[t][4 * q + 1] += v.y;
-        G[t][4 * q + 2] += v.z;
-        G[t][4 * q + 3] += v.w;
-      }
-  // the lane that has element (n, n) of the trace: row 8 (i / 4) + 4 g + i % 4 of tile `wave` is l32
+    for (int t = 0; t < TN; ++t) v[t] += *(const f32x4*)(src + (size_t)p * (NP * NP) + 16 * t);
+  // the lane that has element (n, n): row 4 q + i of tile `wave` is l16
+  const auto diagonal = [&](int t, int i) { return t == wave && 4 * q + i == l16; };
   float d = 0.f;
 #pragma unroll
-  for (int t = 0; t < RB; ++t)
+  for (int t = 0; t < TN; ++t)
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (t == wave && 8 * (i >> 2) + 4 * g + (i & 3) == l32) d = G[t][i];
+    for (int i = 0; i < 4; ++i)
+      if (diagonal(t, i)) d = v[t][i];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) d += __shfl_xor(d, o, 64);
   float* scr = (float*)(fmlp_lds + SCR);
@@ -137,125 +125,130 @@ __global__ void __launch_bounds__(NP * 2, 2) iter_kernel(const float* __restrict
   __syncthreads();
   float trace = 0.f;
 #pragma unroll
-  for (int w = 0; w < RB; ++w) trace += scr[w];
+  for (int w = 0; w < TN; ++w) trace += scr[w];
   float inv;
   const MuonInfo fo = info_of(trace, s, s.p_scale[s.steps - 1], &inv);
   if (threadIdx.x == 0) info[m] = fo;
 #pragma unroll
-  for (int t = 0; t < RB; ++t)
+  for (int t = 0; t < TN; ++t)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) G[t][i] = G[t][i] * inv * inv;
+    for (int i = 0; i < 4; ++i) v[t][i] = v[t][i] * inv * inv;
 
+  Cols<NP> G, P;
+  pack_cols<NP>(v, s.g_scale[0], G);
   for (int k = 0; k < s.steps; ++k) {
     const float sg = s.g_scale[k], sq = s.q_scale[k];
-    put_left<NP>(G, sg, n, g);
+    const bool last = k + 1 == s.steps;
+    put_left<NP>(G, n, q);
     __syncthreads();
-    product<NP>(T, G, sg, 1.f / sg / sg, g, l32);
+    product<NP>(v, G, q, l16);
+    // Q = a + b G + c G^2, in G's place
+    const float cc = s.c[k] / sg / sg, cb = s.b[k] / sg, ca = s.a[k];
 #pragma unroll
-    for (int t = 0; t < RB; ++t)
+    for (int u = 0; u < NP / 32; ++u) {
+      float f[8];
+      const u32x4 gh = G.hi[u], gl = G.lo[u];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float one = t == wave && 8 * (i >> 2) + 4 * g + (i & 3) == l32 ? s.a[k] : 0.f;
-        T[t][i] = __builtin_fmaf(s.c[k], T[t][i], __builtin_fmaf(s.b[k], G[t][i], one));
+      for (int j = 0; j < 8; ++j) {
+        const float x = j & 1 ? hi_f32<false>(gh[j >> 1]) + hi_f32<false>(gl[j >> 1])
+                              : lo_f32<false>(gh[j >> 1]) + lo_f32<false>(gl[j >> 1]);
+        f[j] = __builtin_fmaf(cc, v[2 * u + (j >> 2)][j & 3], __builtin_fmaf(cb, x, diagonal(2 * u + (j >> 2), j & 3) ? ca : 0.f));
       }
-    if (k + 1 < s.steps) product<NP>(G, T, sq, 1.f / sg / sq, g, l32);  // G Q, in G's place
-    __syncthreads();
-    put_left<NP>(T, sq, n, g);
-    __syncthreads();
-    if (k == 0) {
-#pragma unroll
-      for (int t = 0; t < RB; ++t) P[t] = T[t];
-    } else {
-      const float sp = s.p_scale[k - 1];
-      product<NP>(T, P, sp, 1.f / sq / sp, g, l32);
-#pragma unroll
-      for (int t = 0; t < RB; ++t) P[t] = T[t];
+      split8(f, sq, G.hi[u], G.lo[u]);
     }
-    if (k + 1 < s.steps) {
-      const float st = sg * sq * 0x1p-14f;  // G Q has G's bound times Q's
-      product<NP>(T, G, st, 1.f / sq / st, g, l32);
-#pragma unroll
-      for (int t = 0; t < RB; ++t) G[t] = T[t];
-    }
+    if (!last) product<NP>(v, G, q, l16);  // G Q
     __syncthreads();
+    put_left<NP>(G, n, q);
+    __syncthreads();
+    // G Q has G's bound times Q's
+    const float st = sg * sq * 0x1p-14f;
+    if (k == 0) P = G;
+    if (!last) pack_cols<NP>(v, st / sg / sq, G);
+    if (k > 0) {
+      product<NP>(v, P, q, l16);
+      pack_cols<NP>(v, s.p_scale[k] / sq / s.p_scale[k - 1], P);
+    }
+    if (!last) {
+      product<NP>(v, G, q, l16);
+      pack_cols<NP>(v, s.g_scale[k + 1] / sq / st, G);
+      __syncthreads();
+    }
   }
-  const float sp = s.p_scale[s.steps - 1];
-  u16* dst = P0 + m * (2 * NP * NP) + (size_t)n * NP + 4 * g;
+  // rows 32 k + 16 h + 4 q ..: half q / 2 of unit q % 2 of 16 inner indices
+  u16* dst = P0 + m * (2 * NP * NP) + muon_chunk<NP>(n, 0, q & 1) + 4 * (q >> 1);
 #pragma unroll
-  for (int t = 0; t < RB; ++t)
+  for (int k = 0; k < NP / 32; ++k)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float f[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = P[t][8 * h + j];
-      u32x4 hi, lo;
-      split8(f, sp, hi, lo);
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        *(u32x2*)(dst + 32 * t + 16 * h + 8 * q) = u32x2{hi[2 * q], hi[2 * q + 1]};
-        *(u32x2*)(dst + NP * NP + 32 * t + 16 * h + 8 * q) = u32x2{lo[2 * q], lo[2 * q + 1]};
-      }
+      *(u32x2*)(dst + (2 * k + h) * 512) = u32x2{P.hi[k][2 * h], P.hi[k][2 * h + 1]};
+      *(u32x2*)(dst + NP * NP + (2 * k + h) * 512) = u32x2{P.lo[k][2 * h], P.lo[k][2 * h + 1]};
     }
 }
 
 template <int NP>
 hipError_t launch_one(long long matrices, const float* G, int parts, u16* P, MuonInfo* info, const MuonSteps& s, hipStream_t st) {
-  constexpr int lds = NP * NP * 4 + 64;
+  constexpr int lds = NP * NP * 4 + 64;  // (the waves' sums behind the operand)
   auto k = iter_kernel<NP>;
   static std::atomic<unsigned long long> done{0};
   const hipError_t e = set_lds_once((const void*)k, lds, done);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(k, dim3((unsigned)matrices), dim3(NP * 2), lds, st, G, parts, P, info, s);
+  hipLaunchKernelGGL(k, dim3((unsigned)matrices), dim3(NP * 4), lds, st, G, parts, P, info, s);
   return hipGetLastError();
 }
 
 // ---------------------------------------------------------------------------------------------
 // NP = 256: neither LDS nor a wave's registers hold a matrix; each product is a launch of 32 x 32 tiles, its operands from L2
 // ---------------------------------------------------------------------------------------------
-constexpr int N2 = 256, kMat = 2 * N2 * N2;  // fp16 values of a matrix, first terms, then second ones
+constexpr int N2 = 256, kMat = 2 * N2 * N2;  // fp16 values of a matrix, first terms, then second ones (muon_chunk's order)
 
-__device__ __forceinline__ void put4(u16* dst, float s, const float* f) {
-  float v[8];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    v[j] = f[j];
-    v[4 + j] = 0.f;
-  }
-  u32x4 hi, lo;
-  split8(v, s, hi, lo);
-  *(u32x2*)dst = u32x2{hi[0], hi[1]};
-  *(u32x2*)(dst + N2 * N2) = u32x2{lo[0], lo[1]};
+// Workgroup b of tiles of many matrices: matrix and tile. Workgroups go to the eight XCDs in turn; a matrix stays on
+// one, whose L2 then holds what the launches before wrote of it.
+__device__ __forceinline__ bool place(long long matrices, long long* m, int* tile) {
+  const unsigned b = blockIdx.x >> 3;
+  *m = (long long)(b >> 4) * 8 + (blockIdx.x & 7);
+  *tile = b & 15;
+  return *m < matrices;
 }
+unsigned place_blocks(long long matrices) { return (unsigned)((matrices + 7) / 8 * 128); }
 
-// G as fp16 terms from its partial sums; block b: 16 rows of matrix b / 16
+// G as fp16 terms from its partial sums; a tile is 16 rows
 __global__ void __launch_bounds__(256) sum256_kernel(const float* __restrict__ G0, int parts, u16* __restrict__ G,
-                                                     MuonInfo* __restrict__ info, MuonSteps s) {
+                                                     MuonInfo* __restrict__ info, MuonSteps s, long long matrices) {
   __shared__ float scr[4];
-  const long long m = blockIdx.x >> 4;
+  long long m;
+  int tile;
+  if (!place(matrices, &m, &tile)) return;
   const float* src = G0 + m * parts * (N2 * N2);
   float d = 0.f;
-  for (int p = 0; p < parts; ++p) d += src[(size_t)p * (N2 * N2) + (size_t)threadIdx.x * (N2 + 1)];
+  f32x4 f[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) f[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const float* mine = src + tile * (16 * N2) + threadIdx.x * 4;
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    d += src[(size_t)p * (N2 * N2) + (size_t)threadIdx.x * (N2 + 1)];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) f[u] += *(const f32x4*)(mine + (size_t)p * (N2 * N2) + u * 1024);
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) d += __shfl_xor(d, o, 64);
   if ((threadIdx.x & 63) == 0) scr[threadIdx.x >> 6] = d;
   __syncthreads();
   float inv;
   const MuonInfo fo = info_of((scr[0] + scr[1]) + (scr[2] + scr[3]), s, s.p_scale[s.steps - 1], &inv);
-  if (threadIdx.x == 0 && (blockIdx.x & 15) == 0) info[m] = fo;
+  if (threadIdx.x == 0 && tile == 0) info[m] = fo;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    const size_t at = (size_t)(blockIdx.x & 15) * (16 * N2) + (size_t)(u * 256 + threadIdx.x) * 4;
-    float f[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < parts; ++p) {
-      const float4 v = *(const float4*)(src + (size_t)p * (N2 * N2) + at);
-      f[0] += v.x;
-      f[1] += v.y;
-      f[2] += v.z;
-      f[3] += v.w;
-    }
+    // row and inner indices k .. k + 3: half of a unit
+    const int row = tile * 16 + u * 4 + ((int)threadIdx.x >> 6), k = ((int)threadIdx.x & 63) * 4;
+    float v[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = f[j] * inv * inv;
-    put4(G + m * kMat + at, s.g_scale[0], f);
+    for (int j = 0; j < 8; ++j) v[j] = j < 4 ? f[u][j] * inv * inv : 0.f;
+    u32x4 hi, lo;
+    split8(v, s.g_scale[0], hi, lo);
+    u16* dst = G + m * kMat + muon_chunk<N2>(row, k >> 4, (k >> 2) & 1) + (k & 8) / 2;
+    *(u32x2*)dst = u32x2{hi[0], hi[1]};
+    *(u32x2*)(dst + N2 * N2) = u32x2{lo[0], lo[1]};
   }
 }
 
@@ -267,42 +260,68 @@ struct Prod256 {
   float ca, cb, cc, cg;  // where one of the first three is not 0: ca 1 + cb cg A + cc A B
 };
 
-// 64 x 64 tiles of out, a wave 32 x 32; blockIdx.y picks one of two independent products
-__global__ void __launch_bounds__(256) prod256_kernel(Prod256 p0, Prod256 p1) {
+// 64 x 64 tiles of out, 32 x 32 and half of the inner dimension a wave, whose loads are all in flight at once; blockIdx.y
+// picks one of two independent products
+__global__ void __launch_bounds__(512) prod256_kernel(Prod256 p0, Prod256 p1, long long matrices) {
+  __shared__ f32x4 half[4][4][64];
   const Prod256 p = blockIdx.y == 0 ? p0 : p1;
   const int lane = (int)threadIdx.x & 63, g = lane >> 5, l32 = lane & 31, wave = (int)threadIdx.x >> 6;
-  const long long m = blockIdx.x >> 4;
-  const int tile = blockIdx.x & 15;
-  const int r0 = (tile >> 2) * 64 + (wave >> 1) * 32, c0 = (tile & 3) * 64 + (wave & 1) * 32;
-  const u16* A = p.a + m * kMat + (size_t)(r0 + l32) * N2 + 8 * g;
-  const u16* B = p.b + m * kMat + (size_t)(c0 + l32) * N2 + 8 * g;
-  f32x16 acc = zero16();
-#pragma unroll 4
-  for (int k = 0; k < N2; k += 16) {
-    const u32x4 ah = *(const u32x4*)(A + k), al = *(const u32x4*)(A + N2 * N2 + k);
-    const u32x4 bh = *(const u32x4*)(B + k), bl = *(const u32x4*)(B + N2 * N2 + k);
-    acc = mfma<false>(al, bh, acc);
-    acc = mfma<false>(ah, bl, acc);
-    acc = mfma<false>(ah, bh, acc);
+  long long m;
+  int tile;
+  if (!place(matrices, &m, &tile)) return;
+  const int quad = wave & 3, k0 = (wave >> 2) * (N2 / 2);
+  const int r0 = (tile >> 2) * 64 + (quad >> 1) * 32, c0 = (tile & 3) * 64 + (quad & 1) * 32;
+  const u16* A = p.a + m * kMat + muon_chunk<N2>(r0 + l32, k0 / 16, g);
+  const u16* B = p.b + m * kMat + muon_chunk<N2>(c0 + l32, k0 / 16, g);
+  constexpr int KS = N2 / 32;
+  u32x4 ah[KS], al[KS], bh[KS], bl[KS];
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    ah[k] = *(const u32x4*)(A + 512 * k);
+    al[k] = *(const u32x4*)(A + N2 * N2 + 512 * k);
+    bh[k] = *(const u32x4*)(B + 512 * k);
+    bl[k] = *(const u32x4*)(B + N2 * N2 + 512 * k);
   }
-  // lane: column c0 + l32, rows r0 + 8 q + 4 g ..; stored as row c0 + l32 (the matrices are symmetric)
+  __builtin_amdgcn_sched_barrier(0);
+  f32x16 acc = zero16();
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    acc = mfma<false>(al[k], bh[k], acc);
+    acc = mfma<false>(ah[k], bl[k], acc);
+    acc = mfma<false>(ah[k], bh[k], acc);
+  }
+  if (wave >= 4)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) half[quad][q][lane] = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+  __syncthreads();
+  if (wave >= 4) return;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const int r = r0 + 8 * q + 4 * g;
-    const size_t at = (size_t)(c0 + l32) * N2 + r;
-    float f[4];
+    const f32x4 v = half[quad][q][lane];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = acc[4 * q + j] * p.back;
+    for (int j = 0; j < 4; ++j) acc[4 * q + j] += v[j];
+  }
+  // lane: column c0 + l32, rows r0 + 16 h + 4 g + {0..3, 8..11}; stored as that unit of row c0 + l32 (the matrices are symmetric)
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const size_t at = m * kMat + muon_chunk<N2>(c0 + l32, r0 / 16 + h, g);
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = acc[8 * h + j] * p.back;
     if (p.cc != 0.f || p.ca != 0.f || p.cb != 0.f) {
-      const u16* a = p.a + m * kMat + at;
-      const u32x2 h = *(const u32x2*)a, l = *(const u32x2*)(a + N2 * N2);
-      const float v[4] = {lo_f32<false>(h[0]) + lo_f32<false>(l[0]), hi_f32<false>(h[0]) + hi_f32<false>(l[0]),
-                          lo_f32<false>(h[1]) + lo_f32<false>(l[1]), hi_f32<false>(h[1]) + hi_f32<false>(l[1])};
+      const u32x4 vh = *(const u32x4*)(p.a + at), vl = *(const u32x4*)(p.a + at + N2 * N2);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        f[j] = __builtin_fmaf(p.cc, f[j], __builtin_fmaf(p.cb, v[j] * p.cg, r + j == c0 + l32 ? p.ca : 0.f));
+      for (int j = 0; j < 8; ++j) {
+        const float x = j & 1 ? hi_f32<false>(vh[j >> 1]) + hi_f32<false>(vl[j >> 1])
+                              : lo_f32<false>(vh[j >> 1]) + lo_f32<false>(vl[j >> 1]);
+        const int r = r0 + 16 * h + 4 * g + (j & 3) + (j & 4) * 2;
+        f[j] = __builtin_fmaf(p.cc, f[j], __builtin_fmaf(p.cb, x * p.cg, r == c0 + l32 ? p.ca : 0.f));
+      }
     }
-    put4(p.out + m * kMat + at, p.scale, f);
+    u32x4 hi, lo;
+    split8(f, p.scale, hi, lo);
+    *(u32x4*)(p.out + at) = hi;
+    *(u32x4*)(p.out + at + N2 * N2) = lo;
   }
 }
 
@@ -311,11 +330,11 @@ hipError_t launch_256(long long matrices, const float* G0, int parts, u16* P, Mu
   const size_t one = (size_t)matrices * kMat;
   u16* G = (u16*)ws;
   u16 *Q = G + one, *T = Q + one, *R = T + one;
-  hipLaunchKernelGGL(sum256_kernel, dim3((unsigned)(matrices * 16)), dim3(256), 0, st, G0, parts, G, info, s);
+  hipLaunchKernelGGL(sum256_kernel, dim3(place_blocks(matrices)), dim3(256), 0, st, G0, parts, G, info, s, matrices);
   hipError_t e = hipGetLastError();
   const auto run = [&](const Prod256& a, const Prod256* b) {
     if (e != hipSuccess) return;
-    hipLaunchKernelGGL(prod256_kernel, dim3((unsigned)(matrices * 16), b ? 2 : 1), dim3(256), 0, st, a, b ? *b : a);
+    hipLaunchKernelGGL(prod256_kernel, dim3(place_blocks(matrices), b ? 2 : 1), dim3(512), 0, st, a, b ? *b : a, matrices);
     e = hipGetLastError();
   };
   // P_k, the product of the steps' polynomials so far, takes turns in R and P, the last one in P; the first step's Q is P_0
@@ -323,10 +342,11 @@ hipError_t launch_256(long long matrices, const float* G0, int parts, u16* P, Mu
   for (int k = 0; k < s.steps; ++k) {
     const float sg = s.g_scale[k], sq = s.q_scale[k];
     u16* q = k == 0 ? pk(0) : Q;
+    const bool last = k + 1 == s.steps;
     run(Prod256{G, G, q, 1.f / sg / sg, sq, s.a[k], s.b[k], s.c[k], 1.f / sg}, nullptr);
     Prod256 next{};
     if (k > 0) next = Prod256{q, pk(k - 1), pk(k), 1.f / sq / s.p_scale[k - 1], s.p_scale[k], 0.f, 0.f, 0.f, 0.f};
-    if (k + 1 == s.steps) {
+    if (last) {
       if (k > 0) run(next, nullptr);
       break;
     }
