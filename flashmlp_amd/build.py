@@ -24,11 +24,13 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libflashmlp.so"
-# fmlp_bwd.hip and fmlp_gated_dw.hip are compiled once per part (file:part): the kernels of one D each, and the rest
+# fmlp_bwd.hip, fmlp_gated_dw.hip and fmlp_muon.hip are compiled once per part (file:part): the kernels of one D (padded
+# small side) each, and the rest
 SOURCES = ["fmlp_bwd.hip:64", "fmlp_bwd.hip:128", "fmlp_bwd.hip:0", "fmlp_bwd.hip:32", "fmlp_fwd.hip", "fmlp_f32.hip", "fmlp_gen.hip",
-           "fmlp_gated_fwd.hip", "fmlp_gated_dx.hip", "fmlp_gated_dw.hip:128", "fmlp_gated_dw.hip:0", "fmlp_gated_f32.hip", "fmlp_gated_util.hip", "fmlp_join.hip", "fmlp_clip.hip", "fmlp_route.hip", "fmlp_experts.hip", "fmlp_muon.hip", "fmlp_muon_iter.hip", "fmlp_scratch.hip", "fmlp_abi.cpp",
+           "fmlp_gated_fwd.hip", "fmlp_gated_dx.hip", "fmlp_gated_dw.hip:128", "fmlp_gated_dw.hip:0", "fmlp_gated_f32.hip", "fmlp_gated_util.hip", "fmlp_join.hip", "fmlp_clip.hip", "fmlp_route.hip", "fmlp_experts.hip", "fmlp_muon.hip:128", "fmlp_muon.hip:64", "fmlp_muon.hip:32", "fmlp_muon.hip:256",
+           "fmlp_muon_iter.hip", "fmlp_muon_plan.hip", "fmlp_scratch.hip", "fmlp_abi.cpp",
            "fmlp_block_abi.cpp", "fmlp_experts_abi.cpp", "fmlp_muon_abi.cpp"]
-PART_MACRO = {"fmlp_bwd.hip": "FMLP_BWD_PART", "fmlp_gated_dw.hip": "FMLP_GATED_DW_PART"}
+PART_MACRO = {"fmlp_bwd.hip": "FMLP_BWD_PART", "fmlp_gated_dw.hip": "FMLP_GATED_DW_PART", "fmlp_muon.hip": "FMLP_MUON_PART"}
 # Products that write vector registers: with the compiler's choice (accumulation registers, as the kernel holds more
 # than 256 values) every value the activation takes is copied first. dW at H=32 B=16384 D=128 E=1024 bf16 SiLU 728 us,
 # so 707; at D = 256 it is slower (90 us, so 110), the other D do not hold as many.

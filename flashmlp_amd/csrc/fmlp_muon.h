@@ -16,13 +16,13 @@ struct MuonTensor {
   long long H;
   int R, C;
   int x_io, m_io, out_io;  // IoType
-  float lr, keep;          // update: keep out - lr O
+  float lr;                // update: keep out - lr O
 };
 
 // What a call does with every tensor: u = x, or with momenta m' = mu m + nu x, u = m' or (nesterov) nu x + mu m';
 // X = u / (|u| + eps); q(l) = a + b l + c l^2 for each step.
 struct MuonCall {
-  float mu, nu;
+  float mu, nu, keep;
   int nesterov, update;
   float eps;
   int steps;
@@ -51,6 +51,39 @@ struct MuonSteps {
 struct MuonInfo {
   float u_scale, factor;
 };
+// Tensors of a launch, in its arguments.
+constexpr int kMuonTable = 76;
+struct MuonRef {
+  const void* x;
+  void* m;
+  void* out;
+  int R, C;
+  unsigned block0, matrix0;  // the tensor's first workgroup and matrix
+  float lr;
+  unsigned char x_io, m_io, out_io, pad;
+};
+struct MuonTable {
+  MuonRef t[kMuonTable];
+  int n;
+};
+static_assert(sizeof(MuonTable) <= 3712, "kernel arguments");
+// What decides a tensor's kernels beside its padded small side: the terms and type of its Gram matrix's operands (1: 16-bit values as
+// they are, 3: bf16 terms of 32-bit ones), and whether its rows are whole 16-byte vectors.
+struct MuonKind {
+  int terms;
+  bool bf, vec;
+};
+// `parts` workgroups a matrix: partial Gram matrices (and m'); the result from P; all of it by one workgroup a matrix
+// (NP <= 128)
+template <int NP>
+hipError_t muon_gram(const MuonKind& kind, const MuonTable& tab, unsigned blocks, float* G, int parts, const MuonCall& c, hipStream_t st);
+template <int NP>
+hipError_t muon_apply(const MuonKind& kind, const MuonTable& tab, unsigned blocks, const unsigned short* P, const MuonInfo* info,
+                      int parts, const MuonCall& c, int update, hipStream_t st);
+template <int NP>
+hipError_t muon_whole(const MuonKind& kind, const MuonTable& tab, unsigned blocks, const MuonSteps& s, const MuonCall& c, int update,
+                      hipStream_t st);
+
 size_t muon_iter_ws_bytes(int NP, long long matrices);
 hipError_t launch_muon_iter(int NP, long long matrices, const float* G, int parts, unsigned short* P, MuonInfo* info,
                             const MuonSteps& s, void* ws, hipStream_t st);

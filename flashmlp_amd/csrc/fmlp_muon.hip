@@ -17,31 +17,14 @@
 // The long side is contiguous (WIDE) or the small one is (TALL): the same tile, once read along rows and once with the
 // transposing LDS reads, the other way round in the second pass.
 #include <algorithm>
-#include <cmath>
-#include <vector>
+#include <type_traits>
 
 #include "fmlp_muon_device.h"
 
 namespace fmlp {
 namespace {
 
-constexpr int kTable = 64;
-struct Ref {
-  const void* x;
-  void* m;
-  void* out;
-  int R, C;
-  unsigned block0, matrix0;  // the tensor's first workgroup and matrix
-  float lr, keep;
-  unsigned char x_io, m_io, out_io, pad;
-};
-struct Table {
-  Ref t[kTable];
-  int n;
-};
-static_assert(sizeof(Table) <= 3840, "kernel arguments");
-
-__device__ __forceinline__ const Ref& tensor_of(const Table& t, unsigned b) {
+__device__ __forceinline__ const MuonRef& tensor_of(const MuonTable& t, unsigned b) {
   int lo = 0, hi = t.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -55,14 +38,6 @@ __device__ __forceinline__ const Ref& tensor_of(const Table& t, unsigned b) {
 struct Raw {
   u32x4 a, b;
 };
-__device__ __forceinline__ void load_raw(int io, const void* base, long long i, int n, Raw& r) {
-  if (io == IO_F32) {
-    r.a = load_piece<IO_F32>(base, i, n);
-    r.b = load_piece<IO_F32>(base, i + 4, n - 4);
-  } else {
-    r.a = load_piece<IO_F16>(base, i, n);  // (16 bits of any kind)
-  }
-}
 __device__ __forceinline__ void unpack_raw(int io, const Raw& r, float (&f)[8]) {
   if (io == IO_F32) {
 #pragma unroll
@@ -76,22 +51,73 @@ __device__ __forceinline__ void unpack_raw(int io, const Raw& r, float (&f)[8]) 
     unpack_piece<IO_F16>(r.a, f);
   }
 }
-// rounded to the type, stored, and what was stored
-__device__ __forceinline__ void store_rounded(int io, void* base, long long i, int n, float (&f)[8]) {
+// rounded to the type
+__device__ __forceinline__ void pack_raw(int io, const float (&f)[8], Raw& r) {
   if (io == IO_F32) {
-    const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
-    store_piece<IO_F32>(base, i, n, pack_piece<IO_F32>(lo));
-    if (n > 4) store_piece<IO_F32>(base, i + 4, n - 4, pack_piece<IO_F32>(hi));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      r.a[j] = __float_as_uint(f[j]);
+      r.b[j] = __float_as_uint(f[4 + j]);
+    }
   } else if (io == IO_BF16) {
-    const u32x4 v = pack_piece<IO_BF16>(f);
-    store_piece<IO_BF16>(base, i, n, v);
-    unpack_piece<IO_BF16>(v, f);
+    r.a = pack_piece<IO_BF16>(f);
   } else {
-    const u32x4 v = pack_piece<IO_F16>(f);
-    store_piece<IO_F16>(base, i, n, v);
-    unpack_piece<IO_F16>(v, f);
+    r.a = pack_piece<IO_F16>(f);
   }
 }
+
+// A matrix in memory, or none. VEC: rows of whole 16-byte vectors, less than 2^31 bytes: 8 elements are there or not, and loads
+// and stores are the same instructions for every type and place (what is not there is an offset beyond the buffer's end).
+// Branches around them would have the compiler wait for each load where the paths join again: 302 M weights
+// NOVEC us so, VECUS.
+template <bool VEC>
+struct Mat;
+template <>
+struct Mat<true> {
+  Rsrc r;
+  int io;
+  __device__ __forceinline__ Mat(const void* stack, int type, long long h, int R, int C) : io(type) {
+    const int bytes = R * C * (io == IO_F32 ? 4 : 2);
+    r = make_rsrc((const char*)stack + (stack ? (size_t)h * bytes : 0), stack ? bytes : 0);
+  }
+  __device__ __forceinline__ unsigned offset(long long i, int n) const { return n > 0 ? (unsigned)i << (io == IO_F32 ? 2 : 1) : BUF_OOB; }
+  __device__ __forceinline__ void load(long long i, int n, Raw& v) const {
+    const unsigned o = offset(i, n);
+    v.a = buf_load16(r, o);
+    v.b = buf_load16(r, io == IO_F32 ? o + 16 : BUF_OOB);
+  }
+  __device__ __forceinline__ u32x4 load16(long long i, int n) const { return buf_load16(r, n > 0 ? (unsigned)i << 1 : BUF_OOB); }
+  __device__ __forceinline__ void store(long long i, int n, const Raw& v) const {
+    const unsigned o = offset(i, n);
+    __builtin_amdgcn_raw_buffer_store_b128(v.a, r, (int)o, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(v.b, r, (int)(io == IO_F32 ? o + 16 : BUF_OOB), 0, 0);
+  }
+};
+template <>
+struct Mat<false> {
+  char* base;
+  int io;
+  __device__ __forceinline__ Mat(const void* stack, int type, long long h, int R, int C)
+      : base(stack ? (char*)stack + (size_t)h * R * C * (type == IO_F32 ? 4 : 2) : nullptr), io(type) {}
+  __device__ __forceinline__ void load(long long i, int n, Raw& v) const {
+    if (base == nullptr) return;
+    if (io == IO_F32) {
+      v.a = load_piece<IO_F32>(base, i, n);
+      v.b = load_piece<IO_F32>(base, i + 4, n - 4);
+    } else {
+      v.a = load_piece<IO_F16>(base, i, n);  // (16 bits of any kind)
+    }
+  }
+  __device__ __forceinline__ u32x4 load16(long long i, int n) const { return load_piece<IO_F16>(base, i, n); }
+  __device__ __forceinline__ void store(long long i, int n, const Raw& v) const {
+    if (io == IO_F32) {
+      store_piece<IO_F32>(base, i, n, v.a);
+      store_piece<IO_F32>(base, i + 4, n - 4, v.b);
+    } else {
+      store_piece<IO_F16>(base, i, n, v.a);
+    }
+  }
+};
 
 template <int NP>
 constexpr int kTile = NP == 256 ? 32 : 8192 / NP;  // columns of the long side
@@ -187,196 +213,234 @@ __device__ __forceinline__ void split3(const float (&f)[8], u32x4 (&t)[3]) {
   }
 }
 
-// Gram matrices: `parts` workgroups a matrix, each a range of the long side, their partial sums whole and symmetric.
-// TERMS 1: x as it is (BF its type); 3: u in fp32, from x and m.
-template <int NP, bool TALL, int TERMS, bool BF>
-__global__ void __launch_bounds__(256) gram_kernel(Table tab, float* __restrict__ G, int parts, float mu, float nu, int nesterov) {
-  using T = Tile<NP, TALL>;
-  constexpr int KT = T::KT, RB = NP / 32, PAIRS = RB * (RB + 1) / 2;
-  constexpr int KQ = NP <= 64 ? 4 : 1;                   // waves that share the long side's 16s of a tile
-  constexpr int MP = KQ == 4 ? PAIRS : (PAIRS + 3) / 4;  // tile pairs of a wave
-  constexpr int Q = T::UNITS / 256;
-  const Ref& t = tensor_of(tab, blockIdx.x);
+// A workgroup's matrix, and the tiles of it that are its own.
+struct Part {
+  long long h, t0, t1;
+  int part;
+};
+template <int NP, bool TALL>
+__device__ __forceinline__ Part part_of(const MuonRef& t, int parts) {
   const unsigned local = blockIdx.x - t.block0;
-  const long long h = local / (unsigned)parts;
-  const int part = (int)(local % (unsigned)parts);
-  const int R = t.R, C = t.C;
-  const long long L = TALL ? R : C, tiles = (L + KT - 1) / KT, per = (tiles + parts - 1) / parts;
-  const long long t0 = part * per, t1 = min(tiles, t0 + per);
-  const size_t es_x = t.x_io == IO_F32 ? 4 : 2, es_m = t.m_io == IO_F32 ? 4 : 2;
-  const char* X = (const char*)t.x + (size_t)h * R * C * es_x;
-  char* M = t.m ? (char*)t.m + (size_t)h * R * C * es_m : nullptr;
-  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  Part p;
+  p.h = local / (unsigned)parts;
+  p.part = (int)(local % (unsigned)parts);
+  const long long L = TALL ? t.R : t.C, tiles = (L + kTile<NP> - 1) / kTile<NP>, per = (tiles + parts - 1) / parts;
+  p.t0 = p.part * per;
+  p.t1 = min(tiles, p.t0 + per);
+  return p;
+}
+// The 32 x 32 tiles i <= j of a Gram matrix among four waves. From four blocks on a wave has rows i0 and i1 = RB - 1 - i0 of tiles,
+// RB + 1 of them whose operands it reads once each (RB = 8: i0 is the wave, RB = 4: wave / 2); KQ waves share the long side's
+// 16s of a tile of data. Below, every wave has all tiles and a quarter of the 16s.
+template <int NP>
+struct Pairs {
+  static constexpr int RB = NP / 32, KQ = NP == 256 ? 1 : NP == 128 ? 2 : 4;
+  static constexpr int MP = RB >= 4 ? RB + RB / 2 : RB * (RB + 1) / 2;  // sums: row i0's by column, then row i1's from RB / 2 on
+  // tile p of the wave: row, column, whether it has it
+  static __device__ __forceinline__ int i0(int wave) { return wave / KQ; }
+  static __device__ __forceinline__ int kq(int wave) { return wave % KQ; }
+  static __device__ __forceinline__ int row(int p, int wave) { return RB >= 4 ? p < RB ? i0(wave) : RB - 1 - i0(wave) : p < RB ? 0 : 1; }
+  static __device__ __forceinline__ int col(int p, int) { return p < RB ? p : p - RB + RB / 2; }
+  static __device__ __forceinline__ bool has(int p, int wave) { return col(p, wave) >= row(p, wave); }
+};
 
-  // the wave's pairs of 32-row blocks, i <= j
-  int pi[MP], pj[MP];
-  f32x16 acc[MP];
+// The wave's tiles of G over the data tiles [t0, t1), and with a momentum m' on the way. With KQ = 4 the sums are wave
+// 0's. TERMS 1: x as it is (BF its type); 3: u in fp32, from x and m. 256 threads.
+template <int NP, bool TALL, int TERMS, bool BF, bool VEC>
+__device__ __forceinline__ void gram_tiles(f32x16 (&acc)[Pairs<NP>::MP], const MuonRef& t, const Part& part, float mu, float nu,
+                                           int nesterov, int wave) {
+  using T = Tile<NP, TALL>;
+  constexpr int KT = T::KT, KQ = Pairs<NP>::KQ, MP = Pairs<NP>::MP, Q = T::UNITS / 256;
+  const int R = t.R, C = t.C, lane = (int)threadIdx.x & 63;
+  const long long t0 = part.t0, t1 = part.t1;
+  const Mat<VEC> X(t.x, t.x_io, part.h, R, C), M(t.m, t.m_io, part.h, R, C);
+  const bool momentum = t.m != nullptr;
 #pragma unroll
-  for (int p = 0; p < MP; ++p) {
-    int id = KQ == 4 ? p : min(p * 4 + wave, PAIRS - 1), i = 0;
-    while (id >= RB - i) {
-      id -= RB - i;
-      ++i;
-    }
-    pi[p] = i;
-    pj[p] = i + id;
-    acc[p] = zero16();
-  }
+  for (int p = 0; p < MP; ++p) acc[p] = zero16();
 
   Raw x[Q], m[TERMS == 3 ? Q : 1];
-  const auto load = [&](long long tile) {
-#pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const Piece<NP, TALL, 256> at(q, tile * KT, R, C);
-      if constexpr (TERMS == 3) {
-        load_raw(t.x_io, X, at.i, at.n, x[q]);
-        if (M) load_raw(t.m_io, M, at.i, at.n, m[q]);
-      } else {
-        x[q].a = load_piece<IO_F16>(X, at.i, at.n);
-      }
+  const auto load = [&](long long tile, int q) {
+    const Piece<NP, TALL, 256> at(q, tile * KT, R, C);
+    if constexpr (TERMS == 3) {
+      X.load(at.i, at.n, x[q]);
+      M.load(at.i, at.n, m[q]);
+    } else {
+      x[q].a = X.load16(at.i, at.n);
     }
   };
-  const auto put = [&](long long tile) {
+  const auto put = [&](long long tile, int q) {
+    const Piece<NP, TALL, 256> at(q, tile * KT, R, C);
+    const int o = T::at(at.row, at.u);
+    if constexpr (TERMS == 3) {
+      float f[8];
+      unpack_raw(X.io, x[q], f);
+      if (momentum) {
+        float v[8];
+        unpack_raw(M.io, m[q], v);
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const Piece<NP, TALL, 256> at(q, tile * KT, R, C);
-      const int o = T::at(at.row, at.u);
-      if constexpr (TERMS == 3) {
-        float f[8];
-        unpack_raw(t.x_io, x[q], f);
-        if (M) {
-          float v[8];
-          unpack_raw(t.m_io, m[q], v);
+        for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(mu, v[j], nu * f[j]);
+        pack_raw(M.io, v, m[q]);
+        M.store(at.i, at.n, m[q]);
+        unpack_raw(M.io, m[q], v);  // (as it is stored)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(mu, v[j], nu * f[j]);
-          store_rounded(t.m_io, M, at.i, at.n, v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = nesterov ? __builtin_fmaf(mu, v[j], nu * f[j]) : v[j];
-        }
-        u32x4 s[3];
-        split3(f, s);
-#pragma unroll
-        for (int k = 0; k < 3; ++k) lds_write16(k * T::TERM + o, s[k]);
-      } else {
-        lds_write16(o, x[q].a);
+        for (int j = 0; j < 8; ++j) f[j] = nesterov ? __builtin_fmaf(mu, v[j], nu * f[j]) : v[j];
       }
+      u32x4 s[3];
+      split3(f, s);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) lds_write16(k * T::TERM + o, s[k]);
+    } else {
+      lds_write16(o, x[q].a);
     }
   };
 
-  if (t0 < t1) load(t0);
+  if (t0 < t1)
+#pragma unroll
+    for (int q = 0; q < Q; ++q) load(t0, q);
+  using PR = Pairs<NP>;
   for (long long tile = t0; tile < t1; ++tile) {
-    put(tile);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {  // the next tile's loads go out as soon as their registers are free
+      put(tile, q);
+      if (tile + 1 < t1) load(tile + 1, q);
+    }
     __syncthreads();
-    if (tile + 1 < t1) load(tile + 1);
 #pragma unroll
     for (int k = 0; k < KT / 16 / KQ; ++k) {
-      const int k0 = 16 * (KQ == 4 ? k * 4 + wave : k);
+      const int k0 = 16 * (k * KQ + PR::kq(wave));
+      const auto fetch = [&](int block, u32x4 (&v)[TERMS]) {
 #pragma unroll
-      for (int p = 0; p < MP; ++p) {
-        u32x4 a[TERMS], b[TERMS];
+        for (int e = 0; e < TERMS; ++e) v[e] = T::by_small(e * T::TERM, block * 32, k0, lane);
+      };
+      if constexpr (PR::RB >= 4) {
+        u32x4 a[TERMS], c[TERMS];
+        fetch(PR::i0(wave), a);
+        fetch(PR::RB - 1 - PR::i0(wave), c);
 #pragma unroll
-        for (int e = 0; e < TERMS; ++e) {
-          a[e] = T::by_small(e * T::TERM, pi[p] * 32, k0, lane);
-          b[e] = T::by_small(e * T::TERM, pj[p] * 32, k0, lane);
+        for (int j = 0; j < PR::RB; ++j) {
+          if (j < PR::i0(wave)) continue;
+          u32x4 b[TERMS];
+          fetch(j, b);
+          acc[j] = mfma_terms<TERMS, BF>(a, b, acc[j]);
+          if (j >= PR::RB / 2)
+            if (j >= PR::RB - 1 - PR::i0(wave)) acc[PR::RB / 2 + j] = mfma_terms<TERMS, BF>(c, b, acc[PR::RB / 2 + j]);
         }
-        acc[p] = mfma_terms<TERMS, BF>(a, b, acc[p]);
+      } else {
+        u32x4 b[PR::RB][TERMS];
+#pragma unroll
+        for (int j = 0; j < PR::RB; ++j) fetch(j, b[j]);
+#pragma unroll
+        for (int p = 0; p < MP; ++p) acc[p] = mfma_terms<TERMS, BF>(b[PR::row(p, 0)], b[p < PR::RB ? p : 1], acc[p]);
       }
     }
     __syncthreads();
   }
 
-  if constexpr (KQ == 4) {
-    // the four waves' sums, in order
+  if constexpr (KQ > 1) {
+    // the sums of the waves that shared, in order: the first one's
     float* scr = (float*)fmlp_lds;
-    static_assert(3 * MP * 4096 <= 3 * 8192 * 2, "the sums fit a tile's three terms");
-    if (wave > 0)
+    const int kq = PR::kq(wave), set = wave / KQ * (KQ - 1);
+    if (kq > 0)
 #pragma unroll
       for (int p = 0; p < MP; ++p)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) scr[(((wave - 1) * MP + p) * 16 + i) * 64 + lane] = acc[p][i];
+        for (int i = 0; i < 16; ++i) scr[(((set + kq - 1) * MP + p) * 16 + i) * 64 + lane] = acc[p][i];
     __syncthreads();
-    if (wave > 0) return;
+    if (kq == 0)
 #pragma unroll
-    for (int w = 0; w < 3; ++w)
+      for (int w = 0; w < KQ - 1; ++w)
 #pragma unroll
-      for (int p = 0; p < MP; ++p)
+        for (int p = 0; p < MP; ++p)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[p][i] += scr[((w * MP + p) * 16 + i) * 64 + lane];
+          for (int i = 0; i < 16; ++i) acc[p][i] += scr[(((set + w) * MP + p) * 16 + i) * 64 + lane];
+    __syncthreads();
   }
-  float* dst = G + ((size_t)(t.matrix0 + h) * parts + part) * (NP * NP);
+}
+template <int NP, bool TALL, int TERMS>
+constexpr int gram_lds() {
+  return std::max(TERMS * Tile<NP, TALL>::TERM, (4 - 4 / Pairs<NP>::KQ) * Pairs<NP>::MP * 4096);
+}
+
+// the wave's tiles as both halves of a symmetric matrix, rows `pitch` floats apart
+template <int NP>
+__device__ __forceinline__ void store_gram(const f32x16 (&acc)[Pairs<NP>::MP], float* dst, int pitch, int wave,
+                                           int lane) {
   const int g = lane >> 5, l32 = lane & 31;
 #pragma unroll
-  for (int p = 0; p < MP; ++p) {
-    if (KQ == 1 && p * 4 + wave >= PAIRS) continue;
-    const int c = pj[p] * 32 + l32, r = pi[p] * 32 + 4 * g;
+  for (int p = 0; p < Pairs<NP>::MP; ++p) {
+    if (Pairs<NP>::kq(wave) > 0 || !Pairs<NP>::has(p, wave)) continue;
+    const int bi = Pairs<NP>::row(p, wave), bj = Pairs<NP>::col(p, wave);
+    const int c = bj * 32 + l32, r = bi * 32 + 4 * g;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      *(float4*)(dst + (size_t)c * NP + r + 8 * q) = float4{acc[p][4 * q], acc[p][4 * q + 1], acc[p][4 * q + 2], acc[p][4 * q + 3]};
-      if (pi[p] != pj[p])
+      *(float4*)(dst + (size_t)c * pitch + r + 8 * q) = float4{acc[p][4 * q], acc[p][4 * q + 1], acc[p][4 * q + 2], acc[p][4 * q + 3]};
+      if (bi != bj)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) dst[(size_t)(r + 8 * q + j) * NP + c] = acc[p][4 * q + j];
+        for (int j = 0; j < 4; ++j) dst[(size_t)(r + 8 * q + j) * pitch + c] = acc[p][4 * q + j];
     }
   }
 }
 
-// O = P u, and what becomes of it. XT: terms of u. Waves: a block of 32 small indices and CT of 32 long ones each.
-template <int NP, bool TALL, int XT>
-__global__ void __launch_bounds__(NP == 256 ? 512 : 256)
-apply_kernel(Table tab, const u16* __restrict__ P, const MuonInfo* __restrict__ info, int parts, float mu, float nu, int nesterov,
-             int update) {
+// Gram matrices: `parts` workgroups a matrix, each a range of the long side, their partial sums whole and symmetric.
+template <int NP, int TERMS, bool BF, bool VEC>
+__global__ void __launch_bounds__(256) gram_kernel(MuonTable tab, float* __restrict__ G, int parts, float mu, float nu, int nesterov) {
+  const MuonRef& t = tensor_of(tab, blockIdx.x);
+  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  f32x16 acc[Pairs<NP>::MP];
+  Part p;
+  const auto run = [&](auto TALL) {
+    constexpr bool L = decltype(TALL)::value;
+    p = part_of<NP, L>(t, parts);
+    gram_tiles<NP, L, TERMS, BF, VEC>(acc, t, p, mu, nu, nesterov, wave);
+  };
+  if (t.R > t.C) run(std::true_type{});
+  else run(std::false_type{});
+  store_gram<NP>(acc, G + ((size_t)(t.matrix0 + p.h) * parts + p.part) * (NP * NP), NP, wave, lane);
+}
+
+// O = P u over the data tiles [t0, t1), and what becomes of it. XT: terms of u. Waves: a block of 32 small indices, whose rows of P
+// are ph and pl, and CT of 32 long ones each.
+template <int NP, bool TALL, int XT, bool VEC>
+__device__ __forceinline__ void apply_tiles(const u32x4 (&ph)[NP / 16], const u32x4 (&pl)[NP / 16], const MuonRef& t, const Part& part,
+                                            MuonInfo fo, float mu, float nu, int nesterov, int update, float keep, int wave) {
   using T = Tile<NP, TALL>;
   constexpr int THREADS = NP == 256 ? 512 : 256;
   constexpr int KT = T::KT, RB = NP / 32, CT = NP == 256 ? 1 : 2, KS = NP / 16, Q = T::UNITS / THREADS;
   constexpr int OPITCH = T::COLS + 4;  // floats between the result's rows in LDS
-  const Ref& t = tensor_of(tab, blockIdx.x);
-  const unsigned local = blockIdx.x - t.block0;
-  const long long h = local / (unsigned)parts;
-  const int part = (int)(local % (unsigned)parts);
-  const int R = t.R, C = t.C;
-  const long long L = TALL ? R : C, tiles = (L + KT - 1) / KT, per = (tiles + parts - 1) / parts;
-  const long long t0 = part * per, t1 = min(tiles, t0 + per);
-  if (t0 >= t1) return;
-  const size_t es_x = t.x_io == IO_F32 ? 4 : 2, es_m = t.m_io == IO_F32 ? 4 : 2, es_o = t.out_io == IO_F32 ? 4 : 2;
-  const char* X = (const char*)t.x + (size_t)h * R * C * es_x;
-  const char* M = t.m ? (const char*)t.m + (size_t)h * R * C * es_m : nullptr;
-  char* O = (char*)t.out + (size_t)h * R * C * es_o;
-  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int g = lane >> 5, l32 = lane & 31;
+  const int R = t.R, C = t.C, lane = (int)threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
   const int s0 = (wave % RB) * 32, c0 = wave / RB * CT * 32;
-  const MuonInfo fo = info[t.matrix0 + h];
-
-  // the wave's rows of P
-  u32x4 ph[KS], pl[KS];
-  const u16* src = P + (size_t)(t.matrix0 + h) * (2 * NP * NP) + muon_chunk<NP>(s0 + l32, 0, g);
-#pragma unroll
-  for (int k = 0; k < KS; ++k) {
-    ph[k] = *(const u32x4*)(src + 512 * k);
-    pl[k] = *(const u32x4*)(src + NP * NP + 512 * k);
-  }
-
+  const long long t0 = part.t0, t1 = part.t1;
+  const Mat<VEC> X(t.x, t.x_io, part.h, R, C), M(t.m, t.m_io, part.h, R, C), O(t.out, t.out_io, part.h, R, C);
+  const bool momentum = t.m != nullptr;
   Raw x[Q], m[Q], w[Q];
-  const auto load = [&](long long tile) {
-#pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const Piece<NP, TALL, THREADS> at(q, tile * KT, R, C);
-      load_raw(t.x_io, X, at.i, at.n, x[q]);
-      if (M) load_raw(t.m_io, M, at.i, at.n, m[q]);
-    }
+  const auto load = [&](long long tile, int q) {
+    const Piece<NP, TALL, THREADS> at(q, tile * KT, R, C);
+    X.load(at.i, at.n, x[q]);
+    M.load(at.i, at.n, m[q]);
   };
   float* res = (float*)fmlp_lds;  // the result takes the tile's place
-  load(t0);
+#pragma unroll
+  for (int q = 0; q < Q; ++q) load(t0, q);
   for (long long tile = t0; tile < t1; ++tile) {
+    if (update) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const Piece<NP, TALL, THREADS> at(q, tile * KT, R, C);
+        O.load(at.i, at.n, w[q]);
+      }
+    }
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const Piece<NP, TALL, THREADS> at(q, tile * KT, R, C);
       float f[8];
-      unpack_raw(t.x_io, x[q], f);
-      if (M) {
+      unpack_raw(X.io, x[q], f);
+      if (momentum) {
         float v[8];
-        unpack_raw(t.m_io, m[q], v);
+        unpack_raw(M.io, m[q], v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = nesterov ? __builtin_fmaf(mu, v[j], nu * f[j]) : v[j];
       }
+      if (tile + 1 < t1) load(tile + 1, q);
       u32x4 hi, lo;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -388,14 +452,6 @@ apply_kernel(Table tab, const u16* __restrict__ P, const MuonInfo* __restrict__ 
       if constexpr (XT == 2) T::put_by_long(T::TERM, at.row, at.u, lo);
     }
     __syncthreads();
-    if (update) {
-#pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        const Piece<NP, TALL, THREADS> at(q, tile * KT, R, C);
-        load_raw(t.out_io, O, at.i, at.n, w[q]);
-      }
-    }
-    if (tile + 1 < t1) load(tile + 1);
     f32x16 acc[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[c] = zero16();
@@ -434,266 +490,297 @@ apply_kernel(Table tab, const u16* __restrict__ P, const MuonInfo* __restrict__ 
       }
       if (update) {
         float v[8];
-        unpack_raw(t.out_io, w[q], v);
+        unpack_raw(O.io, w[q], v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = __builtin_fmaf(-t.lr, f[j], v[j] * t.keep);
+        for (int j = 0; j < 8; ++j) f[j] = __builtin_fmaf(-t.lr, f[j], v[j] * keep);
       }
-      store_rounded(t.out_io, O, at.i, at.n, f);
+      pack_raw(O.io, f, w[q]);
+      O.store(at.i, at.n, w[q]);
     }
     __syncthreads();
   }
 }
-
-template <int NP, bool TALL, int TERMS, bool BF>
-hipError_t run_gram(const Table& tab, unsigned blocks, float* G, int parts, const MuonCall& c, hipStream_t st) {
-  using T = Tile<NP, TALL>;
-  constexpr int lds = std::max(TERMS * T::TERM, NP <= 64 ? 3 * NP / 32 * (NP / 32 + 1) / 2 * 4096 : 0);
-  auto k = gram_kernel<NP, TALL, TERMS, BF>;
-  static std::atomic<unsigned long long> done{0};
-  const hipError_t e = set_lds_once((const void*)k, lds, done);
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(k, dim3(blocks), dim3(256), lds, st, tab, G, parts, c.mu, c.nu, c.nesterov);
-  return hipGetLastError();
-}
 template <int NP, bool TALL, int XT>
-hipError_t run_apply(const Table& tab, unsigned blocks, const u16* P, const MuonInfo* info, int parts, const MuonCall& c,
-                     int update, hipStream_t st) {
-  using T = Tile<NP, TALL>;
-  constexpr int lds = std::max(XT * T::TERM, T::ROWS * (T::COLS + 4) * 4);
-  auto k = apply_kernel<NP, TALL, XT>;
-  static std::atomic<unsigned long long> done{0};
-  const hipError_t e = set_lds_once((const void*)k, lds, done);
+constexpr int apply_lds() {
+  return std::max(XT * Tile<NP, TALL>::TERM, Tile<NP, TALL>::ROWS * (Tile<NP, TALL>::COLS + 4) * 4);
+}
+
+template <int NP, int XT, bool VEC>
+__global__ void __launch_bounds__(NP == 256 ? 512 : 256)
+apply_kernel(MuonTable tab, const u16* __restrict__ P, const MuonInfo* __restrict__ info, int parts, float mu, float nu, int nesterov,
+             int update, float keep) {
+  const MuonRef& t = tensor_of(tab, blockIdx.x);
+  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const auto run = [&](auto TALL) {
+    constexpr bool L = decltype(TALL)::value;
+    const Part p = part_of<NP, L>(t, parts);
+    if (p.t0 >= p.t1) return;
+    u32x4 ph[NP / 16], pl[NP / 16];
+    const u16* src = P + (size_t)(t.matrix0 + p.h) * (2 * NP * NP) + muon_chunk<NP>((wave % (NP / 32)) * 32 + (lane & 31), 0, lane >> 5);
+#pragma unroll
+    for (int k = 0; k < NP / 16; ++k) {
+      ph[k] = *(const u32x4*)(src + 512 * k);
+      pl[k] = *(const u32x4*)(src + NP * NP + 512 * k);
+    }
+    apply_tiles<NP, L, XT, VEC>(ph, pl, t, p, info[t.matrix0 + p.h], mu, nu, nesterov, update, keep, wave);
+  };
+  if (t.R > t.C) run(std::true_type{});
+  else run(std::false_type{});
+}
+
+// ---------------------------------------------------------------------------------------------
+// a workgroup a matrix from end to end, NP <= 128
+// ---------------------------------------------------------------------------------------------
+// byte offset of 16-byte unit u of row r of a [NP][NP] fp16 matrix: units are swapped within a row so that 16
+// consecutive rows' units lie on all banks
+template <int NP>
+__device__ __forceinline__ int unit_off(int r, int u) {
+  constexpr int UR = NP / 8;  // units of a row
+  const int f = UR >= 16 ? r & 15 : UR == 8 ? (r >> 1) & 7 : (r >> 2) & 3;
+  return r * (NP * 2) + ((u ^ f) << 4);
+}
+
+// A wave's 32 columns of a matrix as both fp16 terms: unit (tile t, half h) of the lane of column n and half g holds
+// rows 32 t + 16 h + 4 g + {0..3, 8..11}, the order that a result has them in
+template <int NP>
+struct Cols {
+  u32x4 hi[NP / 16], lo[NP / 16];
+};
+template <int NP>
+__device__ __forceinline__ void pack_cols(const f32x16 (&v)[NP / 32], float s, Cols<NP>& c) {
+#pragma unroll
+  for (int t = 0; t < NP / 32; ++t)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = v[t][8 * h + j];
+      split8(f, s, c.hi[2 * t + h], c.lo[2 * t + h]);
+    }
+}
+// the columns as rows of the left operand
+template <int NP>
+__device__ __forceinline__ void put_left(const Cols<NP>& c, int n, int g) {
+#pragma unroll
+  for (int k = 0; k < NP / 16; ++k) {
+    const int at = unit_off<NP>(n, 2 * k + g);
+    lds_write16(at, c.hi[k]);
+    lds_write16(NP * NP * 2 + at, c.lo[k]);
+  }
+}
+
+// out = (left operand in LDS) * b, in the terms' scales. A step has 16 of the inner dimension for two tiles of rows: their
+// operands are read a step ahead.
+template <int NP>
+__device__ __forceinline__ void product(f32x16 (&out)[NP / 32], const Cols<NP>& b, int g, int l32) {
+  constexpr int RB = NP / 32, TP = RB < 2 ? RB : 2, PAIRS = RB / TP, STEPS = NP / 16 * PAIRS;
+  u32x4 ah[2][TP], al[2][TP];
+  const auto fetch = [&](int j) {
+    const int k = j / PAIRS, p = j % PAIRS;
+#pragma unroll
+    for (int t = 0; t < TP; ++t) {
+      const int at = unit_off<NP>(l32, 2 * k + g) + (p * TP + t) * (32 * NP * 2);
+      ah[j & 1][t] = lds_read16(at);
+      al[j & 1][t] = lds_read16(NP * NP * 2 + at);
+    }
+  };
+  fetch(0);
+#pragma unroll
+  for (int j = 0; j < STEPS; ++j) {
+    const int k = j / PAIRS, p = j % PAIRS;
+    if (j + 1 < STEPS) fetch(j + 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < TP; ++t) out[p * TP + t] = mfma<false>(al[j & 1][t], b.hi[k], k == 0 ? zero16() : out[p * TP + t]);
+#pragma unroll
+    for (int t = 0; t < TP; ++t) out[p * TP + t] = mfma<false>(ah[j & 1][t], b.lo[k], out[p * TP + t]);
+#pragma unroll
+    for (int t = 0; t < TP; ++t) out[p * TP + t] = mfma<false>(ah[j & 1][t], b.hi[k], out[p * TP + t]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// Gram matrix, steps and result of one matrix: two workgroups a CU, one of which streams while the other is at its steps. The steps are
+// those of fmlp_muon_iter.hip with 32 columns a wave (the first NP / 32 waves), which reads a left operand half as often.
+template <int NP, int TERMS, bool BF, bool VEC>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+whole_kernel(MuonTable tab, MuonSteps s, float mu, float nu, int nesterov, int update, float keep) {
+  constexpr int RB = NP / 32, GP = NP + 4, SCR = NP * GP * 4;  // LDS: G or the left operand, then the waves' sums
+  const MuonRef& t = tensor_of(tab, blockIdx.x);
+  const bool tall = t.R > t.C;
+  const Part part = tall ? part_of<NP, true>(t, 1) : part_of<NP, false>(t, 1);
+  const int lane = (int)threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = wave * 32 + l32;
+  float* lds = (float*)fmlp_lds;
+  {
+      f32x16 acc[Pairs<NP>::MP];
+    if (tall) gram_tiles<NP, true, TERMS, BF, VEC>(acc, t, part, mu, nu, nesterov, wave);
+    else gram_tiles<NP, false, TERMS, BF, VEC>(acc, t, part, mu, nu, nesterov, wave);
+    store_gram<NP>(acc, lds, GP, wave, lane);
+  }
+  __syncthreads();
+  const bool on = wave < RB;
+  f32x16 v[RB];
+  const auto diagonal = [&](int tile, int i) { return tile == wave && 8 * (i >> 2) + 4 * g + (i & 3) == l32; };
+  float d = 0.f;
+  if (on) {
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 f = *(const float4*)(lds + n * GP + 32 * r + 8 * q + 4 * g);
+        v[r][4 * q] = f.x;
+        v[r][4 * q + 1] = f.y;
+        v[r][4 * q + 2] = f.z;
+        v[r][4 * q + 3] = f.w;
+      }
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (diagonal(r, i)) d = v[r][i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) d += __shfl_xor(d, o, 64);
+    if (lane == 0) *(float*)(fmlp_lds + SCR + 4 * wave) = d;
+  }
+  __syncthreads();
+  float trace = 0.f;
+#pragma unroll
+  for (int w = 0; w < RB; ++w) trace += *(const float*)(fmlp_lds + SCR + 4 * w);
+  float inv;
+  const MuonInfo fo = info_of(trace, s, s.p_scale[s.steps - 1], &inv);
+  Cols<NP> G, P;
+  if (on) {
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[r][i] = v[r][i] * inv * inv;
+    pack_cols<NP>(v, s.g_scale[0], G);
+  }
+  for (int k = 0; k < s.steps; ++k) {
+    const float sg = s.g_scale[k], sq = s.q_scale[k], st = sg * sq * 0x1p-14f;
+    const bool last = k + 1 == s.steps;
+    if (on) put_left<NP>(G, n, g);
+    __syncthreads();
+    if (on) {
+      product<NP>(v, G, g, l32);
+      const float cc = s.c[k] / sg / sg, cb = s.b[k] / sg, ca = s.a[k];
+#pragma unroll
+      for (int u = 0; u < NP / 16; ++u) {
+        float f[8];
+        const u32x4 gh = G.hi[u], gl = G.lo[u];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float x = j & 1 ? hi_f32<false>(gh[j >> 1]) + hi_f32<false>(gl[j >> 1])
+                                : lo_f32<false>(gh[j >> 1]) + lo_f32<false>(gl[j >> 1]);
+          const int i = 8 * (u & 1) + j;
+          f[j] = __builtin_fmaf(cc, v[u >> 1][i], __builtin_fmaf(cb, x, diagonal(u >> 1, i) ? ca : 0.f));
+        }
+        split8(f, sq, G.hi[u], G.lo[u]);
+      }
+      if (!last) product<NP>(v, G, g, l32);
+    }
+    __syncthreads();
+    if (on) put_left<NP>(G, n, g);
+    __syncthreads();
+    if (on) {
+      if (k == 0) P = G;
+      if (!last) pack_cols<NP>(v, st / sg / sq, G);
+      if (k > 0) {
+        product<NP>(v, P, g, l32);
+        pack_cols<NP>(v, s.p_scale[k] / sq / s.p_scale[k - 1], P);
+      }
+      if (!last) {
+        product<NP>(v, G, g, l32);
+        pack_cols<NP>(v, s.g_scale[k + 1] / sq / st, G);
+      }
+    }
+    __syncthreads();
+  }
+  // every wave's rows of P
+  if (on) put_left<NP>(P, n, g);
+  __syncthreads();
+  u32x4 ph[NP / 16], pl[NP / 16];
+  const int row = (wave % RB) * 32 + l32;
+#pragma unroll
+  for (int k = 0; k < NP / 16; ++k) {
+    ph[k] = lds_read16(unit_off<NP>(row, 2 * k + g));
+    pl[k] = lds_read16(NP * NP * 2 + unit_off<NP>(row, 2 * k + g));
+  }
+  __syncthreads();
+  constexpr int XT = TERMS == 3 ? 2 : 1;
+  if (tall) apply_tiles<NP, true, XT, VEC>(ph, pl, t, part, fo, mu, nu, nesterov, update, keep, wave);
+  else apply_tiles<NP, false, XT, VEC>(ph, pl, t, part, fo, mu, nu, nesterov, update, keep, wave);
+}
+
+template <int NP, int TERMS>
+constexpr int both_gram_lds() {
+  return std::max(gram_lds<NP, true, TERMS>(), gram_lds<NP, false, TERMS>());
+}
+template <int NP, int XT>
+constexpr int both_apply_lds() {
+  return std::max(apply_lds<NP, true, XT>(), apply_lds<NP, false, XT>());
+}
+// f(terms of G, whether they are bf16, whole vectors) as constants
+template <typename F>
+hipError_t by_kind(const MuonKind& k, F f) {
+  const auto v = [&](auto terms, auto bf) { return k.vec ? f(terms, bf, std::true_type{}) : f(terms, bf, std::false_type{}); };
+  if (k.terms == 3) return v(std::integral_constant<int, 3>{}, std::true_type{});
+  return k.bf ? v(std::integral_constant<int, 1>{}, std::true_type{}) : v(std::integral_constant<int, 1>{}, std::false_type{});
+}
+template <int LDS, typename K, typename... A>
+hipError_t launch(K k, std::atomic<unsigned long long>& done, unsigned blocks, int threads, hipStream_t st, A... args) {
+  const hipError_t e = set_lds_once((const void*)k, LDS, done);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(k, dim3(blocks), dim3(NP == 256 ? 512 : 256), lds, st, tab, P, info, parts, c.mu, c.nu, c.nesterov, update);
+  hipLaunchKernelGGL(k, dim3(blocks), dim3(threads), LDS, st, args...);
   return hipGetLastError();
 }
-
-// f(NP, TALL) as constants
-template <typename F>
-hipError_t by_shape(int NP, bool tall, F f) {
-  const auto t = [&](auto n) { return tall ? f(n, std::true_type{}) : f(n, std::false_type{}); };
-  switch (NP) {
-    case 32: return t(std::integral_constant<int, 32>{});
-    case 64: return t(std::integral_constant<int, 64>{});
-    case 128: return t(std::integral_constant<int, 128>{});
-    default: return t(std::integral_constant<int, 256>{});
-  }
-}
-
-int padded(const MuonTensor& t) {
-  const int n = std::min(t.R, t.C);
-  return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : 256;
-}
-// what decides a tensor's kernels: padded small side, orientation, the terms and type of its Gram matrix
-struct Kind {
-  int NP;
-  bool tall;
-  int terms;  // 1: 16-bit values as they are
-  bool bf;
-  bool operator==(const Kind& o) const { return NP == o.NP && tall == o.tall && terms == o.terms && bf == o.bf; }
-};
-Kind kind_of(const MuonTensor& t) {
-  const bool raw = t.m == nullptr && t.x_io != IO_F32;
-  return Kind{padded(t), t.R > t.C, raw ? 1 : 3, !raw || t.x_io == IO_BF16};
-}
-
-// The matrices of one padded size: their Gram matrices and what comes of them go through the workspace together.
-struct Group {
-  int NP;
-  long long matrices, tiles;  // tiles: of the longest one
-  int gram_parts, apply_parts;
-  size_t g_off, p_off, info_off, iter_off, end;
-};
-Group group_of(int NP, int n, const MuonTensor* t, int cus) {
-  Group r{};
-  r.NP = NP;
-  const int KT = NP == 256 ? 32 : 8192 / NP;
-  for (int i = 0; i < n; ++i)
-    if (t[i].H > 0 && t[i].R > 0 && t[i].C > 0 && padded(t[i]) == NP) {
-      r.matrices += t[i].H;
-      r.tiles = std::max(r.tiles, ((long long)std::max(t[i].R, t[i].C) + KT - 1) / KT);
-    }
-  if (r.matrices == 0) return r;
-  // three workgroups a CU at least, as far as there are tiles; of Gram matrices no more than pay: a tile takes about
-  // 2.5 us, a part's sums are written and read at about 4 TB/s (8 matrices of 256 x 1024: 32 parts 18 + 46 us, 9 PARTS9)
-  const long long want = (3LL * cus + r.matrices - 1) / r.matrices;
-  const double part_us = (double)r.matrices * NP * NP * 8 / 4e6;
-  const long long pays = std::max(1LL, std::llround(std::sqrt((double)r.tiles * 2.5 / part_us)));
-  r.gram_parts = (int)std::max(1LL, std::min(std::min(want, pays), r.tiles));
-  r.apply_parts = (int)std::max(1LL, std::min(want, r.tiles));
-  const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
-  r.p_off = up((size_t)r.matrices * r.gram_parts * NP * NP * 4);
-  r.info_off = r.p_off + up((size_t)r.matrices * NP * NP * 4);
-  r.iter_off = r.info_off + up((size_t)r.matrices * sizeof(MuonInfo));
-  r.end = r.iter_off + up(muon_iter_ws_bytes(NP, r.matrices));
-  return r;
-}
-constexpr int kSizes[4] = {32, 64, 128, 256};
-
-// Powers of two that bring each stage's values to at most 2^14 as fp16: bounds of the eigenvalues of G, Q and P from
-// the steps' polynomials over the range that G's have, which is [0, 1] at first. Returns the range after the steps.
-double set_steps(MuonSteps* s, const MuonCall& c, int first, int steps, bool normalise, double range) {
-  s->steps = steps;
-  s->normalise = normalise;
-  s->eps = c.eps;
-  double p = 1;
-  const auto scale = [](double bound) {
-    int e = 0;
-    if (!(bound < 1e30)) bound = 1e30;
-    (void)std::frexp(std::max(bound, 1e-30), &e);
-    return std::ldexp(1.f, 14 - e);
-  };
-  for (int k = 0; k < steps; ++k) {
-    const float* v = c.abc[first + k];
-    s->a[k] = v[0];
-    s->b[k] = v[1];
-    s->c[k] = v[2];
-    double q = 0, next = 0;
-    const int N = 512;
-    for (int i = 0; i <= N; ++i) {
-      const double l = range * 1.02 * i / N, y = v[0] + l * (v[1] + l * v[2]);
-      q = std::max(q, std::fabs(y));
-      next = std::max(next, l * y * y);
-    }
-    q *= 1.02;
-    p *= q;
-    s->g_scale[k] = scale(range * 1.02);
-    s->q_scale[k] = scale(q);
-    s->p_scale[k] = scale(p);
-    range = next * 1.02;
-  }
-  return range;
-}
-
-struct Pass {
-  const void* x;
-  void* m;
-  void* out;
-  int x_io, m_io, out_io, update;
-};
 
 }  // namespace
 
-MuonPlan muon_plan(int n, const MuonTensor* t, const MuonCall& c, int num_cus) {
-  MuonPlan p{};
-  for (int NP : kSizes) {
-    const Group g = group_of(NP, n, t, num_cus);
-    if (g.matrices) p.ws_bytes = std::max(p.ws_bytes, g.end);
-  }
-  // more steps than a Gram matrix serves: the matrices between the stages in fp32, in the result where that is fp32
-  size_t between = 0;
-  if (c.steps > c.stage)
-    for (int i = 0; i < n; ++i)
-      if (c.update || t[i].out_io != IO_F32) between += ((size_t)t[i].H * t[i].R * t[i].C * 4 + 255) / 256 * 256;
-  p.ws_bytes += between;
-  return p;
+template <int NP>
+hipError_t muon_gram(const MuonKind& kind, const MuonTable& tab, unsigned blocks, float* G, int parts, const MuonCall& c, hipStream_t st) {
+  return by_kind(kind, [&](auto T, auto B, auto V) {
+    constexpr int TERMS = decltype(T)::value;
+    static std::atomic<unsigned long long> done{0};
+    return launch<both_gram_lds<NP, TERMS>()>(gram_kernel<NP, TERMS, decltype(B)::value, decltype(V)::value>, done, blocks, 256, st,
+                                              tab, G, parts, c.mu, c.nu, c.nesterov);
+  });
+}
+template <int NP>
+hipError_t muon_apply(const MuonKind& kind, const MuonTable& tab, unsigned blocks, const unsigned short* P, const MuonInfo* info,
+                      int parts, const MuonCall& c, int update, hipStream_t st) {
+  return by_kind(kind, [&](auto T, auto B, auto V) -> hipError_t {
+    constexpr int XT = decltype(T)::value == 3 ? 2 : 1;
+    if constexpr (XT == 1 && !decltype(B)::value) {
+      return hipErrorInvalidValue;  // (16-bit values of either type are one kind here: muon_apply's callers say bf)
+    } else {
+      static std::atomic<unsigned long long> done{0};
+      return launch<both_apply_lds<NP, XT>()>(apply_kernel<NP, XT, decltype(V)::value>, done, blocks, NP == 256 ? 512 : 256, st, tab, P,
+                                              info, parts, c.mu, c.nu, c.nesterov, update, c.keep);
+    }
+  });
+}
+template <int NP>
+hipError_t muon_whole(const MuonKind& kind, const MuonTable& tab, unsigned blocks, const MuonSteps& s, const MuonCall& c, int update,
+                      hipStream_t st) {
+  return by_kind(kind, [&](auto T, auto B, auto V) {
+    constexpr int TERMS = decltype(T)::value;
+    constexpr int lds = std::max(std::max(both_gram_lds<NP, TERMS>(), both_apply_lds<NP, TERMS == 3 ? 2 : 1>()), NP * (NP + 4) * 4 + 16);
+    static_assert(lds <= 80 * 1024, "two workgroups a CU");
+    static std::atomic<unsigned long long> done{0};
+    return launch<lds>(whole_kernel<NP, TERMS, decltype(B)::value, decltype(V)::value>, done, blocks, 256, st, tab, s, c.mu, c.nu,
+                       c.nesterov, update, c.keep);
+  });
 }
 
-hipError_t launch_muon(int n, const MuonTensor* t, const MuonCall& c, int num_cus, void* ws, hipStream_t st) {
-  size_t shared = 0;
-  for (int NP : kSizes) {
-    const Group g = group_of(NP, n, t, num_cus);
-    if (g.matrices) shared = std::max(shared, g.end);
-  }
-  char* between0 = (char*)ws + shared;
-  for (int NP : kSizes) {
-    const Group gr = group_of(NP, n, t, num_cus);
-    if (gr.matrices == 0) continue;
-    float* G = (float*)ws;
-    u16* P = (u16*)((char*)ws + gr.p_off);
-    MuonInfo* info = (MuonInfo*)((char*)ws + gr.info_off);
-    double range = 1;
-    for (int first = 0; first < c.steps; first += c.stage) {
-      const int steps = std::min(c.stage, c.steps - first);
-      const bool start = first == 0, last = first + steps == c.steps;
-      MuonSteps s{};
-      range = set_steps(&s, c, first, steps, start, range);
-      const auto pass_of = [&](int i, char* y) {
-        Pass p{t[i].x, t[i].m, t[i].out, t[i].x_io, t[i].m_io, t[i].out_io, c.update};
-        const bool own = !c.update && t[i].out_io == IO_F32;  // the result holds what is between the stages
-        void* b = own ? t[i].out : (void*)y;
-        if (!start) p = Pass{b, nullptr, p.out, IO_F32, 0, p.out_io, p.update};
-        if (!last) {
-          p.out = b;
-          p.out_io = IO_F32;
-          p.update = 0;
-        }
-        return p;
-      };
-      // f(kind, table, workgroups, update) for tables of tensors of one kind
-      const auto tables = [&](int parts, bool gram, auto f) -> hipError_t {
-        std::vector<Kind> done;
-        for (int a = 0; a < n; ++a) {
-          if (t[a].H == 0 || t[a].R == 0 || t[a].C == 0 || padded(t[a]) != NP) continue;
-          const auto kind_at = [&](int i) {
-            MuonTensor u = t[i];
-            if (!start) {
-              u.m = nullptr;
-              u.x_io = IO_F32;
-            }
-            return kind_of(u);
-          };
-          const Kind k = kind_at(a);
-          if (std::find(done.begin(), done.end(), k) != done.end()) continue;
-          done.push_back(k);
-          Table tab{};
-          long long blocks = 0, matrix = 0;
-          char* y = between0;
-          const auto flush = [&]() -> hipError_t {
-            const hipError_t e = tab.n ? f(k, tab, (unsigned)blocks) : hipSuccess;
-            tab.n = 0;
-            blocks = 0;
-            return e;
-          };
-          for (int i = 0; i < n; ++i) {
-            char* mine = y;
-            if (c.steps > c.stage && (c.update || t[i].out_io != IO_F32)) y += ((size_t)t[i].H * t[i].R * t[i].C * 4 + 255) / 256 * 256;
-            if (t[i].H == 0 || t[i].R == 0 || t[i].C == 0 || padded(t[i]) != NP) continue;
-            const long long first_matrix = matrix;
-            matrix += t[i].H;
-            if (i < a || !(kind_at(i) == k)) continue;
-            const long long b = t[i].H * parts;
-            if (b > 0x7fffffffLL) return hipErrorInvalidValue;
-            if (tab.n == kTable || blocks + b > 0x7fffffffLL) {
-              const hipError_t e = flush();
-              if (e != hipSuccess) return e;
-            }
-            const Pass p = pass_of(i, mine);
-            Ref& r = tab.t[tab.n++];
-            r = Ref{p.x, p.m, p.out, t[i].R, t[i].C, (unsigned)blocks, (unsigned)first_matrix, t[i].lr, t[i].keep,
-                    (unsigned char)p.x_io, (unsigned char)p.m_io, (unsigned char)p.out_io, 0};
-            blocks += b;
-          }
-          const hipError_t e = flush();
-          if (e != hipSuccess) return e;
-        }
-        (void)gram;
-        return hipSuccess;
-      };
-      hipError_t e = tables(gr.gram_parts, true, [&](const Kind& k, const Table& tab, unsigned blocks) {
-        return by_shape(NP, k.tall, [&](auto np, auto tall) {
-          constexpr int N = decltype(np)::value;
-          constexpr bool L = decltype(tall)::value;
-          if (k.terms == 3) return run_gram<N, L, 3, true>(tab, blocks, G, gr.gram_parts, c, st);
-          return k.bf ? run_gram<N, L, 1, true>(tab, blocks, G, gr.gram_parts, c, st)
-                      : run_gram<N, L, 1, false>(tab, blocks, G, gr.gram_parts, c, st);
-        });
-      });
-      if (e == hipSuccess) e = launch_muon_iter(NP, gr.matrices, G, gr.gram_parts, P, info, s, (char*)ws + gr.iter_off, st);
-      if (e == hipSuccess)
-        e = tables(gr.apply_parts, false, [&](const Kind& k, const Table& tab, unsigned blocks) {
-          return by_shape(NP, k.tall, [&](auto np, auto tall) {
-            constexpr int N = decltype(np)::value;
-            constexpr bool L = decltype(tall)::value;
-            const int update = c.update && last;
-            return k.terms == 3 ? run_apply<N, L, 2>(tab, blocks, P, info, gr.apply_parts, c, update, st)
-                                : run_apply<N, L, 1>(tab, blocks, P, info, gr.apply_parts, c, update, st);
-          });
-        });
-      if (e != hipSuccess) return e;
-    }
-  }
-  return hipSuccess;
-}
+// this part's kernels
+template hipError_t muon_gram<FMLP_MUON_PART>(const MuonKind&, const MuonTable&, unsigned, float*, int, const MuonCall&, hipStream_t);
+template hipError_t muon_apply<FMLP_MUON_PART>(const MuonKind&, const MuonTable&, unsigned, const unsigned short*, const MuonInfo*, int,
+                                               const MuonCall&, int, hipStream_t);
+#if FMLP_MUON_PART <= 128
+template hipError_t muon_whole<FMLP_MUON_PART>(const MuonKind&, const MuonTable&, unsigned, const MuonSteps&, const MuonCall&, int,
+                                               hipStream_t);
+#endif
 
 }  // namespace fmlp

@@ -123,7 +123,7 @@ FMLP_EXPORT int fmlp_orthogonalize(const void* x, void* out, int64_t H, int64_t 
 
 namespace {
 
-int take(int n, const fmlp_muon_tensor* tensors, double lr, double weight_decay, bool pointers, std::vector<fmlp::MuonTensor>* out,
+int take(int n, const fmlp_muon_tensor* tensors, double lr, bool pointers, std::vector<fmlp::MuonTensor>* out,
          std::vector<fmlp::MemRange>* ranges) {
   if (n < 0) return abi_fail(FMLP_ERR_INVALID_ARG, "%d stacks", n);
   if (n > 0 && tensors == nullptr) return abi_fail(FMLP_ERR_INVALID_ARG, "tensors is NULL");
@@ -162,7 +162,6 @@ int take(int n, const fmlp_muon_tensor* tensors, double lr, double weight_decay,
     t.m_io = io_type(v.m_dtype);
     t.out_io = io_type(v.w_dtype);
     t.lr = (float)(lr * (double)v.scale);
-    t.keep = (float)(1.0 - lr * weight_decay);
     out->push_back(t);
   }
   return FMLP_OK;
@@ -173,7 +172,7 @@ int take(int n, const fmlp_muon_tensor* tensors, double lr, double weight_decay,
 FMLP_EXPORT size_t fmlp_muon_workspace_bytes(int n, const fmlp_muon_tensor* tensors, int steps) {
   int cus = 0;
   std::vector<fmlp::MuonTensor> t;
-  if (check_steps(steps) || take(n, tensors, 0, 0, false, &t, nullptr) || fmlp::abi_num_cus(&cus)) return 0;
+  if (check_steps(steps) || take(n, tensors, 0, false, &t, nullptr) || fmlp::abi_num_cus(&cus)) return 0;
   fmlp::MuonCall c{};
   c.steps = steps;
   c.stage = kStage16;
@@ -193,7 +192,7 @@ FMLP_EXPORT int fmlp_muon_step(int n, const fmlp_muon_tensor* tensors, double lr
     return abi_fail(FMLP_ERR_INVALID_ARG, "lr or weight_decay is negative or NaN, or momentum outside [0, 1]");
   std::vector<fmlp::MuonTensor> t;
   std::vector<fmlp::MemRange> ranges;
-  if ((st = take(n, tensors, lr, weight_decay, true, &t, &ranges))) return st;
+  if ((st = take(n, tensors, lr, true, &t, &ranges))) return st;
   int one, two;
   if (fmlp::mem_overlap(ranges, &one, &two))
     return abi_fail(FMLP_ERR_INVALID_ARG, "the weights or momenta of stack %d or %d overlap another tensor of the call", one, two);
@@ -201,6 +200,7 @@ FMLP_EXPORT int fmlp_muon_step(int n, const fmlp_muon_tensor* tensors, double lr
   c.mu = (float)momentum;
   c.nu = (float)(1.0 - momentum);
   c.nesterov = nesterov != 0;
+  c.keep = (float)(1.0 - lr * weight_decay);
   c.update = 1;
   c.stage = kStage16;
   return run((int)t.size(), t.data(), c, workspace, workspace_bytes, stream, "muon step");

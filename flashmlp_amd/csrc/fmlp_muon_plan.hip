@@ -1,0 +1,223 @@
+// Host side of the orthogonalised updates: which kernels take a call's stacks of matrices, the workspace they share and the scales of
+// their terms.
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "fmlp_muon.h"
+
+namespace fmlp {
+namespace {
+
+int padded(const MuonTensor& t) {
+  const int n = std::min(t.R, t.C);
+  return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : 256;
+}
+MuonKind kind_of(const MuonTensor& t) {
+  const bool raw = t.m == nullptr && t.x_io != IO_F32;
+  const auto whole = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  const bool vec = t.C % 8 == 0 && (long long)t.R * t.C < 1LL << 29 && whole(t.x) && whole(t.m) && whole(t.out);
+  return MuonKind{raw ? 1 : 3, !raw || t.x_io == IO_BF16, vec};
+}
+
+// The matrices of one padded size: their Gram matrices and what comes of them go through the workspace together.
+struct Group {
+  int NP;
+  long long matrices, tiles;  // tiles: of the longest one
+  bool whole;  // a workgroup a matrix from end to end: no workspace
+  int gram_parts, apply_parts;
+  size_t g_off, p_off, info_off, iter_off, end;
+};
+Group group_of(int NP, int n, const MuonTensor* t, int cus) {
+  Group r{};
+  r.NP = NP;
+  const int KT = NP == 256 ? 32 : 8192 / NP;
+  for (int i = 0; i < n; ++i)
+    if (t[i].H > 0 && t[i].R > 0 && t[i].C > 0 && padded(t[i]) == NP) {
+      r.matrices += t[i].H;
+      r.tiles = std::max(r.tiles, ((long long)std::max(t[i].R, t[i].C) + KT - 1) / KT);
+    }
+  if (r.matrices == 0) return r;
+  // two workgroups for each CU at least: below, CUs idle that parts of matrices would fill
+  r.whole = NP <= 128 && r.matrices >= 2 * cus;
+  if (r.whole) return r;
+  // three workgroups a CU at least, as far as there are tiles; of Gram matrices no more than pay: a tile takes about
+  // 3 us (6 at NP = 256, whose workgroups are alone on their CUs), a part's sums are written and read at about 4 TB/s
+  const long long want = (3LL * cus + r.matrices - 1) / r.matrices;
+  const double part_us = (double)r.matrices * NP * NP * 8 / 4e6;
+  const long long pays = std::max(1LL, std::llround(std::sqrt((double)r.tiles * (NP == 256 ? 6 : 3) / part_us)));
+  r.gram_parts = (int)std::max(1LL, std::min(std::min(want, pays), r.tiles));
+  r.apply_parts = (int)std::max(1LL, std::min(want, r.tiles));
+  const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+  r.p_off = up((size_t)r.matrices * r.gram_parts * NP * NP * 4);
+  r.info_off = r.p_off + up((size_t)r.matrices * NP * NP * 4);
+  r.iter_off = r.info_off + up((size_t)r.matrices * sizeof(MuonInfo));
+  r.end = r.iter_off + up(muon_iter_ws_bytes(NP, r.matrices));
+  return r;
+}
+constexpr int kSizes[4] = {32, 64, 128, 256};
+
+// Powers of two that bring each stage's values to at most 2^14 as fp16: bounds of the eigenvalues of G, Q and P from
+// the steps' polynomials over the range that G's have, which is [0, 1] at first. Returns the range after the steps.
+double set_steps(MuonSteps* s, const MuonCall& c, int first, int steps, bool normalise, double range) {
+  s->steps = steps;
+  s->normalise = normalise;
+  s->eps = c.eps;
+  double p = 1;
+  const auto scale = [](double bound) {
+    int e = 0;
+    if (!(bound < 1e30)) bound = 1e30;
+    (void)std::frexp(std::max(bound, 1e-30), &e);
+    return std::ldexp(1.f, 14 - e);
+  };
+  for (int k = 0; k < steps; ++k) {
+    const float* v = c.abc[first + k];
+    s->a[k] = v[0];
+    s->b[k] = v[1];
+    s->c[k] = v[2];
+    double q = 0, next = 0;
+    const int N = 512;
+    for (int i = 0; i <= N; ++i) {
+      const double l = range * 1.02 * i / N, y = v[0] + l * (v[1] + l * v[2]);
+      q = std::max(q, std::fabs(y));
+      next = std::max(next, l * y * y);
+    }
+    q *= 1.02;
+    p *= q;
+    s->g_scale[k] = scale(range * 1.02);
+    s->q_scale[k] = scale(q);
+    s->p_scale[k] = scale(p);
+    range = next * 1.02;
+  }
+  return range;
+}
+
+bool empty(const MuonTensor& t) { return t.H == 0 || t.R == 0 || t.C == 0; }
+
+// A stage's tensors of one padded size: what it reads and writes of each, and the number of the first matrix.
+struct Item {
+  MuonTensor t;
+  MuonKind kind;
+  long long matrix0;
+};
+
+// f(kind, table, workgroups) for tables of items of one kind, `parts` workgroups a matrix
+template <typename F>
+hipError_t for_tables(const std::vector<Item>& items, int parts, bool any_type, F f) {
+  for (int code = 0; code < 8; ++code) {  // (kinds in a fixed order)
+    const MuonKind k{code & 1 ? 3 : 1, (code & 2) != 0, (code & 4) != 0};
+    MuonTable tab{};
+    long long blocks = 0;
+    for (size_t i = 0; i <= items.size(); ++i) {
+      const bool end = i == items.size();
+      const Item* it = end ? nullptr : &items[i];
+      if (!end && !(it->kind.terms == k.terms && (any_type || it->kind.bf == k.bf) && it->kind.vec == k.vec)) continue;
+      if (!end && any_type && !k.bf) continue;  // (both 16-bit types at once)
+      const long long b = end ? 0 : it->t.H * parts;
+      if (b > 0x7fffffffLL) return hipErrorInvalidValue;
+      if (tab.n > 0 && (end || tab.n == kMuonTable || blocks + b > 0x7fffffffLL)) {
+        const hipError_t e = f(k, tab, (unsigned)blocks);
+        if (e != hipSuccess) return e;
+        tab.n = 0;
+        blocks = 0;
+      }
+      if (end) break;
+      const MuonTensor& t = it->t;
+      tab.t[tab.n++] = MuonRef{t.x, t.m, t.out, t.R, t.C, (unsigned)blocks, (unsigned)it->matrix0, t.lr,
+                               (unsigned char)t.x_io, (unsigned char)t.m_io, (unsigned char)t.out_io, 0};
+      blocks += b;
+    }
+  }
+  return hipSuccess;
+}
+
+size_t between_bytes(const MuonTensor& t, const MuonCall& c) {
+  // matrices between stages are in fp32: in the result where that is what it is
+  if (c.steps <= c.stage || (!c.update && t.out_io == IO_F32)) return 0;
+  return ((size_t)t.H * t.R * t.C * 4 + 255) / 256 * 256;
+}
+
+}  // namespace
+
+MuonPlan muon_plan(int n, const MuonTensor* t, const MuonCall& c, int num_cus) {
+  MuonPlan p{};
+  for (int NP : kSizes) {
+    const Group g = group_of(NP, n, t, num_cus);
+    if (g.matrices) p.ws_bytes = std::max(p.ws_bytes, g.end);
+  }
+  for (int i = 0; i < n; ++i) p.ws_bytes += between_bytes(t[i], c);
+  return p;
+}
+
+hipError_t launch_muon(int n, const MuonTensor* t, const MuonCall& c, int num_cus, void* ws, hipStream_t st) {
+  size_t shared = 0;
+  for (int NP : kSizes) {
+    const Group g = group_of(NP, n, t, num_cus);
+    if (g.matrices) shared = std::max(shared, g.end);
+  }
+  for (int NP : kSizes) {
+    const Group gr = group_of(NP, n, t, num_cus);
+    if (gr.matrices == 0) continue;
+    float* G = (float*)ws;
+    unsigned short* P = (unsigned short*)((char*)ws + gr.p_off);
+    MuonInfo* info = (MuonInfo*)((char*)ws + gr.info_off);
+    double range = 1;
+    for (int first = 0; first < c.steps; first += c.stage) {
+      const int steps = std::min(c.stage, c.steps - first);
+      const bool start = first == 0, last = first + steps == c.steps;
+      const int update = c.update && last;
+      MuonSteps s{};
+      range = set_steps(&s, c, first, steps, start, range);
+      std::vector<Item> items;
+      long long matrix = 0;
+      char* between = (char*)ws + shared;
+      for (int i = 0; i < n; ++i) {
+        const size_t bytes = between_bytes(t[i], c);
+        if (!empty(t[i]) && padded(t[i]) == NP) {
+          MuonTensor v = t[i];
+          void* y = bytes ? (void*)between : t[i].out;
+          if (!start) {
+            v.x = y;
+            v.m = nullptr;
+            v.x_io = IO_F32;
+          }
+          if (!last) {
+            v.out = y;
+            v.out_io = IO_F32;
+          }
+          items.push_back(Item{v, kind_of(v), matrix});
+          matrix += v.H;
+        }
+        between += bytes;
+      }
+      hipError_t e;
+      if (gr.whole) {
+        e = for_tables(items, 1, false, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
+          return NP == 32   ? muon_whole<32>(k, tab, blocks, s, c, update, st)
+                 : NP == 64 ? muon_whole<64>(k, tab, blocks, s, c, update, st)
+                            : muon_whole<128>(k, tab, blocks, s, c, update, st);
+        });
+        if (e != hipSuccess) return e;
+        continue;
+      }
+      e = for_tables(items, gr.gram_parts, false, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
+        return NP == 32    ? muon_gram<32>(k, tab, blocks, G, gr.gram_parts, c, st)
+               : NP == 64  ? muon_gram<64>(k, tab, blocks, G, gr.gram_parts, c, st)
+               : NP == 128 ? muon_gram<128>(k, tab, blocks, G, gr.gram_parts, c, st)
+                           : muon_gram<256>(k, tab, blocks, G, gr.gram_parts, c, st);
+      });
+      if (e == hipSuccess) e = launch_muon_iter(NP, gr.matrices, G, gr.gram_parts, P, info, s, (char*)ws + gr.iter_off, st);
+      if (e == hipSuccess)
+        e = for_tables(items, gr.apply_parts, true, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
+          return NP == 32    ? muon_apply<32>(k, tab, blocks, P, info, gr.apply_parts, c, update, st)
+                 : NP == 64  ? muon_apply<64>(k, tab, blocks, P, info, gr.apply_parts, c, update, st)
+                 : NP == 128 ? muon_apply<128>(k, tab, blocks, P, info, gr.apply_parts, c, update, st)
+                             : muon_apply<256>(k, tab, blocks, P, info, gr.apply_parts, c, update, st);
+        });
+      if (e != hipSuccess) return e;
+    }
+  }
+  return hipSuccess;
+}
+
+}  // namespace fmlp

@@ -220,6 +220,31 @@ def test_graph():
         assert all(torch.equal(a, b) for a, b in zip(w + m, we + me)), i
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tall", [False, True])
+@pytest.mark.parametrize("n,e", [(7, 300), (32, 20), (50, 129), (64, 128), (100, 65), (128, 200)])
+def test_many_matrices(n, e, tall, dtype):
+    """as many as take a workgroup each from end to end"""
+    x = torch.randn(700, n, e, generator=gen(n * e)).mul(1e-2)
+    x = (x.mT.contiguous() if tall else x).to(dtype)
+    check(x, orthogonalize(x.cuda()))
+
+
+@pytest.mark.parametrize("types", [(FL, BF, FL), (BF, HF, BF)])
+def test_muon_step_of_many_matrices(types):
+    """the same with weights and momenta, in stacks of both orientations and several sizes"""
+    shapes = [(300, 40, 70), (400, 70, 40), (350, 64, 33), (350, 128, 140), (513, 20, 30), (1, 20, 31), (3, 140, 128)]
+    w, g, m = stacks(shapes, types, 13)
+    dw, dg, dm = ([t.cuda() for t in v] for v in (w, g, m))
+    muon_step(dw, dg, dm, 0.02, weight_decay=0.1)
+    for i in range(len(w)):
+        want = om.step64(w[i], g[i], m[i], 0.02, weight_decay=0.1)
+        for t, got in (("w", dw[i]), ("m", dm[i])):
+            ref, tol = want[t]
+            tiny = 2.0 ** -25 if got.dtype == HF else 2.0 ** -130
+            assert ((got.double().cpu() - ref).abs() <= 1.01 * tol + tiny).all(), (i, t)
+
+
 def test_a_matrix_does_not_depend_on_what_is_beside_it():
     x = torch.randn(9, 64, 500, generator=gen(12)).to(BF).cuda()
     assert (orthogonalize(x)[4].float() - orthogonalize(x[4]).float()).abs().max() <= 2.0 ** -8 * 0.3
