@@ -20,14 +20,15 @@ struct RouteArgs {
 hipError_t launch_route_fwd(const RouteArgs& a, hipStream_t st);
 hipError_t launch_route_bwd(const RouteArgs& a, hipStream_t st);
 
-// The sort of M assignments by expert: chunks of `chunk` assignments, a workgroup each; with more than one, their
-// histograms ([chunks][N]) take ws_bytes.
+// The sort of M assignments by expert: chunks of `threads` times `items` assignments, a workgroup each; with more than one, their
+// histograms ([chunks][N]) take ws_bytes. scan: these are summed up in a launch of its own.
 struct ExpertPlan {
-  long long chunk, chunks;
-  int threads;
+  long long chunks;
+  int threads, items;
+  bool scan;
   size_t ws_bytes;
 };
-ExpertPlan expert_plan(int64_t M, int64_t N, int num_cus);
+ExpertPlan expert_plan(int64_t M, int64_t N);
 hipError_t launch_expert_plan(const void* experts, bool wide, long long M, int N, long long capacity, int32_t* slots,
                               int32_t* counts, const ExpertPlan& p, void* ws, hipStream_t st);
 

@@ -22,58 +22,108 @@ namespace {
 // ---------------------------------------------------------------------------------------------
 // plan
 // ---------------------------------------------------------------------------------------------
-constexpr int kItems = 16;  // assignments of a lane
+constexpr int kItems = 16;  // assignments of a lane, at most
 
+// expert of assignment i, -1 for none; past the last one too, whose load is then the last one's (a branch around it would have
+// every load waited for before the next)
 template <bool WIDE>
-__device__ __forceinline__ int expert_at(const void* experts, long long i, int N) {
-  if constexpr (WIDE) {
-    const long long e = ((const long long*)experts)[i];
-    return e >= 0 && e < N ? (int)e : -1;
-  } else {
-    const int e = ((const int*)experts)[i];
-    return e >= 0 && e < N ? e : -1;
-  }
+__device__ __forceinline__ int expert_at(const void* experts, long long i, long long M, int N) {
+  const long long at = i < M ? i : M - 1;
+  long long e;
+  if constexpr (WIDE) e = ((const long long*)experts)[at];
+  else e = ((const int*)experts)[at];
+  return i < M && e >= 0 && e < N ? (int)e : -1;
 }
 
 template <bool WIDE>
 __global__ void __launch_bounds__(256) plan_count_kernel(const void* experts, long long M, int N, int* hist) {
   extern __shared__ int plan_lds[];
+  const long long i0 = (long long)blockIdx.x * (256 * kItems) + threadIdx.x;
+  int ex[kItems];
+#pragma unroll
+  for (int u = 0; u < kItems; ++u) ex[u] = expert_at<WIDE>(experts, i0 + u * 256, M, N);
   for (int e = threadIdx.x; e < N; e += 256) plan_lds[e] = 0;
   __syncthreads();
-  const long long i0 = (long long)blockIdx.x * (256 * kItems);
 #pragma unroll
-  for (int u = 0; u < kItems; ++u) {
-    const long long i = i0 + u * 256 + threadIdx.x;
-    const int e = i < M ? expert_at<WIDE>(experts, i, N) : -1;
-    if (e >= 0) atomicAdd(&plan_lds[e], 1);
-  }
+  for (int u = 0; u < kItems; ++u)
+    if (ex[u] >= 0) atomicAdd(&plan_lds[ex[u]], 1);
   __syncthreads();
   for (int e = threadIdx.x; e < N; e += 256) hist[(long long)blockIdx.x * N + e] = plan_lds[e];
 }
 
-// THREADS * kItems assignments of workgroup blockIdx.x; hist: every chunk's counts, null for one chunk
+__global__ void __launch_bounds__(256) plan_none_kernel(int* counts, int N) {
+  for (int e = threadIdx.x; e < N; e += 256) counts[e] = 0;
+}
+
+// hist[c][e] = the sum of hist[c'][e] over c' < c, a wave an expert
+__global__ void __launch_bounds__(256) plan_scan_kernel(int* hist, long long chunks, int N) {
+  const int e = (int)(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = (int)threadIdx.x & 63;
+  if (e >= N) return;
+  int base = 0;
+  for (long long c0 = 0; c0 < chunks; c0 += 256) {
+    int v[4], sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // four chunks a lane
+      const long long c = c0 + lane * 4 + j;
+      v[j] = c < chunks ? hist[c * N + e] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum += v[j];
+    int upto = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(upto, d, 64);
+      if (lane >= d) upto += o;
+    }
+    int at = base + upto - sum;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const long long c = c0 + lane * 4 + j;
+      if (c < chunks) hist[c * N + e] = at;
+      at += v[j];
+    }
+    base += __shfl(upto, 63, 64);
+  }
+}
+
+// THREADS * items assignments of workgroup blockIdx.x. hist: null for one workgroup; else every chunk's counts, or where
+// `scanned` what the chunks before it have.
 template <bool WIDE, int THREADS>
 __global__ void __launch_bounds__(THREADS) plan_kernel(const void* experts, long long M, int N, int bits, long long capacity,
-                                                       int* slots, int* counts, const int* hist) {
-  extern __shared__ int plan_lds[];  // [waves][N]: the wave's counts, then its next position of each expert
+                                                       int* slots, int* counts, const int* hist, int scanned, int items) {
+  extern __shared__ int plan_lds[];  // [waves][N]: the wave's counts, then its next position of each expert; [N] what is before
   constexpr int W = THREADS / 64;
   const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63;
-  for (int e = threadIdx.x; e < W * N; e += THREADS) plan_lds[e] = 0;
-  __syncthreads();
   int* mine = plan_lds + wave * N;
-  const long long i0 = ((long long)blockIdx.x * W + wave) * (64 * kItems) + lane;
+  int* before = plan_lds + W * N;
+  const long long i0 = ((long long)blockIdx.x * W + wave) * (64 * items) + lane;
   int ex[kItems];
 #pragma unroll
-  for (int u = 0; u < kItems; ++u) {
-    const long long i = i0 + u * 64;
-    ex[u] = i < M ? expert_at<WIDE>(experts, i, N) : -1;
+  for (int u = 0; u < kItems; ++u) ex[u] = u < items ? expert_at<WIDE>(experts, i0 + u * 64, M, N) : -1;
+  for (int e = threadIdx.x; e < (W + 1) * N; e += THREADS) plan_lds[e] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kItems; ++u)
     if (ex[u] >= 0) atomicAdd(&mine[ex[u]], 1);
+  if (hist != nullptr) {
+    if (scanned) {
+      for (int e = threadIdx.x; e < N; e += THREADS) before[e] = hist[(long long)blockIdx.x * N + e];
+    } else {
+      // the chunks before this one, dealt to as many groups of threads as there are for the experts
+      int lanes = 1;
+      while (lanes < N) lanes <<= 1;
+      const int parts = THREADS / min(lanes, THREADS), e = (int)threadIdx.x & (lanes - 1), part = (int)threadIdx.x / min(lanes, THREADS);
+      for (int e1 = e; e1 < N; e1 += THREADS) {
+        int sum = 0;
+#pragma unroll 8
+        for (int c = part; c < (int)blockIdx.x; c += parts) sum += hist[(long long)c * N + e1];
+        if (sum) atomicAdd(&before[e1], sum);
+      }
+    }
   }
   __syncthreads();
   for (int e = threadIdx.x; e < N; e += THREADS) {
-    int at = 0;
-    if (hist != nullptr)
-      for (unsigned c = 0; c < blockIdx.x; ++c) at += hist[(long long)c * N + e];
+    int at = before[e];
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       const int n = plan_lds[w * N + e];
@@ -85,6 +135,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const void* experts, long
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < kItems; ++u) {
+    if (u >= items) break;
     const int e = ex[u];
     unsigned long long same = __ballot(e >= 0);
     for (int b = 0; b < bits; ++b) {
@@ -92,18 +143,18 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const void* experts, long
       same &= (e >> b) & 1 ? v : ~v;
     }
     const long long i = i0 + u * 64;
-    const int before = __popcll(same & ((1ull << lane) - 1));
+    const int rank = __popcll(same & ((1ull << lane) - 1));
     int base = 0;
     if (e >= 0) {
       base = mine[e];
       // (the wave's lanes have all read before the last one of each expert writes: one wave's LDS operations keep
       // their order)
       asm volatile("" ::: "memory");
-      if ((same >> lane) == 1) mine[e] = base + before + 1;
+      if ((same >> lane) == 1) mine[e] = base + rank + 1;
     }
     asm volatile("" ::: "memory");
     if (i < M) {
-      const long long p = (long long)base + before;
+      const long long p = (long long)base + rank;
       slots[i] = e >= 0 && p < capacity ? (int)(e * capacity + p) : -1;
     }
   }
@@ -253,14 +304,19 @@ void by_choices(int k, F f) {
 
 }  // namespace
 
-ExpertPlan expert_plan(int64_t M, int64_t N, int num_cus) {
-  (void)num_cus;
+ExpertPlan expert_plan(int64_t M, int64_t N) {
   ExpertPlan p{};
   // one workgroup of up to 16 waves does all where its lanes' items suffice: no second launch
   p.threads = M <= 256 * kItems || M > 1024 * kItems ? 256 : 1024;
-  p.chunk = (long long)p.threads * kItems;
-  p.chunks = M > 0 ? (M + p.chunk - 1) / p.chunk : 1;
+  const long long most = (long long)p.threads * kItems;
+  p.chunks = M > most ? (M + most - 1) / most : 1;
+  p.items = p.chunks > 1 ? kItems : (int)std::max<long long>(1, (M + p.threads - 1) / p.threads);
   p.ws_bytes = p.chunks > 1 ? (size_t)(p.chunks * N) * sizeof(int) : 0;
+  // The workgroups add up the chunks before them themselves where that is at most 32 rounds of their 256 threads (M = 2^20, N = 32:
+  // PLANA us, a scan in a launch of its own PLANB); a scan takes over from there (M = 2^20, N = 256: PLANC, PLAND).
+  long long lanes = 1;
+  while (lanes < N) lanes <<= 1;
+  p.scan = p.chunks > 1 && p.chunks * lanes > 32 * 256;
   return p;
 }
 
@@ -276,14 +332,25 @@ hipError_t launch_expert_plan(const void* experts, bool wide, long long M, int N
     if (hist != nullptr) {
       hipLaunchKernelGGL((plan_count_kernel<V>), grid, dim3(256), (size_t)N * 4, st, experts, M, N, hist);
       if ((e = hipGetLastError()) != hipSuccess) return;
+      if (p.scan) {
+        hipLaunchKernelGGL(plan_scan_kernel, dim3((unsigned)((N + 3) / 4)), dim3(256), 0, st, hist, p.chunks, N);
+        if ((e = hipGetLastError()) != hipSuccess) return;
+      }
     }
-    const size_t lds = (size_t)p.threads / 64 * N * 4;
-    if (p.threads == 1024)
-      hipLaunchKernelGGL((plan_kernel<V, 1024>), grid, dim3(1024), lds, st, experts, M, N, bits, capacity, slots, counts, hist);
-    else
-      hipLaunchKernelGGL((plan_kernel<V, 256>), grid, dim3(256), lds, st, experts, M, N, bits, capacity, slots, counts, hist);
-    e = hipGetLastError();
+    const size_t lds = ((size_t)p.threads / 64 + 1) * N * 4;
+    const auto go = [&](auto k) {
+      static std::atomic<unsigned long long> done{0};
+      if (lds > 65536 && (e = set_lds_once((const void*)k, 17 * (int)kMaxExperts * 4, done)) != hipSuccess) return;
+      hipLaunchKernelGGL(k, grid, dim3(p.threads), lds, st, experts, M, N, bits, capacity, slots, counts, hist, (int)p.scan, p.items);
+      e = hipGetLastError();
+    };
+    if (p.threads == 1024) go(plan_kernel<V, 1024>);
+    else go(plan_kernel<V, 256>);
   };
+  if (M == 0) {  // (nothing to read; the counts are zeros)
+    hipLaunchKernelGGL(plan_none_kernel, dim3(1), dim3(256), 0, st, counts, N);
+    return hipGetLastError();
+  }
   if (wide) run(std::true_type{});
   else run(std::false_type{});
   return e;

@@ -105,9 +105,7 @@ FMLP_EXPORT int fmlp_route_bwd(const void* logits, const float* weights, const i
 }
 
 FMLP_EXPORT size_t fmlp_expert_plan_workspace_bytes(int64_t T, int64_t k, int64_t N) {
-  int cus = 0;
-  if (check_counts(T, N, k) || fmlp::abi_num_cus(&cus)) return 0;
-  return fmlp::expert_plan(T * k, N, cus).ws_bytes;
+  return check_counts(T, N, k) ? 0 : fmlp::expert_plan(T * k, N).ws_bytes;
 }
 
 FMLP_EXPORT int fmlp_expert_plan(const void* experts, int index_bytes, int32_t* slots, int32_t* counts, int64_t T, int64_t k,
@@ -119,9 +117,7 @@ FMLP_EXPORT int fmlp_expert_plan(const void* experts, int index_bytes, int32_t* 
   if ((st = check_ptr(experts, "experts", T > 0, (size_t)index_bytes)) || (st = check_ptr(slots, "slots", T > 0, 4)) ||
       (st = check_ptr(counts, "counts", true, 4)) || (st = check_ptr(workspace, "workspace", false, 4)))
     return st;
-  int cus = 0;
-  if ((st = fmlp::abi_num_cus(&cus))) return st;
-  const fmlp::ExpertPlan p = fmlp::expert_plan(T * k, N, cus);
+  const fmlp::ExpertPlan p = fmlp::expert_plan(T * k, N);
   if (p.ws_bytes > 0 && (workspace == nullptr || workspace_bytes < p.ws_bytes))
     return abi_fail(FMLP_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, p.ws_bytes);
   return finish(fmlp::launch_expert_plan(experts, index_bytes == 8, T * k, (int)N, capacity, slots, counts, p, workspace,

@@ -1,5 +1,6 @@
 // _fmlp_fast: the per-call fast path of flashmlp_fwd / flashmlp_bwd (flashmlp_amd/flashmlp.py), and of the gated
-// block's operators (gated.py, block.py, clip.py; below).
+// block's operators, the experts' and the orthogonalised updates (gated.py, block.py, clip.py, experts.py, muon.py;
+// below).
 //
 // A CPython module (METH_FASTCALL) over the C ABI of libflashmlp.so for the common case:
 // inputs on one GPU, a shape with kernels of its own (views that they do not read in place are copied
@@ -817,6 +818,347 @@ PyObject* fast_clip(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- experts ----
+// a strided tensor on a GPU with memory of its own
+bool on_gpu(const at::Tensor& t) {
+  return t.is_cuda() && t.layout() == at::kStrided && !t.is_neg() && (t.numel() == 0 || t.data_ptr() != nullptr);
+}
+// a dense tensor of `type` on the device of `like`
+bool dense_beside(const at::Tensor& t, const at::Tensor& like, at::ScalarType type) {
+  return on_gpu(t) && t.device() == like.device() && t.scalar_type() == type && t.is_contiguous();
+}
+at::Tensor dense(const at::Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
+bool wants_node(std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)  // (a tensor with a tangent goes to the node too, which refuses forward mode)
+    if (t->defined() && ((at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
+  return false;
+}
+hipStream_t stream_on(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+bool route_ok(const at::Tensor& l, int64_t k) {
+  return on_gpu(l) && io_code(l) >= 0 && l.dim() == 2 && k >= 1 && k <= l.size(1) && cols1(l);
+}
+std::pair<at::Tensor, at::Tensor> route_run(const at::Tensor& l, int64_t k, bool normalize) {
+  c10::DeviceGuard guard(l.device());
+  const int64_t T = l.size(0);
+  at::Tensor w = at::empty({T, k}, l.options().dtype(at::kFloat)), e = at::empty({T, k}, l.options().dtype(at::kInt));
+  check_status(fmlp_route_fwd(l.data_ptr(), w.data_ptr<float>(), e.data_ptr<int>(), T, l.size(1), l.stride(0), k, normalize,
+                              io_code(l), stream_on(l)),
+               "route forward");
+  return {w, e};
+}
+
+struct RouteFn : torch::autograd::Function<RouteFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& l, int64_t k, bool normalize) {
+    auto [w, e] = route_run(l, k, normalize);
+    ctx->save_for_backward({normalize ? at::Tensor() : l, w, e});
+    ctx->saved_data["normalize"] = normalize;
+    ctx->saved_data["N"] = l.size(1);
+    ctx->saved_data["dtype"] = (int64_t)l.scalar_type();
+    ctx->mark_non_differentiable({e});
+    return {w, e};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    return once(joined({grads[0]}, s), [&] { return first(ctx, s, grads); });
+  }
+  static variable_list first(AutogradContext* ctx, const variable_list& s, const variable_list& grads) {
+    variable_list r(3);
+    if (!grads[0].defined()) return r;
+    const bool normalize = ctx->saved_data["normalize"].toBool();
+    const int64_t N = ctx->saved_data["N"].toInt();
+    const auto dtype = (at::ScalarType)ctx->saved_data["dtype"].toInt();
+    const at::Tensor w = dense(s[1]), e = dense(s[2]), dw = dense(grads[0]), l = s[0].defined() ? cols(s[0]) : s[0];
+    TORCH_CHECK(w.dim() == 2 && dense_beside(w, w, at::kFloat) && dense_beside(e, w, at::kInt) && dense_beside(dw, w, at::kFloat) &&
+                    e.sizes() == w.sizes() && dw.sizes() == w.sizes() &&
+                    (normalize || (route_ok(l, w.size(1)) && l.device() == w.device() && l.scalar_type() == dtype &&
+                                   l.size(0) == w.size(0) && l.size(1) == N)),
+                "a saved tensor of the routing came back with another size, type or device");
+    c10::DeviceGuard guard(w.device());
+    r[0] = at::empty({w.size(0), N}, w.options().dtype(dtype));
+    check_status(fmlp_route_bwd(normalize ? nullptr : l.data_ptr(), w.data_ptr<float>(), e.data_ptr<int>(), dw.data_ptr<float>(),
+                                r[0].data_ptr(), w.size(0), N, normalize ? 0 : l.stride(0), w.size(1), normalize, code_of(dtype),
+                                stream_on(w)),
+                 "route backward");
+    return r;
+  }
+};
+
+// whole numbers as Python has them
+bool whole(PyObject* o, int64_t* v) {
+  if (!PyLong_Check(o) || PyBool_Check(o)) return false;
+  *v = PyLong_AsLongLong(o);
+  if (*v == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return true;
+}
+
+// expert_route(logits, k, normalize) -> (weights, experts), or None
+PyObject* fast_route(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* l;
+  int64_t k;
+  if (nargs != 3 || !unpack(args, 1, &l) || !whole(args[1], &k) || !route_ok(*l, k)) Py_RETURN_NONE;
+  const bool normalize = PyObject_IsTrue(args[2]) == 1;
+  at::Tensor w, e;
+  if (wants_node({l})) {
+    variable_list out = RouteFn::apply(*l, k, normalize);
+    w = out[0];
+    e = out[1];
+  } else {
+    std::tie(w, e) = route_run(*l, k, normalize);
+  }
+  return Py_BuildValue("(NN)", THPVariable_Wrap(w), THPVariable_Wrap(e));
+  END_HANDLE_TH_ERRORS
+}
+
+// expert_plan(experts, num_experts, capacity) -> (slots, counts), or None
+PyObject* fast_plan(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* ex;
+  int64_t N, capacity;
+  if (nargs != 3 || !unpack(args, 1, &ex) || !whole(args[1], &N) || !whole(args[2], &capacity) || N < 1 || capacity < 0) Py_RETURN_NONE;
+  const at::Tensor& e = *ex;
+  const bool wide = e.scalar_type() == at::kLong;
+  if (!on_gpu(e) || (!wide && e.scalar_type() != at::kInt) || e.dim() != 2 || e.size(1) < 1 || !e.is_contiguous()) Py_RETURN_NONE;
+  c10::DeviceGuard guard(e.device());
+  const int64_t T = e.size(0), k = e.size(1);
+  const auto opt = e.options().dtype(at::kInt);
+  at::Tensor slots = at::empty({T, k}, opt), counts = at::empty({N}, opt), ws;
+  const size_t n = fmlp_expert_plan_workspace_bytes(T, k, N);
+  if (n) ws = bytes_on(e, n);
+  check_status(fmlp_expert_plan(e.data_ptr(), wide ? 8 : 4, slots.data_ptr<int>(), counts.data_ptr<int>(), T, k, N, capacity,
+                                n ? ws.data_ptr() : nullptr, n, stream_on(e)),
+               "expert plan");
+  return Py_BuildValue("(NN)", THPVariable_Wrap(slots), THPVariable_Wrap(counts));
+  END_HANDLE_TH_ERRORS
+}
+
+// slots (T, k), counts (N) of a plan for T tokens, or for any number where T < 0
+bool plan_ok(const at::Tensor& slots, const at::Tensor& counts, const at::Tensor& like, int64_t T, int64_t N, int64_t capacity) {
+  return N >= 1 && capacity >= 0 && dense_beside(slots, like, at::kInt) && slots.dim() == 2 && slots.size(1) >= 1 &&
+         (T < 0 || slots.size(0) == T) && dense_beside(counts, like, at::kInt) && counts.dim() == 1 && counts.size(0) == N;
+}
+const float* weights_ptr(const at::Tensor& w) { return w.defined() ? w.data_ptr<float>() : nullptr; }
+
+// (rows, dweights); those that are not wanted undefined
+std::pair<at::Tensor, at::Tensor> scatter_run(const at::Tensor& x, const at::Tensor& w, const at::Tensor& slots, const at::Tensor& counts,
+                                              int64_t N, int64_t capacity, const at::Tensor& rows_in, bool want_rows, bool want_dw) {
+  c10::DeviceGuard guard(x.device());
+  at::Tensor rows, dw;
+  if (want_rows) rows = at::empty({N, capacity, x.size(1)}, x.options());
+  if (want_dw) dw = at::empty(slots.sizes(), x.options().dtype(at::kFloat));
+  if (!want_rows && !want_dw) return {rows, dw};
+  check_status(fmlp_expert_scatter(x.data_ptr(), x.stride(0), weights_ptr(w), slots.data_ptr<int>(), counts.data_ptr<int>(),
+                                   want_dw ? rows_in.data_ptr() : nullptr, mptr(rows), want_dw ? dw.data_ptr<float>() : nullptr,
+                                   slots.size(0), slots.size(1), N, capacity, x.size(1), io_code(x), stream_on(x)),
+               "expert scatter");
+  return {rows, dw};
+}
+at::Tensor gather_run(const at::Tensor& rows, const at::Tensor& w, const at::Tensor& slots) {
+  c10::DeviceGuard guard(rows.device());
+  at::Tensor o = at::empty({slots.size(0), rows.size(2)}, rows.options());
+  check_status(fmlp_expert_gather(rows.data_ptr(), weights_ptr(w), slots.data_ptr<int>(), o.data_ptr(), slots.size(0), slots.size(1),
+                                  rows.size(0), rows.size(1), rows.size(2), io_code(rows), stream_on(rows)),
+               "expert gather");
+  return o;
+}
+
+struct DispatchFn : torch::autograd::Function<DispatchFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& slots, const at::Tensor& counts, int64_t N,
+                            int64_t capacity) {
+    ctx->save_for_backward({slots});
+    ctx->saved_data["T"] = x.size(0);
+    return scatter_run(x, at::Tensor(), slots, counts, N, capacity, at::Tensor(), true, false).first;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    return once(joined(grads, s), [&] { return first(ctx, s, grads); });
+  }
+  static variable_list first(AutogradContext* ctx, const variable_list& s, const variable_list& grads) {
+    variable_list r(5);
+    if (!grads[0].defined()) return r;
+    const at::Tensor drows = dense(grads[0]), slots = dense(s[0]);
+    TORCH_CHECK(dense_beside(slots, drows, at::kInt) && slots.dim() == 2 && slots.size(0) == ctx->saved_data["T"].toInt(),
+                "a saved tensor of the dispatch came back with another size, type or device");
+    r[0] = gather_run(drows, at::Tensor(), slots);
+    return r;
+  }
+};
+
+bool rows_ok(const at::Tensor& rows) {
+  return on_gpu(rows) && io_code(rows) >= 0 && rows.dim() == 3 && rows.size(2) >= 1 && rows.is_contiguous();
+}
+
+struct CombineFn : torch::autograd::Function<CombineFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& rows, const std::optional<at::Tensor>& w_, const at::Tensor& slots,
+                            const at::Tensor& counts) {
+    const at::Tensor w = w_.value_or(at::Tensor());
+    ctx->save_for_backward({rows, w, slots, counts});
+    return gather_run(rows, w, slots);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    return once(joined(grads, s), [&] { return first(ctx, s, grads); });
+  }
+  static variable_list first(AutogradContext* ctx, const variable_list& s, const variable_list& grads) {
+    variable_list r(4);
+    if (!grads[0].defined()) return r;
+    const bool weighted = s[1].defined();
+    const at::Tensor dout = cols(grads[0]), rows = dense(s[0]), w = dense(s[1]), slots = dense(s[2]), counts = dense(s[3]);
+    TORCH_CHECK(rows_ok(rows) && dout.dim() == 2 && dout.size(1) == rows.size(2) && dout.scalar_type() == rows.scalar_type() &&
+                    dout.device() == rows.device() && plan_ok(slots, counts, rows, dout.size(0), rows.size(0), rows.size(1)) &&
+                    (!weighted || (dense_beside(w, rows, at::kFloat) && w.sizes() == slots.sizes())),
+                "a saved tensor of the combination came back with another size, type or device");
+    // (the node has an edge for each tensor that is there: rows, then the weights)
+    auto g = scatter_run(dout, w, slots, counts, rows.size(0), rows.size(1), rows, ctx->needs_input_grad(0),
+                         weighted && ctx->needs_input_grad(1));
+    r[0] = g.first;
+    r[1] = g.second;
+    return r;
+  }
+};
+
+// expert_dispatch(x, slots, counts, num_experts, capacity) -> rows, or None
+PyObject* fast_dispatch(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* t[3];
+  int64_t N, capacity;
+  if (nargs != 5 || !unpack(args, 3, t) || !whole(args[3], &N) || !whole(args[4], &capacity)) Py_RETURN_NONE;
+  const at::Tensor& x = *t[0];
+  if (!on_gpu(x) || io_code(x) < 0 || x.dim() != 2 || x.size(1) < 1 || !cols1(x) || !plan_ok(*t[1], *t[2], x, x.size(0), N, capacity))
+    Py_RETURN_NONE;
+  if (wants_node({&x})) return THPVariable_Wrap(DispatchFn::apply(x, *t[1], *t[2], N, capacity));
+  return THPVariable_Wrap(scatter_run(x, at::Tensor(), *t[1], *t[2], N, capacity, at::Tensor(), true, false).first);
+  END_HANDLE_TH_ERRORS
+}
+
+// expert_combine(rows, weights, slots, counts, num_experts, capacity) -> o, or None
+PyObject* fast_combine(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  int64_t N, capacity;
+  if (nargs != 6 || traced() || !whole(args[4], &N) || !whole(args[5], &capacity)) Py_RETURN_NONE;
+  bool ok = true;
+  at::Tensor t[4];
+  for (int i = 0; i < 4; ++i) t[i] = or_none(args[i], &ok);
+  const at::Tensor &rows = t[0], &w = t[1], &slots = t[2], &counts = t[3];
+  if (!ok || !rows.defined() || !slots.defined() || !counts.defined()) Py_RETURN_NONE;
+  if (!rows_ok(rows) || rows.size(0) != N || rows.size(1) != capacity || !plan_ok(slots, counts, rows, -1, N, capacity)) Py_RETURN_NONE;
+  if (w.defined() && (!dense_beside(w, rows, at::kFloat) || w.sizes() != slots.sizes())) Py_RETURN_NONE;
+  if (wants_node({&rows, &w}))
+    return THPVariable_Wrap(CombineFn::apply(rows, w.defined() ? std::optional<at::Tensor>(w) : std::optional<at::Tensor>(), slots, counts));
+  return THPVariable_Wrap(gather_run(rows, w, slots));
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- orthogonalised updates ----
+// a, b, c of every step, from one triple of numbers
+bool triple(PyObject* o, int64_t steps, std::vector<float>* abc) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 3 || steps < 1 || steps > 10) return false;
+  float v[3];
+  for (int i = 0; i < 3; ++i) {
+    PyObject* x = PyTuple_GET_ITEM(o, i);
+    if (!PyFloat_Check(x)) return false;
+    v[i] = (float)PyFloat_AS_DOUBLE(x);
+  }
+  for (int64_t i = 0; i < steps; ++i) abc->insert(abc->end(), v, v + 3);
+  return true;
+}
+bool number(PyObject* o, double* v) {
+  if (!PyFloat_Check(o) && !(PyLong_Check(o) && !PyBool_Check(o))) return false;
+  *v = PyFloat_AsDouble(o);
+  if (!PyErr_Occurred()) return true;
+  PyErr_Clear();
+  return false;
+}
+// a dense stack of matrices of a type that the kernels take
+bool stack_ok(const at::Tensor& t) { return on_gpu(t) && io_code(t) >= 0 && t.dim() >= 2 && t.is_contiguous(); }
+int64_t heads_of(const at::Tensor& t) {
+  int64_t h = 1;
+  for (int64_t i = 0; i + 2 < t.dim(); ++i) h *= t.size(i);
+  return h;
+}
+void changed(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// orthogonalize(x, out, steps, coefficients, eps) -> the result, or None; out None: a new tensor
+PyObject* fast_ortho(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* px;
+  int64_t steps;
+  double eps;
+  bool ok = true;
+  std::vector<float> abc;
+  if (nargs != 5 || !unpack(args, 1, &px) || !whole(args[2], &steps) || !triple(args[3], steps, &abc) || !number(args[4], &eps))
+    Py_RETURN_NONE;
+  const at::Tensor& x = *px;
+  at::Tensor out = or_none(args[1], &ok);
+  if (!ok || !stack_ok(x)) Py_RETURN_NONE;
+  if (out.defined() && (!stack_ok(out) || out.device() != x.device() || out.scalar_type() != x.scalar_type() || out.sizes() != x.sizes()))
+    Py_RETURN_NONE;
+  c10::DeviceGuard guard(x.device());
+  const bool mine = !out.defined();
+  if (mine) out = at::empty(x.sizes(), x.options());
+  const int64_t H = heads_of(x), R = x.size(-2), C = x.size(-1);
+  const size_t n = fmlp_orthogonalize_workspace_bytes(H, R, C, io_code(x), (int)steps);
+  at::Tensor ws;
+  if (n) ws = bytes_on(x, n);
+  check_status(fmlp_orthogonalize(x.data_ptr(), out.data_ptr(), H, R, C, io_code(x), (int)steps, abc.data(), (float)eps,
+                                  n ? ws.data_ptr() : nullptr, n, stream_on(x)),
+               "orthogonalisation");
+  if (!mine) changed(out);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// muon_step(params, grads, momenta, lr, momentum, nesterov, weight_decay, scale, steps, coefficients, eps) -> True, or None;
+// lists, scale None: sqrt(max(1, R / C))
+PyObject* fast_muon(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 11 || traced()) Py_RETURN_NONE;
+  for (int i = 0; i < 3; ++i)
+    if (!PyList_Check(args[i])) Py_RETURN_NONE;
+  const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+  double lr, momentum, decay, scale = 0, eps;
+  int64_t steps;
+  std::vector<float> abc;
+  if (n == 0 || n > (1 << 24) || PyList_GET_SIZE(args[1]) != n || PyList_GET_SIZE(args[2]) != n || !number(args[3], &lr) ||
+      !number(args[4], &momentum) || !number(args[6], &decay) || (args[7] != Py_None && !number(args[7], &scale)) ||
+      !whole(args[8], &steps) || !triple(args[9], steps, &abc) || !number(args[10], &eps))
+    Py_RETURN_NONE;
+  if (!(lr >= 0) || !(decay >= 0) || !(momentum >= 0 && momentum <= 1)) Py_RETURN_NONE;
+  std::vector<fmlp_muon_tensor> t((size_t)n);
+  const at::Tensor* first = nullptr;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const at::Tensor* v[3];
+    for (int k = 0; k < 3; ++k) {
+      PyObject* o = PyList_GET_ITEM(args[k], i);
+      if (!THPVariable_Check(o)) Py_RETURN_NONE;
+      v[k] = &THPVariable_Unpack(o);
+      if (first == nullptr) first = v[k];
+      if (!stack_ok(*v[k]) || v[k]->device() != first->device() || v[k]->sizes() != v[0]->sizes()) Py_RETURN_NONE;
+    }
+    const int64_t R = v[0]->size(-2), C = v[0]->size(-1);
+    const double s = args[7] != Py_None ? scale : std::sqrt(std::max(1.0, C ? (double)R / (double)C : 1.0));
+    t[(size_t)i] = fmlp_muon_tensor{v[0]->data_ptr(), v[1]->data_ptr(), v[2]->data_ptr(), heads_of(*v[0]), R, C,
+                                    io_code(*v[0]), io_code(*v[1]), io_code(*v[2]), (float)s};
+  }
+  c10::DeviceGuard guard(first->device());
+  const size_t bytes = fmlp_muon_workspace_bytes((int)n, t.data(), (int)steps);
+  at::Tensor ws;
+  if (bytes) ws = bytes_on(*first, bytes);
+  check_status(fmlp_muon_step((int)n, t.data(), lr, momentum, PyObject_IsTrue(args[5]) == 1, decay, (int)steps, abc.data(), (float)eps,
+                              bytes ? ws.data_ptr() : nullptr, bytes, stream_on(*first)),
+               "muon step");
+  for (Py_ssize_t i = 0; i < n; ++i)
+    for (int k : {0, 2}) changed(THPVariable_Unpack(PyList_GET_ITEM(args[k], i)));
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
     {"fwd", (PyCFunction)(void (*)(void))fast_fwd, METH_FASTCALL, "fwd(x, w1, w2, act) -> (status, o) or None"},
     {"bwd", (PyCFunction)(void (*)(void))fast_bwd, METH_FASTCALL,
@@ -830,6 +1172,18 @@ PyMethodDef kMethods[] = {
     {"join", (PyCFunction)(void (*)(void))fast_join, METH_FASTCALL,
      "join(r, o, w_post, gate, w_pre, scale, post, eps, heads, dtype) -> (r', y) or None"},
     {"clip", (PyCFunction)(void (*)(void))fast_clip, METH_FASTCALL, "clip(grads, outs, max_norm) -> norm or None"},
+    {"expert_route", (PyCFunction)(void (*)(void))fast_route, METH_FASTCALL,
+     "expert_route(logits, k, normalize) -> (weights, experts) or None"},
+    {"expert_plan", (PyCFunction)(void (*)(void))fast_plan, METH_FASTCALL,
+     "expert_plan(experts, num_experts, capacity) -> (slots, counts) or None"},
+    {"expert_dispatch", (PyCFunction)(void (*)(void))fast_dispatch, METH_FASTCALL,
+     "expert_dispatch(x, slots, counts, num_experts, capacity) -> rows or None"},
+    {"expert_combine", (PyCFunction)(void (*)(void))fast_combine, METH_FASTCALL,
+     "expert_combine(rows, weights, slots, counts, num_experts, capacity) -> o or None"},
+    {"orthogonalize", (PyCFunction)(void (*)(void))fast_ortho, METH_FASTCALL,
+     "orthogonalize(x, out, steps, coefficients, eps) -> the result or None"},
+    {"muon_step", (PyCFunction)(void (*)(void))fast_muon, METH_FASTCALL,
+     "muon_step(params, grads, momenta, lr, momentum, nesterov, weight_decay, scale, steps, coefficients, eps) -> True or None"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fmlp_fast", "fast path of the Python wrappers", -1, kMethods};

@@ -24,7 +24,7 @@ from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 from .block import _dense_cols, _input
-from .flashmlp import _DTYPES, _alloc_ws, _ptr
+from .flashmlp import _DTYPES, _alloc_ws, _fast, _ptr
 from .gated import GatedFlashMLP, _not_traced, _On, first_derivatives_only
 
 _MAX_ROWS = 2 ** 31 - 1
@@ -121,6 +121,10 @@ def expert_route(logits: torch.Tensor, k: int, *, normalize: bool = True) -> Tup
         (weights, experts): (T, k) fp32, and (T, k) int32 in falling order of the logits. A token with fewer
         than k experts that are not masked has -1 with the weight 0 in place of the rest.
     """
+    if _fast is not None:  # tensors that need no copies and no error: else None
+        r = _fast.expert_route(logits, k, normalize)
+        if r is not None:
+            return r
     _not_traced("expert_route")
     assert logits.dim() == 2, "Logits must be (tokens, experts)"
     T, N = logits.shape
@@ -144,6 +148,11 @@ def expert_plan(experts: torch.Tensor, num_experts: int, capacity: Optional[int]
         num_experts: at most 1024; capacity: rows of each expert, None for T, so that none is dropped (as long as a
         token's choices differ).
     """
+    if _fast is not None:  # as in expert_route
+        rows = capacity if capacity is not None else len(experts) if experts.dim() else -1
+        r = _fast.expert_plan(experts, num_experts, rows)
+        if r is not None:
+            return ExpertPlan(*r, num_experts, rows)
     _not_traced("expert_plan")
     assert experts.dim() == 2, "Experts must be (tokens, choices)"
     T, k = experts.shape
@@ -237,6 +246,10 @@ class _CombineFunction(torch.autograd.Function):
 @torch.compiler.disable
 def expert_dispatch(x: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
     """Tokens x (T, D) at their experts' rows: (num_experts, capacity, D), zeros where no token is."""
+    if _fast is not None:  # as in expert_route
+        rows = _fast.expert_dispatch(x, *plan)
+        if rows is not None:
+            return rows
     _not_traced("expert_dispatch")
     assert x.dim() == 2 and x.shape[1] >= 1, "Tokens must be (tokens, columns)"
     dev = _gpu(x)
@@ -251,6 +264,10 @@ def expert_dispatch(x: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
 def expert_combine(rows: torch.Tensor, plan: ExpertPlan, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The tokens' sums of their experts' rows (num_experts, capacity, D), with weights (T, k) fp32 or plainly: (T, D) in
     the rows' dtype. A choice that was dropped adds nothing."""
+    if _fast is not None:  # as in expert_route
+        o = _fast.expert_combine(rows, weights, *plan)
+        if o is not None:
+            return o
     _not_traced("expert_combine")
     assert rows.dim() == 3 and rows.shape[2] >= 1, "Rows must be (experts, capacity, columns)"
     assert rows.shape[:2] == (plan.num_experts, plan.capacity), "Rows must be the plan's"

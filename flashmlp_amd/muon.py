@@ -26,7 +26,7 @@ from typing import Iterable, Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
-from .flashmlp import _DTYPES, _alloc_ws, _ptr
+from .flashmlp import _DTYPES, _alloc_ws, _fast, _ptr
 from .gated import _not_traced, _On
 
 _COEFFICIENTS = (3.4445, -4.775, 2.0315)
@@ -75,7 +75,6 @@ def _plain(t: torch.Tensor) -> bool:
     return t.is_contiguous() and not t.is_neg()
 
 
-@torch.no_grad()
 def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence = _COEFFICIENTS, eps: float = 1e-7,
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The matrices of x (..., R, C) orthogonalised: singular values brought towards one, singular vectors kept.
@@ -85,6 +84,10 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence = _
         out: of x's shape and type, or x itself.
     No gradient is kept.
     """
+    if _fast is not None:  # dense tensors on one GPU and no error: else None
+        r = _fast.orthogonalize(x, out, steps, coefficients, eps)
+        if r is not None:
+            return out if out is not None else r
     _not_traced("orthogonalize")
     H, R, C = _stack(x, "x")
     abc = _coefficients(coefficients, steps)
@@ -95,6 +98,7 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence = _
         if out.shape != x.shape or out.dtype != x.dtype:
             raise ValueError(f"out must be {x.dtype} of shape {tuple(x.shape)}, got {out.dtype} of {tuple(out.shape)}")
     same = out is x
+    x = x.detach()
     xd = x if _plain(x) else x.resolve_neg().contiguous()
     o = out if out is not None and _plain(out) else xd if same else torch.empty(x.shape, dtype=x.dtype, device=x.device)
     L = _lib.lib()
@@ -109,11 +113,11 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence = _
         if not out.is_inference():
             torch.autograd.graph.increment_version(out)
     else:
-        out.copy_(o)
+        with torch.no_grad():
+            out.copy_(o)
     return out
 
 
-@torch.no_grad()
 def muon_step(params: Union[torch.Tensor, Iterable[torch.Tensor]], grads: Union[torch.Tensor, Iterable[torch.Tensor]],
               momenta: Union[torch.Tensor, Iterable[torch.Tensor]], lr: float, *, momentum: float = 0.95, nesterov: bool = True,
               weight_decay: float = 0.0, scale: Optional[float] = None, steps: int = 5,
@@ -127,8 +131,11 @@ def muon_step(params: Union[torch.Tensor, Iterable[torch.Tensor]], grads: Union[
         steps, coefficients, eps: as orthogonalize's.
     A tensor that is in the call twice, or overlaps another one that is written, is refused.
     """
-    _not_traced("muon_step")
     params, grads, momenta = ([t] if isinstance(t, torch.Tensor) else list(t) for t in (params, grads, momenta))
+    if _fast is not None and _fast.muon_step(params, grads, momenta, lr, momentum, nesterov, weight_decay, scale, steps, coefficients,
+                                             eps):  # as in orthogonalize
+        return
+    _not_traced("muon_step")
     if not len(params) == len(grads) == len(momenta):
         raise ValueError(f"{len(params)} parameters, {len(grads)} gradients, {len(momenta)} momenta")
     lr, momentum, weight_decay, eps = (_number(v, n) for v, n in ((lr, "lr"), (momentum, "momentum"),
@@ -147,13 +154,13 @@ def muon_step(params: Union[torch.Tensor, Iterable[torch.Tensor]], grads: Union[
             raise ValueError(f"a parameter of shape {tuple(w.shape)} with a gradient of {tuple(g.shape)}, a momentum of {tuple(m.shape)}")
         for t, what in ((w, "parameters"), (g, "gradients"), (m, "momenta")):
             _check(t, what, dev)
-        g = g if _plain(g) else g.resolve_neg().contiguous()
+        g = g if _plain(g) else g.detach().resolve_neg().contiguous()
         held.append(g)
         dense = []
         for t in (w, m):  # other layouts through dense tensors
             d = t
             if not _plain(t):
-                d = t.resolve_neg().contiguous()
+                d = t.detach().resolve_neg().contiguous()
                 back.append((t, d))
             dense.append(d)
         held.extend(dense)
@@ -170,5 +177,6 @@ def muon_step(params: Union[torch.Tensor, Iterable[torch.Tensor]], grads: Union[
     _lib.check(st, "muon step")
     seen = {id(t) for t, _ in back}
     torch.autograd.graph.increment_version([t for t in (*params, *momenta) if id(t) not in seen and not t.is_inference()])
-    for t, d in back:
-        t.copy_(d)
+    with torch.no_grad():
+        for t, d in back:
+            t.copy_(d)

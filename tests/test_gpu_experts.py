@@ -95,7 +95,8 @@ def test_route_views():
 # ---- plan ----
 @pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("T,k,N", [(0, 2, 3), (1, 1, 1), (1, 32, 5), (63, 1, 2), (64, 1, 64), (65, 3, 7), (2047, 2, 32),
-                                   (2048, 2, 32), (2049, 2, 1000), (8191, 2, 1024), (8192, 2, 16), (8193, 2, 16), (40000, 3, 12)])
+                                   (2048, 2, 32), (2049, 2, 1000), (8191, 2, 1024), (8192, 2, 16), (8193, 2, 16), (40000, 3, 12), (30000, 3, 1000),
+                                   (300000, 4, 5), (60000, 4, 700)])
 def test_plan(T, k, N, wide):
     g = gen(T + k + N)
     experts = (N * torch.rand(T, k, generator=g) ** 2).long().clamp(max=N - 1)
