@@ -22,7 +22,7 @@ namespace {
 // ---------------------------------------------------------------------------------------------
 // plan
 // ---------------------------------------------------------------------------------------------
-constexpr int kItems = 16;  // assignments of a lane, at most
+constexpr int kItems = 16;  // assignments of a lane, at most; a power of two
 
 // expert of assignment i, -1 for none; past the last one too, whose load is then the last one's (a branch around it would have
 // every load waited for before the next)
@@ -35,17 +35,17 @@ __device__ __forceinline__ int expert_at(const void* experts, long long i, long 
   return i < M && e >= 0 && e < N ? (int)e : -1;
 }
 
-template <bool WIDE>
+template <bool WIDE, int ITEMS>
 __global__ void __launch_bounds__(256) plan_count_kernel(const void* experts, long long M, int N, int* hist) {
   extern __shared__ int plan_lds[];
-  const long long i0 = (long long)blockIdx.x * (256 * kItems) + threadIdx.x;
-  int ex[kItems];
+  const long long i0 = (long long)blockIdx.x * (256 * ITEMS) + threadIdx.x;
+  int ex[ITEMS];
 #pragma unroll
-  for (int u = 0; u < kItems; ++u) ex[u] = expert_at<WIDE>(experts, i0 + u * 256, M, N);
+  for (int u = 0; u < ITEMS; ++u) ex[u] = expert_at<WIDE>(experts, i0 + u * 256, M, N);
   for (int e = threadIdx.x; e < N; e += 256) plan_lds[e] = 0;
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < kItems; ++u)
+  for (int u = 0; u < ITEMS; ++u)
     if (ex[u] >= 0) atomicAdd(&plan_lds[ex[u]], 1);
   __syncthreads();
   for (int e = threadIdx.x; e < N; e += 256) hist[(long long)blockIdx.x * N + e] = plan_lds[e];
@@ -86,24 +86,24 @@ __global__ void __launch_bounds__(256) plan_scan_kernel(int* hist, long long chu
   }
 }
 
-// THREADS * items assignments of workgroup blockIdx.x. hist: null for one workgroup; else every chunk's counts, or where
+// THREADS * ITEMS assignments of workgroup blockIdx.x. hist: null for one workgroup; else every chunk's counts, or where
 // `scanned` what the chunks before it have.
-template <bool WIDE, int THREADS>
+template <bool WIDE, int THREADS, int ITEMS>
 __global__ void __launch_bounds__(THREADS) plan_kernel(const void* experts, long long M, int N, int bits, long long capacity,
-                                                       int* slots, int* counts, const int* hist, int scanned, int items) {
+                                                       int* slots, int* counts, const int* hist, int scanned) {
   extern __shared__ int plan_lds[];  // [waves][N]: the wave's counts, then its next position of each expert; [N] what is before
   constexpr int W = THREADS / 64;
   const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63;
   int* mine = plan_lds + wave * N;
   int* before = plan_lds + W * N;
-  const long long i0 = ((long long)blockIdx.x * W + wave) * (64 * items) + lane;
-  int ex[kItems];
+  const long long i0 = ((long long)blockIdx.x * W + wave) * (64 * ITEMS) + lane;
+  int ex[ITEMS];
 #pragma unroll
-  for (int u = 0; u < kItems; ++u) ex[u] = u < items ? expert_at<WIDE>(experts, i0 + u * 64, M, N) : -1;
+  for (int u = 0; u < ITEMS; ++u) ex[u] = expert_at<WIDE>(experts, i0 + u * 64, M, N);
   for (int e = threadIdx.x; e < (W + 1) * N; e += THREADS) plan_lds[e] = 0;
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < kItems; ++u)
+  for (int u = 0; u < ITEMS; ++u)
     if (ex[u] >= 0) atomicAdd(&mine[ex[u]], 1);
   if (hist != nullptr) {
     if (scanned) {
@@ -134,8 +134,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const void* experts, long
   }
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < kItems; ++u) {
-    if (u >= items) break;
+  for (int u = 0; u < ITEMS; ++u) {
     const int e = ex[u];
     unsigned long long same = __ballot(e >= 0);
     for (int b = 0; b < bits; ++b) {
@@ -306,14 +305,16 @@ void by_choices(int k, F f) {
 
 ExpertPlan expert_plan(int64_t M, int64_t N) {
   ExpertPlan p{};
-  // one workgroup of up to 16 waves does all where its lanes' items suffice: no second launch
-  p.threads = M <= 256 * kItems || M > 1024 * kItems ? 256 : 1024;
-  const long long most = (long long)p.threads * kItems;
-  p.chunks = M > most ? (M + most - 1) / most : 1;
-  p.items = p.chunks > 1 ? kItems : (int)std::max<long long>(1, (M + p.threads - 1) / p.threads);
+  // One workgroup of 16 waves does all where a lane has at most 4 items: no second launch. Else about 256 workgroups, whose
+  // lanes' items follow one another: 16384 assignments by one workgroup 14 us, by 64 9.
+  p.threads = M <= 1024 * 4 ? 1024 : 256;
+  const long long per = p.threads == 1024 ? 1024 : 65536;
+  p.items = 1;
+  while (p.items < kItems && p.items * per < M) p.items *= 2;
+  p.chunks = p.threads == 1024 ? 1 : (M + 256 * p.items - 1) / (256 * p.items);
   p.ws_bytes = p.chunks > 1 ? (size_t)(p.chunks * N) * sizeof(int) : 0;
-  // The workgroups add up the chunks before them themselves where that is at most 32 rounds of their 256 threads (M = 2^20, N = 32:
-  // PLANA us, a scan in a launch of its own PLANB); a scan takes over from there (M = 2^20, N = 256: PLANC, PLAND).
+  // The workgroups add up the chunks before them themselves where that is at most 32 rounds of their 256 threads (M = 196608, N = 12:
+  // 14 us, with a scan in a launch of its own 15.6); a scan takes over from there (M = 2^20, N = 256: 28 us without, 20 with it).
   long long lanes = 1;
   while (lanes < N) lanes <<= 1;
   p.scan = p.chunks > 1 && p.chunks * lanes > 32 * 256;
@@ -327,32 +328,49 @@ hipError_t launch_expert_plan(const void* experts, bool wide, long long M, int N
   int* hist = p.chunks > 1 ? (int*)ws : nullptr;
   const dim3 grid((unsigned)p.chunks);
   hipError_t e = hipSuccess;
-  const auto run = [&](auto WIDE) {
+  const auto run = [&](auto WIDE, auto THREADS, auto ITEMS) {
     constexpr bool V = decltype(WIDE)::value;
+    constexpr int TH = decltype(THREADS)::value, IT = decltype(ITEMS)::value;
     if (hist != nullptr) {
-      hipLaunchKernelGGL((plan_count_kernel<V>), grid, dim3(256), (size_t)N * 4, st, experts, M, N, hist);
+      hipLaunchKernelGGL((plan_count_kernel<V, IT>), grid, dim3(256), (size_t)N * 4, st, experts, M, N, hist);
       if ((e = hipGetLastError()) != hipSuccess) return;
       if (p.scan) {
         hipLaunchKernelGGL(plan_scan_kernel, dim3((unsigned)((N + 3) / 4)), dim3(256), 0, st, hist, p.chunks, N);
         if ((e = hipGetLastError()) != hipSuccess) return;
       }
     }
-    const size_t lds = ((size_t)p.threads / 64 + 1) * N * 4;
-    const auto go = [&](auto k) {
-      static std::atomic<unsigned long long> done{0};
-      if (lds > 65536 && (e = set_lds_once((const void*)k, 17 * (int)kMaxExperts * 4, done)) != hipSuccess) return;
-      hipLaunchKernelGGL(k, grid, dim3(p.threads), lds, st, experts, M, N, bits, capacity, slots, counts, hist, (int)p.scan, p.items);
-      e = hipGetLastError();
-    };
-    if (p.threads == 1024) go(plan_kernel<V, 1024>);
-    else go(plan_kernel<V, 256>);
+    const size_t lds = ((size_t)TH / 64 + 1) * N * 4;
+    auto k = plan_kernel<V, TH, IT>;
+    static std::atomic<unsigned long long> done{0};
+    if (lds > 65536 && (e = set_lds_once((const void*)k, 17 * (int)kMaxExperts * 4, done)) != hipSuccess) return;
+    hipLaunchKernelGGL(k, grid, dim3(TH), lds, st, experts, M, N, bits, capacity, slots, counts, hist, (int)p.scan);
+    e = hipGetLastError();
+  };
+  const auto by_items = [&](auto WIDE) {
+    const auto one = [&](auto THREADS, auto ITEMS) { run(WIDE, THREADS, ITEMS); };
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I4 = std::integral_constant<int, 4>;
+    using I8 = std::integral_constant<int, 8>;
+    using I16 = std::integral_constant<int, kItems>;
+    using T256 = std::integral_constant<int, 256>;
+    using T1024 = std::integral_constant<int, 1024>;
+    if (p.threads == 1024) {
+      if (p.items == 1) one(T1024{}, I1{});
+      else if (p.items == 2) one(T1024{}, I2{});
+      else one(T1024{}, I4{});
+    } else if (p.items == 1) one(T256{}, I1{});
+    else if (p.items == 2) one(T256{}, I2{});
+    else if (p.items == 4) one(T256{}, I4{});
+    else if (p.items == 8) one(T256{}, I8{});
+    else one(T256{}, I16{});
   };
   if (M == 0) {  // (nothing to read; the counts are zeros)
     hipLaunchKernelGGL(plan_none_kernel, dim3(1), dim3(256), 0, st, counts, N);
     return hipGetLastError();
   }
-  if (wide) run(std::true_type{});
-  else run(std::false_type{});
+  if (wide) by_items(std::true_type{});
+  else by_items(std::false_type{});
   return e;
 }
 
