@@ -43,15 +43,41 @@ __device__ __forceinline__ void load_logits(const void* logits, long long row, i
   }
 }
 
-template <int IO, int VPL>
-__global__ void __launch_bounds__(kThreads) route_fwd_kernel(RouteArgs a, int lg) {
+// The largest v, and the sum, over a group of 1 << LG lanes: within 16 lanes by DPP (lanes swapped in pairs, pairs in quads, quads and
+// halves mirrored), beyond by the LDS crossbar.
+template <int CTRL>
+__device__ __forceinline__ int dpp(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true);
+}
+template <int LG, typename OP>
+__device__ __forceinline__ int group_reduce(int v, OP op) {
+  if constexpr (LG > 0) v = op(v, dpp<0xB1>(v));
+  if constexpr (LG > 1) v = op(v, dpp<0x4E>(v));
+  if constexpr (LG > 2) v = op(v, dpp<0x141>(v));
+  if constexpr (LG > 3) v = op(v, dpp<0x140>(v));
+  if constexpr (LG > 4) v = op(v, __shfl_xor(v, 16, 64));
+  if constexpr (LG > 5) v = op(v, __shfl_xor(v, 32, 64));
+  return v;
+}
+template <int LG>
+__device__ __forceinline__ unsigned group_max(unsigned v) {
+  return (unsigned)group_reduce<LG>((int)v, [](int a, int b) { return (int)max((unsigned)a, (unsigned)b); });
+}
+template <int LG>
+__device__ __forceinline__ float group_sum(float v) {
+  return __int_as_float(group_reduce<LG>(__float_as_int(v), [](int a, int b) { return __float_as_int(__int_as_float(a) + __int_as_float(b)); }));
+}
+
+template <int IO, int VPL, int LG>
+__global__ void __launch_bounds__(kThreads) route_fwd_kernel(RouteArgs a) {
   extern __shared__ float route_lds[];
-  const int G = 1 << lg, rows = kThreads >> lg, k = a.k;
-  float* ew = route_lds;             // [rows][k] exponentials of the chosen
-  int* ei = (int*)(ew + rows * k);   // [rows][k] their experts
-  float* inv = (float*)(ei + rows * k);  // [rows] factor of the row's weights
-  const int r = (int)threadIdx.x >> lg, g = (int)threadIdx.x & (G - 1);
-  const long long t0 = (long long)blockIdx.x * rows, t = t0 + r;
+  constexpr int G = 1 << LG, ROWS = kThreads >> LG;
+  const int k = a.k;
+  float* ew = route_lds;                 // [ROWS][k] exponentials of the chosen
+  int* ei = (int*)(ew + ROWS * k);       // [ROWS][k] their experts
+  float* inv = (float*)(ei + ROWS * k);  // [ROWS] factor of the row's weights
+  const int r = (int)threadIdx.x >> LG, g = (int)threadIdx.x & (G - 1), first = (int)threadIdx.x & 63 & ~(G - 1);
+  const long long t0 = (long long)blockIdx.x * ROWS, t = t0 + r;
   float v[VPL];
   load_logits<IO, VPL>(a.logits, t * a.stride, g * VPL, a.N, t < a.T, v);
   unsigned key[VPL];
@@ -59,44 +85,39 @@ __global__ void __launch_bounds__(kThreads) route_fwd_kernel(RouteArgs a, int lg
   for (int i = 0; i < VPL; ++i) key[i] = key_of(v[i]);
   float top = 0.f, sum = 0.f;
   for (int j = 0; j < k; ++j) {
-    unsigned bk = key[0];
-    int bi = 0;
+    unsigned mk = key[0];
+    int mi = 0;
 #pragma unroll
     for (int i = 1; i < VPL; ++i)
-      if (key[i] > bk) {
-        bk = key[i];
-        bi = i;
+      if (key[i] > mk) {
+        mk = key[i];
+        mi = i;
       }
-    bi += g * VPL;
-    for (int d = 1; d < G; d <<= 1) {
-      const unsigned ok = (unsigned)__shfl_xor((int)bk, d, 64);
-      const int oi = __shfl_xor(bi, d, 64);
-      if (ok > bk || (ok == bk && oi < bi)) {
-        bk = ok;
-        bi = oi;
-      }
-    }
+    const unsigned bk = group_max<LG>(mk);
+    // the first lane that has it: lanes' logits follow one another
+    const unsigned long long has = (__ballot(mk == bk) >> first) & (G == 64 ? ~0ull : (1ull << (G & 63)) - 1);
+    const bool mine = __ffsll((long long)has) - 1 == g;
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
-      if (bi == g * VPL + i) key[i] = 0u;
+      if (mine && i == mi) key[i] = 0u;
     const float l = of_key(bk);
     if (j == 0) top = l;
     const float e = bk == 0u ? 0.f : exp_of(l - top);
     sum += e;
-    if (g == 0) {
+    if (mine) {
       ew[r * k + j] = e;
-      ei[r * k + j] = bk == 0u ? -1 : bi;
+      ei[r * k + j] = bk == 0u ? -1 : g * VPL + mi;
     }
   }
   if (!a.normalize) {
     sum = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) sum += v[i] == -__builtin_inff() ? 0.f : exp_of(v[i] - top);
-    for (int d = 1; d < G; d <<= 1) sum += __shfl_xor(sum, d, 64);
+    sum = group_sum<LG>(sum);
   }
   if (g == 0) inv[r] = sum == 0.f ? 0.f : 1.f / sum;
   __syncthreads();
-  for (int i = threadIdx.x; i < rows * k; i += kThreads) {
+  for (int i = threadIdx.x; i < ROWS * k; i += kThreads) {
     const int row = i / k;
     if (t0 + row >= a.T) break;
     const int e = ei[i];
@@ -105,51 +126,53 @@ __global__ void __launch_bounds__(kThreads) route_fwd_kernel(RouteArgs a, int lg
   }
 }
 
-template <int IO, int VPL>
-__global__ void __launch_bounds__(kThreads) route_bwd_kernel(RouteArgs a, int lg) {
-  const int G = 1 << lg, k = a.k;
-  const int r = (int)threadIdx.x >> lg, g = (int)threadIdx.x & (G - 1);
-  const long long t = (long long)blockIdx.x * (kThreads >> lg) + r;
+template <int IO, int VPL, int LG>
+__global__ void __launch_bounds__(kThreads) route_bwd_kernel(RouteArgs a) {
+  extern __shared__ float route_lds[];
+  constexpr int G = 1 << LG, ROWS = kThreads >> LG;
+  const int k = a.k;
+  float* lw = route_lds;             // [ROWS][k] w dw of the chosen
+  float* lv = lw + ROWS * k;         // [ROWS][k] w
+  int* le = (int*)(lv + ROWS * k);   // [ROWS][k] experts
+  const int r = (int)threadIdx.x >> LG, g = (int)threadIdx.x & (G - 1);
+  const long long t0 = (long long)blockIdx.x * ROWS, t = t0 + r;
   const bool there = t < a.T;
-  const float* w = a.weights + t * k;
-  const float* dw = a.dweights + t * k;
-  const int32_t* ex = a.experts + t * k;
-  float inner = 0.f;
-  if (there)
-    for (int j = 0; j < k; ++j)
-      if (ex[j] >= 0) inner += w[j] * dw[j];
   float d[VPL];
+  if (!a.normalize) load_logits<IO, VPL>(a.logits, t * a.stride, g * VPL, a.N, there, d);
+  for (int i = threadIdx.x; i < ROWS * k; i += kThreads) {
+    const bool in = i < (a.T - t0) * k;
+    const int e = in ? a.experts[t0 * k + i] : -1;
+    const float w = in ? a.weights[t0 * k + i] : 0.f, dw = in ? a.dweights[t0 * k + i] : 0.f;
+    lw[i] = e < 0 ? 0.f : w * dw;
+    lv[i] = w;
+    le[i] = e;
+  }
+  __syncthreads();
+  float inner = 0.f;
+  for (int j = 0; j < k; ++j) inner += lw[r * k + j];
   if (a.normalize) {
 #pragma unroll
     for (int i = 0; i < VPL; ++i) d[i] = 0.f;
   } else {
-    float v[VPL], top = -__builtin_inff(), sum = 0.f;
-    load_logits<IO, VPL>(a.logits, t * a.stride, g * VPL, a.N, there, v);
-    bool nan = false;
+    unsigned tk = 0u;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) tk = max(tk, key_of(d[i]));
+    const float top = of_key(group_max<LG>(tk));
+    float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      nan = nan || v[i] != v[i];
-      top = fmaxf(top, v[i]);
-    }
-    if (nan) top = __uint_as_float(0x7fc00000u);
-    for (int s = 1; s < G; s <<= 1) {
-      const float o = __shfl_xor(top, s, 64);
-      top = o != o || top != top ? __uint_as_float(0x7fc00000u) : fmaxf(top, o);
-    }
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      d[i] = v[i] == -__builtin_inff() ? 0.f : exp_of(v[i] - top);
+      d[i] = d[i] == -__builtin_inff() ? 0.f : exp_of(d[i] - top);
       sum += d[i];
     }
-    for (int s = 1; s < G; s <<= 1) sum += __shfl_xor(sum, s, 64);
+    sum = group_sum<LG>(sum);
     const float f = sum == 0.f ? 0.f : -inner / sum;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) d[i] *= f;
   }
   if (!there) return;
   for (int j = 0; j < k; ++j) {
-    const int at = ex[j] - g * VPL;
-    const float add = a.normalize ? w[j] * (dw[j] - inner) : w[j] * dw[j];
+    const int e = le[r * k + j], at = e < 0 ? -1 : e - g * VPL;
+    const float add = a.normalize ? __builtin_fmaf(-lv[r * k + j], inner, lw[r * k + j]) : lw[r * k + j];
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
       if (at == i) d[i] += add;
@@ -165,22 +188,31 @@ __global__ void __launch_bounds__(kThreads) route_bwd_kernel(RouteArgs a, int lg
   }
 }
 
+// f(io, logits of a lane, log2 of a row's lanes): 8 logits a lane, 16 where 64 lanes would not do
 template <typename F>
 hipError_t by_form(const RouteArgs& a, F f) {
-  // 8 logits a lane, 16 where 64 lanes would not do
-  const int vpl = a.N <= 512 ? 8 : 16;
   int lg = 0;
-  while ((vpl << lg) < a.N) ++lg;
+  while (lg < 6 && (8 << lg) < a.N) ++lg;
   const long long rows = kThreads >> lg, blocks = (a.T + rows - 1) / rows;
   if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
   const dim3 grid((unsigned)blocks);
-  const auto io = [&](auto VPL) {
-    if (a.io == IO_F32) f(std::integral_constant<int, IO_F32>{}, VPL, grid, lg);
-    else if (a.io == IO_BF16) f(std::integral_constant<int, IO_BF16>{}, VPL, grid, lg);
-    else f(std::integral_constant<int, IO_F16>{}, VPL, grid, lg);
+  const auto io = [&](auto VPL, auto LG) {
+    if (a.io == IO_F32) f(std::integral_constant<int, IO_F32>{}, VPL, LG, grid);
+    else if (a.io == IO_BF16) f(std::integral_constant<int, IO_BF16>{}, VPL, LG, grid);
+    else f(std::integral_constant<int, IO_F16>{}, VPL, LG, grid);
   };
-  if (vpl == 8) io(std::integral_constant<int, 8>{});
-  else io(std::integral_constant<int, 16>{});
+  const auto eight = std::integral_constant<int, 8>{};
+  switch (lg) {
+    case 0: io(eight, std::integral_constant<int, 0>{}); break;
+    case 1: io(eight, std::integral_constant<int, 1>{}); break;
+    case 2: io(eight, std::integral_constant<int, 2>{}); break;
+    case 3: io(eight, std::integral_constant<int, 3>{}); break;
+    case 4: io(eight, std::integral_constant<int, 4>{}); break;
+    case 5: io(eight, std::integral_constant<int, 5>{}); break;
+    default:
+      if (a.N <= 512) io(eight, std::integral_constant<int, 6>{});
+      else io(std::integral_constant<int, 16>{}, std::integral_constant<int, 6>{});
+  }
   return hipGetLastError();
 }
 
@@ -188,16 +220,19 @@ hipError_t by_form(const RouteArgs& a, F f) {
 
 hipError_t launch_route_fwd(const RouteArgs& a, hipStream_t st) {
   if (a.T == 0) return hipSuccess;
-  return by_form(a, [&](auto IO, auto VPL, dim3 grid, int lg) {
-    const size_t rows = (size_t)kThreads >> lg, lds = rows * (2 * (size_t)a.k + 1) * 4;
-    hipLaunchKernelGGL((route_fwd_kernel<decltype(IO)::value, decltype(VPL)::value>), grid, dim3(kThreads), lds, st, a, lg);
+  return by_form(a, [&](auto IO, auto VPL, auto LG, dim3 grid) {
+    constexpr int L = decltype(LG)::value;
+    const size_t lds = (size_t)(kThreads >> L) * (2 * (size_t)a.k + 1) * 4;
+    hipLaunchKernelGGL((route_fwd_kernel<decltype(IO)::value, decltype(VPL)::value, L>), grid, dim3(kThreads), lds, st, a);
   });
 }
 
 hipError_t launch_route_bwd(const RouteArgs& a, hipStream_t st) {
   if (a.T == 0) return hipSuccess;
-  return by_form(a, [&](auto IO, auto VPL, dim3 grid, int lg) {
-    hipLaunchKernelGGL((route_bwd_kernel<decltype(IO)::value, decltype(VPL)::value>), grid, dim3(kThreads), 0, st, a, lg);
+  return by_form(a, [&](auto IO, auto VPL, auto LG, dim3 grid) {
+    constexpr int L = decltype(LG)::value;
+    const size_t lds = (size_t)(kThreads >> L) * 3 * (size_t)a.k * 4;
+    hipLaunchKernelGGL((route_bwd_kernel<decltype(IO)::value, decltype(VPL)::value, L>), grid, dim3(kThreads), lds, st, a);
   });
 }
 
