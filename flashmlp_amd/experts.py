@@ -68,6 +68,20 @@ def _needs_function(*ts) -> bool:
     return torch.is_grad_enabled() and any(t.requires_grad for t in ts) or any(unpack_dual(t).tangent is not None for t in ts)
 
 
+def _save(ctx, *ts):
+    ctx.save_for_backward(*ts)
+    ctx.saved_as = [None if t is None else (t.shape, t.dtype, t.device) for t in ts]
+
+
+def _saved(ctx):
+    # hooks may bring a tensor back in any layout: the kernels are given dense ones of the size, type and device that were saved
+    ts = ctx.saved_tensors  # (each is unpacked once)
+    for t, was in zip(ts, ctx.saved_as):
+        if t is not None and (t.shape, t.dtype, t.device) != was:
+            raise RuntimeError("a saved tensor of the experts' operators came back with another size, type or device")
+    return ts
+
+
 # ---------------------------------------------------------------------------------------------
 # route
 # ---------------------------------------------------------------------------------------------
@@ -89,7 +103,7 @@ class _RouteFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, k, normalize):
         weights, experts = _route_fwd(logits, k, normalize)
-        ctx.save_for_backward(None if normalize else logits, weights, experts)
+        _save(ctx, None if normalize else logits, weights, experts)
         ctx.args = (logits.shape, logits.dtype, normalize)
         ctx.mark_non_differentiable(experts)
         return weights, experts
@@ -97,7 +111,7 @@ class _RouteFunction(torch.autograd.Function):
     @staticmethod
     @first_derivatives_only
     def backward(ctx, dw, _):
-        logits, weights, experts = ctx.saved_tensors
+        logits, weights, experts = _saved(ctx)
         (T, N), dtype, normalize = ctx.args
         weights, experts, dw = _dense(weights), _dense(experts), _dense(dw)
         logits = None if logits is None else _dense_cols(logits)
@@ -149,7 +163,7 @@ def expert_plan(experts: torch.Tensor, num_experts: int, capacity: Optional[int]
         token's choices differ).
     """
     if _fast is not None:  # as in expert_route
-        rows = capacity if capacity is not None else len(experts) if experts.dim() else -1
+        rows = capacity if capacity is not None else experts.shape[0] if experts.dim() else -1
         r = _fast.expert_plan(experts, num_experts, rows)
         if r is not None:
             return ExpertPlan(*r, num_experts, rows)
@@ -218,25 +232,25 @@ def _gather(rows, weights, slots):
 class _DispatchFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, slots, counts, N, capacity):
-        ctx.save_for_backward(slots)
+        _save(ctx, slots)
         return _scatter(x, None, slots, counts, N, capacity, None, True, False)[0]
 
     @staticmethod
     @first_derivatives_only
     def backward(ctx, drows):
-        return (_gather(drows, None, *ctx.saved_tensors),) + (None,) * 4
+        return (_gather(drows, None, *_saved(ctx)),) + (None,) * 4
 
 
 class _CombineFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, slots, counts):
-        ctx.save_for_backward(rows, weights, slots, counts)
+        _save(ctx, rows, weights, slots, counts)
         return _gather(rows, weights, slots)
 
     @staticmethod
     @first_derivatives_only
     def backward(ctx, do):
-        rows, weights, slots, counts = ctx.saved_tensors
+        rows, weights, slots, counts = _saved(ctx)
         N, capacity, _ = rows.shape
         drows, dw = _scatter(do, weights, slots, counts, N, capacity, rows, ctx.needs_input_grad[0],
                              weights is not None and ctx.needs_input_grad[1])

@@ -26,6 +26,7 @@ from typing import Iterable, Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
+from .block import _input
 from .flashmlp import _DTYPES, _alloc_ws, _fast, _ptr
 from .gated import _not_traced, _On
 
@@ -62,6 +63,7 @@ def _check(t: torch.Tensor, what: str, dev=None):
         raise TypeError(f"FlashMLP supports float16, bfloat16 and float32 {what}, got {t.dtype}")
     if t.layout != torch.strided:
         raise TypeError(f"{what} must be dense tensors, got {t.layout}")
+    _input(t)  # (memory of its own)
 
 
 def _number(v, name):
