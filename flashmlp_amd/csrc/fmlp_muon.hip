@@ -229,28 +229,39 @@ __device__ __forceinline__ Part part_of(const MuonRef& t, int parts) {
   p.t1 = min(tiles, p.t0 + per);
   return p;
 }
-// The 32 x 32 tiles i <= j of a Gram matrix among four waves. From four blocks on a wave has rows i0 and i1 = RB - 1 - i0 of tiles,
-// RB + 1 of them whose operands it reads once each (RB = 8: i0 is the wave, RB = 4: wave / 2); KQ waves share the long side's
-// 16s of a tile of data. Below, every wave has all tiles and a quarter of the 16s.
+// The 32 x 32 tiles i <= j of a Gram matrix among a workgroup's waves, so that each reads few operands for its tiles.
+//   NP = 256, eight waves: rows i0 = wave / 2 and 7 - i0 have nine tiles; one wave takes i0's first five, the other the rest.
+//   NP = 128, four waves: rows i0 = wave / 2 and 3 - i0 have five; the two waves that have them share the long side's 16s.
+//   Below, every wave has all tiles and a quarter of the 16s.
 template <int NP>
 struct Pairs {
-  static constexpr int RB = NP / 32, KQ = NP == 256 ? 1 : NP == 128 ? 2 : 4;
-  static constexpr int MP = RB >= 4 ? RB + RB / 2 : RB * (RB + 1) / 2;  // sums: row i0's by column, then row i1's from RB / 2 on
+  static constexpr int WAVES = NP == 256 ? 8 : 4, RB = NP / 32, KQ = NP == 256 ? 1 : NP == 128 ? 2 : 4;
+  static constexpr int MP = NP == 256 ? 5 : NP == 128 ? 6 : RB * (RB + 1) / 2;  // sums (128: row i0's by column, then the other's from 2 on)
   // tile p of the wave: row, column, whether it has it
-  static __device__ __forceinline__ int i0(int wave) { return wave / KQ; }
+  static __device__ __forceinline__ int i0(int wave) { return wave / 2; }
   static __device__ __forceinline__ int kq(int wave) { return wave % KQ; }
-  static __device__ __forceinline__ int row(int p, int wave) { return RB >= 4 ? p < RB ? i0(wave) : RB - 1 - i0(wave) : p < RB ? 0 : 1; }
-  static __device__ __forceinline__ int col(int p, int) { return p < RB ? p : p - RB + RB / 2; }
-  static __device__ __forceinline__ bool has(int p, int wave) { return col(p, wave) >= row(p, wave); }
+  static __device__ __forceinline__ int row(int p, int wave) {
+    if constexpr (NP == 256) return (wave & 1) == 0 || p < 3 - i0(wave) ? i0(wave) : 7 - i0(wave);
+    else if constexpr (NP == 128) return p < RB ? i0(wave) : RB - 1 - i0(wave);
+    else return p < RB ? 0 : 1;
+  }
+  static __device__ __forceinline__ int col(int p, int wave) {
+    if constexpr (NP == 256) return (wave & 1) == 0 ? i0(wave) + p : p < 3 - i0(wave) ? i0(wave) + 5 + p : 4 + p;
+    else return p < RB ? p : p - RB + RB / 2;
+  }
+  static __device__ __forceinline__ bool has(int p, int wave) {
+    if constexpr (NP == 256) return (wave & 1) == 0 || p < 4;
+    else return col(p, wave) >= row(p, wave);
+  }
 };
 
 // The wave's tiles of G over the data tiles [t0, t1), and with a momentum m' on the way. With KQ = 4 the sums are wave
-// 0's. TERMS 1: x as it is (BF its type); 3: u in fp32, from x and m. 256 threads.
+// 0's. TERMS 1: x as it is (BF its type); 3: u in fp32, from x and m.
 template <int NP, bool TALL, int TERMS, bool BF, bool VEC>
 __device__ __forceinline__ void gram_tiles(f32x16 (&acc)[Pairs<NP>::MP], const MuonRef& t, const Part& part, float mu, float nu,
                                            int nesterov, int wave) {
   using T = Tile<NP, TALL>;
-  constexpr int KT = T::KT, KQ = Pairs<NP>::KQ, MP = Pairs<NP>::MP, Q = T::UNITS / 256;
+  constexpr int THREADS = Pairs<NP>::WAVES * 64, KT = T::KT, KQ = Pairs<NP>::KQ, MP = Pairs<NP>::MP, Q = T::UNITS / THREADS;
   const int R = t.R, C = t.C, lane = (int)threadIdx.x & 63;
   const long long t0 = part.t0, t1 = part.t1;
   const Mat<VEC> X(t.x, t.x_io, part.h, R, C), M(t.m, t.m_io, part.h, R, C);
@@ -260,7 +271,7 @@ __device__ __forceinline__ void gram_tiles(f32x16 (&acc)[Pairs<NP>::MP], const M
 
   Raw x[Q], m[TERMS == 3 ? Q : 1];
   const auto load = [&](long long tile, int q) {
-    const Piece<NP, TALL, 256> at(q, tile * KT, R, C);
+    const Piece<NP, TALL, THREADS> at(q, tile * KT, R, C);
     if constexpr (TERMS == 3) {
       X.load(at.i, at.n, x[q]);
       M.load(at.i, at.n, m[q]);
@@ -269,7 +280,7 @@ __device__ __forceinline__ void gram_tiles(f32x16 (&acc)[Pairs<NP>::MP], const M
     }
   };
   const auto put = [&](long long tile, int q) {
-    const Piece<NP, TALL, 256> at(q, tile * KT, R, C);
+    const Piece<NP, TALL, THREADS> at(q, tile * KT, R, C);
     const int o = T::at(at.row, at.u);
     if constexpr (TERMS == 3) {
       float f[8];
@@ -312,7 +323,17 @@ __device__ __forceinline__ void gram_tiles(f32x16 (&acc)[Pairs<NP>::MP], const M
 #pragma unroll
         for (int e = 0; e < TERMS; ++e) v[e] = T::by_small(e * T::TERM, block * 32, k0, lane);
       };
-      if constexpr (PR::RB >= 4) {
+      if constexpr (NP == 256) {
+        u32x4 a[TERMS], b[TERMS];
+        fetch(PR::row(0, wave), a);
+#pragma unroll
+        for (int p = 0; p < MP; ++p) {
+          if (!PR::has(p, wave)) continue;
+          if (p > 0 && PR::row(p, wave) != PR::row(p - 1, wave)) fetch(PR::row(p, wave), a);
+          fetch(PR::col(p, wave), b);
+          acc[p] = mfma_terms<TERMS, BF>(a, b, acc[p]);
+        }
+      } else if constexpr (NP == 128) {
         u32x4 a[TERMS], c[TERMS];
         fetch(PR::i0(wave), a);
         fetch(PR::RB - 1 - PR::i0(wave), c);
@@ -358,7 +379,7 @@ __device__ __forceinline__ void gram_tiles(f32x16 (&acc)[Pairs<NP>::MP], const M
 }
 template <int NP, bool TALL, int TERMS>
 constexpr int gram_lds() {
-  return std::max(TERMS * Tile<NP, TALL>::TERM, (4 - 4 / Pairs<NP>::KQ) * Pairs<NP>::MP * 4096);
+  return std::max(TERMS * Tile<NP, TALL>::TERM, (Pairs<NP>::WAVES - Pairs<NP>::WAVES / Pairs<NP>::KQ) * Pairs<NP>::MP * 4096);
 }
 
 // the wave's tiles as both halves of a symmetric matrix, rows `pitch` floats apart
@@ -383,7 +404,7 @@ __device__ __forceinline__ void store_gram(const f32x16 (&acc)[Pairs<NP>::MP], f
 
 // Gram matrices: `parts` workgroups a matrix, each a range of the long side, their partial sums whole and symmetric.
 template <int NP, int TERMS, bool BF, bool VEC>
-__global__ void __launch_bounds__(256) gram_kernel(MuonTable tab, float* __restrict__ G, int parts, float mu, float nu, int nesterov) {
+__global__ void __launch_bounds__(Pairs<NP>::WAVES * 64) gram_kernel(MuonTable tab, float* __restrict__ G, int parts, float mu, float nu, int nesterov) {
   const MuonRef& t = tensor_of(tab, blockIdx.x);
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   f32x16 acc[Pairs<NP>::MP];
@@ -743,8 +764,8 @@ hipError_t muon_gram(const MuonKind& kind, const MuonTable& tab, unsigned blocks
   return by_kind(kind, [&](auto T, auto B, auto V) {
     constexpr int TERMS = decltype(T)::value;
     static std::atomic<unsigned long long> done{0};
-    return launch<both_gram_lds<NP, TERMS>()>(gram_kernel<NP, TERMS, decltype(B)::value, decltype(V)::value>, done, blocks, 256, st,
-                                              tab, G, parts, c.mu, c.nu, c.nesterov);
+    return launch<both_gram_lds<NP, TERMS>()>(gram_kernel<NP, TERMS, decltype(B)::value, decltype(V)::value>, done, blocks,
+                                              Pairs<NP>::WAVES * 64, st, tab, G, parts, c.mu, c.nu, c.nesterov);
   });
 }
 template <int NP>

@@ -203,13 +203,17 @@ constexpr int N2 = 256, kMat = 2 * N2 * N2;  // fp16 values of a matrix, first t
 
 // Workgroup b of tiles of many matrices: matrix and tile. Workgroups go to the eight XCDs in turn; a matrix stays on
 // one, whose L2 then holds what the launches before wrote of it.
+template <int TILES>
 __device__ __forceinline__ bool place(long long matrices, long long* m, int* tile) {
   const unsigned b = blockIdx.x >> 3;
-  *m = (long long)(b >> 4) * 8 + (blockIdx.x & 7);
-  *tile = b & 15;
+  *m = (long long)(b / TILES) * 8 + (blockIdx.x & 7);
+  *tile = b % TILES;
   return *m < matrices;
 }
-unsigned place_blocks(long long matrices) { return (unsigned)((matrices + 7) / 8 * 128); }
+template <int TILES>
+unsigned place_blocks(long long matrices) {
+  return (unsigned)((matrices + 7) / 8 * 8 * TILES);
+}
 
 // G as fp16 terms from its partial sums; a tile is 16 rows
 __global__ void __launch_bounds__(256) sum256_kernel(const float* __restrict__ G0, int parts, u16* __restrict__ G,
@@ -217,7 +221,7 @@ __global__ void __launch_bounds__(256) sum256_kernel(const float* __restrict__ G
   __shared__ float scr[4];
   long long m;
   int tile;
-  if (!place(matrices, &m, &tile)) return;
+  if (!place<16>(matrices, &m, &tile)) return;
   const float* src = G0 + m * parts * (N2 * N2);
   float d = 0.f;
   f32x4 f[4];
@@ -260,6 +264,32 @@ struct Prod256 {
   float ca, cb, cc, cg;  // where one of the first three is not 0: ca 1 + cb cg A + cc A B
 };
 
+// what becomes of a 32 x 32 tile of a product at row r, column c
+__device__ __forceinline__ void finish256(const Prod256& p, const f32x16& acc, long long m, int r, int c, int g, int l32) {
+  // lane: column c + l32, rows r + 16 h + 4 g + {0..3, 8..11}; stored as that unit of row c + l32 (the matrices are symmetric)
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const size_t at = m * kMat + muon_chunk<N2>(c + l32, r / 16 + h, g);
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = acc[8 * h + j] * p.back;
+    if (p.cc != 0.f || p.ca != 0.f || p.cb != 0.f) {
+      const u32x4 vh = *(const u32x4*)(p.a + at), vl = *(const u32x4*)(p.a + at + N2 * N2);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = j & 1 ? hi_f32<false>(vh[j >> 1]) + hi_f32<false>(vl[j >> 1])
+                              : lo_f32<false>(vh[j >> 1]) + lo_f32<false>(vl[j >> 1]);
+        const int at_r = r + 16 * h + 4 * g + (j & 3) + (j & 4) * 2;
+        f[j] = __builtin_fmaf(p.cc, f[j], __builtin_fmaf(p.cb, x * p.cg, at_r == c + l32 ? p.ca : 0.f));
+      }
+    }
+    u32x4 hi, lo;
+    split8(f, p.scale, hi, lo);
+    *(u32x4*)(p.out + at) = hi;
+    *(u32x4*)(p.out + at + N2 * N2) = lo;
+  }
+}
+
 // 64 x 64 tiles of out, 32 x 32 and half of the inner dimension a wave, whose loads are all in flight at once; blockIdx.y
 // picks one of two independent products
 __global__ void __launch_bounds__(512) prod256_kernel(Prod256 p0, Prod256 p1, long long matrices) {
@@ -268,7 +298,7 @@ __global__ void __launch_bounds__(512) prod256_kernel(Prod256 p0, Prod256 p1, lo
   const int lane = (int)threadIdx.x & 63, g = lane >> 5, l32 = lane & 31, wave = (int)threadIdx.x >> 6;
   long long m;
   int tile;
-  if (!place(matrices, &m, &tile)) return;
+  if (!place<16>(matrices, &m, &tile)) return;
   const int quad = wave & 3, k0 = (wave >> 2) * (N2 / 2);
   const int r0 = (tile >> 2) * 64 + (quad >> 1) * 32, c0 = (tile & 3) * 64 + (quad & 1) * 32;
   const u16* A = p.a + m * kMat + muon_chunk<N2>(r0 + l32, k0 / 16, g);
@@ -301,40 +331,67 @@ __global__ void __launch_bounds__(512) prod256_kernel(Prod256 p0, Prod256 p1, lo
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[4 * q + j] += v[j];
   }
-  // lane: column c0 + l32, rows r0 + 16 h + 4 g + {0..3, 8..11}; stored as that unit of row c0 + l32 (the matrices are symmetric)
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const size_t at = m * kMat + muon_chunk<N2>(c0 + l32, r0 / 16 + h, g);
-    float f[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = acc[8 * h + j] * p.back;
-    if (p.cc != 0.f || p.ca != 0.f || p.cb != 0.f) {
-      const u32x4 vh = *(const u32x4*)(p.a + at), vl = *(const u32x4*)(p.a + at + N2 * N2);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x = j & 1 ? hi_f32<false>(vh[j >> 1]) + hi_f32<false>(vl[j >> 1])
-                              : lo_f32<false>(vh[j >> 1]) + lo_f32<false>(vl[j >> 1]);
-        const int r = r0 + 16 * h + 4 * g + (j & 3) + (j & 4) * 2;
-        f[j] = __builtin_fmaf(p.cc, f[j], __builtin_fmaf(p.cb, x * p.cg, r == c0 + l32 ? p.ca : 0.f));
-      }
-    }
-    u32x4 hi, lo;
-    split8(f, p.scale, hi, lo);
-    *(u32x4*)(p.out + at) = hi;
-    *(u32x4*)(p.out + at + N2 * N2) = lo;
-  }
+  finish256(p, acc, m, r0, c0, g, l32);
 }
 
-hipError_t launch_256(long long matrices, const float* G0, int parts, u16* P, MuonInfo* info, const MuonSteps& s, void* ws,
+// The same in tiles of 128 x 128, 32 x 64 a wave, which reads half as much for a result: for many matrices, where the CU's path to
+// its L2 is the bound
+__global__ void __launch_bounds__(512) prod256_wide_kernel(Prod256 p0, Prod256 p1, long long matrices) {
+  const Prod256 p = blockIdx.y == 0 ? p0 : p1;
+  const int lane = (int)threadIdx.x & 63, g = lane >> 5, l32 = lane & 31, wave = (int)threadIdx.x >> 6;
+  long long m;
+  int tile;
+  if (!place<4>(matrices, &m, &tile)) return;
+  const int r0 = (tile >> 1) * 128 + (wave & 3) * 32, c0 = (tile & 1) * 128 + (wave >> 2) * 64;
+  const u16* A = p.a + m * kMat + muon_chunk<N2>(r0 + l32, 0, g);
+  const u16* B = p.b + m * kMat + muon_chunk<N2>(c0 + l32, 0, g);
+  constexpr int KS = N2 / 16, AHEAD = 3;
+  constexpr size_t NEXT = (size_t)KS * 512;  // the next 32 rows
+  f32x16 acc[2] = {zero16(), zero16()};
+  u32x4 ring[AHEAD + 1][6];
+  const auto fetch = [&](int k) {
+    u32x4(&v)[6] = ring[k % (AHEAD + 1)];
+    v[0] = *(const u32x4*)(A + 512 * k);
+    v[1] = *(const u32x4*)(A + N2 * N2 + 512 * k);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      v[2 + 2 * c] = *(const u32x4*)(B + c * NEXT + 512 * k);
+      v[3 + 2 * c] = *(const u32x4*)(B + c * NEXT + N2 * N2 + 512 * k);
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) fetch(k);
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    if (k + AHEAD < KS) fetch(k + AHEAD);
+    __builtin_amdgcn_sched_barrier(0);
+    const u32x4(&v)[6] = ring[k % (AHEAD + 1)];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) acc[c] = mfma<false>(v[1], v[2 + 2 * c], acc[c]);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) acc[c] = mfma<false>(v[0], v[3 + 2 * c], acc[c]);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) acc[c] = mfma<false>(v[0], v[2 + 2 * c], acc[c]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) finish256(p, acc[c], m, r0, c0 + 32 * c, g, l32);
+}
+
+hipError_t steps_256(long long matrices, const float* G0, int parts, u16* P, MuonInfo* info, const MuonSteps& s, void* ws,
                       hipStream_t st) {
   const size_t one = (size_t)matrices * kMat;
   u16* G = (u16*)ws;
   u16 *Q = G + one, *T = Q + one, *R = T + one;
-  hipLaunchKernelGGL(sum256_kernel, dim3(place_blocks(matrices)), dim3(256), 0, st, G0, parts, G, info, s, matrices);
+  hipLaunchKernelGGL(sum256_kernel, dim3(place_blocks<16>(matrices)), dim3(256), 0, st, G0, parts, G, info, s, matrices);
   hipError_t e = hipGetLastError();
   const auto run = [&](const Prod256& a, const Prod256* b) {
     if (e != hipSuccess) return;
-    hipLaunchKernelGGL(prod256_kernel, dim3(place_blocks(matrices), b ? 2 : 1), dim3(512), 0, st, a, b ? *b : a, matrices);
+    // (one product of 32 matrices 10.0 us, 9.0 in the smaller tiles; of 192 33 us, 43)
+    if (matrices >= 64)
+      hipLaunchKernelGGL(prod256_wide_kernel, dim3(place_blocks<4>(matrices), b ? 2 : 1), dim3(512), 0, st, a, b ? *b : a, matrices);
+    else
+      hipLaunchKernelGGL(prod256_kernel, dim3(place_blocks<16>(matrices), b ? 2 : 1), dim3(512), 0, st, a, b ? *b : a, matrices);
     e = hipGetLastError();
   };
   // P_k, the product of the steps' polynomials so far, takes turns in R and P, the last one in P; the first step's Q is P_0
@@ -357,10 +414,28 @@ hipError_t launch_256(long long matrices, const float* G0, int parts, u16* P, Mu
   return e;
 }
 
+// As many matrices at once as leave all that the launches pass on in the last cache (192: 200 MB): a product of 342 at once
+// takes 76 us, of 171 33
+long long at_once(long long matrices) {
+  const long long parts = (matrices + 191) / 192;
+  return parts ? (matrices + parts - 1) / parts : 0;
+}
+
+hipError_t launch_256(long long matrices, const float* G0, int parts, u16* P, MuonInfo* info, const MuonSteps& s, void* ws,
+                      hipStream_t st) {
+  const long long chunk = at_once(matrices);
+  for (long long m = 0; m < matrices; m += chunk) {
+    const long long n = matrices - m < chunk ? matrices - m : chunk;
+    const hipError_t e = steps_256(n, G0 + m * parts * (N2 * N2), parts, P + m * kMat, info + m, s, ws, st);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 }  // namespace
 
 size_t muon_iter_ws_bytes(int NP, long long matrices) {
-  return NP == 256 ? (size_t)matrices * kMat * 4 * sizeof(u16) : 0;
+  return NP == 256 ? (size_t)at_once(matrices) * kMat * 4 * sizeof(u16) : 0;
 }
 
 hipError_t launch_muon_iter(int NP, long long matrices, const float* G, int parts, unsigned short* P, MuonInfo* info,

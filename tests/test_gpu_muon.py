@@ -230,6 +230,14 @@ def test_many_matrices(n, e, tall, dtype):
     check(x, orthogonalize(x.cuda()))
 
 
+@pytest.mark.parametrize("dtype", [BF, FL])
+@pytest.mark.parametrize("H,n,e", [(70, 200, 210), (64, 256, 300), (65, 129, 136), (400, 140, 150)])
+def test_many_wide_matrices(H, n, e, dtype):
+    x = torch.randn(H, n, e, generator=gen(n * e)).to(dtype)
+    check(x, orthogonalize(x.cuda()))
+    check(x[:3].mT.contiguous(), orthogonalize(x.mT.contiguous().cuda())[:3])
+
+
 @pytest.mark.parametrize("types", [(FL, BF, FL), (BF, HF, BF)])
 def test_muon_step_of_many_matrices(types):
     """the same with weights and momenta, in stacks of both orientations and several sizes"""
