@@ -67,7 +67,7 @@ __device__ __forceinline__ void put_left(const Cols<NP>& c, int n, int q) {
 // out = (left operand in LDS) * b, in the terms' scales. A step has 32 of the inner dimension for TP tiles of rows.
 template <int NP>
 __device__ __forceinline__ void product(f32x4 (&out)[NP / 16], const Cols<NP>& b, int q, int l16) {
-  constexpr int TP = 2, GROUPS = NP / 16 / TP, STEPS = NP / 32 * GROUPS, AHEAD = NP == 128 ? 0 : 1;
+  constexpr int TP = 2, GROUPS = NP / 16 / TP, STEPS = NP / 32 * GROUPS, AHEAD = 1;
   u32x4 ah[AHEAD + 1][TP], al[AHEAD + 1][TP];
   const auto fetch = [&](int j) {
     const int k = j / GROUPS, p = j % GROUPS;
@@ -96,7 +96,7 @@ __device__ __forceinline__ void product(f32x4 (&out)[NP / 16], const Cols<NP>& b
 }
 
 template <int NP>
-__global__ void __launch_bounds__(NP * 4) __attribute__((amdgpu_waves_per_eu(4, 4)))
+__global__ void __launch_bounds__(NP * 4) __attribute__((amdgpu_waves_per_eu(2, 2)))
 iter_kernel(const float* __restrict__ G0, int parts, u16* __restrict__ P0, MuonInfo* __restrict__ info, MuonSteps s) {
   constexpr int TN = NP / 16, SCR = NP * NP * 4;  // LDS: the left operand, then the waves' sums
   const int lane = (int)threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
@@ -107,9 +107,20 @@ iter_kernel(const float* __restrict__ G0, int parts, u16* __restrict__ P0, MuonI
   const float* src = G0 + m * parts * (NP * NP) + (size_t)n * NP + 4 * q;
 #pragma unroll
   for (int t = 0; t < TN; ++t) v[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < parts; ++p)
+  constexpr int UP = NP == 128 ? 2 : 1;  // partial sums in flight at once
+  for (int p = 0; p < parts; p += UP) {
+    f32x4 w[UP][TN];
 #pragma unroll
-    for (int t = 0; t < TN; ++t) v[t] += *(const f32x4*)(src + (size_t)p * (NP * NP) + 16 * t);
+    for (int u = 0; u < UP; ++u)
+#pragma unroll
+      for (int t = 0; t < TN; ++t) w[u][t] = *(const f32x4*)(src + (size_t)min(p + u, parts - 1) * (NP * NP) + 16 * t);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < UP; ++u)
+      if (p + u < parts)
+#pragma unroll
+        for (int t = 0; t < TN; ++t) v[t] += w[u][t];
+  }
   // the lane that has element (n, n): row 4 q + i of tile `wave` is l16
   const auto diagonal = [&](int t, int i) { return t == wave && 4 * q + i == l16; };
   float d = 0.f;

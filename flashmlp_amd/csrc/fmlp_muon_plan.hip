@@ -41,11 +41,12 @@ Group group_of(int NP, int n, const MuonTensor* t, int cus) {
   // two workgroups for each CU at least: below, CUs idle that parts of matrices would fill
   r.whole = NP <= 128 && r.matrices >= 2 * cus;
   if (r.whole) return r;
-  // three workgroups a CU at least, as far as there are tiles; of Gram matrices no more than pay: a tile takes about
-  // 3 us (6 at NP = 256, whose workgroups are alone on their CUs), a part's sums are written and read at about 4 TB/s
+  // three workgroups a CU at least, as far as there are tiles. Of Gram matrices no more than pay: a tile takes about 3 us (6 at
+  // NP = 256), and of a part's sums each matrix's are read by one workgroup of the steps (about 40 KB a us; 16 matrices
+  // of 128 x 1024 in 10 parts 11 us and 18 for the reading) or, at NP = 256, by all (written and read at about 4 TB/s)
   const long long want = (3LL * cus + r.matrices - 1) / r.matrices;
-  const double part_us = (double)r.matrices * NP * NP * 8 / 4e6;
-  const long long pays = std::max(1LL, std::llround(std::sqrt((double)r.tiles * (NP == 256 ? 6 : 3) / part_us)));
+  const double tile_us = NP == 256 ? 6 : 3, part_us = NP == 256 ? (double)r.matrices * NP * NP * 8 / 4e6 : NP * NP * 4 / 4e4;
+  const long long pays = std::max(1LL, std::llround(std::sqrt((double)r.tiles * tile_us / part_us)));
   r.gram_parts = (int)std::max(1LL, std::min(std::min(want, pays), r.tiles));
   r.apply_parts = (int)std::max(1LL, std::min(want, r.tiles));
   const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
