@@ -38,8 +38,10 @@ Group group_of(int NP, int n, const MuonTensor* t, int cus) {
       r.tiles = std::max(r.tiles, ((long long)std::max(t[i].R, t[i].C) + KT - 1) / KT);
     }
   if (r.matrices == 0) return r;
-  // two workgroups for each CU at least: below, CUs idle that parts of matrices would fill
-  r.whole = NP <= 128 && r.matrices >= 2 * cus;
+  // Below about a matrix for each CU (NP = 128) or three for two, CUs idle that parts of matrices would fill. Muon step in fp32 whole
+  // and in parts: 128 x 1024, 128 matrices 198 and 176 us, 256 251 and 279, 512 443 and 477, 768 664 and 785; 64 x 768,
+  // 256 matrices 81 and 80 us, 384 99 and 108, 512 113 and 135
+  r.whole = NP <= 128 && 2 * r.matrices >= (NP == 128 ? 2 : 3) * cus;
   if (r.whole) return r;
   // three workgroups a CU at least, as far as there are tiles. Of Gram matrices no more than pay: a tile takes about 3 us (6 at
   // NP = 256), and of a part's sums each matrix's are read by one workgroup of the steps (about 40 KB a us; 16 matrices
