@@ -8,6 +8,10 @@
 // key that is left, compared over the group. Keys are the logits' bits in an order that integers compare, NaN
 // largest; key 0 is what no choice takes: a masked logit (-infinity) and one that is taken. A
 // token with fewer than k unmasked logits has -1 and the weight 0 in place of the rest.
+//
+// Bound by vector issue, about 60 instructions a round and wave of 8 rows at 64 experts: 65536 x 64 bf16, 8 a token, 11.7 us (12 MB),
+// the gradient 7.3 (15 MB). Maxima over the group through the LDS crossbar and every lane's scan of the chosen index: 16.4; the choices
+// of a row read by each of its lanes: 10.4.
 #include "fmlp_experts.h"
 #include "fmlp_vec.h"
 
