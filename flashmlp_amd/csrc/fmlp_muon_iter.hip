@@ -9,7 +9,7 @@
 // rounding leaves none quite symmetric: products are ordered as Q^T G^T Q, whose antisymmetric part
 // shrinks with q^2. (Q^T Q^T G lets it grow 7-fold a step where l is near 1: 2e-4 instead of 3e-6 after five steps at n = 16.)
 //
-// Measured, a step (four products): 0.9 us at NP = 32, 2.4 at 64, 8.6 at 128 (matrix instructions alone 0.2, 0.7 and 5.4: the
+// Measured, a step (four products): 0.7 us at NP = 32, 2.4 at 64, 8.6 at 128 (matrix instructions alone 0.2, 0.7 and 5.4: the
 // rest is the chain of LDS reads, conversions and three barriers, as few matrices leave one workgroup a CU); at 256, whose
 // products are launches, 14.5 for 8 matrices and 125 for 192. 32 columns a wave instead of 16: 64 x 683 24 us instead of 18.
 //
