@@ -10,9 +10,9 @@
     rows[slot(t, j)] = x[t],  o[t] = sum over j of weights[t, j] * rows[slot(t, j)]
 
 `rows` is the (H, B, D) layout that flashmlp_fwd and flashmlp_gated_fwd read, a head for each expert. An expert takes its
-tokens in their order up to `capacity`, further ones are dropped (capacity=None: a row for every token, none is);
-rows without a token are zeros. Nothing waits for the loads: sizes do not depend on them. All but the plan are
-differentiable; sums are fp32, in a fixed order. Tokens and rows are fp16, bf16 or fp32, weights fp32.
+tokens in their order up to `capacity`, further ones are dropped, their weights not given to others (capacity=None: a row
+for every token, none is); rows without a token are zeros. Nothing waits for the loads: sizes do not depend on them. All
+but the plan are differentiable; sums are fp32, in a fixed order. Tokens and rows are fp16, bf16 or fp32, weights fp32.
 """
 from __future__ import annotations
 
@@ -32,7 +32,8 @@ _MAX_ROWS = 2 ** 31 - 1
 
 class ExpertPlan(NamedTuple):
     """Where tokens go (expert_plan): slots (T, k) int32, the row e * capacity + position of each choice, -1 for one that
-    is dropped; counts (num_experts,) int32, the choices of each expert, dropped ones too."""
+    is dropped; counts (num_experts,) int32, the choices of each expert, dropped ones too. To leave a choice out (a padded
+    token's), give expert_plan -1 for its expert: the counts say which rows are zeros, and have to go with the slots."""
     slots: torch.Tensor
     counts: torch.Tensor
     num_experts: int

@@ -14,7 +14,7 @@ fp32; weights, gradients and momenta each of its own type, so that gradients cli
 
 The steps are taken on the smaller side's Gram matrix in 32 bits. Directions whose singular values are far below the largest
 (1e-4 of it) come out within 4e-4 of the formula, below a 16-bit result's rounding; an fp32 `orthogonalize` is as
-exact as the formula's products in fp32.
+exact as the formula's products in fp32. |u|^2 has to be within fp32's range.
 """
 from __future__ import annotations
 
@@ -75,6 +75,38 @@ def _number(v, name):
 
 def _plain(t: torch.Tensor) -> bool:
     return t.is_contiguous() and not t.is_neg()
+
+
+def _box(t: torch.Tensor):
+    """({stride: size} in bytes, largest first), None where two elements may be in one place"""
+    dims = [(s * t.element_size(), n) for s, n in zip(t.stride(), t.shape) if n > 1] + [(1, t.element_size())]
+    dims.sort(reverse=True)
+    if any(s * n > outer for (outer, _), (s, n) in zip(dims, dims[1:])) or dims[-1][0] == 0:
+        return None
+    return dict(dims)
+
+
+def _refuse_overlap(written):
+    """Raises where two of the tensors may share memory, or two elements of one. A tensor's bytes are numbers whose digits
+    have its strides as bases; two tensors are apart where a digit is, as long as all digits stay within the bases."""
+    ts = sorted((t for t in written if t.numel()), key=lambda t: t.data_ptr())
+    boxes = [_box(t) for t in ts]
+    for i, (t, a) in enumerate(zip(ts, boxes)):
+        end = 0 if a is None else t.data_ptr() + 1 + sum(s * (n - 1) for s, n in a.items())
+        for u, b in zip(ts[i + 1:], boxes[i + 1:]):
+            if a is None or b is None or u.data_ptr() >= end:
+                break
+            rest, outer, apart = u.data_ptr() - t.data_ptr(), math.inf, False
+            for s in sorted({*a, *b}, reverse=True):
+                digit, rest = divmod(rest, s)
+                if max(a.get(s, 1), digit + b.get(s, 1)) * s > outer:
+                    apart = False
+                    break
+                outer, apart = s, apart or digit >= a.get(s, 1)
+            if not apart:
+                a = None
+        if a is None:
+            raise RuntimeError("parameters and momenta must not overlap, nor may one's elements share a place")
 
 
 def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence = _COEFFICIENTS, eps: float = 1e-7,
@@ -169,8 +201,8 @@ def muon_step(params: Union[torch.Tensor, Iterable[torch.Tensor]], grads: Union[
         c.w, c.g, c.m = dense[0].data_ptr(), g.data_ptr(), dense[1].data_ptr()
         c.w_dtype, c.g_dtype, c.m_dtype = _DTYPES[w.dtype], _DTYPES[g.dtype], _DTYPES[m.dtype]
         c.scale = math.sqrt(max(1.0, c.R / c.C if c.C else 1.0)) if scale is None else scale
-    if len({(t.data_ptr(), t.shape, t.stride()) for t, _ in back}) < len(back):  # (dense ones: the library's own check)
-        raise RuntimeError("a tensor is listed twice: parameters and momenta must not overlap")
+    if back:  # (dense ones alone: the library's own check)
+        _refuse_overlap([*params, *momenta])
     L = _lib.lib()
     with _On(dev.index) as stream:
         n = L.fmlp_muon_workspace_bytes(len(params), calls, steps)

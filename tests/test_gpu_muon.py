@@ -269,6 +269,23 @@ def test_refusals_of_overlap():
     muon_step([a, c], [b, b], [t, t.clone()], 0.1)  # (gradients are only read)
 
 
+def test_refusals_of_overlap_in_other_layouts():
+    """nothing is written before the refusal; the parts of a fused weight are taken"""
+    t = torch.ones(2, 8, 9, device="cuda")
+    g, other = torch.ones(2, 9, 8, device="cuda"), torch.ones(2, 9, 8, device="cuda")
+    for w, m in ((t.mT, t.view(2, 9, 8)), (other, other.new_ones(2, 9, 1).expand(2, 9, 8))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            muon_step([w], [g], [m], 0.1)
+        assert (w == 1).all() and (m == 1).all()
+    fused, g, m = (v[0].cuda() for v in stacks([(2, 24, 40)], (FL, FL, FL), 13))
+    parts = [[v[..., :17], v[..., 17:]] for v in (fused, g, m)]
+    alone = [[v.contiguous() for v in p] for p in parts]
+    muon_step(*alone, 0.1)
+    muon_step(*parts, 0.1)
+    for p, a in zip(parts, alone):
+        assert all(torch.equal(u, v) for u, v in zip(p, a))
+
+
 def test_learns_with_the_gated_mlp_stacks():
     """the shapes a module's parameters have, gradients from its backward, clipped into full precision"""
     torch.manual_seed(0)

@@ -5,9 +5,49 @@ import pytest
 import torch
 
 from flashmlp_amd import _lib, muon_step, orthogonalize
+from flashmlp_amd.muon import _refuse_overlap
 from oracle import muon as om
 
 INVALID, UNSUPPORTED, WORKSPACE = 1, 2, 4
+
+
+def places(t):
+    """addresses of all bytes"""
+    at = torch.zeros((), dtype=torch.int64)
+    for stride, n in zip(t.stride(), t.shape):
+        at = at.unsqueeze(-1) + stride * t.element_size() * torch.arange(n)
+    return (at.unsqueeze(-1) + t.data_ptr() + torch.arange(t.element_size())).flatten().tolist()
+
+
+def refused(ts):
+    try:
+        _refuse_overlap(ts)
+    except RuntimeError:
+        return True
+    return False
+
+
+def test_overlap_of_strided_tensors():
+    """what shares memory is refused in any layout, views of one buffer side by side are not"""
+    g = torch.Generator().manual_seed(0)
+    buf = torch.zeros(4096)
+    taken = 0
+    for _ in range(3000):
+        ts = []
+        for _ in range(2):
+            n = [int(v) for v in torch.randint(1, 5, (3,), generator=g)]
+            stride = [int(v) for v in torch.tensor([1, 2, 3, 4, 8, 16, 32, 64])[torch.randint(0, 8, (3,), generator=g)]]
+            ts.append(buf.as_strided(n, stride, int(torch.randint(0, 200, (), generator=g))))
+        p = places(ts[0]) + places(ts[1])
+        if not refused(ts):
+            taken += 1
+            assert len(set(p)) == len(p)
+    assert taken > 100
+    x, y = torch.zeros(3, 8, 12), torch.zeros(3, 8, 12).bfloat16()
+    halves = [x[..., :6], x[..., 6:], y[:, :4], y[:, 4:], y.new_zeros(3, 5, 8).mT, torch.zeros(0, 4, 2).mT]
+    assert not refused(halves) and not refused([x[..., 6:], x[:, 1:, :6]]) and not refused([x[:, :, ::2].mT, x[:, :, 1::2].mT])
+    for bad in ([x.mT, x], [x[..., :6], x[..., 5:]], [x[..., 6:], x[:, 1:, :7]], [x[:, :1].expand(3, 8, 12)], halves + [x[0, :, 3:4]]):
+        assert refused(bad)
 
 
 @pytest.fixture(scope="module")
