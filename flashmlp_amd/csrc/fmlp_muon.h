@@ -77,6 +77,11 @@ struct MuonKind {
 // (NP <= 128)
 template <int NP>
 hipError_t muon_gram(const MuonKind& kind, const MuonTable& tab, unsigned blocks, float* G, int parts, const MuonCall& c, hipStream_t st);
+// NP = 256: the same with `parts` workgroups for each of a matrix's kMuonGramTiles tiles, m' being there already, and m' alone
+constexpr int kMuonGramTiles = 10;
+hipError_t muon_gram_tiles(const MuonKind& kind, const MuonTable& tab, unsigned blocks, float* G, int parts, const MuonCall& c,
+                           hipStream_t st);
+hipError_t muon_momentum(const MuonKind& kind, const MuonTable& tab, unsigned blocks, int parts, const MuonCall& c, hipStream_t st);
 template <int NP>
 hipError_t muon_apply(const MuonKind& kind, const MuonTable& tab, unsigned blocks, const unsigned short* P, const MuonInfo* info,
                       int parts, const MuonCall& c, int update, hipStream_t st);

@@ -131,14 +131,14 @@ constexpr int kTile = NP == 256 ? 32 : 8192 / NP;  // columns of the long side
 // The tile in LDS, 16-bit terms one after the other: WIDE rows of the small side ([NP][KT], units of 16 bytes swapped
 // within a row so that 16 rows' units lie on all banks), TALL rows of the long side ([KT][NP], a pitch that spreads the
 // transposing reads' four rows).
-template <int NP, bool TALL>
+template <int NP, bool TALL, int KT_ = kTile<NP>>
 struct Tile {
-  static constexpr int KT = kTile<NP>;
+  static constexpr int KT = KT_;
   static constexpr int ROWS = TALL ? KT : NP, COLS = TALL ? NP : KT;
   static constexpr int UR = COLS / 8;                                            // units of a row
   static constexpr int PITCH = TALL ? NP * 2 + (NP == 32 ? 0 : 64) : KT * 2;     // bytes
   static constexpr int TERM = ROWS * PITCH;
-  static constexpr int UNITS = ROWS * UR;  // 1024
+  static constexpr int UNITS = ROWS * UR;
   static __device__ __forceinline__ int at(int row, int u) {
     if constexpr (TALL) return row * PITCH + u * 16;
     const int f = UR >= 16 ? row & 15 : UR == 8 ? (row >> 1) & 7 : (row >> 2) & 3;
@@ -225,8 +225,8 @@ struct Part {
   int part;
 };
 template <int NP, bool TALL>
-__device__ __forceinline__ Part part_of(const MuonRef& t, int parts) {
-  const unsigned local = blockIdx.x - t.block0;
+__device__ __forceinline__ Part part_of(const MuonRef& t, int parts, unsigned block) {
+  const unsigned local = block - t.block0;
   Part p;
   p.h = local / (unsigned)parts;
   p.part = (int)(local % (unsigned)parts);
@@ -417,12 +417,150 @@ __global__ void __launch_bounds__(Pairs<NP>::WAVES * 64) gram_kernel(MuonTable t
   Part p;
   const auto run = [&](auto TALL) {
     constexpr bool L = decltype(TALL)::value;
-    p = part_of<NP, L>(t, parts);
+    p = part_of<NP, L>(t, parts, blockIdx.x);
     gram_tiles<NP, L, TERMS, BF, VEC>(acc, t, p, mu, nu, nesterov, wave);
   };
   if (t.R > t.C) run(std::true_type{});
   else run(std::false_type{});
   store_gram<NP>(acc, G + ((size_t)(t.matrix0 + p.h) * parts + p.part) * (NP * NP), NP, wave, lane);
+}
+
+// The same for few matrices of 256: 64 x 64 tiles i <= j of a Gram matrix, `parts` workgroups each, which have a range of the long
+// side by 64. Waves: a 32 x 32 quarter of the tile and half of the long side's 16s; half of them is at its matrix instructions while the
+// other brings the next values into terms. m' is in memory already (momentum_kernel).
+template <bool TALL, int TERMS, bool BF, bool VEC>
+__device__ __forceinline__ void gram_tile(const MuonRef& t, unsigned block, float* __restrict__ G, int parts, float mu, float nu,
+                                          int nesterov) {
+  using T = Tile<64, TALL, 64>;
+  constexpr int KT = T::KT, BLOCK = TERMS * T::TERM;
+  static_assert(T::UNITS == 512, "one for each thread");
+  const unsigned local = block - t.block0;
+  const long long h = local / (unsigned)(kMuonGramTiles * parts);
+  const int part = (int)(local / kMuonGramTiles % (unsigned)parts), tile = (int)(local % kMuonGramTiles);
+  const int bi = tile < 4 ? 0 : tile < 7 ? 1 : tile < 9 ? 2 : 3, bj = tile - (bi * (7 - bi)) / 2;
+  const int R = t.R, C = t.C, small = TALL ? C : R, lane = (int)threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), qr = (wave >> 1) & 1, qc = wave & 1, half = wave >> 2;
+  const long long L = TALL ? R : C, tiles = (L + KT - 1) / KT, per = (tiles + parts - 1) / parts;
+  const long long t0 = part * per, t1 = bj * 64 < small ? min(tiles, t0 + per) : t0;
+  const Mat<VEC> X(t.x, t.x_io, h, R, C), M(t.m, t.m_io, h, R, C);
+  const bool momentum = t.m != nullptr, two = bi != bj, has = two || qr <= qc;
+
+  constexpr int AHEAD = 2;
+  Raw x[AHEAD][2], m[AHEAD][TERMS == 3 ? 2 : 1];
+  const int row = (int)threadIdx.x / T::UR, u = (int)threadIdx.x % T::UR;
+  const auto load = [&](long long k, Raw (&xs)[2], Raw (&ms)[TERMS == 3 ? 2 : 1]) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int s0 = (b ? bj : bi) * 64;
+      const long long r = TALL ? k * KT + row : s0 + row, c = TALL ? s0 + u * 8 : k * KT + u * 8, i = r * C + c;
+      const int n = k < t1 && (!b || two) && r < R ? (int)max(0LL, min(8LL, C - c)) : 0;
+      if constexpr (TERMS == 3) {
+        X.load(i, n, xs[b]);
+        M.load(i, n, ms[b]);
+      } else {
+        xs[b].a = X.load16(i, n);
+      }
+    }
+  };
+  const auto put = [&](int buffer, const Raw (&xs)[2], const Raw (&ms)[TERMS == 3 ? 2 : 1]) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      if (b && !two) continue;
+      const int o = (2 * buffer + b) * BLOCK + T::at(row, u);
+      if constexpr (TERMS == 3) {
+        float f[8];
+        unpack_raw(X.io, xs[b], f);
+        if (momentum) {
+          float v[8];
+          unpack_raw(M.io, ms[b], v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = nesterov ? __builtin_fmaf(mu, v[j], nu * f[j]) : v[j];
+        }
+        u32x4 s[3];
+        split3(f, s);
+#pragma unroll
+        for (int e = 0; e < 3; ++e) lds_write16(e * T::TERM + o, s[e]);
+      } else {
+        lds_write16(o, xs[b].a);
+      }
+    }
+  };
+  f32x16 acc = zero16();
+  const auto multiply = [&](int buffer) {
+    if (!has) return;
+#pragma unroll
+    for (int j = 0; j < KT / 32; ++j) {
+      const int k0 = 16 * (half * (KT / 32) + j);
+      u32x4 a[TERMS], b[TERMS];
+#pragma unroll
+      for (int e = 0; e < TERMS; ++e) {
+        a[e] = T::by_small(2 * buffer * BLOCK + e * T::TERM, qr * 32, k0, lane);
+        b[e] = T::by_small((2 * buffer + (two ? 1 : 0)) * BLOCK + e * T::TERM, qc * 32, k0, lane);
+      }
+      acc = mfma_terms<TERMS, BF>(a, b, acc);
+    }
+  };
+  load(t0, x[0], m[0]);
+  load(t0 + 1, x[1], m[1]);
+  put(0, x[0], m[0]);
+  load(t0 + 2, x[0], m[0]);
+  __syncthreads();
+  for (long long k = t0; k < t1; k += 2) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {  // (past the end: zeros)
+      if (half) multiply(p);
+      put(1 - p, x[1 - p], m[1 - p]);
+      load(k + p + 3, x[1 - p], m[1 - p]);
+      if (!half) multiply(p);
+      __syncthreads();
+    }
+  }
+  float* scr = (float*)fmlp_lds + (wave & 3) * 1024 + lane;
+  if (half)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) scr[i * 64] = acc[i];
+  __syncthreads();
+  if (half || !has) return;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] += scr[i * 64];
+  const int g = lane >> 5, l32 = lane & 31, c = bj * 64 + qc * 32 + l32, r = bi * 64 + qr * 32 + 4 * g;
+  float* dst = G + ((size_t)(t.matrix0 + h) * parts + part) * (256 * 256);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    *(float4*)(dst + c * 256 + r + 8 * q) = float4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+    if (two || qr != qc)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) dst[(r + 8 * q + j) * 256 + c] = acc[4 * q + j];
+  }
+}
+template <int TERMS, bool BF, bool VEC>
+__global__ void __launch_bounds__(512) gram_tile_kernel(MuonTable tab, float* __restrict__ G, int parts, float mu, float nu, int nesterov) {
+  const unsigned block = (unsigned)xcd_remap((int)blockIdx.x, (int)gridDim.x);  // (a matrix on one XCD's L2: each value is read four times)
+  const MuonRef& t = tensor_of(tab, block);
+  if (t.R > t.C) gram_tile<true, TERMS, BF, VEC>(t, block, G, parts, mu, nu, nesterov);
+  else gram_tile<false, TERMS, BF, VEC>(t, block, G, parts, mu, nu, nesterov);
+}
+
+// m' = mu m + nu x, `parts` workgroups a matrix
+template <bool VEC>
+__global__ void __launch_bounds__(256) momentum_kernel(MuonTable tab, int parts, float mu, float nu) {
+  const MuonRef& t = tensor_of(tab, blockIdx.x);
+  const unsigned local = blockIdx.x - t.block0;
+  const Mat<VEC> X(t.x, t.x_io, local / (unsigned)parts, t.R, t.C), M(t.m, t.m_io, local / (unsigned)parts, t.R, t.C);
+  const long long n = (long long)t.R * t.C;
+  for (long long i = ((long long)(local % (unsigned)parts) * 256 + threadIdx.x) * 8; i < n; i += (long long)parts * 2048) {
+    const int there = (int)min(8LL, n - i);
+    Raw x, m;
+    X.load(i, there, x);
+    M.load(i, there, m);
+    float f[8], v[8];
+    unpack_raw(X.io, x, f);
+    unpack_raw(M.io, m, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(mu, v[j], nu * f[j]);
+    pack_raw(M.io, v, m);
+    M.store(i, there, m);
+  }
 }
 
 // O = P u over the data tiles [t0, t1), and what becomes of it. XT: terms of u. Waves: a block of 32 small indices, whose rows of P
@@ -536,11 +674,12 @@ template <int NP, int XT, bool VEC>
 __global__ void __launch_bounds__(NP == 256 ? 512 : 256)
 apply_kernel(MuonTable tab, const u16* __restrict__ P, const MuonInfo* __restrict__ info, int parts, float mu, float nu, int nesterov,
              int update, float keep) {
-  const MuonRef& t = tensor_of(tab, blockIdx.x);
+  const unsigned block = (unsigned)xcd_remap((int)blockIdx.x, (int)gridDim.x);  // (a matrix's P on one XCD's L2)
+  const MuonRef& t = tensor_of(tab, block);
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const auto run = [&](auto TALL) {
     constexpr bool L = decltype(TALL)::value;
-    const Part p = part_of<NP, L>(t, parts);
+    const Part p = part_of<NP, L>(t, parts, block);
     if (p.t0 >= p.t1) return;
     u32x4 ph[NP / 16], pl[NP / 16];
     const u16* src = P + (size_t)(t.matrix0 + p.h) * (2 * NP * NP) + muon_chunk<NP>((wave % (NP / 32)) * 32 + (lane & 31), 0, lane >> 5);
@@ -637,7 +776,7 @@ whole_kernel(MuonTable tab, MuonSteps s, float mu, float nu, int nesterov, int u
   constexpr int RB = NP / 32, GP = NP + 4, SCR = NP * GP * 4;  // LDS: G or the left operand, then the waves' sums
   const MuonRef& t = tensor_of(tab, blockIdx.x);
   const bool tall = t.R > t.C;
-  const Part part = tall ? part_of<NP, true>(t, 1) : part_of<NP, false>(t, 1);
+  const Part part = tall ? part_of<NP, true>(t, 1, blockIdx.x) : part_of<NP, false>(t, 1, blockIdx.x);
   const int lane = (int)threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = wave * 32 + l32;
   float* lds = (float*)fmlp_lds;
@@ -802,6 +941,25 @@ hipError_t muon_whole(const MuonKind& kind, const MuonTable& tab, unsigned block
                        c.nesterov, update, c.keep);
   });
 }
+
+#if FMLP_MUON_PART == 256
+hipError_t muon_gram_tiles(const MuonKind& kind, const MuonTable& tab, unsigned blocks, float* G, int parts, const MuonCall& c,
+                           hipStream_t st) {
+  return by_kind(kind, [&](auto T, auto B, auto V) {
+    constexpr int TERMS = decltype(T)::value;
+    constexpr int lds = 4 * TERMS * std::max(Tile<64, true, 64>::TERM, Tile<64, false, 64>::TERM);
+    static_assert(lds <= 160 * 1024 && lds >= 4 * 4096, "the terms, then half of the sums");
+    static std::atomic<unsigned long long> done{0};
+    return launch<lds>(gram_tile_kernel<TERMS, decltype(B)::value, decltype(V)::value>, done, blocks, 512, st, tab, G, parts, c.mu, c.nu,
+                       c.nesterov);
+  });
+}
+hipError_t muon_momentum(const MuonKind& kind, const MuonTable& tab, unsigned blocks, int parts, const MuonCall& c, hipStream_t st) {
+  if (kind.vec) hipLaunchKernelGGL(momentum_kernel<true>, dim3(blocks), dim3(256), 0, st, tab, parts, c.mu, c.nu);
+  else hipLaunchKernelGGL(momentum_kernel<false>, dim3(blocks), dim3(256), 0, st, tab, parts, c.mu, c.nu);
+  return hipGetLastError();
+}
+#endif
 
 // this part's kernels
 template hipError_t muon_gram<FMLP_MUON_PART>(const MuonKind&, const MuonTable&, unsigned, float*, int, const MuonCall&, hipStream_t);

@@ -305,17 +305,17 @@ __device__ __forceinline__ void finish256(const Prod256& p, const f32x16& acc, l
   }
 }
 
-// 64 x 64 tiles of out, 32 x 32 and half of the inner dimension a wave, whose loads are all in flight at once; blockIdx.y
+// 32 x 64 tiles of out, 32 x 32 and half of the inner dimension a wave, whose loads are all in flight at once; blockIdx.y
 // picks one of two independent products
-__global__ void __launch_bounds__(512) prod256_kernel(Prod256 p0, Prod256 p1, long long matrices) {
-  __shared__ f32x4 half[4][4][64];
+__global__ void __launch_bounds__(256) prod256_kernel(Prod256 p0, Prod256 p1, long long matrices) {
+  __shared__ f32x4 half[2][4][64];
   const Prod256 p = blockIdx.y == 0 ? p0 : p1;
   const int lane = (int)threadIdx.x & 63, g = lane >> 5, l32 = lane & 31, wave = (int)threadIdx.x >> 6;
   long long m;
   int tile;
-  if (!place<16>(matrices, &m, &tile)) return;
-  const int quad = wave & 3, k0 = (wave >> 2) * (N2 / 2);
-  const int r0 = (tile >> 2) * 64 + (quad >> 1) * 32, c0 = (tile & 3) * 64 + (quad & 1) * 32;
+  if (!place<32>(matrices, &m, &tile)) return;
+  const int side = wave & 1, k0 = (wave >> 1) * (N2 / 2);
+  const int r0 = (tile >> 2) * 32, c0 = (tile & 3) * 64 + side * 32;
   const u16* A = p.a + m * kMat + muon_chunk<N2>(r0 + l32, k0 / 16, g);
   const u16* B = p.b + m * kMat + muon_chunk<N2>(c0 + l32, k0 / 16, g);
   constexpr int KS = N2 / 32;
@@ -335,14 +335,14 @@ __global__ void __launch_bounds__(512) prod256_kernel(Prod256 p0, Prod256 p1, lo
     acc = mfma<false>(ah[k], bl[k], acc);
     acc = mfma<false>(ah[k], bh[k], acc);
   }
-  if (wave >= 4)
+  if (wave >= 2)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) half[quad][q][lane] = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+    for (int q = 0; q < 4; ++q) half[side][q][lane] = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
   __syncthreads();
-  if (wave >= 4) return;
+  if (wave >= 2) return;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const f32x4 v = half[quad][q][lane];
+    const f32x4 v = half[side][q][lane];
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[4 * q + j] += v[j];
   }
@@ -406,7 +406,7 @@ hipError_t steps_256(long long matrices, const float* G0, int parts, u16* P, Muo
     if (matrices >= 64)
       hipLaunchKernelGGL(prod256_wide_kernel, dim3(place_blocks<4>(matrices), b ? 2 : 1), dim3(512), 0, st, a, b ? *b : a, matrices);
     else
-      hipLaunchKernelGGL(prod256_kernel, dim3(place_blocks<16>(matrices), b ? 2 : 1), dim3(512), 0, st, a, b ? *b : a, matrices);
+      hipLaunchKernelGGL(prod256_kernel, dim3(place_blocks<32>(matrices), b ? 2 : 1), dim3(256), 0, st, a, b ? *b : a, matrices);
     e = hipGetLastError();
   };
   // P_k, the product of the steps' polynomials so far, takes turns in R and P, the last one in P; the first step's Q is P_0

@@ -24,17 +24,22 @@ MuonKind kind_of(const MuonTensor& t) {
 struct Group {
   int NP;
   long long matrices, tiles;  // tiles: of the longest one
+  bool momentum, raw;  // a matrix has a momentum; all are of 16 bits and have none
   bool whole;  // a workgroup a matrix from end to end: no workspace
+  bool by_tiles;  // of the Gram matrices
   int gram_parts, apply_parts;
   size_t g_off, p_off, info_off, iter_off, end;
 };
 Group group_of(int NP, int n, const MuonTensor* t, int cus) {
   Group r{};
   r.NP = NP;
+  r.raw = true;
   const int KT = NP == 256 ? 32 : 8192 / NP;
   for (int i = 0; i < n; ++i)
     if (t[i].H > 0 && t[i].R > 0 && t[i].C > 0 && padded(t[i]) == NP) {
       r.matrices += t[i].H;
+      r.momentum |= t[i].m != nullptr;
+      r.raw &= kind_of(t[i]).terms == 1;
       r.tiles = std::max(r.tiles, ((long long)std::max(t[i].R, t[i].C) + KT - 1) / KT);
     }
   if (r.matrices == 0) return r;
@@ -50,6 +55,15 @@ Group group_of(int NP, int n, const MuonTensor* t, int cus) {
   const double tile_us = NP == 256 ? 6 : 3, part_us = NP == 256 ? (double)r.matrices * NP * NP * 8 / 4e6 : NP * NP * 4 / 4e4;
   const long long pays = std::max(1LL, std::llround(std::sqrt((double)r.tiles * tile_us / part_us)));
   r.gram_parts = (int)std::max(1LL, std::min(std::min(want, pays), r.tiles));
+  // Few Gram matrices of 256 by tiles: fewer parts and sums to pass on, but every value is brought into terms four times (not so
+  // 16-bit ones, which are their own), and m' takes a launch. Whole and by tiles, 256 x 1024: fp32 orthogonalised, 8 matrices 146 and
+  // 124 us, 16 177 and 174, 32 282 and 298; bf16, 8 104 and 92, 64 281 and 271, 128 498 and 495; the Muon step, 3 109 and
+  // 101, 8 116 and 110, 16 145 and 152
+  if (NP == 256 && r.matrices <= (r.raw ? cus / 2 : r.momentum ? cus / 32 : cus / 20)) {
+    const long long fill = cus / (r.matrices * kMuonGramTiles), blocks = (r.tiles + 1) / 2;  // (64 columns)
+    r.by_tiles = true;
+    r.gram_parts = (int)std::max(1LL, std::min(fill, blocks));
+  }
   r.apply_parts = (int)std::max(1LL, std::min(want, r.tiles));
   const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   r.p_off = up((size_t)r.matrices * r.gram_parts * NP * NP * 4);
@@ -203,7 +217,19 @@ hipError_t launch_muon(int n, const MuonTensor* t, const MuonCall& c, int num_cu
         if (e != hipSuccess) return e;
         continue;
       }
-      e = for_tables(items, gr.gram_parts, false, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
+      e = hipSuccess;
+      if (gr.by_tiles) {
+        // (all have a momentum, or none has)
+        if (items[0].t.m != nullptr)
+          e = for_tables(items, gr.apply_parts, false, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
+            return muon_momentum(k, tab, blocks, gr.apply_parts, c, st);
+          });
+        if (e == hipSuccess)
+          e = for_tables(items, kMuonGramTiles * gr.gram_parts, false, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
+            return muon_gram_tiles(k, tab, blocks, G, gr.gram_parts, c, st);
+          });
+      }
+      else e = for_tables(items, gr.gram_parts, false, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
         return NP == 32    ? muon_gram<32>(k, tab, blocks, G, gr.gram_parts, c, st)
                : NP == 64  ? muon_gram<64>(k, tab, blocks, G, gr.gram_parts, c, st)
                : NP == 128 ? muon_gram<128>(k, tab, blocks, G, gr.gram_parts, c, st)
