@@ -48,13 +48,30 @@ Group group_of(int NP, int n, const MuonTensor* t, int cus) {
   // 256 matrices 81 and 80 us, 384 99 and 108, 512 113 and 135
   r.whole = NP <= 128 && 2 * r.matrices >= (NP == 128 ? 2 : 3) * cus;
   if (r.whole) return r;
-  // three workgroups a CU at least, as far as there are tiles. Of Gram matrices no more than pay: a tile takes about 3 us (6 at
-  // NP = 256), and of a part's sums each matrix's are read by one workgroup of the steps (about 40 KB a us; 16 matrices
-  // of 128 x 1024 in 10 parts 11 us and 18 for the reading) or, at NP = 256, by all (written and read at about 4 TB/s)
-  const long long want = (3LL * cus + r.matrices - 1) / r.matrices;
-  const double tile_us = NP == 256 ? 6 : 3, part_us = NP == 256 ? (double)r.matrices * NP * NP * 8 / 4e6 : NP * NP * 4 / 4e4;
-  const long long pays = std::max(1LL, std::llround(std::sqrt((double)r.tiles * tile_us / part_us)));
-  r.gram_parts = (int)std::max(1LL, std::min(std::min(want, pays), r.tiles));
+  if (NP < 256) {
+    // Three workgroups a CU at least, as far as there are tiles. Of Gram matrices no more than pay: a tile takes about 3 us, and of
+    // a part's sums each matrix's are read by one workgroup of the steps (about 40 KB a us; 16 matrices of 128 x 1024 in 10
+    // parts 11 us and 18 for the reading)
+    const long long want = (3LL * cus + r.matrices - 1) / r.matrices;
+    const long long pays = std::max(1LL, std::llround(std::sqrt((double)r.tiles * 3 / (NP * NP * 4 / 4e4))));
+    r.gram_parts = (int)std::max(1LL, std::min(std::min(want, pays), r.tiles));
+    r.apply_parts = (int)std::max(1LL, std::min(want, r.tiles));
+  } else {
+    // A workgroup a CU at a time, so whole rounds of them: the number with the least of rounds, tiles (5 us) and, for Gram
+    // matrices, the parts' sums (written and read at about 4 TB/s), for results the reading of P. (Three a CU for results and
+    // the square root for Gram matrices, as above: 64 matrices of 256 x 1024 fp32 438 us, Muon step 376; so 375 and 335)
+    const auto best = [&](double fixed_us, double part_us) {
+      long long at = 1;
+      double least = 1e300;
+      for (long long p = 1; p <= std::min(r.tiles, std::max(1LL, 3LL * cus / r.matrices)); ++p) {
+        const double us = (double)((r.matrices * p + cus - 1) / cus) * (fixed_us + 5.0 * ((r.tiles + p - 1) / p)) + part_us * p;
+        if (us < least) least = us, at = p;
+      }
+      return (int)at;
+    };
+    r.gram_parts = best(3, (double)r.matrices * NP * NP * 8 / 4e6);
+    r.apply_parts = best(4, 0);
+  }
   // Few Gram matrices of 256 by tiles: fewer parts and sums to pass on, but every value is brought into terms four times (not so
   // 16-bit ones, which are their own), and m' takes a launch. Whole and by tiles, 256 x 1024: fp32 orthogonalised, 8 matrices 146 and
   // 124 us, 16 177 and 174, 32 282 and 298; bf16, 8 104 and 92, 64 281 and 271, 128 498 and 495; the Muon step, 3 109 and
@@ -64,7 +81,6 @@ Group group_of(int NP, int n, const MuonTensor* t, int cus) {
     r.by_tiles = true;
     r.gram_parts = (int)std::max(1LL, std::min(fill, blocks));
   }
-  r.apply_parts = (int)std::max(1LL, std::min(want, r.tiles));
   const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   r.p_off = up((size_t)r.matrices * r.gram_parts * NP * NP * 4);
   r.info_off = r.p_off + up((size_t)r.matrices * NP * NP * 4);
