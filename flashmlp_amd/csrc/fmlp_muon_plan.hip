@@ -74,8 +74,8 @@ Group group_of(int NP, int n, const MuonTensor* t, int cus) {
   }
   // Few Gram matrices of 256 by tiles: fewer parts and sums to pass on, but every value is brought into terms four times (not so
   // 16-bit ones, which are their own), and m' takes a launch. Whole and by tiles, 256 x 1024: fp32 orthogonalised, 8 matrices 146 and
-  // 124 us, 16 177 and 174, 32 282 and 298; bf16, 8 104 and 92, 64 281 and 271, 128 498 and 495; the Muon step, 3 109 and
-  // 101, 8 116 and 110, 16 145 and 152
+  // 104 us, 16 173 and 171, 32 266 and 277; bf16, 8 104 and 76, 64 260 and 257, 128 477 and 481; the Muon step, 8 116 and
+  // 98, 16 139 and 146
   if (NP == 256 && r.matrices <= (r.raw ? cus / 2 : r.momentum ? cus / 32 : cus / 20)) {
     const long long fill = cus / (r.matrices * kMuonGramTiles), blocks = (r.tiles + 1) / 2;  // (64 columns)
     r.by_tiles = true;
