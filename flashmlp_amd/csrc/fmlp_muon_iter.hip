@@ -11,7 +11,7 @@
 //
 // Measured, a step (four products): 0.7 us at NP = 32, 2.4 at 64, 8.6 at 128 (matrix instructions alone 0.2, 0.7 and 5.4: the
 // rest is the chain of LDS reads, conversions and three barriers, as few matrices leave one workgroup a CU); at 256, whose
-// products are launches, 14.5 for 8 matrices and 125 for 192. 32 columns a wave instead of 16: 64 x 683 24 us instead of 18.
+// products are launches, 15 for 8 matrices and 120 for 192. 32 columns a wave instead of 16: 64 x 683 24 us instead of 18.
 //
 // 32-bit values go through the matrix units as two fp16 terms, hi + lo, of the value times a power of two (22 bits; the
 // host's bounds of the eigenvalues keep them in range), three products with fp32 sums: 3/16 of the time of fp32
@@ -276,37 +276,49 @@ struct Prod256 {
   const u16* b;
   u16* out;
   float back, scale;  // 1 / (the operands' scales), the result's scale
-  float ca, cb, cc, cg;  // where one of the first three is not 0: ca 1 + cb cg A + cc A B
+  float ca, cb, cc, cg;  // with POLY: ca 1 + cb cg A + cc A B
 };
 
-// what becomes of a 32 x 32 tile of a product at row r, column c
-__device__ __forceinline__ void finish256(const Prod256& p, const f32x16& acc, long long m, int r, int c, int g, int l32) {
-  // lane: column c + l32, rows r + 16 h + 4 g + {0..3, 8..11}; stored as that unit of row c + l32 (the matrices are symmetric)
+// A's own values where a lane has a 32 x 32 tile of a product at row r, column c: column c + l32, rows r + 16 h + 4 g + {0..3, 8..11},
+// which are a unit of row c + l32 (the matrices are symmetric); and what becomes of the tile. POLY: ca 1 + cb cg A + cc A B
+struct Own {
+  u32x4 hi[2], lo[2];
+};
+__device__ __forceinline__ void own256(Own& o, const Prod256& p, long long m, int r, int c, int g, int l32) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const size_t at = m * kMat + muon_chunk<N2>(c + l32, r / 16 + h, g);
+    const u16* at = p.a + m * kMat + muon_chunk<N2>(c + l32, r / 16 + h, g);
+    o.hi[h] = *(const u32x4*)at;
+    o.lo[h] = *(const u32x4*)(at + N2 * N2);
+  }
+}
+template <bool POLY>
+__device__ __forceinline__ void finish256(const Prod256& p, const f32x16& acc, const Own& o, long long m, int r, int c, int g, int l32) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
     float f[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = acc[8 * h + j] * p.back;
-    if (p.cc != 0.f || p.ca != 0.f || p.cb != 0.f) {
-      const u32x4 vh = *(const u32x4*)(p.a + at), vl = *(const u32x4*)(p.a + at + N2 * N2);
+    if constexpr (POLY) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float x = j & 1 ? hi_f32<false>(vh[j >> 1]) + hi_f32<false>(vl[j >> 1])
-                              : lo_f32<false>(vh[j >> 1]) + lo_f32<false>(vl[j >> 1]);
+        const float x = j & 1 ? hi_f32<false>(o.hi[h][j >> 1]) + hi_f32<false>(o.lo[h][j >> 1])
+                              : lo_f32<false>(o.hi[h][j >> 1]) + lo_f32<false>(o.lo[h][j >> 1]);
         const int at_r = r + 16 * h + 4 * g + (j & 3) + (j & 4) * 2;
         f[j] = __builtin_fmaf(p.cc, f[j], __builtin_fmaf(p.cb, x * p.cg, at_r == c + l32 ? p.ca : 0.f));
       }
     }
     u32x4 hi, lo;
     split8(f, p.scale, hi, lo);
-    *(u32x4*)(p.out + at) = hi;
-    *(u32x4*)(p.out + at + N2 * N2) = lo;
+    u16* at = p.out + m * kMat + muon_chunk<N2>(c + l32, r / 16 + h, g);
+    *(u32x4*)at = hi;
+    *(u32x4*)(at + N2 * N2) = lo;
   }
 }
 
 // 32 x 64 tiles of out, 32 x 32 and half of the inner dimension a wave, whose loads are all in flight at once; blockIdx.y
 // picks one of two independent products
+template <bool POLY>
 __global__ void __launch_bounds__(256) prod256_kernel(Prod256 p0, Prod256 p1, long long matrices) {
   __shared__ f32x4 half[2][4][64];
   const Prod256 p = blockIdx.y == 0 ? p0 : p1;
@@ -327,6 +339,8 @@ __global__ void __launch_bounds__(256) prod256_kernel(Prod256 p0, Prod256 p1, lo
     bh[k] = *(const u32x4*)(B + 512 * k);
     bl[k] = *(const u32x4*)(B + N2 * N2 + 512 * k);
   }
+  Own own;
+  if (POLY && wave < 2) own256(own, p, m, r0, c0, g, l32);
   __builtin_amdgcn_sched_barrier(0);
   f32x16 acc = zero16();
 #pragma unroll
@@ -346,51 +360,71 @@ __global__ void __launch_bounds__(256) prod256_kernel(Prod256 p0, Prod256 p1, lo
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[4 * q + j] += v[j];
   }
-  finish256(p, acc, m, r0, c0, g, l32);
+  finish256<POLY>(p, acc, own, m, r0, c0, g, l32);
 }
 
-// The same in tiles of 128 x 128, 32 x 64 a wave, which reads half as much for a result: for many matrices, where the CU's path to
-// its L2 is the bound
-__global__ void __launch_bounds__(512) prod256_wide_kernel(Prod256 p0, Prod256 p1, long long matrices) {
+// The same in tiles of 128 x 128, 64 x 64 a wave, for many matrices: the operands go through LDS, each once for a workgroup, and
+// three workgroups a CU hide each other's beginnings and ends. A step has 16 of the inner dimension, 16 runs of 1 KB, four a
+// wave. 0.165 us a matrix, 610 TFLOP/s of 16-bit products (waves that load their own operands: 0.195; two workgroups a CU with a
+// step more ahead: 0.17)
+constexpr int kWideAhead = 3, kWideStep = 16 * 1024;
+template <bool POLY>
+__global__ void __launch_bounds__(256, 3) prod256_wide_kernel(Prod256 p0, Prod256 p1, long long matrices) {
   const Prod256 p = blockIdx.y == 0 ? p0 : p1;
-  const int lane = (int)threadIdx.x & 63, g = lane >> 5, l32 = lane & 31, wave = (int)threadIdx.x >> 6;
+  const int lane = (int)threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   long long m;
   int tile;
   if (!place<4>(matrices, &m, &tile)) return;
-  const int r0 = (tile >> 1) * 128 + (wave & 3) * 32, c0 = (tile & 1) * 128 + (wave >> 2) * 64;
-  const u16* A = p.a + m * kMat + muon_chunk<N2>(r0 + l32, 0, g);
-  const u16* B = p.b + m * kMat + muon_chunk<N2>(c0 + l32, 0, g);
-  constexpr int KS = N2 / 16, AHEAD = 3;
-  constexpr size_t NEXT = (size_t)KS * 512;  // the next 32 rows
-  f32x16 acc[2] = {zero16(), zero16()};
-  u32x4 ring[AHEAD + 1][6];
-  const auto fetch = [&](int k) {
-    u32x4(&v)[6] = ring[k % (AHEAD + 1)];
-    v[0] = *(const u32x4*)(A + 512 * k);
-    v[1] = *(const u32x4*)(A + N2 * N2 + 512 * k);
+  const int tr = tile >> 1, tc = tile & 1, wr = wave & 1, wc = wave >> 1;
+  constexpr int KS = N2 / 16, PF = kWideAhead;
+  // waves 0 and 1 bring the first and second terms of A, the others B's
+  const i32x4 src = make_rsrc_words((wave < 2 ? p.a : p.b) + m * kMat, kMat * 2);
+  const unsigned from = (unsigned)((wave & 1) * (N2 * N2 * 2) + (wave < 2 ? tr : tc) * (4 * KS * 1024) + lane * 16);
+  const auto bring = [&](int k) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      v[2 + 2 * c] = *(const u32x4*)(B + c * NEXT + 512 * k);
-      v[3 + 2 * c] = *(const u32x4*)(B + c * NEXT + N2 * N2 + 512 * k);
-    }
+    for (int j = 0; j < 4; ++j) buf_load16_lds(src, from + (unsigned)((j * KS + k) * 1024), k % PF * kWideStep + (wave * 4 + j) * 1024);
   };
 #pragma unroll
-  for (int k = 0; k < AHEAD; ++k) fetch(k);
+  for (int k = 0; k < PF - 1; ++k) bring(k);
+  f32x16 acc[2][2];
 #pragma unroll
-  for (int k = 0; k < KS; ++k) {
-    if (k + AHEAD < KS) fetch(k + AHEAD);
-    __builtin_amdgcn_sched_barrier(0);
-    const u32x4(&v)[6] = ring[k % (AHEAD + 1)];
+  for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = zero16();
+  Own own[4];
+  static_for<KS>([&](auto step) {
+    constexpr int k = decltype(step)::value;
+    // this wave's runs of step k; A's own values are asked for behind the last runs
+    wait_vmcnt<4 * (KS - 1 - k < PF - 2 ? KS - 1 - k : PF - 2) + (POLY && k + PF > KS ? 16 : 0)>();
+    __builtin_amdgcn_s_waitcnt(0xC07F);                             // lgkmcnt(0): the reads of step k - 1, whose place is taken next
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if constexpr (k + PF - 1 < KS) bring(k + PF - 1);
+    if constexpr (POLY && k + PF == KS) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) acc[c] = mfma<false>(v[1], v[2 + 2 * c], acc[c]);
+      for (int i = 0; i < 4; ++i) own256(own[i], p, m, tr * 128 + wr * 64 + 32 * (i >> 1), tc * 128 + wc * 64 + 32 * (i & 1), g, l32);
+    }
+    const int at = k % PF * kWideStep + lane * 16;
+    u32x4 a[2][2], b[2][2];  // [term][block]
 #pragma unroll
-    for (int c = 0; c < 2; ++c) acc[c] = mfma<false>(v[0], v[3 + 2 * c], acc[c]);
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-    for (int c = 0; c < 2; ++c) acc[c] = mfma<false>(v[0], v[2 + 2 * c], acc[c]);
-    __builtin_amdgcn_sched_barrier(0);
-  }
+      for (int i = 0; i < 2; ++i) {
+        a[e][i] = lds_read16(at + (e * 4 + 2 * wr + i) * 1024);
+        b[e][i] = lds_read16(at + (8 + e * 4 + 2 * wc + i) * 1024);
+      }
 #pragma unroll
-  for (int c = 0; c < 2; ++c) finish256(p, acc[c], m, r0, c0 + 32 * c, g, l32);
+    for (int e = 0; e < 3; ++e)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma<false>(a[e == 0][i], b[e == 1][j], acc[i][j]);
+  });
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      finish256<POLY>(p, acc[i][j], own[2 * i + j], m, tr * 128 + wr * 64 + 32 * i, tc * 128 + wc * 64 + 32 * j, g, l32);
 }
 
 hipError_t steps_256(long long matrices, const float* G0, int parts, u16* P, MuonInfo* info, const MuonSteps& s, void* ws,
@@ -400,31 +434,35 @@ hipError_t steps_256(long long matrices, const float* G0, int parts, u16* P, Muo
   u16 *Q = G + one, *T = Q + one, *R = T + one;
   hipLaunchKernelGGL(sum256_kernel, dim3(place_blocks<16>(matrices)), dim3(256), 0, st, G0, parts, G, info, s, matrices);
   hipError_t e = hipGetLastError();
-  const auto run = [&](const Prod256& a, const Prod256* b) {
+  const auto run = [&](auto POLY, const Prod256& a, const Prod256* b) {
+    constexpr bool poly = decltype(POLY)::value;
     if (e != hipSuccess) return;
-    // (one product of 32 matrices 10.0 us, 9.0 in the smaller tiles; of 192 33 us, 43)
-    if (matrices >= 64)
-      hipLaunchKernelGGL(prod256_wide_kernel, dim3(place_blocks<4>(matrices), b ? 2 : 1), dim3(512), 0, st, a, b ? *b : a, matrices);
+    // (16 matrices 7.4 us, in the smaller tiles 5.8; 32 8.6 and 9.4; 64 13.5 and 17; two products of 16 8.5 and 10.7)
+    if (matrices * (b ? 2 : 1) >= 32)
+      hipLaunchKernelGGL(prod256_wide_kernel<poly>, dim3(place_blocks<4>(matrices), b ? 2 : 1), dim3(256), kWideAhead * kWideStep, st, a,
+                         b ? *b : a, matrices);
     else
-      hipLaunchKernelGGL(prod256_kernel, dim3(place_blocks<32>(matrices), b ? 2 : 1), dim3(256), 0, st, a, b ? *b : a, matrices);
+      hipLaunchKernelGGL(prod256_kernel<poly>, dim3(place_blocks<32>(matrices), b ? 2 : 1), dim3(256), 0, st, a, b ? *b : a, matrices);
     e = hipGetLastError();
   };
+  constexpr std::true_type poly{};
+  constexpr std::false_type plain{};
   // P_k, the product of the steps' polynomials so far, takes turns in R and P, the last one in P; the first step's Q is P_0
   const auto pk = [&](int k) { return (s.steps - 1 - k) % 2 == 0 ? P : R; };
   for (int k = 0; k < s.steps; ++k) {
     const float sg = s.g_scale[k], sq = s.q_scale[k];
     u16* q = k == 0 ? pk(0) : Q;
     const bool last = k + 1 == s.steps;
-    run(Prod256{G, G, q, 1.f / sg / sg, sq, s.a[k], s.b[k], s.c[k], 1.f / sg}, nullptr);
+    run(poly, Prod256{G, G, q, 1.f / sg / sg, sq, s.a[k], s.b[k], s.c[k], 1.f / sg}, nullptr);
     Prod256 next{};
     if (k > 0) next = Prod256{q, pk(k - 1), pk(k), 1.f / sq / s.p_scale[k - 1], s.p_scale[k], 0.f, 0.f, 0.f, 0.f};
     if (last) {
-      if (k > 0) run(next, nullptr);
+      if (k > 0) run(plain, next, nullptr);
       break;
     }
     const float stt = sg * sq * 0x1p-14f;  // G Q has G's bound times Q's
-    run(Prod256{G, q, T, 1.f / sg / sq, stt, 0.f, 0.f, 0.f, 0.f}, k > 0 ? &next : nullptr);
-    run(Prod256{q, T, G, 1.f / sq / stt, s.g_scale[k + 1], 0.f, 0.f, 0.f, 0.f}, nullptr);
+    run(plain, Prod256{G, q, T, 1.f / sg / sq, stt, 0.f, 0.f, 0.f, 0.f}, k > 0 ? &next : nullptr);
+    run(plain, Prod256{q, T, G, 1.f / sq / stt, s.g_scale[k + 1], 0.f, 0.f, 0.f, 0.f}, nullptr);
   }
   return e;
 }
