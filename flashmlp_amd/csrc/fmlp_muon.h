@@ -27,7 +27,8 @@ struct MuonCall {
   float eps;
   int steps;
   float abc[kMuonMaxSteps][3];
-  int stage;  // steps taken on one Gram matrix
+  int stages;                    // of steps taken on one Gram matrix
+  int first[kMuonMaxSteps + 1];  // their first steps, then `steps`
 };
 
 // Bytes of workspace and where things are in it, for the call's tensors.

@@ -15,10 +15,19 @@ using fmlp::abi_ok;
 
 namespace {
 
-// Steps on one Gram matrix. Rounding of it at the smallest eigenvalues grows by a^2 a step, 12 for the usual a = 3.44:
-// after five 16-bit results still hide it (4e-4 at worst, measured on spectra of four decades), after three fp32
-// ones do (1e-6 to 1e-5, as fp32 products of the matrices themselves).
-constexpr int kStage16 = 5, kStage32 = 3;
+// Steps on one Gram matrix. Rounding of it at the smallest eigenvalues grows by a^2 a step, 12 for the usual a = 3.44, until they
+// are of the size of one. Up to five steps 16-bit results still hide it (4e-4 at worst, measured on spectra of four decades).
+// fp32 results of noise around a low rank, where fp32 products of the matrices themselves are 1.0 to 1.8e-6 off: three steps on the
+// first Gram matrix, whose spectrum is the widest, and two on another 2 to 5.6e-6; two, then three, 0.8 to 1.8e-6, but 3 to 7e-6
+// where the sides are alike, whose noise reaches the smallest singular values (2 2 1 1.5 to 2.2e-6): there two, then
+// one each, 0.8 to 1.1e-6.
+void set_stages(fmlp::MuonCall* c, int steps, int dtype, int64_t R, int64_t C) {
+  const bool full = dtype == FMLP_DTYPE_F32, alike = std::max(R, C) < 2 * std::min(R, C);
+  c->steps = steps;
+  c->stages = !full ? (steps + 4) / 5 : alike ? std::max(1, steps - 1) : (steps + 3) / 3;
+  for (int i = 0; i <= c->stages; ++i)  // even ones, the longer ones last
+    c->first[i] = full && alike ? (i == 0 ? 0 : std::min(i + 1, steps)) : steps * i / c->stages;
+}
 
 bool known_dtype(int d) { return d == FMLP_DTYPE_F16 || d == FMLP_DTYPE_BF16 || d == FMLP_DTYPE_F32; }
 int io_type(int d) { return d == FMLP_DTYPE_F32 ? fmlp::IO_F32 : d == FMLP_DTYPE_BF16 ? fmlp::IO_BF16 : fmlp::IO_F16; }
@@ -58,7 +67,6 @@ int set_call(fmlp::MuonCall* c, int steps, const float* coefficients, float eps)
       return abi_fail(FMLP_ERR_INVALID_ARG, "coefficient %d is beyond 1e4 or NaN", i);
     c->abc[i / 3][i % 3] = coefficients[i];
   }
-  c->steps = steps;
   c->eps = eps;
   return FMLP_OK;
 }
@@ -95,8 +103,7 @@ FMLP_EXPORT size_t fmlp_orthogonalize_workspace_bytes(int64_t H, int64_t R, int6
   fmlp::MuonTensor t = stack_of(H, R, C);
   t.x_io = t.out_io = io_type(dtype);
   fmlp::MuonCall c{};
-  c.steps = steps;
-  c.stage = dtype == FMLP_DTYPE_F32 ? kStage32 : kStage16;
+  set_stages(&c, steps, dtype, R, C);
   return fmlp::muon_plan(1, &t, c, cus).ws_bytes;
 }
 
@@ -108,7 +115,7 @@ FMLP_EXPORT int fmlp_orthogonalize(const void* x, void* out, int64_t H, int64_t 
   if (!known_dtype(dtype)) return abi_fail(FMLP_ERR_UNSUPPORTED, "dtype code %d: fp16 (0), bf16 (1) or fp32 (2)", dtype);
   fmlp::MuonCall c{};
   if ((st = set_call(&c, steps, coefficients, eps))) return st;
-  c.stage = dtype == FMLP_DTYPE_F32 ? kStage32 : kStage16;
+  set_stages(&c, steps, dtype, R, C);
   if (H == 0 || R == 0 || C == 0) return abi_ok();
   const size_t es = elem_bytes(dtype), bytes = (size_t)H * (size_t)R * (size_t)C * es;
   if ((st = check_ptr(x, "x", 0, es)) || (st = check_ptr(out, "out", 0, es))) return st;
@@ -174,8 +181,7 @@ FMLP_EXPORT size_t fmlp_muon_workspace_bytes(int n, const fmlp_muon_tensor* tens
   std::vector<fmlp::MuonTensor> t;
   if (check_steps(steps) || take(n, tensors, 0, false, &t, nullptr) || fmlp::abi_num_cus(&cus)) return 0;
   fmlp::MuonCall c{};
-  c.steps = steps;
-  c.stage = kStage16;
+  set_stages(&c, steps, FMLP_DTYPE_BF16, 1, 1);  // (weights take the update at lr)
   c.update = 1;
   for (fmlp::MuonTensor& v : t)
     if (v.m == nullptr) v.m = &c;  // (a momentum whose address is not known yet)
@@ -202,6 +208,6 @@ FMLP_EXPORT int fmlp_muon_step(int n, const fmlp_muon_tensor* tensors, double lr
   c.nesterov = nesterov != 0;
   c.keep = (float)(1.0 - lr * weight_decay);
   c.update = 1;
-  c.stage = kStage16;
+  set_stages(&c, steps, FMLP_DTYPE_BF16, 1, 1);  // (weights take the update at lr)
   return run((int)t.size(), t.data(), c, workspace, workspace_bytes, stream, "muon step");
 }

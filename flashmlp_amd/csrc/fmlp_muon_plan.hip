@@ -166,7 +166,7 @@ hipError_t for_tables(const std::vector<Item>& items, int parts, bool any_type, 
 
 size_t between_bytes(const MuonTensor& t, const MuonCall& c) {
   // matrices between stages are in fp32: in the result where that is what it is
-  if (c.steps <= c.stage || (!c.update && t.out_io == IO_F32)) return 0;
+  if (c.stages <= 1 || (!c.update && t.out_io == IO_F32)) return 0;
   return ((size_t)t.H * t.R * t.C * 4 + 255) / 256 * 256;
 }
 
@@ -195,9 +195,9 @@ hipError_t launch_muon(int n, const MuonTensor* t, const MuonCall& c, int num_cu
     unsigned short* P = (unsigned short*)((char*)ws + gr.p_off);
     MuonInfo* info = (MuonInfo*)((char*)ws + gr.info_off);
     double range = 1;
-    for (int first = 0; first < c.steps; first += c.stage) {
-      const int steps = std::min(c.stage, c.steps - first);
-      const bool start = first == 0, last = first + steps == c.steps;
+    for (int stage = 0; stage < c.stages; ++stage) {
+      const int first = c.first[stage], steps = c.first[stage + 1] - first;
+      const bool start = stage == 0, last = stage + 1 == c.stages;
       const int update = c.update && last;
       MuonSteps s{};
       range = set_steps(&s, c, first, steps, start, range);

@@ -61,6 +61,23 @@ def test_steps(n, steps, dtype):
     check(x, orthogonalize(x.cuda(), steps=steps), steps)
 
 
+@pytest.mark.parametrize("R,C", [(32, 33), (64, 64), (64, 128), (96, 128), (100, 400), (140, 128), (201, 220), (256, 256), (300, 256), (256, 400)])
+def test_full_precision_is_that_of_the_products(R, C):
+    """fp32 results of noise around a low rank, whose singular values reach over two to three decades: at most twice as far off, in norm,
+    as fp32 products of the matrices themselves, which have the same number of roundings of the same size"""
+    g = gen(R + C)
+    x = torch.randn(3, R, 8, generator=g) @ torch.randn(3, 8, C, generator=g) / 8 ** 0.5 + 0.5 * torch.randn(3, R, C, generator=g)
+    want = om.orthogonal64(x)
+    y = x.mT if R > C else x
+    y = y / (torch.linalg.matrix_norm(y, keepdim=True) + 1e-7)
+    for a, b, c in om.triples(om.COEFFICIENTS, 5):
+        t = y @ y.mT
+        y = a * y + (b * t + c * (t @ t)) @ y
+    y = y.mT if R > C else y
+    off = (orthogonalize(x.cuda()).double().cpu() - want).norm()
+    assert off <= 2 * (y.double() - want).norm()
+
+
 def test_coefficients_of_every_step():
     x = torch.randn(3, 60, 200, generator=gen(1))
     c = [(3.4445, -4.775, 2.0315), (2.0, -1.5, 0.5), (1.875, -1.25, 0.375), (1.5, -0.5, 0.0)]
