@@ -385,25 +385,24 @@ __global__ void __launch_bounds__(256, 3) prod256_wide_kernel(Prod256 p0, Prod25
 #pragma unroll
     for (int j = 0; j < 4; ++j) buf_load16_lds(src, from + (unsigned)((j * KS + k) * 1024), k % PF * kWideStep + (wave * 4 + j) * 1024);
   };
+  Own own[4];  // (before the runs, whose waits count what comes behind them)
+  if constexpr (POLY) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) own256(own[i], p, m, tr * 128 + wr * 64 + 32 * (i >> 1), tc * 128 + wc * 64 + 32 * (i & 1), g, l32);
+  }
 #pragma unroll
   for (int k = 0; k < PF - 1; ++k) bring(k);
   f32x16 acc[2][2];
 #pragma unroll
   for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = zero16();
-  Own own[4];
   static_for<KS>([&](auto step) {
     constexpr int k = decltype(step)::value;
-    // this wave's runs of step k; A's own values are asked for behind the last runs
-    wait_vmcnt<4 * (KS - 1 - k < PF - 2 ? KS - 1 - k : PF - 2) + (POLY && k + PF > KS ? 16 : 0)>();
+    wait_vmcnt<4 * (KS - 1 - k < PF - 2 ? KS - 1 - k : PF - 2)>();  // this wave's runs of step k
     __builtin_amdgcn_s_waitcnt(0xC07F);                             // lgkmcnt(0): the reads of step k - 1, whose place is taken next
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     if constexpr (k + PF - 1 < KS) bring(k + PF - 1);
-    if constexpr (POLY && k + PF == KS) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) own256(own[i], p, m, tr * 128 + wr * 64 + 32 * (i >> 1), tc * 128 + wc * 64 + 32 * (i & 1), g, l32);
-    }
     const int at = k % PF * kWideStep + lane * 16;
     u32x4 a[2][2], b[2][2];  // [term][block]
 #pragma unroll
