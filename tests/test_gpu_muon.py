@@ -238,6 +238,20 @@ def test_graph():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H", [1, 12, 13, 31, 32])
+@pytest.mark.parametrize("n,e", [(130, 137), (192, 64 * 5), (256, 2000)])
+def test_few_wide_matrices(H, n, e, dtype):
+    """and a matrix alone in the middle of its memory: what lies around it stays"""
+    x = torch.randn(H, n, e, generator=gen(n + H)).to(dtype)
+    buf = torch.full((H * n * e + 128,), 7.0, dtype=dtype, device="cuda")
+    out = buf[64:-64].view(H, n, e)
+    check(x, orthogonalize(x.cuda(), out=out))
+    assert (buf[:64] == 7).all() and (buf[-64:] == 7).all()
+    t = x.mT.contiguous()
+    check(t, orthogonalize(t.cuda()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("tall", [False, True])
 @pytest.mark.parametrize("n,e", [(7, 300), (32, 20), (50, 129), (64, 128), (100, 65), (128, 200)])
 def test_many_matrices(n, e, tall, dtype):
@@ -264,6 +278,23 @@ def test_muon_step_of_many_matrices(types):
     muon_step(dw, dg, dm, 0.02, weight_decay=0.1)
     for i in range(len(w)):
         want = om.step64(w[i], g[i], m[i], 0.02, weight_decay=0.1)
+        for t, got in (("w", dw[i]), ("m", dm[i])):
+            ref, tol = want[t]
+            tiny = 2.0 ** -25 if got.dtype == HF else 2.0 ** -130
+            assert ((got.double().cpu() - ref).abs() <= 1.01 * tol + tiny).all(), (i, t)
+
+
+@pytest.mark.parametrize("types", [(FL, BF, FL), (HF, FL, BF)])
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("shapes", [[(3, 256, 264), (2, 1000, 133)], [(9, 150, 300)], [(7, 200, 131), (8, 256, 512), (1, 256, 1)], [(30, 129, 200)],
+                                    [(40, 256, 260), (30, 201, 150)]])
+def test_muon_step_of_wide_matrices(shapes, types, nesterov):
+    """small sides above 128: Gram matrices by tiles and by parts, products of few and of many, a small side shorter than a tile's"""
+    w, g, m = stacks(shapes, types, 15)
+    dw, dg, dm = ([t.cuda() for t in v] for v in (w, g, m))
+    muon_step(dw, dg, dm, 0.02, nesterov=nesterov)
+    for i in range(len(w)):
+        want = om.step64(w[i], g[i], m[i], 0.02, nesterov=nesterov)
         for t, got in (("w", dw[i]), ("m", dm[i])):
             ref, tol = want[t]
             tiny = 2.0 ** -25 if got.dtype == HF else 2.0 ** -130
