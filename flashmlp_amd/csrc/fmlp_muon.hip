@@ -411,13 +411,14 @@ __device__ __forceinline__ void store_gram(const f32x16 (&acc)[Pairs<NP>::MP], f
 // Gram matrices: `parts` workgroups a matrix, each a range of the long side, their partial sums whole and symmetric.
 template <int NP, int TERMS, bool BF, bool VEC>
 __global__ void __launch_bounds__(Pairs<NP>::WAVES * 64) gram_kernel(MuonTable tab, float* __restrict__ G, int parts, float mu, float nu, int nesterov) {
-  const MuonRef& t = tensor_of(tab, blockIdx.x);
+  const unsigned block = (unsigned)xcd_remap((int)blockIdx.x, (int)gridDim.x);  // (where the steps read a matrix's sums)
+  const MuonRef& t = tensor_of(tab, block);
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   f32x16 acc[Pairs<NP>::MP];
   Part p;
   const auto run = [&](auto TALL) {
     constexpr bool L = decltype(TALL)::value;
-    p = part_of<NP, L>(t, parts, blockIdx.x);
+    p = part_of<NP, L>(t, parts, block);
     gram_tiles<NP, L, TERMS, BF, VEC>(acc, t, p, mu, nu, nesterov, wave);
   };
   if (t.R > t.C) run(std::true_type{});

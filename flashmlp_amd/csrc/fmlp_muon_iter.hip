@@ -105,7 +105,7 @@ iter_kernel(const float* __restrict__ G0, int parts, u16* __restrict__ P0, MuonI
   constexpr int TN = NP / 16, SCR = NP * NP * 4;  // LDS: the left operand, then the waves' sums
   const int lane = (int)threadIdx.x & 63, q = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = wave * 16 + l16;
-  const long long m = blockIdx.x;
+  const long long m = xcd_remap((int)blockIdx.x, (int)gridDim.x);
 
   f32x4 v[TN];
   const float* src = G0 + m * parts * (NP * NP) + (size_t)n * NP + 4 * q;
@@ -221,7 +221,8 @@ constexpr int N2 = 256, kMat = 2 * N2 * N2;  // fp16 values of a matrix, first t
 template <int TILES>
 __device__ __forceinline__ bool place(long long matrices, long long* m, int* tile) {
   const unsigned b = blockIdx.x >> 3;
-  *m = (long long)(b / TILES) * 8 + (blockIdx.x & 7);
+  const long long each = (matrices + 7) / 8;
+  *m = (blockIdx.x & 7) * each + b / TILES;
   *tile = b % TILES;
   return *m < matrices;
 }
