@@ -49,11 +49,11 @@ Group group_of(int NP, int n, const MuonTensor* t, int cus) {
   r.whole = NP <= 128 && 2 * r.matrices >= (NP == 128 ? 2 : 3) * cus;
   if (r.whole) return r;
   if (NP < 256) {
-    // Three workgroups a CU at least, as far as there are tiles. Of Gram matrices no more than pay: a tile takes about 3 us, and of
-    // a part's sums each matrix's are read by one workgroup of the steps (about 40 KB a us; 16 matrices of 128 x 1024 in 10
-    // parts 11 us and 18 for the reading)
+    // Three workgroups a CU at least, as far as there are tiles. Of Gram matrices no more than pay: a tile takes about 3 us (16-bit
+    // values as they are 1.5), and of a part's sums each matrix's are read by one workgroup of the steps (about 40 KB a us; 16
+    // matrices of 128 x 1024 in 10 parts 11 us and 18 for the reading)
     const long long want = (3LL * cus + r.matrices - 1) / r.matrices;
-    const long long pays = std::max(1LL, std::llround(std::sqrt((double)r.tiles * 3 / (NP * NP * 4 / 4e4))));
+    const long long pays = std::max(1LL, std::llround(std::sqrt((double)r.tiles * (r.raw ? 1.5 : 3) / (NP * NP * 4 / 4e4))));
     r.gram_parts = (int)std::max(1LL, std::min(std::min(want, pays), r.tiles));
     r.apply_parts = (int)std::max(1LL, std::min(want, r.tiles));
   } else {
@@ -81,6 +81,13 @@ Group group_of(int NP, int n, const MuonTensor* t, int cus) {
     r.by_tiles = true;
     r.gram_parts = (int)std::max(1LL, std::min(fill, blocks));
   }
+  // as many as have tiles where each takes as many as the first: 16 tiles in 5 parts are 4, 4, 4, 4 and none
+  const auto even = [](long long tiles, int parts) {
+    const long long each = (tiles + parts - 1) / parts;
+    return (int)((tiles + each - 1) / each);
+  };
+  r.gram_parts = even(r.by_tiles ? (r.tiles + 1) / 2 : r.tiles, r.gram_parts);
+  r.apply_parts = even(r.tiles, r.apply_parts);
   const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   r.p_off = up((size_t)r.matrices * r.gram_parts * NP * NP * 4);
   r.info_off = r.p_off + up((size_t)r.matrices * NP * NP * 4);
