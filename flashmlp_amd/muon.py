@@ -13,7 +13,7 @@ fp32; weights, gradients and momenta each of its own type, so that gradients cli
 (clip_grads) or 16-bit ones go with full precision weights. Calls are asynchronous on torch's current stream.
 
 The steps are taken on the smaller side's Gram matrix in 32 bits. Directions whose singular values are far below the largest
-(1e-4 of it) come out within 4e-4 of the formula, below a 16-bit result's rounding; an fp32 `orthogonalize` is as
+(1e-4 of it) come out within 4e-4 of the formula (measured), below a 16-bit result's rounding; an fp32 `orthogonalize` is as
 exact as the formula's products in fp32. |u|^2 has to be within fp32's range.
 """
 from __future__ import annotations
