@@ -23,6 +23,24 @@ def triples(coefficients, steps):
     return [tuple(coefficients)] * steps if not isinstance(coefficients[0], (tuple, list)) else [tuple(c) for c in coefficients]
 
 
+def polynomials(steps, coefficients):
+    """(largest |q(l)|, largest |(x q(x^2))'|, largest l q(l)^2) of each step, l = x^2 being the eigenvalues that the steps before
+    it leave, [0, 1] at first"""
+    r, out = 1.0, []
+    for a, b, c in triples(coefficients, steps):
+        def among(*inner):
+            return [0.0, r] + [l for l in inner if 0 < l < r]
+
+        q = max(abs(a + l * (b + l * c)) for l in among(*([-b / (2 * c)] if c else [])))
+        slope = max(abs(a + l * (3 * b + l * 5 * c)) for l in among(*([-3 * b / (10 * c)] if c else [])))
+        # (l q^2)' = q (a + 3 b l + 5 c l^2)
+        d = max(9 * b * b - 20 * a * c, 0.0) ** 0.5
+        roots = [(-3 * b + s * d) / (10 * c) for s in (1, -1)] if c else [-a / (3 * b)] if b else []
+        r = max(l * (a + l * (b + l * c)) ** 2 for l in among(*roots))
+        out.append((q, slope, r))
+    return out
+
+
 def orthogonal64(u, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     x = u.double()
     tall = x.shape[-2] > x.shape[-1]
@@ -65,22 +83,31 @@ def bound(u, steps=5, coefficients=COEFFICIENTS, full=False):
     return 2.0 ** -22 * (total + 8) * most
 
 
-def step64(w, g, m, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
-    """dict of (value, bound) of w and m"""
+def step64(w, g, m, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, steps=5, coefficients=COEFFICIENTS, eps=1e-7,
+           kept=None):
+    """dict of (value, bound) of w and m. kept: the momentum that the step has stored, which the update is made of; without it the
+    update's bound allows for every element of it rounded the other way."""
     e = 2.0 ** -24
     wd, gd, md = w.double(), g.double(), m.double()
     m2 = momentum * md + (1 - momentum) * gd
     bm = UNIT[m.dtype] * m2.abs() + 3 * e * (md.abs() + gd.abs())
-    kept = m2.to(torch.float32).to(m.dtype).double()
-    u = (1 - momentum) * gd + momentum * kept if nesterov else kept
+    k = (m2.to(torch.float32).to(m.dtype) if kept is None else kept).double()
+    u = (1 - momentum) * gd + momentum * k if nesterov else k
     R, C = w.shape[-2:]
     s = max(1.0, R / C) ** 0.5 if scale is None else scale
     o = orthogonal64(u, steps, coefficients, eps)
     w2 = (1 - lr * weight_decay) * wd - lr * s * o
-    # the stored momentum's rounding may fall the other way: UNIT of m at single elements, which moves u by as much
+    # what moves u, by its place: the stored momentum's rounding, UNIT of it, or u's own two products and their sum
+    moves = 2 * bm if kept is None else 3 * e * (gd.abs() + k.abs())
     move = 0.0
     if u.numel():
         norm = torch.linalg.matrix_norm(u, keepdim=True).clamp(min=1e-300)
-        move = (2 * bm / norm).amax().item() * 485
+        if kept is None:
+            move = (moves / norm).amax().item() * 485
+        else:  # (no element is above the norm; a step enlarges a change by at most its largest slope at the singular values)
+            grow = 1.0
+            for _, slope, _ in polynomials(steps, coefficients):
+                grow *= slope
+            move = (torch.linalg.matrix_norm(moves, keepdim=True) / norm).amax().item() * grow
     bw = UNIT[w.dtype] * w2.abs() + 4 * e * (wd.abs() + (lr * s * o).abs()) + lr * s * (bound(u, steps, coefficients) + move)
     return {"w": (w2, bw), "m": (m2, bm)}
