@@ -71,6 +71,13 @@ int set_call(fmlp::MuonCall* c, int steps, const float* coefficients, float eps)
   return FMLP_OK;
 }
 
+// (after set_stages)
+int check_bounds(fmlp::MuonCall* c) {
+  const int k = fmlp::muon_bounds(c);
+  if (k < 0) return FMLP_OK;
+  return abi_fail(FMLP_ERR_UNSUPPORTED, "coefficients of step %d: values of singular values up to one may grow beyond 2^16 (squared)", k);
+}
+
 int run(int n, const fmlp::MuonTensor* t, const fmlp::MuonCall& c, void* ws, size_t ws_bytes, void* stream, const char* what) {
   int cus = 0, st;
   if ((st = fmlp::abi_num_cus(&cus))) return st;
@@ -116,6 +123,7 @@ FMLP_EXPORT int fmlp_orthogonalize(const void* x, void* out, int64_t H, int64_t 
   fmlp::MuonCall c{};
   if ((st = set_call(&c, steps, coefficients, eps))) return st;
   set_stages(&c, steps, dtype, R, C);
+  if ((st = check_bounds(&c))) return st;
   if (H == 0 || R == 0 || C == 0) return abi_ok();
   const size_t es = elem_bytes(dtype), bytes = (size_t)H * (size_t)R * (size_t)C * es;
   if ((st = check_ptr(x, "x", 0, es)) || (st = check_ptr(out, "out", 0, es))) return st;
@@ -209,5 +217,6 @@ FMLP_EXPORT int fmlp_muon_step(int n, const fmlp_muon_tensor* tensors, double lr
   c.keep = (float)(1.0 - lr * weight_decay);
   c.update = 1;
   set_stages(&c, steps, FMLP_DTYPE_BF16, 1, 1);  // (weights take the update at lr)
+  if ((st = check_bounds(&c))) return st;
   return run((int)t.size(), t.data(), c, workspace, workspace_bytes, stream, "muon step");
 }

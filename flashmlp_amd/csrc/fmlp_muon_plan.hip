@@ -97,39 +97,27 @@ Group group_of(int NP, int n, const MuonTensor* t, int cus) {
 }
 constexpr int kSizes[4] = {32, 64, 128, 256};
 
-// Powers of two that bring each stage's values to at most 2^14 as fp16: bounds of the eigenvalues of G, Q and P from
-// the steps' polynomials over the range that G's have, which is [0, 1] at first. Returns the range after the steps.
-double set_steps(MuonSteps* s, const MuonCall& c, int first, int steps, bool normalise, double range) {
+// Powers of two that bring a stage's values to at most 2^14 as fp16, a quarter of its range: G's, Q's and P's elements are at most
+// their largest eigenvalues. What is 2^-16 of such a bound still has 22 bits, what is below an error of 2^-39 of it.
+void set_steps(MuonSteps* s, const MuonCall& c, int first, int steps, bool normalise) {
   s->steps = steps;
   s->normalise = normalise;
   s->eps = c.eps;
   double p = 1;
   const auto scale = [](double bound) {
     int e = 0;
-    if (!(bound < 1e30)) bound = 1e30;
-    (void)std::frexp(std::max(bound, 1e-30), &e);
+    (void)std::frexp(std::max(bound, 0x1p-32), &e);  // (products of scales stay within fp32)
     return std::ldexp(1.f, 14 - e);
   };
   for (int k = 0; k < steps; ++k) {
-    const float* v = c.abc[first + k];
-    s->a[k] = v[0];
-    s->b[k] = v[1];
-    s->c[k] = v[2];
-    double q = 0, next = 0;
-    const int N = 512;
-    for (int i = 0; i <= N; ++i) {
-      const double l = range * 1.02 * i / N, y = v[0] + l * (v[1] + l * v[2]);
-      q = std::max(q, std::fabs(y));
-      next = std::max(next, l * y * y);
-    }
-    q *= 1.02;
-    p *= q;
-    s->g_scale[k] = scale(range * 1.02);
-    s->q_scale[k] = scale(q);
+    s->a[k] = c.abc[first + k][0];
+    s->b[k] = c.abc[first + k][1];
+    s->c[k] = c.abc[first + k][2];
+    p *= c.q[first + k];
+    s->g_scale[k] = scale(c.range[first + k]);
+    s->q_scale[k] = scale(c.q[first + k]);
     s->p_scale[k] = scale(p);
-    range = next * 1.02;
   }
-  return range;
 }
 
 bool empty(const MuonTensor& t) { return t.H == 0 || t.R == 0 || t.C == 0; }
@@ -179,6 +167,42 @@ size_t between_bytes(const MuonTensor& t, const MuonCall& c) {
 
 }  // namespace
 
+// The eigenvalues of the first G are in [0, 1], those after a step in [0, r'], r' the largest l q(l)^2 on [0, r]: at an end or
+// where its derivative q (a + 3 b l + 5 c l^2) vanishes. (Taken where they are: with two hundredths more a step, a schedule whose
+// polynomials grow fast behind r had bounds of 1e11 after four steps, and its values vanished below them.)
+int muon_bounds(MuonCall* c) {
+  double r = 1, p = 1;
+  int stage = 0, over = -1;
+  c->range[0] = r;
+  for (int k = 0; k < c->steps; ++k) {
+    const double a = c->abc[k][0], b = c->abc[k][1], d = c->abc[k][2];
+    const auto q = [&](double l) { return a + l * (b + l * d); };
+    double most = std::max(std::fabs(q(0)), std::fabs(q(r))), next = r * q(r) * q(r);
+    const auto at = [&](double l) {
+      if (!(l > 0 && l < r)) return;
+      most = std::max(most, std::fabs(q(l)));
+      next = std::max(next, l * q(l) * q(l));
+    };
+    if (d != 0) {
+      const double root = std::sqrt(std::max(9 * b * b - 20 * a * d, 0.0));
+      at(-b / (2 * d));
+      at((-3 * b + root) / (10 * d));
+      at((-3 * b - root) / (10 * d));
+    } else if (b != 0) {
+      at(-a / (3 * b));
+    }
+    if (stage + 1 <= c->stages && k == c->first[stage]) {
+      p = 1;
+      ++stage;
+    }
+    p *= most;
+    c->q[k] = most;
+    c->range[k + 1] = r = next;
+    if (over < 0 && (!(p <= kMuonMaxBound) || (k + 1 < c->steps && !(r <= kMuonMaxBound)))) over = k;
+  }
+  return over;
+}
+
 MuonPlan muon_plan(int n, const MuonTensor* t, const MuonCall& c, int num_cus) {
   MuonPlan p{};
   for (int NP : kSizes) {
@@ -201,13 +225,12 @@ hipError_t launch_muon(int n, const MuonTensor* t, const MuonCall& c, int num_cu
     float* G = (float*)ws;
     unsigned short* P = (unsigned short*)((char*)ws + gr.p_off);
     MuonInfo* info = (MuonInfo*)((char*)ws + gr.info_off);
-    double range = 1;
     for (int stage = 0; stage < c.stages; ++stage) {
       const int first = c.first[stage], steps = c.first[stage + 1] - first;
       const bool start = stage == 0, last = stage + 1 == c.stages;
       const int update = c.update && last;
       MuonSteps s{};
-      range = set_steps(&s, c, first, steps, start, range);
+      set_steps(&s, c, first, steps, start);
       std::vector<Item> items;
       long long matrix = 0;
       char* between = (char*)ws + shared;

@@ -401,7 +401,9 @@ int fmlp_expert_gather(const void* rows, const float* weights, const int32_t* sl
  * Orthogonalised matrices by Newton-Schulz products, and the optimizer's step around them (Muon). No counterpart in the
  * reference. For a matrix u, R x C, with n = min(R, C) <= 256:
  *   X = u / (|u| + eps), |u| its Frobenius norm;  for each of `steps` (1 to 10) steps  X <- a X + b (X X^T) X + c (X X^T)^2 X
- * coefficients: a, b, c of every step, 3 * steps numbers that are read on the host. The steps are taken on the n x n Gram matrix in
+ * coefficients: a, b, c of every step, 3 * steps numbers that are read on the host, under which no singular value up to one
+ * may become one above 2^8 before the last step, nor all steps on one Gram matrix enlarge one 2^16 times
+ * (FMLP_ERR_UNSUPPORTED). Values are held to 2^-39 of the most that they may be. The steps are taken on the n x n Gram matrix in
  * 32 bits. Singular values far below the largest come out with an absolute error (of an orthogonal result, relative to 1)
  * of up to 4e-4 after five steps (measured on spectra of four decades) where the result has 16 bits or goes into weights; an
  * fp32 result of fmlp_orthogonalize takes the Gram matrix anew after two steps, then after three, or after every one where

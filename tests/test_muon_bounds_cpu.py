@@ -1,10 +1,12 @@
 """What the bounds of a Muon step (oracle/muon.py) can tell apart, with the momenta as they are stored: a step that leaves the
 weights, the other rule of momentum, a step fewer, the other sign, for every mix of types."""
+import ctypes
 import itertools
 
 import pytest
 import torch
 
+from flashmlp_amd import _lib
 from oracle import muon as om
 
 BF, HF, FL = torch.bfloat16, torch.float16, torch.float32
@@ -46,3 +48,21 @@ def test_largest_values_of_the_steps():
             r = min(after, 100.0)
             if after > 100:
                 break
+
+
+@pytest.mark.parametrize("coefficients,steps,step", [((4.0, -4.0, 1.5), 5, 2), ((0.0, 0.0, 300.0), 2, 0), ((50.0, 0.0, 0.0), 3, 1),
+                                                     ((1e4, 1e4, 1e4), 2, 0), ((3e4, 0.0, 0.0), 1, None)])
+def test_refusal_of_coefficients(coefficients, steps, step):
+    """whose values the steps' terms would not hold (300^2, 50^4 and 3e8 are above 2^16); on the host, as calls for no matrices show.
+    step None: beyond the limit of a coefficient"""
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("libflashmlp.so not built (python -m flashmlp_amd.build)")
+    L = _lib.lib()
+    abc = (ctypes.c_float * (3 * steps))(*coefficients * steps)
+    for dtype in (0, 1, 2):
+        assert L.fmlp_orthogonalize(None, None, 0, 8, 9, dtype, steps, abc, 1e-7, None, 0, None) != 0
+        assert "coefficient" in L.fmlp_last_error().decode()
+    t = (_lib.MuonTensor * 1)(_lib.MuonTensor(4096, 1 << 20, 2 << 20, 2, 8, 9, 2, 2, 2, 1.0))
+    assert L.fmlp_muon_step(1, t, 0.1, 0.9, 1, 0.0, steps, abc, 1e-7, None, 0, None) != 0
+    message = L.fmlp_last_error().decode()
+    assert "coefficient" in message and (step is None or f"step {step}" in message)
