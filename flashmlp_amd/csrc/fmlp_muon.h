@@ -32,10 +32,8 @@ struct MuonCall {
   // largest eigenvalue of G before each step and after the last one, largest |q| of each step (muon_bounds)
   double range[kMuonMaxSteps + 1], q[kMuonMaxSteps];
 };
-// Sets range and q from the steps' polynomials. The first step (0 on) that leaves an eigenvalue, or whose product of polynomials
-// within its stage has a value, above kMuonMaxBound; -1 if none does.
-constexpr double kMuonMaxBound = 65536;
-int muon_bounds(MuonCall* c);
+// Sets range and q from the steps' polynomials.
+void muon_bounds(MuonCall* c);
 
 // Bytes of workspace and where things are in it, for the call's tensors.
 struct MuonPlan {

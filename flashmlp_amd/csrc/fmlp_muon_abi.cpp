@@ -15,18 +15,24 @@ using fmlp::abi_ok;
 
 namespace {
 
-// Steps on one Gram matrix. Rounding of it at the smallest eigenvalues grows by a^2 a step, 12 for the usual a = 3.44, until they
-// are of the size of one. Up to five steps 16-bit results still hide it (4e-4 at worst, measured on spectra of four decades).
-// fp32 results of noise around a low rank, where fp32 products of the matrices themselves are 1.0 to 1.8e-6 off: three steps on the
-// first Gram matrix, whose spectrum is the widest, and two on another 2 to 5.6e-6; two, then three, 0.8 to 1.8e-6, but 3 to 7e-6
-// where the sides are alike, whose noise reaches the smallest singular values (2 2 1 1.5 to 2.2e-6): there two, then
-// one each, 0.8 to 1.1e-6.
-void set_stages(fmlp::MuonCall* c, int steps, int dtype, int64_t R, int64_t C) {
-  const bool full = dtype == FMLP_DTYPE_F32, alike = std::max(R, C) < 2 * std::min(R, C);
-  c->steps = steps;
-  c->stages = !full ? (steps + 4) / 5 : alike ? std::max(1, steps - 1) : (steps + 3) / 3;
-  for (int i = 0; i <= c->stages; ++i)  // even ones, the longer ones last
-    c->first[i] = full && alike ? (i == 0 ? 0 : std::min(i + 1, steps)) : steps * i / c->stages;
+// Steps on one Gram matrix. Rounding of it at the smallest eigenvalues grows by q(0)^2 = a^2 a step, 12 for the usual a = 3.44, until
+// they are of the size of one. Up to five steps 16-bit results still hide it (4e-4 at worst, measured on spectra of four decades).
+// An fp32 result has two steps on the first Gram matrix, where the first of them grows little enough (a up to 4), and from there on
+// a Gram matrix for each step. Off from 64 bits in norm, that and fp32 products of the matrices themselves (64 x 64 to 256 x 1024):
+// noise around a low rank 0.7 to 1.3e-6 and 1.0 to 2.5e-6, singular values that fall evenly over two to five decades 1.0 to 5.7e-6
+// and 1.0 to 5.9e-6 (two steps, then three: 8 to 36e-6 emulated, 2 2 1: 3.5 to 10e-6), a schedule that begins with a = 8.3
+// 2.3 to 19e-6 and 2.2 to 16e-6 (there with two steps first up to seven times the products).
+void set_stages(fmlp::MuonCall* c, int dtype) {
+  const int steps = c->steps;
+  if (dtype == FMLP_DTYPE_F32) {
+    const bool two = steps > 1 && c->q[0] * c->q[0] <= 16;
+    c->stages = steps - two;
+    c->first[0] = 0;
+    for (int i = 1; i <= c->stages; ++i) c->first[i] = i + two;
+    return;
+  }
+  c->stages = (steps + 4) / 5;
+  for (int i = 0; i <= c->stages; ++i) c->first[i] = steps * i / c->stages;  // even ones, the longer ones last
 }
 
 bool known_dtype(int d) { return d == FMLP_DTYPE_F16 || d == FMLP_DTYPE_BF16 || d == FMLP_DTYPE_F32; }
@@ -57,7 +63,7 @@ int check_steps(int steps) {
     return abi_fail(FMLP_ERR_UNSUPPORTED, "%d steps: 1 to %d", steps, fmlp::kMuonMaxSteps);
   return FMLP_OK;
 }
-int set_call(fmlp::MuonCall* c, int steps, const float* coefficients, float eps) {
+int set_call(fmlp::MuonCall* c, int steps, const float* coefficients, float eps, int dtype) {
   int st = check_steps(steps);
   if (st) return st;
   if (coefficients == nullptr) return abi_fail(FMLP_ERR_INVALID_ARG, "coefficients is NULL");
@@ -68,14 +74,18 @@ int set_call(fmlp::MuonCall* c, int steps, const float* coefficients, float eps)
     c->abc[i / 3][i % 3] = coefficients[i];
   }
   c->eps = eps;
+  c->steps = steps;
+  fmlp::muon_bounds(c);
+  set_stages(c, dtype);
+  // what the terms of the steps hold: G's eigenvalues, and those of each stage's product of polynomials
+  constexpr double most = 65536;
+  for (int i = 0; i < c->stages; ++i) {
+    double p = 1;
+    for (int k = c->first[i]; k < c->first[i + 1]; ++k)
+      if (!((p *= c->q[k]) <= most) || (k + 1 < steps && !(c->range[k + 1] <= most)))
+        return abi_fail(FMLP_ERR_UNSUPPORTED, "coefficients of step %d: singular values up to one may grow too far (above 2^8, or 2^16 times)", k);
+  }
   return FMLP_OK;
-}
-
-// (after set_stages)
-int check_bounds(fmlp::MuonCall* c) {
-  const int k = fmlp::muon_bounds(c);
-  if (k < 0) return FMLP_OK;
-  return abi_fail(FMLP_ERR_UNSUPPORTED, "coefficients of step %d: values of singular values up to one may grow beyond 2^16 (squared)", k);
 }
 
 int run(int n, const fmlp::MuonTensor* t, const fmlp::MuonCall& c, void* ws, size_t ws_bytes, void* stream, const char* what) {
@@ -110,7 +120,8 @@ FMLP_EXPORT size_t fmlp_orthogonalize_workspace_bytes(int64_t H, int64_t R, int6
   fmlp::MuonTensor t = stack_of(H, R, C);
   t.x_io = t.out_io = io_type(dtype);
   fmlp::MuonCall c{};
-  set_stages(&c, steps, dtype, R, C);
+  c.steps = steps;
+  set_stages(&c, dtype);
   return fmlp::muon_plan(1, &t, c, cus).ws_bytes;
 }
 
@@ -121,9 +132,7 @@ FMLP_EXPORT int fmlp_orthogonalize(const void* x, void* out, int64_t H, int64_t 
   if (st) return st;
   if (!known_dtype(dtype)) return abi_fail(FMLP_ERR_UNSUPPORTED, "dtype code %d: fp16 (0), bf16 (1) or fp32 (2)", dtype);
   fmlp::MuonCall c{};
-  if ((st = set_call(&c, steps, coefficients, eps))) return st;
-  set_stages(&c, steps, dtype, R, C);
-  if ((st = check_bounds(&c))) return st;
+  if ((st = set_call(&c, steps, coefficients, eps, dtype))) return st;
   if (H == 0 || R == 0 || C == 0) return abi_ok();
   const size_t es = elem_bytes(dtype), bytes = (size_t)H * (size_t)R * (size_t)C * es;
   if ((st = check_ptr(x, "x", 0, es)) || (st = check_ptr(out, "out", 0, es))) return st;
@@ -189,7 +198,8 @@ FMLP_EXPORT size_t fmlp_muon_workspace_bytes(int n, const fmlp_muon_tensor* tens
   std::vector<fmlp::MuonTensor> t;
   if (check_steps(steps) || take(n, tensors, 0, false, &t, nullptr) || fmlp::abi_num_cus(&cus)) return 0;
   fmlp::MuonCall c{};
-  set_stages(&c, steps, FMLP_DTYPE_BF16, 1, 1);  // (weights take the update at lr)
+  c.steps = steps;
+  set_stages(&c, FMLP_DTYPE_BF16);  // (weights take the update at lr)
   c.update = 1;
   for (fmlp::MuonTensor& v : t)
     if (v.m == nullptr) v.m = &c;  // (a momentum whose address is not known yet)
@@ -200,7 +210,7 @@ FMLP_EXPORT int fmlp_muon_step(int n, const fmlp_muon_tensor* tensors, double lr
                                double weight_decay, int steps, const float* coefficients, float eps, void* workspace,
                                size_t workspace_bytes, void* stream) {
   fmlp::MuonCall c{};
-  int st = set_call(&c, steps, coefficients, eps);
+  int st = set_call(&c, steps, coefficients, eps, FMLP_DTYPE_BF16);  // (weights take the update at lr)
   if (st) return st;
   if (!(lr >= 0) || !(weight_decay >= 0) || !(momentum >= 0 && momentum <= 1))
     return abi_fail(FMLP_ERR_INVALID_ARG, "lr or weight_decay is negative or NaN, or momentum outside [0, 1]");
@@ -216,7 +226,5 @@ FMLP_EXPORT int fmlp_muon_step(int n, const fmlp_muon_tensor* tensors, double lr
   c.nesterov = nesterov != 0;
   c.keep = (float)(1.0 - lr * weight_decay);
   c.update = 1;
-  set_stages(&c, steps, FMLP_DTYPE_BF16, 1, 1);  // (weights take the update at lr)
-  if ((st = check_bounds(&c))) return st;
   return run((int)t.size(), t.data(), c, workspace, workspace_bytes, stream, "muon step");
 }

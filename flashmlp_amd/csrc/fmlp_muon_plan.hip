@@ -170,9 +170,8 @@ size_t between_bytes(const MuonTensor& t, const MuonCall& c) {
 // The eigenvalues of the first G are in [0, 1], those after a step in [0, r'], r' the largest l q(l)^2 on [0, r]: at an end or
 // where its derivative q (a + 3 b l + 5 c l^2) vanishes. (Taken where they are: with two hundredths more a step, a schedule whose
 // polynomials grow fast behind r had bounds of 1e11 after four steps, and its values vanished below them.)
-int muon_bounds(MuonCall* c) {
-  double r = 1, p = 1;
-  int stage = 0, over = -1;
+void muon_bounds(MuonCall* c) {
+  double r = 1;
   c->range[0] = r;
   for (int k = 0; k < c->steps; ++k) {
     const double a = c->abc[k][0], b = c->abc[k][1], d = c->abc[k][2];
@@ -191,16 +190,9 @@ int muon_bounds(MuonCall* c) {
     } else if (b != 0) {
       at(-a / (3 * b));
     }
-    if (stage + 1 <= c->stages && k == c->first[stage]) {
-      p = 1;
-      ++stage;
-    }
-    p *= most;
     c->q[k] = most;
     c->range[k + 1] = r = next;
-    if (over < 0 && (!(p <= kMuonMaxBound) || (k + 1 < c->steps && !(r <= kMuonMaxBound)))) over = k;
   }
-  return over;
 }
 
 MuonPlan muon_plan(int n, const MuonTensor* t, const MuonCall& c, int num_cus) {

@@ -5,10 +5,8 @@
 The kernels take the steps on the Gram matrix G in values of 22 bits and 32-bit sums. An error e of G at an eigenvalue l near 0 grows by
 a^2 a step as l itself does, until l is of the size of one: by at most min(a^(2 (s - 1)), 1 / l) over the s steps that one Gram matrix
 serves, and changes the polynomial's value there by b / a of it. Rounding gives e = 2^-22 of G's norm, which is at most 1: so a singular
-value near one is off by 1.4 2^-22 min(...), and no element by more. A Gram matrix serves up to five steps where the
-result has 16 bits; where it has 32, the first up to two and later ones three, or one where one side is less than twice the
-other (`stages`); in between, the matrices themselves are rounded to 2^-24, twice (the products and their factor), which what
-follows multiplies by a a step.
+value near one is off by 1.4 2^-22 min(...), and no element by more. Which steps share a Gram matrix: `stages`; in between, the
+matrices themselves are rounded to 2^-24, twice (the products and their factor), which what follows multiplies by a a step.
 """
 from __future__ import annotations
 
@@ -52,11 +50,14 @@ def orthogonal64(u, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     return x.mT if tall else x
 
 
-def stages(steps, full, small, long):
-    """first steps of the Gram matrices, and the number of steps"""
-    if full and long < 2 * small:
-        return [0] + [min(i + 1, steps) for i in range(1, max(1, steps - 1) + 1)]
-    n = (steps + 3) // 3 if full else (steps + 4) // 5
+def stages(steps, full, coefficients=COEFFICIENTS):
+    """first steps of the Gram matrices, and the number of steps: for fp32 results two (one where the first grows an eigenvalue near 0
+    more than 16 times), then one each; for others up to five each"""
+    grow = [q * q for q, _, _ in polynomials(steps, coefficients)]
+    if full:
+        two = steps > 1 and grow[0] <= 16
+        return [0, *range(1 + two, steps + 1)]
+    n = (steps + 4) // 5
     return [steps * i // n for i in range(n + 1)]
 
 
@@ -69,7 +70,7 @@ def bound(u, steps=5, coefficients=COEFFICIENTS, full=False):
     least = (s.reshape(-1, s.shape[-1])[:, -1].min() ** 2).item()  # the smallest eigenvalue of a G
     most = 1.0
     a = [abs(c[0]) for c in triples(coefficients, steps)]
-    total, at = 0.0, stages(steps, full, *sorted(u.shape[-2:]))
+    total, at = 0.0, stages(steps, full, coefficients)
     for first, end in zip(at, at[1:]):
         grow = 1.0
         for v in a[first:end - 1]:
