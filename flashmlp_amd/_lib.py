@@ -101,9 +101,11 @@ SIGNATURES = {
     "fmlp_expert_scatter": (ctypes.c_int, [_vp, _i64] + [_vp] * 6 + [_i64] * 5 + [ctypes.c_int, _vp]),
     "fmlp_expert_gather": (ctypes.c_int, [_vp] * 4 + [_i64] * 5 + [ctypes.c_int, _vp]),
     "fmlp_orthogonalize_workspace_bytes": (ctypes.c_size_t, [_i64] * 3 + [ctypes.c_int, ctypes.c_int]),
+    "fmlp_orthogonalize_workspace_bytes_for": (ctypes.c_size_t, [_i64] * 3 + [ctypes.c_int, ctypes.c_int, _f32p]),
     "fmlp_orthogonalize": (ctypes.c_int, [_vp, _vp] + [_i64] * 3 + [ctypes.c_int, ctypes.c_int, _f32p, ctypes.c_float, _vp,
                                                                     ctypes.c_size_t, _vp]),
     "fmlp_muon_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.POINTER(MuonTensor), ctypes.c_int]),
+    "fmlp_muon_workspace_bytes_for": (ctypes.c_size_t, [ctypes.c_int, ctypes.POINTER(MuonTensor), ctypes.c_int, _f32p]),
     "fmlp_muon_step": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(MuonTensor), ctypes.c_double, ctypes.c_double,
                                       ctypes.c_int, ctypes.c_double, ctypes.c_int, _f32p, ctypes.c_float, _vp,
                                       ctypes.c_size_t, _vp]),

@@ -16,7 +16,10 @@ using fmlp::abi_ok;
 namespace {
 
 // Steps on one Gram matrix. Rounding of it at the smallest eigenvalues grows by q(0)^2 = a^2 a step, 12 for the usual a = 3.44, until
-// they are of the size of one. Up to five steps 16-bit results still hide it (4e-4 at worst, measured on spectra of four decades).
+// they are of the size of one. 16-bit results hide a growth of 2e4 before the stage's last step: five usual steps, whose results are
+// off by 4e-6 to 4e-4 in norm and up to 1.4e-3 at a singular value (64 x 64 to 256 x 1024, noise around a low rank and spectra
+// of one to five decades; a bf16 result's rounding is 1.7e-3, at a singular value 1.6 to 3e-3). Five steps of a schedule that
+// begins with a = 8.3, 2e5, were off by up to 2.4e-3 and 1.5e-2; in three and two 4e-5 and 3e-4.
 // An fp32 result has two steps on the first Gram matrix, where the first of them grows little enough (a up to 4), and from there on
 // a Gram matrix for each step. Off from 64 bits in norm, that and fp32 products of the matrices themselves (64 x 64 to 256 x 1024):
 // noise around a low rank 0.7 to 1.3e-6 and 1.0 to 2.5e-6, singular values that fall evenly over two to five decades 1.0 to 5.7e-6
@@ -31,8 +34,18 @@ void set_stages(fmlp::MuonCall* c, int dtype) {
     for (int i = 1; i <= c->stages; ++i) c->first[i] = i + two;
     return;
   }
-  c->stages = (steps + 4) / 5;
-  for (int i = 0; i <= c->stages; ++i) c->first[i] = steps * i / c->stages;  // even ones, the longer ones last
+  // as few even ones as are of five steps at most and grow no further
+  for (c->stages = (steps + 4) / 5; c->stages <= steps; ++c->stages) {
+    const int n = c->stages;
+    bool fits = true;
+    for (int i = 0; i <= n; ++i) c->first[i] = (steps * i + n - 1) / n;
+    for (int i = 0; i < n; ++i) {
+      double grow = 1;
+      for (int k = c->first[i]; k + 1 < c->first[i + 1]; ++k) grow *= c->q[k] * c->q[k];
+      fits = fits && grow <= 2e4;
+    }
+    if (fits) break;
+  }
 }
 
 bool known_dtype(int d) { return d == FMLP_DTYPE_F16 || d == FMLP_DTYPE_BF16 || d == FMLP_DTYPE_F32; }
@@ -88,6 +101,16 @@ int set_call(fmlp::MuonCall* c, int steps, const float* coefficients, float eps,
   return FMLP_OK;
 }
 
+// the stages of a workspace's query; without coefficients those that take the most, which is any number above one
+int query_call(fmlp::MuonCall* c, int steps, const float* coefficients, int dtype) {
+  if (coefficients != nullptr) return set_call(c, steps, coefficients, 0.f, dtype);
+  const int st = check_steps(steps);
+  c->stages = c->steps = steps;
+  return st;
+}
+// weights take the update at lr: as exact as a 16-bit result
+constexpr int kUpdate = FMLP_DTYPE_BF16;
+
 int run(int n, const fmlp::MuonTensor* t, const fmlp::MuonCall& c, void* ws, size_t ws_bytes, void* stream, const char* what) {
   int cus = 0, st;
   if ((st = fmlp::abi_num_cus(&cus))) return st;
@@ -114,15 +137,18 @@ fmlp::MuonTensor stack_of(int64_t H, int64_t R, int64_t C) {
 
 }  // namespace
 
-FMLP_EXPORT size_t fmlp_orthogonalize_workspace_bytes(int64_t H, int64_t R, int64_t C, int dtype, int steps) {
+FMLP_EXPORT size_t fmlp_orthogonalize_workspace_bytes_for(int64_t H, int64_t R, int64_t C, int dtype, int steps,
+                                                          const float* coefficients) {
   int cus = 0;
-  if (check_stack(H, R, C, 0) || !known_dtype(dtype) || check_steps(steps) || fmlp::abi_num_cus(&cus)) return 0;
+  fmlp::MuonCall c{};
+  if (check_stack(H, R, C, 0) || !known_dtype(dtype) || query_call(&c, steps, coefficients, dtype) || fmlp::abi_num_cus(&cus)) return 0;
   fmlp::MuonTensor t = stack_of(H, R, C);
   t.x_io = t.out_io = io_type(dtype);
-  fmlp::MuonCall c{};
-  c.steps = steps;
-  set_stages(&c, dtype);
   return fmlp::muon_plan(1, &t, c, cus).ws_bytes;
+}
+
+FMLP_EXPORT size_t fmlp_orthogonalize_workspace_bytes(int64_t H, int64_t R, int64_t C, int dtype, int steps) {
+  return fmlp_orthogonalize_workspace_bytes_for(H, R, C, dtype, steps, nullptr);
 }
 
 FMLP_EXPORT int fmlp_orthogonalize(const void* x, void* out, int64_t H, int64_t R, int64_t C, int dtype, int steps,
@@ -193,24 +219,26 @@ int take(int n, const fmlp_muon_tensor* tensors, double lr, bool pointers, std::
 
 }  // namespace
 
-FMLP_EXPORT size_t fmlp_muon_workspace_bytes(int n, const fmlp_muon_tensor* tensors, int steps) {
+FMLP_EXPORT size_t fmlp_muon_workspace_bytes_for(int n, const fmlp_muon_tensor* tensors, int steps, const float* coefficients) {
   int cus = 0;
   std::vector<fmlp::MuonTensor> t;
-  if (check_steps(steps) || take(n, tensors, 0, false, &t, nullptr) || fmlp::abi_num_cus(&cus)) return 0;
   fmlp::MuonCall c{};
-  c.steps = steps;
-  set_stages(&c, FMLP_DTYPE_BF16);  // (weights take the update at lr)
+  if (query_call(&c, steps, coefficients, kUpdate) || take(n, tensors, 0, false, &t, nullptr) || fmlp::abi_num_cus(&cus)) return 0;
   c.update = 1;
   for (fmlp::MuonTensor& v : t)
     if (v.m == nullptr) v.m = &c;  // (a momentum whose address is not known yet)
   return fmlp::muon_plan((int)t.size(), t.data(), c, cus).ws_bytes;
 }
 
+FMLP_EXPORT size_t fmlp_muon_workspace_bytes(int n, const fmlp_muon_tensor* tensors, int steps) {
+  return fmlp_muon_workspace_bytes_for(n, tensors, steps, nullptr);
+}
+
 FMLP_EXPORT int fmlp_muon_step(int n, const fmlp_muon_tensor* tensors, double lr, double momentum, int nesterov,
                                double weight_decay, int steps, const float* coefficients, float eps, void* workspace,
                                size_t workspace_bytes, void* stream) {
   fmlp::MuonCall c{};
-  int st = set_call(&c, steps, coefficients, eps, FMLP_DTYPE_BF16);  // (weights take the update at lr)
+  int st = set_call(&c, steps, coefficients, eps, kUpdate);
   if (st) return st;
   if (!(lr >= 0) || !(weight_decay >= 0) || !(momentum >= 0 && momentum <= 1))
     return abi_fail(FMLP_ERR_INVALID_ARG, "lr or weight_decay is negative or NaN, or momentum outside [0, 1]");

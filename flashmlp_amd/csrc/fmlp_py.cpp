@@ -1103,7 +1103,7 @@ PyObject* fast_ortho(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const bool mine = !out.defined();
   if (mine) out = at::empty(x.sizes(), x.options());
   const int64_t H = heads_of(x), R = x.size(-2), C = x.size(-1);
-  const size_t n = fmlp_orthogonalize_workspace_bytes(H, R, C, io_code(x), (int)steps);
+  const size_t n = fmlp_orthogonalize_workspace_bytes_for(H, R, C, io_code(x), (int)steps, abc.data());
   at::Tensor ws;
   if (n) ws = bytes_on(x, n);
   check_status(fmlp_orthogonalize(x.data_ptr(), out.data_ptr(), H, R, C, io_code(x), (int)steps, abc.data(), (float)eps,
@@ -1147,7 +1147,7 @@ PyObject* fast_muon(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                                     io_code(*v[0]), io_code(*v[1]), io_code(*v[2]), (float)s};
   }
   c10::DeviceGuard guard(first->device());
-  const size_t bytes = fmlp_muon_workspace_bytes((int)n, t.data(), (int)steps);
+  const size_t bytes = fmlp_muon_workspace_bytes_for((int)n, t.data(), (int)steps, abc.data());
   at::Tensor ws;
   if (bytes) ws = bytes_on(*first, bytes);
   check_status(fmlp_muon_step((int)n, t.data(), lr, momentum, PyObject_IsTrue(args[5]) == 1, decay, (int)steps, abc.data(), (float)eps,

@@ -12,9 +12,10 @@ Every matrix of a stack (..., R, C) stands by itself, as the heads of the MLPs' 
 fp32; weights, gradients and momenta each of its own type, so that gradients clipped into full precision buffers
 (clip_grads) or 16-bit ones go with full precision weights. Calls are asynchronous on torch's current stream.
 
-The steps are taken on the smaller side's Gram matrix in 32 bits. Directions whose singular values are far below the largest
-(1e-4 of it) come out within 4e-4 of the formula (measured), below a 16-bit result's rounding; an fp32 `orthogonalize` is as
-exact as the formula's products in fp32. |u|^2 has to be within fp32's range.
+The steps are taken on the smaller side's Gram matrix in 32 bits. 16-bit results, and the update that weights take, are off by up
+to 4e-4 in norm and 1.4e-3 in directions whose singular values are far below the largest (measured with the usual coefficients),
+below a 16-bit result's rounding; an fp32 `orthogonalize` is as exact as the formula's products in fp32. |u|^2 has to be
+within fp32's range; coefficients under which singular values up to one may grow beyond 2^8 in between are refused.
 """
 from __future__ import annotations
 
@@ -137,7 +138,7 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence = _
     o = out if out is not None and _plain(out) else xd if same else torch.empty(x.shape, dtype=x.dtype, device=x.device)
     L = _lib.lib()
     with _On(x.get_device()) as stream:
-        n = L.fmlp_orthogonalize_workspace_bytes(H, R, C, _DTYPES[x.dtype], steps)
+        n = L.fmlp_orthogonalize_workspace_bytes_for(H, R, C, _DTYPES[x.dtype], steps, abc)
         ws = _alloc_ws(n, x.device)
         st = L.fmlp_orthogonalize(xd.data_ptr(), o.data_ptr(), H, R, C, _DTYPES[x.dtype], steps, abc, eps, _ptr(ws), n, stream)
     _lib.check(st, "orthogonalisation")
@@ -205,7 +206,7 @@ def muon_step(params: Union[torch.Tensor, Iterable[torch.Tensor]], grads: Union[
         _refuse_overlap([*params, *momenta])
     L = _lib.lib()
     with _On(dev.index) as stream:
-        n = L.fmlp_muon_workspace_bytes(len(params), calls, steps)
+        n = L.fmlp_muon_workspace_bytes_for(len(params), calls, steps, abc)
         ws = _alloc_ws(n, dev)
         st = L.fmlp_muon_step(len(params), calls, lr, momentum, int(nesterov), weight_decay, steps, abc, eps, _ptr(ws), n, stream)
     _lib.check(st, "muon step")

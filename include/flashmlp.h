@@ -403,19 +403,22 @@ int fmlp_expert_gather(const void* rows, const float* weights, const int32_t* sl
  *   X = u / (|u| + eps), |u| its Frobenius norm;  for each of `steps` (1 to 10) steps  X <- a X + b (X X^T) X + c (X X^T)^2 X
  * coefficients: a, b, c of every step, 3 * steps numbers that are read on the host, under which no singular value up to one
  * may become one above 2^8 before the last step, nor all steps on one Gram matrix enlarge one 2^16 times
- * (FMLP_ERR_UNSUPPORTED). Values are held to 2^-39 of the most that they may be. The steps are taken on the n x n Gram matrix in
- * 32 bits. Singular values far below the largest come out with an absolute error (of an orthogonal result, relative to 1)
- * of up to 4e-4 after five steps (measured on spectra of four decades) where the result has 16 bits or goes into weights; an
- * fp32 result of fmlp_orthogonalize takes the Gram matrix anew after two steps (one where the first a is above 4) and then after
- * every one, and is as exact as the products above in fp32 (measured on noise around a low rank and on spectra of one to five
- * decades: 0.3 to 1.6 times their error, up to 2.3 times with coefficients that begin at a = 8.3). |u|^2 has to be within fp32 (|u| < 1.8e19).
+ * (FMLP_ERR_UNSUPPORTED). Values are held to 2^-39 of the most that they may be. The steps are taken on n x n Gram matrices in
+ * 32 bits. Where the result has 16 bits or goes into weights, one Gram matrix serves up to five steps, fewer where their
+ * coefficients enlarge small singular values more than the usual ones (a = 3.4445) do. Such results are off, before they are rounded, by
+ * 4e-6 to 4e-4 in norm, and by up to 1.4e-3 (of an orthogonal result, relative to 1) at the singular values that were far below the
+ * largest (measured with the usual coefficients on noise around a low rank and on spectra of one to five decades; a
+ * bf16 result's rounding is 1.7e-3 and 3e-3). An fp32 result of fmlp_orthogonalize takes the Gram matrix anew after two steps (one where
+ * the first a is above 4) and then after every one, and is as exact as the products above in fp32 (on the same inputs 0.3 to
+ * 1.6 times their error, up to 2.3 times with coefficients that begin at a = 8.3). |u|^2 has to be within fp32 (|u| < 1.8e19).
  *
  * fmlp_orthogonalize: out[h] = X of x[h] for a stack of H matrices, dense, both of dtype; out may be x.
  * fmlp_muon_step, in place for n stacks of H[i] matrices each (weights w, gradients g, momenta m, dense, each of a type of its own):
  *   m = momentum m + (1 - momentum) g;  u = m, or with nesterov (1 - momentum) g + momentum m (m as it is stored)
  *   w = (1 - lr weight_decay) w - lr scale X
  * Any alignment to the elements. Memory that the call writes (w, m) must not be in it twice (FMLP_ERR_INVALID_ARG). Arrays
- * are read on the host before the call returns. Sums in a fixed order. workspace: 16-byte aligned, of the *_workspace_bytes.
+ * are read on the host before the call returns. Sums in a fixed order. workspace: 16-byte aligned, of the *_workspace_bytes_for, or of the
+ * *_workspace_bytes, which do for any coefficients (fp32 matrices in between in full).
  */
 typedef struct {
   void* w;
@@ -426,9 +429,11 @@ typedef struct {
   float scale;
 } fmlp_muon_tensor;
 size_t fmlp_orthogonalize_workspace_bytes(int64_t H, int64_t R, int64_t C, int dtype, int steps);
+size_t fmlp_orthogonalize_workspace_bytes_for(int64_t H, int64_t R, int64_t C, int dtype, int steps, const float* coefficients);
 int fmlp_orthogonalize(const void* x, void* out, int64_t H, int64_t R, int64_t C, int dtype, int steps,
                        const float* coefficients, float eps, void* workspace, size_t workspace_bytes, void* stream);
 size_t fmlp_muon_workspace_bytes(int n, const fmlp_muon_tensor* tensors, int steps);
+size_t fmlp_muon_workspace_bytes_for(int n, const fmlp_muon_tensor* tensors, int steps, const float* coefficients);
 int fmlp_muon_step(int n, const fmlp_muon_tensor* tensors, double lr, double momentum, int nesterov, double weight_decay,
                    int steps, const float* coefficients, float eps, void* workspace, size_t workspace_bytes, void* stream);
 

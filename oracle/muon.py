@@ -10,6 +10,8 @@ matrices themselves are rounded to 2^-24, twice (the products and their factor),
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from .gated import UNIT
@@ -52,13 +54,15 @@ def orthogonal64(u, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
 
 def stages(steps, full, coefficients=COEFFICIENTS):
     """first steps of the Gram matrices, and the number of steps: for fp32 results two (one where the first grows an eigenvalue near 0
-    more than 16 times), then one each; for others up to five each"""
+    more than 16 times), then one each; for others as few even ones as are of five at most and grow one by 2e4 at most before their last"""
     grow = [q * q for q, _, _ in polynomials(steps, coefficients)]
     if full:
         two = steps > 1 and grow[0] <= 16
         return [0, *range(1 + two, steps + 1)]
-    n = (steps + 4) // 5
-    return [steps * i // n for i in range(n + 1)]
+    for n in range((steps + 4) // 5, steps + 1):
+        at = [(steps * i + n - 1) // n for i in range(n + 1)]
+        if all(math.prod(grow[i:j - 1]) <= 2e4 for i, j in zip(at, at[1:])):
+            return at
 
 
 def bound(u, steps=5, coefficients=COEFFICIENTS, full=False):
