@@ -378,42 +378,63 @@ hipError_t launch_expert_plan(const void* experts, bool wide, long long M, int N
   return e;
 }
 
-hipError_t launch_expert_scatter(const ExpertCopyArgs& a, hipStream_t st) {
-  const int lg = lanes_log2(a.D, a.io);
-  const long long per = 256 >> lg, blocks = (a.T + per - 1) / per;
-  const long long row_bytes = a.D * (a.io == IO_F32 ? 4 : 2);
-  const long long chunk = std::max(1LL, kFillBytes / row_bytes);
-  const long long chunks = a.rows_out != nullptr ? (a.capacity + chunk - 1) / chunk : 0, fill = chunks * a.N;
-  if (blocks + fill > 0x7fffffffLL) return hipErrorInvalidValue;
-  if (blocks + fill == 0) return hipSuccess;
-  const dim3 grid((unsigned)(blocks + fill));
-  by_io(a.io, [&](auto IO) {
-    by_choices(a.k, [&](auto KB) {
-      constexpr int I = decltype(IO)::value, K = decltype(KB)::value;
-      const auto go = [&](auto k) {
-        hipLaunchKernelGGL(k, grid, dim3(256), 0, st, a, lg, (unsigned)fill, (unsigned)std::max(chunks, 1LL), chunk);
-      };
-      if (a.dweights != nullptr) a.weights ? go(scatter_kernel<I, K, true, true>) : go(scatter_kernel<I, K, false, true>);
-      else a.weights ? go(scatter_kernel<I, K, true, false>) : go(scatter_kernel<I, K, false, false>);
-    });
-  });
-  return hipGetLastError();
+// Tokens of a launch: those beyond kLaunchThreads' (2^25 of more than 512 bytes) take another.
+ExpertCopyArgs from_token(const ExpertCopyArgs& all, long long t0, long long most) {
+  const long long es = all.io == IO_F32 ? 4 : 2;
+  ExpertCopyArgs a = all;
+  a.T = std::min(most, all.T - t0);
+  a.x = (const char*)all.x + t0 * all.stride * es;
+  if (all.o) a.o = (char*)all.o + t0 * all.D * es;
+  a.slots += t0 * all.k;
+  if (all.weights) a.weights += t0 * all.k;
+  if (all.dweights) a.dweights += t0 * all.k;
+  return a;
 }
 
-hipError_t launch_expert_gather(const ExpertCopyArgs& a, hipStream_t st) {
-  const int lg = lanes_log2(a.D, a.io);
-  const long long per = 256 >> lg, blocks = (a.T + per - 1) / per;
-  if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-  if (blocks == 0) return hipSuccess;
-  const dim3 grid((unsigned)blocks);
-  by_io(a.io, [&](auto IO) {
-    by_choices(a.k, [&](auto KB) {
-      constexpr int I = decltype(IO)::value, K = decltype(KB)::value;
-      if (a.weights) hipLaunchKernelGGL((gather_kernel<I, K, true>), grid, dim3(256), 0, st, a, lg);
-      else hipLaunchKernelGGL((gather_kernel<I, K, false>), grid, dim3(256), 0, st, a, lg);
+hipError_t launch_expert_scatter(const ExpertCopyArgs& all, hipStream_t st) {
+  const int lg = lanes_log2(all.D, all.io);
+  const long long per = 256 >> lg, most = kLaunchThreads / 256;
+  const long long row_bytes = all.D * (all.io == IO_F32 ? 4 : 2);
+  const long long chunk = std::max(1LL, kFillBytes / row_bytes);
+  const long long chunks = all.rows_out != nullptr ? (all.capacity + chunk - 1) / chunk : 0;
+  if (chunks * all.N >= most) return hipErrorInvalidValue;  // (2^23 times 64 KB)
+  for (long long t0 = 0; t0 < all.T || t0 == 0; t0 += most * per) {
+    const ExpertCopyArgs a = from_token(all, t0, most * per);
+    const long long fill = t0 == 0 ? chunks * a.N : 0, grid = (a.T + per - 1) / per + fill;
+    if (grid == 0) return hipSuccess;
+    by_io(a.io, [&](auto IO) {
+      by_choices(a.k, [&](auto KB) {
+        constexpr int I = decltype(IO)::value, K = decltype(KB)::value;
+        const auto go = [&](auto k) {
+          hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(256), 0, st, a, lg, (unsigned)fill, (unsigned)std::max(chunks, 1LL), chunk);
+        };
+        if (a.dweights != nullptr) a.weights ? go(scatter_kernel<I, K, true, true>) : go(scatter_kernel<I, K, false, true>);
+        else a.weights ? go(scatter_kernel<I, K, true, false>) : go(scatter_kernel<I, K, false, false>);
+      });
     });
-  });
-  return hipGetLastError();
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+hipError_t launch_expert_gather(const ExpertCopyArgs& all, hipStream_t st) {
+  const int lg = lanes_log2(all.D, all.io);
+  const long long per = 256 >> lg, most = kLaunchThreads / 256 * per;
+  for (long long t0 = 0; t0 < all.T; t0 += most) {
+    const ExpertCopyArgs a = from_token(all, t0, most);
+    const dim3 grid((unsigned)((a.T + per - 1) / per));
+    by_io(a.io, [&](auto IO) {
+      by_choices(a.k, [&](auto KB) {
+        constexpr int I = decltype(IO)::value, K = decltype(KB)::value;
+        if (a.weights) hipLaunchKernelGGL((gather_kernel<I, K, true>), grid, dim3(256), 0, st, a, lg);
+        else hipLaunchKernelGGL((gather_kernel<I, K, false>), grid, dim3(256), 0, st, a, lg);
+      });
+    });
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace fmlp

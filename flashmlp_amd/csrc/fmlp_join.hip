@@ -527,9 +527,7 @@ RowShape row_shape(int64_t C) {
   return {vpt, true, (vecs + vpt * 64 - 1) / (vpt * 64) * 64};
 }
 
-// A launch holds fewer than 2^32 threads: rows beyond 2^31 threads' (2^25 rows of up to 1024 columns) take another.
-constexpr long long kLaunchThreads = 1LL << 31;
-
+// Rows beyond kLaunchThreads' (2^25 rows of up to 1024 columns) take another launch.
 template <int IO, int RIO>
 hipError_t fwd_launch(const JoinArgs& a, const RowShape& s, long long grid, hipStream_t st) {
   return by_shape(s.vpt, [&](auto V) {

@@ -16,6 +16,9 @@ int env_int(const char* name, int dflt);
 // skip the runtime call.
 hipError_t set_lds_once(const void* kernel, int bytes, std::atomic<unsigned long long>& done);
 
+// A launch holds fewer than 2^32 threads: workgroups beyond 2^31 threads' take another.
+constexpr long long kLaunchThreads = 1LL << 31;
+
 // Row pitch the kernels read W1 with (elements of es bytes): E rounded up to whole 16-byte
 // vectors. Where E is no such multiple the caller's W1 rows are copied to this pitch first
 // (launch_pad_w1), into w1_pad_bytes of workspace (a multiple of 256 bytes).

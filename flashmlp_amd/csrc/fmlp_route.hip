@@ -12,6 +12,8 @@
 // Bound by vector issue, about 60 instructions a round and wave of 8 rows at 64 experts: 65536 x 64 bf16, 8 a token, 11.7 us (12 MB),
 // the gradient 7.3 (15 MB). Maxima over the group through the LDS crossbar and every lane's scan of the chosen index: 16.4; the choices
 // of a row read by each of its lanes: 10.4.
+#include <algorithm>
+
 #include "fmlp_experts.h"
 #include "fmlp_vec.h"
 
@@ -192,48 +194,60 @@ __global__ void __launch_bounds__(kThreads) route_bwd_kernel(RouteArgs a) {
   }
 }
 
-// f(io, logits of a lane, log2 of a row's lanes): 8 logits a lane, 16 where 64 lanes would not do
+// f(io, logits of a lane, log2 of a row's lanes, workgroups, arguments): 8 logits a lane, 16 where 64 lanes would not do. Rows beyond
+// kLaunchThreads' (2^25 of more than 256 experts) take another launch.
 template <typename F>
-hipError_t by_form(const RouteArgs& a, F f) {
+hipError_t by_form(const RouteArgs& all, F f) {
   int lg = 0;
-  while (lg < 6 && (8 << lg) < a.N) ++lg;
-  const long long rows = kThreads >> lg, blocks = (a.T + rows - 1) / rows;
-  if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)blocks);
+  while (lg < 6 && (8 << lg) < all.N) ++lg;
+  const long long rows = kThreads >> lg, most = kLaunchThreads / kThreads * rows, es = all.io == IO_F32 ? 4 : 2;
+  RouteArgs a = all;
+  dim3 grid;
   const auto io = [&](auto VPL, auto LG) {
-    if (a.io == IO_F32) f(std::integral_constant<int, IO_F32>{}, VPL, LG, grid);
-    else if (a.io == IO_BF16) f(std::integral_constant<int, IO_BF16>{}, VPL, LG, grid);
-    else f(std::integral_constant<int, IO_F16>{}, VPL, LG, grid);
+    if (a.io == IO_F32) f(std::integral_constant<int, IO_F32>{}, VPL, LG, grid, a);
+    else if (a.io == IO_BF16) f(std::integral_constant<int, IO_BF16>{}, VPL, LG, grid, a);
+    else f(std::integral_constant<int, IO_F16>{}, VPL, LG, grid, a);
   };
   const auto eight = std::integral_constant<int, 8>{};
-  switch (lg) {
-    case 0: io(eight, std::integral_constant<int, 0>{}); break;
-    case 1: io(eight, std::integral_constant<int, 1>{}); break;
-    case 2: io(eight, std::integral_constant<int, 2>{}); break;
-    case 3: io(eight, std::integral_constant<int, 3>{}); break;
-    case 4: io(eight, std::integral_constant<int, 4>{}); break;
-    case 5: io(eight, std::integral_constant<int, 5>{}); break;
-    default:
-      if (a.N <= 512) io(eight, std::integral_constant<int, 6>{});
-      else io(std::integral_constant<int, 16>{}, std::integral_constant<int, 6>{});
+  for (long long t0 = 0; t0 < all.T; t0 += most) {
+    a.T = std::min(most, all.T - t0);
+    a.logits = all.logits == nullptr ? nullptr : (const char*)all.logits + t0 * all.stride * es;
+    a.weights = all.weights + t0 * all.k;
+    a.experts = all.experts + t0 * all.k;
+    if (all.dweights != nullptr) {
+      a.dweights = all.dweights + t0 * all.k;
+      a.dlogits = (char*)all.dlogits + t0 * all.N * es;
+    }
+    grid = dim3((unsigned)((a.T + rows - 1) / rows));
+    switch (lg) {
+      case 0: io(eight, std::integral_constant<int, 0>{}); break;
+      case 1: io(eight, std::integral_constant<int, 1>{}); break;
+      case 2: io(eight, std::integral_constant<int, 2>{}); break;
+      case 3: io(eight, std::integral_constant<int, 3>{}); break;
+      case 4: io(eight, std::integral_constant<int, 4>{}); break;
+      case 5: io(eight, std::integral_constant<int, 5>{}); break;
+      default:
+        if (a.N <= 512) io(eight, std::integral_constant<int, 6>{});
+        else io(std::integral_constant<int, 16>{}, std::integral_constant<int, 6>{});
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
   }
-  return hipGetLastError();
+  return hipSuccess;
 }
 
 }  // namespace
 
-hipError_t launch_route_fwd(const RouteArgs& a, hipStream_t st) {
-  if (a.T == 0) return hipSuccess;
-  return by_form(a, [&](auto IO, auto VPL, auto LG, dim3 grid) {
+hipError_t launch_route_fwd(const RouteArgs& all, hipStream_t st) {
+  return by_form(all, [&](auto IO, auto VPL, auto LG, dim3 grid, const RouteArgs& a) {
     constexpr int L = decltype(LG)::value;
     const size_t lds = (size_t)(kThreads >> L) * (2 * (size_t)a.k + 1) * 4;
     hipLaunchKernelGGL((route_fwd_kernel<decltype(IO)::value, decltype(VPL)::value, L>), grid, dim3(kThreads), lds, st, a);
   });
 }
 
-hipError_t launch_route_bwd(const RouteArgs& a, hipStream_t st) {
-  if (a.T == 0) return hipSuccess;
-  return by_form(a, [&](auto IO, auto VPL, auto LG, dim3 grid) {
+hipError_t launch_route_bwd(const RouteArgs& all, hipStream_t st) {
+  return by_form(all, [&](auto IO, auto VPL, auto LG, dim3 grid, const RouteArgs& a) {
     constexpr int L = decltype(LG)::value;
     const size_t lds = (size_t)(kThreads >> L) * 3 * (size_t)a.k * 4;
     hipLaunchKernelGGL((route_bwd_kernel<decltype(IO)::value, decltype(VPL)::value, L>), grid, dim3(kThreads), lds, st, a);
