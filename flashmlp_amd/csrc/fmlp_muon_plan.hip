@@ -129,7 +129,8 @@ struct Item {
   long long matrix0;
 };
 
-// f(kind, table, workgroups) for tables of items of one kind, `parts` workgroups a matrix
+// f(kind, table, workgroups) for tables of items of one kind, `parts` workgroups a matrix, and no more of 512 threads than a launch
+// holds
 template <typename F>
 hipError_t for_tables(const std::vector<Item>& items, int parts, bool any_type, F f) {
   for (int code = 0; code < 8; ++code) {  // (kinds in a fixed order)
@@ -142,8 +143,9 @@ hipError_t for_tables(const std::vector<Item>& items, int parts, bool any_type, 
       if (!end && !(it->kind.terms == k.terms && (any_type || it->kind.bf == k.bf) && it->kind.vec == k.vec)) continue;
       if (!end && any_type && !k.bf) continue;  // (both 16-bit types at once)
       const long long b = end ? 0 : it->t.H * parts;
-      if (b > 0x7fffffffLL) return hipErrorInvalidValue;
-      if (tab.n > 0 && (end || tab.n == kMuonTable || blocks + b > 0x7fffffffLL)) {
+      constexpr long long most = kLaunchThreads / 512;
+      if (b > most) return hipErrorInvalidValue;
+      if (tab.n > 0 && (end || tab.n == kMuonTable || blocks + b > most)) {
         const hipError_t e = f(k, tab, (unsigned)blocks);
         if (e != hipSuccess) return e;
         tab.n = 0;
