@@ -17,6 +17,7 @@ struct MuonTensor {
   int R, C;
   int x_io, m_io, out_io;  // IoType
   float lr;                // update: keep out - lr O
+  size_t between;          // launch_muon: where its matrices are between stages
 };
 
 // What a call does with every tensor: u = x, or with momenta m' = mu m + nu x, u = m' or (nesterov) nu x + mu m';

@@ -167,6 +167,52 @@ size_t between_bytes(const MuonTensor& t, const MuonCall& c) {
   return ((size_t)t.H * t.R * t.C * 4 + 255) / 256 * 256;
 }
 
+// The call's stacks of one padded size, or runs of a stack's matrices, that go through the workspace together.
+struct Batch {
+  std::vector<MuonTensor> t;
+  Group g;
+  size_t between, end;  // bytes before the matrices between stages, and of it all
+};
+// In even batches of 1024 matrices of 256 at most, whose Gram matrices and P are 512 MB (a Muon step of 2048 of
+// 256 x 300 takes 7.6 ms, at once 7.6; of 4096 15.2 and 15.1); of as many of the others as have a launch of a workgroup each.
+constexpr long long kBatch256 = 1024, kBatch = kLaunchThreads / 512;
+std::vector<Batch> batches_of(int NP, int n, const MuonTensor* t, const MuonCall& c, int cus) {
+  long long matrices = 0;
+  for (int i = 0; i < n; ++i)
+    if (!empty(t[i]) && padded(t[i]) == NP) matrices += t[i].H;
+  std::vector<Batch> out;
+  if (matrices == 0) return out;
+  const long long most = NP == 256 ? kBatch256 : kBatch, number = (matrices + most - 1) / most, each = (matrices + number - 1) / number;
+  long long room = 0;
+  for (int i = 0; i < n; ++i) {
+    if (empty(t[i]) || padded(t[i]) != NP) continue;
+    const auto bytes = [](int io) { return io == IO_F32 ? 4 : 2; };
+    for (long long h = 0; h < t[i].H;) {
+      if (room == 0) {
+        out.emplace_back();
+        room = each;
+      }
+      MuonTensor v = t[i];
+      v.H = std::min(t[i].H - h, room);
+      const size_t at = (size_t)h * t[i].R * t[i].C;
+      v.x = (const char*)v.x + at * bytes(v.x_io);
+      if (v.m != nullptr) v.m = (char*)v.m + at * bytes(v.m_io);
+      v.out = (char*)v.out + at * bytes(v.out_io);
+      v.between = out.back().between;
+      out.back().between += between_bytes(v, c);
+      out.back().t.push_back(v);
+      h += v.H;
+      room -= v.H;
+    }
+  }
+  for (Batch& b : out) {
+    b.g = group_of(NP, (int)b.t.size(), b.t.data(), cus);
+    b.end = b.g.end + b.between;
+    b.between = b.g.end;
+  }
+  return out;
+}
+
 }  // namespace
 
 // The eigenvalues of the first G are in [0, 1], those after a step in [0, r'], r' the largest l q(l)^2 on [0, r]: at an end or
@@ -199,93 +245,85 @@ void muon_bounds(MuonCall* c) {
 
 MuonPlan muon_plan(int n, const MuonTensor* t, const MuonCall& c, int num_cus) {
   MuonPlan p{};
-  for (int NP : kSizes) {
-    const Group g = group_of(NP, n, t, num_cus);
-    if (g.matrices) p.ws_bytes = std::max(p.ws_bytes, g.end);
-  }
-  for (int i = 0; i < n; ++i) p.ws_bytes += between_bytes(t[i], c);
+  for (int NP : kSizes)
+    for (const Batch& b : batches_of(NP, n, t, c, num_cus)) p.ws_bytes = std::max(p.ws_bytes, b.end);
   return p;
 }
 
-hipError_t launch_muon(int n, const MuonTensor* t, const MuonCall& c, int num_cus, void* ws, hipStream_t st) {
-  size_t shared = 0;
-  for (int NP : kSizes) {
-    const Group g = group_of(NP, n, t, num_cus);
-    if (g.matrices) shared = std::max(shared, g.end);
-  }
-  for (int NP : kSizes) {
-    const Group gr = group_of(NP, n, t, num_cus);
-    if (gr.matrices == 0) continue;
-    float* G = (float*)ws;
-    unsigned short* P = (unsigned short*)((char*)ws + gr.p_off);
-    MuonInfo* info = (MuonInfo*)((char*)ws + gr.info_off);
-    for (int stage = 0; stage < c.stages; ++stage) {
-      const int first = c.first[stage], steps = c.first[stage + 1] - first;
-      const bool start = stage == 0, last = stage + 1 == c.stages;
-      const int update = c.update && last;
-      MuonSteps s{};
-      set_steps(&s, c, first, steps, start);
-      std::vector<Item> items;
-      long long matrix = 0;
-      char* between = (char*)ws + shared;
-      for (int i = 0; i < n; ++i) {
-        const size_t bytes = between_bytes(t[i], c);
-        if (!empty(t[i]) && padded(t[i]) == NP) {
-          MuonTensor v = t[i];
-          void* y = bytes ? (void*)between : t[i].out;
-          if (!start) {
-            v.x = y;
-            v.m = nullptr;
-            v.x_io = IO_F32;
-          }
-          if (!last) {
-            v.out = y;
-            v.out_io = IO_F32;
-          }
-          items.push_back(Item{v, kind_of(v), matrix});
-          matrix += v.H;
-        }
-        between += bytes;
+static hipError_t launch_batch(int NP, const Batch& b, const MuonCall& c, void* ws, hipStream_t st) {
+  const Group& gr = b.g;
+  float* G = (float*)ws;
+  unsigned short* P = (unsigned short*)((char*)ws + gr.p_off);
+  MuonInfo* info = (MuonInfo*)((char*)ws + gr.info_off);
+  for (int stage = 0; stage < c.stages; ++stage) {
+    const int first = c.first[stage], steps = c.first[stage + 1] - first;
+    const bool start = stage == 0, last = stage + 1 == c.stages;
+    const int update = c.update && last;
+    MuonSteps s{};
+    set_steps(&s, c, first, steps, start);
+    std::vector<Item> items;
+    long long matrix = 0;
+    for (MuonTensor v : b.t) {
+      void* y = between_bytes(v, c) ? (void*)((char*)ws + b.between + v.between) : v.out;
+      if (!start) {
+        v.x = y;
+        v.m = nullptr;
+        v.x_io = IO_F32;
       }
-      hipError_t e;
-      if (gr.whole) {
-        e = for_tables(items, 1, false, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
-          return NP == 32   ? muon_whole<32>(k, tab, blocks, s, c, update, st)
-                 : NP == 64 ? muon_whole<64>(k, tab, blocks, s, c, update, st)
-                            : muon_whole<128>(k, tab, blocks, s, c, update, st);
-        });
-        if (e != hipSuccess) return e;
-        continue;
+      if (!last) {
+        v.out = y;
+        v.out_io = IO_F32;
       }
-      e = hipSuccess;
-      if (gr.by_tiles) {
-        // (all have a momentum, or none has)
-        if (items[0].t.m != nullptr)
-          e = for_tables(items, gr.apply_parts, false, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
-            return muon_momentum(k, tab, blocks, gr.apply_parts, c, st);
-          });
-        if (e == hipSuccess)
-          e = for_tables(items, kMuonGramTiles * gr.gram_parts, false, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
-            return muon_gram_tiles(k, tab, blocks, G, gr.gram_parts, c, st);
-          });
-      }
-      else e = for_tables(items, gr.gram_parts, false, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
-        return NP == 32    ? muon_gram<32>(k, tab, blocks, G, gr.gram_parts, c, st)
-               : NP == 64  ? muon_gram<64>(k, tab, blocks, G, gr.gram_parts, c, st)
-               : NP == 128 ? muon_gram<128>(k, tab, blocks, G, gr.gram_parts, c, st)
-                           : muon_gram<256>(k, tab, blocks, G, gr.gram_parts, c, st);
+      items.push_back(Item{v, kind_of(v), matrix});
+      matrix += v.H;
+    }
+    hipError_t e;
+    if (gr.whole) {
+      e = for_tables(items, 1, false, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
+        return NP == 32   ? muon_whole<32>(k, tab, blocks, s, c, update, st)
+               : NP == 64 ? muon_whole<64>(k, tab, blocks, s, c, update, st)
+                          : muon_whole<128>(k, tab, blocks, s, c, update, st);
       });
-      if (e == hipSuccess) e = launch_muon_iter(NP, gr.matrices, G, gr.gram_parts, P, info, s, (char*)ws + gr.iter_off, st);
-      if (e == hipSuccess)
-        e = for_tables(items, gr.apply_parts, true, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
-          return NP == 32    ? muon_apply<32>(k, tab, blocks, P, info, gr.apply_parts, c, update, st)
-                 : NP == 64  ? muon_apply<64>(k, tab, blocks, P, info, gr.apply_parts, c, update, st)
-                 : NP == 128 ? muon_apply<128>(k, tab, blocks, P, info, gr.apply_parts, c, update, st)
-                             : muon_apply<256>(k, tab, blocks, P, info, gr.apply_parts, c, update, st);
+      if (e != hipSuccess) return e;
+      continue;
+    }
+    e = hipSuccess;
+    if (gr.by_tiles) {
+      // (all have a momentum, or none has)
+      if (items[0].t.m != nullptr)
+        e = for_tables(items, gr.apply_parts, false, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
+          return muon_momentum(k, tab, blocks, gr.apply_parts, c, st);
         });
+      if (e == hipSuccess)
+        e = for_tables(items, kMuonGramTiles * gr.gram_parts, false, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
+          return muon_gram_tiles(k, tab, blocks, G, gr.gram_parts, c, st);
+        });
+    }
+    else e = for_tables(items, gr.gram_parts, false, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
+      return NP == 32    ? muon_gram<32>(k, tab, blocks, G, gr.gram_parts, c, st)
+             : NP == 64  ? muon_gram<64>(k, tab, blocks, G, gr.gram_parts, c, st)
+             : NP == 128 ? muon_gram<128>(k, tab, blocks, G, gr.gram_parts, c, st)
+                         : muon_gram<256>(k, tab, blocks, G, gr.gram_parts, c, st);
+    });
+    if (e == hipSuccess) e = launch_muon_iter(NP, gr.matrices, G, gr.gram_parts, P, info, s, (char*)ws + gr.iter_off, st);
+    if (e == hipSuccess)
+      e = for_tables(items, gr.apply_parts, true, [&](const MuonKind& k, const MuonTable& tab, unsigned blocks) {
+        return NP == 32    ? muon_apply<32>(k, tab, blocks, P, info, gr.apply_parts, c, update, st)
+               : NP == 64  ? muon_apply<64>(k, tab, blocks, P, info, gr.apply_parts, c, update, st)
+               : NP == 128 ? muon_apply<128>(k, tab, blocks, P, info, gr.apply_parts, c, update, st)
+                           : muon_apply<256>(k, tab, blocks, P, info, gr.apply_parts, c, update, st);
+      });
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+hipError_t launch_muon(int n, const MuonTensor* t, const MuonCall& c, int num_cus, void* ws, hipStream_t st) {
+  for (int NP : kSizes)
+    for (const Batch& b : batches_of(NP, n, t, c, num_cus)) {
+      const hipError_t e = launch_batch(NP, b, c, ws, st);
       if (e != hipSuccess) return e;
     }
-  }
   return hipSuccess;
 }
 
