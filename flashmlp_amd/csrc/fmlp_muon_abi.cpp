@@ -59,7 +59,8 @@ int check_stack(int64_t H, int64_t R, int64_t C, int i) {
   if (std::min(R, C) > fmlp::kMuonMaxSmall)
     return abi_fail(FMLP_ERR_UNSUPPORTED, "stack %d: matrices of %lld x %lld: the smaller side is at most %d", i, (long long)R,
                     (long long)C, fmlp::kMuonMaxSmall);
-  if (R > 0x3fffffffLL || C > 0x3fffffffLL || H > 0x3ffffLL)
+  // (2^40 elements are 2 TB at least)
+  if (R > 0x3fffffffLL || C > 0x3fffffffLL || H > (1LL << 40) / std::max<int64_t>(1, R * C))
     return abi_fail(FMLP_ERR_INVALID_ARG, "stack %d: dimension too large (H=%lld R=%lld C=%lld)", i, (long long)H, (long long)R,
                     (long long)C);
   return FMLP_OK;
@@ -111,6 +112,14 @@ int query_call(fmlp::MuonCall* c, int steps, const float* coefficients, int dtyp
 // weights take the update at lr: as exact as a 16-bit result
 constexpr int kUpdate = FMLP_DTYPE_BF16;
 
+size_t plan_bytes(int n, const fmlp::MuonTensor* t, const fmlp::MuonCall& c, int cus) {
+  try {
+    return fmlp::muon_plan(n, t, c, cus).ws_bytes;
+  } catch (const std::bad_alloc&) {  // (the call refuses)
+    return 0;
+  }
+}
+
 int run(int n, const fmlp::MuonTensor* t, const fmlp::MuonCall& c, void* ws, size_t ws_bytes, void* stream, const char* what) {
   int cus = 0, st;
   if ((st = fmlp::abi_num_cus(&cus))) return st;
@@ -144,7 +153,7 @@ FMLP_EXPORT size_t fmlp_orthogonalize_workspace_bytes_for(int64_t H, int64_t R, 
   if (check_stack(H, R, C, 0) || !known_dtype(dtype) || query_call(&c, steps, coefficients, dtype) || fmlp::abi_num_cus(&cus)) return 0;
   fmlp::MuonTensor t = stack_of(H, R, C);
   t.x_io = t.out_io = io_type(dtype);
-  return fmlp::muon_plan(1, &t, c, cus).ws_bytes;
+  return plan_bytes(1, &t, c, cus);
 }
 
 FMLP_EXPORT size_t fmlp_orthogonalize_workspace_bytes(int64_t H, int64_t R, int64_t C, int dtype, int steps) {
@@ -227,7 +236,7 @@ FMLP_EXPORT size_t fmlp_muon_workspace_bytes_for(int n, const fmlp_muon_tensor* 
   c.update = 1;
   for (fmlp::MuonTensor& v : t)
     if (v.m == nullptr) v.m = &c;  // (a momentum whose address is not known yet)
-  return fmlp::muon_plan((int)t.size(), t.data(), c, cus).ws_bytes;
+  return plan_bytes((int)t.size(), t.data(), c, cus);
 }
 
 FMLP_EXPORT size_t fmlp_muon_workspace_bytes(int n, const fmlp_muon_tensor* tensors, int steps) {

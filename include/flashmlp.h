@@ -416,7 +416,7 @@ int fmlp_expert_gather(const void* rows, const float* weights, const int32_t* sl
  * fmlp_muon_step, in place for n stacks of H[i] matrices each (weights w, gradients g, momenta m, dense, each of a type of its own):
  *   m = momentum m + (1 - momentum) g;  u = m, or with nesterov (1 - momentum) g + momentum m (m as it is stored)
  *   w = (1 - lr weight_decay) w - lr scale X
- * Any alignment to the elements. Memory that the call writes (w, m) must not be in it twice (FMLP_ERR_INVALID_ARG). Arrays
+ * At most 2^40 elements a stack. Any alignment to the elements. Memory that the call writes (w, m) must not be in it twice (FMLP_ERR_INVALID_ARG). Arrays
  * are read on the host before the call returns. Sums in a fixed order. workspace: 16-byte aligned, of the *_workspace_bytes_for, or of the
  * *_workspace_bytes, which do for any coefficients (fp32 matrices in between in full).
  */

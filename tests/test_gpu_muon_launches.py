@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from flashmlp_amd import muon_step
+from flashmlp_amd import muon_step, orthogonalize
 from oracle import muon as om
 
 pytestmark = pytest.mark.gpu
@@ -21,3 +21,23 @@ def test_stacks_of_more_matrices_than_one_launch_has_workgroups():
         for a, c, d in om.triples(om.COEFFICIENTS, 5):
             x = x * (a + x * x * (c + x * x * d))
         assert ((t + x).abs() <= 1e-3).all()
+
+
+def usual(x):
+    for a, c, d in om.triples(om.COEFFICIENTS, 5):
+        x = x * (a + x * x * (c + x * x * d))
+    return x
+
+
+def test_a_stack_of_more_matrices_than_one_launch_has_workgroups():
+    """matrices of one row, whose result is the row times a number; every launch's first and last matrices are among them"""
+    H = (1 << 24) + 3
+    x = torch.randn(H, 1, 2, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda")
+    n = x.double().norm(dim=(1, 2), keepdim=True)
+    s = n / (n + 1e-7)
+    want = x.double() / n * usual(s)
+    assert ((orthogonalize(x) - want).abs() <= 1e-5).all()
+    w, m = torch.zeros_like(x), torch.zeros_like(x)
+    muon_step([w, w.new_zeros(5, 40, 50)], [x, x[:1000].view(1, 40, 50).expand(5, 40, 50)], [m, m.new_zeros(5, 40, 50)], 1.0, momentum=0.0,
+              nesterov=False, scale=1.0)
+    assert ((w + want).abs() <= 1e-3).all()

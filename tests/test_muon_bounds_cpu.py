@@ -66,3 +66,14 @@ def test_refusal_of_coefficients(coefficients, steps, step):
     assert L.fmlp_muon_step(1, t, 0.1, 0.9, 1, 0.0, steps, abc, 1e-7, None, 0, None) != 0
     message = L.fmlp_last_error().decode()
     assert "coefficient" in message and (step is None or f"step {step}" in message)
+
+
+def test_sizes_past_64_bits_are_refused():
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("libflashmlp.so not built (python -m flashmlp_amd.build)")
+    L = _lib.lib()
+    abc = (ctypes.c_float * 3)(1.5, -0.5, 0.0)
+    for H, R, C in ((1 << 62, 2, 2), (1 << 30, 256, 1 << 28), ((1 << 63) - 1, 1, 1), (1 << 40, 1, 1 << 30), (1, 200, 1 << 30)):
+        assert L.fmlp_orthogonalize(4096, 1 << 20, H, R, C, 2, 1, abc, 1e-7, None, 0, None) == 1
+        assert "too large" in L.fmlp_last_error().decode()
+        assert L.fmlp_orthogonalize_workspace_bytes(H, R, C, 2, 1) == 0
