@@ -1073,8 +1073,10 @@ bool number(PyObject* o, double* v) {
   PyErr_Clear();
   return false;
 }
-// a dense stack of matrices of a type that the kernels take
-bool stack_ok(const at::Tensor& t) { return on_gpu(t) && io_code(t) >= 0 && t.dim() >= 2 && t.is_contiguous(); }
+// a dense stack of matrices of a type that the kernels take (one with a tangent goes to Python, which refuses forward mode)
+bool stack_ok(const at::Tensor& t) {
+  return on_gpu(t) && io_code(t) >= 0 && t.dim() >= 2 && t.is_contiguous() && !t._fw_grad(0).defined();
+}
 int64_t heads_of(const at::Tensor& t) {
   int64_t h = 1;
   for (int64_t i = 0; i + 2 < t.dim(); ++i) h *= t.size(i);

@@ -25,6 +25,7 @@ import numbers
 from typing import Iterable, Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 from .block import _input
@@ -65,6 +66,8 @@ def _check(t: torch.Tensor, what: str, dev=None):
     if t.layout != torch.strided:
         raise TypeError(f"{what} must be dense tensors, got {t.layout}")
     _input(t)  # (memory of its own)
+    if unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"orthogonalised updates have no forward mode (jvp): {what} with a tangent")
 
 
 def _number(v, name):
@@ -117,7 +120,7 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence = _
     Args:
         steps: 1 to 10; coefficients: (a, b, c), or one such triple for each step;
         out: of x's shape and type, or x itself.
-    No gradient is kept.
+    No gradient is kept; forward mode is refused.
     """
     if _fast is not None:  # dense tensors on one GPU and no error: else None
         r = _fast.orthogonalize(x, out, steps, coefficients, eps)
