@@ -992,11 +992,14 @@ bool rows_ok(const at::Tensor& rows) {
   return on_gpu(rows) && io_code(rows) >= 0 && rows.dim() == 3 && rows.size(2) >= 1 && rows.is_contiguous();
 }
 
+// Saves the rows for the weights' gradient alone.
 struct CombineFn : torch::autograd::Function<CombineFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& rows, const std::optional<at::Tensor>& w_, const at::Tensor& slots,
                             const at::Tensor& counts) {
     const at::Tensor w = w_.value_or(at::Tensor());
-    ctx->save_for_backward({rows, w, slots, counts});
+    ctx->save_for_backward({w.defined() && w.requires_grad() ? rows : at::Tensor(), w, slots, counts});
+    ctx->saved_data["rows"] = rows.sizes();
+    ctx->saved_data["dtype"] = (int64_t)rows.scalar_type();
     return gather_run(rows, w, slots);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -1006,15 +1009,17 @@ struct CombineFn : torch::autograd::Function<CombineFn> {
   static variable_list first(AutogradContext* ctx, const variable_list& s, const variable_list& grads) {
     variable_list r(4);
     if (!grads[0].defined()) return r;
-    const bool weighted = s[1].defined();
+    const auto shape = ctx->saved_data["rows"].toIntVector();
+    const auto dtype = (at::ScalarType)ctx->saved_data["dtype"].toInt();
     const at::Tensor dout = cols(grads[0]), rows = dense(s[0]), w = dense(s[1]), slots = dense(s[2]), counts = dense(s[3]);
-    TORCH_CHECK(rows_ok(rows) && dout.dim() == 2 && dout.size(1) == rows.size(2) && dout.scalar_type() == rows.scalar_type() &&
-                    dout.device() == rows.device() && plan_ok(slots, counts, rows, dout.size(0), rows.size(0), rows.size(1)) &&
-                    (!weighted || (dense_beside(w, rows, at::kFloat) && w.sizes() == slots.sizes())),
+    TORCH_CHECK(dout.dim() == 2 && dout.size(1) == shape[2] && dout.scalar_type() == dtype &&
+                    plan_ok(slots, counts, dout, dout.size(0), shape[0], shape[1]) &&
+                    (!rows.defined() || (dense_beside(rows, dout, dtype) && rows.sizes() == shape)) &&
+                    (!w.defined() || (dense_beside(w, dout, at::kFloat) && w.sizes() == slots.sizes())),
                 "a saved tensor of the combination came back with another size, type or device");
     // (the node has an edge for each tensor that is there: rows, then the weights)
-    auto g = scatter_run(dout, w, slots, counts, rows.size(0), rows.size(1), rows, ctx->needs_input_grad(0),
-                         weighted && ctx->needs_input_grad(1));
+    auto g = scatter_run(dout, w, slots, counts, shape[0], shape[1], rows, ctx->needs_input_grad(0),
+                         rows.defined() && ctx->needs_input_grad(1));
     r[0] = g.first;
     r[1] = g.second;
     return r;

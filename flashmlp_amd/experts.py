@@ -243,17 +243,19 @@ class _DispatchFunction(torch.autograd.Function):
 
 
 class _CombineFunction(torch.autograd.Function):
+    """Saves the rows for the weights' gradient alone."""
+
     @staticmethod
     def forward(ctx, rows, weights, slots, counts):
-        _save(ctx, rows, weights, slots, counts)
+        _save(ctx, rows if weights is not None and ctx.needs_input_grad[1] else None, weights, slots, counts)
+        ctx.args = rows.shape[:2]
         return _gather(rows, weights, slots)
 
     @staticmethod
     @first_derivatives_only
     def backward(ctx, do):
         rows, weights, slots, counts = _saved(ctx)
-        N, capacity, _ = rows.shape
-        drows, dw = _scatter(do, weights, slots, counts, N, capacity, rows, ctx.needs_input_grad[0],
+        drows, dw = _scatter(do, weights, slots, counts, *ctx.args, rows, ctx.needs_input_grad[0],
                              weights is not None and ctx.needs_input_grad[1])
         return drows, dw, None, None
 
