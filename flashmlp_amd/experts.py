@@ -131,7 +131,8 @@ def expert_route(logits: torch.Tensor, k: int, *, normalize: bool = True) -> Tup
 
     Args:
         logits: (T, N), fp16, bf16 or fp32; -infinity masks an expert; N <= 1024, k <= 32;
-        normalize: the weights are softmax probabilities over their sum over the k; else as they are.
+        normalize: the weights are softmax probabilities over their sum over the k; else as they are. (With k = 1 the
+        weight is 1 whatever the logits, which get no gradient then.)
     Returns:
         (weights, experts): (T, k) fp32, and (T, k) int32 in falling order of the logits. A token with fewer
         than k experts that are not masked has -1 with the weight 0 in place of the rest.
@@ -307,18 +308,18 @@ class GatedExperts(torch.nn.Module):
         experts_per_token: k
         capacity_factor: an expert has ceil(T k / N * capacity_factor) rows for T tokens, what comes beyond is
             dropped; None: T rows, none is dropped
-        normalize: as expert_route's
+        normalize: as expert_route's; None: where experts_per_token is above one, so that the router always learns
 
     The input is (..., D): rows of tokens, or the MLP's (H, B, D) layout, whose heads' rows are tokens of their own.
     Parameters: router (D, N) ~ randn / sqrt(D), and the experts' (experts.wg, experts.wu, experts.w2).
     """
 
     def __init__(self, num_experts: int, hidden_dim: int, intermediate_dim: int, experts_per_token: int = 2,
-                 capacity_factor: Optional[float] = None, activation: str = "silu", normalize: bool = True,
-                 dtype=torch.float16, device="cuda"):
+                 capacity_factor: Optional[float] = None, activation: str = "silu",
+                 normalize: Optional[bool] = None, dtype=torch.float16, device="cuda"):
         super().__init__()
         self.num_experts, self.experts_per_token = num_experts, experts_per_token
-        self.capacity_factor, self.normalize = capacity_factor, normalize
+        self.capacity_factor, self.normalize = capacity_factor, experts_per_token > 1 if normalize is None else normalize
         self.router = torch.nn.Parameter(torch.randn(hidden_dim, num_experts, dtype=dtype, device=device) / hidden_dim ** 0.5)
         self.experts = GatedFlashMLP(num_experts, hidden_dim, intermediate_dim, activation, dtype=dtype, device=device)
 
