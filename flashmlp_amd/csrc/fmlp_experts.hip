@@ -12,7 +12,7 @@
 // The copies are bound by HBM. A token has a group of lanes, 16 bytes a lane; it is read once and written to its k rows (dispatch), so
 // that no inverse map is needed: what is left of an expert's capacity is filled with zeros by workgroups of their own.
 //
-// Measured, 2^19 tokens of 128 bf16 columns, 32 experts of 40960 rows, 2 a token: plan 17 us (2 launches), scatter 82 (470 MB,
+// Measured, 2^19 tokens of 128 bf16 columns, 32 experts of 40960 rows, 2 a token: plan 18 us (2 launches), scatter 82 (470 MB,
 // 5.7 TB/s), gather 75-83 (403 MB, 4.9 to 5.4 TB/s), scatter with weights and their gradient 138 (737 MB, 5.3 TB/s); a copy reaches 5.2.
 // Loads without branches around them (dropped choices read some row and throw it away) measured the same.
 #include <algorithm>

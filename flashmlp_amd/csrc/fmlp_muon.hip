@@ -14,7 +14,7 @@
 // error is below that of the fp32 sums, at any scale. P u takes fp16 terms, two of P and one (16-bit u) or two of u, scaled by
 // powers of two: |u| is known by then.
 //
-// Measured: 2304 matrices of 128 x 1024 (302 M fp32 weights and momenta, bf16 gradients) 1.73 ms, 24 bytes an element at 4.2 TB/s
+// Measured: 2304 matrices of 128 x 1024 (302 M fp32 weights and momenta, bf16 gradients) 1.75 ms, 24 bytes an element at 4.1 TB/s
 // where a copy reaches 5.2; matrix instructions 31 % and vector ones 37 % of the SIMDs' cycles, which the steps and the
 // terms take beside the stream. One step instead of five: 4.5 TB/s. Three matrices of 12 x 64 x 768: 35 us in three launches, half
 // of it the steps' chain. Tried and not kept: the second pass from the last tile on (512 matrices 447 -> 428 us, 1536 1222 ->
@@ -767,7 +767,7 @@ __device__ __forceinline__ void product(f32x16 (&out)[NP / 32], const Cols<NP>& 
 }
 
 // Gram matrix, steps and result of one matrix: two workgroups a CU, one of which streams while the other is at its steps (2304
-// matrices of 128 x 1024 in launches of their own: 2232 us, 475 of them steps; here 1.73 ms). The steps are those of
+// matrices of 128 x 1024 in launches of their own: 2232 us, 475 of them steps; here 1.75 ms). The steps are those of
 // fmlp_muon_iter.hip with 32 columns a wave (the first NP / 32 waves), which reads a left operand half as often. NP = 128 spills 44
 // registers of 256, between the passes.
 template <int NP, int TERMS, bool BF, bool VEC>

@@ -33,7 +33,8 @@ _MAX_ROWS = 2 ** 31 - 1
 class ExpertPlan(NamedTuple):
     """Where tokens go (expert_plan): slots (T, k) int32, the row e * capacity + position of each choice, -1 for one that
     is dropped; counts (num_experts,) int32, the choices of each expert, dropped ones too. To leave a choice out (a padded
-    token's), give expert_plan -1 for its expert: the counts say which rows are zeros, and have to go with the slots."""
+    token's), give expert_plan -1 for its expert: the counts say which rows are zeros, and have to go with the slots (rows
+    below an expert's count that no slot names are not written)."""
     slots: torch.Tensor
     counts: torch.Tensor
     num_experts: int
@@ -307,7 +308,8 @@ class GatedExperts(torch.nn.Module):
         num_experts: number of experts N; hidden_dim: D; intermediate_dim: E; activation, dtype, device: as GatedFlashMLP's
         experts_per_token: k
         capacity_factor: an expert has ceil(T k / N * capacity_factor) rows for T tokens, what comes beyond is
-            dropped; None: T rows, none is dropped
+            dropped; None: T rows, none is dropped, and the experts' MLP runs on N T rows for the T k that hold tokens,
+            N / k times their work
         normalize: as expert_route's; None: where experts_per_token is above one, so that the router always learns
 
     The input is (..., D): rows of tokens, or the MLP's (H, B, D) layout, whose heads' rows are tokens of their own.

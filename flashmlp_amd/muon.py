@@ -8,9 +8,11 @@
     w = (1 - lr weight_decay) w - lr scale X
 
 Every matrix of a stack (..., R, C) stands by itself, as the heads of the MLPs' weights (H, D, E) and (H, E, D) do; min(R, C) <=
-256, the other side is any. torch.optim.Muon, whose conventions these are, takes single matrices only. fp16, bf16 or
-fp32; weights, gradients and momenta each of its own type, so that gradients clipped into full precision buffers
-(clip_grads) or 16-bit ones go with full precision weights. Calls are asynchronous on torch's current stream.
+256, the other side is any. torch.optim.Muon, whose momentum, decoupled decay and scale these are, takes single matrices
+only, decays by 0.1 by default where this does not, and divides by the norm or eps, whichever is more, where this divides by their
+sum, which differs for gradients near eps alone. fp16, bf16 or fp32; weights, gradients and momenta each of its own type, so that
+gradients clipped into full precision buffers (clip_grads) or 16-bit ones go with full precision weights. Calls are asynchronous on
+torch's current stream.
 
 The steps are taken on the smaller side's Gram matrix in 32 bits. 16-bit results, and the update that weights take, are off by up
 to 4e-4 in norm and 1.4e-3 in directions whose singular values are far below the largest (measured with the usual coefficients),

@@ -386,7 +386,8 @@ int fmlp_route_bwd(const void* logits, const float* weights, const int32_t* expe
  * tokens to their experts, and the backward of fmlp_expert_gather (x its output's gradient).
  * fmlp_expert_gather: o[t] = sum over j of weights[t][j] * rows[slot], summed in fp32 in the order of j (dropped choices left out);
  * the way back, and with weights NULL the backward of the copy. slots and counts are those of one fmlp_expert_plan
- * call: no slot is there twice. Slots out of range count as -1. Any alignment, any D < 2^24. rows_out must not overlap an input.
+ * call: no slot is there twice, and every row below an expert's count is some slot's (fmlp_expert_scatter leaves others as they
+ * are). Slots out of range count as -1. Any alignment, any D < 2^24. rows_out must not overlap an input.
  */
 size_t fmlp_expert_plan_workspace_bytes(int64_t T, int64_t k, int64_t N);
 int fmlp_expert_plan(const void* experts, int index_bytes, int32_t* slots, int32_t* counts, int64_t T, int64_t k, int64_t N,
