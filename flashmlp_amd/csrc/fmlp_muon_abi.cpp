@@ -16,10 +16,10 @@ using fmlp::abi_ok;
 namespace {
 
 // Steps on one Gram matrix. Rounding of it at the smallest eigenvalues grows by q(0)^2 = a^2 a step, 12 for the usual a = 3.44, until
-// they are of the size of one. 16-bit results hide a growth of 2e4 before the stage's last step: five usual steps, whose results are
+// they are of the size of one. bf16 results hide a growth of 2e4 before the stage's last step: five usual steps, whose results are
 // off by 4e-6 to 4e-4 in norm and up to 1.4e-3 at a singular value (64 x 64 to 256 x 1024, noise around a low rank and spectra
 // of one to five decades; a bf16 result's rounding is 1.7e-3, at a singular value 1.6 to 3e-3). Five steps of a schedule that
-// begins with a = 8.3, 2e5, were off by up to 2.4e-3 and 1.5e-2; in three and two 4e-5 and 3e-4.
+// begins with a = 8.3, 2e5, were off by up to 2.4e-3 and 1.5e-2, in three and two 4e-5 and 3e-4; of one that grows 3e4 5.9e-4 and 3e-3.
 // An fp32 result has two steps on the first Gram matrix, where the first of them grows little enough (a up to 4), and from there on
 // a Gram matrix for each step. Off from 64 bits in norm, that and fp32 products of the matrices themselves (64 x 64 to 256 x 1024):
 // noise around a low rank 0.7 to 1.3e-6 and 1.0 to 2.5e-6, singular values that fall evenly over two to five decades 1.0 to 5.7e-6

@@ -15,8 +15,8 @@ gradients clipped into full precision buffers (clip_grads) or 16-bit ones go wit
 torch's current stream.
 
 The steps are taken on the smaller side's Gram matrix in 32 bits. 16-bit results, and the update that weights take, are off by up
-to 4e-4 in norm and 1.4e-3 in directions whose singular values are far below the largest (measured with the usual coefficients),
-below a 16-bit result's rounding; an fp32 `orthogonalize` is as exact as the formula's products in fp32. |u|^2 has to be
+to 4e-4 in norm and 1.4e-3 in directions whose singular values are far below the largest (measured with the usual coefficients; a
+bf16 result's rounding is 1.7e-3 and 3e-3, an fp16 one's an eighth of that); an fp32 `orthogonalize` is as exact as the formula's products in fp32. |u|^2 has to be
 within fp32's range; coefficients under which singular values up to one may grow beyond 2^8 in between are refused.
 """
 from __future__ import annotations

@@ -408,17 +408,17 @@ int fmlp_expert_gather(const void* rows, const float* weights, const int32_t* sl
  * 32 bits. Where the result has 16 bits or goes into weights, one Gram matrix serves up to five steps, fewer where their
  * coefficients enlarge small singular values more than the usual ones (a = 3.4445) do. Such results are off, before they are rounded, by
  * 4e-6 to 4e-4 in norm, and by up to 1.4e-3 (of an orthogonal result, relative to 1) at the singular values that were far below the
- * largest (measured with the usual coefficients on noise around a low rank and on spectra of one to five decades; a
- * bf16 result's rounding is 1.7e-3 and 3e-3). An fp32 result of fmlp_orthogonalize takes the Gram matrix anew after two steps (one where
- * the first a is above 4) and then after every one, and is as exact as the products above in fp32 (on the same inputs 0.3 to
- * 1.6 times their error, up to 2.3 times with coefficients that begin at a = 8.3). |u|^2 has to be within fp32 (|u| < 1.8e19).
+ * largest (measured with the usual coefficients on noise around a low rank and on spectra of one to five decades; a bf16
+ * result's rounding is 1.7e-3 and 3e-3, an fp16 one's an eighth of that). An fp32 result of fmlp_orthogonalize takes the Gram
+ * matrix anew after two steps (one where the first a is above 4) and then after every one, and is as exact as the products above in
+ * fp32 (on the same inputs 0.3 to 1.6 times their error, up to 2.3 times with coefficients that begin at a = 8.3). |u|^2 has to be within fp32 (|u| < 1.8e19).
  *
  * fmlp_orthogonalize: out[h] = X of x[h] for a stack of H matrices, dense, both of dtype; out may be x.
  * fmlp_muon_step, in place for n stacks of H[i] matrices each (weights w, gradients g, momenta m, dense, each of a type of its own):
  *   m = momentum m + (1 - momentum) g;  u = m, or with nesterov (1 - momentum) g + momentum m (m as it is stored)
  *   w = (1 - lr weight_decay) w - lr scale X
- * At most 2^40 elements a stack. Any alignment to the elements. Memory that the call writes (w, m) must not be in it twice (FMLP_ERR_INVALID_ARG). Arrays
- * are read on the host before the call returns. Sums in a fixed order. workspace: 16-byte aligned, of the *_workspace_bytes_for, or of the
+ * At most 2^40 elements a stack. Any alignment to the elements. Memory that the call writes (w, m) must not be in it twice
+ * (FMLP_ERR_INVALID_ARG). Arrays are read on the host before the call returns. Sums in a fixed order. workspace: 16-byte aligned, of the *_workspace_bytes_for, or of the
  * *_workspace_bytes, which do for any coefficients (fp32 matrices in between in full).
  */
 typedef struct {
